@@ -19,6 +19,8 @@ enum : int {
     B2_DEV_ERR_TIMEOUT = 1,
     B2_DEV_ERR_KV_OVERFLOW = 2,
     B2_DEV_ERR_BAD_TOKEN = 3,
+    B2_DEV_ERR_BAD_PAGE = 4,       // page table entry outside the pool
+    B2_DEV_ERR_BAD_ROWS = 5,       // row ranges that overlap
 };
 
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s per wait

@@ -1,0 +1,223 @@
+// paged.cu — entry points of the paged 8-bit KV cache (paged.cuh): argument checks
+// and launches. Device pointers in and out, caller's stream, nothing allocated,
+// nothing synchronised, and nothing read from device memory on the host.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "../../include/b2dec.h"
+#include "paged.cuh"
+
+void b2_internal_set_error(const std::string& msg);   // runtime.cu
+
+using namespace b2;
+
+namespace {
+
+int refuse(const char* fn, const std::string& why) {
+    b2_internal_set_error(std::string(fn) + ": " + why);
+    return B2_E_INVALID;
+}
+
+int status(const char* fn, cudaError_t e) {
+    if (e == cudaSuccess) return B2_OK;
+    b2_internal_set_error(std::string(fn) + ": " + cudaGetErrorString(e));
+    return B2_E_CUDA;
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool al4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+// f32 rows of `width` elements, `ld` apart, read and written 16 bytes at a time
+bool rows_ok(const float* p, int64_t ld, int64_t width) { return p && al16(p) && ld >= width && ld % 4 == 0; }
+
+const char* head_dim_bad(int dh) {
+    return dh < 16 || dh > 256 || dh % 16 ? "d_head must be a multiple of 16 from 16 to 256" : nullptr;
+}
+
+constexpr int kMaxPagedHeads = 1024;
+
+// the cache and the rows of a call, checked; false: refused with a message
+bool view(const char* fn, const b2_kv_pages* kv, const b2_kv_rows* rows, PagedKv& c, PagedRows& r) {
+    auto bad = [&](const char* why) { refuse(fn, why); return false; };
+    if (!kv || !rows) return bad("NULL cache or rows");
+    if (const char* why = head_dim_bad(kv->d_head)) return bad(why);
+    if (kv->n_kv_heads <= 0 || kv->n_kv_heads > kMaxPagedHeads) return bad("n_kv_heads must be 1 to 1024");
+    if (kv->page_size < kKvBlock || kv->page_size > 1024 || (kv->page_size & (kv->page_size - 1)))
+        return bad("page_size must be a power of two from 16 to 1024");
+    if (kv->n_pages <= 0) return bad("n_pages must be positive");
+    if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale || !al16(kv->k) || !al16(kv->v) || !al4(kv->k_scale) ||
+        !al4(kv->v_scale))
+        return bad("cache pointers must be set, the codes' aligned to 16 bytes");
+    if (rows->n_rows < 0 || rows->n_seq < 0 || rows->max_pages < 0) return bad("negative count");
+    if (rows->n_rows > 0 && rows->n_seq > 0 &&
+        (!rows->row_start || !rows->kv_len || (!rows->page_table && rows->max_pages) || !al4(rows->row_start) ||
+         !al4(rows->kv_len) || !al4(rows->page_table)))
+        return bad("row_start, kv_len and page_table must be set");
+    if (rows->n_seq > (1 << 20)) return bad("n_seq above 1048576");
+    const int64_t cap = (int64_t)rows->max_pages * kv->page_size;
+    if (cap > (1 << 30)) return bad("max_pages * page_size above 2^30");
+    if (rows->max_keys < 0 || rows->max_rows < 0) return bad("negative max_keys or max_rows");
+    c.k = kv->k; c.v = kv->v; c.ks = kv->k_scale; c.vs = kv->v_scale;
+    c.n_pages = kv->n_pages; c.KVH = kv->n_kv_heads; c.dh = kv->d_head;
+    c.page_log2 = 0;
+    while ((1 << c.page_log2) < kv->page_size) ++c.page_log2;
+    r.row_start = rows->row_start; r.kv_len = rows->kv_len; r.table = rows->page_table;
+    r.n_seq = rows->n_seq; r.max_pages = rows->max_pages; r.n_rows = rows->n_rows;
+    r.cap = rows->max_keys > 0 && rows->max_keys < cap ? rows->max_keys : (int)cap;
+    return true;
+}
+
+// most (sequence, block) runs that n_rows rows in n_seq ranges can make: a range of
+// L rows touches at most (L - 2) / 16 + 2 blocks, and no more than L
+int run_bound(const PagedRows& r) {
+    const long long by_block = (long long)r.n_rows / kKvBlock + 2ll * r.n_seq;
+    return (int)(by_block < r.n_rows ? by_block : r.n_rows);
+}
+
+// lanes and float4s that hold a head vector of dh elements
+#define B2_BY_HEAD_DIM(dh, CALL)                 \
+    (dh) <= 16   ? CALL(4, 1)                    \
+    : (dh) <= 32 ? CALL(8, 1)                    \
+    : (dh) <= 64 ? CALL(16, 1)                   \
+    : (dh) <= 128 ? CALL(32, 1) : CALL(32, 2)
+
+template <int LPH, int VPL>
+cudaError_t launch_norm_rope(const NormRopeParams& p, cudaStream_t s) {
+    const int heads = p.H + p.KVH;
+    // four vectors a lane group once there is work for the whole GPU (their loads are
+    // in flight together and share the table row), one before that
+    const long long lanes = (long long)p.n_rows * heads * LPH;
+    if (lanes >= 4ll * 148 * 1024) {
+        const long long n = (long long)p.n_rows * ((heads + 3) / 4) * LPH;
+        norm_rope_kernel<LPH, VPL, 4><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
+    } else {
+        norm_rope_kernel<LPH, VPL, 1><<<(unsigned)((lanes + 255) / 256), 256, 0, s>>>(p);
+    }
+    return cudaGetLastError();
+}
+
+template <int LPH, int VPL>
+cudaError_t launch_append(AppendParams p, bool queries, cudaStream_t s) {
+    p.kv_ctas = (2 * p.c.KVH + 7) / 8;
+    int y = p.kv_ctas;
+    if (queries) y += (kKvBlock * ((p.nr.H + 3) / 4) * LPH + 255) / 256;
+    kv_append_kernel<LPH, VPL><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, float* q_out, int64_t ldqo, float* k_out,
+                    int64_t ldko, const float* q_gain, const float* k_gain, float eps, float q_scale, const float* table,
+                    int table_rows, const int32_t* pos, int n_rows, int n_heads, int n_kv_heads, int d_head,
+                    int32_t* err, void* stream) {
+    const char* fn = "b2_qk_norm_rope";
+    if (const char* why = head_dim_bad(d_head)) return refuse(fn, why);
+    if (n_rows < 0 || n_heads < 0 || n_kv_heads < 0 || n_heads > kMaxPagedHeads || n_kv_heads > kMaxPagedHeads ||
+        n_heads + n_kv_heads == 0)
+        return refuse(fn, "n_rows must be 0 or more, the head counts 0 to 1024 and not both 0");
+    if (n_rows == 0) return B2_OK;
+    if ((n_heads && (!rows_ok(q, ldq, (int64_t)n_heads * d_head) || !rows_ok(q_out, ldqo, (int64_t)n_heads * d_head))) ||
+        (n_kv_heads && (!rows_ok(k, ldk, (int64_t)n_kv_heads * d_head) || !rows_ok(k_out, ldko, (int64_t)n_kv_heads * d_head))))
+        return refuse(fn, "q, k and their outputs: 16-byte aligned, row strides a multiple of 4 that hold a row");
+    if ((q_gain && !al16(q_gain)) || (k_gain && !al16(k_gain)) || (table && !al16(table)) || !al4(pos) || !al4(err))
+        return refuse(fn, "gains and table must be 16-byte aligned, pos and err 4");
+    if (table && (!pos || table_rows <= 0)) return refuse(fn, "a table needs pos and table_rows");
+    if ((q_gain || k_gain) && !(eps >= 0.0f && std::isfinite(eps))) return refuse(fn, "eps must be finite and not negative");
+    if ((long long)n_rows * (n_heads + n_kv_heads) > (1ll << 31)) return refuse(fn, "more than 2^31 head vectors");
+    NormRopeParams p{};
+    p.q = q; p.k = k; p.qo = q_out; p.ko = k_out;
+    p.ldq = ldq; p.ldk = ldk; p.ldqo = ldqo; p.ldko = ldko;
+    p.gq = q_gain; p.gk = k_gain; p.eps = eps; p.q_scale = q_scale;
+    p.table = table; p.table_rows = table_rows; p.pos = pos;
+    p.n_rows = n_rows; p.H = n_heads; p.KVH = n_kv_heads; p.dh = d_head; p.err = err;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define B2_CALL(L, V) launch_norm_rope<L, V>(p, s)
+    return status(fn, B2_BY_HEAD_DIM(d_head, B2_CALL));
+#undef B2_CALL
+}
+
+int b2_kv_append_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* k, int64_t ldk, const float* v,
+                    int64_t ldv, const float* k_gain, float eps, const float* table, int table_rows, const float* q,
+                    int64_t ldq, float* q_out, int64_t ldqo, const float* q_gain, float q_scale, int n_heads,
+                    int32_t* err, void* stream) {
+    const char* fn = "b2_kv_append_i8";
+    AppendParams p{};
+    if (!view(fn, kv, rows, p.c, p.r)) return B2_E_INVALID;
+    if (p.r.n_rows == 0 || p.r.n_seq == 0) return B2_OK;
+    const int64_t width = (int64_t)kv->n_kv_heads * kv->d_head;
+    if (!rows_ok(k, ldk, width) || !rows_ok(v, ldv, width))
+        return refuse(fn, "k and v: 16-byte aligned, row strides a multiple of 4 that hold a row");
+    if (q && (n_heads <= 0 || n_heads > kMaxPagedHeads)) return refuse(fn, "n_heads must be 1 to 1024");
+    if (q && (!rows_ok(q, ldq, (int64_t)n_heads * kv->d_head) || !rows_ok(q_out, ldqo, (int64_t)n_heads * kv->d_head)))
+        return refuse(fn, "q and q_out: 16-byte aligned, row strides a multiple of 4 that hold a row");
+    if ((q_gain && !al16(q_gain)) || (k_gain && !al16(k_gain)) || (table && !al16(table)) || !al4(err))
+        return refuse(fn, "gains and table must be 16-byte aligned, err 4");
+    if (table && table_rows <= 0) return refuse(fn, "a table needs table_rows");
+    if ((q_gain || k_gain) && !(eps >= 0.0f && std::isfinite(eps))) return refuse(fn, "eps must be finite and not negative");
+    p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
+    p.nr.q = q; p.nr.qo = q_out; p.nr.ldq = ldq; p.nr.ldqo = ldqo;
+    p.nr.gq = q_gain; p.nr.gk = k_gain; p.nr.eps = eps; p.nr.q_scale = q_scale;
+    p.nr.table = table; p.nr.table_rows = table_rows;
+    p.nr.n_rows = p.r.n_rows; p.nr.H = q ? n_heads : 0; p.nr.KVH = 0; p.nr.dh = kv->d_head; p.nr.err = err;
+    p.items = run_bound(p.r);
+    p.err = err;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define B2_CALL(L, V) launch_append<L, V>(p, q != nullptr, s)
+    return status(fn, B2_BY_HEAD_DIM(kv->d_head, B2_CALL));
+#undef B2_CALL
+}
+
+int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, void* v_out, int64_t ld, int bf16,
+                  int32_t* err, void* stream) {
+    const char* fn = "b2_kv_read_i8";
+    ReadParams p{};
+    if (!view(fn, kv, rows, p.c, p.r)) return B2_E_INVALID;
+    if (p.r.n_rows == 0 || p.r.n_seq == 0) return B2_OK;
+    if (!k_out || !v_out || !al16(k_out) || !al16(v_out) || ld < (int64_t)kv->n_kv_heads * kv->d_head ||
+        ld % (bf16 ? 8 : 4))
+        return refuse(fn, "k_out and v_out: 16-byte aligned, ld holding a row and a multiple of 16 bytes");
+    if (!al4(err)) return refuse(fn, "err must be 4-byte aligned");
+    p.k = k_out; p.v = v_out; p.ld = ld;
+    p.items = run_bound(p.r);
+    p.err = err;
+    const dim3 grid((unsigned)p.items, (unsigned)((2 * p.c.KVH + 7) / 8));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (bf16) kv_read_kernel<true><<<grid, 256, 0, s>>>(p);
+    else kv_read_kernel<false><<<grid, 256, 0, s>>>(p);
+    return status(fn, cudaGetLastError());
+}
+
+size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads) {
+    (void)kv; (void)rows; (void)n_heads;
+    return 0;
+}
+
+int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* q, int64_t ldq, float* out, int64_t ldo,
+                     int n_heads, void* workspace, size_t workspace_bytes, int32_t* err, void* stream) {
+    const char* fn = "b2_attn_paged_i8";
+    PagedAttnParams p{};
+    if (!view(fn, kv, rows, p.c, p.r)) return B2_E_INVALID;
+    if (n_heads <= 0 || n_heads > kMaxPagedHeads || n_heads % kv->n_kv_heads)
+        return refuse(fn, "n_heads must be a multiple of n_kv_heads up to 1024");
+    if (p.r.n_rows == 0 || p.r.n_seq == 0) return B2_OK;
+    const int64_t width = (int64_t)n_heads * kv->d_head;
+    if (!rows_ok(q, ldq, width) || !rows_ok(out, ldo, width))
+        return refuse(fn, "q and out: 16-byte aligned, row strides a multiple of 4 that hold a row");
+    if (!al4(err)) return refuse(fn, "err must be 4-byte aligned");
+    const size_t need = b2_attn_paged_i8_workspace(kv, rows, n_heads);
+    if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
+        return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+    if (q == out) return refuse(fn, "out must not be q");
+    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.err = err;
+    const long long items = (long long)p.r.n_rows * n_heads;
+    if (items > (1ll << 31)) return refuse(fn, "more than 2^31 (row, head) pairs");
+    paged_attn_kernel<<<(unsigned)((items + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return status(fn, cudaGetLastError());
+}
+
+}  // extern "C"

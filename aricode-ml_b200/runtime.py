@@ -96,6 +96,14 @@ def _declare(L):
                                  C.c_size_t, vp]
     L.b2_attn_decode_static.argtypes = [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int,
                                         C.c_int, vp]
+    L.b2_qk_norm_rope.argtypes = [vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, vp, C.c_float,
+                                  C.c_float, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]
+    L.b2_kv_append_i8.argtypes = [vp, vp, vp, C.c_int64, vp, C.c_int64, vp, C.c_float, vp, C.c_int, vp, C.c_int64, vp,
+                                  C.c_int64, vp, C.c_float, C.c_int, vp, vp]
+    L.b2_kv_read_i8.argtypes = [vp, vp, vp, vp, C.c_int64, C.c_int, vp, vp]
+    L.b2_attn_paged_i8_workspace.restype = C.c_size_t
+    L.b2_attn_paged_i8_workspace.argtypes = [vp, vp, C.c_int]
+    L.b2_attn_paged_i8.argtypes = [vp, vp, vp, C.c_int64, vp, C.c_int64, C.c_int, vp, C.c_size_t, vp, vp]
     L.b2_argmax.argtypes = [vp, C.c_int64, vp, vp]
     L.b2_silu_mul.argtypes = [vp, vp, vp, C.c_int, vp]
     L.b2_gelu.argtypes = [vp, vp, C.c_int, vp]
@@ -439,6 +447,264 @@ def attn_decode_static(q, K, V, n_heads, n_kv_heads, d_head, n, max_seq, stream=
     out = torch.empty(n_heads * d_head, dtype=torch.float32, device=q.device)
     check(lib().b2_attn_decode_static(_ptr(q), _ptr(K), _ptr(V), _ptr(out), n_heads, n_kv_heads,
                                       d_head, int(n), int(max_seq), _stream(stream)))
+    return out
+
+
+# ----------------------------------------------------------------- paged 8-bit KV cache
+KV_BLOCK = 16                    # tokens that share a scale (B2_KV_BLOCK)
+ROWS_ERRORS = {2: "a position past the sequence's capacity or the rotation table",
+               4: "a page-table entry outside the pool", 5: "row ranges that overlap"}
+
+
+class _KvPages(C.Structure):     # b2_kv_pages
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("d_head", C.c_int32)]
+
+
+class _KvRows(C.Structure):      # b2_kv_rows
+    _fields_ = [("row_start", vp), ("kv_len", vp), ("page_table", vp), ("n_seq", C.c_int32),
+                ("max_pages", C.c_int32), ("n_rows", C.c_int32), ("max_keys", C.c_int32), ("max_rows", C.c_int32)]
+
+
+def _invalid(msg):
+    return B2Error(-1, msg)
+
+
+def _tensor(name, t, dtype, dev, shape=None):
+    """A contiguous CUDA tensor of this type on `dev` (None: any GPU)."""
+    if not t.is_cuda or t.dtype != dtype or not t.is_contiguous() or (dev is not None and t.device != dev):
+        raise _invalid(f"{name} must be a contiguous {dtype} tensor on {dev or 'a GPU'}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise _invalid(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    return t
+
+
+def _f32_rows(name, t, dev, n_rows, width):
+    """(pointer, row stride) of an f32 [n_rows, width] tensor whose rows are contiguous."""
+    import torch
+    if t.dtype != torch.float32 or t.device != dev or t.dim() != 2:
+        raise _invalid(f"{name} must be a 2-D float32 tensor on {dev}")
+    if t.shape[0] < n_rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise _invalid(f"{name} must hold {n_rows} rows of {width} contiguous elements")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else (width + 3) // 4 * 4)
+
+
+def _opt(name, t, dtype, dev, shape):
+    return None if t is None else _tensor(name, t, dtype, dev, shape).data_ptr()
+
+
+class _on:
+    """The device and stream of a call: `dev` current inside (the C calls run on the current device); `stream` a
+    handle or None (the device's current stream). Tensors made inside belong to that stream."""
+
+    def __init__(self, dev, stream):
+        import torch
+        self._guards = []
+        if torch.cuda.current_device() != dev.index:
+            self._guards.append(torch.cuda.device(dev))
+        if stream is None:
+            self.handle = torch.cuda.current_stream(dev).cuda_stream
+        else:
+            self.handle = int(stream)
+            if self.handle != torch.cuda.current_stream(dev).cuda_stream:
+                self._guards.append(torch.cuda.stream(torch.cuda.ExternalStream(self.handle, device=dev)))
+
+    def __enter__(self):
+        for g in self._guards:
+            g.__enter__()
+        return self.handle
+
+    def __exit__(self, *a):
+        for g in reversed(self._guards):
+            g.__exit__(*a)
+
+
+class PagedKV:
+    """A pool of pages of int8 keys and values with a scale per 16 tokens and head (b2_kv_pages): k and v
+    [pages, kv_heads, page_size, d_head] int8, k_scale and v_scale [pages, kv_heads, page_size / 16] f32. `err` is
+    the device word that calls on this cache set; check() reads it."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        if k.dim() != 4:
+            raise _invalid("k must be [pages, kv_heads, page_size, d_head]")
+        n, h, page, d = k.shape
+        if n < 1 or h < 1 or d < 16 or d > 256 or d % 16 or page < 16 or page > 1024 or page & (page - 1):
+            raise _invalid("page_size must be a power of two from 16 to 1024, d_head a multiple of 16 up to 256")
+        _tensor("k", k, torch.int8, None)
+        self.device = k.device
+        _tensor("v", v, torch.int8, self.device, (n, h, page, d))
+        _tensor("k_scale", k_scale, torch.float32, self.device, (n, h, page // KV_BLOCK))
+        _tensor("v_scale", v_scale, torch.float32, self.device, (n, h, page // KV_BLOCK))
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_kv_heads, self.page_size, self.d_head = n, h, page, d
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._err = self.err.data_ptr()
+        self._c = _KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, page, h, d)
+        self._p = C.addressof(self._c)
+
+    @classmethod
+    def empty(cls, n_pages, page_size, n_kv_heads, d_head, device="cuda"):
+        import torch
+        shape = (n_pages, n_kv_heads, page_size)
+        code = [torch.zeros(*shape, d_head, dtype=torch.int8, device=device) for _ in range(2)]
+        scale = [torch.zeros(n_pages, n_kv_heads, page_size // KV_BLOCK, device=device) for _ in range(2)]
+        return cls(*code, *scale)
+
+    def check(self):
+        """Waits for the device, and raises if a call on this cache met bad rows or pages (which it left out)."""
+        e = int(self.err.item())
+        if e:
+            self.err.zero_()
+            raise B2Error(-8, ROWS_ERRORS.get(e, f"device error {e}"))
+
+
+class KVRows:
+    """The rows of a call (b2_kv_rows): int32 tensors row_start [n_seq + 1], kv_len [n_seq] (this call's rows
+    included) and page_table [n_seq, max_pages]. They are read when the kernels run: refill them in place to replay a
+    captured call. max_keys bounds every kv_len (0: what the table can hold); max_rows says how many rows the longest
+    sequence has, if that is known (0: not)."""
+
+    def __init__(self, row_start, kv_len, page_table, n_rows, max_keys=0, max_rows=0):
+        import torch
+        _tensor("kv_len", kv_len, torch.int32, None)
+        self.device = kv_len.device
+        if kv_len.dim() != 1 or page_table.dim() != 2:
+            raise _invalid("kv_len must be 1-D and page_table 2-D")
+        n = kv_len.shape[0]
+        _tensor("row_start", row_start, torch.int32, self.device, (n + 1,))
+        _tensor("page_table", page_table, torch.int32, self.device, (n, page_table.shape[1]))
+        if n_rows < 0 or max_keys < 0 or max_rows < 0:
+            raise _invalid("n_rows, max_keys and max_rows must not be negative")
+        self.row_start, self.kv_len, self.page_table = row_start, kv_len, page_table
+        self.n_rows = int(n_rows)
+        self._c = _KvRows(row_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), n, page_table.shape[1],
+                          self.n_rows, int(max_keys), int(max_rows))
+        self._p = C.addressof(self._c)
+
+
+def _pair(kv, rows):
+    if kv.device != rows.device:
+        raise _invalid("the cache and the rows must be on one device")
+    return kv.device
+
+
+def qk_norm_rope(q, k, d_head, pos=None, table=None, q_gain=None, k_gain=None, eps=1e-5, q_scale=1.0, q_out=None,
+                 k_out=None, err=None, stream=None):
+    """RMS norm of each query and key head (where a gain [d_head] is given), then the rotation by table row pos[i]
+    (where a table [positions, d_head] is given), queries times q_scale. q [n, heads * d_head] and k
+    [n, kv_heads * d_head] f32, their rows may be strided (slices of a fused projection); either may be None. Rows
+    with pos < 0 are left alone in the outputs. The outputs may be the inputs; new ones are made where none are
+    given. Returns (q_out, k_out)."""
+    import torch
+    one = q if q is not None else k
+    if one is None:
+        raise _invalid("q or k must be given")
+    dev, n = one.device, one.shape[0]
+    if not one.is_cuda or one.dim() != 2 or d_head <= 0:
+        raise _invalid("q and k must be 2-D CUDA tensors, d_head positive")
+    with _on(dev, stream) as h:
+        widths = []
+        for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+            if x is None:
+                widths.append((None, 0, None, 0, 0, None))
+                continue
+            w = x.shape[-1]
+            if w % d_head or x.shape[0] != n:
+                raise _invalid(f"{name} must hold whole heads, and as many rows as the other")
+            src = _f32_rows(name, x, dev, n, w)
+            if out is None:
+                out = torch.empty(n, w, device=dev)
+            widths.append((*src, *_f32_rows(name + "_out", out, dev, n, w), w // d_head, out))
+        (qp, ldq, qop, ldqo, H, q_out), (kp, ldk, kop, ldko, K, k_out) = widths
+        if table is not None and (pos is None or table.dim() != 2):
+            raise _invalid("a table [positions, d_head] needs pos")
+        check(lib().b2_qk_norm_rope(
+            qp, ldq, kp, ldk, qop, ldqo, kop, ldko, _opt("q_gain", q_gain, torch.float32, dev, (d_head,)),
+            _opt("k_gain", k_gain, torch.float32, dev, (d_head,)), eps, q_scale,
+            None if table is None else _tensor("table", table, torch.float32, dev, (table.shape[0], d_head)).data_ptr(),
+            0 if table is None else table.shape[0], _opt("pos", pos, torch.int32, dev, (n,)), n, H, K, d_head,
+            _opt("err", err, torch.int32, dev, (1,)), h))
+    return q_out, k_out
+
+
+def kv_append_i8(kv, rows, k, v, table=None, k_gain=None, eps=1e-5, q=None, q_gain=None, q_scale=1.0, q_out=None,
+                 stream=None):
+    """Append the call's rows k and v [n_rows, kv_heads * d_head] f32 to the cache, keys normed (k_gain) and rotated
+    (table) on the way; with q, the queries likewise (times q_scale) into q_out, which is returned."""
+    import torch
+    dev, d, n = _pair(kv, rows), kv.d_head, rows.n_rows
+    w = kv.n_kv_heads * d
+    kp, ldk = _f32_rows("k", k, dev, n, w)
+    vp_, ldv = _f32_rows("v", v, dev, n, w)
+    with _on(dev, stream) as h:
+        qp, ldq, qop, ldqo, H = None, 0, None, 0, 0
+        if q is not None:
+            wq = q.shape[-1]
+            if wq % d:
+                raise _invalid("q must hold whole heads")
+            qp, ldq = _f32_rows("q", q, dev, n, wq)
+            if q_out is None:
+                q_out = torch.empty(q.shape[0], wq, device=dev)
+            qop, ldqo = _f32_rows("q_out", q_out, dev, n, wq)
+            H = wq // d
+        if table is not None and table.dim() != 2:
+            raise _invalid("table must be [positions, d_head]")
+        check(lib().b2_kv_append_i8(
+            kv._p, rows._p, kp, ldk, vp_, ldv, _opt("k_gain", k_gain, torch.float32, dev, (d,)), eps,
+            None if table is None else _tensor("table", table, torch.float32, dev, (table.shape[0], d)).data_ptr(),
+            0 if table is None else table.shape[0], qp, ldq, qop, ldqo, _opt("q_gain", q_gain, torch.float32, dev, (d,)),
+            q_scale, H, kv._err, h))
+    return q_out
+
+
+def kv_read_i8(kv, rows, dtype=None, k_out=None, v_out=None, stream=None):
+    """The rows' cached keys and values as (k, v) [n_rows, kv_heads * d_head] of dtype float32 (the default) or
+    bfloat16. Rows that belong to no sequence stay as they are in the outputs (unset in new ones)."""
+    import torch
+    dev, n, w = _pair(kv, rows), rows.n_rows, kv.n_kv_heads * kv.d_head
+    if k_out is not None:
+        dtype = dtype or k_out.dtype
+    dtype = dtype or torch.float32
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise _invalid("dtype must be float32 or bfloat16")
+    with _on(dev, stream) as h:
+        outs = [torch.empty(n, w, dtype=dtype, device=dev) if o is None else _tensor("k_out and v_out", o, dtype, dev, (n, w))
+                for o in (k_out, v_out)]
+        check(lib().b2_kv_read_i8(kv._p, rows._p, outs[0].data_ptr(), outs[1].data_ptr(), w, dtype == torch.bfloat16,
+                                  kv._err, h))
+    return outs[0], outs[1]
+
+
+def attn_paged_workspace(kv, rows, n_heads, stream=None):
+    """A workspace tensor that attn_paged_i8 calls of these sizes can share, one after another."""
+    import torch
+    dev = _pair(kv, rows)
+    with _on(dev, stream):
+        return torch.empty(lib().b2_attn_paged_i8_workspace(kv._p, rows._p, int(n_heads)), dtype=torch.uint8, device=dev)
+
+
+def attn_paged_i8(kv, rows, q, out=None, workspace=None, stream=None):
+    """Attention of rows q [n_rows, heads * d_head] f32 (rotated and pre-scaled) over the cache, each row over its
+    sequence's keys up to its own position. Rows that belong to no sequence stay as they are in `out` (unset in a new
+    one). Without a workspace the call makes its own."""
+    import torch
+    dev, n = _pair(kv, rows), rows.n_rows
+    w = q.shape[-1]
+    if w % kv.d_head:
+        raise _invalid("q must hold whole heads")
+    H = w // kv.d_head
+    qp, ldq = _f32_rows("q", q, dev, n, w)
+    with _on(dev, stream) as h:
+        if out is None:
+            out = torch.empty(q.shape[0], w, device=dev)
+        op, ldo = _f32_rows("out", out, dev, n, w)
+        if workspace is None:
+            workspace = attn_paged_workspace(kv, rows, H)
+        else:
+            _tensor("workspace", workspace, torch.uint8, dev)
+        check(lib().b2_attn_paged_i8(kv._p, rows._p, qp, ldq, op, ldo, H, workspace.data_ptr(), workspace.numel(),
+                                     kv._err, h))
     return out
 
 

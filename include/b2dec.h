@@ -266,6 +266,92 @@ int b2_attn_decode_static(const float* q, const float* K, const float* V, float*
                           int n_heads, int n_kv_heads, int d_head, int n, int max_seq,
                           void* stream);
 
+/* ---- paged 8-bit KV cache
+ * For serving many sequences: K and V as int8 codes in pages, with one f32 scale
+ * per block of B2_KV_BLOCK tokens and KV head (a quarter of the f32 cache's bytes,
+ * and no max_seq rows set aside per sequence). No counterpart in the reference,
+ * whose caches are f32 [kv_head][max_seq][d_head].
+ *
+ * The calls read lengths, row ranges and pages on the device only, so a captured
+ * launch replays with new ones. What they find wrong there they leave out, and set
+ * *err (device int32, optional, first error kept; the caller zeroes it):
+ *   B2_ROWS_OVERFLOW  a position at or past the sequence's capacity (the smaller of
+ *                     max_keys and max_pages * page_size), or past the table
+ *   B2_ROWS_BAD_PAGE  a page-table entry outside [0, n_pages)
+ *   B2_ROWS_OVERLAP   row ranges that overlap
+ * d_head: a multiple of 16 from 16 to 256. f32 rows: 16-byte aligned, row strides in
+ * elements, a multiple of 4. Calls on one cache must be ordered by the caller. */
+#define B2_KV_BLOCK 16
+enum { B2_ROWS_OVERFLOW = 2, B2_ROWS_BAD_PAGE = 4, B2_ROWS_OVERLAP = 5 };
+
+typedef struct b2_kv_pages {
+    int8_t* k;               /* [n_pages][n_kv_heads][page_size][d_head], 16-byte aligned */
+    int8_t* v;
+    float* k_scale;          /* [n_pages][n_kv_heads][page_size / B2_KV_BLOCK] */
+    float* v_scale;
+    int32_t n_pages;
+    int32_t page_size;       /* tokens: a power of two from 16 to 1024 */
+    int32_t n_kv_heads;
+    int32_t d_head;
+} b2_kv_pages;
+
+/* A call's rows. Sequence s has rows row_start[s] .. row_start[s + 1] - 1 (possibly
+ * none); they are the last of its kv_len[s] keys, so row i of it stands at position
+ * kv_len[s] - (its rows) + i. Key j lies in page page_table[s][j / page_size]. Rows
+ * before position 0 (fewer keys than rows) stand nowhere; rows from row_start[n_seq]
+ * on belong to nobody and their outputs stay as they were. */
+typedef struct b2_kv_rows {
+    const int32_t* row_start;   /* device [n_seq + 1], not decreasing */
+    const int32_t* kv_len;      /* device [n_seq] */
+    const int32_t* page_table;  /* device [n_seq][max_pages] */
+    int32_t n_seq;
+    int32_t max_pages;
+    int32_t n_rows;             /* rows of the buffers */
+    int32_t max_keys;           /* no kv_len is larger (0: max_pages * page_size) */
+    int32_t max_rows;           /* a hint: the most rows of one sequence (0: n_rows) */
+} b2_kv_rows;
+
+/* Each query and key head: RMS norm over its d_head elements (x / sqrt(mean x^2 +
+ * eps) * gain; a NULL gain: no norm), then the rotation of b2_rope_apply with table
+ * row pos[i] (table [table_rows][d_head], NULL: no rotation), queries times q_scale.
+ * q [n_rows][ldq] holds n_heads heads side by side, k n_kv_heads (either count may be
+ * 0). Outputs may be the inputs. Rows with pos < 0 are left alone; pos may be NULL
+ * without a table. */
+int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, float* q_out, int64_t ldqo,
+                    float* k_out, int64_t ldko, const float* q_gain, const float* k_gain, float eps, float q_scale,
+                    const float* table, int table_rows, const int32_t* pos, int n_rows, int n_heads,
+                    int n_kv_heads, int d_head, int32_t* err, void* stream);
+
+/* Write the call's K and V rows [n_rows][n_kv_heads * d_head] into the cache, keys
+ * normed (k_gain) and rotated (table, at the row's position) on the way as in
+ * b2_qk_norm_rope; with q, the queries likewise into q_out in the same launch (not
+ * cached).
+ * A block's scale is max|x| / 127 over its values; a row that needs a larger one
+ * grows it and brings the block's older codes to it (rint(code * old / new)). A
+ * block whose first token is written starts afresh. Codes are rint(x / scale). A NaN or
+ * infinity makes the block's scale NaN, so that every row that sees it becomes NaN.
+ * A page that is appended to must belong to one sequence and be listed once. */
+int b2_kv_append_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* k, int64_t ldk, const float* v,
+                    int64_t ldv, const float* k_gain, float eps, const float* table, int table_rows,
+                    const float* q, int64_t ldq, float* q_out, int64_t ldqo, const float* q_gain, float q_scale,
+                    int n_heads, int32_t* err, void* stream);
+
+/* The rows' cached keys and values as f32 (bf16 = 0) or bf16: k_out, v_out
+ * [n_rows][ld], for moving a sequence or handing it to the f32-cache calls. Rows on
+ * a page outside the pool become zeros. */
+int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, void* v_out, int64_t ld, int bf16,
+                  int32_t* err, void* stream);
+
+/* Attention of every row over its sequence's keys up to its own position: q [n_rows]
+ * [ldq] (rotated and pre-scaled, n_heads heads), out [n_rows][ldo]; the softmax runs
+ * over those keys alone (no -60 tail). Keys on a page outside the pool are left out;
+ * a row that sees no key becomes zeros. Any mix of single tokens, pieces of prompts
+ * and whole prompts. workspace: b2_attn_paged_i8_workspace() bytes (may be 0), 16-byte
+ * aligned, no initialisation; calls that may overlap on the GPU need one each. */
+size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads);
+int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* q, int64_t ldq, float* out,
+                     int64_t ldo, int n_heads, void* workspace, size_t workspace_bytes, int32_t* err, void* stream);
+
 /* out[0] = first index of the maximum (NaN never wins; logits[0] NaN -> 0).
  * Replaces: sample_greedy_f32 (sampling_f32.ari:10-24). */
 int b2_argmax(const float* v, int64_t n, int32_t* out, void* stream);
