@@ -107,6 +107,40 @@ cudaError_t launch_append(AppendParams p, bool queries, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// keys per split: small ones fill the GPU when there are few rows; with long caches
+// larger ones bound the partial results and their joining (a function of the capacity
+// alone, so that a sequence's result does not depend on the others in the call)
+void attn_splits(PagedAttnParams& p) {
+    p.kc_log2 = p.r.cap <= 16384 ? 8 : p.r.cap <= 65536 ? 9 : 10;
+    p.nsplit = (p.r.cap + (1 << p.kc_log2) - 1) >> p.kc_log2;
+    if (p.nsplit < 1) p.nsplit = 1;
+}
+
+size_t part_bytes(const PagedAttnParams& p) {
+    return p.nsplit > 1 ? (size_t)p.r.n_rows * p.H * p.nsplit * (p.c.dh + 4) * sizeof(float) : 0;
+}
+
+int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
+
+template <int DP>
+cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
+    using Sh = SplitShape<DP>;
+    auto k = paged_attn_split_kernel<DP>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
+    if (e != cudaSuccess) return e;
+    // tiles over all sequences: at most one partly filled one each
+    const long long tiles = ((long long)p.r.n_rows * p.G / kSplitCols + p.r.n_seq) * p.c.KVH;
+    const long long most = tiles * p.nsplit, resident = (long long)sm_count() * (DP == 256 ? 2 : 4);
+    k<<<(unsigned)(most < resident ? most : resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess || p.nsplit == 1) return e;
+    paged_attn_join_kernel<<<dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), 256, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
 }  // namespace
 
 extern "C" {
@@ -193,8 +227,11 @@ int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, vo
 }
 
 size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads) {
-    (void)kv; (void)rows; (void)n_heads;
-    return 0;
+    PagedAttnParams p{};
+    if (!view("b2_attn_paged_i8_workspace", kv, rows, p.c, p.r) || n_heads <= 0 || n_heads % kv->n_kv_heads) return 0;
+    p.H = n_heads;
+    attn_splits(p);
+    return part_bytes(p);
 }
 
 int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* q, int64_t ldq, float* out, int64_t ldo,
@@ -209,15 +246,17 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     if (!rows_ok(q, ldq, width) || !rows_ok(out, ldo, width))
         return refuse(fn, "q and out: 16-byte aligned, row strides a multiple of 4 that hold a row");
     if (!al4(err)) return refuse(fn, "err must be 4-byte aligned");
-    const size_t need = b2_attn_paged_i8_workspace(kv, rows, n_heads);
+    if (q == out) return refuse(fn, "out must not be q");
+    if ((int64_t)p.r.n_rows * n_heads > (1ll << 30)) return refuse(fn, "more than 2^30 (row, head) pairs");
+    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.G = n_heads / kv->n_kv_heads; p.err = err;
+    attn_splits(p);
+    const size_t need = part_bytes(p);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
-    if (q == out) return refuse(fn, "out must not be q");
-    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.err = err;
-    const long long items = (long long)p.r.n_rows * n_heads;
-    if (items > (1ll << 31)) return refuse(fn, "more than 2^31 (row, head) pairs");
-    paged_attn_kernel<<<(unsigned)((items + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return status(fn, cudaGetLastError());
+    p.part = static_cast<float*>(workspace);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return status(fn, kv->d_head <= 64 ? launch_attn_split<64>(p, s)
+                      : kv->d_head <= 128 ? launch_attn_split<128>(p, s) : launch_attn_split<256>(p, s));
 }
 
 }  // extern "C"

@@ -434,94 +434,470 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
 }
 
 // ------------------------------------------------------------------ attention
+// The codes are exact small integers, so both products run as integer dots on the
+// tensor cores (warp-level s8 MMAs) with the f32 side split into three signed
+// base-256 digits: X = rint(x 2^..) with |X| <= kDigitMax = d2 65536 + d1 256 + d0,
+// 23 bits below the row's largest element. The digit sums are exact in int32 and
+// are joined in f32, so a score or an output carries the error of one 23-bit
+// rounding per factor instead of a chain of f32 roundings, at a third of the int8
+// rate and without converting a single code.
+// three digits in [-128, 127] reach 2^23 - 1 - 0x8080 = 8355711; a little below it,
+// so that the roundings of factor and product stay inside
+constexpr int kDigitMax = 8355700;
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// digits of four integers: word e of d holds digit e of x[0 .. 3] in its bytes
+__device__ __forceinline__ void digits4(int x0, int x1, int x2, int x3, uint32_t (&d)[3]) {
+    const uint32_t y0 = (uint32_t)x0 + 0x8080u, y1 = (uint32_t)x1 + 0x8080u, y2 = (uint32_t)x2 + 0x8080u,
+                   y3 = (uint32_t)x3 + 0x8080u;
+    const uint32_t l = __byte_perm(y0, y1, 0x5140), m = __byte_perm(y2, y3, 0x5140);
+    d[0] = __byte_perm(l, m, 0x5410) ^ 0x80808080u;
+    d[1] = __byte_perm(l, m, 0x7632) ^ 0x80808080u;
+    d[2] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
+}
+
+__device__ __forceinline__ float join_digits(int d2, int d1, int d0) {
+    return ffma((float)d2, 65536.0f, ffma((float)d1, 256.0f, (float)d0));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// the factor that takes values up to `top` (>= 0) to integers up to kDigitMax; tiny
+// tops (below 1e-31) keep fewer bits, 0 gives 0, NaN and infinity NaN
+__device__ __forceinline__ float digit_factor(float top) {
+    if (!(top < __int_as_float(0x7f800000))) return __int_as_float(0x7fffffff);
+    return top > 0.0f ? fminf(fdiv((float)kDigitMax, top), 0x1p126f) : 0.0f;
+}
+
 struct PagedAttnParams {
     PagedKv c;
     PagedRows r;
     const float* q;          // [n_rows][ldq], rotated and pre-scaled
     float* out;              // [n_rows][ldo]
     long long ldq, ldo;
-    int H;
+    int H, G;                // G = H / KVH
+    int kc_log2;             // keys per split
+    int nsplit;              // splits of a sequence of cap keys
+    float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
 };
 
-// One warp per (row, head): 32 keys at a time, a lane per key for the scores, then
-// the lanes over the head's elements for the sum.
-static __global__ void __launch_bounds__(128) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
-    __shared__ __align__(16) float qs[4][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.c.dh;
-    const long long item = (long long)blockIdx.x * 4 + warp;
-    if (item >= (long long)p.r.n_rows * p.H) return;
-    const int row = (int)(item / p.H), h = (int)(item % p.H), kvh = h / (p.H / p.c.KVH);
-    int s = -1, kv = 0, pos = -1;
-    for (int base = 0; base < p.r.n_seq && s < 0; base += 32) {
+// A unit of attention work: columns col0 .. of one KV head's (row, head) pairs of a
+// sequence, against keys of split `split`.
+struct AttnItem {
+    int s, a, len, kv;       // sequence and its rows (s < 0: none left)
+    int kvh, tile, split;
+};
+
+__device__ __forceinline__ long long shfl64(unsigned m, long long v, int src) {
+    return (long long)(((unsigned long long)(unsigned)__shfl_sync(m, (int)(v >> 32), src) << 32) |
+                       (unsigned)__shfl_sync(m, (int)v, src));
+}
+
+// item number `item` of the call (tiles of NC columns), found by one warp
+template <int NC>
+__device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, long long item, int lane) {
+    AttnItem out{-1, 0, 0, 0, 0, 0, 0};
+    long long before = 0;
+    for (int base = 0; base < p.r.n_seq; base += 32) {
+        const int s = base + lane;
+        SeqRows q{0, 0, 0};
+        long long cnt = 0;
+        int tiles = 0;
+        if (s < p.r.n_seq) {
+            q = seq_rows(p.r, s);
+            if (q.len > 0) {
+                if (q.kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
+                const int n = min(q.kv, p.r.cap);
+                tiles = (q.len * p.G + NC - 1) / NC;
+                cnt = (long long)tiles * p.c.KVH * max((n + (1 << p.kc_log2) - 1) >> p.kc_log2, 1);
+            }
+        }
+        long long incl = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = shfl64(0xffffffffu, incl, (lane - o) & 31);
+            if (lane >= o) incl += v;
+        }
+        const long long total = shfl64(0xffffffffu, incl, 31);
+        if (item < before + total) {
+            const int src = __ffs(__ballot_sync(0xffffffffu, before + incl > item)) - 1;
+            const long long idx = item - before - shfl64(0xffffffffu, incl - cnt, src);
+            out.s = base + src;
+            out.a = __shfl_sync(0xffffffffu, q.a, src);
+            out.len = __shfl_sync(0xffffffffu, q.len, src);
+            out.kv = __shfl_sync(0xffffffffu, q.kv, src);
+            tiles = __shfl_sync(0xffffffffu, tiles, src);
+            out.tile = (int)(idx % tiles);
+            const long long rest = idx / tiles;
+            out.kvh = (int)(rest % p.c.KVH);
+            out.split = (int)(rest / p.c.KVH);
+            return out;
+        }
+        before += total;
+    }
+    return out;
+}
+
+// splits that a row at position pos has (at least one: it also writes empty rows)
+__device__ __forceinline__ int row_splits(const PagedAttnParams& p, int pos) {
+    return max((min(pos + 1, p.r.cap) + (1 << p.kc_log2) - 1) >> p.kc_log2, 1);
+}
+
+// ---- few rows per sequence: a CTA of 4 warps takes 8 columns (token, head) of one KV
+// head against one split of the keys; warp w the 32-key steps w, w + 4, .... The codes
+// go from global memory straight into MMA fragments (A = keys x d for the scores,
+// d x keys for the output), so a warp keeps 64 * dh bytes of loads in flight and
+// nothing is staged; the four warps' (m, l, o) meet in shared memory.
+constexpr int kSplitWarps = 4;
+constexpr int kSplitCols = 8;
+
+template <int DP>
+struct SplitShape {
+    static constexpr int NH = DP / 64;             // 64-byte parts of a key row
+    static constexpr int VW = DP / 32;             // 32-bit words of a value row that a lane holds
+    static constexpr int NM = DP / 16;             // output tiles of 16 elements
+    static constexpr int QBytes = 3 * kSplitCols * DP;
+    static constexpr int WStride = 36;             // ints; column rows 4 banks apart
+    static constexpr int MergeFloats = kSplitWarps * kSplitCols * (DP + 2);
+    static constexpr int WBytes = kSplitWarps * kSplitCols * WStride * 4;
+    static constexpr int Smem = QBytes + WBytes + MergeFloats * 4 + 64;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kSplitWarps * 32, DP == 256 ? 2 : 4)
+paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
+    using Sh = SplitShape<DP>;
+    extern __shared__ __align__(16) unsigned char ps_raw[];
+    uint8_t* qd = ps_raw;                                                  // [3][8][DP] digits of the queries
+    float* sq = reinterpret_cast<float*>(ps_raw + Sh::QBytes);             // [8] their units (log2 e in)
+    int* wx = reinterpret_cast<int*>(ps_raw + Sh::QBytes + 64);            // [4][8][WStride] weights
+    float* mo = reinterpret_cast<float*>(ps_raw + Sh::QBytes + 64 + Sh::WBytes);   // [4][8][DP]
+    float* ml = mo + kSplitWarps * kSplitCols * DP;                        // [4][8][2]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int dh = p.c.dh, psz = 1 << p.c.page_log2;
+    int* wxw = wx + warp * kSplitCols * Sh::WStride;
+
+    for (long long item = blockIdx.x;; item += gridDim.x) {
+        const AttnItem it = find_item<kSplitCols>(p, item, lane);
+        if (it.s < 0) return;
+        const int cols = min(it.len * p.G - it.tile * kSplitCols, kSplitCols);
+        const int col0 = it.tile * kSplitCols;                             // column = token * G + head
+        const int pos_last = it.kv - it.len + (col0 + cols - 1) / p.G;     // of the tile's last row
+        const int n = min(pos_last + 1, p.r.cap);                          // keys that any column sees
+        const int j0 = it.split << p.kc_log2;
+        if (j0 >= n && it.split > 0) continue;                             // the tile ends before this split
+        const int jend = min(n, j0 + (1 << p.kc_log2));
+
+        // queries -> digits: 16 lanes a column
+        {
+            const int col = tid >> 4, l16 = tid & 15;
+            const int cc = col0 + col;
+            const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
+            constexpr int NE = DP / 64;                                    // float4s a lane
+            float4 x[NE];
+            float top = 0.0f;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const int d = 4 * (l16 + 16 * i);
+                x[i] = (col < cols && d < dh) ? __ldg(reinterpret_cast<const float4*>(qr + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float mx = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+                bad |= x[i].x != x[i].x || x[i].y != x[i].y || x[i].z != x[i].z || x[i].w != x[i].w;
+                top = fmaxf(top, mx);
+            }
+            if (bad) top = __int_as_float(0x7f800000);
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float f = digit_factor(top);
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const int d = 4 * (l16 + 16 * i);
+                uint32_t w[3];
+                digits4(__float2int_rn(x[i].x * f), __float2int_rn(x[i].y * f), __float2int_rn(x[i].z * f),
+                        __float2int_rn(x[i].w * f), w);
+#pragma unroll
+                for (int e = 0; e < 3; ++e) *reinterpret_cast<uint32_t*>(qd + (e * kSplitCols + col) * DP + d) = w[e];
+            }
+            // unit of the scores in base 2; NaN for a query that is not finite
+            if (l16 == 0) sq[col] = f > 0.0f ? __fdividef(1.4426950408889634f, f) : (f == 0.0f ? 0.0f : f);
+        }
+        __syncthreads();
+        uint32_t qb[3][Sh::NH][4];                                         // B fragments of column g
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+#pragma unroll
+            for (int h = 0; h < Sh::NH; ++h) {
+                const uint4 w = lds128(qd + (e * kSplitCols + g) * DP + 64 * h + 16 * t);
+                qb[e][h][0] = w.x; qb[e][h][1] = w.y; qb[e][h][2] = w.z; qb[e][h][3] = w.w;
+            }
+        const float sq0 = sq[2 * t], sq1 = sq[2 * t + 1];
+        // keys that columns 2t and 2t + 1 see
+        const int pos0 = it.kv - it.len;
+        const int lim0 = 2 * t < cols ? min(pos0 + (col0 + 2 * t) / p.G + 1, n) : 0;
+        const int lim1 = 2 * t + 1 < cols ? min(pos0 + (col0 + 2 * t + 1) / p.G + 1, n) : 0;
+
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;        // running max; this lane's part of the sum
+        float o[Sh::NM][4];
+#pragma unroll
+        for (int i = 0; i < Sh::NM; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+        for (int j = j0 + warp * 32; j < jend; j += kSplitWarps * 32) {
+            // the step's two blocks: where they are and their scales
+            size_t at[2];
+            float sk[2], sv[2];
+            bool there[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int jb = j + 16 * b;
+                const int page = jb < jend ? page_of(p.c, p.r, it.s, jb) : -1;
+                there[b] = page >= 0;
+                if (jb < jend && page < 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+                const size_t cell = ((size_t)max(page, 0) * p.c.KVH + it.kvh) * (psz >> 4) + ((jb & (psz - 1)) >> 4);
+                at[b] = cell * kKvBlock * dh;
+                sk[b] = there[b] ? __ldg(p.c.ks + cell) : 0.0f;
+                sv[b] = there[b] ? __ldg(p.c.vs + cell) : 0.0f;
+            }
+            uint4 kf[2][2][Sh::NH];                                        // [block][row g, g + 8][part]
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int h = 0; h < Sh::NH; ++h) {
+                        const int d = 64 * h + 16 * t;
+                        kf[b][r][h] = (there[b] && d < dh)
+                                          ? __ldg(reinterpret_cast<const uint4*>(p.c.k + at[b] + (size_t)(g + 8 * r) * dh + d))
+                                          : make_uint4(0u, 0u, 0u, 0u);
+                    }
+            uint32_t vf[2][4][Sh::VW];                                     // [block][key 4t + i][words]
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int8_t* vr = p.c.v + at[b] + (size_t)(4 * t + i) * dh;
+                    if constexpr (Sh::VW == 2) {
+                        const int d = 8 * g;
+                        const uint2 w = (there[b] && d < dh) ? __ldg(reinterpret_cast<const uint2*>(vr + d)) : make_uint2(0u, 0u);
+                        vf[b][i][0] = w.x; vf[b][i][1] = w.y;
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < Sh::VW / 4; ++u) {
+                            const int d = (DP / 8) * g + 16 * u;
+                            const uint4 w = (there[b] && d < dh) ? __ldg(reinterpret_cast<const uint4*>(vr + d))
+                                                                 : make_uint4(0u, 0u, 0u, 0u);
+                            vf[b][i][4 * u] = w.x; vf[b][i][4 * u + 1] = w.y; vf[b][i][4 * u + 2] = w.z; vf[b][i][4 * u + 3] = w.w;
+                        }
+                    }
+                }
+
+            // scores (base 2): rows g, g + 8 of each block, columns 2t, 2t + 1
+            float s[2][4];
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                int c[3][4] = {};
+#pragma unroll
+                for (int h = 0; h < Sh::NH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        mma_s8(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
+                        mma_s8(c[e], kf[b][0][h].z, kf[b][1][h].z, kf[b][0][h].w, kf[b][1][h].w, qb[e][h][2], qb[e][h][3]);
+                    }
+                const float u0 = sq0 * sk[b], u1 = sq1 * sk[b];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int key = j + 16 * b + 8 * r + g;
+                    const float a0 = join_digits(c[2][2 * r], c[1][2 * r], c[0][2 * r]) * u0;
+                    const float a1 = join_digits(c[2][2 * r + 1], c[1][2 * r + 1], c[0][2 * r + 1]) * u1;
+                    s[b][2 * r] = there[b] && key < lim0 ? a0 : -INFINITY;
+                    s[b][2 * r + 1] = there[b] && key < lim1 ? a1 : -INFINITY;
+                    mx0 = fmaxf(mx0, s[b][2 * r]);
+                    mx1 = fmaxf(mx1, s[b][2 * r + 1]);
+                }
+            }
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) {
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+            }
+            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+            const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
+            const float back0 = exp2_fast(m0 - b0), back1 = exp2_fast(m1 - b1);
+            m0 = n0; m1 = n1;
+            l0 *= back0; l1 *= back1;
+            // weights p v_scale; -inf scores (masked) give 0 even where a scale is NaN
+            float wt0 = 0.0f, wt1 = 0.0f;                                  // largest weights; NaN if one is
+            bool nan0 = false, nan1 = false;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float e0 = exp2_fast(s[b][2 * r] - b0), e1 = exp2_fast(s[b][2 * r + 1] - b1);
+                    l0 += e0; l1 += e1;
+                    const float w0 = s[b][2 * r] == -INFINITY ? 0.0f : e0 * sv[b];
+                    const float w1 = s[b][2 * r + 1] == -INFINITY ? 0.0f : e1 * sv[b];
+                    s[b][2 * r] = w0; s[b][2 * r + 1] = w1;
+                    wt0 = fmaxf(wt0, fabsf(w0)); wt1 = fmaxf(wt1, fabsf(w1));
+                    nan0 |= w0 != w0; nan1 |= w1 != w1;
+                }
+            if (nan0) wt0 = INFINITY;
+            if (nan1) wt1 = INFINITY;
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) {
+                wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
+                wt1 = fmaxf(wt1, __shfl_xor_sync(0xffffffffu, wt1, x));
+            }
+            const float f0 = digit_factor(wt0), f1 = digit_factor(wt1);
+            __syncwarp();
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    wxw[2 * t * Sh::WStride + 16 * b + 8 * r + g] = __float2int_rn(s[b][2 * r] * f0);
+                    wxw[(2 * t + 1) * Sh::WStride + 16 * b + 8 * r + g] = __float2int_rn(s[b][2 * r + 1] * f1);
+                }
+            __syncwarp();
+            uint32_t wb[2][3];                                             // B fragments: keys 4t .., 16 + 4t .. of column g
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const uint4 w = lds128(wxw + g * Sh::WStride + 16 * b + 4 * t);
+                digits4((int)w.x, (int)w.y, (int)w.z, (int)w.w, wb[b]);
+            }
+            const float u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0, u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
+            // output elements (DP / 8) g + 2 m, + 1 (rows g and g + 8 of tile m): four keys' bytes of one element
+            // make one A register
+#pragma unroll
+            for (int w = 0; w < Sh::VW; ++w) {
+                uint32_t a[2][4];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint32_t x = __byte_perm(vf[b][0][w], vf[b][1][w], 0x5140), y = __byte_perm(vf[b][2][w], vf[b][3][w], 0x5140);
+                    const uint32_t z = __byte_perm(vf[b][0][w], vf[b][1][w], 0x7362), v = __byte_perm(vf[b][2][w], vf[b][3][w], 0x7362);
+                    a[b][0] = __byte_perm(x, y, 0x5410); a[b][1] = __byte_perm(x, y, 0x7632);
+                    a[b][2] = __byte_perm(z, v, 0x5410); a[b][3] = __byte_perm(z, v, 0x7632);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    int c[3][4] = {};
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        mma_s8(c[e], a[0][2 * k], a[0][2 * k + 1], a[1][2 * k], a[1][2 * k + 1], wb[0][e], wb[1][e]);
+                    float(&oo)[4] = o[2 * w + k];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        oo[i] = ffma(join_digits(c[2][i], c[1][i], c[0][i]), i & 1 ? u1 : u0, oo[i] * (i & 1 ? back1 : back0));
+                }
+            }
+        }
+        // this warp's columns: sum over the lanes of a column, then all to shared memory
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+        }
+        if (g == 0) {
+            float* q = ml + (warp * kSplitCols + 2 * t) * 2;
+            q[0] = m0; q[1] = l0; q[2] = m1; q[3] = l1;
+        }
+        float* ow = mo + warp * kSplitCols * DP;
+#pragma unroll
+        for (int i = 0; i < Sh::NM; ++i) {
+            const int d = (DP / 8) * g + 2 * i;
+            *reinterpret_cast<float2*>(ow + (2 * t) * DP + d) = make_float2(o[i][0], o[i][2]);
+            *reinterpret_cast<float2*>(ow + (2 * t + 1) * DP + d) = make_float2(o[i][1], o[i][3]);
+        }
+        __syncthreads();
+        for (int i = tid; i < cols * (DP / 4); i += kSplitWarps * 32) {
+            const int col = i / (DP / 4), d = 4 * (i % (DP / 4)), cc = col0 + col;
+            const int pos = pos0 + cc / p.G, splits = row_splits(p, pos);
+            if (d >= dh || it.split >= splits) continue;
+            float M = -INFINITY, L = 0.0f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kSplitWarps; ++w) M = fmaxf(M, ml[(w * kSplitCols + col) * 2]);
+            const float B = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < kSplitWarps; ++w) {
+                const float e = exp2_fast(ml[(w * kSplitCols + col) * 2] - B);
+                const float4 x = lds128f(mo + (w * kSplitCols + col) * DP + d);
+                L = ffma(ml[(w * kSplitCols + col) * 2 + 1], e, L);
+                acc.x = ffma(x.x, e, acc.x); acc.y = ffma(x.y, e, acc.y);
+                acc.z = ffma(x.z, e, acc.z); acc.w = ffma(x.w, e, acc.w);
+            }
+            const int row = it.a + cc / p.G, h = it.kvh * p.G + cc % p.G;
+            if (splits == 1) {
+                const float inv = L == 0.0f ? 0.0f : fdiv(1.0f, L);
+                *reinterpret_cast<float4*>(p.out + (size_t)row * p.ldo + (size_t)h * dh + d) =
+                    make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            } else {
+                float* pp = p.part + (((size_t)row * p.H + h) * p.nsplit + it.split) * (dh + 4);
+                *reinterpret_cast<float4*>(pp + d) = acc;
+                if (d == 0) { pp[dh] = M; pp[dh + 1] = L; }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// One warp per (row, head) with more than one split: joins them in split order. Grid
+// (rows, CTAs of 8 heads).
+static __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x, h = blockIdx.y * 8 + (threadIdx.x >> 5), dh = p.c.dh;
+    if (h >= p.H) return;
+    int pos = 0;
+    bool found = false;
+    for (int base = 0; base < p.r.n_seq && !found; base += 32) {
         SeqRows q{0, 0, 0};
         if (base + lane < p.r.n_seq) q = seq_rows(p.r, base + lane);
         const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
         if (m) {
-            const int src = __ffs(m) - 1;
-            s = base + src;
-            kv = __shfl_sync(0xffffffffu, q.kv, src);
-            pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, src);
+            pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, __ffs(m) - 1);
+            found = true;
         }
     }
-    if (s < 0) return;                                             // behind the last sequence
-    if (kv > p.r.cap && lane == 0) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
-    for (int d = lane; d < dh; d += 32) qs[warp][d] = p.q[(size_t)row * p.ldq + (size_t)h * dh + d];
-    __syncwarp();
-    const int n = min(pos + 1, p.r.cap), psz = 1 << p.c.page_log2;
-    float m = -INFINITY, l = 0.0f, o[8];
+    const int n = found ? row_splits(p, pos) : 0;
+    if (n < 2) return;
+    const int stride = dh + 4;
+    const float* base = p.part + ((size_t)row * p.H + h) * p.nsplit * stride;
+    float M = -INFINITY;
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, base[(size_t)s * stride + dh]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = 0.0f;
-    for (int j0 = 0; j0 < n; j0 += 32) {
-        const int j = j0 + lane;
-        float sc = -INFINITY, vs = 0.0f;
-        long long at = -1;
-        if (j < n) {
-            const int page = page_of(p.c, p.r, s, j);
-            if (page >= 0) {
-                const size_t head = (size_t)page * p.c.KVH + kvh;
-                const size_t cell = head * (psz / kKvBlock) + (j & (psz - 1)) / kKvBlock;
-                at = (long long)((head * psz + (j & (psz - 1))) * dh);
-                float a = 0.0f;
-                for (int d = 0; d < dh; d += 4) {
-                    const char4 w = *reinterpret_cast<const char4*>(p.c.k + at + d);
-                    a = ffma((float)w.x, qs[warp][d], a);
-                    a = ffma((float)w.y, qs[warp][d + 1], a);
-                    a = ffma((float)w.z, qs[warp][d + 2], a);
-                    a = ffma((float)w.w, qs[warp][d + 3], a);
-                }
-                sc = fmul(a, p.c.ks[cell]);
-                vs = p.c.vs[cell];
-            } else {
-                set_err(p.err, B2_DEV_ERR_BAD_PAGE);
-            }
-        }
-        float mx = sc;
-        for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        mx = fmaxf(mx, m);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        const float e = at < 0 ? 0.0f : exp_f(fsub(sc, base));
-        const float back = exp_f(fsub(m, base));
-        m = mx;
-        l = ffma(l, back, butterfly32(e));
+    for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    const float B = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int s = 0; s < n; ++s) {
+        const float* ps = base + (size_t)s * stride;
+        const float e = exp2_fast(ps[dh] - B);
+        L = ffma(ps[dh + 1], e, L);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmul(o[i], back);
-        const float w = at < 0 ? 0.0f : fmul(e, vs);
-        for (int t = 0; t < min(32, n - j0); ++t) {
-            const long long a = __shfl_sync(0xffffffffu, at, t);
-            const float wt = __shfl_sync(0xffffffffu, w, t);
-            if (a < 0) continue;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int d = lane + 32 * i;
-                if (d < dh) o[i] = ffma(wt, (float)p.c.v[a + d], o[i]);
-            }
+        for (int i = 0; i < 2; ++i) {
+            const int d = 4 * lane + 128 * i;
+            if (d >= dh) continue;
+            const float4 x = *reinterpret_cast<const float4*>(ps + d);
+            acc[i].x = ffma(x.x, e, acc[i].x); acc[i].y = ffma(x.y, e, acc[i].y);
+            acc[i].z = ffma(x.z, e, acc[i].z); acc[i].w = ffma(x.w, e, acc[i].w);
         }
     }
+    const float inv = L == 0.0f ? 0.0f : fdiv(1.0f, L);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        if (d < dh) p.out[(size_t)row * p.ldo + (size_t)h * dh + d] = l == 0.0f ? 0.0f : fdiv(o[i], l);
+    for (int i = 0; i < 2; ++i) {
+        const int d = 4 * lane + 128 * i;
+        if (d < dh)
+            *reinterpret_cast<float4*>(p.out + (size_t)row * p.ldo + (size_t)h * dh + d) =
+                make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
     }
 }
 
