@@ -3,6 +3,7 @@
 // nothing synchronised, and nothing read from device memory on the host.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -107,13 +108,27 @@ cudaError_t launch_append(AppendParams p, bool queries, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// keys per split: small ones fill the GPU when there are few rows; with long caches
-// larger ones bound the partial results and their joining (a function of the capacity
-// alone, so that a sequence's result does not depend on the others in the call)
-void attn_splits(PagedAttnParams& p) {
-    p.kc_log2 = p.r.cap <= 16384 ? 8 : p.r.cap <= 65536 ? 9 : 10;
-    p.nsplit = (p.r.cap + (1 << p.kc_log2) - 1) >> p.kc_log2;
-    if (p.nsplit < 1) p.nsplit = 1;
+// Which kernel, and the keys per split.
+//  few rows (up to 16 columns (token, head) of a KV head in the longest sequence, or on
+//  average if the caller does not say): 8 columns a CTA. Small splits fill the GPU when
+//  there are few rows; with long caches larger ones bound the partial results and their
+//  joining. A function of the capacity alone, so that a sequence's result does not
+//  depend on the others in the call.
+//  more: 64 rows a CTA; keys are split only while there are too few tiles for two
+//  rounds of the GPU.
+bool attn_plan(PagedAttnParams& p, int max_rows) {
+    const int G = p.H / p.c.KVH;
+    const long long cols = (max_rows > 0 ? max_rows : (p.r.n_rows + p.r.n_seq - 1) / std::max(p.r.n_seq, 1)) * (long long)G;
+    const bool few = cols <= 16;
+    if (few) {
+        p.kc = p.r.cap <= 16384 ? 256 : p.r.cap <= 65536 ? 512 : 1024;
+    } else {
+        const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / kTileRows), want = 2 * 148 * 3;
+        const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
+        p.kc = (int)std::max(256ll, ((p.r.cap + splits - 1) / splits + kTileKeys - 1) / kTileKeys * kTileKeys);
+    }
+    p.nsplit = std::max(1, (p.r.cap + p.kc - 1) / p.kc);
+    return few;
 }
 
 size_t part_bytes(const PagedAttnParams& p) {
@@ -126,6 +141,25 @@ int sm_count() {
     return n;
 }
 
+cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || p.nsplit == 1) return e;
+    paged_attn_join_kernel<<<dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), 256, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t launch_attn_tile(const PagedAttnParams& p, cudaStream_t s) {
+    using Sh = TileShape<DP>;
+    auto k = paged_attn_tile_kernel<DP>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
+    if (e != cudaSuccess) return e;
+    const long long most = ((long long)p.r.n_rows * p.G / kTileRows + p.r.n_seq) * p.c.KVH * p.nsplit;
+    if (most >= (1ll << 31)) return cudaErrorInvalidValue;
+    k<<<(unsigned)most, 128, Sh::Smem, s>>>(p);
+    return launch_join(p, s);
+}
+
 template <int DP>
 cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
     using Sh = SplitShape<DP>;
@@ -136,9 +170,12 @@ cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
     const long long tiles = ((long long)p.r.n_rows * p.G / kSplitCols + p.r.n_seq) * p.c.KVH;
     const long long most = tiles * p.nsplit, resident = (long long)sm_count() * (DP == 256 ? 2 : 4);
     k<<<(unsigned)(most < resident ? most : resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess || p.nsplit == 1) return e;
-    paged_attn_join_kernel<<<dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), 256, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_join(p, s);
+}
+
+template <int DP>
+cudaError_t launch_attn(const PagedAttnParams& p, bool few, cudaStream_t s) {
+    return few ? launch_attn_split<DP>(p, s) : launch_attn_tile<DP>(p, s);
 }
 
 }  // namespace
@@ -230,7 +267,7 @@ size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows,
     PagedAttnParams p{};
     if (!view("b2_attn_paged_i8_workspace", kv, rows, p.c, p.r) || n_heads <= 0 || n_heads % kv->n_kv_heads) return 0;
     p.H = n_heads;
-    attn_splits(p);
+    attn_plan(p, rows->max_rows);
     return part_bytes(p);
 }
 
@@ -249,14 +286,14 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     if (q == out) return refuse(fn, "out must not be q");
     if ((int64_t)p.r.n_rows * n_heads > (1ll << 30)) return refuse(fn, "more than 2^30 (row, head) pairs");
     p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.G = n_heads / kv->n_kv_heads; p.err = err;
-    attn_splits(p);
+    const bool few = attn_plan(p, rows->max_rows);
     const size_t need = part_bytes(p);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
     p.part = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return status(fn, kv->d_head <= 64 ? launch_attn_split<64>(p, s)
-                      : kv->d_head <= 128 ? launch_attn_split<128>(p, s) : launch_attn_split<256>(p, s));
+    return status(fn, kv->d_head <= 64 ? launch_attn<64>(p, few, s)
+                      : kv->d_head <= 128 ? launch_attn<128>(p, few, s) : launch_attn<256>(p, few, s));
 }
 
 }  // extern "C"

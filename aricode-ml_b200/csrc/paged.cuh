@@ -487,7 +487,7 @@ struct PagedAttnParams {
     float* out;              // [n_rows][ldo]
     long long ldq, ldo;
     int H, G;                // G = H / KVH
-    int kc_log2;             // keys per split
+    int kc;                  // keys per split
     int nsplit;              // splits of a sequence of cap keys
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
@@ -505,6 +505,9 @@ __device__ __forceinline__ long long shfl64(unsigned m, long long v, int src) {
                        (unsigned)__shfl_sync(m, (int)v, src));
 }
 
+// splits of n keys (at least one: it also writes rows that see none)
+__device__ __forceinline__ int splits_of(const PagedAttnParams& p, int n) { return max((n + p.kc - 1) / p.kc, 1); }
+
 // item number `item` of the call (tiles of NC columns), found by one warp
 template <int NC>
 __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, long long item, int lane) {
@@ -521,7 +524,7 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, long lon
                 if (q.kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
                 const int n = min(q.kv, p.r.cap);
                 tiles = (q.len * p.G + NC - 1) / NC;
-                cnt = (long long)tiles * p.c.KVH * max((n + (1 << p.kc_log2) - 1) >> p.kc_log2, 1);
+                cnt = (long long)tiles * p.c.KVH * splits_of(p, n);
             }
         }
         long long incl = cnt;
@@ -538,11 +541,12 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, long lon
             out.a = __shfl_sync(0xffffffffu, q.a, src);
             out.len = __shfl_sync(0xffffffffu, q.len, src);
             out.kv = __shfl_sync(0xffffffffu, q.kv, src);
-            tiles = __shfl_sync(0xffffffffu, tiles, src);
-            out.tile = (int)(idx % tiles);
-            const long long rest = idx / tiles;
-            out.kvh = (int)(rest % p.c.KVH);
-            out.split = (int)(rest / p.c.KVH);
+            // the last rows first: with causal lengths they are the longest
+            const int splits = splits_of(p, min(out.kv, p.r.cap));
+            const long long rest = idx / p.c.KVH;
+            out.kvh = (int)(idx % p.c.KVH);
+            out.split = (int)(rest % splits);
+            out.tile = __shfl_sync(0xffffffffu, tiles, src) - 1 - (int)(rest / splits);
             return out;
         }
         before += total;
@@ -550,9 +554,40 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, long lon
     return out;
 }
 
-// splits that a row at position pos has (at least one: it also writes empty rows)
+// splits that a row at position pos has
 __device__ __forceinline__ int row_splits(const PagedAttnParams& p, int pos) {
-    return max((min(pos + 1, p.r.cap) + (1 << p.kc_log2) - 1) >> p.kc_log2, 1);
+    return splits_of(p, min(pos + 1, p.r.cap));
+}
+
+// One query row (16 lanes, lane l16 the elements 4 l16 + 64 i ..) as digits: store(e, d,
+// word) takes digit e of elements d .. d + 3. *unit = the score of one integer unit in
+// base 2, NaN for a row that is not finite, 0 for one of zeros (`live` false: zeros).
+template <int DP, typename Store>
+__device__ __forceinline__ void query_digits(const float* qr, bool live, int dh, int l16, Store store, float* unit) {
+    constexpr int NE = DP / 64;
+    float4 x[NE];
+    float top = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const int d = 4 * (l16 + 16 * i);
+        x[i] = (live && d < dh) ? __ldg(reinterpret_cast<const float4*>(qr + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        bad |= x[i].x != x[i].x || x[i].y != x[i].y || x[i].z != x[i].z || x[i].w != x[i].w;
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+    }
+    if (bad) top = INFINITY;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float f = digit_factor(top);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        uint32_t w[3];
+        digits4(__float2int_rn(x[i].x * f), __float2int_rn(x[i].y * f), __float2int_rn(x[i].z * f),
+                __float2int_rn(x[i].w * f), w);
+#pragma unroll
+        for (int e = 0; e < 3; ++e) store(e, 4 * (l16 + 16 * i), w[e]);
+    }
+    if (l16 == 0) *unit = f > 0.0f ? __fdividef(1.4426950408889634f, f) : f;   // log2 e
 }
 
 // ---- few rows per sequence: a CTA of 4 warps takes 8 columns (token, head) of one KV
@@ -596,42 +631,17 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         const int col0 = it.tile * kSplitCols;                             // column = token * G + head
         const int pos_last = it.kv - it.len + (col0 + cols - 1) / p.G;     // of the tile's last row
         const int n = min(pos_last + 1, p.r.cap);                          // keys that any column sees
-        const int j0 = it.split << p.kc_log2;
+        const int j0 = it.split * p.kc;
         if (j0 >= n && it.split > 0) continue;                             // the tile ends before this split
-        const int jend = min(n, j0 + (1 << p.kc_log2));
+        const int jend = min(n, j0 + p.kc);
 
         // queries -> digits: 16 lanes a column
         {
-            const int col = tid >> 4, l16 = tid & 15;
-            const int cc = col0 + col;
-            const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
-            constexpr int NE = DP / 64;                                    // float4s a lane
-            float4 x[NE];
-            float top = 0.0f;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const int d = 4 * (l16 + 16 * i);
-                x[i] = (col < cols && d < dh) ? __ldg(reinterpret_cast<const float4*>(qr + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float mx = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-                bad |= x[i].x != x[i].x || x[i].y != x[i].y || x[i].z != x[i].z || x[i].w != x[i].w;
-                top = fmaxf(top, mx);
-            }
-            if (bad) top = __int_as_float(0x7f800000);
-#pragma unroll
-            for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float f = digit_factor(top);
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const int d = 4 * (l16 + 16 * i);
-                uint32_t w[3];
-                digits4(__float2int_rn(x[i].x * f), __float2int_rn(x[i].y * f), __float2int_rn(x[i].z * f),
-                        __float2int_rn(x[i].w * f), w);
-#pragma unroll
-                for (int e = 0; e < 3; ++e) *reinterpret_cast<uint32_t*>(qd + (e * kSplitCols + col) * DP + d) = w[e];
-            }
-            // unit of the scores in base 2; NaN for a query that is not finite
-            if (l16 == 0) sq[col] = f > 0.0f ? __fdividef(1.4426950408889634f, f) : (f == 0.0f ? 0.0f : f);
+            const int col = tid >> 4, cc = col0 + col;
+            query_digits<DP>(p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh, col < cols, dh,
+                             tid & 15, [&](int e, int d, uint32_t w) {
+                                 *reinterpret_cast<uint32_t*>(qd + (e * kSplitCols + col) * DP + d) = w;
+                             }, sq + col);
         }
         __syncthreads();
         uint32_t qb[3][Sh::NH][4];                                         // B fragments of column g
@@ -848,6 +858,309 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             }
         }
         __syncthreads();
+    }
+}
+
+// ---- many rows per sequence: a CTA of 4 warps takes 64 rows ((token, head) pairs of
+// one KV head), warp w 16 of them, against a split of the keys in tiles of 64. A =
+// query or weight digits (rows x 32), B = codes: keys as they lie, values turned to
+// [d][key] on their way into shared memory (byte permutes, once for the CTA). The
+// key order inside a B fragment of the values is the one that the score fragments
+// already have, so weights go from scores to A fragments inside their thread.
+// Codes of tile i + 1 are on their way while tile i is computed.
+constexpr int kTileRows = 64;
+constexpr int kTileKeys = 64;
+
+template <int DP>
+struct TileShape {
+    static constexpr int NH = DP / 64;
+    static constexpr int NT = DP / 8;                          // output tiles of 8 elements
+    static constexpr int QBytes = 3 * kTileRows * DP;
+    static constexpr int KBytes = kTileKeys * DP;
+    static constexpr int Smem = QBytes + 4 * KBytes + kTileRows * 4 + 2 * 12 * 4 + 2 * 4 * 4;
+};
+
+// 16-byte unit u of a row of DP bytes, swapped between halves in odd rows so that the
+// fragment loads of two neighbouring rows meet no bank twice
+template <int DP>
+__device__ __forceinline__ int unit_at(int row, int u) {
+    return row * DP + 16 * (DP >= 128 ? u ^ ((row & 1) << 2) : u);
+}
+
+// row d of the turned values ([DP][64 keys] bytes): neighbours swapped in every other
+// group of 16, so that the stores of two groups meet no bank twice
+__device__ __forceinline__ int value_row(int d) { return (d ^ ((d >> 4) & 1)) * kTileKeys; }
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+template <int DP>
+__global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel(const __grid_constant__ PagedAttnParams p) {
+    using Sh = TileShape<DP>;
+    extern __shared__ __align__(16) unsigned char pt_raw[];
+    uint8_t* qd = pt_raw;                                      // [3][64][DP]
+    uint8_t* kt = qd + Sh::QBytes;                             // [2][64][DP]
+    uint8_t* vt = kt + 2 * Sh::KBytes;                         // [2][DP][64]
+    float* sq = reinterpret_cast<float*>(vt + 2 * Sh::KBytes); // [64]
+    float* sc = sq + kTileRows;                                // [2][12]: 4 key scales, 4 value scales, 4 "there"
+    int* pg = reinterpret_cast<int*>(sc + 24);                 // [2][4] pages of a tile's blocks
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int dh = p.c.dh, psz = 1 << p.c.page_log2;
+
+    const AttnItem it = find_item<kTileRows>(p, blockIdx.x, lane);
+    if (it.s < 0) return;
+    const int row0 = it.tile * kTileRows, rows = min(it.len * p.G - row0, kTileRows);
+    const int pos0 = it.kv - it.len;
+    const int n = min(pos0 + (row0 + rows - 1) / p.G + 1, p.r.cap);      // keys that any row sees
+    const int j0 = it.split * p.kc, jend = min(n, j0 + p.kc);
+    if (j0 >= n && it.split > 0) return;
+    const int ntiles = max((jend - j0 + kTileKeys - 1) / kTileKeys, 0);
+
+    auto page_at = [&](int j) { return j < jend ? page_of(p.c, p.r, it.s, j) : -2; };   // -2: past the end
+    auto cell_at = [&](int page, int j) {
+        return ((size_t)max(page, 0) * p.c.KVH + it.kvh) * (psz >> 4) + ((j & (psz - 1)) >> 4);
+    };
+    if (tid < 8 && ntiles > 0) pg[tid] = page_at(j0 + 16 * tid);
+
+    // queries -> digits: 16 lanes a row
+#pragma unroll 1
+    for (int r = tid >> 4; r < kTileRows; r += 8) {
+        const int l16 = tid & 15, cc = row0 + r;
+        const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
+        query_digits<DP>(qr, r < rows, dh, l16, [&](int e, int d, uint32_t w) {
+            *reinterpret_cast<uint32_t*>(qd + e * kTileRows * DP + unit_at<DP>(r, d >> 4) + (d & 15)) = w;
+        }, sq + r);
+    }
+    __syncthreads();
+
+    // this thread's part of a value tile: block vb, keys 2 vt_ + {0, 1, 8, 9} of it, 16 elements from 16 vc
+    const int vb = lane >> 3, vq = (lane >> 1) & 3;
+    constexpr int VC = DP == 256 ? 2 : 1;
+    uint4 vr[VC][4];
+    auto load_tile = [&](int i) {                              // keys by cp.async, values into registers
+        const int j = j0 + i * kTileKeys, b = i & 1;
+        uint8_t* kd = kt + b * Sh::KBytes;
+#pragma unroll
+        for (int x = 0; x < kTileKeys * DP / 16 / 128; ++x) {
+            const int unit = x * 128 + tid, key = unit / (DP / 16), u = unit % (DP / 16);
+            const int page = pg[4 * b + (key >> 4)];
+            const bool there = page >= 0 && 16 * u < dh;
+            const size_t at = there ? (cell_at(page, j + key) * kKvBlock + (key & 15)) * dh + 16 * u : 0;
+            cp_async16(kd + unit_at<DP>(key, u), p.c.k + at, there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const int page = pg[4 * b + vb];
+#pragma unroll
+        for (int x = 0; x < VC; ++x) {
+            const int d = 16 * (2 * warp + (lane & 1) + 8 * x);
+            const bool there = page >= 0 && d < dh;
+            const int8_t* src = p.c.v + (there ? (cell_at(page, j + 16 * vb) * kKvBlock + 2 * vq) * dh + d : 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                vr[x][k] = there ? __ldg(reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (tid < 8) {                                         // scales of the tile's blocks
+            const int pb = pg[4 * b + (tid & 3)];
+            const size_t cell = cell_at(pb, j + 16 * (tid & 3));
+            sc[12 * b + tid] = pb >= 0 ? __ldg((tid < 4 ? p.c.ks : p.c.vs) + cell) : 0.0f;
+            if (tid < 4) sc[12 * b + 8 + tid] = pb >= 0 ? 1.0f : 0.0f;
+            if (pb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+        }
+    };
+    auto store_values = [&](int i) {
+        uint8_t* vd = vt + (i & 1) * Sh::KBytes;
+#pragma unroll
+        for (int x = 0; x < VC; ++x) {
+            const int d = 16 * (2 * warp + (lane & 1) + 8 * x);
+            if (d >= DP) continue;
+            const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[x][0]);
+            const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[x][1]);
+            const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[x][2]);
+            const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[x][3]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t a = __byte_perm(w0[w], w1[w], 0x5140), b = __byte_perm(w2[w], w3[w], 0x5140);
+                const uint32_t c = __byte_perm(w0[w], w1[w], 0x7362), e = __byte_perm(w2[w], w3[w], 0x7362);
+                const int at = 16 * vq + 4 * vb;
+                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w) + at) = __byte_perm(a, b, 0x5410);
+                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w + 1) + at) = __byte_perm(a, b, 0x7632);
+                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w + 2) + at) = __byte_perm(c, e, 0x5410);
+                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w + 3) + at) = __byte_perm(c, e, 0x7632);
+            }
+        }
+    };
+
+    // rows ra = 16 warp + g and ra + 8
+    const int ra = 16 * warp + g;
+    const int lim0 = ra < rows ? min(pos0 + (row0 + ra) / p.G + 1, n) : 0;
+    const int lim1 = ra + 8 < rows ? min(pos0 + (row0 + ra + 8) / p.G + 1, n) : 0;
+    int wmin = min(lim0, lim1), wmax = max(lim0, lim1);        // of the warp's rows
+    wmin = __reduce_min_sync(0xffffffffu, wmin);
+    wmax = __reduce_max_sync(0xffffffffu, wmax);
+    const float sq0 = sq[ra], sq1 = sq[ra + 8];
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    float o[Sh::NT][4];
+#pragma unroll
+    for (int i = 0; i < Sh::NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+    if (ntiles > 0) {
+        load_tile(0);
+        store_values(0);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+    }
+#pragma unroll 1
+    for (int i = 0; i < ntiles; ++i) {
+        const int j = j0 + i * kTileKeys;
+        const bool more = i + 1 < ntiles;
+        if (more) load_tile(i + 1);
+        if (tid >= 120 && tid < 124) pg[4 * (i & 1) + tid - 120] = page_at(j + 2 * kTileKeys + 16 * (tid - 120));
+        if (wmax > j) {
+            const uint8_t* kd = kt + (i & 1) * Sh::KBytes;
+            const float* scb = sc + 12 * (i & 1);
+            float s[8][4];                                     // rows g (0, 1), g + 8 (2, 3); keys 8 nt + 2t, + 1
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {             // 32 keys at a time
+                int c[4][3][4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) c[x][e][0] = c[x][e][1] = c[x][e][2] = c[x][e][3] = 0;
+#pragma unroll
+                for (int h = 0; h < Sh::NH; ++h) {
+                    uint4 b[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) b[x] = lds128(kd + unit_at<DP>(32 * half + 8 * x + g, 4 * h + t));
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        const uint4 a0 = lds128(qd + e * kTileRows * DP + unit_at<DP>(ra, 4 * h + t));
+                        const uint4 a1 = lds128(qd + e * kTileRows * DP + unit_at<DP>(ra + 8, 4 * h + t));
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            mma_s8(c[x][e], a0.x, a1.x, a0.y, a1.y, b[x].x, b[x].y);
+                            mma_s8(c[x][e], a0.z, a1.z, a0.w, a1.w, b[x].z, b[x].w);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float u = scb[2 * half + (x >> 1)];
+                    const float u0 = sq0 * u, u1 = sq1 * u;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        s[4 * half + x][y] = join_digits(c[x][2][y], c[x][1][y], c[x][0][y]) * (y < 2 ? u0 : u1);
+                }
+            }
+            const bool whole = j + kTileKeys <= wmin && scb[8] + scb[9] + scb[10] + scb[11] == 4.0f;
+            if (!whole) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        if (!(j + 8 * x + 2 * t + (y & 1) < (y < 2 ? lim0 : lim1) && scb[8 + (x >> 1)] != 0.0f)) s[x][y] = -INFINITY;
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                mx0 = fmaxf(mx0, fmaxf(s[x][0], s[x][1]));
+                mx1 = fmaxf(mx1, fmaxf(s[x][2], s[x][3]));
+            }
+#pragma unroll
+            for (int x = 1; x <= 2; x <<= 1) {
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+            }
+            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+            const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
+            const float back0 = exp2_fast(m0 - b0), back1 = exp2_fast(m1 - b1);
+            m0 = n0; m1 = n1;
+            l0 *= back0; l1 *= back1;
+            float wt0 = 0.0f, wt1 = 0.0f;
+            bool nan0 = false, nan1 = false;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const float sv = scb[4 + (x >> 1)];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float ev = exp2_fast(s[x][y] - (y < 2 ? b0 : b1));
+                    if (y < 2) l0 += ev; else l1 += ev;
+                    float w = ev * sv;
+                    if (!whole && s[x][y] == -INFINITY) w = 0.0f;          // even where the scale is NaN
+                    s[x][y] = w;
+                    if (y < 2) { wt0 = fmaxf(wt0, w); nan0 |= w != w; }
+                    else { wt1 = fmaxf(wt1, w); nan1 |= w != w; }
+                }
+            }
+            if (nan0) wt0 = INFINITY;
+            if (nan1) wt1 = INFINITY;
+#pragma unroll
+            for (int x = 1; x <= 2; x <<= 1) {
+                wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
+                wt1 = fmaxf(wt1, __shfl_xor_sync(0xffffffffu, wt1, x));
+            }
+            const float f0 = digit_factor(wt0), f1 = digit_factor(wt1);
+            const float u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0, u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
+            // weights as digits: A fragments [32-key step][digit][register]
+            uint32_t wa[2][3][4];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)                    // 16 keys: registers 2 b (row g) and 2 b + 1 (row g + 8)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float f = r ? f1 : f0;
+                        const float(&x0)[4] = s[4 * ks + 2 * b];
+                        const float(&x1)[4] = s[4 * ks + 2 * b + 1];
+                        // adding 2^23 leaves the rounded integer in the low bits (0 <= w f < 2^23)
+                        uint32_t dg[3];
+                        digits4(__float_as_int(ffma(x0[2 * r], f, 8388608.0f)), __float_as_int(ffma(x0[2 * r + 1], f, 8388608.0f)),
+                                __float_as_int(ffma(x1[2 * r], f, 8388608.0f)), __float_as_int(ffma(x1[2 * r + 1], f, 8388608.0f)), dg);
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) wa[ks][e][2 * b + r] = dg[e];
+                    }
+            const uint8_t* vd = vt + (i & 1) * Sh::KBytes;
+#pragma unroll
+            for (int x = 0; x < Sh::NT; ++x) {
+                const uint4 b = lds128(vd + value_row(8 * x + g) + 16 * t);
+                int c[3][4] = {};
+#pragma unroll
+                for (int e = 0; e < 3; ++e) {
+                    mma_s8(c[e], wa[0][e][0], wa[0][e][1], wa[0][e][2], wa[0][e][3], b.x, b.y);
+                    mma_s8(c[e], wa[1][e][0], wa[1][e][1], wa[1][e][2], wa[1][e][3], b.z, b.w);
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    o[x][y] = ffma(join_digits(c[2][y], c[1][y], c[0][y]), y < 2 ? u0 : u1, o[x][y] * (y < 2 ? back0 : back1));
+            }
+        }
+        if (more) {
+            store_values(i + 1);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int rr = ra + 8 * r, cc = row0 + rr;
+        if (rr >= rows) continue;
+        const int splits = row_splits(p, pos0 + cc / p.G);
+        if (it.split >= splits) continue;
+        const int row = it.a + cc / p.G, h = it.kvh * p.G + cc % p.G;
+        const float L = r ? l1 : l0, inv = splits > 1 ? 1.0f : L == 0.0f ? 0.0f : fdiv(1.0f, L);
+        float* dst = splits > 1 ? p.part + (((size_t)row * p.H + h) * p.nsplit + it.split) * (dh + 4)
+                                : p.out + (size_t)row * p.ldo + (size_t)h * dh;
+#pragma unroll
+        for (int x = 0; x < Sh::NT; ++x) {
+            const int d = 8 * x + 2 * t;
+            if (d < dh) *reinterpret_cast<float2*>(dst + d) = make_float2(o[x][2 * r] * inv, o[x][2 * r + 1] * inv);
+        }
+        if (splits > 1 && t == 0) { dst[dh] = r ? m1 : m0; dst[dh + 1] = L; }
     }
 }
 
