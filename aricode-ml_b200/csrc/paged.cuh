@@ -453,10 +453,29 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// digits of four integers: word e of d holds digit e of x[0 .. 3] in its bytes
-__device__ __forceinline__ void digits4(int x0, int x1, int x2, int x3, uint32_t (&d)[3]) {
-    const uint32_t y0 = (uint32_t)x0 + 0x8080u, y1 = (uint32_t)x1 + 0x8080u, y2 = (uint32_t)x2 + 0x8080u,
-                   y3 = (uint32_t)x3 + 0x8080u;
+// The first of a chain: the sums start at kSumBase, the bits of 1.5 * 2^23 in f32, so
+// that a sum (at most 2^22: 256 products of two signed bytes) is read as the float
+// kSumF + sum and one subtraction makes it a number; nothing is cleared or converted.
+constexpr int kSumBase = 0x4B400000;
+constexpr float kSumF = 12582912.0f;
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kSumBase));
+}
+__device__ __forceinline__ float sum_of(int c) { return fsub(__int_as_float(c), kSumF); }
+
+// rint(x f) + 0x8080 for |x f| <= kDigitMax, in the low 24 bits
+__device__ __forceinline__ uint32_t digit_bits(float x, float f) { return (uint32_t)__float2int_rn(x * f) + 0x8080u; }
+// the same for x >= 0 in one operation: the f32 addition rounds x f to an integer
+__device__ __forceinline__ uint32_t digit_bits_pos(float x, float f) {
+    return __float_as_uint(ffma(x, f, 8388608.0f + (float)0x8080));
+}
+
+// digits of four integers given as digit_bits: word e of d holds digit e of each in its bytes
+__device__ __forceinline__ void digits4(uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3, uint32_t (&d)[3]) {
     const uint32_t l = __byte_perm(y0, y1, 0x5140), m = __byte_perm(y2, y3, 0x5140);
     d[0] = __byte_perm(l, m, 0x5410) ^ 0x80808080u;
     d[1] = __byte_perm(l, m, 0x7632) ^ 0x80808080u;
@@ -464,7 +483,7 @@ __device__ __forceinline__ void digits4(int x0, int x1, int x2, int x3, uint32_t
 }
 
 __device__ __forceinline__ float join_digits(int d2, int d1, int d0) {
-    return ffma((float)d2, 65536.0f, ffma((float)d1, 256.0f, (float)d0));
+    return ffma(sum_of(d2), 65536.0f, ffma(sum_of(d1), 256.0f, sum_of(d0)));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -582,8 +601,7 @@ __device__ __forceinline__ void query_digits(const float* qr, bool live, int dh,
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
         uint32_t w[3];
-        digits4(__float2int_rn(x[i].x * f), __float2int_rn(x[i].y * f), __float2int_rn(x[i].z * f),
-                __float2int_rn(x[i].w * f), w);
+        digits4(digit_bits(x[i].x, f), digit_bits(x[i].y, f), digit_bits(x[i].z, f), digit_bits(x[i].w, f), w);
 #pragma unroll
         for (int e = 0; e < 3; ++e) store(e, 4 * (l16 + 16 * i), w[e]);
     }
@@ -617,12 +635,12 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(16) unsigned char ps_raw[];
     uint8_t* qd = ps_raw;                                                  // [3][8][DP] digits of the queries
     float* sq = reinterpret_cast<float*>(ps_raw + Sh::QBytes);             // [8] their units (log2 e in)
-    int* wx = reinterpret_cast<int*>(ps_raw + Sh::QBytes + 64);            // [4][8][WStride] weights
+    uint32_t* wx = reinterpret_cast<uint32_t*>(ps_raw + Sh::QBytes + 64);            // [4][8][WStride] weights
     float* mo = reinterpret_cast<float*>(ps_raw + Sh::QBytes + 64 + Sh::WBytes);   // [4][8][DP]
     float* ml = mo + kSplitWarps * kSplitCols * DP;                        // [4][8][2]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int dh = p.c.dh, psz = 1 << p.c.page_log2;
-    int* wxw = wx + warp * kSplitCols * Sh::WStride;
+    uint32_t* wxw = wx + warp * kSplitCols * Sh::WStride;
 
     for (long long item = blockIdx.x;; item += gridDim.x) {
         const AttnItem it = find_item<kSplitCols>(p, item, lane);
@@ -717,12 +735,13 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                int c[3][4] = {};
+                int c[3][4];
 #pragma unroll
                 for (int h = 0; h < Sh::NH; ++h)
 #pragma unroll
                     for (int e = 0; e < 3; ++e) {
-                        mma_s8(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
+                        if (h == 0) mma_s8_first(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
+                        else mma_s8(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
                         mma_s8(c[e], kf[b][0][h].z, kf[b][1][h].z, kf[b][0][h].w, kf[b][1][h].w, qb[e][h][2], qb[e][h][3]);
                     }
                 const float u0 = sq0 * sk[b], u1 = sq1 * sk[b];
@@ -759,7 +778,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                     const float w0 = s[b][2 * r] == -INFINITY ? 0.0f : e0 * sv[b];
                     const float w1 = s[b][2 * r + 1] == -INFINITY ? 0.0f : e1 * sv[b];
                     s[b][2 * r] = w0; s[b][2 * r + 1] = w1;
-                    wt0 = fmaxf(wt0, fabsf(w0)); wt1 = fmaxf(wt1, fabsf(w1));
+                    wt0 = fmaxf(wt0, w0); wt1 = fmaxf(wt1, w1);
                     nan0 |= w0 != w0; nan1 |= w1 != w1;
                 }
             if (nan0) wt0 = INFINITY;
@@ -775,15 +794,15 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    wxw[2 * t * Sh::WStride + 16 * b + 8 * r + g] = __float2int_rn(s[b][2 * r] * f0);
-                    wxw[(2 * t + 1) * Sh::WStride + 16 * b + 8 * r + g] = __float2int_rn(s[b][2 * r + 1] * f1);
+                    wxw[2 * t * Sh::WStride + 16 * b + 8 * r + g] = digit_bits_pos(s[b][2 * r], f0);
+                    wxw[(2 * t + 1) * Sh::WStride + 16 * b + 8 * r + g] = digit_bits_pos(s[b][2 * r + 1], f1);
                 }
             __syncwarp();
             uint32_t wb[2][3];                                             // B fragments: keys 4t .., 16 + 4t .. of column g
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const uint4 w = lds128(wxw + g * Sh::WStride + 16 * b + 4 * t);
-                digits4((int)w.x, (int)w.y, (int)w.z, (int)w.w, wb[b]);
+                digits4(w.x, w.y, w.z, w.w, wb[b]);
             }
             const float u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0, u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
             // output elements (DP / 8) g + 2 m, + 1 (rows g and g + 8 of tile m): four keys' bytes of one element
@@ -800,10 +819,10 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    int c[3][4] = {};
+                    int c[3][4];
 #pragma unroll
                     for (int e = 0; e < 3; ++e)
-                        mma_s8(c[e], a[0][2 * k], a[0][2 * k + 1], a[1][2 * k], a[1][2 * k + 1], wb[0][e], wb[1][e]);
+                        mma_s8_first(c[e], a[0][2 * k], a[0][2 * k + 1], a[1][2 * k], a[1][2 * k + 1], wb[0][e], wb[1][e]);
                     float(&oo)[4] = o[2 * w + k];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -877,7 +896,7 @@ struct TileShape {
     static constexpr int NT = DP / 8;                          // output tiles of 8 elements
     static constexpr int QBytes = 3 * kTileRows * DP;
     static constexpr int KBytes = kTileKeys * DP;
-    static constexpr int Smem = QBytes + 4 * KBytes + kTileRows * 4 + 2 * 12 * 4 + 2 * 4 * 4;
+    static constexpr int Smem = QBytes + 4 * KBytes + kTileRows * 4 + 2 * 12 * 4 + 2 * 4 * 8;
 };
 
 // 16-byte unit u of a row of DP bytes, swapped between halves in odd rows so that the
@@ -904,7 +923,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
     uint8_t* vt = kt + 2 * Sh::KBytes;                         // [2][DP][64]
     float* sq = reinterpret_cast<float*>(vt + 2 * Sh::KBytes); // [64]
     float* sc = sq + kTileRows;                                // [2][12]: 4 key scales, 4 value scales, 4 "there"
-    int* pg = reinterpret_cast<int*>(sc + 24);                 // [2][4] pages of a tile's blocks
+    long long* cell = reinterpret_cast<long long*>(sc + 24);   // [2][4] a tile's blocks in the pool
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int dh = p.c.dh, psz = 1 << p.c.page_log2;
 
@@ -917,11 +936,14 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
     if (j0 >= n && it.split > 0) return;
     const int ntiles = max((jend - j0 + kTileKeys - 1) / kTileKeys, 0);
 
-    auto page_at = [&](int j) { return j < jend ? page_of(p.c, p.r, it.s, j) : -2; };   // -2: past the end
-    auto cell_at = [&](int page, int j) {
-        return ((size_t)max(page, 0) * p.c.KVH + it.kvh) * (psz >> 4) + ((j & (psz - 1)) >> 4);
+    // a block's number in the pool (its codes start at 16 dh times that); -1: page outside
+    // the pool, -2: past the end
+    auto cell_at = [&](int j) -> long long {
+        if (j >= jend) return -2;
+        const int page = page_of(p.c, p.r, it.s, j);
+        return page < 0 ? -1 : ((long long)page * p.c.KVH + it.kvh) * (psz >> 4) + ((j & (psz - 1)) >> 4);
     };
-    if (tid < 8 && ntiles > 0) pg[tid] = page_at(j0 + 16 * tid);
+    if (tid < 8 && ntiles > 0) cell[tid] = cell_at(j0 + 16 * tid);
 
     // queries -> digits: 16 lanes a row
 #pragma unroll 1
@@ -939,33 +961,31 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
     constexpr int VC = DP == 256 ? 2 : 1;
     uint4 vr[VC][4];
     auto load_tile = [&](int i) {                              // keys by cp.async, values into registers
-        const int j = j0 + i * kTileKeys, b = i & 1;
+        const int b = i & 1;
         uint8_t* kd = kt + b * Sh::KBytes;
 #pragma unroll
         for (int x = 0; x < kTileKeys * DP / 16 / 128; ++x) {
             const int unit = x * 128 + tid, key = unit / (DP / 16), u = unit % (DP / 16);
-            const int page = pg[4 * b + (key >> 4)];
-            const bool there = page >= 0 && 16 * u < dh;
-            const size_t at = there ? (cell_at(page, j + key) * kKvBlock + (key & 15)) * dh + 16 * u : 0;
-            cp_async16(kd + unit_at<DP>(key, u), p.c.k + at, there);
+            const long long at = cell[4 * b + (key >> 4)];
+            const bool there = at >= 0 && 16 * u < dh;
+            cp_async16(kd + unit_at<DP>(key, u), p.c.k + (there ? at * (kKvBlock * dh) + (key & 15) * dh + 16 * u : 0), there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const int page = pg[4 * b + vb];
+        const long long at = cell[4 * b + vb];
 #pragma unroll
         for (int x = 0; x < VC; ++x) {
             const int d = 16 * (2 * warp + (lane & 1) + 8 * x);
-            const bool there = page >= 0 && d < dh;
-            const int8_t* src = p.c.v + (there ? (cell_at(page, j + 16 * vb) * kKvBlock + 2 * vq) * dh + d : 0);
+            const bool there = at >= 0 && d < dh;
+            const int8_t* src = p.c.v + (there ? at * (kKvBlock * dh) + 2 * vq * dh + d : 0);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 vr[x][k] = there ? __ldg(reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh)) : make_uint4(0u, 0u, 0u, 0u);
         }
         if (tid < 8) {                                         // scales of the tile's blocks
-            const int pb = pg[4 * b + (tid & 3)];
-            const size_t cell = cell_at(pb, j + 16 * (tid & 3));
-            sc[12 * b + tid] = pb >= 0 ? __ldg((tid < 4 ? p.c.ks : p.c.vs) + cell) : 0.0f;
-            if (tid < 4) sc[12 * b + 8 + tid] = pb >= 0 ? 1.0f : 0.0f;
-            if (pb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+            const long long cb = cell[4 * b + (tid & 3)];
+            sc[12 * b + tid] = cb >= 0 ? __ldg((tid < 4 ? p.c.ks : p.c.vs) + cb) : 0.0f;
+            if (tid < 4) sc[12 * b + 8 + tid] = cb >= 0 ? 1.0f : 0.0f;
+            if (cb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
         }
     };
     auto store_values = [&](int i) {
@@ -1015,7 +1035,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
         const int j = j0 + i * kTileKeys;
         const bool more = i + 1 < ntiles;
         if (more) load_tile(i + 1);
-        if (tid >= 120 && tid < 124) pg[4 * (i & 1) + tid - 120] = page_at(j + 2 * kTileKeys + 16 * (tid - 120));
+        if (tid >= 120 && tid < 124) cell[4 * (i & 1) + tid - 120] = cell_at(j + 2 * kTileKeys + 16 * (tid - 120));
         if (wmax > j) {
             const uint8_t* kd = kt + (i & 1) * Sh::KBytes;
             const float* scb = sc + 12 * (i & 1);
@@ -1024,10 +1044,6 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
 #pragma unroll
             for (int half = 0; half < 2; ++half) {             // 32 keys at a time
                 int c[4][3][4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int e = 0; e < 3; ++e) c[x][e][0] = c[x][e][1] = c[x][e][2] = c[x][e][3] = 0;
 #pragma unroll
                 for (int h = 0; h < Sh::NH; ++h) {
                     uint4 b[4];
@@ -1039,7 +1055,8 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
                         const uint4 a1 = lds128(qd + e * kTileRows * DP + unit_at<DP>(ra + 8, 4 * h + t));
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            mma_s8(c[x][e], a0.x, a1.x, a0.y, a1.y, b[x].x, b[x].y);
+                            if (h == 0) mma_s8_first(c[x][e], a0.x, a1.x, a0.y, a1.y, b[x].x, b[x].y);
+                            else mma_s8(c[x][e], a0.x, a1.x, a0.y, a1.y, b[x].x, b[x].y);
                             mma_s8(c[x][e], a0.z, a1.z, a0.w, a1.w, b[x].z, b[x].w);
                         }
                     }
@@ -1076,24 +1093,36 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
             const float back0 = exp2_fast(m0 - b0), back1 = exp2_fast(m1 - b1);
             m0 = n0; m1 = n1;
             l0 *= back0; l1 *= back1;
+            // weights p v_scale. A score that is not a number has made l NaN, which is
+            // enough; a value scale that is not one needs the checks
             float wt0 = 0.0f, wt1 = 0.0f;
-            bool nan0 = false, nan1 = false;
+            const float svs = scb[4] + scb[5] + scb[6] + scb[7];
+            if (svs == svs) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                const float sv = scb[4 + (x >> 1)];
+                for (int x = 0; x < 8; ++x) {
+                    const float sv = scb[4 + (x >> 1)];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const float ev = exp2_fast(s[x][y] - (y < 2 ? b0 : b1));
-                    if (y < 2) l0 += ev; else l1 += ev;
-                    float w = ev * sv;
-                    if (!whole && s[x][y] == -INFINITY) w = 0.0f;          // even where the scale is NaN
-                    s[x][y] = w;
-                    if (y < 2) { wt0 = fmaxf(wt0, w); nan0 |= w != w; }
-                    else { wt1 = fmaxf(wt1, w); nan1 |= w != w; }
+                    for (int y = 0; y < 4; ++y) {
+                        const float ev = exp2_fast(s[x][y] - (y < 2 ? b0 : b1));
+                        if (y < 2) l0 += ev; else l1 += ev;
+                        s[x][y] = ev * sv;
+                        if (y < 2) wt0 = fmaxf(wt0, s[x][y]); else wt1 = fmaxf(wt1, s[x][y]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const float sv = scb[4 + (x >> 1)];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const float ev = exp2_fast(s[x][y] - (y < 2 ? b0 : b1));
+                        if (y < 2) l0 += ev; else l1 += ev;
+                        s[x][y] = s[x][y] == -INFINITY ? 0.0f : ev * sv;   // masked: nothing, whatever the scale
+                        if (s[x][y] != s[x][y]) { if (y < 2) wt0 = INFINITY; else wt1 = INFINITY; }
+                        if (y < 2) wt0 = fmaxf(wt0, s[x][y]); else wt1 = fmaxf(wt1, s[x][y]);
+                    }
                 }
             }
-            if (nan0) wt0 = INFINITY;
-            if (nan1) wt1 = INFINITY;
 #pragma unroll
             for (int x = 1; x <= 2; x <<= 1) {
                 wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
@@ -1112,10 +1141,9 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
                         const float f = r ? f1 : f0;
                         const float(&x0)[4] = s[4 * ks + 2 * b];
                         const float(&x1)[4] = s[4 * ks + 2 * b + 1];
-                        // adding 2^23 leaves the rounded integer in the low bits (0 <= w f < 2^23)
                         uint32_t dg[3];
-                        digits4(__float_as_int(ffma(x0[2 * r], f, 8388608.0f)), __float_as_int(ffma(x0[2 * r + 1], f, 8388608.0f)),
-                                __float_as_int(ffma(x1[2 * r], f, 8388608.0f)), __float_as_int(ffma(x1[2 * r + 1], f, 8388608.0f)), dg);
+                        digits4(digit_bits_pos(x0[2 * r], f), digit_bits_pos(x0[2 * r + 1], f), digit_bits_pos(x1[2 * r], f),
+                                digit_bits_pos(x1[2 * r + 1], f), dg);
 #pragma unroll
                         for (int e = 0; e < 3; ++e) wa[ks][e][2 * b + r] = dg[e];
                     }
@@ -1123,10 +1151,10 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
 #pragma unroll
             for (int x = 0; x < Sh::NT; ++x) {
                 const uint4 b = lds128(vd + value_row(8 * x + g) + 16 * t);
-                int c[3][4] = {};
+                int c[3][4];
 #pragma unroll
                 for (int e = 0; e < 3; ++e) {
-                    mma_s8(c[e], wa[0][e][0], wa[0][e][1], wa[0][e][2], wa[0][e][3], b.x, b.y);
+                    mma_s8_first(c[e], wa[0][e][0], wa[0][e][1], wa[0][e][2], wa[0][e][3], b.x, b.y);
                     mma_s8(c[e], wa[1][e][0], wa[1][e][1], wa[1][e][2], wa[1][e][3], b.z, b.w);
                 }
 #pragma unroll
