@@ -465,14 +465,48 @@ __device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t 
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kSumBase));
 }
-__device__ __forceinline__ float sum_of(int c) { return fsub(__int_as_float(c), kSumF); }
+
+// two f32 in one instruction: the attention kernels are bound by what the schedulers
+// issue, and a packed operation takes one slot for two (same rounding)
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 pack2i(int a, int b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// two neighbouring digit sums as numbers
+__device__ __forceinline__ f32x2 sums_of(int a, int b) { return add2(pack2i(a, b), pack2(-kSumF, -kSumF)); }
 
 // rint(x f) + 0x8080 for |x f| <= kDigitMax, in the low 24 bits
 __device__ __forceinline__ uint32_t digit_bits(float x, float f) { return (uint32_t)__float2int_rn(x * f) + 0x8080u; }
 // the same for x >= 0 in one operation: the f32 addition rounds x f to an integer
-__device__ __forceinline__ uint32_t digit_bits_pos(float x, float f) {
-    return __float_as_uint(ffma(x, f, 8388608.0f + (float)0x8080));
-}
+constexpr float kDigitBase = 8388608.0f + (float)0x8080;
+__device__ __forceinline__ uint32_t digit_bits_pos(float x, float f) { return __float_as_uint(ffma(x, f, kDigitBase)); }
 
 // digits of four integers given as digit_bits: word e of d holds digit e of each in its bytes
 __device__ __forceinline__ void digits4(uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3, uint32_t (&d)[3]) {
@@ -482,8 +516,10 @@ __device__ __forceinline__ void digits4(uint32_t y0, uint32_t y1, uint32_t y2, u
     d[2] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
 }
 
-__device__ __forceinline__ float join_digits(int d2, int d1, int d0) {
-    return ffma(sum_of(d2), 65536.0f, ffma(sum_of(d1), 256.0f, sum_of(d0)));
+// d2 65536 + d1 256 + d0 of two neighbouring sums (elements y, y + 1 of the fragments)
+__device__ __forceinline__ f32x2 join_digits(const int (&c)[3][4], int y) {
+    return fma2(sums_of(c[2][y], c[2][y + 1]), pack2(65536.0f, 65536.0f),
+                fma2(sums_of(c[1][y], c[1][y + 1]), pack2(256.0f, 256.0f), sums_of(c[0][y], c[0][y + 1])));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -677,9 +713,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         const int lim1 = 2 * t + 1 < cols ? min(pos0 + (col0 + 2 * t + 1) / p.G + 1, n) : 0;
 
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;        // running max; this lane's part of the sum
-        float o[Sh::NM][4];
+        f32x2 o[Sh::NM][2];                                                // elements, columns (2t, 2t + 1)
 #pragma unroll
-        for (int i = 0; i < Sh::NM; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < Sh::NM; ++i) o[i][0] = o[i][1] = 0ull;
 
         for (int j = j0 + warp * 32; j < jend; j += kSplitWarps * 32) {
             // the step's two blocks: where they are and their scales
@@ -744,14 +780,13 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                         else mma_s8(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
                         mma_s8(c[e], kf[b][0][h].z, kf[b][1][h].z, kf[b][0][h].w, kf[b][1][h].w, qb[e][h][2], qb[e][h][3]);
                     }
-                const float u0 = sq0 * sk[b], u1 = sq1 * sk[b];
+                const f32x2 u = pack2(sq0 * sk[b], sq1 * sk[b]);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int key = j + 16 * b + 8 * r + g;
-                    const float a0 = join_digits(c[2][2 * r], c[1][2 * r], c[0][2 * r]) * u0;
-                    const float a1 = join_digits(c[2][2 * r + 1], c[1][2 * r + 1], c[0][2 * r + 1]) * u1;
-                    s[b][2 * r] = there[b] && key < lim0 ? a0 : -INFINITY;
-                    s[b][2 * r + 1] = there[b] && key < lim1 ? a1 : -INFINITY;
+                    const float2 a = unpack2(mul2(join_digits(c, 2 * r), u));
+                    s[b][2 * r] = there[b] && key < lim0 ? a.x : -INFINITY;
+                    s[b][2 * r + 1] = there[b] && key < lim1 ? a.y : -INFINITY;
                     mx0 = fmaxf(mx0, s[b][2 * r]);
                     mx1 = fmaxf(mx1, s[b][2 * r + 1]);
                 }
@@ -804,7 +839,8 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 const uint4 w = lds128(wxw + g * Sh::WStride + 16 * b + 4 * t);
                 digits4(w.x, w.y, w.z, w.w, wb[b]);
             }
-            const float u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0, u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
+            const f32x2 u = pack2(f0 > 0.0f ? __fdividef(1.0f, f0) : f0, f1 > 0.0f ? __fdividef(1.0f, f1) : f1);
+            const f32x2 back = pack2(back0, back1);
             // output elements (DP / 8) g + 2 m, + 1 (rows g and g + 8 of tile m): four keys' bytes of one element
             // make one A register
 #pragma unroll
@@ -823,10 +859,8 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
 #pragma unroll
                     for (int e = 0; e < 3; ++e)
                         mma_s8_first(c[e], a[0][2 * k], a[0][2 * k + 1], a[1][2 * k], a[1][2 * k + 1], wb[0][e], wb[1][e]);
-                    float(&oo)[4] = o[2 * w + k];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        oo[i] = ffma(join_digits(c[2][i], c[1][i], c[0][i]), i & 1 ? u1 : u0, oo[i] * (i & 1 ? back1 : back0));
+                    for (int i = 0; i < 2; ++i) o[2 * w + k][i] = fma2(join_digits(c, 2 * i), u, mul2(o[2 * w + k][i], back));
                 }
             }
         }
@@ -844,8 +878,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
 #pragma unroll
         for (int i = 0; i < Sh::NM; ++i) {
             const int d = (DP / 8) * g + 2 * i;
-            *reinterpret_cast<float2*>(ow + (2 * t) * DP + d) = make_float2(o[i][0], o[i][2]);
-            *reinterpret_cast<float2*>(ow + (2 * t + 1) * DP + d) = make_float2(o[i][1], o[i][3]);
+            const float2 x = unpack2(o[i][0]), y = unpack2(o[i][1]);
+            *reinterpret_cast<float2*>(ow + (2 * t) * DP + d) = make_float2(x.x, y.x);
+            *reinterpret_cast<float2*>(ow + (2 * t + 1) * DP + d) = make_float2(x.y, y.y);
         }
         __syncthreads();
         for (int i = tid; i < cols * (DP / 4); i += kSplitWarps * 32) {
@@ -1020,9 +1055,9 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
     wmax = __reduce_max_sync(0xffffffffu, wmax);
     const float sq0 = sq[ra], sq1 = sq[ra + 8];
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-    float o[Sh::NT][4];
+    f32x2 o[Sh::NT][2];                                        // elements 8 x + 2t, + 1 of rows ra, ra + 8
 #pragma unroll
-    for (int i = 0; i < Sh::NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    for (int i = 0; i < Sh::NT; ++i) o[i][0] = o[i][1] = 0ull;
 
     if (ntiles > 0) {
         load_tile(0);
@@ -1039,7 +1074,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
         if (wmax > j) {
             const uint8_t* kd = kt + (i & 1) * Sh::KBytes;
             const float* scb = sc + 12 * (i & 1);
-            float s[8][4];                                     // rows g (0, 1), g + 8 (2, 3); keys 8 nt + 2t, + 1
+            float2 s[8][2];                                    // keys 8 x + 2t, + 1 of rows ra, ra + 8
             float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {             // 32 keys at a time
@@ -1064,10 +1099,9 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const float u = scb[2 * half + (x >> 1)];
-                    const float u0 = sq0 * u, u1 = sq1 * u;
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        s[4 * half + x][y] = join_digits(c[x][2][y], c[x][1][y], c[x][0][y]) * (y < 2 ? u0 : u1);
+                    for (int r = 0; r < 2; ++r)
+                        s[4 * half + x][r] = unpack2(mul2(join_digits(c[x], 2 * r), pack2((r ? sq1 : sq0) * u, (r ? sq1 : sq0) * u)));
                 }
             }
             const bool whole = j + kTileKeys <= wmin && scb[8] + scb[9] + scb[10] + scb[11] == 4.0f;
@@ -1075,13 +1109,16 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        if (!(j + 8 * x + 2 * t + (y & 1) < (y < 2 ? lim0 : lim1) && scb[8 + (x >> 1)] != 0.0f)) s[x][y] = -INFINITY;
+                    for (int r = 0; r < 2; ++r) {
+                        const int key = j + 8 * x + 2 * t, lim = scb[8 + (x >> 1)] != 0.0f ? (r ? lim1 : lim0) : 0;
+                        if (key >= lim) s[x][r].x = -INFINITY;
+                        if (key + 1 >= lim) s[x][r].y = -INFINITY;
+                    }
             }
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                mx0 = fmaxf(mx0, fmaxf(s[x][0], s[x][1]));
-                mx1 = fmaxf(mx1, fmaxf(s[x][2], s[x][3]));
+                mx0 = fmaxf(mx0, fmaxf(s[x][0].x, s[x][0].y));
+                mx1 = fmaxf(mx1, fmaxf(s[x][1].x, s[x][1].y));
             }
 #pragma unroll
             for (int x = 1; x <= 2; x <<= 1) {
@@ -1097,32 +1134,26 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
             // enough; a value scale that is not one needs the checks
             float wt0 = 0.0f, wt1 = 0.0f;
             const float svs = scb[4] + scb[5] + scb[6] + scb[7];
-            if (svs == svs) {
+            f32x2 ls0 = 0ull, ls1 = 0ull;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const float sv = scb[4 + (x >> 1)];
+            for (int x = 0; x < 8; ++x)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float ev = exp2_fast(s[x][y] - (y < 2 ? b0 : b1));
-                        if (y < 2) l0 += ev; else l1 += ev;
-                        s[x][y] = ev * sv;
-                        if (y < 2) wt0 = fmaxf(wt0, s[x][y]); else wt1 = fmaxf(wt1, s[x][y]);
+                for (int r = 0; r < 2; ++r) {
+                    const f32x2 nb = pack2(r ? -b1 : -b0, r ? -b1 : -b0), sv = pack2(scb[4 + (x >> 1)], scb[4 + (x >> 1)]);
+                    const float2 z = unpack2(add2(pack2(s[x][r].x, s[x][r].y), nb));
+                    const f32x2 ev = pack2(exp2_fast(z.x), exp2_fast(z.y));
+                    if (r) ls1 = add2(ls1, ev); else ls0 = add2(ls0, ev);
+                    float2 w = unpack2(mul2(ev, sv));
+                    if (svs != svs) {                          // masked: nothing, whatever the scale
+                        if (s[x][r].x == -INFINITY) w.x = 0.0f;
+                        if (s[x][r].y == -INFINITY) w.y = 0.0f;
+                        if (w.x != w.x || w.y != w.y) { if (r) wt1 = INFINITY; else wt0 = INFINITY; }
                     }
+                    s[x][r] = w;
+                    if (r) wt1 = fmaxf(wt1, fmaxf(w.x, w.y)); else wt0 = fmaxf(wt0, fmaxf(w.x, w.y));
                 }
-            } else {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const float sv = scb[4 + (x >> 1)];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float ev = exp2_fast(s[x][y] - (y < 2 ? b0 : b1));
-                        if (y < 2) l0 += ev; else l1 += ev;
-                        s[x][y] = s[x][y] == -INFINITY ? 0.0f : ev * sv;   // masked: nothing, whatever the scale
-                        if (s[x][y] != s[x][y]) { if (y < 2) wt0 = INFINITY; else wt1 = INFINITY; }
-                        if (y < 2) wt0 = fmaxf(wt0, s[x][y]); else wt1 = fmaxf(wt1, s[x][y]);
-                    }
-                }
-            }
+            l0 += unpack2(ls0).x + unpack2(ls0).y;
+            l1 += unpack2(ls1).x + unpack2(ls1).y;
 #pragma unroll
             for (int x = 1; x <= 2; x <<= 1) {
                 wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
@@ -1138,12 +1169,11 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
                 for (int b = 0; b < 2; ++b)                    // 16 keys: registers 2 b (row g) and 2 b + 1 (row g + 8)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float f = r ? f1 : f0;
-                        const float(&x0)[4] = s[4 * ks + 2 * b];
-                        const float(&x1)[4] = s[4 * ks + 2 * b + 1];
+                        const f32x2 f = pack2(r ? f1 : f0, r ? f1 : f0), base = pack2(kDigitBase, kDigitBase);
+                        const float2 x0 = s[4 * ks + 2 * b][r], x1 = s[4 * ks + 2 * b + 1][r];
+                        const float2 y0 = unpack2(fma2(pack2(x0.x, x0.y), f, base)), y1 = unpack2(fma2(pack2(x1.x, x1.y), f, base));
                         uint32_t dg[3];
-                        digits4(digit_bits_pos(x0[2 * r], f), digit_bits_pos(x0[2 * r + 1], f), digit_bits_pos(x1[2 * r], f),
-                                digit_bits_pos(x1[2 * r + 1], f), dg);
+                        digits4(__float_as_uint(y0.x), __float_as_uint(y0.y), __float_as_uint(y1.x), __float_as_uint(y1.y), dg);
 #pragma unroll
                         for (int e = 0; e < 3; ++e) wa[ks][e][2 * b + r] = dg[e];
                     }
@@ -1158,8 +1188,9 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
                     mma_s8(c[e], wa[1][e][0], wa[1][e][1], wa[1][e][2], wa[1][e][3], b.z, b.w);
                 }
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
-                    o[x][y] = ffma(join_digits(c[2][y], c[1][y], c[0][y]), y < 2 ? u0 : u1, o[x][y] * (y < 2 ? back0 : back1));
+                for (int r = 0; r < 2; ++r)
+                    o[x][r] = fma2(join_digits(c, 2 * r), pack2(r ? u1 : u0, r ? u1 : u0),
+                                   mul2(o[x][r], pack2(r ? back1 : back0, r ? back1 : back0)));
             }
         }
         if (more) {
@@ -1186,7 +1217,8 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
 #pragma unroll
         for (int x = 0; x < Sh::NT; ++x) {
             const int d = 8 * x + 2 * t;
-            if (d < dh) *reinterpret_cast<float2*>(dst + d) = make_float2(o[x][2 * r] * inv, o[x][2 * r + 1] * inv);
+            const float2 y = unpack2(o[x][r]);
+            if (d < dh) *reinterpret_cast<float2*>(dst + d) = make_float2(y.x * inv, y.y * inv);
         }
         if (splits > 1 && t == 0) { dst[dh] = r ? m1 : m0; dst[dh + 1] = L; }
     }
