@@ -125,7 +125,7 @@ bool attn_plan(PagedAttnParams& p, int max_rows) {
     } else {
         const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / kTileRows), want = 2 * 148 * 3;
         const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
-        p.kc = (int)std::max(256ll, ((p.r.cap + splits - 1) / splits + kTileKeys - 1) / kTileKeys * kTileKeys);
+        p.kc = (int)std::max(256ll, ((p.r.cap + splits - 1) / splits + 127) / 128 * 128);
     }
     p.nsplit = std::max(1, (p.r.cap + p.kc - 1) / p.kc);
     return few;

@@ -447,23 +447,18 @@ constexpr int kDigitMax = 8355700;
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The first of a chain: the sums start at kSumBase, the bits of 1.5 * 2^23 in f32, so
-// that a sum (at most 2^22: 256 products of two signed bytes) is read as the float
-// kSumF + sum and one subtraction makes it a number; nothing is cleared or converted.
-constexpr int kSumBase = 0x4B400000;
-constexpr float kSumF = 12582912.0f;
+// the first of a chain: from zero, so that nothing has to be cleared
 __device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kSumBase));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
 // two f32 in one instruction: the attention kernels are bound by what the schedulers
@@ -472,11 +467,6 @@ typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack2(float a, float b) {
     f32x2 r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 pack2i(int a, int b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
     return r;
 }
 __device__ __forceinline__ float2 unpack2(f32x2 v) {
@@ -499,8 +489,6 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-// two neighbouring digit sums as numbers
-__device__ __forceinline__ f32x2 sums_of(int a, int b) { return add2(pack2i(a, b), pack2(-kSumF, -kSumF)); }
 
 // rint(x f) + 0x8080 for |x f| <= kDigitMax, in the low 24 bits
 __device__ __forceinline__ uint32_t digit_bits(float x, float f) { return (uint32_t)__float2int_rn(x * f) + 0x8080u; }
@@ -516,10 +504,11 @@ __device__ __forceinline__ void digits4(uint32_t y0, uint32_t y1, uint32_t y2, u
     d[2] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
 }
 
-// d2 65536 + d1 256 + d0 of two neighbouring sums (elements y, y + 1 of the fragments)
+// d2 65536 + d1 256 + d0 of two neighbouring sums (elements y, y + 1 of the fragments):
+// the lower two joined as integers (256 products: below 2^30)
 __device__ __forceinline__ f32x2 join_digits(const int (&c)[3][4], int y) {
-    return fma2(sums_of(c[2][y], c[2][y + 1]), pack2(65536.0f, 65536.0f),
-                fma2(sums_of(c[1][y], c[1][y + 1]), pack2(256.0f, 256.0f), sums_of(c[0][y], c[0][y + 1])));
+    return fma2(pack2((float)c[2][y], (float)c[2][y + 1]), pack2(65536.0f, 65536.0f),
+                pack2((float)(c[1][y] * 256 + c[0][y]), (float)(c[1][y + 1] * 256 + c[0][y + 1])));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -916,49 +905,49 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
 }
 
 // ---- many rows per sequence: a CTA of 4 warps takes 64 rows ((token, head) pairs of
-// one KV head), warp w 16 of them, against a split of the keys in tiles of 64. A =
+// one KV head), warp w 16 of them, against a split of the keys in tiles of KT. A =
 // query or weight digits (rows x 32), B = codes: keys as they lie, values turned to
 // [d][key] on their way into shared memory (byte permutes, once for the CTA). The
 // key order inside a B fragment of the values is the one that the score fragments
 // already have, so weights go from scores to A fragments inside their thread.
-// Codes of tile i + 1 are on their way while tile i is computed.
+// Codes of tile i + 1 are on their way while tile i is computed. Every tile ends with
+// folding the output's digit sums into f32 (their unit changes with the row's
+// maximum), which is why KT is as large as the registers allow.
 constexpr int kTileRows = 64;
-constexpr int kTileKeys = 64;
 
 template <int DP>
 struct TileShape {
+    static constexpr int KT = DP == 256 ? 64 : 128;            // keys per tile
+    static constexpr int NB = KT / 16;                         // blocks per tile
     static constexpr int NH = DP / 64;
     static constexpr int NT = DP / 8;                          // output tiles of 8 elements
     static constexpr int QBytes = 3 * kTileRows * DP;
-    static constexpr int KBytes = kTileKeys * DP;
-    static constexpr int Smem = QBytes + 4 * KBytes + kTileRows * 4 + 2 * 12 * 4 + 2 * 4 * 8;
+    static constexpr int KBytes = KT * DP;
+    static constexpr int Smem = QBytes + 4 * KBytes + kTileRows * 4 + 2 * 3 * NB * 4 + 2 * NB * 8;
 };
 
-// 16-byte unit u of a row of DP bytes, swapped between halves in odd rows so that the
-// fragment loads of two neighbouring rows meet no bank twice
-template <int DP>
+// byte offset of 16-byte unit u of row `row` of `width` bytes: swapped between halves in
+// odd rows so that the fragment loads of two neighbouring rows meet no bank twice
+template <int width>
 __device__ __forceinline__ int unit_at(int row, int u) {
-    return row * DP + 16 * (DP >= 128 ? u ^ ((row & 1) << 2) : u);
+    return row * width + 16 * (width >= 128 ? u ^ ((row & 1) << 2) : u);
 }
-
-// row d of the turned values ([DP][64 keys] bytes): neighbours swapped in every other
-// group of 16, so that the stores of two groups meet no bank twice
-__device__ __forceinline__ int value_row(int d) { return (d ^ ((d >> 4) & 1)) * kTileKeys; }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
 template <int DP>
-__global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel(const __grid_constant__ PagedAttnParams p) {
     using Sh = TileShape<DP>;
+    constexpr int KT = Sh::KT, NB = Sh::NB;
     extern __shared__ __align__(16) unsigned char pt_raw[];
-    uint8_t* qd = pt_raw;                                      // [3][64][DP]
-    uint8_t* kt = qd + Sh::QBytes;                             // [2][64][DP]
-    uint8_t* vt = kt + 2 * Sh::KBytes;                         // [2][DP][64]
+    uint8_t* qd = pt_raw;                                      // A fragments [3][4 warps][DP / 32][lane][16]
+    uint8_t* kt = qd + Sh::QBytes;                             // [2][KT][DP]
+    uint8_t* vt = kt + 2 * Sh::KBytes;                         // [2][DP][KT]
     float* sq = reinterpret_cast<float*>(vt + 2 * Sh::KBytes); // [64]
-    float* sc = sq + kTileRows;                                // [2][12]: 4 key scales, 4 value scales, 4 "there"
-    long long* cell = reinterpret_cast<long long*>(sc + 24);   // [2][4] a tile's blocks in the pool
+    float* sc = sq + kTileRows;                                // [2][3][NB]: key scales, value scales, 1 where there
+    long long* cell = reinterpret_cast<long long*>(sc + 6 * NB);   // [2][NB] a tile's blocks in the pool
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int dh = p.c.dh, psz = 1 << p.c.page_log2;
 
@@ -969,7 +958,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
     const int n = min(pos0 + (row0 + rows - 1) / p.G + 1, p.r.cap);      // keys that any row sees
     const int j0 = it.split * p.kc, jend = min(n, j0 + p.kc);
     if (j0 >= n && it.split > 0) return;
-    const int ntiles = max((jend - j0 + kTileKeys - 1) / kTileKeys, 0);
+    const int ntiles = max((jend - j0 + KT - 1) / KT, 0);
 
     // a block's number in the pool (its codes start at 16 dh times that); -1: page outside
     // the pool, -2: past the end
@@ -978,7 +967,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
         const int page = page_of(p.c, p.r, it.s, j);
         return page < 0 ? -1 : ((long long)page * p.c.KVH + it.kvh) * (psz >> 4) + ((j & (psz - 1)) >> 4);
     };
-    if (tid < 8 && ntiles > 0) cell[tid] = cell_at(j0 + 16 * tid);
+    if (tid < 2 * NB && ntiles > 0) cell[tid] = cell_at(j0 + 16 * tid);
 
     // queries -> digits: 16 lanes a row
 #pragma unroll 1
@@ -986,49 +975,55 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
         const int l16 = tid & 15, cc = row0 + r;
         const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
         query_digits<DP>(qr, r < rows, dh, l16, [&](int e, int d, uint32_t w) {
-            *reinterpret_cast<uint32_t*>(qd + e * kTileRows * DP + unit_at<DP>(r, d >> 4) + (d & 15)) = w;
+            // elements d .. d + 3: lane 4 (row & 7) + quad of the row's 16-byte unit, word by row half and k half
+            const int step = 2 * (d >> 6) + ((d >> 3) & 1), word = ((r >> 3) & 1) + 2 * ((d >> 2) & 1);
+            *reinterpret_cast<uint32_t*>(qd + (((e * 4 + (r >> 4)) * (DP / 32) + step) * 32 + 4 * (r & 7) + ((d >> 4) & 3)) * 16 + 4 * word) = w;
         }, sq + r);
     }
     __syncthreads();
 
-    // this thread's part of a value tile: block vb, keys 2 vt_ + {0, 1, 8, 9} of it, 16 elements from 16 vc
-    const int vb = lane >> 3, vq = (lane >> 1) & 3;
-    constexpr int VC = DP == 256 ? 2 : 1;
-    uint4 vr[VC][4];
-    auto load_tile = [&](int i) {                              // keys by cp.async, values into registers
+    auto load_keys = [&](int i) {                              // and the scales
         const int b = i & 1;
         uint8_t* kd = kt + b * Sh::KBytes;
 #pragma unroll
-        for (int x = 0; x < kTileKeys * DP / 16 / 128; ++x) {
+        for (int x = 0; x < KT * DP / 16 / 128; ++x) {
             const int unit = x * 128 + tid, key = unit / (DP / 16), u = unit % (DP / 16);
-            const long long at = cell[4 * b + (key >> 4)];
+            const long long at = cell[NB * b + (key >> 4)];
             const bool there = at >= 0 && 16 * u < dh;
             cp_async16(kd + unit_at<DP>(key, u), p.c.k + (there ? at * (kKvBlock * dh) + (key & 15) * dh + 16 * u : 0), there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const long long at = cell[4 * b + vb];
+        if (tid < 2 * NB) {
+            const long long cb = cell[NB * b + tid % NB];
+            sc[3 * NB * b + tid] = cb >= 0 ? __ldg((tid < NB ? p.c.ks : p.c.vs) + cb) : 0.0f;
+            if (tid < NB) sc[3 * NB * b + 2 * NB + tid] = cb >= 0 ? 1.0f : 0.0f;
+            if (cb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+        }
+    };
+    // This thread's part of a value tile: in block vb four keys vq2 + {0, 1, 8, 9} of 16
+    // elements from d0 + 16 x. The lanes of a warp cover 32 (block, key group) pairs of one
+    // 16-element column (KT = 128), so that its word stores meet no bank twice.
+    constexpr int VH = KT / 64;                                // 64-key halves among a warp's lanes
+    constexpr int VC = KT * DP / 64 / 128;                     // 16-byte columns a thread turns
+    const int vb = (lane & 15) >> 2, vq2 = (lane & 3) * 2, vh = VH == 2 ? lane >> 4 : 0;
+    const int d0 = 16 * (VH == 2 ? VC * warp : VC * (2 * warp + (lane >> 4)));
+    uint4 vr[VC][4];
+    auto load_values = [&](int i) {
+        const long long at = cell[NB * (i & 1) + 4 * vh + vb];
 #pragma unroll
         for (int x = 0; x < VC; ++x) {
-            const int d = 16 * (2 * warp + (lane & 1) + 8 * x);
+            const int d = d0 + 16 * x;
             const bool there = at >= 0 && d < dh;
-            const int8_t* src = p.c.v + (there ? at * (kKvBlock * dh) + 2 * vq * dh + d : 0);
+            const int8_t* src = p.c.v + (there ? at * (kKvBlock * dh) + vq2 * dh + d : 0);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 vr[x][k] = there ? __ldg(reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh)) : make_uint4(0u, 0u, 0u, 0u);
-        }
-        if (tid < 8) {                                         // scales of the tile's blocks
-            const long long cb = cell[4 * b + (tid & 3)];
-            sc[12 * b + tid] = cb >= 0 ? __ldg((tid < 4 ? p.c.ks : p.c.vs) + cb) : 0.0f;
-            if (tid < 4) sc[12 * b + 8 + tid] = cb >= 0 ? 1.0f : 0.0f;
-            if (cb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
         }
     };
     auto store_values = [&](int i) {
         uint8_t* vd = vt + (i & 1) * Sh::KBytes;
 #pragma unroll
         for (int x = 0; x < VC; ++x) {
-            const int d = 16 * (2 * warp + (lane & 1) + 8 * x);
-            if (d >= DP) continue;
             const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[x][0]);
             const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[x][1]);
             const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[x][2]);
@@ -1037,11 +1032,11 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
             for (int w = 0; w < 4; ++w) {
                 const uint32_t a = __byte_perm(w0[w], w1[w], 0x5140), b = __byte_perm(w2[w], w3[w], 0x5140);
                 const uint32_t c = __byte_perm(w0[w], w1[w], 0x7362), e = __byte_perm(w2[w], w3[w], 0x7362);
-                const int at = 16 * vq + 4 * vb;
-                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w) + at) = __byte_perm(a, b, 0x5410);
-                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w + 1) + at) = __byte_perm(a, b, 0x7632);
-                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w + 2) + at) = __byte_perm(c, e, 0x5410);
-                *reinterpret_cast<uint32_t*>(vd + value_row(d + 4 * w + 3) + at) = __byte_perm(c, e, 0x7632);
+                const uint32_t y[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, e, 0x5410),
+                                       __byte_perm(c, e, 0x7632)};
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                    *reinterpret_cast<uint32_t*>(vd + unit_at<KT>(d0 + 16 * x + 4 * w + z, 4 * vh + (vq2 >> 1)) + 4 * vb) = y[z];
             }
         }
     };
@@ -1060,63 +1055,70 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
     for (int i = 0; i < Sh::NT; ++i) o[i][0] = o[i][1] = 0ull;
 
     if (ntiles > 0) {
-        load_tile(0);
+        load_keys(0);
+        load_values(0);
         store_values(0);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
     }
 #pragma unroll 1
     for (int i = 0; i < ntiles; ++i) {
-        const int j = j0 + i * kTileKeys;
+        const int j = j0 + i * KT;
         const bool more = i + 1 < ntiles;
-        if (more) load_tile(i + 1);
-        if (tid >= 120 && tid < 124) cell[4 * (i & 1) + tid - 120] = cell_at(j + 2 * kTileKeys + 16 * (tid - 120));
-        if (wmax > j) {
+        if (more) load_keys(i + 1);
+        const bool busy = wmax > j;                            // the warp has a row that sees the tile
+        uint32_t wa[KT / 32][3][4];                            // weight digits: A fragments [32 keys][digit]
+        float back0 = 1.0f, back1 = 1.0f, u0 = 0.0f, u1 = 0.0f;
+        if (busy) {
             const uint8_t* kd = kt + (i & 1) * Sh::KBytes;
-            const float* scb = sc + 12 * (i & 1);
-            float2 s[8][2];                                    // keys 8 x + 2t, + 1 of rows ra, ra + 8
-            float mx0 = -INFINITY, mx1 = -INFINITY;
+            const float* scb = sc + 3 * NB * (i & 1);
+            float2 s[KT / 8][2];                               // keys 8 x + 2t, + 1 of rows ra, ra + 8
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {             // 32 keys at a time
+            for (int part = 0; part < KT / 32; ++part) {       // 32 keys at a time
                 int c[4][3][4];
 #pragma unroll
                 for (int h = 0; h < Sh::NH; ++h) {
                     uint4 b[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) b[x] = lds128(kd + unit_at<DP>(32 * half + 8 * x + g, 4 * h + t));
+                    for (int x = 0; x < 4; ++x)
+                        b[x] = *reinterpret_cast<const uint4*>(kd + unit_at<DP>(32 * part + 8 * x + g, 4 * h + t));
 #pragma unroll
                     for (int e = 0; e < 3; ++e) {
-                        const uint4 a0 = lds128(qd + e * kTileRows * DP + unit_at<DP>(ra, 4 * h + t));
-                        const uint4 a1 = lds128(qd + e * kTileRows * DP + unit_at<DP>(ra + 8, 4 * h + t));
+                        const uint8_t* qa = qd + (((e * 4 + warp) * (DP / 32) + 2 * h) * 32 + lane) * 16;
+                        const uint4 a0 = *reinterpret_cast<const uint4*>(qa), a1 = *reinterpret_cast<const uint4*>(qa + 512);
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            if (h == 0) mma_s8_first(c[x][e], a0.x, a1.x, a0.y, a1.y, b[x].x, b[x].y);
-                            else mma_s8(c[x][e], a0.x, a1.x, a0.y, a1.y, b[x].x, b[x].y);
-                            mma_s8(c[x][e], a0.z, a1.z, a0.w, a1.w, b[x].z, b[x].w);
+                            if (h == 0) mma_s8_first(c[x][e], a0.x, a0.y, a0.z, a0.w, b[x].x, b[x].y);
+                            else mma_s8(c[x][e], a0.x, a0.y, a0.z, a0.w, b[x].x, b[x].y);
                         }
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) mma_s8(c[x][e], a1.x, a1.y, a1.z, a1.w, b[x].z, b[x].w);
                     }
                 }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const float u = scb[2 * half + (x >> 1)];
+                    const float u = scb[2 * part + (x >> 1)];
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        s[4 * half + x][r] = unpack2(mul2(join_digits(c[x], 2 * r), pack2((r ? sq1 : sq0) * u, (r ? sq1 : sq0) * u)));
+                        s[4 * part + x][r] = unpack2(mul2(join_digits(c[x], 2 * r), pack2((r ? sq1 : sq0) * u, (r ? sq1 : sq0) * u)));
                 }
             }
-            const bool whole = j + kTileKeys <= wmin && scb[8] + scb[9] + scb[10] + scb[11] == 4.0f;
-            if (!whole) {
+            float there = 0.0f, svs = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
+            for (int x = 0; x < NB; ++x) { svs += scb[NB + x]; there += scb[2 * NB + x]; }
+            if (j + KT > wmin || there != (float)NB) {
+#pragma unroll
+                for (int x = 0; x < KT / 8; ++x)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const int key = j + 8 * x + 2 * t, lim = scb[8 + (x >> 1)] != 0.0f ? (r ? lim1 : lim0) : 0;
+                        const int key = j + 8 * x + 2 * t, lim = scb[2 * NB + (x >> 1)] != 0.0f ? (r ? lim1 : lim0) : 0;
                         if (key >= lim) s[x][r].x = -INFINITY;
                         if (key + 1 >= lim) s[x][r].y = -INFINITY;
                     }
             }
+            float mx0 = m0, mx1 = m1;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
+            for (int x = 0; x < KT / 8; ++x) {
                 mx0 = fmaxf(mx0, fmaxf(s[x][0].x, s[x][0].y));
                 mx1 = fmaxf(mx1, fmaxf(s[x][1].x, s[x][1].y));
             }
@@ -1125,48 +1127,57 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
                 mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
                 mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
             }
-            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-            const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
-            const float back0 = exp2_fast(m0 - b0), back1 = exp2_fast(m1 - b1);
-            m0 = n0; m1 = n1;
-            l0 *= back0; l1 *= back1;
-            // weights p v_scale. A score that is not a number has made l NaN, which is
-            // enough; a value scale that is not one needs the checks
-            float wt0 = 0.0f, wt1 = 0.0f;
-            const float svs = scb[4] + scb[5] + scb[6] + scb[7];
+            const float b0 = mx0 == -INFINITY ? 0.0f : mx0, b1 = mx1 == -INFINITY ? 0.0f : mx1;
+            back0 = exp2_fast(m0 - b0); back1 = exp2_fast(m1 - b1);
+            m0 = mx0; m1 = mx1;
+            // weights p v_scale. A score that is not a number makes l NaN, which is enough; a
+            // value scale that is not one needs checks
             f32x2 ls0 = 0ull, ls1 = 0ull;
 #pragma unroll
-            for (int x = 0; x < 8; ++x)
+            for (int x = 0; x < KT / 8; ++x)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const f32x2 nb = pack2(r ? -b1 : -b0, r ? -b1 : -b0), sv = pack2(scb[4 + (x >> 1)], scb[4 + (x >> 1)]);
-                    const float2 z = unpack2(add2(pack2(s[x][r].x, s[x][r].y), nb));
+                    const float2 z = unpack2(add2(pack2(s[x][r].x, s[x][r].y), pack2(r ? -b1 : -b0, r ? -b1 : -b0)));
                     const f32x2 ev = pack2(exp2_fast(z.x), exp2_fast(z.y));
                     if (r) ls1 = add2(ls1, ev); else ls0 = add2(ls0, ev);
-                    float2 w = unpack2(mul2(ev, sv));
-                    if (svs != svs) {                          // masked: nothing, whatever the scale
-                        if (s[x][r].x == -INFINITY) w.x = 0.0f;
-                        if (s[x][r].y == -INFINITY) w.y = 0.0f;
-                        if (w.x != w.x || w.y != w.y) { if (r) wt1 = INFINITY; else wt0 = INFINITY; }
-                    }
-                    s[x][r] = w;
-                    if (r) wt1 = fmaxf(wt1, fmaxf(w.x, w.y)); else wt0 = fmaxf(wt0, fmaxf(w.x, w.y));
+                    s[x][r] = unpack2(ev);
                 }
-            l0 += unpack2(ls0).x + unpack2(ls0).y;
-            l1 += unpack2(ls1).x + unpack2(ls1).y;
+            l0 = ffma(l0, back0, unpack2(ls0).x + unpack2(ls0).y);
+            l1 = ffma(l1, back1, unpack2(ls1).x + unpack2(ls1).y);
+            float wt0 = 0.0f, wt1 = 0.0f;
+            if (svs == svs) {
+#pragma unroll
+                for (int x = 0; x < KT / 8; ++x)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        s[x][r] = unpack2(mul2(pack2(s[x][r].x, s[x][r].y), pack2(scb[NB + (x >> 1)], scb[NB + (x >> 1)])));
+                        if (r) wt1 = fmaxf(wt1, fmaxf(s[x][r].x, s[x][r].y)); else wt0 = fmaxf(wt0, fmaxf(s[x][r].x, s[x][r].y));
+                    }
+            } else {
+#pragma unroll
+                for (int x = 0; x < KT / 8; ++x)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        // a key that is masked weighs nothing, whatever its scale
+                        const int key = j + 8 * x + 2 * t, lim = r ? lim1 : lim0;
+                        s[x][r].x = key < lim ? s[x][r].x * scb[NB + (x >> 1)] : 0.0f;
+                        s[x][r].y = key + 1 < lim ? s[x][r].y * scb[NB + (x >> 1)] : 0.0f;
+                        float& wt = r ? wt1 : wt0;
+                        wt = s[x][r].x != s[x][r].x || s[x][r].y != s[x][r].y ? INFINITY : fmaxf(wt, fmaxf(s[x][r].x, s[x][r].y));
+                    }
+            }
 #pragma unroll
             for (int x = 1; x <= 2; x <<= 1) {
                 wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
                 wt1 = fmaxf(wt1, __shfl_xor_sync(0xffffffffu, wt1, x));
             }
             const float f0 = digit_factor(wt0), f1 = digit_factor(wt1);
-            const float u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0, u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
-            // weights as digits: A fragments [32-key step][digit][register]
-            uint32_t wa[2][3][4];
+            u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0;
+            u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int ks = 0; ks < KT / 32; ++ks)
 #pragma unroll
-                for (int b = 0; b < 2; ++b)                    // 16 keys: registers 2 b (row g) and 2 b + 1 (row g + 8)
+                for (int b = 0; b < 2; ++b)                    // 16 keys: registers 2 b (row ra) and 2 b + 1 (row ra + 8)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const f32x2 f = pack2(r ? f1 : f0, r ? f1 : f0), base = pack2(kDigitBase, kDigitBase);
@@ -1177,24 +1188,46 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 3) paged_attn_tile_kernel
 #pragma unroll
                         for (int e = 0; e < 3; ++e) wa[ks][e][2 * b + r] = dg[e];
                     }
+        }
+        if (more) load_values(i + 1);                          // into registers while the output is computed
+        if (busy) {
             const uint8_t* vd = vt + (i & 1) * Sh::KBytes;
 #pragma unroll
-            for (int x = 0; x < Sh::NT; ++x) {
-                const uint4 b = lds128(vd + value_row(8 * x + g) + 16 * t);
-                int c[3][4];
+            for (int x = 0; x < Sh::NT; x += 2) {              // two output tiles at a time: six independent chains
+                int c[2][3][4];
 #pragma unroll
-                for (int e = 0; e < 3; ++e) {
-                    mma_s8_first(c[e], wa[0][e][0], wa[0][e][1], wa[0][e][2], wa[0][e][3], b.x, b.y);
-                    mma_s8(c[e], wa[1][e][0], wa[1][e][1], wa[1][e][2], wa[1][e][3], b.z, b.w);
+                for (int h = 0; h < VH; ++h) {
+                    uint4 b[2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) b[z] = *reinterpret_cast<const uint4*>(vd + unit_at<KT>(8 * (x + z) + g, 4 * h + t));
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            const uint32_t(&a)[4] = wa[2 * h][e];
+                            if (h == 0) mma_s8_first(c[z][e], a[0], a[1], a[2], a[3], b[z].x, b[z].y);
+                            else mma_s8(c[z][e], a[0], a[1], a[2], a[3], b[z].x, b[z].y);
+                        }
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            const uint32_t(&a)[4] = wa[2 * h + 1][e];
+                            mma_s8(c[z][e], a[0], a[1], a[2], a[3], b[z].z, b[z].w);
+                        }
                 }
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    o[x][r] = fma2(join_digits(c, 2 * r), pack2(r ? u1 : u0, r ? u1 : u0),
-                                   mul2(o[x][r], pack2(r ? back1 : back0, r ? back1 : back0)));
+                for (int z = 0; z < 2; ++z)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        o[x + z][r] = fma2(join_digits(c[z], 2 * r), pack2(r ? u1 : u0, r ? u1 : u0),
+                                           mul2(o[x + z][r], pack2(r ? back1 : back0, r ? back1 : back0)));
             }
         }
         if (more) {
             store_values(i + 1);
+            // blocks of tile i + 2 (those of tile i are not needed any more)
+            if (tid < NB) cell[NB * (i & 1) + tid] = cell_at(j + 2 * KT + 16 * tid);
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         __syncthreads();
