@@ -59,6 +59,7 @@ bool view(const char* fn, const b2_kv_pages* kv, const b2_kv_rows* rows, PagedKv
     if (rows->n_seq > (1 << 20)) return bad("n_seq above 1048576");
     const int64_t cap = (int64_t)rows->max_pages * kv->page_size;
     if (cap > (1 << 30)) return bad("max_pages * page_size above 2^30");
+    if ((int64_t)kv->n_pages * kv->n_kv_heads * (kv->page_size / kKvBlock) >= (1ll << 31)) return bad("2^31 or more blocks in the pool");
     if (rows->max_keys < 0 || rows->max_rows < 0) return bad("negative max_keys or max_rows");
     c.k = kv->k; c.v = kv->v; c.ks = kv->k_scale; c.vs = kv->v_scale;
     c.n_pages = kv->n_pages; c.KVH = kv->n_kv_heads; c.dh = kv->d_head;
@@ -121,13 +122,14 @@ bool attn_plan(PagedAttnParams& p, int max_rows) {
     const long long cols = (max_rows > 0 ? max_rows : (p.r.n_rows + p.r.n_seq - 1) / std::max(p.r.n_seq, 1)) * (long long)G;
     const bool few = cols <= 16;
     if (few) {
-        p.kc = p.r.cap <= 16384 ? 256 : p.r.cap <= 65536 ? 512 : 1024;
+        p.kc_log2 = p.r.cap <= 4096 ? 8 : 9;
     } else {
         const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / kTileRows), want = 2 * 148 * 3;
         const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
-        p.kc = (int)std::max(256ll, ((p.r.cap + splits - 1) / splits + 127) / 128 * 128);
+        p.kc_log2 = 8;
+        while (p.kc_log2 < 30 && ((long long)splits << p.kc_log2) < p.r.cap) ++p.kc_log2;
     }
-    p.nsplit = std::max(1, (p.r.cap + p.kc - 1) / p.kc);
+    p.nsplit = std::max(1, (int)((p.r.cap + (1ll << p.kc_log2) - 1) >> p.kc_log2));
     return few;
 }
 
@@ -155,7 +157,6 @@ cudaError_t launch_attn_tile(const PagedAttnParams& p, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
     if (e != cudaSuccess) return e;
     const long long most = ((long long)p.r.n_rows * p.G / kTileRows + p.r.n_seq) * p.c.KVH * p.nsplit;
-    if (most >= (1ll << 31)) return cudaErrorInvalidValue;
     k<<<(unsigned)most, 128, Sh::Smem, s>>>(p);
     return launch_join(p, s);
 }
@@ -168,7 +169,7 @@ cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     // tiles over all sequences: at most one partly filled one each
     const long long tiles = ((long long)p.r.n_rows * p.G / kSplitCols + p.r.n_seq) * p.c.KVH;
-    const long long most = tiles * p.nsplit, resident = (long long)sm_count() * (DP == 256 ? 2 : 4);
+    const long long most = tiles * p.nsplit, resident = (long long)sm_count() * (DP == 256 ? 2 : DP == 128 ? 3 : 4);
     k<<<(unsigned)(most < resident ? most : resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
     return launch_join(p, s);
 }
@@ -287,6 +288,8 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     if ((int64_t)p.r.n_rows * n_heads > (1ll << 30)) return refuse(fn, "more than 2^30 (row, head) pairs");
     p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.G = n_heads / kv->n_kv_heads; p.err = err;
     const bool few = attn_plan(p, rows->max_rows);
+    const long long items = ((long long)p.r.n_rows * p.G / (few ? kSplitCols : kTileRows) + p.r.n_seq) * p.c.KVH * p.nsplit;
+    if (items >= kMaxItems) return refuse(fn, "too many (row, head, split) pieces for one call: use fewer rows");
     const size_t need = part_bytes(p);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");

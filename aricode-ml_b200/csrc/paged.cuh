@@ -504,11 +504,13 @@ __device__ __forceinline__ void digits4(uint32_t y0, uint32_t y1, uint32_t y2, u
     d[2] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
 }
 
-// d2 65536 + d1 256 + d0 of two neighbouring sums (elements y, y + 1 of the fragments):
-// the lower two joined as integers (256 products: below 2^30)
+// d2 65536 + d1 256 + d0 of two neighbouring sums a, b: the lower two digits joined as
+// integers (256 products: below 2^30)
+__device__ __forceinline__ f32x2 join_digits(int a2, int b2, int a1, int b1, int a0, int b0) {
+    return fma2(pack2((float)a2, (float)b2), pack2(65536.0f, 65536.0f), pack2((float)(a1 * 256 + a0), (float)(b1 * 256 + b0)));
+}
 __device__ __forceinline__ f32x2 join_digits(const int (&c)[3][4], int y) {
-    return fma2(pack2((float)c[2][y], (float)c[2][y + 1]), pack2(65536.0f, 65536.0f),
-                pack2((float)(c[1][y] * 256 + c[0][y]), (float)(c[1][y + 1] * 256 + c[0][y + 1])));
+    return join_digits(c[2][y], c[2][y + 1], c[1][y], c[1][y + 1], c[0][y], c[0][y + 1]);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -531,7 +533,7 @@ struct PagedAttnParams {
     float* out;              // [n_rows][ldo]
     long long ldq, ldo;
     int H, G;                // G = H / KVH
-    int kc;                  // keys per split
+    int kc_log2;             // keys per split
     int nsplit;              // splits of a sequence of cap keys
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
@@ -544,51 +546,50 @@ struct AttnItem {
     int kvh, tile, split;
 };
 
-__device__ __forceinline__ long long shfl64(unsigned m, long long v, int src) {
-    return (long long)(((unsigned long long)(unsigned)__shfl_sync(m, (int)(v >> 32), src) << 32) |
-                       (unsigned)__shfl_sync(m, (int)v, src));
+// splits of n keys (at least one: it also writes rows that see none)
+__device__ __forceinline__ int splits_of(const PagedAttnParams& p, int n) {
+    return max((n + (1 << p.kc_log2) - 1) >> p.kc_log2, 1);
 }
 
-// splits of n keys (at least one: it also writes rows that see none)
-__device__ __forceinline__ int splits_of(const PagedAttnParams& p, int n) { return max((n + p.kc - 1) / p.kc, 1); }
+// Most items of one sequence (the host refuses calls that could have more): the sums
+// over 32 lanes stay in 32 bits whatever the row ranges are.
+constexpr int kMaxItems = 1 << 26;
 
-// item number `item` of the call (tiles of NC columns), found by one warp
+// item number `item` of the call (tiles of NC rows), found by one warp
 template <int NC>
-__device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, long long item, int lane) {
+__device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned item, int lane) {
     AttnItem out{-1, 0, 0, 0, 0, 0, 0};
-    long long before = 0;
-    for (int base = 0; base < p.r.n_seq; base += 32) {
+    unsigned before = 0;
+    for (int base = 0; base < p.r.n_seq && before < (1u << 31); base += 32) {
         const int s = base + lane;
         SeqRows q{0, 0, 0};
-        long long cnt = 0;
+        unsigned cnt = 0;
         int tiles = 0;
         if (s < p.r.n_seq) {
             q = seq_rows(p.r, s);
             if (q.len > 0) {
                 if (q.kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
-                const int n = min(q.kv, p.r.cap);
                 tiles = (q.len * p.G + NC - 1) / NC;
-                cnt = (long long)tiles * p.c.KVH * splits_of(p, n);
+                cnt = (unsigned)min((long long)tiles * p.c.KVH * splits_of(p, min(q.kv, p.r.cap)), (long long)kMaxItems);
             }
         }
-        long long incl = cnt;
+        const unsigned total = __reduce_add_sync(0xffffffffu, cnt);
+        if (item - before < total) {
+            unsigned incl = cnt;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = shfl64(0xffffffffu, incl, (lane - o) & 31);
-            if (lane >= o) incl += v;
-        }
-        const long long total = shfl64(0xffffffffu, incl, 31);
-        if (item < before + total) {
-            const int src = __ffs(__ballot_sync(0xffffffffu, before + incl > item)) - 1;
-            const long long idx = item - before - shfl64(0xffffffffu, incl - cnt, src);
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const int src = __ffs(__ballot_sync(0xffffffffu, incl > item - before)) - 1;
+            const unsigned idx = item - before - __shfl_sync(0xffffffffu, incl - cnt, src);
             out.s = base + src;
             out.a = __shfl_sync(0xffffffffu, q.a, src);
             out.len = __shfl_sync(0xffffffffu, q.len, src);
             out.kv = __shfl_sync(0xffffffffu, q.kv, src);
             // the last rows first: with causal lengths they are the longest
-            const int splits = splits_of(p, min(out.kv, p.r.cap));
-            const long long rest = idx / p.c.KVH;
-            out.kvh = (int)(idx % p.c.KVH);
+            const unsigned splits = splits_of(p, min(out.kv, p.r.cap)), rest = idx / (unsigned)p.c.KVH;
+            out.kvh = (int)(idx % (unsigned)p.c.KVH);
             out.split = (int)(rest % splits);
             out.tile = __shfl_sync(0xffffffffu, tiles, src) - 1 - (int)(rest / splits);
             return out;
@@ -635,203 +636,217 @@ __device__ __forceinline__ void query_digits(const float* qr, bool live, int dh,
 
 // ---- few rows per sequence: a CTA of 4 warps takes 8 columns (token, head) of one KV
 // head against one split of the keys; warp w the 32-key steps w, w + 4, .... The codes
-// go from global memory straight into MMA fragments (A = keys x d for the scores,
-// d x keys for the output), so a warp keeps 64 * dh bytes of loads in flight and
-// nothing is staged; the four warps' (m, l, o) meet in shared memory.
+// go from global memory straight into B fragments (keys as they lie; values turned by
+// byte permutes inside a thread), nothing is staged. A step's keys are requested when
+// the previous step's scores are done, its values when the previous step's output is,
+// across items too: each CTA runs through its items with the next item's place, pages,
+// scales and queries fetched one item ahead, so a warp always has loads in flight.
+// A = digits: a 16-row tile holds digit 2 of the 8 columns above digit 1, a second one
+// digit 0, so that a thread gets all three digit sums of its (column, key) pairs. The
+// second one's rows 8 to 15 hold the digits of the other 16 elements of each part: of
+// its two products one counts in the upper, one in the lower half.
+// The four warps' (m, l, o) meet in shared memory, one barrier an item.
 constexpr int kSplitWarps = 4;
 constexpr int kSplitCols = 8;
+constexpr int kSplitMaxKeys = 512;                 // keys per split at most: a block a lane
 
 template <int DP>
 struct SplitShape {
     static constexpr int NH = DP / 64;             // 64-byte parts of a key row
     static constexpr int VW = DP / 32;             // 32-bit words of a value row that a lane holds
-    static constexpr int NM = DP / 16;             // output tiles of 16 elements
-    static constexpr int QBytes = 3 * kSplitCols * DP;
-    static constexpr int WStride = 36;             // ints; column rows 4 banks apart
-    static constexpr int MergeFloats = kSplitWarps * kSplitCols * (DP + 2);
-    static constexpr int WBytes = kSplitWarps * kSplitCols * WStride * 4;
-    static constexpr int Smem = QBytes + WBytes + MergeFloats * 4 + 64;
+    static constexpr int NT = DP / 8;              // output tiles of 8 elements
+    static constexpr int QBytes = NH * 3 * 32 * 16;                        // A fragments [part][hi, hi, lo][lane]
+    static constexpr int MergeBytes = kSplitWarps * kSplitCols * (DP + 4) * 4;
+    static constexpr int Smem = 2 * (QBytes + 32 + MergeBytes);
 };
 
+struct SplitItem {
+    AttnItem it;
+    int cols, col0, n, j0, jend;
+    int cell;                // block `lane` of the split in the pool (codes start at 16 dh
+    float ks, vs;            // times that; -1: page outside the pool, -2: past the end), scales
+};
+
+// the CTA's next item from number `item` on (stride gridDim.x) that has keys to look at
+__device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, unsigned& item, int lane) {
+    SplitItem w;
+    for (;; item += gridDim.x) {
+        w.it = find_item<kSplitCols>(p, item, lane);
+        if (w.it.s < 0) return w;
+        w.col0 = w.it.tile * kSplitCols;
+        w.cols = min(w.it.len * p.G - w.col0, kSplitCols);
+        const int last = w.it.len == 1 ? 0 : (w.col0 + w.cols - 1) / p.G;  // the tile's last token
+        w.n = min(w.it.kv - w.it.len + last + 1, p.r.cap);
+        w.j0 = w.it.split << p.kc_log2;
+        if (w.j0 < w.n || w.it.split == 0) break;                          // else the tile ends before this split
+    }
+    w.jend = min(w.n, w.j0 + (1 << p.kc_log2));
+    const int j = w.j0 + 16 * lane;
+    w.cell = -2;
+    w.ks = w.vs = 0.0f;
+    if (j < w.jend) {
+        const int page = page_of(p.c, p.r, w.it.s, j), b = p.c.page_log2 - 4;
+        w.cell = page < 0 ? -1 : ((page * p.c.KVH + w.it.kvh) << b) + ((j >> 4) & ((1 << b) - 1));
+        if (page < 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+        else { w.ks = __ldg(p.c.ks + w.cell); w.vs = __ldg(p.c.vs + w.cell); }
+    }
+    return w;
+}
+
 template <int DP>
-__global__ void __launch_bounds__(kSplitWarps * 32, DP == 256 ? 2 : 4)
+__global__ void __launch_bounds__(kSplitWarps * 32, DP == 256 ? 2 : DP == 128 ? 3 : 4)
 paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     using Sh = SplitShape<DP>;
     extern __shared__ __align__(16) unsigned char ps_raw[];
-    uint8_t* qd = ps_raw;                                                  // [3][8][DP] digits of the queries
-    float* sq = reinterpret_cast<float*>(ps_raw + Sh::QBytes);             // [8] their units (log2 e in)
-    uint32_t* wx = reinterpret_cast<uint32_t*>(ps_raw + Sh::QBytes + 64);            // [4][8][WStride] weights
-    float* mo = reinterpret_cast<float*>(ps_raw + Sh::QBytes + 64 + Sh::WBytes);   // [4][8][DP]
-    float* ml = mo + kSplitWarps * kSplitCols * DP;                        // [4][8][2]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int dh = p.c.dh, psz = 1 << p.c.page_log2;
-    uint32_t* wxw = wx + warp * kSplitCols * Sh::WStride;
+    const int dh = p.c.dh;
+    unsigned item = blockIdx.x;
+    SplitItem cur = next_split_item(p, item, lane);
+    if (cur.it.s < 0) return;
 
-    for (long long item = blockIdx.x;; item += gridDim.x) {
-        const AttnItem it = find_item<kSplitCols>(p, item, lane);
-        if (it.s < 0) return;
-        const int cols = min(it.len * p.G - it.tile * kSplitCols, kSplitCols);
-        const int col0 = it.tile * kSplitCols;                             // column = token * G + head
-        const int pos_last = it.kv - it.len + (col0 + cols - 1) / p.G;     // of the tile's last row
-        const int n = min(pos_last + 1, p.r.cap);                          // keys that any column sees
-        const int j0 = it.split * p.kc;
-        if (j0 >= n && it.split > 0) continue;                             // the tile ends before this split
-        const int jend = min(n, j0 + p.kc);
-
-        // queries -> digits: 16 lanes a column
-        {
-            const int col = tid >> 4, cc = col0 + col;
-            query_digits<DP>(p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh, col < cols, dh,
-                             tid & 15, [&](int e, int d, uint32_t w) {
-                                 *reinterpret_cast<uint32_t*>(qd + (e * kSplitCols + col) * DP + d) = w;
-                             }, sq + col);
+    uint4 kf[4][Sh::NH];                                                   // a step's keys 8 x + g
+    uint32_t vf[2][4][Sh::VW];                                             // its values: [block][key 2t + {0, 1, 8, 9}][words]
+    auto load_keys = [&](const SplitItem& w, int blk) {
+        const int c0 = __shfl_sync(0xffffffffu, w.cell, blk & 31), c1 = __shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int at = x < 2 ? c0 : c1;
+            const int8_t* kr = p.c.k + ((long long)at * kKvBlock + 8 * (x & 1) + g) * dh + 16 * t;
+#pragma unroll
+            for (int h = 0; h < Sh::NH; ++h)
+                kf[x][h] = at >= 0 && 64 * h + 16 * t < dh ? __ldg(reinterpret_cast<const uint4*>(kr + 64 * h)) : make_uint4(0u, 0u, 0u, 0u);
         }
-        __syncthreads();
-        uint32_t qb[3][Sh::NH][4];                                         // B fragments of column g
+    };
+    auto load_values = [&](const SplitItem& w, int blk) {
+        const int c0 = __shfl_sync(0xffffffffu, w.cell, blk & 31), c1 = __shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31);
 #pragma unroll
-        for (int e = 0; e < 3; ++e)
+        for (int b = 0; b < 2; ++b) {
+            const int at = b ? c1 : c0;
+            const int8_t* vr = p.c.v + ((long long)at * kKvBlock + 2 * t) * dh + (DP / 8) * g;
 #pragma unroll
-            for (int h = 0; h < Sh::NH; ++h) {
-                const uint4 w = lds128(qd + (e * kSplitCols + g) * DP + 64 * h + 16 * t);
-                qb[e][h][0] = w.x; qb[e][h][1] = w.y; qb[e][h][2] = w.z; qb[e][h][3] = w.w;
-            }
-        const float sq0 = sq[2 * t], sq1 = sq[2 * t + 1];
-        // keys that columns 2t and 2t + 1 see
-        const int pos0 = it.kv - it.len;
-        const int lim0 = 2 * t < cols ? min(pos0 + (col0 + 2 * t) / p.G + 1, n) : 0;
-        const int lim1 = 2 * t + 1 < cols ? min(pos0 + (col0 + 2 * t + 1) / p.G + 1, n) : 0;
-
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;        // running max; this lane's part of the sum
-        f32x2 o[Sh::NM][2];                                                // elements, columns (2t, 2t + 1)
+            for (int i = 0; i < 4; ++i) {
+                const int8_t* v = vr + ((i & 1) + 8 * (i >> 1)) * dh;
+                if constexpr (Sh::VW == 2) {
+                    const uint2 x = at >= 0 && 8 * g < dh ? __ldg(reinterpret_cast<const uint2*>(v)) : make_uint2(0u, 0u);
+                    vf[b][i][0] = x.x; vf[b][i][1] = x.y;
+                } else {
 #pragma unroll
-        for (int i = 0; i < Sh::NM; ++i) o[i][0] = o[i][1] = 0ull;
-
-        for (int j = j0 + warp * 32; j < jend; j += kSplitWarps * 32) {
-            // the step's two blocks: where they are and their scales
-            size_t at[2];
-            float sk[2], sv[2];
-            bool there[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int jb = j + 16 * b;
-                const int page = jb < jend ? page_of(p.c, p.r, it.s, jb) : -1;
-                there[b] = page >= 0;
-                if (jb < jend && page < 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
-                const size_t cell = ((size_t)max(page, 0) * p.c.KVH + it.kvh) * (psz >> 4) + ((jb & (psz - 1)) >> 4);
-                at[b] = cell * kKvBlock * dh;
-                sk[b] = there[b] ? __ldg(p.c.ks + cell) : 0.0f;
-                sv[b] = there[b] ? __ldg(p.c.vs + cell) : 0.0f;
-            }
-            uint4 kf[2][2][Sh::NH];                                        // [block][row g, g + 8][part]
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-#pragma unroll
-                    for (int h = 0; h < Sh::NH; ++h) {
-                        const int d = 64 * h + 16 * t;
-                        kf[b][r][h] = (there[b] && d < dh)
-                                          ? __ldg(reinterpret_cast<const uint4*>(p.c.k + at[b] + (size_t)(g + 8 * r) * dh + d))
-                                          : make_uint4(0u, 0u, 0u, 0u);
+                    for (int u = 0; u < Sh::VW / 4; ++u) {
+                        const uint4 x = at >= 0 && (DP / 8) * g + 16 * u < dh ? __ldg(reinterpret_cast<const uint4*>(v + 16 * u))
+                                                                              : make_uint4(0u, 0u, 0u, 0u);
+                        vf[b][i][4 * u] = x.x; vf[b][i][4 * u + 1] = x.y; vf[b][i][4 * u + 2] = x.z; vf[b][i][4 * u + 3] = x.w;
                     }
-            uint32_t vf[2][4][Sh::VW];                                     // [block][key 4t + i][words]
+                }
+            }
+        }
+    };
+    // an item's queries as A fragments in half `b` of the shared memory; 16 lanes a column
+    auto put_queries = [&](const SplitItem& w, int b) {
+        unsigned char* qd = ps_raw + b * (Sh::QBytes + 32);
+        const int col = tid >> 4, cc = w.col0 + col, tok = w.it.len == 1 ? 0 : cc / p.G;
+        query_digits<DP>(p.q + (size_t)(w.it.a + tok) * p.ldq + (size_t)(w.it.kvh * p.G + cc - tok * p.G) * dh, col < w.cols, dh,
+                         tid & 15, [&](int e, int d, uint32_t x) {
+                             // words of the part's 16-byte unit: x, y make step 0, z, w step 1
+                             const int h = d >> 6, q = (d >> 4) & 3, word = (d >> 2) & 3;
+                             const int frag = e ? word >> 1 : 2, reg = e ? 2 * (word & 1) + 2 - e : 2 * (word & 1) + (word >> 1);
+                             *reinterpret_cast<uint32_t*>(qd + ((h * 3 + frag) * 32 + 4 * col + q) * 16 + 4 * reg) = x;
+                         }, reinterpret_cast<float*>(qd + Sh::QBytes) + col);
+    };
+
+    load_keys(cur, 2 * warp);
+    load_values(cur, 2 * warp);
+    put_queries(cur, 0);
+    __syncthreads();
+    for (int buf = 0;; buf ^= 1) {
+        const unsigned char* qd = ps_raw + buf * (Sh::QBytes + 32);
+        const float sqg = reinterpret_cast<const float*>(qd + Sh::QBytes)[g];   // unit of column g's scores
+        const int pos0 = cur.it.kv - cur.it.len;
+        const int lim = g < cur.cols ? min(pos0 + (cur.it.len == 1 ? 0 : (cur.col0 + g) / p.G) + 1, cur.n) : 0;   // keys it sees
+        item += gridDim.x;
+        SplitItem nxt = next_split_item(p, item, lane);
+
+        float m = -INFINITY;
+        f32x2 l2 = 0ull;                                                   // this lane's part of the sum
+        f32x2 o[Sh::NT];                                                   // tile x: elements (DP/4) t + x, + DP/8 of column g
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+        for (int x = 0; x < Sh::NT; ++x) o[x] = 0ull;
+
+        int j = cur.j0 + warp * 32;
+#pragma unroll 1
+        do {                                                               // at least one step, if an empty one
+            const int blk = (j - cur.j0) >> 4;
+            const bool last = j + kSplitWarps * 32 >= cur.jend;
+            const int a0 = __shfl_sync(0xffffffffu, cur.cell, blk), a1 = __shfl_sync(0xffffffffu, cur.cell, blk + 1);
+            const float k0 = __shfl_sync(0xffffffffu, cur.ks, blk), k1 = __shfl_sync(0xffffffffu, cur.ks, blk + 1);
+            const float v0 = __shfl_sync(0xffffffffu, cur.vs, blk), v1 = __shfl_sync(0xffffffffu, cur.vs, blk + 1);
+            // scores (base 2) of keys 8 x + 2t, + 1 for column g
+            float2 s[4];
+            {
+                int hi[4][4], lo[4][2][4];                                 // hi: digit 2 in 0, 1 and digit 1 in 2, 3
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int8_t* vr = p.c.v + at[b] + (size_t)(4 * t + i) * dh;
-                    if constexpr (Sh::VW == 2) {
-                        const int d = 8 * g;
-                        const uint2 w = (there[b] && d < dh) ? __ldg(reinterpret_cast<const uint2*>(vr + d)) : make_uint2(0u, 0u);
-                        vf[b][i][0] = w.x; vf[b][i][1] = w.y;
-                    } else {
+                for (int h = 0; h < Sh::NH; ++h) {
+                    const uint4* fr = reinterpret_cast<const uint4*>(qd) + h * 96 + lane;
+                    const uint4 f0 = fr[0], f1 = fr[32], f2 = fr[64];
 #pragma unroll
-                        for (int u = 0; u < Sh::VW / 4; ++u) {
-                            const int d = (DP / 8) * g + 16 * u;
-                            const uint4 w = (there[b] && d < dh) ? __ldg(reinterpret_cast<const uint4*>(vr + d))
-                                                                 : make_uint4(0u, 0u, 0u, 0u);
-                            vf[b][i][4 * u] = w.x; vf[b][i][4 * u + 1] = w.y; vf[b][i][4 * u + 2] = w.z; vf[b][i][4 * u + 3] = w.w;
+                    for (int x = 0; x < 4; ++x) {
+                        if (h == 0) {
+                            mma_s8_first(hi[x], f0.x, f0.y, f0.z, f0.w, kf[x][h].x, kf[x][h].y);
+                            mma_s8_first(lo[x][0], f2.x, f2.y, f2.z, f2.w, kf[x][h].x, kf[x][h].y);
+                            mma_s8_first(lo[x][1], f2.x, f2.y, f2.z, f2.w, kf[x][h].z, kf[x][h].w);
+                        } else {
+                            mma_s8(hi[x], f0.x, f0.y, f0.z, f0.w, kf[x][h].x, kf[x][h].y);
+                            mma_s8(lo[x][0], f2.x, f2.y, f2.z, f2.w, kf[x][h].x, kf[x][h].y);
+                            mma_s8(lo[x][1], f2.x, f2.y, f2.z, f2.w, kf[x][h].z, kf[x][h].w);
                         }
+                        mma_s8(hi[x], f1.x, f1.y, f1.z, f1.w, kf[x][h].z, kf[x][h].w);
                     }
                 }
-
-            // scores (base 2): rows g, g + 8 of each block, columns 2t, 2t + 1
-            float s[2][4];
-            float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                int c[3][4];
-#pragma unroll
-                for (int h = 0; h < Sh::NH; ++h)
-#pragma unroll
-                    for (int e = 0; e < 3; ++e) {
-                        if (h == 0) mma_s8_first(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
-                        else mma_s8(c[e], kf[b][0][h].x, kf[b][1][h].x, kf[b][0][h].y, kf[b][1][h].y, qb[e][h][0], qb[e][h][1]);
-                        mma_s8(c[e], kf[b][0][h].z, kf[b][1][h].z, kf[b][0][h].w, kf[b][1][h].w, qb[e][h][2], qb[e][h][3]);
-                    }
-                const f32x2 u = pack2(sq0 * sk[b], sq1 * sk[b]);
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int key = j + 16 * b + 8 * r + g;
-                    const float2 a = unpack2(mul2(join_digits(c, 2 * r), u));
-                    s[b][2 * r] = there[b] && key < lim0 ? a.x : -INFINITY;
-                    s[b][2 * r + 1] = there[b] && key < lim1 ? a.y : -INFINITY;
-                    mx0 = fmaxf(mx0, s[b][2 * r]);
-                    mx1 = fmaxf(mx1, s[b][2 * r + 1]);
+                for (int x = 0; x < 4; ++x) {
+                    const float u = sqg * (x < 2 ? k0 : k1);
+                    s[x] = unpack2(mul2(join_digits(hi[x][0], hi[x][1], hi[x][2], hi[x][3], lo[x][0][0] + lo[x][1][2],
+                                                    lo[x][0][1] + lo[x][1][3]), pack2(u, u)));
                 }
             }
+            // the keys of the next step, of the next item after the last one
+            if (!last) load_keys(cur, blk + 2 * kSplitWarps);
+            else if (nxt.it.s >= 0) load_keys(nxt, 2 * warp);
+            float mx = m;
 #pragma unroll
-            for (int x = 4; x <= 16; x <<= 1) {
-                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
-                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+            for (int x = 0; x < 4; ++x) {
+                const int key = j + 8 * x + 2 * t, lx = (x < 2 ? a0 : a1) >= 0 ? lim : 0;
+                if (key >= lx) s[x].x = -INFINITY;
+                if (key + 1 >= lx) s[x].y = -INFINITY;
+                mx = fmaxf(mx, fmaxf(s[x].x, s[x].y));
             }
-            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-            const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
-            const float back0 = exp2_fast(m0 - b0), back1 = exp2_fast(m1 - b1);
-            m0 = n0; m1 = n1;
-            l0 *= back0; l1 *= back1;
-            // weights p v_scale; -inf scores (masked) give 0 even where a scale is NaN
-            float wt0 = 0.0f, wt1 = 0.0f;                                  // largest weights; NaN if one is
-            bool nan0 = false, nan1 = false;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            const float back = exp2_fast(m - base);
+            m = mx;
+            // weights p v_scale; a masked key weighs nothing even where the scale is NaN
+            float wt = 0.0f;
+            f32x2 ls = 0ull;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float sv = x < 2 ? v0 : v1;
+                const float2 e = make_float2(exp2_fast(s[x].x - base), exp2_fast(s[x].y - base));
+                ls = add2(ls, pack2(e.x, e.y));
+                s[x].x = s[x].x == -INFINITY ? 0.0f : e.x * sv;
+                s[x].y = s[x].y == -INFINITY ? 0.0f : e.y * sv;
+                wt = s[x].x != s[x].x || s[x].y != s[x].y ? INFINITY : fmaxf(wt, fmaxf(s[x].x, s[x].y));
+            }
+            l2 = fma2(l2, pack2(back, back), ls);
+            wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, 1));
+            wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, 2));
+            const float f = digit_factor(wt), u = f > 0.0f ? __fdividef(1.0f, f) : f;
+            uint32_t wd[2][3];                                             // digits of a block's four weights
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float e0 = exp2_fast(s[b][2 * r] - b0), e1 = exp2_fast(s[b][2 * r + 1] - b1);
-                    l0 += e0; l1 += e1;
-                    const float w0 = s[b][2 * r] == -INFINITY ? 0.0f : e0 * sv[b];
-                    const float w1 = s[b][2 * r + 1] == -INFINITY ? 0.0f : e1 * sv[b];
-                    s[b][2 * r] = w0; s[b][2 * r + 1] = w1;
-                    wt0 = fmaxf(wt0, w0); wt1 = fmaxf(wt1, w1);
-                    nan0 |= w0 != w0; nan1 |= w1 != w1;
-                }
-            if (nan0) wt0 = INFINITY;
-            if (nan1) wt1 = INFINITY;
-#pragma unroll
-            for (int x = 4; x <= 16; x <<= 1) {
-                wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
-                wt1 = fmaxf(wt1, __shfl_xor_sync(0xffffffffu, wt1, x));
-            }
-            const float f0 = digit_factor(wt0), f1 = digit_factor(wt1);
-            __syncwarp();
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    wxw[2 * t * Sh::WStride + 16 * b + 8 * r + g] = digit_bits_pos(s[b][2 * r], f0);
-                    wxw[(2 * t + 1) * Sh::WStride + 16 * b + 8 * r + g] = digit_bits_pos(s[b][2 * r + 1], f1);
-                }
-            __syncwarp();
-            uint32_t wb[2][3];                                             // B fragments: keys 4t .., 16 + 4t .. of column g
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const uint4 w = lds128(wxw + g * Sh::WStride + 16 * b + 4 * t);
-                digits4(w.x, w.y, w.z, w.w, wb[b]);
-            }
-            const f32x2 u = pack2(f0 > 0.0f ? __fdividef(1.0f, f0) : f0, f1 > 0.0f ? __fdividef(1.0f, f1) : f1);
-            const f32x2 back = pack2(back0, back1);
-            // output elements (DP / 8) g + 2 m, + 1 (rows g and g + 8 of tile m): four keys' bytes of one element
-            // make one A register
+                digits4(digit_bits_pos(s[2 * b].x, f), digit_bits_pos(s[2 * b].y, f), digit_bits_pos(s[2 * b + 1].x, f),
+                        digit_bits_pos(s[2 * b + 1].y, f), wd[b]);
+            // output: column n of tile x is element (DP/8) n + x: four keys' bytes of one
+            // element make one B register
 #pragma unroll
             for (int w = 0; w < Sh::VW; ++w) {
                 uint32_t a[2][4];
@@ -842,65 +857,69 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                     a[b][0] = __byte_perm(x, y, 0x5410); a[b][1] = __byte_perm(x, y, 0x7632);
                     a[b][2] = __byte_perm(z, v, 0x5410); a[b][3] = __byte_perm(z, v, 0x7632);
                 }
+                int hi[4][4], lo[4][4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    int c[3][4];
+                for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wd[0][2], wd[0][1], wd[1][2], wd[1][1], a[0][k], a[1][k]);
 #pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        mma_s8_first(c[e], a[0][2 * k], a[0][2 * k + 1], a[1][2 * k], a[1][2 * k + 1], wb[0][e], wb[1][e]);
+                for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wd[0][0], wd[0][0], wd[1][0], wd[1][0], a[0][k], a[1][k]);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) o[2 * w + k][i] = fma2(join_digits(c, 2 * i), u, mul2(o[2 * w + k][i], back));
-                }
+                for (int k = 0; k < 4; ++k)
+                    o[4 * w + k] = fma2(join_digits(hi[k][0], hi[k][1], hi[k][2], hi[k][3], lo[k][0], lo[k][1]), pack2(u, u),
+                                        mul2(o[4 * w + k], pack2(back, back)));
+            }
+            if (!last) load_values(cur, blk + 2 * kSplitWarps);
+            else if (nxt.it.s >= 0) load_values(nxt, 2 * warp);
+            j += kSplitWarps * 32;
+        } while (j < cur.jend);
+        // this warp's columns: sum over the lanes of a column, then all to shared memory
+        float* mo = reinterpret_cast<float*>(ps_raw + 2 * (Sh::QBytes + 32) + buf * Sh::MergeBytes);   // [4][8][DP + 4]
+        float l = unpack2(l2).x + unpack2(l2).y;
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        float* ow = mo + (warp * kSplitCols + g) * (DP + 4);
+        if (g < cur.cols) {
+            if (t == 0) { ow[DP] = m; ow[DP + 1] = l; }
+#pragma unroll
+            for (int x = 0; x < Sh::NT; x += 4) {
+                const float2 a = unpack2(o[x]), b = unpack2(o[x + 1]), c = unpack2(o[x + 2]), d = unpack2(o[x + 3]);
+                *reinterpret_cast<float4*>(ow + (DP / 4) * t + x) = make_float4(a.x, b.x, c.x, d.x);
+                *reinterpret_cast<float4*>(ow + (DP / 4) * t + DP / 8 + x) = make_float4(a.y, b.y, c.y, d.y);
             }
         }
-        // this warp's columns: sum over the lanes of a column, then all to shared memory
-#pragma unroll
-        for (int x = 4; x <= 16; x <<= 1) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-        }
-        if (g == 0) {
-            float* q = ml + (warp * kSplitCols + 2 * t) * 2;
-            q[0] = m0; q[1] = l0; q[2] = m1; q[3] = l1;
-        }
-        float* ow = mo + warp * kSplitCols * DP;
-#pragma unroll
-        for (int i = 0; i < Sh::NM; ++i) {
-            const int d = (DP / 8) * g + 2 * i;
-            const float2 x = unpack2(o[i][0]), y = unpack2(o[i][1]);
-            *reinterpret_cast<float2*>(ow + (2 * t) * DP + d) = make_float2(x.x, y.x);
-            *reinterpret_cast<float2*>(ow + (2 * t + 1) * DP + d) = make_float2(x.y, y.y);
-        }
+        if (nxt.it.s >= 0) put_queries(nxt, buf ^ 1);
         __syncthreads();
-        for (int i = tid; i < cols * (DP / 4); i += kSplitWarps * 32) {
-            const int col = i / (DP / 4), d = 4 * (i % (DP / 4)), cc = col0 + col;
-            const int pos = pos0 + cc / p.G, splits = row_splits(p, pos);
-            if (d >= dh || it.split >= splits) continue;
+        for (int i = tid; i < cur.cols * (DP / 4); i += kSplitWarps * 32) {
+            const int col = i / (DP / 4), d = 4 * (i % (DP / 4)), cc = cur.col0 + col, tok = cur.it.len == 1 ? 0 : cc / p.G;
+            const int splits = row_splits(p, pos0 + tok);
+            if (d >= dh || cur.it.split >= splits) continue;
+            const float* mc = mo + col * (DP + 4);
+            constexpr int W = kSplitCols * (DP + 4);
             float M = -INFINITY, L = 0.0f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kSplitWarps; ++w) M = fmaxf(M, ml[(w * kSplitCols + col) * 2]);
+            for (int w = 0; w < kSplitWarps; ++w) M = fmaxf(M, mc[w * W + DP]);
             const float B = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int w = 0; w < kSplitWarps; ++w) {
-                const float e = exp2_fast(ml[(w * kSplitCols + col) * 2] - B);
-                const float4 x = lds128f(mo + (w * kSplitCols + col) * DP + d);
-                L = ffma(ml[(w * kSplitCols + col) * 2 + 1], e, L);
+                const float e = exp2_fast(mc[w * W + DP] - B);
+                const float4 x = *reinterpret_cast<const float4*>(mc + w * W + d);
+                L = ffma(mc[w * W + DP + 1], e, L);
                 acc.x = ffma(x.x, e, acc.x); acc.y = ffma(x.y, e, acc.y);
                 acc.z = ffma(x.z, e, acc.z); acc.w = ffma(x.w, e, acc.w);
             }
-            const int row = it.a + cc / p.G, h = it.kvh * p.G + cc % p.G;
+            const int row = cur.it.a + tok, h = cur.it.kvh * p.G + cc - tok * p.G;
             if (splits == 1) {
                 const float inv = L == 0.0f ? 0.0f : fdiv(1.0f, L);
                 *reinterpret_cast<float4*>(p.out + (size_t)row * p.ldo + (size_t)h * dh + d) =
                     make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             } else {
-                float* pp = p.part + (((size_t)row * p.H + h) * p.nsplit + it.split) * (dh + 4);
+                float* pp = p.part + (((size_t)row * p.H + h) * p.nsplit + cur.it.split) * (dh + 4);
                 *reinterpret_cast<float4*>(pp + d) = acc;
                 if (d == 0) { pp[dh] = M; pp[dh + 1] = L; }
             }
         }
-        __syncthreads();
+        if (nxt.it.s < 0) return;
+        cur = nxt;
     }
 }
 
@@ -956,7 +975,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
     const int row0 = it.tile * kTileRows, rows = min(it.len * p.G - row0, kTileRows);
     const int pos0 = it.kv - it.len;
     const int n = min(pos0 + (row0 + rows - 1) / p.G + 1, p.r.cap);      // keys that any row sees
-    const int j0 = it.split * p.kc, jend = min(n, j0 + p.kc);
+    const int j0 = it.split << p.kc_log2, jend = min(n, j0 + (1 << p.kc_log2));
     if (j0 >= n && it.split > 0) return;
     const int ntiles = max((jend - j0 + KT - 1) / KT, 0);
 
