@@ -526,6 +526,19 @@ __device__ __forceinline__ float digit_factor(float top) {
     return top > 0.0f ? fminf(fdiv((float)kDigitMax, top), 0x1p126f) : 0.0f;
 }
 
+// the same for weights, whose largest is a probability times a value scale: the
+// approximate reciprocal is within 2^-22, and kDigitMax leaves room for that
+__device__ __forceinline__ float weight_factor(float top) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top));
+    return fminf(r * (float)kDigitMax, 0x1p126f);
+}
+__device__ __forceinline__ float weight_unit(float f) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(f));
+    return r;
+}
+
 struct PagedAttnParams {
     PagedKv c;
     PagedRows r;
@@ -706,34 +719,37 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
 
     uint4 kf[4][Sh::NH];                                                   // a step's keys 8 x + g
     uint32_t vf[2][4][Sh::VW];                                             // its values: [block][key 2t + {0, 1, 8, 9}][words]
+    // Blocks that are not there and elements past dh are read from the pool's first block and
+    // row: they meet masked weights and zero digits, or make elements that are not stored.
+    int kd[Sh::NH], vd[(Sh::VW + 3) / 4];                                  // element offsets inside a row
+#pragma unroll
+    for (int h = 0; h < Sh::NH; ++h) kd[h] = 64 * h + 16 * t < dh ? 64 * h + 16 * t : 0;
+#pragma unroll
+    for (int u = 0; u < (Sh::VW + 3) / 4; ++u) vd[u] = (DP / 8) * g + 16 * u < dh ? (DP / 8) * g + 16 * u : 0;
     auto load_keys = [&](const SplitItem& w, int blk) {
-        const int c0 = __shfl_sync(0xffffffffu, w.cell, blk & 31), c1 = __shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31);
+        const int c0 = max(__shfl_sync(0xffffffffu, w.cell, blk & 31), 0), c1 = max(__shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31), 0);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            const int at = x < 2 ? c0 : c1;
-            const int8_t* kr = p.c.k + ((long long)at * kKvBlock + 8 * (x & 1) + g) * dh + 16 * t;
+            const int8_t* kr = p.c.k + ((long long)(x < 2 ? c0 : c1) * kKvBlock + 8 * (x & 1) + g) * dh;
 #pragma unroll
-            for (int h = 0; h < Sh::NH; ++h)
-                kf[x][h] = at >= 0 && 64 * h + 16 * t < dh ? __ldg(reinterpret_cast<const uint4*>(kr + 64 * h)) : make_uint4(0u, 0u, 0u, 0u);
+            for (int h = 0; h < Sh::NH; ++h) kf[x][h] = __ldg(reinterpret_cast<const uint4*>(kr + kd[h]));
         }
     };
     auto load_values = [&](const SplitItem& w, int blk) {
-        const int c0 = __shfl_sync(0xffffffffu, w.cell, blk & 31), c1 = __shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31);
+        const int c0 = max(__shfl_sync(0xffffffffu, w.cell, blk & 31), 0), c1 = max(__shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31), 0);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const int at = b ? c1 : c0;
-            const int8_t* vr = p.c.v + ((long long)at * kKvBlock + 2 * t) * dh + (DP / 8) * g;
+            const int8_t* vr = p.c.v + ((long long)(b ? c1 : c0) * kKvBlock + 2 * t) * dh;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int8_t* v = vr + ((i & 1) + 8 * (i >> 1)) * dh;
                 if constexpr (Sh::VW == 2) {
-                    const uint2 x = at >= 0 && 8 * g < dh ? __ldg(reinterpret_cast<const uint2*>(v)) : make_uint2(0u, 0u);
+                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(v + vd[0]));
                     vf[b][i][0] = x.x; vf[b][i][1] = x.y;
                 } else {
 #pragma unroll
                     for (int u = 0; u < Sh::VW / 4; ++u) {
-                        const uint4 x = at >= 0 && (DP / 8) * g + 16 * u < dh ? __ldg(reinterpret_cast<const uint4*>(v + 16 * u))
-                                                                              : make_uint4(0u, 0u, 0u, 0u);
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(v + vd[u]));
                         vf[b][i][4 * u] = x.x; vf[b][i][4 * u + 1] = x.y; vf[b][i][4 * u + 2] = x.z; vf[b][i][4 * u + 3] = x.w;
                     }
                 }
@@ -762,6 +778,8 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         const float sqg = reinterpret_cast<const float*>(qd + Sh::QBytes)[g];   // unit of column g's scores
         const int pos0 = cur.it.kv - cur.it.len;
         const int lim = g < cur.cols ? min(pos0 + (cur.it.len == 1 ? 0 : (cur.col0 + g) / p.G) + 1, cur.n) : 0;   // keys it sees
+        // up to here no column needs a mask (idle columns have zero digits and no output)
+        const int whole_end = __reduce_min_sync(0xffffffffu, g < cur.cols ? lim : cur.n);
         item += gridDim.x;
         SplitItem nxt = next_split_item(p, item, lane);
 
@@ -811,40 +829,55 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             // the keys of the next step, of the next item after the last one
             if (!last) load_keys(cur, blk + 2 * kSplitWarps);
             else if (nxt.it.s >= 0) load_keys(nxt, 2 * warp);
+            const bool whole = j + 32 <= whole_end && (a0 | a1) >= 0 && v0 + v1 == v0 + v1;
+            if (!whole) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int key = j + 8 * x + 2 * t, lx = (x < 2 ? a0 : a1) >= 0 ? lim : 0;
+                    if (key >= lx) s[x].x = -INFINITY;
+                    if (key + 1 >= lx) s[x].y = -INFINITY;
+                }
+            }
             float mx = m;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int key = j + 8 * x + 2 * t, lx = (x < 2 ? a0 : a1) >= 0 ? lim : 0;
-                if (key >= lx) s[x].x = -INFINITY;
-                if (key + 1 >= lx) s[x].y = -INFINITY;
-                mx = fmaxf(mx, fmaxf(s[x].x, s[x].y));
-            }
+            for (int x = 0; x < 4; ++x) mx = fmaxf(mx, fmaxf(s[x].x, s[x].y));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const float base = mx == -INFINITY ? 0.0f : mx;
             const float back = exp2_fast(m - base);
             m = mx;
-            // weights p v_scale; a masked key weighs nothing even where the scale is NaN
-            float wt = 0.0f;
             f32x2 ls = 0ull;
+            float2 e[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
+                e[x] = make_float2(exp2_fast(s[x].x - base), exp2_fast(s[x].y - base));
+                ls = add2(ls, pack2(e[x].x, e[x].y));
                 const float sv = x < 2 ? v0 : v1;
-                const float2 e = make_float2(exp2_fast(s[x].x - base), exp2_fast(s[x].y - base));
-                ls = add2(ls, pack2(e.x, e.y));
-                s[x].x = s[x].x == -INFINITY ? 0.0f : e.x * sv;
-                s[x].y = s[x].y == -INFINITY ? 0.0f : e.y * sv;
-                wt = s[x].x != s[x].x || s[x].y != s[x].y ? INFINITY : fmaxf(wt, fmaxf(s[x].x, s[x].y));
+                e[x] = unpack2(mul2(pack2(e[x].x, e[x].y), pack2(sv, sv)));
             }
             l2 = fma2(l2, pack2(back, back), ls);
+            // weights p v_scale; a masked key weighs nothing even where the scale is NaN. A
+            // score that is not a number has made the sum NaN, which is enough
+            bool bad = false;
+            if (!whole) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if (s[x].x == -INFINITY) e[x].x = 0.0f;
+                    if (s[x].y == -INFINITY) e[x].y = 0.0f;
+                    bad |= e[x].x != e[x].x || e[x].y != e[x].y;
+                }
+            }
+            float wt = bad ? INFINITY : 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) wt = fmaxf(wt, fmaxf(e[x].x, e[x].y));
             wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, 1));
             wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, 2));
-            const float f = digit_factor(wt), u = f > 0.0f ? __fdividef(1.0f, f) : f;
+            const float f = weight_factor(wt), u = wt < INFINITY ? weight_unit(f) : __int_as_float(0x7fffffff);
             uint32_t wd[2][3];                                             // digits of a block's four weights
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-                digits4(digit_bits_pos(s[2 * b].x, f), digit_bits_pos(s[2 * b].y, f), digit_bits_pos(s[2 * b + 1].x, f),
-                        digit_bits_pos(s[2 * b + 1].y, f), wd[b]);
+                digits4(digit_bits_pos(e[2 * b].x, f), digit_bits_pos(e[2 * b].y, f), digit_bits_pos(e[2 * b + 1].x, f),
+                        digit_bits_pos(e[2 * b + 1].y, f), wd[b]);
             // output: column n of tile x is element (DP/8) n + x: four keys' bytes of one
             // element make one B register
 #pragma unroll
@@ -1031,12 +1064,12 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
         const long long at = cell[NB * (i & 1) + 4 * vh + vb];
 #pragma unroll
         for (int x = 0; x < VC; ++x) {
-            const int d = d0 + 16 * x;
-            const bool there = at >= 0 && d < dh;
-            const int8_t* src = p.c.v + (there ? at * (kKvBlock * dh) + vq2 * dh + d : 0);
+            // what is not there is read from the pool's first block: its weights are 0, and
+            // elements past dh are not stored
+            const int d = d0 + 16 * x < dh ? d0 + 16 * x : 0;
+            const int8_t* src = p.c.v + (max(at, 0ll) * kKvBlock + vq2) * dh + d;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                vr[x][k] = there ? __ldg(reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh)) : make_uint4(0u, 0u, 0u, 0u);
+            for (int k = 0; k < 4; ++k) vr[x][k] = __ldg(reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh));
         }
     };
     auto store_values = [&](int i) {
@@ -1190,9 +1223,9 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
                 wt0 = fmaxf(wt0, __shfl_xor_sync(0xffffffffu, wt0, x));
                 wt1 = fmaxf(wt1, __shfl_xor_sync(0xffffffffu, wt1, x));
             }
-            const float f0 = digit_factor(wt0), f1 = digit_factor(wt1);
-            u0 = f0 > 0.0f ? __fdividef(1.0f, f0) : f0;
-            u1 = f1 > 0.0f ? __fdividef(1.0f, f1) : f1;
+            const float f0 = weight_factor(wt0), f1 = weight_factor(wt1);
+            u0 = wt0 < INFINITY ? weight_unit(f0) : __int_as_float(0x7fffffff);
+            u1 = wt1 < INFINITY ? weight_unit(f1) : __int_as_float(0x7fffffff);
 #pragma unroll
             for (int ks = 0; ks < KT / 32; ++ks)
 #pragma unroll
