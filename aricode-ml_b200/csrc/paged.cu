@@ -146,8 +146,10 @@ int sm_count() {
 cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || p.nsplit == 1) return e;
-    paged_attn_join_kernel<<<dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), 256, 0, s>>>(p);
-    return cudaGetLastError();
+    // up to 8 splits: a warp each (row, head), else 8
+    if (p.nsplit <= 8)
+        return launch_ex(paged_attn_join_kernel<1>, dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
+    return launch_ex(paged_attn_join_kernel<8>, dim3((unsigned)p.r.n_rows, (unsigned)p.H), dim3(256), 0, s, true, p);
 }
 
 template <int DP>

@@ -461,6 +461,12 @@ __device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
+// four registers for an A operand. `zero` is a 0 that the compiler does not know: with a
+// plain copy it would gather the operand again for every MMA that uses it
+__device__ __forceinline__ void own_quad(uint32_t (&q)[4], uint32_t zero, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    q[0] = a ^ zero; q[1] = b ^ zero; q[2] = c ^ zero; q[3] = d ^ zero;
+}
+
 // two f32 in one instruction: the attention kernels are bound by what the schedulers
 // issue, and a packed operation takes one slot for two (same rounding)
 typedef unsigned long long f32x2;
@@ -548,6 +554,7 @@ struct PagedAttnParams {
     int H, G;                // G = H / KVH
     int kc_log2;             // keys per split
     int nsplit;              // splits of a sequence of cap keys
+    unsigned zero;           // 0
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
 };
@@ -685,6 +692,7 @@ __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, u
     SplitItem w;
     for (;; item += gridDim.x) {
         w.it = find_item<kSplitCols>(p, item, lane);
+        w.cell = -2;
         if (w.it.s < 0) return w;
         w.col0 = w.it.tile * kSplitCols;
         w.cols = min(w.it.len * p.G - w.col0, kSplitCols);
@@ -695,7 +703,6 @@ __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, u
     }
     w.jend = min(w.n, w.j0 + (1 << p.kc_log2));
     const int j = w.j0 + 16 * lane;
-    w.cell = -2;
     w.ks = w.vs = 0.0f;
     if (j < w.jend) {
         const int page = page_of(p.c, p.r, w.it.s, j), b = p.c.page_log2 - 4;
@@ -726,8 +733,8 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     for (int h = 0; h < Sh::NH; ++h) kd[h] = 64 * h + 16 * t < dh ? 64 * h + 16 * t : 0;
 #pragma unroll
     for (int u = 0; u < (Sh::VW + 3) / 4; ++u) vd[u] = (DP / 8) * g + 16 * u < dh ? (DP / 8) * g + 16 * u : 0;
-    auto load_keys = [&](const SplitItem& w, int blk) {
-        const int c0 = max(__shfl_sync(0xffffffffu, w.cell, blk & 31), 0), c1 = max(__shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31), 0);
+    auto load_keys = [&](int c0, int c1) {
+        c0 = max(c0, 0); c1 = max(c1, 0);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int8_t* kr = p.c.k + ((long long)(x < 2 ? c0 : c1) * kKvBlock + 8 * (x & 1) + g) * dh;
@@ -735,8 +742,8 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             for (int h = 0; h < Sh::NH; ++h) kf[x][h] = __ldg(reinterpret_cast<const uint4*>(kr + kd[h]));
         }
     };
-    auto load_values = [&](const SplitItem& w, int blk) {
-        const int c0 = max(__shfl_sync(0xffffffffu, w.cell, blk & 31), 0), c1 = max(__shfl_sync(0xffffffffu, w.cell, (blk + 1) & 31), 0);
+    auto load_values = [&](int c0, int c1) {
+        c0 = max(c0, 0); c1 = max(c1, 0);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int8_t* vr = p.c.v + ((long long)(b ? c1 : c0) * kKvBlock + 2 * t) * dh;
@@ -769,8 +776,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                          }, reinterpret_cast<float*>(qd + Sh::QBytes) + col);
     };
 
-    load_keys(cur, 2 * warp);
-    load_values(cur, 2 * warp);
+    int a0 = __shfl_sync(0xffffffffu, cur.cell, 2 * warp), a1 = __shfl_sync(0xffffffffu, cur.cell, 2 * warp + 1);
+    load_keys(a0, a1);
+    load_values(a0, a1);
     put_queries(cur, 0);
     __syncthreads();
     for (int buf = 0;; buf ^= 1) {
@@ -794,7 +802,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         do {                                                               // at least one step, if an empty one
             const int blk = (j - cur.j0) >> 4;
             const bool last = j + kSplitWarps * 32 >= cur.jend;
-            const int a0 = __shfl_sync(0xffffffffu, cur.cell, blk), a1 = __shfl_sync(0xffffffffu, cur.cell, blk + 1);
+            // the next step's blocks, of the next item after the last one
+            const int nblk = last ? 2 * warp : blk + 2 * kSplitWarps, ncell = last ? nxt.cell : cur.cell;
+            const int na0 = __shfl_sync(0xffffffffu, ncell, nblk), na1 = __shfl_sync(0xffffffffu, ncell, nblk + 1);
             const float k0 = __shfl_sync(0xffffffffu, cur.ks, blk), k1 = __shfl_sync(0xffffffffu, cur.ks, blk + 1);
             const float v0 = __shfl_sync(0xffffffffu, cur.vs, blk), v1 = __shfl_sync(0xffffffffu, cur.vs, blk + 1);
             // scores (base 2) of keys 8 x + 2t, + 1 for column g
@@ -826,9 +836,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                                                     lo[x][0][1] + lo[x][1][3]), pack2(u, u)));
                 }
             }
-            // the keys of the next step, of the next item after the last one
-            if (!last) load_keys(cur, blk + 2 * kSplitWarps);
-            else if (nxt.it.s >= 0) load_keys(nxt, 2 * warp);
+            load_keys(na0, na1);
             const bool whole = j + 32 <= whole_end && (a0 | a1) >= 0 && v0 + v1 == v0 + v1;
             if (!whole) {
 #pragma unroll
@@ -878,6 +886,11 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             for (int b = 0; b < 2; ++b)
                 digits4(digit_bits_pos(e[2 * b].x, f), digit_bits_pos(e[2 * b].y, f), digit_bits_pos(e[2 * b + 1].x, f),
                         digit_bits_pos(e[2 * b + 1].y, f), wd[b]);
+            // A registers of their own, so that no MMA has to gather them (rows 8 to 15 of the
+            // second one are not used)
+            uint32_t wh[4], wl[4];
+            own_quad(wh, p.zero, wd[0][2], wd[0][1], wd[1][2], wd[1][1]);
+            own_quad(wl, p.zero, wd[0][0], wd[0][0], wd[1][0], wd[1][0]);
             // output: column n of tile x is element (DP/8) n + x: four keys' bytes of one
             // element make one B register
 #pragma unroll
@@ -892,16 +905,16 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 }
                 int hi[4][4], lo[4][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wd[0][2], wd[0][1], wd[1][2], wd[1][1], a[0][k], a[1][k]);
+                for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wh[0], wh[1], wh[2], wh[3], a[0][k], a[1][k]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wd[0][0], wd[0][0], wd[1][0], wd[1][0], a[0][k], a[1][k]);
+                for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wl[0], wl[1], wl[2], wl[3], a[0][k], a[1][k]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     o[4 * w + k] = fma2(join_digits(hi[k][0], hi[k][1], hi[k][2], hi[k][3], lo[k][0], lo[k][1]), pack2(u, u),
                                         mul2(o[4 * w + k], pack2(back, back)));
             }
-            if (!last) load_values(cur, blk + 2 * kSplitWarps);
-            else if (nxt.it.s >= 0) load_values(nxt, 2 * warp);
+            load_values(na0, na1);
+            a0 = na0; a1 = na1;
             j += kSplitWarps * 32;
         } while (j < cur.jend);
         // this warp's columns: sum over the lanes of a column, then all to shared memory
@@ -951,7 +964,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 if (d == 0) { pp[dh] = M; pp[dh + 1] = L; }
             }
         }
-        if (nxt.it.s < 0) return;
+        if (nxt.it.s < 0) return;                                          // (a CTA's end lets the join start)
         cur = nxt;
     }
 }
@@ -1309,11 +1322,18 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
     }
 }
 
-// One warp per (row, head) with more than one split: joins them in split order. Grid
-// (rows, CTAs of 8 heads).
-static __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x, h = blockIdx.y * 8 + (threadIdx.x >> 5), dh = p.c.dh;
-    if (h >= p.H) return;
+// Joins a (row, head)'s splits in a fixed order: WPH warps a pair, warp w the splits w,
+// w + WPH, ..., then the warps in order. Bound by latency: the splits' maxima and sums are
+// read a lane each, so that the partial outputs' loads depend on nothing and overlap.
+// (One warp for 79 splits took 35 us where the attention itself took 26.) Grid (rows,
+// heads * WPH / 8).
+template <int WPH>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p) {
+    __shared__ __align__(16) float so[8][256];
+    __shared__ float sm[8][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x, dh = p.c.dh;
+    const int h = blockIdx.y * (8 / WPH) + warp / WPH, part = warp % WPH;
+    pdl_wait();                                                    // the splits are written
     int pos = 0;
     bool found = false;
     for (int base = 0; base < p.r.n_seq && !found; base += 32) {
@@ -1325,30 +1345,70 @@ static __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __gri
             found = true;
         }
     }
-    const int n = found ? row_splits(p, pos) : 0;
+    const int n = found ? row_splits(p, pos) : 0;                  // the same for the whole CTA
     if (n < 2) return;
     const int stride = dh + 4;
-    const float* base = p.part + ((size_t)row * p.H + h) * p.nsplit * stride;
-    float M = -INFINITY;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, base[(size_t)s * stride + dh]);
-#pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    const float B = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
+    const float* base = p.part + ((size_t)row * p.H + min(h, p.H - 1)) * p.nsplit * stride;
+    float M = -INFINITY, L = 0.0f;
     float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    for (int s = 0; s < n; ++s) {
-        const float* ps = base + (size_t)s * stride;
-        const float e = exp2_fast(ps[dh] - B);
-        L = ffma(ps[dh + 1], e, L);
+    for (int s0 = part; s0 < n; s0 += 32 * WPH) {                  // 32 of this warp's splits at a time
+        const int s = s0 + lane * WPH;
+        const bool live = s < n;
+        const float ms = live ? base[(size_t)s * stride + dh] : -INFINITY, ls = live ? base[(size_t)s * stride + dh + 1] : 0.0f;
+        float top = ms;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int d = 4 * lane + 128 * i;
-            if (d >= dh) continue;
-            const float4 x = *reinterpret_cast<const float4*>(ps + d);
-            acc[i].x = ffma(x.x, e, acc[i].x); acc[i].y = ffma(x.y, e, acc[i].y);
-            acc[i].z = ffma(x.z, e, acc[i].z); acc[i].w = ffma(x.w, e, acc[i].w);
+        for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, M);
+        const float B = top == -INFINITY ? 0.0f : top, back = exp2_fast(M - B), e = live ? exp2_fast(ms - B) : 0.0f;
+        M = top;
+        float add = e * ls;
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) add += __shfl_xor_sync(0xffffffffu, add, x);
+        L = ffma(L, back, add);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { acc[i].x *= back; acc[i].y *= back; acc[i].z *= back; acc[i].w *= back; }
+        const int cnt = min((n - s0 + WPH - 1) / WPH, 32);
+#pragma unroll 8
+        for (int k = 0; k < cnt; ++k) {
+            const float w = __shfl_sync(0xffffffffu, e, k);
+            const float* ps = base + (size_t)(s0 + k * WPH) * stride;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = 4 * lane + 128 * i;
+                if (d >= dh) continue;
+                const float4 x = *reinterpret_cast<const float4*>(ps + d);
+                acc[i].x = ffma(x.x, w, acc[i].x); acc[i].y = ffma(x.y, w, acc[i].y);
+                acc[i].z = ffma(x.z, w, acc[i].z); acc[i].w = ffma(x.w, w, acc[i].w);
+            }
         }
     }
+    if constexpr (WPH > 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (4 * lane + 128 * i < dh) *reinterpret_cast<float4*>(&so[warp][4 * lane + 128 * i]) = acc[i];
+        if (lane == 0) { sm[warp][0] = M; sm[warp][1] = L; }
+        __syncthreads();
+        if (part != 0) return;
+        M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WPH; ++w) M = fmaxf(M, sm[warp + w][0]);
+        const float B = M == -INFINITY ? 0.0f : M;
+        L = 0.0f;
+        acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WPH; ++w) {
+            const float e = exp2_fast(sm[warp + w][0] - B);
+            L = ffma(sm[warp + w][1], e, L);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (4 * lane + 128 * i >= dh) continue;
+                const float4 x = *reinterpret_cast<const float4*>(&so[warp + w][4 * lane + 128 * i]);
+                acc[i].x = ffma(x.x, e, acc[i].x); acc[i].y = ffma(x.y, e, acc[i].y);
+                acc[i].z = ffma(x.z, e, acc[i].z); acc[i].w = ffma(x.w, e, acc[i].w);
+            }
+        }
+    }
+    if (h >= p.H) return;
     const float inv = L == 0.0f ? 0.0f : fdiv(1.0f, L);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
