@@ -101,11 +101,20 @@ cudaError_t launch_norm_rope(const NormRopeParams& p, cudaStream_t s) {
 }
 
 template <int LPH, int VPL>
-cudaError_t launch_append(AppendParams p, bool queries, cudaStream_t s) {
+cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream_t s) {
     p.kv_ctas = (2 * p.c.KVH + 7) / 8;
-    int y = p.kv_ctas;
-    if (queries) y += (kKvBlock * ((p.nr.H + 3) / 4) * LPH + 255) / 256;
-    kv_append_kernel<LPH, VPL><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
+    // single rows (said by the caller, or on average): one row in registers, queries along
+    if (max_rows == 1 || p.r.n_rows <= p.r.n_seq) {
+        const int y = p.kv_ctas + (queries ? (p.nr.H * LPH + 255) / 256 : 0);
+        kv_append_kernel<LPH, VPL, 1><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
+        return cudaGetLastError();
+    }
+    kv_append_kernel<LPH, VPL, kKvBlock * LPH / 32><<<dim3((unsigned)p.items, (unsigned)p.kv_ctas), 256, 0, s>>>(p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || !queries) return e;
+    // about four units of 4 vectors a lane group
+    const int y = (kKvBlock * ((p.nr.H + 3) / 4) * LPH / 4 + 255) / 256;
+    append_queries_kernel<LPH, VPL><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -241,7 +250,7 @@ int b2_kv_append_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* 
     p.items = run_bound(p.r);
     p.err = err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define B2_CALL(L, V) launch_append<L, V>(p, q != nullptr, s)
+#define B2_CALL(L, V) launch_append<L, V>(p, q != nullptr, rows->max_rows, s)
     return status(fn, B2_BY_HEAD_DIM(kv->d_head, B2_CALL));
 #undef B2_CALL
 }

@@ -248,62 +248,18 @@ struct AppendParams {
     int* err;
 };
 
-// One warp: the run's rows of one head's K or V. It holds all of them in registers
-// (lane group i the rows i, i + RPW, ...), so the block's new scale is known before
-// a code is written.
-template <int LPH, int VPL>
+// One warp: the run's rows of one head's K or V, NP passes of 32 / LPH rows (lane group i
+// the rows i, i + 32 / LPH, ...) held in registers. The block's new scale is known when
+// all rows have been seen; if they are more than the registers hold they are fetched
+// again for the codes.
+template <int LPH, int VPL, int NP>
 __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRun& run, int page, int head, bool is_k,
                                             int lane) {
     constexpr int RPW = 32 / LPH;                  // rows per pass
-    constexpr int NP = kKvBlock / RPW;             // passes
     const int dh = p.c.dh, gl = lane % LPH, g = lane / LPH;
-    const float* src = is_k ? p.k : p.v;
+    const float* src = (is_k ? p.k : p.v) + (size_t)head * dh;
     const long long ld = is_k ? p.ldk : p.ldv;
     const bool rope = is_k && p.nr.table;
-    float4 x[NP][VPL];
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int i = j * RPW + g;
-#pragma unroll
-        for (int e = 0; e < VPL; ++e) {
-            const int d = 4 * (gl + LPH * e);
-            x[j][e] = (i < run.n && d < dh)
-                          ? __ldg(reinterpret_cast<const float4*>(src + (size_t)(run.row + i) * ld + (size_t)head * dh + d))
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    }
-    if (is_k && p.nr.gk) {
-        float4 gv[VPL];
-#pragma unroll
-        for (int e = 0; e < VPL; ++e) {
-            const int d = 4 * (gl + LPH * e);
-            gv[e] = d < dh ? __ldg(reinterpret_cast<const float4*>(p.nr.gk + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int j = 0; j < NP; ++j)
-            if (j * RPW < run.n) head_norm<LPH, VPL>(x[j], gv, dh, p.nr.eps);
-    }
-    if (rope) {
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const int i = j * RPW + g;
-#pragma unroll
-            for (int e = 0; e < VPL; ++e) {
-                const int d = 4 * (gl + LPH * e);
-                if (i < run.n && d < dh)
-                    x[j][e] = rotate4(x[j][e], __ldg(reinterpret_cast<const float4*>(
-                                                   p.nr.table + (size_t)(run.pos + i) * dh + d)));
-            }
-        }
-    }
-    unsigned am = 0u;                              // largest |x| as bits: a NaN or infinity is above 0x7f7fffff
-#pragma unroll
-    for (int j = 0; j < NP; ++j)
-#pragma unroll
-        for (int e = 0; e < VPL; ++e)
-            am = max(am, max(max(__float_as_uint(x[j][e].x) & 0x7fffffffu, __float_as_uint(x[j][e].y) & 0x7fffffffu),
-                             max(__float_as_uint(x[j][e].z) & 0x7fffffffu, __float_as_uint(x[j][e].w) & 0x7fffffffu)));
-    am = __reduce_max_sync(0xffffffffu, am);
     const int psz = 1 << p.c.page_log2;
     const int off = run.pos & (psz - 1), o0 = run.pos % kKvBlock;
     const size_t cell = ((size_t)page * p.c.KVH + head) * (psz / kKvBlock) + off / kKvBlock;
@@ -311,6 +267,54 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
     int8_t* codes = (is_k ? p.c.k : p.c.v) + cell * kKvBlock * dh;    // the block's 16 rows
     // a block that starts with this run has no older rows: its scale starts afresh
     const float old = o0 == 0 ? 0.0f : *sp;
+    float4 x[NP][VPL];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int i = i0 + j * RPW + g;
+#pragma unroll
+            for (int e = 0; e < VPL; ++e) {
+                const int d = 4 * (gl + LPH * e);
+                x[j][e] = (i < run.n && d < dh) ? __ldg(reinterpret_cast<const float4*>(src + (size_t)(run.row + i) * ld + d))
+                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+        if (is_k && p.nr.gk) {
+            float4 gv[VPL];
+#pragma unroll
+            for (int e = 0; e < VPL; ++e) {
+                const int d = 4 * (gl + LPH * e);
+                gv[e] = d < dh ? __ldg(reinterpret_cast<const float4*>(p.nr.gk + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+                if (i0 + j * RPW < run.n) head_norm<LPH, VPL>(x[j], gv, dh, p.nr.eps);
+        }
+        if (rope) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int i = i0 + j * RPW + g;
+#pragma unroll
+                for (int e = 0; e < VPL; ++e) {
+                    const int d = 4 * (gl + LPH * e);
+                    if (i < run.n && d < dh)
+                        x[j][e] = rotate4(x[j][e], __ldg(reinterpret_cast<const float4*>(
+                                                       p.nr.table + (size_t)(run.pos + i) * dh + d)));
+                }
+            }
+        }
+    };
+    unsigned am = 0u;                              // largest |x| as bits: a NaN or infinity is above 0x7f7fffff
+    for (int i0 = 0; i0 < run.n; i0 += NP * RPW) {
+        fetch(i0);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int e = 0; e < VPL; ++e)
+                am = max(am, max(max(__float_as_uint(x[j][e].x) & 0x7fffffffu, __float_as_uint(x[j][e].y) & 0x7fffffffu),
+                                 max(__float_as_uint(x[j][e].z) & 0x7fffffffu, __float_as_uint(x[j][e].w) & 0x7fffffffu)));
+    }
+    am = __reduce_max_sync(0xffffffffu, am);
     float now = am >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fdiv(__uint_as_float(am), 127.0f);
     if (!(now <= old)) {                           // grown (or NaN on either side)
         if (old != old) now = old;
@@ -334,31 +338,53 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
     auto code = [&](float v) {
         return some ? (signed char)max(-127, min(127, __float2int_rn(fdiv(v, now)))) : (signed char)0;
     };
+    for (int i0 = 0; i0 < run.n; i0 += NP * RPW) {
+        if (run.n > NP * RPW) fetch(i0);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int i = j * RPW + g;
+        for (int j = 0; j < NP; ++j) {
+            const int i = i0 + j * RPW + g;
 #pragma unroll
-        for (int e = 0; e < VPL; ++e) {
-            const int d = 4 * (gl + LPH * e);
-            if (i < run.n && d < dh)
-                *reinterpret_cast<char4*>(codes + (size_t)(o0 + i) * dh + d) =
-                    make_char4(code(x[j][e].x), code(x[j][e].y), code(x[j][e].z), code(x[j][e].w));
+            for (int e = 0; e < VPL; ++e) {
+                const int d = 4 * (gl + LPH * e);
+                if (i < run.n && d < dh)
+                    *reinterpret_cast<char4*>(codes + (size_t)(o0 + i) * dh + d) =
+                        make_char4(code(x[j][e].x), code(x[j][e].y), code(x[j][e].z), code(x[j][e].w));
+            }
         }
     }
 }
 
-// Grid (runs, CTAs of a run): every warp finds the run; a warp of the first kv_ctas
-// takes one head's K or V of it, a group of lanes of the others 4 query vectors of a row.
-template <int LPH, int VPL>
-__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// the run of this CTA without the rows that lie past the table (they have no rotation)
+__device__ __forceinline__ BlockRun run_in_table(const AppendParams& p, int lane) {
     BlockRun run = find_run(p.r, blockIdx.x, p.items, p.err, lane);
-    if (run.s < 0) return;
-    if (p.nr.table && run.pos + run.n > p.nr.table_rows) {          // rows past the table have no rotation
+    if (run.s >= 0 && p.nr.table && run.pos + run.n > p.nr.table_rows) {
         if (lane == 0) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
-        run.n = p.nr.table_rows - run.pos;
-        if (run.n <= 0) return;
+        run.n = max(p.nr.table_rows - run.pos, 0);
     }
+    return run;
+}
+
+// a run's queries, HPU vectors of a row at a time: unit numbers from `unit` on
+template <int LPH, int VPL, int HPU>
+__device__ __forceinline__ void append_queries(const AppendParams& p, const BlockRun& run, int unit, int step, int lane) {
+    const int per_row = (p.nr.H + HPU - 1) / HPU, units = run.n * per_row;
+    for (int first = unit - lane / LPH; first < units; first += step, unit += step) {   // whole warps
+        const int i = unit / per_row;
+        const bool live = unit < units;
+        norm_rope_heads<LPH, VPL, HPU>(p.nr, live ? run.row + i : 0, unit % per_row * HPU, lane % LPH, live,
+                                       live ? run.pos + i : 0);
+    }
+}
+
+// Grid (runs, CTAs of a run): every warp finds the run; a warp of the first kv_ctas
+// takes one head's K or V of it, those of the others queries.
+// NP = 1: for calls of single rows. Few registers, so that a whole decode step is on the
+// SMs at once: it is bound by the latency of run -> page -> scale and older codes.
+template <int LPH, int VPL, int NP>
+__global__ void __launch_bounds__(256, NP == 1 && VPL == 1 ? 5 : 2) kv_append_kernel(const __grid_constant__ AppendParams p) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const BlockRun run = run_in_table(p, lane);
+    if (run.s < 0 || run.n == 0) return;
     if ((int)blockIdx.y < p.kv_ctas) {
         const int task = blockIdx.y * 8 + warp;
         if (task >= 2 * p.c.KVH) return;
@@ -367,16 +393,20 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
             if (lane == 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
             return;
         }
-        append_head<LPH, VPL>(p, run, page, task >> 1, (task & 1) == 0, lane);
+        append_head<LPH, VPL, NP>(p, run, page, task >> 1, (task & 1) == 0, lane);
         return;
     }
-    constexpr int HPU = 4;
-    const int per_row = (p.nr.H + HPU - 1) / HPU;
-    const int unit = ((blockIdx.y - p.kv_ctas) * 256 + threadIdx.x) / LPH;
-    const int i = unit / per_row;
-    const bool live = i < run.n;
-    norm_rope_heads<LPH, VPL, HPU>(p.nr, live ? run.row + i : 0, unit % per_row * HPU, lane % LPH, live,
-                                   live ? run.pos + i : 0);
+    append_queries<LPH, VPL, 1>(p, run, ((blockIdx.y - p.kv_ctas) * 256 + threadIdx.x) / LPH,
+                                (gridDim.y - p.kv_ctas) * 256 / LPH, lane);
+}
+
+// the queries of long calls, in a launch of their own: the registers that hold a block's
+// rows above would leave them too few warps to keep the memory busy
+template <int LPH, int VPL>
+__global__ void __launch_bounds__(256) append_queries_kernel(const __grid_constant__ AppendParams p) {
+    const BlockRun run = run_in_table(p, threadIdx.x & 31);
+    if (run.s < 0) return;
+    append_queries<LPH, VPL, 4>(p, run, (blockIdx.y * 256 + threadIdx.x) / LPH, gridDim.y * 256 / LPH, threadIdx.x & 31);
 }
 
 // ------------------------------------------------------------------ read back

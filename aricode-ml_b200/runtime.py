@@ -10,6 +10,7 @@ memory and pass raw pointers to the C ABI.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import json
 from pathlib import Path
@@ -470,53 +471,45 @@ def _invalid(msg):
     return B2Error(-1, msg)
 
 
-def _tensor(name, t, dtype, dev, shape=None):
-    """A contiguous CUDA tensor of this type on `dev` (None: any GPU)."""
-    if not t.is_cuda or t.dtype != dtype or not t.is_contiguous() or (dev is not None and t.device != dev):
-        raise _invalid(f"{name} must be a contiguous {dtype} tensor on {dev or 'a GPU'}")
-    if shape is not None and tuple(t.shape) != shape:
+def _tensor(name, t, dtype, gpu, shape=None):
+    """The address of a contiguous CUDA tensor of this type and shape on GPU number `gpu` (None: any)."""
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous() or (gpu is not None and t.get_device() != gpu):
+        raise _invalid(f"{name} must be a contiguous {dtype} tensor on {'a GPU' if gpu is None else f'cuda:{gpu}'}")
+    if shape is not None and t.shape != shape:
         raise _invalid(f"{name} must have shape {shape}, not {tuple(t.shape)}")
-    return t
+    return t.data_ptr()
 
 
-def _f32_rows(name, t, dev, n_rows, width):
-    """(pointer, row stride) of an f32 [n_rows, width] tensor whose rows are contiguous."""
-    import torch
-    if t.dtype != torch.float32 or t.device != dev or t.dim() != 2:
-        raise _invalid(f"{name} must be a 2-D float32 tensor on {dev}")
-    if t.shape[0] < n_rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+def _f32_rows(name, t, f32, gpu, n_rows, width):
+    """(address, row stride) of an f32 [n_rows, width] tensor whose rows are contiguous."""
+    shape, step = t.shape, t.stride()
+    if t.dtype is not f32 or len(shape) != 2 or t.get_device() != gpu:
+        raise _invalid(f"{name} must be a 2-D float32 tensor on cuda:{gpu}")
+    n = shape[0]
+    if n < n_rows or shape[1] != width or (step[1] != 1 and width > 1):
         raise _invalid(f"{name} must hold {n_rows} rows of {width} contiguous elements")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else (width + 3) // 4 * 4)
+    return t.data_ptr(), (step[0] if n > 1 else (width + 3) // 4 * 4)
 
 
-def _opt(name, t, dtype, dev, shape):
-    return None if t is None else _tensor(name, t, dtype, dev, shape).data_ptr()
+def _here(torch, gpu, stream):
+    """The stream handle for a call on GPU `gpu` if nothing has to be switched for it (the C calls run on the current
+    device, and tensors that a call makes belong to the current stream), else None."""
+    if torch.cuda.current_device() != gpu:
+        return None
+    # the handle alone: building a Stream object costs more than the launch
+    cur = torch._C._cuda_getCurrentRawStream(gpu)
+    return cur if stream is None or int(stream) == cur else None
 
 
-class _on:
-    """The device and stream of a call: `dev` current inside (the C calls run on the current device); `stream` a
-    handle or None (the device's current stream). Tensors made inside belong to that stream."""
-
-    def __init__(self, dev, stream):
-        import torch
-        self._guards = []
-        if torch.cuda.current_device() != dev.index:
-            self._guards.append(torch.cuda.device(dev))
+@contextlib.contextmanager
+def _there(torch, gpu, stream):
+    """`gpu` and `stream` (a handle; None: that GPU's current one) as the current device and stream."""
+    with torch.cuda.device(gpu):
         if stream is None:
-            self.handle = torch.cuda.current_stream(dev).cuda_stream
+            yield
         else:
-            self.handle = int(stream)
-            if self.handle != torch.cuda.current_stream(dev).cuda_stream:
-                self._guards.append(torch.cuda.stream(torch.cuda.ExternalStream(self.handle, device=dev)))
-
-    def __enter__(self):
-        for g in self._guards:
-            g.__enter__()
-        return self.handle
-
-    def __exit__(self, *a):
-        for g in reversed(self._guards):
-            g.__exit__(*a)
+            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=gpu)):
+                yield
 
 
 class PagedKV:
@@ -532,10 +525,10 @@ class PagedKV:
         if n < 1 or h < 1 or d < 16 or d > 256 or d % 16 or page < 16 or page > 1024 or page & (page - 1):
             raise _invalid("page_size must be a power of two from 16 to 1024, d_head a multiple of 16 up to 256")
         _tensor("k", k, torch.int8, None)
-        self.device = k.device
-        _tensor("v", v, torch.int8, self.device, (n, h, page, d))
-        _tensor("k_scale", k_scale, torch.float32, self.device, (n, h, page // KV_BLOCK))
-        _tensor("v_scale", v_scale, torch.float32, self.device, (n, h, page // KV_BLOCK))
+        self.device, self.gpu = k.device, k.get_device()
+        _tensor("v", v, torch.int8, self.gpu, (n, h, page, d))
+        _tensor("k_scale", k_scale, torch.float32, self.gpu, (n, h, page // KV_BLOCK))
+        _tensor("v_scale", v_scale, torch.float32, self.gpu, (n, h, page // KV_BLOCK))
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.d_head = n, h, page, d
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -568,12 +561,12 @@ class KVRows:
     def __init__(self, row_start, kv_len, page_table, n_rows, max_keys=0, max_rows=0):
         import torch
         _tensor("kv_len", kv_len, torch.int32, None)
-        self.device = kv_len.device
+        self.device, self.gpu = kv_len.device, kv_len.get_device()
         if kv_len.dim() != 1 or page_table.dim() != 2:
             raise _invalid("kv_len must be 1-D and page_table 2-D")
         n = kv_len.shape[0]
-        _tensor("row_start", row_start, torch.int32, self.device, (n + 1,))
-        _tensor("page_table", page_table, torch.int32, self.device, (n, page_table.shape[1]))
+        _tensor("row_start", row_start, torch.int32, self.gpu, (n + 1,))
+        _tensor("page_table", page_table, torch.int32, self.gpu, (n, page_table.shape[1]))
         if n_rows < 0 or max_keys < 0 or max_rows < 0:
             raise _invalid("n_rows, max_keys and max_rows must not be negative")
         self.row_start, self.kv_len, self.page_table = row_start, kv_len, page_table
@@ -581,12 +574,6 @@ class KVRows:
         self._c = _KvRows(row_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), n, page_table.shape[1],
                           self.n_rows, int(max_keys), int(max_rows))
         self._p = C.addressof(self._c)
-
-
-def _pair(kv, rows):
-    if kv.device != rows.device:
-        raise _invalid("the cache and the rows must be on one device")
-    return kv.device
 
 
 def qk_norm_rope(q, k, d_head, pos=None, table=None, q_gain=None, k_gain=None, eps=1e-5, q_scale=1.0, q_out=None,
@@ -598,33 +585,43 @@ def qk_norm_rope(q, k, d_head, pos=None, table=None, q_gain=None, k_gain=None, e
     given. Returns (q_out, k_out)."""
     import torch
     one = q if q is not None else k
-    if one is None:
-        raise _invalid("q or k must be given")
-    dev, n = one.device, one.shape[0]
-    if not one.is_cuda or one.dim() != 2 or d_head <= 0:
-        raise _invalid("q and k must be 2-D CUDA tensors, d_head positive")
-    with _on(dev, stream) as h:
-        widths = []
-        for name, x, out in (("q", q, q_out), ("k", k, k_out)):
-            if x is None:
-                widths.append((None, 0, None, 0, 0, None))
-                continue
-            w = x.shape[-1]
-            if w % d_head or x.shape[0] != n:
-                raise _invalid(f"{name} must hold whole heads, and as many rows as the other")
-            src = _f32_rows(name, x, dev, n, w)
-            if out is None:
-                out = torch.empty(n, w, device=dev)
-            widths.append((*src, *_f32_rows(name + "_out", out, dev, n, w), w // d_head, out))
-        (qp, ldq, qop, ldqo, H, q_out), (kp, ldk, kop, ldko, K, k_out) = widths
-        if table is not None and (pos is None or table.dim() != 2):
+    if one is None or not one.is_cuda or one.dim() != 2 or d_head <= 0:
+        raise _invalid("q or k must be given as 2-D CUDA tensors, d_head positive")
+    gpu, n, f32, i32 = one.get_device(), one.shape[0], torch.float32, torch.int32
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return qk_norm_rope(q, k, d_head, pos, table, q_gain, k_gain, eps, q_scale, q_out, k_out, err)
+    qp = kp = qop = kop = None
+    ldq = ldk = ldqo = ldko = H = K = rows = 0
+    if q is not None:
+        w = q.shape[-1]
+        H = w // d_head
+        if w != H * d_head:
+            raise _invalid("q must hold whole heads")
+        qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
+        q_out = torch.empty(n, w, device=q.device) if q_out is None else q_out
+        qop, ldqo = _f32_rows("q_out", q_out, f32, gpu, n, w)
+    if k is not None:
+        w = k.shape[-1]
+        K = w // d_head
+        if w != K * d_head or k.shape[0] != n:
+            raise _invalid("k must hold whole heads, and as many rows as q")
+        kp, ldk = _f32_rows("k", k, f32, gpu, n, w)
+        k_out = torch.empty(n, w, device=k.device) if k_out is None else k_out
+        kop, ldko = _f32_rows("k_out", k_out, f32, gpu, n, w)
+    if table is not None:
+        if pos is None or table.dim() != 2:
             raise _invalid("a table [positions, d_head] needs pos")
-        check(lib().b2_qk_norm_rope(
-            qp, ldq, kp, ldk, qop, ldqo, kop, ldko, _opt("q_gain", q_gain, torch.float32, dev, (d_head,)),
-            _opt("k_gain", k_gain, torch.float32, dev, (d_head,)), eps, q_scale,
-            None if table is None else _tensor("table", table, torch.float32, dev, (table.shape[0], d_head)).data_ptr(),
-            0 if table is None else table.shape[0], _opt("pos", pos, torch.int32, dev, (n,)), n, H, K, d_head,
-            _opt("err", err, torch.int32, dev, (1,)), h))
+        rows = table.shape[0]
+        table = _tensor("table", table, f32, gpu, (rows, d_head))
+    rc = lib().b2_qk_norm_rope(
+        qp, ldq, kp, ldk, qop, ldqo, kop, ldko, q_gain if q_gain is None else _tensor("q_gain", q_gain, f32, gpu, (d_head,)),
+        k_gain if k_gain is None else _tensor("k_gain", k_gain, f32, gpu, (d_head,)), eps, q_scale, table, rows,
+        pos if pos is None else _tensor("pos", pos, i32, gpu, (n,)), n, H, K, d_head,
+        err if err is None else _tensor("err", err, i32, gpu, (1,)), h)
+    if rc:
+        check(rc)
     return q_out, k_out
 
 
@@ -633,28 +630,37 @@ def kv_append_i8(kv, rows, k, v, table=None, k_gain=None, eps=1e-5, q=None, q_ga
     """Append the call's rows k and v [n_rows, kv_heads * d_head] f32 to the cache, keys normed (k_gain) and rotated
     (table) on the way; with q, the queries likewise (times q_scale) into q_out, which is returned."""
     import torch
-    dev, d, n = _pair(kv, rows), kv.d_head, rows.n_rows
+    gpu, d, n, f32 = kv.gpu, kv.d_head, rows.n_rows, torch.float32
+    if rows.gpu != gpu:
+        raise _invalid("the cache and the rows must be on one device")
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return kv_append_i8(kv, rows, k, v, table, k_gain, eps, q, q_gain, q_scale, q_out)
     w = kv.n_kv_heads * d
-    kp, ldk = _f32_rows("k", k, dev, n, w)
-    vp_, ldv = _f32_rows("v", v, dev, n, w)
-    with _on(dev, stream) as h:
-        qp, ldq, qop, ldqo, H = None, 0, None, 0, 0
-        if q is not None:
-            wq = q.shape[-1]
-            if wq % d:
-                raise _invalid("q must hold whole heads")
-            qp, ldq = _f32_rows("q", q, dev, n, wq)
-            if q_out is None:
-                q_out = torch.empty(q.shape[0], wq, device=dev)
-            qop, ldqo = _f32_rows("q_out", q_out, dev, n, wq)
-            H = wq // d
-        if table is not None and table.dim() != 2:
+    kp, ldk = _f32_rows("k", k, f32, gpu, n, w)
+    v_, ldv = _f32_rows("v", v, f32, gpu, n, w)
+    qp = qop = None
+    ldq = ldqo = H = t_rows = 0
+    if q is not None:
+        w = q.shape[-1]
+        H = w // d
+        if w != H * d:
+            raise _invalid("q must hold whole heads")
+        qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
+        q_out = torch.empty(q.shape[0], w, device=q.device) if q_out is None else q_out
+        qop, ldqo = _f32_rows("q_out", q_out, f32, gpu, n, w)
+    if table is not None:
+        if table.dim() != 2:
             raise _invalid("table must be [positions, d_head]")
-        check(lib().b2_kv_append_i8(
-            kv._p, rows._p, kp, ldk, vp_, ldv, _opt("k_gain", k_gain, torch.float32, dev, (d,)), eps,
-            None if table is None else _tensor("table", table, torch.float32, dev, (table.shape[0], d)).data_ptr(),
-            0 if table is None else table.shape[0], qp, ldq, qop, ldqo, _opt("q_gain", q_gain, torch.float32, dev, (d,)),
-            q_scale, H, kv._err, h))
+        t_rows = table.shape[0]
+        table = _tensor("table", table, f32, gpu, (t_rows, d))
+    rc = lib().b2_kv_append_i8(
+        kv._p, rows._p, kp, ldk, v_, ldv, k_gain if k_gain is None else _tensor("k_gain", k_gain, f32, gpu, (d,)), eps,
+        table, t_rows, qp, ldq, qop, ldqo, q_gain if q_gain is None else _tensor("q_gain", q_gain, f32, gpu, (d,)), q_scale,
+        H, kv._err, h)
+    if rc:
+        check(rc)
     return q_out
 
 
@@ -662,26 +668,33 @@ def kv_read_i8(kv, rows, dtype=None, k_out=None, v_out=None, stream=None):
     """The rows' cached keys and values as (k, v) [n_rows, kv_heads * d_head] of dtype float32 (the default) or
     bfloat16. Rows that belong to no sequence stay as they are in the outputs (unset in new ones)."""
     import torch
-    dev, n, w = _pair(kv, rows), rows.n_rows, kv.n_kv_heads * kv.d_head
-    if k_out is not None:
-        dtype = dtype or k_out.dtype
-    dtype = dtype or torch.float32
-    if dtype not in (torch.float32, torch.bfloat16):
+    gpu, n, w = kv.gpu, rows.n_rows, kv.n_kv_heads * kv.d_head
+    if rows.gpu != gpu:
+        raise _invalid("the cache and the rows must be on one device")
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return kv_read_i8(kv, rows, dtype, k_out, v_out)
+    if dtype is None:
+        dtype = torch.float32 if k_out is None else k_out.dtype
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise _invalid("dtype must be float32 or bfloat16")
-    with _on(dev, stream) as h:
-        outs = [torch.empty(n, w, dtype=dtype, device=dev) if o is None else _tensor("k_out and v_out", o, dtype, dev, (n, w))
-                for o in (k_out, v_out)]
-        check(lib().b2_kv_read_i8(kv._p, rows._p, outs[0].data_ptr(), outs[1].data_ptr(), w, dtype == torch.bfloat16,
-                                  kv._err, h))
-    return outs[0], outs[1]
+    k_out = torch.empty(n, w, dtype=dtype, device=kv.device) if k_out is None else k_out
+    v_out = torch.empty(n, w, dtype=dtype, device=kv.device) if v_out is None else v_out
+    rc = lib().b2_kv_read_i8(kv._p, rows._p, _tensor("k_out", k_out, dtype, gpu, (n, w)),
+                             _tensor("v_out", v_out, dtype, gpu, (n, w)), w, dtype is torch.bfloat16, kv._err, h)
+    if rc:
+        check(rc)
+    return k_out, v_out
 
 
 def attn_paged_workspace(kv, rows, n_heads, stream=None):
     """A workspace tensor that attn_paged_i8 calls of these sizes can share, one after another."""
     import torch
-    dev = _pair(kv, rows)
-    with _on(dev, stream):
-        return torch.empty(lib().b2_attn_paged_i8_workspace(kv._p, rows._p, int(n_heads)), dtype=torch.uint8, device=dev)
+    if _here(torch, kv.gpu, stream) is None:
+        with _there(torch, kv.gpu, stream):
+            return attn_paged_workspace(kv, rows, n_heads)
+    return torch.empty(lib().b2_attn_paged_i8_workspace(kv._p, rows._p, int(n_heads)), dtype=torch.uint8, device=kv.device)
 
 
 def attn_paged_i8(kv, rows, q, out=None, workspace=None, stream=None):
@@ -689,22 +702,26 @@ def attn_paged_i8(kv, rows, q, out=None, workspace=None, stream=None):
     sequence's keys up to its own position. Rows that belong to no sequence stay as they are in `out` (unset in a new
     one). Without a workspace the call makes its own."""
     import torch
-    dev, n = _pair(kv, rows), rows.n_rows
+    gpu, n, f32 = kv.gpu, rows.n_rows, torch.float32
+    if rows.gpu != gpu:
+        raise _invalid("the cache and the rows must be on one device")
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return attn_paged_i8(kv, rows, q, out, workspace)
     w = q.shape[-1]
-    if w % kv.d_head:
-        raise _invalid("q must hold whole heads")
     H = w // kv.d_head
-    qp, ldq = _f32_rows("q", q, dev, n, w)
-    with _on(dev, stream) as h:
-        if out is None:
-            out = torch.empty(q.shape[0], w, device=dev)
-        op, ldo = _f32_rows("out", out, dev, n, w)
-        if workspace is None:
-            workspace = attn_paged_workspace(kv, rows, H)
-        else:
-            _tensor("workspace", workspace, torch.uint8, dev)
-        check(lib().b2_attn_paged_i8(kv._p, rows._p, qp, ldq, op, ldo, H, workspace.data_ptr(), workspace.numel(),
-                                     kv._err, h))
+    if w != H * kv.d_head:
+        raise _invalid("q must hold whole heads")
+    qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
+    out = torch.empty(q.shape[0], w, device=q.device) if out is None else out
+    op, ldo = _f32_rows("out", out, f32, gpu, n, w)
+    if workspace is None:
+        workspace = attn_paged_workspace(kv, rows, H)
+    rc = lib().b2_attn_paged_i8(kv._p, rows._p, qp, ldq, op, ldo, H, _tensor("workspace", workspace, torch.uint8, gpu),
+                                workspace.numel(), kv._err, h)
+    if rc:
+        check(rc)
     return out
 
 
