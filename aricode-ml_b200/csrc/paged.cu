@@ -87,16 +87,14 @@ int run_bound(const PagedRows& r) {
 
 template <int LPH, int VPL>
 cudaError_t launch_norm_rope(const NormRopeParams& p, cudaStream_t s) {
-    const int heads = p.H + p.KVH;
     // four vectors a lane group once there is work for the whole GPU (their loads are
     // in flight together and share the table row), one before that
-    const long long lanes = (long long)p.n_rows * heads * LPH;
-    if (lanes >= 4ll * 148 * 1024) {
-        const long long n = (long long)p.n_rows * ((heads + 3) / 4) * LPH;
-        norm_rope_kernel<LPH, VPL, 4><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
-    } else {
-        norm_rope_kernel<LPH, VPL, 1><<<(unsigned)((lanes + 255) / 256), 256, 0, s>>>(p);
-    }
+    const bool four = (long long)p.n_rows * (p.H + p.KVH) * LPH >= 4ll * 148 * 1024;
+    const int hpu = four ? 4 : 1;
+    const long long lanes = (long long)p.n_rows * ((p.H + hpu - 1) / hpu + (p.KVH + hpu - 1) / hpu) * LPH;
+    const unsigned grid = (unsigned)((lanes + 255) / 256);
+    if (four) norm_rope_kernel<LPH, VPL, 4><<<grid, 256, 0, s>>>(p);
+    else norm_rope_kernel<LPH, VPL, 1><<<grid, 256, 0, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -211,11 +209,12 @@ int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, fl
         return refuse(fn, "gains and table must be 16-byte aligned, pos and err 4");
     if (table && (!pos || table_rows <= 0)) return refuse(fn, "a table needs pos and table_rows");
     if ((q_gain || k_gain) && !(eps >= 0.0f && std::isfinite(eps))) return refuse(fn, "eps must be finite and not negative");
-    if ((long long)n_rows * (n_heads + n_kv_heads) > (1ll << 31)) return refuse(fn, "more than 2^31 head vectors");
+    if ((long long)n_rows * (n_heads + n_kv_heads) >= (1ll << 26)) return refuse(fn, "2^26 or more head vectors");
     NormRopeParams p{};
     p.q = q; p.k = k; p.qo = q_out; p.ko = k_out;
     p.ldq = ldq; p.ldk = ldk; p.ldqo = ldqo; p.ldko = ldko;
     p.gq = q_gain; p.gk = k_gain; p.eps = eps; p.q_scale = q_scale;
+    p.inv_dh = 1.0f / (float)d_head;
     p.table = table; p.table_rows = table_rows; p.pos = pos;
     p.n_rows = n_rows; p.H = n_heads; p.KVH = n_kv_heads; p.dh = d_head; p.err = err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -245,6 +244,7 @@ int b2_kv_append_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* 
     p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
     p.nr.q = q; p.nr.qo = q_out; p.nr.ldq = ldq; p.nr.ldqo = ldqo;
     p.nr.gq = q_gain; p.nr.gk = k_gain; p.nr.eps = eps; p.nr.q_scale = q_scale;
+    p.nr.inv_dh = 1.0f / (float)kv->d_head;
     p.nr.table = table; p.nr.table_rows = table_rows;
     p.nr.n_rows = p.r.n_rows; p.nr.H = q ? n_heads : 0; p.nr.KVH = 0; p.nr.dh = kv->d_head; p.nr.err = err;
     p.items = run_bound(p.r);

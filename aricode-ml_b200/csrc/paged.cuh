@@ -105,34 +105,36 @@ __device__ __forceinline__ BlockRun find_run(const PagedRows& r, int item, int m
 
 // ------------------------------------------------------------------ norm + rotation
 // Head vectors in registers: LPH lanes hold a vector, VPL float4s each (lane l of
-// the group the elements 4 l + 128 i ..), so dh <= 4 LPH VPL.
+// the group the elements 4 l + 4 LPH i ..), so dh <= 4 LPH VPL.
+
+// 1 / sqrt(mean x^2 + eps) of a vector (inv_dh = 1 / dh); rsqrtf is within 2^-22.9, no
+// more than the sum's own roundings
 template <int LPH, int VPL>
-__device__ __forceinline__ void head_norm(float4 (&x)[VPL], const float4 (&g)[VPL], int dh, float eps) {
+__device__ __forceinline__ float head_rms(const float4 (&x)[VPL], float inv_dh, float eps) {
     float a = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-        a = fadd(a, fadd(fadd(fmul(x[i].x, x[i].x), fmul(x[i].y, x[i].y)),
-                         fadd(fmul(x[i].z, x[i].z), fmul(x[i].w, x[i].w))));
+    for (int i = 0; i < VPL; ++i) a = ffma(x[i].x, x[i].x, ffma(x[i].y, x[i].y, ffma(x[i].z, x[i].z, ffma(x[i].w, x[i].w, a))));
 #pragma unroll
     for (int o = LPH / 2; o >= 1; o >>= 1) a = fadd(a, __shfl_xor_sync(0xffffffffu, a, o));
-    const float r = fdiv(1.0f, __fsqrt_rn(fadd(fdiv(a, (float)dh), eps)));
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        x[i].x = fmul(fmul(x[i].x, r), g[i].x);
-        x[i].y = fmul(fmul(x[i].y, r), g[i].y);
-        x[i].z = fmul(fmul(x[i].z, r), g[i].z);
-        x[i].w = fmul(fmul(x[i].w, r), g[i].w);
-    }
+    return rsqrtf(ffma(a, inv_dh, eps));
 }
 
-// two neighbouring pairs by (cos, sin, cos, sin): b2_rope_apply's arithmetic
-__device__ __forceinline__ float4 rotate4(const float4& x, const float4& t) {
-    float4 y;
-    y.x = fsub(fmul(x.x, t.x), fmul(x.y, t.y));
-    y.y = fadd(fmul(x.x, t.y), fmul(x.y, t.x));
-    y.z = fsub(fmul(x.z, t.z), fmul(x.w, t.w));
-    y.w = fadd(fmul(x.z, t.w), fmul(x.w, t.z));
-    return y;
+// The norm's gains and the rotation of two neighbouring pairs in one: the products of
+// gain and (cos, sin) are made once for all vectors of a row, then a vector costs what
+// the rotation alone would. Without gains this is b2_rope_apply's arithmetic.
+struct Turn {
+    float4 c, s;             // own and the other element's factor, signs in
+};
+__device__ __forceinline__ Turn make_turn(const float4& t, const float4& g) {
+    Turn r;
+    r.c = make_float4(fmul(g.x, t.x), fmul(g.y, t.x), fmul(g.z, t.z), fmul(g.w, t.z));
+    r.s = make_float4(-fmul(g.y, t.y), fmul(g.x, t.y), -fmul(g.w, t.w), fmul(g.z, t.w));
+    return r;
+}
+// b * s + a * c with two products and a sum, so that nothing depends on which is fused
+__device__ __forceinline__ float4 turn4(const float4& x, const Turn& t) {
+    return make_float4(fadd(fmul(x.x, t.c.x), fmul(x.y, t.s.x)), fadd(fmul(x.x, t.s.y), fmul(x.y, t.c.y)),
+                       fadd(fmul(x.z, t.c.z), fmul(x.w, t.s.z)), fadd(fmul(x.z, t.s.w), fmul(x.w, t.c.w)));
 }
 
 struct NormRopeParams {
@@ -143,7 +145,7 @@ struct NormRopeParams {
     long long ldq, ldk, ldqo, ldko;
     const float* gq;         // [dh] or nullptr: no norm
     const float* gk;
-    float eps, q_scale;
+    float eps, q_scale, inv_dh;
     const float* table;      // [table_rows][dh] (cos, sin) pairs or nullptr: no rotation
     int table_rows;
     const int* pos;          // [n_rows]; negative: the row is left alone
@@ -151,78 +153,59 @@ struct NormRopeParams {
     int* err;
 };
 
-// HPU vectors of one row through norm, rotation and scale, all loads first. `h0`
-// the first of them in the row's list (queries, then keys); `live`: the group has
-// work (every lane of the warp runs along for the shuffles).
+// HPU neighbouring vectors of one row's queries or keys (group number `grp` of them: H /
+// HPU groups of queries, then the keys') through norm, rotation and scale, all loads
+// first. `live`: the lane group has work (every lane of the warp runs along for the
+// shuffles).
 template <int LPH, int VPL, int HPU>
-__device__ __forceinline__ void norm_rope_heads(const NormRopeParams& p, int row, int h0, int gl, bool live,
-                                                int pos) {
-    const int NH = p.H + p.KVH;
+__device__ __forceinline__ void norm_rope_heads(const NormRopeParams& p, int row, int grp, int gl, bool live, int pos) {
+    const int qgroups = (p.H + HPU - 1) / HPU;
+    const bool isq = grp < qgroups;
+    const int h0 = (isq ? grp : grp - qgroups) * HPU, cnt = live ? min((isq ? p.H : p.KVH) - h0, HPU) : 0;
+    const float* src = (isq ? p.q + (size_t)row * p.ldq : p.k + (size_t)row * p.ldk) + (size_t)h0 * p.dh + 4 * gl;
+    float* dst = (isq ? p.qo + (size_t)row * p.ldqo : p.ko + (size_t)row * p.ldko) + (size_t)h0 * p.dh + 4 * gl;
     float4 x[HPU][VPL];
 #pragma unroll
-    for (int u = 0; u < HPU; ++u) {
-        const int h = h0 + u;
-        const float* src = h < p.H ? p.q + (size_t)row * p.ldq + (size_t)h * p.dh
-                                   : p.k + (size_t)row * p.ldk + (size_t)(h - p.H) * p.dh;
+    for (int u = 0; u < HPU; ++u)
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const int d = 4 * (gl + LPH * i);
-            x[u][i] = (live && h < NH && d < p.dh) ? *reinterpret_cast<const float4*>(src + d)
-                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    }
-    float4 t[VPL];
+        for (int i = 0; i < VPL; ++i)
+            x[u][i] = u < cnt && 4 * (gl + LPH * i) < p.dh ? *reinterpret_cast<const float4*>(src + u * p.dh + 4 * LPH * i)
+                                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* g = isq ? p.gq : p.gk;
+    Turn t[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
         const int d = 4 * (gl + LPH * i);
-        t[i] = (live && p.table && d < p.dh)
-                   ? __ldg(reinterpret_cast<const float4*>(p.table + (size_t)pos * p.dh + d))
-                   : make_float4(1.f, 0.f, 1.f, 0.f);
+        t[i] = make_turn(cnt > 0 && p.table && d < p.dh ? __ldg(reinterpret_cast<const float4*>(p.table + (size_t)pos * p.dh + d))
+                                                        : make_float4(1.f, 0.f, 1.f, 0.f),
+                         g && d < p.dh ? __ldg(reinterpret_cast<const float4*>(g + d)) : make_float4(1.f, 1.f, 1.f, 1.f));
     }
+    const bool norm = p.gq || p.gk;                            // the same for the whole warp: it shuffles
+    const float sc = isq ? p.q_scale : 1.0f;
 #pragma unroll
     for (int u = 0; u < HPU; ++u) {
-        const int h = h0 + u;
-        const bool isq = h < p.H;
-        const float* g = isq ? p.gq : p.gk;
-        // the shuffles of the norm need the whole warp: every lane takes them when
-        // either gain is given, and a vector without one keeps its values
-        if (p.gq || p.gk) {
-            float4 y[VPL], gv[VPL];
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const int d = 4 * (gl + LPH * i);
-                y[i] = x[u][i];
-                gv[i] = (g && d < p.dh) ? __ldg(reinterpret_cast<const float4*>(g + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            head_norm<LPH, VPL>(y, gv, p.dh, p.eps);
-            if (g)
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) x[u][i] = y[i];
+        float r = sc;
+        if (norm) {
+            const float m = head_rms<LPH, VPL>(x[u], p.inv_dh, p.eps);
+            if (g) r = fmul(m, sc);
         }
-        if (!live || h >= NH) continue;
-        float* dst = isq ? p.qo + (size_t)row * p.ldqo + (size_t)h * p.dh
-                         : p.ko + (size_t)row * p.ldko + (size_t)(h - p.H) * p.dh;
-        const float sc = isq ? p.q_scale : 1.0f;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int d = 4 * (gl + LPH * i);
-            if (d >= p.dh) continue;
-            float4 y = p.table ? rotate4(x[u][i], t[i]) : x[u][i];
-            if (isq) { y.x = fmul(y.x, sc); y.y = fmul(y.y, sc); y.z = fmul(y.z, sc); y.w = fmul(y.w, sc); }
-            *reinterpret_cast<float4*>(dst + d) = y;
+            float4 y = turn4(x[u][i], t[i]);
+            y = make_float4(fmul(y.x, r), fmul(y.y, r), fmul(y.z, r), fmul(y.w, r));
+            if (u < cnt && 4 * (gl + LPH * i) < p.dh) *reinterpret_cast<float4*>(dst + u * p.dh + 4 * LPH * i) = y;
         }
     }
 }
 
-// One lane group per (row, HPU heads). The row's table entries are loaded once for
-// its HPU heads.
+// One lane group per (row, HPU heads). Bound by memory once there are enough rows; what
+// a vector costs in instructions comes next (see make_turn).
 template <int LPH, int VPL, int HPU>
 __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
-    const int per_row = (p.H + p.KVH + HPU - 1) / HPU;
-    const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) / LPH;
+    const unsigned per_row = (p.H + HPU - 1) / HPU + (p.KVH + HPU - 1) / HPU;
+    const unsigned unit = (blockIdx.x * 256u + threadIdx.x) / LPH, row = unit / per_row;
     const int gl = threadIdx.x % LPH;
-    const long long row = unit / per_row;
-    bool live = row < p.n_rows;
+    bool live = row < (unsigned)p.n_rows;
     int pos = 0;
     if (live && p.pos) {
         pos = __ldg(p.pos + row);
@@ -232,7 +215,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
             set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
         }
     }
-    norm_rope_heads<LPH, VPL, HPU>(p, live ? (int)row : 0, (int)(unit % per_row) * HPU, gl, live, live ? pos : 0);
+    norm_rope_heads<LPH, VPL, HPU>(p, live ? (int)row : 0, (int)(unit % per_row), gl, live, live ? pos : 0);
 }
 
 // ------------------------------------------------------------------ append
@@ -287,8 +270,14 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
                 gv[e] = d < dh ? __ldg(reinterpret_cast<const float4*>(p.nr.gk + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
-            for (int j = 0; j < NP; ++j)
-                if (i0 + j * RPW < run.n) head_norm<LPH, VPL>(x[j], gv, dh, p.nr.eps);
+            for (int j = 0; j < NP; ++j) {
+                if (i0 + j * RPW >= run.n) continue;
+                const float r = head_rms<LPH, VPL>(x[j], p.nr.inv_dh, p.nr.eps);
+#pragma unroll
+                for (int e = 0; e < VPL; ++e)
+                    x[j][e] = make_float4(fmul(fmul(x[j][e].x, r), gv[e].x), fmul(fmul(x[j][e].y, r), gv[e].y),
+                                          fmul(fmul(x[j][e].z, r), gv[e].z), fmul(fmul(x[j][e].w, r), gv[e].w));
+            }
         }
         if (rope) {
 #pragma unroll
@@ -298,14 +287,14 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
                 for (int e = 0; e < VPL; ++e) {
                     const int d = 4 * (gl + LPH * e);
                     if (i < run.n && d < dh)
-                        x[j][e] = rotate4(x[j][e], __ldg(reinterpret_cast<const float4*>(
-                                                       p.nr.table + (size_t)(run.pos + i) * dh + d)));
+                        x[j][e] = turn4(x[j][e], make_turn(__ldg(reinterpret_cast<const float4*>(p.nr.table + (size_t)(run.pos + i) * dh + d)),
+                                                           make_float4(1.f, 1.f, 1.f, 1.f)));
                 }
             }
         }
     };
     unsigned am = 0u;                              // largest |x| as bits: a NaN or infinity is above 0x7f7fffff
-    for (int i0 = 0; i0 < run.n; i0 += NP * RPW) {
+    for (int i0 = 0; i0 < (NP * RPW < kKvBlock ? run.n : 1); i0 += NP * RPW) {
         fetch(i0);
 #pragma unroll
         for (int j = 0; j < NP; ++j)
@@ -334,21 +323,35 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
     }
     __syncwarp();
     if (lane == 0) *sp = now;
+    // x / now rounded to an integer: the quotient by the reciprocal and one correction is
+    // the f32 division's (a scale whose reciprocal or remainders could leave f32's normal
+    // range takes the division itself); adding 1.5 * 2^23 rounds it into the low byte
     const bool some = now > 0.0f;                  // false for a block of zeros and for a NaN scale
+    const bool plain = now > 0x1p-100f && now < 0x1p100f;
+    const float inv = fdiv(1.0f, now);
     auto code = [&](float v) {
-        return some ? (signed char)max(-127, min(127, __float2int_rn(fdiv(v, now)))) : (signed char)0;
+        float q;
+        if (plain) {
+            q = fmul(v, inv);
+            q = ffma(ffma(-q, now, v), inv, q);
+        } else {
+            q = some ? fmaxf(-127.0f, fminf(127.0f, fdiv(v, now))) : 0.0f;
+        }
+        return __float_as_uint(fadd(q, 12582912.0f));
     };
-    for (int i0 = 0; i0 < run.n; i0 += NP * RPW) {
-        if (run.n > NP * RPW) fetch(i0);
+    for (int i0 = 0; i0 < (NP * RPW < kKvBlock ? run.n : 1); i0 += NP * RPW) {
+        if constexpr (NP * RPW < kKvBlock)
+            if (run.n > NP * RPW) fetch(i0);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int i = i0 + j * RPW + g;
 #pragma unroll
             for (int e = 0; e < VPL; ++e) {
                 const int d = 4 * (gl + LPH * e);
+                const uint32_t lo = __byte_perm(code(x[j][e].x), code(x[j][e].y), 0x0040),
+                               hi = __byte_perm(code(x[j][e].z), code(x[j][e].w), 0x0040);
                 if (i < run.n && d < dh)
-                    *reinterpret_cast<char4*>(codes + (size_t)(o0 + i) * dh + d) =
-                        make_char4(code(x[j][e].x), code(x[j][e].y), code(x[j][e].z), code(x[j][e].w));
+                    *reinterpret_cast<uint32_t*>(codes + (size_t)(o0 + i) * dh + d) = __byte_perm(lo, hi, 0x5410);
             }
         }
     }
@@ -371,7 +374,7 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, const Bloc
     for (int first = unit - lane / LPH; first < units; first += step, unit += step) {   // whole warps
         const int i = unit / per_row;
         const bool live = unit < units;
-        norm_rope_heads<LPH, VPL, HPU>(p.nr, live ? run.row + i : 0, unit % per_row * HPU, lane % LPH, live,
+        norm_rope_heads<LPH, VPL, HPU>(p.nr, live ? run.row + i : 0, unit % per_row, lane % LPH, live,
                                        live ? run.pos + i : 0);
     }
 }
@@ -381,7 +384,7 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, const Bloc
 // NP = 1: for calls of single rows. Few registers, so that a whole decode step is on the
 // SMs at once: it is bound by the latency of run -> page -> scale and older codes.
 template <int LPH, int VPL, int NP>
-__global__ void __launch_bounds__(256, NP == 1 && VPL == 1 ? 5 : 2) kv_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256, VPL == 2 && NP > 1 ? 1 : NP == 1 && VPL == 1 ? 5 : 2) kv_append_kernel(const __grid_constant__ AppendParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const BlockRun run = run_in_table(p, lane);
     if (run.s < 0 || run.n == 0) return;
