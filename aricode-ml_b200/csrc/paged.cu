@@ -100,14 +100,15 @@ cudaError_t launch_norm_rope(const NormRopeParams& p, cudaStream_t s) {
 
 template <int LPH, int VPL>
 cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream_t s) {
-    p.kv_ctas = (2 * p.c.KVH + 7) / 8;
     // single rows (said by the caller, or on average): one row in registers, queries along
     if (max_rows == 1 || p.r.n_rows <= p.r.n_seq) {
+        p.kv_ctas = (2 * p.c.KVH + 7) / 8;
         const int y = p.kv_ctas + (queries ? (p.nr.H * LPH + 255) / 256 : 0);
-        kv_append_kernel<LPH, VPL, 1><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
+        kv_append_kernel<LPH, VPL, 1, 1><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
         return cudaGetLastError();
     }
-    kv_append_kernel<LPH, VPL, kKvBlock * LPH / 32><<<dim3((unsigned)p.items, (unsigned)p.kv_ctas), 256, 0, s>>>(p);
+    p.kv_ctas = p.c.KVH;
+    kv_append_kernel<LPH, VPL, LPH <= 8 ? 1 : LPH / 8, 4><<<dim3((unsigned)p.items, (unsigned)p.kv_ctas), 256, 0, s>>>(p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !queries) return e;
     // about four units of 4 vectors a lane group

@@ -231,15 +231,15 @@ struct AppendParams {
     int* err;
 };
 
-// One warp: the run's rows of one head's K or V, NP passes of 32 / LPH rows (lane group i
-// the rows i, i + 32 / LPH, ...) held in registers. The block's new scale is known when
-// all rows have been seen; if they are more than the registers hold they are fetched
-// again for the codes.
-template <int LPH, int VPL, int NP>
+// The run's rows of one head's K or V by WPT warps (this one is number `part`, `top` a
+// word of theirs in shared memory, 0): NP passes of WPT * 32 / LPH rows in registers. The
+// block's new scale is known when all rows have been seen; if they are more than the
+// registers hold (WPT = 1) they are fetched again for the codes.
+template <int LPH, int VPL, int NP, int WPT>
 __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRun& run, int page, int head, bool is_k,
-                                            int lane) {
-    constexpr int RPW = 32 / LPH;                  // rows per pass
-    const int dh = p.c.dh, gl = lane % LPH, g = lane / LPH;
+                                            int lane, int part, unsigned* top) {
+    constexpr int RPW = 32 / LPH * WPT;            // rows per pass
+    const int dh = p.c.dh, gl = lane % LPH, g = part * (32 / LPH) + lane / LPH;
     const float* src = (is_k ? p.k : p.v) + (size_t)head * dh;
     const long long ld = is_k ? p.ldk : p.ldv;
     const bool rope = is_k && p.nr.table;
@@ -304,12 +304,17 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
                                  max(__float_as_uint(x[j][e].z) & 0x7fffffffu, __float_as_uint(x[j][e].w) & 0x7fffffffu)));
     }
     am = __reduce_max_sync(0xffffffffu, am);
+    if constexpr (WPT > 1) {
+        if (lane == 0) atomicMax(top, am);
+        __syncthreads();                           // also: every warp has read the old scale
+        am = *top;
+    }
     float now = am >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fdiv(__uint_as_float(am), 127.0f);
     if (!(now <= old)) {                           // grown (or NaN on either side)
         if (old != old) now = old;
         else if (now == now && o0 > 0) {           // older rows to the new scale
             const float ratio = fdiv(old, now);
-            for (int b = lane * 4; b < o0 * dh; b += 128) {
+            for (int b = (part * 32 + lane) * 4; b < o0 * dh; b += 128 * WPT) {
                 char4 w = *reinterpret_cast<char4*>(codes + b);
                 w.x = (signed char)__float2int_rn(fmul((float)w.x, ratio));
                 w.y = (signed char)__float2int_rn(fmul((float)w.y, ratio));
@@ -322,7 +327,7 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
         now = old;
     }
     __syncwarp();
-    if (lane == 0) *sp = now;
+    if (lane == 0 && part == 0) *sp = now;
     // x / now rounded to an integer: the quotient by the reciprocal and one correction is
     // the f32 division's (a scale whose reciprocal or remainders could leave f32's normal
     // range takes the division itself); adding 1.5 * 2^23 rounds it into the low byte
@@ -379,24 +384,31 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, const Bloc
     }
 }
 
-// Grid (runs, CTAs of a run): every warp finds the run; a warp of the first kv_ctas
-// takes one head's K or V of it, those of the others queries.
-// NP = 1: for calls of single rows. Few registers, so that a whole decode step is on the
-// SMs at once: it is bound by the latency of run -> page -> scale and older codes.
-template <int LPH, int VPL, int NP>
-__global__ void __launch_bounds__(256, VPL == 2 && NP > 1 ? 1 : NP == 1 && VPL == 1 ? 5 : 2) kv_append_kernel(const __grid_constant__ AppendParams p) {
+// Grid (runs, CTAs of a run): every warp finds the run; WPT warps of the first kv_ctas
+// take one head's K or V of it, those of the others queries.
+// WPT = 1, NP = 1: for calls of single rows. WPT = 4: up to 16 rows; with one warp holding
+// all of them (120 registers, 16 warps an SM) 6300 rows took 41 us. Few registers, so
+// that many runs are on the SMs at once: it is bound by the latency of run -> page ->
+// scale and older codes.
+template <int LPH, int VPL, int NP, int WPT>
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
+    __shared__ unsigned top[8 / WPT];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if constexpr (WPT > 1) {
+        if (threadIdx.x < 8 / WPT) top[threadIdx.x] = 0u;
+        __syncthreads();
+    }
     const BlockRun run = run_in_table(p, lane);
     if (run.s < 0 || run.n == 0) return;
     if ((int)blockIdx.y < p.kv_ctas) {
-        const int task = blockIdx.y * 8 + warp;
+        const int task = (blockIdx.y * 8 + warp) / WPT;        // (WPT = 4: two tasks a CTA, K and V of a head)
         if (task >= 2 * p.c.KVH) return;
         const int page = page_of(p.c, p.r, run.s, run.pos);
         if (page < 0) {
             if (lane == 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
             return;
         }
-        append_head<LPH, VPL, NP>(p, run, page, task >> 1, (task & 1) == 0, lane);
+        append_head<LPH, VPL, NP, WPT>(p, run, page, task >> 1, (task & 1) == 0, lane, warp % WPT, top + warp / WPT);
         return;
     }
     append_queries<LPH, VPL, 1>(p, run, ((blockIdx.y - p.kv_ctas) * 256 + threadIdx.x) / LPH,
