@@ -117,19 +117,19 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
     return cudaGetLastError();
 }
 
-// Which kernel, and the keys per split.
-//  few rows (up to 16 columns (token, head) of a KV head in the longest sequence, or on
-//  average if the caller does not say): 8 columns a CTA. Small splits fill the GPU when
-//  there are few rows; with long caches larger ones bound the partial results and their
-//  joining. A function of the capacity alone, so that a sequence's result does not
-//  depend on the others in the call.
-//  more: 64 rows a CTA; keys are split only while there are too few tiles for two
-//  rounds of the GPU.
-bool attn_plan(PagedAttnParams& p, int max_rows) {
+// Columns (token, head) of a KV head that a CTA takes, which says the kernel, and the
+// keys per split.
+//  up to 16 columns in the longest sequence (on average if the caller does not say): 8, or
+//  2 where there are not more. Small splits fill the GPU when there are few rows; with
+//  long caches larger ones bound the partial results and their joining. A function of
+//  the capacity alone, so that a sequence's result does not depend on the others in
+//  the call.
+//  more: 64; keys are split only while there are too few tiles for two rounds of the GPU.
+int attn_plan(PagedAttnParams& p, int max_rows) {
     const int G = p.H / p.c.KVH;
     const long long cols = (max_rows > 0 ? max_rows : (p.r.n_rows + p.r.n_seq - 1) / std::max(p.r.n_seq, 1)) * (long long)G;
-    const bool few = cols <= 16;
-    if (few) {
+    const int tile = cols <= 2 ? 2 : cols <= 16 ? kSplitCols : kTileRows;
+    if (tile != kTileRows) {
         p.kc_log2 = p.r.cap <= 4096 ? 8 : 9;
     } else {
         const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / kTileRows), want = 2 * 148 * 3;
@@ -138,7 +138,7 @@ bool attn_plan(PagedAttnParams& p, int max_rows) {
         while (p.kc_log2 < 30 && ((long long)splits << p.kc_log2) < p.r.cap) ++p.kc_log2;
     }
     p.nsplit = std::max(1, (int)((p.r.cap + (1ll << p.kc_log2) - 1) >> p.kc_log2));
-    return few;
+    return tile;
 }
 
 size_t part_bytes(const PagedAttnParams& p) {
@@ -171,22 +171,22 @@ cudaError_t launch_attn_tile(const PagedAttnParams& p, cudaStream_t s) {
     return launch_join(p, s);
 }
 
-template <int DP>
+template <int DP, int NC>
 cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
-    using Sh = SplitShape<DP>;
-    auto k = paged_attn_split_kernel<DP>;
+    using Sh = SplitShape<DP, NC>;
+    auto k = paged_attn_split_kernel<DP, NC>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
     if (e != cudaSuccess) return e;
     // tiles over all sequences: at most one partly filled one each
-    const long long tiles = ((long long)p.r.n_rows * p.G / kSplitCols + p.r.n_seq) * p.c.KVH;
+    const long long tiles = ((long long)p.r.n_rows * p.G / NC + p.r.n_seq) * p.c.KVH;
     const long long most = tiles * p.nsplit, resident = (long long)sm_count() * (DP == 256 ? 2 : DP == 128 ? 3 : 4);
     k<<<(unsigned)(most < resident ? most : resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
     return launch_join(p, s);
 }
 
 template <int DP>
-cudaError_t launch_attn(const PagedAttnParams& p, bool few, cudaStream_t s) {
-    return few ? launch_attn_split<DP>(p, s) : launch_attn_tile<DP>(p, s);
+cudaError_t launch_attn(const PagedAttnParams& p, int cols, cudaStream_t s) {
+    return cols == 2 ? launch_attn_split<DP, 2>(p, s) : cols == 8 ? launch_attn_split<DP, 8>(p, s) : launch_attn_tile<DP>(p, s);
 }
 
 }  // namespace
@@ -299,16 +299,16 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     if (q == out) return refuse(fn, "out must not be q");
     if ((int64_t)p.r.n_rows * n_heads > (1ll << 30)) return refuse(fn, "more than 2^30 (row, head) pairs");
     p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.G = n_heads / kv->n_kv_heads; p.err = err;
-    const bool few = attn_plan(p, rows->max_rows);
-    const long long items = ((long long)p.r.n_rows * p.G / (few ? kSplitCols : kTileRows) + p.r.n_seq) * p.c.KVH * p.nsplit;
+    const int cols = attn_plan(p, rows->max_rows);
+    const long long items = ((long long)p.r.n_rows * p.G / cols + p.r.n_seq) * p.c.KVH * p.nsplit;
     if (items >= kMaxItems) return refuse(fn, "too many (row, head, split) pieces for one call: use fewer rows");
     const size_t need = part_bytes(p);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
     p.part = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return status(fn, kv->d_head <= 64 ? launch_attn<64>(p, few, s)
-                      : kv->d_head <= 128 ? launch_attn<128>(p, few, s) : launch_attn<256>(p, few, s));
+    return status(fn, kv->d_head <= 64 ? launch_attn<64>(p, cols, s)
+                      : kv->d_head <= 128 ? launch_attn<128>(p, cols, s) : launch_attn<256>(p, cols, s));
 }
 
 }  // extern "C"

@@ -715,14 +715,19 @@ constexpr int kSplitWarps = 4;
 constexpr int kSplitCols = 8;
 constexpr int kSplitMaxKeys = 512;                 // keys per split at most: a block a lane
 
-template <int DP>
+// NC columns an item: 8, or 2 for calls of one or two columns a KV head (decode without
+// shared heads). Then the digits are the MMA's columns instead: A = codes (16 keys x d,
+// 16 elements x keys), column 4 c + e = digit e of head column c, and every digit column
+// keeps its own f32 output until the end: a quarter of the MMAs and half of the folding.
+template <int DP, int NC>
 struct SplitShape {
     static constexpr int NH = DP / 64;             // 64-byte parts of a key row
     static constexpr int VW = DP / 32;             // 32-bit words of a value row that a lane holds
     static constexpr int NT = DP / 8;              // output tiles of 8 elements
-    static constexpr int QBytes = NH * 3 * 32 * 16;                        // A fragments [part][hi, hi, lo][lane]
-    static constexpr int MergeBytes = kSplitWarps * kSplitCols * (DP + 4) * 4;
-    static constexpr int Smem = 2 * (QBytes + 32 + MergeBytes);
+    static constexpr int QBytes = NH * (NC == 8 ? 3 : 1) * 32 * 16;        // A fragments [part][hi, hi, lo][lane]; B [part][lane]
+    static constexpr int WBytes = NC == 8 ? 0 : kSplitWarps * 2 * 32 * 4;  // narrow: a step's weights [warp][column][key]
+    static constexpr int MergeBytes = kSplitWarps * NC * (DP + 4) * 4;
+    static constexpr int Smem = 2 * (QBytes + 32 + MergeBytes) + WBytes;
 };
 
 struct SplitItem {
@@ -733,14 +738,15 @@ struct SplitItem {
 };
 
 // the CTA's next item from number `item` on (stride gridDim.x) that has keys to look at
+template <int NC>
 __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, unsigned& item, int lane) {
     SplitItem w;
     for (;; item += gridDim.x) {
-        w.it = find_item<kSplitCols>(p, item, lane);
+        w.it = find_item<NC>(p, item, lane);
         w.cell = -2;
         if (w.it.s < 0) return w;
-        w.col0 = w.it.tile * kSplitCols;
-        w.cols = min(w.it.len * p.G - w.col0, kSplitCols);
+        w.col0 = w.it.tile * NC;
+        w.cols = min(w.it.len * p.G - w.col0, NC);
         const int last = w.it.len == 1 ? 0 : (w.col0 + w.cols - 1) / p.G;  // the tile's last token
         w.n = min(w.it.kv - w.it.len + last + 1, p.r.cap);
         w.j0 = w.it.split << p.kc_log2;
@@ -758,19 +764,21 @@ __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, u
     return w;
 }
 
-template <int DP>
+template <int DP, int NC>
 __global__ void __launch_bounds__(kSplitWarps * 32, DP == 256 ? 2 : DP == 128 ? 3 : 4)
 paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
-    using Sh = SplitShape<DP>;
+    using Sh = SplitShape<DP, NC>;
+    constexpr bool kNarrow = NC == 2;
     extern __shared__ __align__(16) unsigned char ps_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int dh = p.c.dh;
     unsigned item = blockIdx.x;
-    SplitItem cur = next_split_item(p, item, lane);
+    SplitItem cur = next_split_item<NC>(p, item, lane);
     if (cur.it.s < 0) return;
 
     uint4 kf[4][Sh::NH];                                                   // a step's keys 8 x + g
-    uint32_t vf[2][4][Sh::VW];                                             // its values: [block][key 2t + {0, 1, 8, 9}][words]
+    uint32_t vf[2][4][Sh::VW];                                             // its values: [block][key][words], keys 2t + {0, 1, 8, 9},
+                                                                           // narrow 4t + {0, 1, 2, 3}
     // Blocks that are not there and elements past dh are read from the pool's first block and
     // row: they meet masked weights and zero digits, or make elements that are not stored.
     int kd[Sh::NH], vd[(Sh::VW + 3) / 4];                                  // element offsets inside a row
@@ -791,10 +799,10 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         c0 = max(c0, 0); c1 = max(c1, 0);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const int8_t* vr = p.c.v + ((long long)(b ? c1 : c0) * kKvBlock + 2 * t) * dh;
+            const int8_t* vr = p.c.v + ((long long)(b ? c1 : c0) * kKvBlock + (kNarrow ? 4 : 2) * t) * dh;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int8_t* v = vr + ((i & 1) + 8 * (i >> 1)) * dh;
+                const int8_t* v = vr + (kNarrow ? i : (i & 1) + 8 * (i >> 1)) * dh;
                 if constexpr (Sh::VW == 2) {
                     const uint2 x = __ldg(reinterpret_cast<const uint2*>(v + vd[0]));
                     vf[b][i][0] = x.x; vf[b][i][1] = x.y;
@@ -808,14 +816,19 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             }
         }
     };
-    // an item's queries as A fragments in half `b` of the shared memory; 16 lanes a column
+    // an item's queries as fragments in half `b` of the shared memory; 16 lanes a column
     auto put_queries = [&](const SplitItem& w, int b) {
+        if (tid >= 16 * NC) return;                                        // (whole warps)
         unsigned char* qd = ps_raw + b * (Sh::QBytes + 32);
         const int col = tid >> 4, cc = w.col0 + col, tok = w.it.len == 1 ? 0 : cc / p.G;
         query_digits<DP>(p.q + (size_t)(w.it.a + tok) * p.ldq + (size_t)(w.it.kvh * p.G + cc - tok * p.G) * dh, col < w.cols, dh,
                          tid & 15, [&](int e, int d, uint32_t x) {
                              // words of the part's 16-byte unit: x, y make step 0, z, w step 1
                              const int h = d >> 6, q = (d >> 4) & 3, word = (d >> 2) & 3;
+                             if constexpr (kNarrow) {
+                                 *reinterpret_cast<uint32_t*>(qd + (h * 32 + 4 * (4 * col + e) + q) * 16 + 4 * word) = x;
+                                 return;
+                             }
                              const int frag = e ? word >> 1 : 2, reg = e ? 2 * (word & 1) + 2 - e : 2 * (word & 1) + (word >> 1);
                              *reinterpret_cast<uint32_t*>(qd + ((h * 3 + frag) * 32 + 4 * col + q) * 16 + 4 * reg) = x;
                          }, reinterpret_cast<float*>(qd + Sh::QBytes) + col);
@@ -824,21 +837,32 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     int a0 = __shfl_sync(0xffffffffu, cur.cell, 2 * warp), a1 = __shfl_sync(0xffffffffu, cur.cell, 2 * warp + 1);
     load_keys(a0, a1);
     load_values(a0, a1);
+    if constexpr (kNarrow)                                                 // columns 3 and 7 stay zero
+        for (int i = tid; i < Sh::NH * 64; i += kSplitWarps * 32)
+            *reinterpret_cast<uint32_t*>(ps_raw + (i & 1) * (Sh::QBytes + 32) + ((i >> 6) * 32 + 16 * ((i >> 5) & 1) + 12) * 16 +
+                                         4 * ((i >> 1) & 15)) = 0u;
     put_queries(cur, 0);
     __syncthreads();
     for (int buf = 0;; buf ^= 1) {
         const unsigned char* qd = ps_raw + buf * (Sh::QBytes + 32);
-        const float sqg = reinterpret_cast<const float*>(qd + Sh::QBytes)[g];   // unit of column g's scores
+        const int col = kNarrow ? t >> 1 : g;                              // the column of this lane's scores
+        const float sqg = reinterpret_cast<const float*>(qd + Sh::QBytes)[col];   // their unit
         const int pos0 = cur.it.kv - cur.it.len;
-        const int lim = g < cur.cols ? min(pos0 + (cur.it.len == 1 ? 0 : (cur.col0 + g) / p.G) + 1, cur.n) : 0;   // keys it sees
+        const int lim = col < cur.cols ? min(pos0 + (cur.it.len == 1 ? 0 : (cur.col0 + col) / p.G) + 1, cur.n) : 0;   // keys it sees
         // up to here no column needs a mask (idle columns have zero digits and no output)
-        const int whole_end = __reduce_min_sync(0xffffffffu, g < cur.cols ? lim : cur.n);
+        const int whole_end = __reduce_min_sync(0xffffffffu, col < cur.cols ? lim : cur.n);
+        uint4 qb[Sh::NH];                                                  // narrow: the B fragments of column g's digit
+        if constexpr (kNarrow)
+#pragma unroll
+            for (int h = 0; h < Sh::NH; ++h) qb[h] = reinterpret_cast<const uint4*>(qd)[h * 32 + lane];
         item += gridDim.x;
-        SplitItem nxt = next_split_item(p, item, lane);
+        SplitItem nxt = next_split_item<NC>(p, item, lane);
 
         float m = -INFINITY;
         f32x2 l2 = 0ull;                                                   // this lane's part of the sum
-        f32x2 o[Sh::NT];                                                   // tile x: elements (DP/4) t + x, + DP/8 of column g
+        // wide: tile x: elements (DP/4) t + x, + DP/8 of column g; narrow: element (DP/8) g + x
+        // of digit columns 2t, 2t + 1
+        f32x2 o[Sh::NT];
 #pragma unroll
         for (int x = 0; x < Sh::NT; ++x) o[x] = 0ull;
 
@@ -852,9 +876,27 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             const int na0 = __shfl_sync(0xffffffffu, ncell, nblk), na1 = __shfl_sync(0xffffffffu, ncell, nblk + 1);
             const float k0 = __shfl_sync(0xffffffffu, cur.ks, blk), k1 = __shfl_sync(0xffffffffu, cur.ks, blk + 1);
             const float v0 = __shfl_sync(0xffffffffu, cur.vs, blk), v1 = __shfl_sync(0xffffffffu, cur.vs, blk + 1);
-            // scores (base 2) of keys 8 x + 2t, + 1 for column g
-            float2 s[4];
-            {
+            // scores (base 2): keys 8 x + 2t, + 1 for column g; narrow: keys 16 x + g, + 8 for column t / 2
+            constexpr int NS = kNarrow ? 2 : 4;
+            float2 s[NS];
+            if constexpr (kNarrow) {
+                const float up = t & 1 ? 65536.0f : 1.0f;                  // odd lanes have digit 2, even ones 0 and 1
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    int c[4];
+#pragma unroll
+                    for (int h = 0; h < Sh::NH; ++h) {
+                        const uint4 k0 = kf[2 * x][h], k8 = kf[2 * x + 1][h];
+                        if (h == 0) mma_s8_first(c, k0.x, k8.x, k0.y, k8.y, qb[h].x, qb[h].y);
+                        else mma_s8(c, k0.x, k8.x, k0.y, k8.y, qb[h].x, qb[h].y);
+                        mma_s8(c, k0.z, k8.z, k0.w, k8.w, qb[h].z, qb[h].w);
+                    }
+                    const float u = sqg * (x ? k1 : k0) * up;
+                    s[x] = unpack2(mul2(pack2((float)(c[1] * 256 + c[0]), (float)(c[3] * 256 + c[2])), pack2(u, u)));
+                    s[x].x += __shfl_xor_sync(0xffffffffu, s[x].x, 1);
+                    s[x].y += __shfl_xor_sync(0xffffffffu, s[x].y, 1);
+                }
+            } else {
                 int hi[4][4], lo[4][2][4];                                 // hi: digit 2 in 0, 1 and digit 1 in 2, 3
 #pragma unroll
                 for (int h = 0; h < Sh::NH; ++h) {
@@ -885,27 +927,37 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             const bool whole = j + 32 <= whole_end && (a0 | a1) >= 0 && v0 + v1 == v0 + v1;
             if (!whole) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int key = j + 8 * x + 2 * t, lx = (x < 2 ? a0 : a1) >= 0 ? lim : 0;
+                for (int x = 0; x < NS; ++x) {
+                    const int key = kNarrow ? j + 16 * x + g : j + 8 * x + 2 * t, lx = (x < NS / 2 ? a0 : a1) >= 0 ? lim : 0;
                     if (key >= lx) s[x].x = -INFINITY;
-                    if (key + 1 >= lx) s[x].y = -INFINITY;
+                    if (key + (kNarrow ? 8 : 1) >= lx) s[x].y = -INFINITY;
                 }
             }
+            // over the lanes that hold a column's keys
+            auto lanes_max = [](float v) {
+                if constexpr (kNarrow) {
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                } else {
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                }
+            };
             float mx = m;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) mx = fmaxf(mx, fmaxf(s[x].x, s[x].y));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            for (int x = 0; x < NS; ++x) mx = fmaxf(mx, fmaxf(s[x].x, s[x].y));
+            mx = lanes_max(mx);
             const float base = mx == -INFINITY ? 0.0f : mx;
             const float back = exp2_fast(m - base);
             m = mx;
             f32x2 ls = 0ull;
-            float2 e[4];
+            float2 e[NS];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < NS; ++x) {
                 e[x] = make_float2(exp2_fast(s[x].x - base), exp2_fast(s[x].y - base));
                 ls = add2(ls, pack2(e[x].x, e[x].y));
-                const float sv = x < 2 ? v0 : v1;
+                const float sv = x < NS / 2 ? v0 : v1;
                 e[x] = unpack2(mul2(pack2(e[x].x, e[x].y), pack2(sv, sv)));
             }
             l2 = fma2(l2, pack2(back, back), ls);
@@ -914,7 +966,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             bool bad = false;
             if (!whole) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
+                for (int x = 0; x < NS; ++x) {
                     if (s[x].x == -INFINITY) e[x].x = 0.0f;
                     if (s[x].y == -INFINITY) e[x].y = 0.0f;
                     bad |= e[x].x != e[x].x || e[x].y != e[x].y;
@@ -922,41 +974,85 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             }
             float wt = bad ? INFINITY : 0.0f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) wt = fmaxf(wt, fmaxf(e[x].x, e[x].y));
-            wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, 1));
-            wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, 2));
+            for (int x = 0; x < NS; ++x) wt = fmaxf(wt, fmaxf(e[x].x, e[x].y));
+            wt = lanes_max(wt);
             const float f = weight_factor(wt), u = wt < INFINITY ? weight_unit(f) : __int_as_float(0x7fffffff);
-            uint32_t wd[2][3];                                             // digits of a block's four weights
+            if constexpr (kNarrow) {
+                // weights to the lanes of their digit: column g = 4 c + e takes digit e of column
+                // c's keys 4t .. 4t + 3 of each block
+                uint32_t* wx = reinterpret_cast<uint32_t*>(ps_raw + 2 * (Sh::QBytes + 32 + Sh::MergeBytes)) + warp * 64;
+                __syncwarp();
+                if (!(t & 1)) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-                digits4(digit_bits_pos(e[2 * b].x, f), digit_bits_pos(e[2 * b].y, f), digit_bits_pos(e[2 * b + 1].x, f),
-                        digit_bits_pos(e[2 * b + 1].y, f), wd[b]);
-            // A registers of their own, so that no MMA has to gather them (rows 8 to 15 of the
-            // second one are not used)
-            uint32_t wh[4], wl[4];
-            own_quad(wh, p.zero, wd[0][2], wd[0][1], wd[1][2], wd[1][1]);
-            own_quad(wl, p.zero, wd[0][0], wd[0][0], wd[1][0], wd[1][0]);
-            // output: column n of tile x is element (DP/8) n + x: four keys' bytes of one
-            // element make one B register
-#pragma unroll
-            for (int w = 0; w < Sh::VW; ++w) {
-                uint32_t a[2][4];
+                    for (int x = 0; x < 2; ++x) {
+                        wx[32 * col + 16 * x + g] = digit_bits_pos(e[x].x, f);
+                        wx[32 * col + 16 * x + 8 + g] = digit_bits_pos(e[x].y, f);
+                    }
+                }
+                __syncwarp();
+                const int dig = g & 3;
+                const uint32_t sel = (uint32_t)dig | ((uint32_t)(4 + dig) << 4), flip = dig < 2 ? 0x80808080u : 0u, keep = dig < 3 ? ~0u : 0u;
+                uint32_t wb[2];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const uint32_t x = __byte_perm(vf[b][0][w], vf[b][1][w], 0x5140), y = __byte_perm(vf[b][2][w], vf[b][3][w], 0x5140);
-                    const uint32_t z = __byte_perm(vf[b][0][w], vf[b][1][w], 0x7362), v = __byte_perm(vf[b][2][w], vf[b][3][w], 0x7362);
-                    a[b][0] = __byte_perm(x, y, 0x5410); a[b][1] = __byte_perm(x, y, 0x7632);
-                    a[b][2] = __byte_perm(z, v, 0x5410); a[b][3] = __byte_perm(z, v, 0x7632);
+                    const uint4 y = *reinterpret_cast<const uint4*>(wx + 32 * (g >> 2) + 16 * b + 4 * t);
+                    wb[b] = (__byte_perm(__byte_perm(y.x, y.y, sel), __byte_perm(y.z, y.w, sel), 0x5410) ^ flip) & keep;
                 }
-                int hi[4][4], lo[4][4];
+                // output: row g of tile x is element (DP/8) g + 2 x, row g + 8 the next: four keys'
+                // bytes of one element make one A register
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wh[0], wh[1], wh[2], wh[3], a[0][k], a[1][k]);
+                for (int w = 0; w < Sh::VW; ++w) {
+                    uint32_t a[2][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wl[0], wl[1], wl[2], wl[3], a[0][k], a[1][k]);
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t x = __byte_perm(vf[b][0][w], vf[b][1][w], 0x5140), y = __byte_perm(vf[b][2][w], vf[b][3][w], 0x5140);
+                        const uint32_t z = __byte_perm(vf[b][0][w], vf[b][1][w], 0x7362), v = __byte_perm(vf[b][2][w], vf[b][3][w], 0x7362);
+                        a[b][0] = __byte_perm(x, y, 0x5410); a[b][1] = __byte_perm(x, y, 0x7632);
+                        a[b][2] = __byte_perm(z, v, 0x5410); a[b][3] = __byte_perm(z, v, 0x7632);
+                    }
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    o[4 * w + k] = fma2(join_digits(hi[k][0], hi[k][1], hi[k][2], hi[k][3], lo[k][0], lo[k][1]), pack2(u, u),
-                                        mul2(o[4 * w + k], pack2(back, back)));
+                    for (int k = 0; k < 2; ++k) {
+                        int c[4];
+                        mma_s8_first(c, a[0][2 * k], a[0][2 * k + 1], a[1][2 * k], a[1][2 * k + 1], wb[0], wb[1]);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            o[4 * w + 2 * k + r] = fma2(pack2((float)c[2 * r], (float)c[2 * r + 1]), pack2(u, u),
+                                                        mul2(o[4 * w + 2 * k + r], pack2(back, back)));
+                    }
+                }
+            } else {
+                uint32_t wd[2][3];                                             // digits of a block's four weights
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    digits4(digit_bits_pos(e[2 * b].x, f), digit_bits_pos(e[2 * b].y, f), digit_bits_pos(e[2 * b + 1].x, f),
+                            digit_bits_pos(e[2 * b + 1].y, f), wd[b]);
+                // A registers of their own, so that no MMA has to gather them (rows 8 to 15 of the
+                // second one are not used)
+                uint32_t wh[4], wl[4];
+                own_quad(wh, p.zero, wd[0][2], wd[0][1], wd[1][2], wd[1][1]);
+                own_quad(wl, p.zero, wd[0][0], wd[0][0], wd[1][0], wd[1][0]);
+                // output: column n of tile x is element (DP/8) n + x: four keys' bytes of one
+                // element make one B register
+#pragma unroll
+                for (int w = 0; w < Sh::VW; ++w) {
+                    uint32_t a[2][4];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t x = __byte_perm(vf[b][0][w], vf[b][1][w], 0x5140), y = __byte_perm(vf[b][2][w], vf[b][3][w], 0x5140);
+                        const uint32_t z = __byte_perm(vf[b][0][w], vf[b][1][w], 0x7362), v = __byte_perm(vf[b][2][w], vf[b][3][w], 0x7362);
+                        a[b][0] = __byte_perm(x, y, 0x5410); a[b][1] = __byte_perm(x, y, 0x7632);
+                        a[b][2] = __byte_perm(z, v, 0x5410); a[b][3] = __byte_perm(z, v, 0x7632);
+                    }
+                    int hi[4][4], lo[4][4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wh[0], wh[1], wh[2], wh[3], a[0][k], a[1][k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wl[0], wl[1], wl[2], wl[3], a[0][k], a[1][k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        o[4 * w + k] = fma2(join_digits(hi[k][0], hi[k][1], hi[k][2], hi[k][3], lo[k][0], lo[k][1]), pack2(u, u),
+                                            mul2(o[4 * w + k], pack2(back, back)));
+                }
             }
             load_values(na0, na1);
             a0 = na0; a1 = na1;
@@ -965,10 +1061,24 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         // this warp's columns: sum over the lanes of a column, then all to shared memory
         float* mo = reinterpret_cast<float*>(ps_raw + 2 * (Sh::QBytes + 32) + buf * Sh::MergeBytes);   // [4][8][DP + 4]
         float l = unpack2(l2).x + unpack2(l2).y;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        float* ow = mo + (warp * kSplitCols + g) * (DP + 4);
-        if (g < cur.cols) {
+        float* ow = mo + (warp * NC + col) * (DP + 4);
+        if constexpr (kNarrow) {
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+            float v[Sh::NT];                                               // the digits together
+#pragma unroll
+            for (int x = 0; x < Sh::NT; ++x) {
+                const float2 c = unpack2(o[x]);
+                v[x] = t & 1 ? c.x * 65536.0f : ffma(c.y, 256.0f, c.x);
+                v[x] += __shfl_xor_sync(0xffffffffu, v[x], 1);
+            }
+            if (!(t & 1) && col < cur.cols) {
+                if (g == 0) { ow[DP] = m; ow[DP + 1] = l; }
+#pragma unroll
+                for (int x = 0; x < Sh::NT; x += 4)
+                    *reinterpret_cast<float4*>(ow + (DP / 8) * g + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+            }
+        } else if (l += __shfl_xor_sync(0xffffffffu, l, 1), l += __shfl_xor_sync(0xffffffffu, l, 2); col < cur.cols) {
             if (t == 0) { ow[DP] = m; ow[DP + 1] = l; }
 #pragma unroll
             for (int x = 0; x < Sh::NT; x += 4) {
@@ -984,7 +1094,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             const int splits = row_splits(p, pos0 + tok);
             if (d >= dh || cur.it.split >= splits) continue;
             const float* mc = mo + col * (DP + 4);
-            constexpr int W = kSplitCols * (DP + 4);
+            constexpr int W = NC * (DP + 4);
             float M = -INFINITY, L = 0.0f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
