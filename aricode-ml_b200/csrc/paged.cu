@@ -130,7 +130,7 @@ int attn_plan(PagedAttnParams& p, int max_rows) {
     const long long cols = (max_rows > 0 ? max_rows : (p.r.n_rows + p.r.n_seq - 1) / std::max(p.r.n_seq, 1)) * (long long)G;
     const int tile = cols <= 2 ? 2 : cols <= 16 ? kSplitCols : kTileRows;
     if (tile != kTileRows) {
-        p.kc_log2 = p.r.cap <= 4096 ? 8 : 9;
+        p.kc_log2 = p.r.cap <= 1024 ? 8 : 9;
     } else {
         const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / kTileRows), want = 2 * 148 * 3;
         const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));

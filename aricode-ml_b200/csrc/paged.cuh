@@ -818,9 +818,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     };
     // an item's queries as fragments in half `b` of the shared memory; 16 lanes a column
     auto put_queries = [&](const SplitItem& w, int b) {
-        if (tid >= 16 * NC) return;                                        // (whole warps)
+        if (kNarrow && warp != kSplitWarps - 1) return;                    // two columns: the last warp's lanes
         unsigned char* qd = ps_raw + b * (Sh::QBytes + 32);
-        const int col = tid >> 4, cc = w.col0 + col, tok = w.it.len == 1 ? 0 : cc / p.G;
+        const int col = kNarrow ? lane >> 4 : tid >> 4, cc = w.col0 + col, tok = w.it.len == 1 ? 0 : cc / p.G;
         query_digits<DP>(p.q + (size_t)(w.it.a + tok) * p.ldq + (size_t)(w.it.kvh * p.G + cc - tok * p.G) * dh, col < w.cols, dh,
                          tid & 15, [&](int e, int d, uint32_t x) {
                              // words of the part's 16-byte unit: x, y make step 0, z, w step 1
@@ -857,6 +857,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             for (int h = 0; h < Sh::NH; ++h) qb[h] = reinterpret_cast<const uint4*>(qd)[h * 32 + lane];
         item += gridDim.x;
         SplitItem nxt = next_split_item<NC>(p, item, lane);
+        if (kNarrow && nxt.it.s >= 0) put_queries(nxt, buf ^ 1);           // (its last readers are past their barrier)
 
         float m = -INFINITY;
         f32x2 l2 = 0ull;                                                   // this lane's part of the sum
@@ -1087,8 +1088,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 *reinterpret_cast<float4*>(ow + (DP / 4) * t + DP / 8 + x) = make_float4(a.y, b.y, c.y, d.y);
             }
         }
-        if (nxt.it.s >= 0) put_queries(nxt, buf ^ 1);
+        if (!kNarrow && nxt.it.s >= 0) put_queries(nxt, buf ^ 1);
         __syncthreads();
+        // (narrow: not by the warp that also has the next queries to fetch)
         for (int i = tid; i < cur.cols * (DP / 4); i += kSplitWarps * 32) {
             const int col = i / (DP / 4), d = 4 * (i % (DP / 4)), cc = cur.col0 + col, tok = cur.it.len == 1 ? 0 : cc / p.G;
             const int splits = row_splits(p, pos0 + tok);
