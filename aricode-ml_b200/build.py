@@ -22,7 +22,7 @@ OBJ = CSRC / "_obj"
 LIB = PKG / "libb2dec.so"
 FRONT = PKG / "b2run"                    # stdin-tokens front end (host program over the library)
 SOURCES = ["runtime.cu", "launch.cu", "token.cu", "prefill.cu", "capi.cu", "noalloc.cu", "paged.cu"]
-HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "json.h"]
+HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "umma.cuh", "json.h"]
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",

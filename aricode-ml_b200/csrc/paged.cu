@@ -128,11 +128,11 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
 int attn_plan(PagedAttnParams& p, int max_rows) {
     const int G = p.H / p.c.KVH;
     const long long cols = (max_rows > 0 ? max_rows : (p.r.n_rows + p.r.n_seq - 1) / std::max(p.r.n_seq, 1)) * (long long)G;
-    const int tile = cols <= 2 ? 2 : cols <= 16 ? kSplitCols : kTileRows;
-    if (tile != kTileRows) {
+    const int tile = cols <= 2 ? 2 : cols <= 16 ? kSplitCols : p.c.dh <= 128 ? kMmaRows : kTileRows;
+    if (cols <= 16) {
         p.kc_log2 = p.r.cap <= 1024 ? 8 : 9;
     } else {
-        const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / kTileRows), want = 2 * 148 * 3;
+        const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / tile), want = tile == kMmaRows ? 4 * 148 : 6 * 148;
         const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
         p.kc_log2 = 8;
         while (p.kc_log2 < 30 && ((long long)splits << p.kc_log2) < p.r.cap) ++p.kc_log2;
@@ -158,6 +158,14 @@ cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
     if (p.nsplit <= 8)
         return launch_ex(paged_attn_join_kernel<1>, dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
     return launch_ex(paged_attn_join_kernel<8>, dim3((unsigned)p.r.n_rows, (unsigned)p.H), dim3(256), 0, s, true, p);
+}
+
+cudaError_t launch_attn_mma(const PagedAttnParams& p, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(paged_attn_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaSmem::Alloc);
+    if (e != cudaSuccess) return e;
+    const long long most = ((long long)p.r.n_rows * p.G / kMmaRows + p.r.n_seq) * p.c.KVH * p.nsplit;
+    paged_attn_mma_kernel<<<(unsigned)most, kMmaThreads, MmaSmem::Alloc, s>>>(p);
+    return launch_join(p, s);
 }
 
 template <int DP>
@@ -186,7 +194,8 @@ cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
 
 template <int DP>
 cudaError_t launch_attn(const PagedAttnParams& p, int cols, cudaStream_t s) {
-    return cols == 2 ? launch_attn_split<DP, 2>(p, s) : cols == 8 ? launch_attn_split<DP, 8>(p, s) : launch_attn_tile<DP>(p, s);
+    return cols == 2 ? launch_attn_split<DP, 2>(p, s) : cols == 8 ? launch_attn_split<DP, 8>(p, s)
+           : cols == kMmaRows ? launch_attn_mma(p, s) : launch_attn_tile<DP>(p, s);
 }
 
 }  // namespace

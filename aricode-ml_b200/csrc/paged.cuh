@@ -9,6 +9,7 @@
 // ones); every value is checked before it becomes an address.
 #pragma once
 #include "kernels.cuh"
+#include "umma.cuh"
 
 namespace b2 {
 
@@ -1477,6 +1478,426 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
         }
         if (splits > 1 && t == 0) { dst[dh] = r ? m1 : m0; dst[dh + 1] = L; }
     }
+}
+
+// ---- many rows per sequence, d_head up to 128: the 5th-generation tensor cores. A CTA
+// takes 128 rows against a split of the keys in tiles of 128.
+//   S = Q K^T, O = W V, each three MMA chains (tcgen05 kind::i8, one per digit) of
+//   128 x 128 x d_head (x 128 keys) into one TMEM region of 3 x 128 columns, which S and O
+//   take in turn: scores of tile i | output of tile i - 1 | scores of tile i + 1 | ...
+//   (a second region does not fit: 512 columns.) A pass of MMAs runs while the softmax
+//   warps work on what they have read before it, so that the matrix unit is never
+//   waited for long; what bounds the kernel is what the softmax warps issue.
+// Warps 0 .. 15, softmax: warp w reads TMEM lanes 32 (w % 4) .. + 31, a row a thread, and
+//   set w / 4 has keys 32 (w / 4) .. + 31 of the tile and elements 32 (w / 4) .. + 31 of the
+//   output: no shuffles; a row's four threads exchange (maximum, largest weight) through
+//   shared memory, a barrier of 128 threads.
+// Warps 16 .. 18, copies: keys by cp.async, values turned to [element][key] by byte
+//   permutes, both in the 128-byte-swizzled K-major layout, two buffers each; scales.
+// Warp 19: issues the MMAs. (20 warps: 96 registers a thread; 21 would leave 80.)
+// Every wait is bounded; a warp whose wait ran out goes on without waiting (its barriers
+// still meet), sets the error word and the outputs are garbage.
+constexpr int kMmaRows = 128;
+constexpr int kMmaKeys = 128;
+constexpr int kMmaSoftWarps = 16;
+constexpr int kMmaCopyWarps = 3;
+constexpr int kMmaThreads = (kMmaSoftWarps + kMmaCopyWarps + 1) * 32;
+
+struct MmaSmem {
+    static constexpr int Tile = 128 * 128;                     // one 128 x 128-byte operand
+    static constexpr int Q = 0;                                // [3 digits]
+    static constexpr int P = Q + 3 * Tile;                     // [2 tiles][3 digits] weights
+    static constexpr int K = P + 6 * Tile;                     // [2]
+    static constexpr int V = K + 2 * Tile;                     // [2]
+    static constexpr int Xm = V + 2 * Tile;                    // [2][4 sets][128 rows] (maximum, largest weight)
+    static constexpr int Sc = Xm + 2 * 4 * 128 * 8;            // [4 tiles][3][8]: key scales, value scales, 1 where there
+    static constexpr int Sq = Sc + 4 * 24 * 4;                 // [128] units of the rows' scores
+    static constexpr int Bars = Sq + 128 * 4;                  // 15 barriers, TMEM address, fail
+    static constexpr int Bytes = Bars + 16 * 8 + 16;
+    static constexpr int Alloc = Bytes + 1024;                 // operands start on 1024 bytes
+};
+
+static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(const __grid_constant__ PagedAttnParams p) {
+    using Sm = MmaSmem;
+    extern __shared__ unsigned char pm_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pm_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + Sm::Bars);      // [2] copies -> MMA
+    uint64_t* kempty = kfull + 2;                                      // [2] MMA -> copies
+    uint64_t* vfull = kempty + 2;                                      // [2]
+    uint64_t* vempty = vfull + 2;                                      // [2]
+    uint64_t* sfull = vempty + 2;                                      // scores in TMEM
+    uint64_t* sfree = sfull + 1;                                       // scores read
+    uint64_t* pfull = sfree + 1;                                       // [2] weights written
+    uint64_t* ofull = pfull + 2;                                       // output sums in TMEM
+    uint64_t* ofree = ofull + 1;                                       // output sums read
+    uint64_t* done = ofree + 1;                                        // every MMA complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float2* xm = reinterpret_cast<float2*>(sm + Sm::Xm);
+    float* sc = reinterpret_cast<float*>(sm + Sm::Sc);
+    float* sq = reinterpret_cast<float*>(sm + Sm::Sq);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int dh = p.c.dh, psz = 1 << p.c.page_log2;
+
+    const AttnItem it = find_item<kMmaRows>(p, blockIdx.x, lane);
+    if (it.s < 0) return;
+    const int row0 = it.tile * kMmaRows, rows = min(it.len * p.G - row0, kMmaRows);
+    const int pos0 = it.kv - it.len;
+    const int n = min(pos0 + (row0 + rows - 1) / p.G + 1, p.r.cap);      // keys that any row sees
+    const int j0 = it.split << p.kc_log2, jend = min(n, j0 + (1 << p.kc_log2));
+    if (j0 >= n && it.split > 0) return;
+    const int ntiles = max((jend - j0 + kMmaKeys - 1) / kMmaKeys, 0);
+
+    if (tid == 0) {
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&kfull[b], kMmaCopyWarps * 32); mbar_init(&kempty[b], 1);
+            mbar_init(&vfull[b], kMmaCopyWarps * 32); mbar_init(&vempty[b], 1);
+            mbar_init(&pfull[b], kMmaSoftWarps);
+        }
+        mbar_init(sfull, 2); mbar_init(sfree, kMmaSoftWarps);
+        mbar_init(ofull, 1); mbar_init(ofree, kMmaSoftWarps); mbar_init(done, 1);
+        fence_mbar_init();
+        *fail = 0;
+    }
+    if (warp == kMmaSoftWarps + kMmaCopyWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // queries -> digits: 16 lanes a row (whole warps; rows past the last are zeros)
+    for (int r = tid >> 4; r < kMmaRows; r += kMmaThreads / 16) {
+        const int l16 = tid & 15, cc = row0 + r;
+        const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
+        query_digits<128>(qr, r < rows, dh, l16, [&](int e, int d, uint32_t w) {
+            *reinterpret_cast<uint32_t*>(sm + Sm::Q + e * Sm::Tile + r * 128 + (((d >> 4) ^ (r & 7)) << 4) + (d & 15)) = w;
+        }, sq + r);
+    }
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    bool dead = false;                                         // a wait ran out: wait no more
+    auto wait = [&](uint64_t* bar, int parity) {
+        if (!dead && !mbar_wait_bounded(bar, (uint32_t)parity)) {
+            dead = true;
+            *fail = 1;
+        }
+    };
+    auto wait_warp = [&](uint64_t* bar, int parity) {          // by a whole warp
+        wait(bar, parity);
+        dead = __any_sync(0xffffffffu, dead);
+    };
+
+    if (warp == kMmaSoftWarps + kMmaCopyWarps) {
+        // ---- MMAs (one lane)
+        if (lane == 0) {
+            const uint32_t id = umma_idesc_i8(128, true), base = smem_u32(sm);
+            const int ksteps = (dh + 31) / 32;
+            auto scores = [&](int i) {
+                for (int k = 0; k < ksteps; ++k) {
+                    const uint64_t bd = umma_desc_sw128(base + Sm::K + (i & 1) * Sm::Tile + 32 * k);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        umma_i8(tmem + 128u * e, umma_desc_sw128(base + Sm::Q + e * Sm::Tile + 32 * k), bd, id, k > 0 ? 1u : 0u);
+                }
+                umma_commit(&kempty[i & 1]);
+                umma_commit(sfull);
+                mbar_arrive(sfull);                            // passes on what the copies wrote: the scales
+            };
+            auto output = [&](int i) {
+                for (int k = 0; k < kMmaKeys / 32; ++k) {
+                    const uint64_t bd = umma_desc_sw128(base + Sm::V + (i & 1) * Sm::Tile + 32 * k);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        umma_i8(tmem + 128u * e, umma_desc_sw128(base + Sm::P + (3 * (i & 1) + e) * Sm::Tile + 32 * k), bd, id,
+                                k > 0 ? 1u : 0u);
+                }
+                umma_commit(&vempty[i & 1]);
+                umma_commit(ofull);
+            };
+            if (ntiles > 0) {
+                wait(&kfull[0], 0);
+                tc_fence_after();
+                scores(0);
+            }
+            for (int i = 0; i < ntiles; ++i) {
+                wait(sfree, i & 1);
+                if (i > 0) {
+                    wait(&pfull[(i - 1) & 1], ((i - 1) >> 1) & 1);
+                    wait(&vfull[(i - 1) & 1], ((i - 1) >> 1) & 1);
+                    tc_fence_after();
+                    output(i - 1);
+                }
+                if (i + 1 < ntiles) {
+                    if (i > 0) wait(ofree, (i - 1) & 1);
+                    wait(&kfull[(i + 1) & 1], ((i + 1) >> 1) & 1);
+                    tc_fence_after();
+                    scores(i + 1);
+                }
+            }
+            if (ntiles > 0) {
+                const int i = ntiles - 1;
+                if (i > 0) wait(ofree, (i - 1) & 1);
+                wait(&pfull[i & 1], (i >> 1) & 1);
+                wait(&vfull[i & 1], (i >> 1) & 1);
+                tc_fence_after();
+                output(i);
+            }
+            umma_commit(done);                                 // also after a wait that ran out: no MMA may
+            if (!mbar_wait_bounded(done, 0)) *fail = 1;        // be under way when its memory is given up
+        }
+    } else if (warp >= kMmaSoftWarps) {
+        // ---- copies
+        const int ct = tid - kMmaSoftWarps * 32, cw = warp - kMmaSoftWarps;
+        for (int i = 0; i < ntiles; ++i) {
+            const int j = j0 + i * kMmaKeys, b = i & 1;
+            // the tile's blocks in the pool, block `lane & 7` (-1: page outside it, -2: past the end)
+            long long cell = -2;
+            const int jb = j + 16 * (lane & 7);
+            if (jb < jend) {
+                const int page = page_of(p.c, p.r, it.s, jb);
+                cell = page < 0 ? -1 : ((long long)page * p.c.KVH + it.kvh) * (psz >> 4) + ((jb & (psz - 1)) >> 4);
+            }
+            if (i > 1) wait_warp(&kempty[b], ((i >> 1) - 1) & 1);
+            unsigned char* kd = sm + Sm::K + b * Sm::Tile;
+            auto cell_of = [&](int blk) {                      // (whole warps)
+                return (long long)(((unsigned long long)(unsigned)__shfl_sync(0xffffffffu, (int)(cell >> 32), blk) << 32) |
+                                   (unsigned)__shfl_sync(0xffffffffu, (int)cell, blk));
+            };
+#pragma unroll
+            for (int x = 0; x < (1024 + kMmaCopyWarps * 32 - 1) / (kMmaCopyWarps * 32); ++x) {
+                const int unit = x * kMmaCopyWarps * 32 + ct, u = unit & 7, key = unit >> 3;
+                if (unit >= 1024) break;                       // (whole warps)
+                const long long at = cell_of(key >> 4);
+                const bool there = at >= 0 && 16 * u < dh;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                             ::"r"(smem_u32(kd + key * 128 + ((u ^ (key & 7)) << 4))),
+                               "l"(p.c.k + (there ? (at * kKvBlock + (key & 15)) * dh + 16 * u : 0)), "r"(there ? 16 : 0) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            // values: keys 4 lane .. + 3 of 16-element columns cw, cw + 3, cw + 6
+            uint4 vr[3][4];
+            {
+                const long long at = max(cell_of(lane >> 2), 0ll);     // what is not there has no weight
+                const int8_t* src = p.c.v + (at * kKvBlock + 4 * (lane & 3)) * dh;
+#pragma unroll
+                for (int x = 0; x < 3; ++x) {
+                    const int d = 16 * (cw + 3 * x) < dh ? 16 * (cw + 3 * x) : 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) vr[x][k] = __ldg(reinterpret_cast<const uint4*>(src + k * dh + d));
+                }
+            }
+            if (ct < 8) {
+                float* s = sc + (i & 3) * 24 + ct;
+                s[0] = cell >= 0 ? __ldg(p.c.ks + cell) : 0.0f;
+                s[8] = cell >= 0 ? __ldg(p.c.vs + cell) : 0.0f;
+                s[16] = cell >= 0 ? 1.0f : 0.0f;
+                if (cell == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            fence_async_smem();
+            mbar_arrive(&kfull[b]);
+            if (i > 1) wait_warp(&vempty[b], ((i >> 1) - 1) & 1);
+            unsigned char* vd = sm + Sm::V + b * Sm::Tile;
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                if (cw + 3 * x >= 8) break;
+                const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[x][0]);
+                const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[x][1]);
+                const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[x][2]);
+                const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[x][3]);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t a = __byte_perm(w0[w], w1[w], 0x5140), c = __byte_perm(w2[w], w3[w], 0x5140);
+                    const uint32_t d = __byte_perm(w0[w], w1[w], 0x7362), e = __byte_perm(w2[w], w3[w], 0x7362);
+                    const uint32_t y[4] = {__byte_perm(a, c, 0x5410), __byte_perm(a, c, 0x7632), __byte_perm(d, e, 0x5410),
+                                           __byte_perm(d, e, 0x7632)};
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const int el = 16 * (cw + 3 * x) + 4 * w + z;
+                        *reinterpret_cast<uint32_t*>(vd + el * 128 + (((lane >> 2) ^ (el & 7)) << 4) + 4 * (lane & 3)) = y[z];
+                    }
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&vfull[b]);
+        }
+    } else {
+        // ---- softmax and output
+        const int quarter = warp & 3, set = warp >> 2, row = 32 * quarter + lane, col0 = 32 * set;
+        const uint32_t trow = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)col0;
+        const int lim = row < rows ? min(pos0 + (row0 + row) / p.G + 1, n) : 0;   // keys the row sees
+        const int wmin = __reduce_min_sync(0xffffffffu, lim), wmax = __reduce_max_sync(0xffffffffu, lim);
+        const float sqr = sq[row];
+        float m = -INFINITY, l = 0.0f;                         // l: this set's keys
+        float back = 1.0f, u = 0.0f;                           // of the tile whose output is pending
+        bool pending = false;                                  // that output has this row quarter's weights
+        f32x2 o[16];                                           // elements col0 + 2 x, + 1
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[x] = 0ull;
+        auto fold = [&](int i) {                               // output sums of tile i
+            wait_warp(ofull, i & 1);
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (!pending || col0 + 8 * q >= dh) continue;  // (the same for the whole warp)
+                uint32_t c[3][8];
+#pragma unroll
+                for (int e = 0; e < 3; ++e) tmem_ld8(trow + 128u * e + 8u * q, c[e]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    o[4 * q + x] = fma2(join_digits((int)c[2][2 * x], (int)c[2][2 * x + 1], (int)c[1][2 * x], (int)c[1][2 * x + 1],
+                                                    (int)c[0][2 * x], (int)c[0][2 * x + 1]),
+                                        pack2(u, u), mul2(o[4 * q + x], pack2(back, back)));
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ofree);
+        };
+        for (int i = 0; i < ntiles; ++i) {
+            const int j = j0 + i * kMmaKeys;
+            const bool busy = wmax > j;                        // the same for the quarter's four warps
+            wait_warp(sfull, i & 1);
+            tc_fence_after();
+            float2 s[16];                                      // keys j + col0 + 2 x, + 1
+            const float* scb = sc + (i & 3) * 24 + 2 * set;
+            if (busy) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t c[3][8];
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) tmem_ld8(trow + 128u * e + 8u * q, c[e]);
+                    tmem_wait_ld();
+                    const float us = sqr * scb[q >> 1];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        s[4 * q + x] = unpack2(mul2(join_digits((int)c[2][2 * x], (int)c[2][2 * x + 1], (int)c[1][2 * x], (int)c[1][2 * x + 1],
+                                                                (int)c[0][2 * x], (int)c[0][2 * x + 1]), pack2(us, us)));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfree);
+            float nback = 1.0f, nu = 0.0f;
+            if (busy) {
+                const float t0 = scb[16], t1 = scb[17], v0 = scb[8], v1 = scb[9];
+                const int jk = j + col0;
+                if (jk + 32 > wmin || t0 + t1 != 2.0f) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int lx = (x < 8 ? t0 : t1) != 0.0f ? lim : 0;
+                        if (jk + 2 * x >= lx) s[x].x = -INFINITY;
+                        if (jk + 2 * x + 1 >= lx) s[x].y = -INFINITY;
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) mx = fmaxf(mx, fmaxf(s[x].x, s[x].y));
+                // exponentials and weights p v_scale relative to the set's own maximum. A score that
+                // is not a number makes l NaN, which is enough; a value scale that is not one
+                // needs checks
+                const float h = mx == -INFINITY ? 0.0f : mx;
+                f32x2 ls = 0ull;
+                float wt = 0.0f;
+                const bool sane = v0 + v1 == v0 + v1;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const float2 z = unpack2(add2(pack2(s[x].x, s[x].y), pack2(-h, -h)));
+                    const f32x2 ev = pack2(exp2_fast(z.x), exp2_fast(z.y));
+                    ls = add2(ls, ev);
+                    const float v = x < 8 ? v0 : v1;
+                    s[x] = unpack2(mul2(ev, pack2(v, v)));
+                }
+                if (!sane) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {             // a masked key weighs nothing, whatever its scale
+                        if (jk + 2 * x >= lim) s[x].x = 0.0f;
+                        if (jk + 2 * x + 1 >= lim) s[x].y = 0.0f;
+                        if (s[x].x != s[x].x || s[x].y != s[x].y) wt = INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 16; ++x) wt = fmaxf(wt, fmaxf(s[x].x, s[x].y));
+                // the other sets' keys: common maximum, one factor for all weights
+                float2* xt = xm + (i & 1) * 512 + row;
+                xt[128 * set] = make_float2(mx, wt);
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+                float2 y[4];
+                float top = m;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) { y[q] = xt[128 * q]; top = fmaxf(top, y[q].x); }
+                const float b = top == -INFINITY ? 0.0f : top;
+                nback = exp2_fast(m - b);
+                m = top;
+                const float corr = exp2_fast(mx - b);
+                l = ffma(l, nback, (unpack2(ls).x + unpack2(ls).y) * corr);
+                float big = 0.0f;
+                bool nan = false;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    big = fmaxf(big, y[q].y * exp2_fast(y[q].x - b));
+                    nan |= y[q].y == INFINITY;
+                }
+                const float f = weight_factor(big), fe = f * corr;
+                nu = nan ? __int_as_float(0x7fffffff) : weight_unit(f);
+                unsigned char* pd = sm + Sm::P + 3 * (i & 1) * Sm::Tile + row * 128;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {               // 16 keys: one 16-byte unit a digit
+                    uint32_t w[3][4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float2 a = s[8 * hh + 2 * x], c = s[8 * hh + 2 * x + 1];
+                        const float2 z0 = unpack2(fma2(pack2(a.x, a.y), pack2(fe, fe), pack2(kDigitBase, kDigitBase)));
+                        const float2 z1 = unpack2(fma2(pack2(c.x, c.y), pack2(fe, fe), pack2(kDigitBase, kDigitBase)));
+                        uint32_t d[3];
+                        digits4(__float_as_uint(z0.x), __float_as_uint(z0.y), __float_as_uint(z1.x), __float_as_uint(z1.y), d);
+                        w[0][x] = d[0]; w[1][x] = d[1]; w[2][x] = d[2];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        *reinterpret_cast<uint4*>(pd + e * Sm::Tile + (((2 * set + hh) ^ (row & 7)) << 4)) =
+                            make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+                }
+                fence_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[i & 1]);
+            if (i > 0) fold(i - 1);
+            back = nback; u = nu; pending = busy;
+        }
+        if (ntiles > 0) fold(ntiles - 1);
+        // the row's sum over its four sets
+        xm[set * 128 + row].x = l;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+        float L = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) L += xm[q * 128 + row].x;
+        if (row < rows) {
+            const int cc = row0 + row, splits = row_splits(p, pos0 + cc / p.G);
+            const int orow = it.a + cc / p.G, h = it.kvh * p.G + cc % p.G;
+            if (it.split < splits) {
+                const float inv = splits > 1 ? 1.0f : L == 0.0f ? 0.0f : fdiv(1.0f, L);
+                float* dst = splits > 1 ? p.part + (((size_t)orow * p.H + h) * p.nsplit + it.split) * (dh + 4)
+                                        : p.out + (size_t)orow * p.ldo + (size_t)h * dh;
+#pragma unroll
+                for (int x = 0; x < 16; x += 2) {
+                    const float2 a = unpack2(o[x]), c = unpack2(o[x + 1]);
+                    if (col0 + 2 * x < dh)
+                        *reinterpret_cast<float4*>(dst + col0 + 2 * x) = make_float4(a.x * inv, a.y * inv, c.x * inv, c.y * inv);
+                }
+                if (splits > 1 && set == 0) { dst[dh] = m; dst[dh + 1] = L; }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaSoftWarps + kMmaCopyWarps) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    if (tid == 0 && *fail) set_err(p.err, B2_DEV_ERR_TIMEOUT);
 }
 
 // Joins a (row, head)'s splits in a fixed order: WPH warps a pair, warp w the splits w,
