@@ -1520,7 +1520,7 @@ struct MmaSmem {
 static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(const __grid_constant__ PagedAttnParams p) {
     using Sm = MmaSmem;
     extern __shared__ unsigned char pm_raw[];
-    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pm_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* sm = pm_raw + ((1024u - (smem_u32(pm_raw) & 1023u)) & 1023u);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + Sm::Bars);      // [2] copies -> MMA
     uint64_t* kempty = kfull + 2;                                      // [2] MMA -> copies
     uint64_t* vfull = kempty + 2;                                      // [2]
@@ -1578,14 +1578,21 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool dead = false;                                         // a wait ran out: wait no more
-    auto wait = [&](uint64_t* bar, int parity) {
-        if (!dead && !mbar_wait_bounded(bar, (uint32_t)parity)) {
-            dead = true;
-            *fail = 1;
+    // bounded (1 s); `pause` ns between polls, which take issue slots from the warps that work
+    auto wait = [&](uint64_t* bar, int parity, unsigned pause) {
+        if (dead || mbar_try_wait(bar, (uint32_t)parity)) return;
+        const uint64_t t0 = globaltimer_ns();
+        for (unsigned k = 1; !mbar_try_wait(bar, (uint32_t)parity); ++k) {
+            __nanosleep(pause);
+            if ((k & 63u) == 0 && globaltimer_ns() - t0 > kWaitLimitNs) {
+                dead = true;
+                *fail = 1;
+                return;
+            }
         }
     };
-    auto wait_warp = [&](uint64_t* bar, int parity) {          // by a whole warp
-        wait(bar, parity);
+    auto wait_warp = [&](uint64_t* bar, int parity, unsigned pause) {   // by a whole warp
+        wait(bar, parity, pause);
         dead = __any_sync(0xffffffffu, dead);
     };
 
@@ -1617,30 +1624,30 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
                 umma_commit(ofull);
             };
             if (ntiles > 0) {
-                wait(&kfull[0], 0);
+                wait(&kfull[0], 0, 20);
                 tc_fence_after();
                 scores(0);
             }
             for (int i = 0; i < ntiles; ++i) {
-                wait(sfree, i & 1);
+                wait(sfree, i & 1, 20);
                 if (i > 0) {
-                    wait(&pfull[(i - 1) & 1], ((i - 1) >> 1) & 1);
-                    wait(&vfull[(i - 1) & 1], ((i - 1) >> 1) & 1);
+                    wait(&pfull[(i - 1) & 1], ((i - 1) >> 1) & 1, 20);
+                    wait(&vfull[(i - 1) & 1], ((i - 1) >> 1) & 1, 20);
                     tc_fence_after();
                     output(i - 1);
                 }
                 if (i + 1 < ntiles) {
-                    if (i > 0) wait(ofree, (i - 1) & 1);
-                    wait(&kfull[(i + 1) & 1], ((i + 1) >> 1) & 1);
+                    if (i > 0) wait(ofree, (i - 1) & 1, 20);
+                    wait(&kfull[(i + 1) & 1], ((i + 1) >> 1) & 1, 20);
                     tc_fence_after();
                     scores(i + 1);
                 }
             }
             if (ntiles > 0) {
                 const int i = ntiles - 1;
-                if (i > 0) wait(ofree, (i - 1) & 1);
-                wait(&pfull[i & 1], (i >> 1) & 1);
-                wait(&vfull[i & 1], (i >> 1) & 1);
+                if (i > 0) wait(ofree, (i - 1) & 1, 20);
+                wait(&pfull[i & 1], (i >> 1) & 1, 20);
+                wait(&vfull[i & 1], (i >> 1) & 1, 20);
                 tc_fence_after();
                 output(i);
             }
@@ -1659,7 +1666,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
                 const int page = page_of(p.c, p.r, it.s, jb);
                 cell = page < 0 ? -1 : ((long long)page * p.c.KVH + it.kvh) * (psz >> 4) + ((jb & (psz - 1)) >> 4);
             }
-            if (i > 1) wait_warp(&kempty[b], ((i >> 1) - 1) & 1);
+            if (i > 1) wait_warp(&kempty[b], ((i >> 1) - 1) & 1, 200);
             unsigned char* kd = sm + Sm::K + b * Sm::Tile;
             auto cell_of = [&](int blk) {                      // (whole warps)
                 return (long long)(((unsigned long long)(unsigned)__shfl_sync(0xffffffffu, (int)(cell >> 32), blk) << 32) |
@@ -1698,7 +1705,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             fence_async_smem();
             mbar_arrive(&kfull[b]);
-            if (i > 1) wait_warp(&vempty[b], ((i >> 1) - 1) & 1);
+            if (i > 1) wait_warp(&vempty[b], ((i >> 1) - 1) & 1, 200);
             unsigned char* vd = sm + Sm::V + b * Sm::Tile;
 #pragma unroll
             for (int x = 0; x < 3; ++x) {
@@ -1737,7 +1744,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
 #pragma unroll
         for (int x = 0; x < 16; ++x) o[x] = 0ull;
         auto fold = [&](int i) {                               // output sums of tile i
-            wait_warp(ofull, i & 1);
+            wait_warp(ofull, i & 1, 20);
             tc_fence_after();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -1759,7 +1766,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
         for (int i = 0; i < ntiles; ++i) {
             const int j = j0 + i * kMmaKeys;
             const bool busy = wmax > j;                        // the same for the quarter's four warps
-            wait_warp(sfull, i & 1);
+            wait_warp(sfull, i & 1, 20);
             tc_fence_after();
             float2 s[16];                                      // keys j + col0 + 2 x, + 1
             const float* scb = sc + (i & 3) * 24 + 2 * set;
