@@ -1483,11 +1483,12 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
 // ---- many rows per sequence, d_head up to 128: the 5th-generation tensor cores. A CTA
 // takes 128 rows against a split of the keys in tiles of 128.
 //   S = Q K^T, O = W V, each three MMA chains (tcgen05 kind::i8, one per digit) of
-//   128 x 128 x d_head (x 128 keys) into one TMEM region of 3 x 128 columns, which S and O
-//   take in turn: scores of tile i | output of tile i - 1 | scores of tile i + 1 | ...
-//   (a second region does not fit: 512 columns.) A pass of MMAs runs while the softmax
-//   warps work on what they have read before it, so that the matrix unit is never
-//   waited for long; what bounds the kernel is what the softmax warps issue.
+//   128 x 128 x d_head (x 128 keys). The passes S(0) S(1) O(0) S(2) O(1) ... take their
+//   three blocks of 128 TMEM columns from a ring of four: a pass's first chain needs the
+//   pass before the last one read, its others the last one. So MMAs run while the
+//   softmax warps work on what they have read before; what bounds the kernel is the
+//   latency of that work (scores 1000 clocks, exponentials 1800, digits 1700, folding
+//   1200 of 7500 a tile, measured), since all four of a row's warps meet every tile.
 // Warps 0 .. 15, softmax: warp w reads TMEM lanes 32 (w % 4) .. + 31, a row a thread, and
 //   set w / 4 has keys 32 (w / 4) .. + 31 of the tile and elements 32 (w / 4) .. + 31 of the
 //   output: no shuffles; a row's four threads exchange (maximum, largest weight) through
@@ -1512,8 +1513,9 @@ struct MmaSmem {
     static constexpr int Xm = V + 2 * Tile;                    // [2][4 sets][128 rows] (maximum, largest weight)
     static constexpr int Sc = Xm + 2 * 4 * 128 * 8;            // [4 tiles][3][8]: key scales, value scales, 1 where there
     static constexpr int Sq = Sc + 4 * 24 * 4;                 // [128] units of the rows' scores
-    static constexpr int Bars = Sq + 128 * 4;                  // 15 barriers, TMEM address, fail
+    static constexpr int Bars = Sq + 128 * 4;                  // 16 barriers, TMEM address, fail
     static constexpr int Bytes = Bars + 16 * 8 + 16;
+    static constexpr int OutStride = 132;                      // floats a row of the staged output (in P)
     static constexpr int Alloc = Bytes + 1024;                 // operands start on 1024 bytes
 };
 
@@ -1531,7 +1533,8 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
     uint64_t* ofull = pfull + 2;                                       // output sums in TMEM
     uint64_t* ofree = ofull + 1;                                       // output sums read
     uint64_t* done = ofree + 1;                                        // every MMA complete
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* qfull = done + 1;                                        // query digits written
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float2* xm = reinterpret_cast<float2*>(sm + Sm::Xm);
     float* sc = reinterpret_cast<float*>(sm + Sm::Sc);
@@ -1555,7 +1558,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
             mbar_init(&pfull[b], kMmaSoftWarps);
         }
         mbar_init(sfull, 2); mbar_init(sfree, kMmaSoftWarps);
-        mbar_init(ofull, 1); mbar_init(ofree, kMmaSoftWarps); mbar_init(done, 1);
+        mbar_init(ofull, 1); mbar_init(ofree, kMmaSoftWarps); mbar_init(done, 1); mbar_init(qfull, kMmaSoftWarps);
         fence_mbar_init();
         *fail = 0;
     }
@@ -1564,15 +1567,6 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
                      ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // queries -> digits: 16 lanes a row (whole warps; rows past the last are zeros)
-    for (int r = tid >> 4; r < kMmaRows; r += kMmaThreads / 16) {
-        const int l16 = tid & 15, cc = row0 + r;
-        const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
-        query_digits<128>(qr, r < rows, dh, l16, [&](int e, int d, uint32_t w) {
-            *reinterpret_cast<uint32_t*>(sm + Sm::Q + e * Sm::Tile + r * 128 + (((d >> 4) ^ (r & 7)) << 4) + (d & 15)) = w;
-        }, sq + r);
-    }
-    fence_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -1601,56 +1595,59 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
         if (lane == 0) {
             const uint32_t id = umma_idesc_i8(128, true), base = smem_u32(sm);
             const int ksteps = (dh + 31) / 32;
+            // chain e (digit 2 - e) of pass `op`: operands at a + (2 - e) tiles and b, `steps` of 32 bytes
+            auto chain = [&](int op, int e, uint32_t a, uint32_t b, int steps) {
+                const uint32_t col = 128u * ((3 * op + e) & 3);
+                for (int k = 0; k < steps; ++k)
+                    umma_i8(tmem + col, umma_desc_sw128(a + (2 - e) * Sm::Tile + 32 * k), umma_desc_sw128(b + 32 * k), id, k > 0 ? 1u : 0u);
+            };
+            // S(i): pass 2 i - 1 (0: pass 0), after O(i - 2) (pass 2 i - 2) and S(i - 1) (2 i - 3)
             auto scores = [&](int i) {
-                for (int k = 0; k < ksteps; ++k) {
-                    const uint64_t bd = umma_desc_sw128(base + Sm::K + (i & 1) * Sm::Tile + 32 * k);
-#pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        umma_i8(tmem + 128u * e, umma_desc_sw128(base + Sm::Q + e * Sm::Tile + 32 * k), bd, id, k > 0 ? 1u : 0u);
+                const int op = max(2 * i - 1, 0);
+                const uint32_t kb = base + Sm::K + (i & 1) * Sm::Tile;
+                wait(&kfull[i & 1], (i >> 1) & 1, 20);
+                if (i == 1) wait(sfree, 0, 20);                // (later ones: waited for by O(i - 2))
+                tc_fence_after();
+                chain(op, 0, base + Sm::Q, kb, ksteps);
+                if (i > 1) {
+                    wait(ofree, i & 1, 20);
+                    tc_fence_after();
                 }
+                chain(op, 1, base + Sm::Q, kb, ksteps);
+                chain(op, 2, base + Sm::Q, kb, ksteps);
                 umma_commit(&kempty[i & 1]);
                 umma_commit(sfull);
                 mbar_arrive(sfull);                            // passes on what the copies wrote: the scales
             };
+            // O(i): pass 2 i + 2, after S(i + 1) (2 i + 1) and O(i - 1) (2 i, whose reading the pass
+            // before has waited for, except at the end, where there is no S(i + 1))
             auto output = [&](int i) {
-                for (int k = 0; k < kMmaKeys / 32; ++k) {
-                    const uint64_t bd = umma_desc_sw128(base + Sm::V + (i & 1) * Sm::Tile + 32 * k);
-#pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        umma_i8(tmem + 128u * e, umma_desc_sw128(base + Sm::P + (3 * (i & 1) + e) * Sm::Tile + 32 * k), bd, id,
-                                k > 0 ? 1u : 0u);
+                const uint32_t pb = base + Sm::P + 3 * (i & 1) * Sm::Tile, vb = base + Sm::V + (i & 1) * Sm::Tile;
+                const bool end = i == ntiles - 1;
+                if (end && i > 0) wait(ofree, (i - 1) & 1, 20);
+                if (end && i == 0) wait(sfree, 0, 20);         // (no S(1) has waited for S(0))
+                wait(&pfull[i & 1], (i >> 1) & 1, 20);
+                wait(&vfull[i & 1], (i >> 1) & 1, 20);
+                tc_fence_after();
+                chain(2 * i + 2, 0, pb, vb, kMmaKeys / 32);
+                if (!end) {
+                    wait(sfree, (i + 1) & 1, 20);
+                    tc_fence_after();
                 }
+                chain(2 * i + 2, 1, pb, vb, kMmaKeys / 32);
+                chain(2 * i + 2, 2, pb, vb, kMmaKeys / 32);
                 umma_commit(&vempty[i & 1]);
                 umma_commit(ofull);
             };
             if (ntiles > 0) {
-                wait(&kfull[0], 0, 20);
-                tc_fence_after();
+                wait(qfull, 0, 20);
                 scores(0);
             }
             for (int i = 0; i < ntiles; ++i) {
-                wait(sfree, i & 1, 20);
-                if (i > 0) {
-                    wait(&pfull[(i - 1) & 1], ((i - 1) >> 1) & 1, 20);
-                    wait(&vfull[(i - 1) & 1], ((i - 1) >> 1) & 1, 20);
-                    tc_fence_after();
-                    output(i - 1);
-                }
-                if (i + 1 < ntiles) {
-                    if (i > 0) wait(ofree, (i - 1) & 1, 20);
-                    wait(&kfull[(i + 1) & 1], ((i + 1) >> 1) & 1, 20);
-                    tc_fence_after();
-                    scores(i + 1);
-                }
+                if (i > 0) output(i - 1);
+                if (i + 1 < ntiles) scores(i + 1);
             }
-            if (ntiles > 0) {
-                const int i = ntiles - 1;
-                if (i > 0) wait(ofree, (i - 1) & 1, 20);
-                wait(&pfull[i & 1], (i >> 1) & 1, 20);
-                wait(&vfull[i & 1], (i >> 1) & 1, 20);
-                tc_fence_after();
-                output(i);
-            }
+            if (ntiles > 0) output(ntiles - 1);
             umma_commit(done);                                 // also after a wait that ran out: no MMA may
             if (!mbar_wait_bounded(done, 0)) *fail = 1;        // be under way when its memory is given up
         }
@@ -1732,6 +1729,19 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
         }
     } else {
         // ---- softmax and output
+        // queries -> digits: 16 lanes a row (rows past the last are zeros)
+#pragma unroll
+        for (int x = 0; x < kMmaRows / 32; ++x) {
+            const int l16 = tid & 15, r = 32 * x + (tid >> 4), cc = row0 + r;
+            const float* qr = p.q + (size_t)(it.a + cc / p.G) * p.ldq + (size_t)(it.kvh * p.G + cc % p.G) * dh;
+            query_digits<128>(qr, r < rows, dh, l16, [&](int e, int d, uint32_t w) {
+                *reinterpret_cast<uint32_t*>(sm + Sm::Q + e * Sm::Tile + r * 128 + (((d >> 4) ^ (r & 7)) << 4) + (d & 15)) = w;
+            }, sq + r);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qfull);
+        asm volatile("bar.sync 5, 512;" ::: "memory");         // the units, too
         const int quarter = warp & 3, set = warp >> 2, row = 32 * quarter + lane, col0 = 32 * set;
         const uint32_t trow = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)col0;
         const int lim = row < rows ? min(pos0 + (row0 + row) / p.G + 1, n) : 0;   // keys the row sees
@@ -1743,6 +1753,8 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
         f32x2 o[16];                                           // elements col0 + 2 x, + 1
 #pragma unroll
         for (int x = 0; x < 16; ++x) o[x] = 0ull;
+        // 8 columns from col0 + 8 q of a pass's digit e (chain 2 - e)
+        auto read8 = [&](int op, int e, int q, uint32_t (&c)[8]) { tmem_ld8(trow + 128u * ((3 * op + 2 - e) & 3) + 8u * q, c); };
         auto fold = [&](int i) {                               // output sums of tile i
             wait_warp(ofull, i & 1, 20);
             tc_fence_after();
@@ -1751,7 +1763,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
                 if (!pending || col0 + 8 * q >= dh) continue;  // (the same for the whole warp)
                 uint32_t c[3][8];
 #pragma unroll
-                for (int e = 0; e < 3; ++e) tmem_ld8(trow + 128u * e + 8u * q, c[e]);
+                for (int e = 0; e < 3; ++e) read8(2 * i + 2, e, q, c[e]);
                 tmem_wait_ld();
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
@@ -1775,7 +1787,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
                 for (int q = 0; q < 4; ++q) {
                     uint32_t c[3][8];
 #pragma unroll
-                    for (int e = 0; e < 3; ++e) tmem_ld8(trow + 128u * e + 8u * q, c[e]);
+                    for (int e = 0; e < 3; ++e) read8(max(2 * i - 1, 0), e, q, c[e]);
                     tmem_wait_ld();
                     const float us = sqr * scb[q >> 1];
 #pragma unroll
@@ -1881,21 +1893,26 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
         float L = 0.0f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) L += xm[q * 128 + row].x;
-        if (row < rows) {
-            const int cc = row0 + row, splits = row_splits(p, pos0 + cc / p.G);
-            const int orow = it.a + cc / p.G, h = it.kvh * p.G + cc % p.G;
-            if (it.split < splits) {
-                const float inv = splits > 1 ? 1.0f : L == 0.0f ? 0.0f : fdiv(1.0f, L);
-                float* dst = splits > 1 ? p.part + (((size_t)orow * p.H + h) * p.nsplit + it.split) * (dh + 4)
-                                        : p.out + (size_t)orow * p.ldo + (size_t)h * dh;
+        // the rows through shared memory (the weights are not needed any more), so that a warp
+        // writes one row at a time
+        float* so = reinterpret_cast<float*>(sm + Sm::P);
+        const int splits = row < rows ? row_splits(p, pos0 + (row0 + row) / p.G) : 1;
+        const float inv = splits > 1 ? 1.0f : L == 0.0f ? 0.0f : fdiv(1.0f, L);
 #pragma unroll
-                for (int x = 0; x < 16; x += 2) {
-                    const float2 a = unpack2(o[x]), c = unpack2(o[x + 1]);
-                    if (col0 + 2 * x < dh)
-                        *reinterpret_cast<float4*>(dst + col0 + 2 * x) = make_float4(a.x * inv, a.y * inv, c.x * inv, c.y * inv);
-                }
-                if (splits > 1 && set == 0) { dst[dh] = m; dst[dh + 1] = L; }
-            }
+        for (int x = 0; x < 16; x += 2) {
+            const float2 a = unpack2(o[x]), c = unpack2(o[x + 1]);
+            *reinterpret_cast<float4*>(so + row * Sm::OutStride + col0 + 2 * x) = make_float4(a.x * inv, a.y * inv, c.x * inv, c.y * inv);
+        }
+        if (set == 0) xm[512 + row] = make_float2(m, L);
+        asm volatile("bar.sync 5, 512;" ::: "memory");
+        for (int r = warp; r < rows; r += kMmaSoftWarps) {
+            const int cc = row0 + r, tok = cc / p.G, ns = row_splits(p, pos0 + tok);
+            const int orow = it.a + tok, h = it.kvh * p.G + cc - tok * p.G;
+            if (it.split >= ns) continue;
+            float* dst = ns > 1 ? p.part + (((size_t)orow * p.H + h) * p.nsplit + it.split) * (dh + 4)
+                                : p.out + (size_t)orow * p.ldo + (size_t)h * dh;
+            if (4 * lane < dh) *reinterpret_cast<float4*>(dst + 4 * lane) = *reinterpret_cast<const float4*>(so + r * Sm::OutStride + 4 * lane);
+            if (ns > 1 && lane < 2) dst[dh + lane] = lane ? xm[512 + r].y : xm[512 + r].x;
         }
     }
     tc_fence_before();
