@@ -117,28 +117,49 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
     return cudaGetLastError();
 }
 
-// Columns (token, head) of a KV head that a CTA takes, which says the kernel, and the
-// keys per split.
-//  up to 16 columns in the longest sequence (on average if the caller does not say): 8, or
-//  2 where there are not more. Small splits fill the GPU when there are few rows; with
-//  long caches larger ones bound the partial results and their joining. A function of
-//  the capacity alone, so that a sequence's result does not depend on the others in
-//  the call.
-//  more: 64; keys are split only while there are too few tiles for two rounds of the GPU.
-int attn_plan(PagedAttnParams& p, int max_rows) {
-    const int G = p.H / p.c.KVH;
-    const long long cols = (max_rows > 0 ? max_rows : (p.r.n_rows + p.r.n_seq - 1) / std::max(p.r.n_seq, 1)) * (long long)G;
-    const int tile = cols <= 2 ? 2 : cols <= 16 ? kSplitCols : p.c.dh <= 128 ? kMmaRows : kTileRows;
-    if (cols <= 16) {
-        p.kc_log2 = p.r.cap <= 1024 ? 8 : 9;
-    } else {
-        const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / tile), want = tile == kMmaRows ? 4 * 148 : 6 * 148;
-        const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
-        p.kc_log2 = 8;
-        while (p.kc_log2 < 30 && ((long long)splits << p.kc_log2) < p.r.cap) ++p.kc_log2;
-    }
-    p.nsplit = std::max(1, (int)((p.r.cap + (1ll << p.kc_log2) - 1) >> p.kc_log2));
-    return tile;
+// A call's sequences are of two kinds, by their columns (token, head) of a KV head, and
+// each kind has a launch (one that finds none of its kind ends at once, in about 2 us; it
+// is left out where the caller's sizes say so). A whole batch on one kernel cost more: a
+// single token in a 128-row tile as much as 128, a prompt in 8-column tiles re-reads its
+// keys 16 times as often.
+//  few, up to 16 columns: 8 a CTA, or 2 where single tokens make no more (decode without
+//  shared heads; beside prompts too). Small splits fill the GPU when there are few
+//  rows; with long caches larger ones bound the partial results and their joining. A
+//  function of the capacity alone, so that a sequence's result does not depend on the
+//  others in the call.
+//  many: 128 a CTA (64 for d_head above 128); keys are split only while there are too few
+//  tiles for several rounds of the GPU.
+constexpr int kFewCols = 16;
+
+struct AttnPlan {
+    bool few, many;
+    int few_cols, many_cols;         // columns a CTA
+    long long few_items, many_items; // at most
+};
+
+AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
+    AttnPlan a{};
+    p.G = p.H / p.c.KVH;
+    const long long longest = (long long)(max_rows > 0 ? std::min(max_rows, p.r.n_rows) : p.r.n_rows) * p.G;
+    a.many = longest > kFewCols;
+    a.few = !a.many || p.r.n_seq > 1;
+    a.few_cols = longest <= 2 || (a.many && p.G <= 2) ? 2 : kSplitCols;
+    a.many_cols = p.c.dh <= 128 ? kMmaRows : kTileRows;
+    p.few = a.few ? (a.many ? kFewCols : INT32_MAX) : 0;
+    p.kc_few = p.r.cap <= 1024 ? 8 : 9;
+    const long long tiles = std::max(1ll, (long long)p.r.n_rows * p.H / a.many_cols), want = p.c.dh <= 128 ? 4 * 148 : 6 * 148;
+    const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
+    p.kc_many = 8;
+    while (p.kc_many < 30 && (splits << p.kc_many) < p.r.cap) ++p.kc_many;
+    const int kc = a.few && a.many ? std::min(p.kc_few, p.kc_many) : a.few ? p.kc_few : p.kc_many;
+    p.nsplit = std::max(1, (int)((p.r.cap + (1ll << kc) - 1) >> kc));
+    // tiles over all sequences: at most one partly filled one each
+    auto items = [&](int cols, int kc_log2) {
+        return ((long long)p.r.n_rows * p.G / cols + p.r.n_seq) * p.c.KVH * std::max(1ll, (p.r.cap + (1ll << kc_log2) - 1) >> kc_log2);
+    };
+    a.few_items = a.few ? items(a.few_cols, p.kc_few) : 0;
+    a.many_items = a.many ? items(a.many_cols, p.kc_many) : 0;
+    return a;
 }
 
 size_t part_bytes(const PagedAttnParams& p) {
@@ -152,50 +173,46 @@ int sm_count() {
 }
 
 cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || p.nsplit == 1) return e;
     // up to 8 splits: a warp each (row, head), else 8
     if (p.nsplit <= 8)
         return launch_ex(paged_attn_join_kernel<1>, dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
     return launch_ex(paged_attn_join_kernel<8>, dim3((unsigned)p.r.n_rows, (unsigned)p.H), dim3(256), 0, s, true, p);
 }
 
-cudaError_t launch_attn_mma(const PagedAttnParams& p, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(paged_attn_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaSmem::Alloc);
-    if (e != cudaSuccess) return e;
-    const long long most = ((long long)p.r.n_rows * p.G / kMmaRows + p.r.n_seq) * p.c.KVH * p.nsplit;
-    paged_attn_mma_kernel<<<(unsigned)most, kMmaThreads, MmaSmem::Alloc, s>>>(p);
-    return launch_join(p, s);
-}
-
-template <int DP>
-cudaError_t launch_attn_tile(const PagedAttnParams& p, cudaStream_t s) {
-    using Sh = TileShape<DP>;
-    auto k = paged_attn_tile_kernel<DP>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
-    if (e != cudaSuccess) return e;
-    const long long most = ((long long)p.r.n_rows * p.G / kTileRows + p.r.n_seq) * p.c.KVH * p.nsplit;
-    k<<<(unsigned)most, 128, Sh::Smem, s>>>(p);
-    return launch_join(p, s);
-}
-
 template <int DP, int NC>
-cudaError_t launch_attn_split(const PagedAttnParams& p, cudaStream_t s) {
+cudaError_t launch_few(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t s) {
     using Sh = SplitShape<DP, NC>;
     auto k = paged_attn_split_kernel<DP, NC>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
     if (e != cudaSuccess) return e;
-    // tiles over all sequences: at most one partly filled one each
-    const long long tiles = ((long long)p.r.n_rows * p.G / NC + p.r.n_seq) * p.c.KVH;
-    const long long most = tiles * p.nsplit, resident = (long long)sm_count() * (DP == 256 ? 2 : DP == 128 ? 3 : 4);
-    k<<<(unsigned)(most < resident ? most : resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
-    return launch_join(p, s);
+    const long long resident = (long long)sm_count() * (DP == 256 ? 2 : DP == 128 ? 3 : 4);
+    k<<<(unsigned)std::min(a.few_items, resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
+    return cudaGetLastError();
 }
 
-template <int DP>
-cudaError_t launch_attn(const PagedAttnParams& p, int cols, cudaStream_t s) {
-    return cols == 2 ? launch_attn_split<DP, 2>(p, s) : cols == 8 ? launch_attn_split<DP, 8>(p, s)
-           : cols == kMmaRows ? launch_attn_mma(p, s) : launch_attn_tile<DP>(p, s);
+cudaError_t launch_many(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t s) {
+    const bool mma = p.c.dh <= 128;
+    auto k = mma ? paged_attn_mma_kernel : paged_attn_tile_kernel<256>;
+    const int smem = mma ? MmaSmem::Alloc : TileShape<256>::Smem;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    k<<<(unsigned)a.many_items, mma ? kMmaThreads : 128, smem, s>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attn(PagedAttnParams p, const AttnPlan& a, cudaStream_t s) {
+    cudaError_t e = cudaSuccess;
+    if (a.many) {
+        p.lo = a.few ? kFewCols + 1 : 0; p.hi = INT32_MAX; p.kc_log2 = p.kc_many;
+        e = launch_many(p, a, s);
+    }
+    if (e == cudaSuccess && a.few) {
+        p.lo = 0; p.hi = p.few; p.kc_log2 = p.kc_few;
+        const int dp = p.c.dh <= 64 ? 64 : p.c.dh <= 128 ? 128 : 256;
+        e = a.few_cols == 2 ? (dp == 64 ? launch_few<64, 2>(p, a, s) : dp == 128 ? launch_few<128, 2>(p, a, s) : launch_few<256, 2>(p, a, s))
+                            : (dp == 64 ? launch_few<64, 8>(p, a, s) : dp == 128 ? launch_few<128, 8>(p, a, s) : launch_few<256, 8>(p, a, s));
+    }
+    return e == cudaSuccess && p.nsplit > 1 ? launch_join(p, s) : e;
 }
 
 }  // namespace
@@ -307,17 +324,15 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     if (!al4(err)) return refuse(fn, "err must be 4-byte aligned");
     if (q == out) return refuse(fn, "out must not be q");
     if ((int64_t)p.r.n_rows * n_heads > (1ll << 30)) return refuse(fn, "more than 2^30 (row, head) pairs");
-    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.G = n_heads / kv->n_kv_heads; p.err = err;
-    const int cols = attn_plan(p, rows->max_rows);
-    const long long items = ((long long)p.r.n_rows * p.G / cols + p.r.n_seq) * p.c.KVH * p.nsplit;
-    if (items >= kMaxItems) return refuse(fn, "too many (row, head, split) pieces for one call: use fewer rows");
+    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.err = err;
+    const AttnPlan plan = attn_plan(p, rows->max_rows);
+    if (plan.few_items >= kMaxItems || plan.many_items >= kMaxItems)
+        return refuse(fn, "too many (row, head, split) pieces for one call: use fewer rows or a smaller max_keys");
     const size_t need = part_bytes(p);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
     p.part = static_cast<float*>(workspace);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return status(fn, kv->d_head <= 64 ? launch_attn<64>(p, cols, s)
-                      : kv->d_head <= 128 ? launch_attn<128>(p, cols, s) : launch_attn<256>(p, cols, s));
+    return status(fn, launch_attn(p, plan, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

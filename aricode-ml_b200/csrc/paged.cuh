@@ -598,8 +598,11 @@ struct PagedAttnParams {
     float* out;              // [n_rows][ldo]
     long long ldq, ldo;
     int H, G;                // G = H / KVH
-    int kc_log2;             // keys per split
-    int nsplit;              // splits of a sequence of cap keys
+    int lo, hi;              // columns (rows * G) of the sequences that this launch takes
+    int kc_log2;             // keys per split of this launch's sequences
+    int few;                 // join: sequences of up to `few` columns have splits of
+    int kc_few, kc_many;     // 2^kc_few keys, the others of 2^kc_many
+    int nsplit;              // splits of a sequence of cap keys, at most
     unsigned zero;           // 0
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
@@ -613,9 +616,7 @@ struct AttnItem {
 };
 
 // splits of n keys (at least one: it also writes rows that see none)
-__device__ __forceinline__ int splits_of(const PagedAttnParams& p, int n) {
-    return max((n + (1 << p.kc_log2) - 1) >> p.kc_log2, 1);
-}
+__device__ __forceinline__ int splits_of(int kc_log2, int n) { return max((n + (1 << kc_log2) - 1) >> kc_log2, 1); }
 
 // Most items of one sequence (the host refuses calls that could have more): the sums
 // over 32 lanes stay in 32 bits whatever the row ranges are.
@@ -633,10 +634,11 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned
         int tiles = 0;
         if (s < p.r.n_seq) {
             q = seq_rows(p.r, s);
-            if (q.len > 0) {
+            const long long cols = (long long)q.len * p.G;
+            if (q.len > 0 && cols >= p.lo && cols <= p.hi) {
                 if (q.kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
                 tiles = (q.len * p.G + NC - 1) / NC;
-                cnt = (unsigned)min((long long)tiles * p.c.KVH * splits_of(p, min(q.kv, p.r.cap)), (long long)kMaxItems);
+                cnt = (unsigned)min((long long)tiles * p.c.KVH * splits_of(p.kc_log2, min(q.kv, p.r.cap)), (long long)kMaxItems);
             }
         }
         const unsigned total = __reduce_add_sync(0xffffffffu, cnt);
@@ -654,7 +656,7 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned
             out.len = __shfl_sync(0xffffffffu, q.len, src);
             out.kv = __shfl_sync(0xffffffffu, q.kv, src);
             // the last rows first: with causal lengths they are the longest
-            const unsigned splits = splits_of(p, min(out.kv, p.r.cap)), rest = idx / (unsigned)p.c.KVH;
+            const unsigned splits = splits_of(p.kc_log2, min(out.kv, p.r.cap)), rest = idx / (unsigned)p.c.KVH;
             out.kvh = (int)(idx % (unsigned)p.c.KVH);
             out.split = (int)(rest % splits);
             out.tile = __shfl_sync(0xffffffffu, tiles, src) - 1 - (int)(rest / splits);
@@ -667,7 +669,7 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned
 
 // splits that a row at position pos has
 __device__ __forceinline__ int row_splits(const PagedAttnParams& p, int pos) {
-    return splits_of(p, min(pos + 1, p.r.cap));
+    return splits_of(p.kc_log2, min(pos + 1, p.r.cap));
 }
 
 // One query row (16 lanes, lane l16 the elements 4 l16 + 64 i ..) as digits: store(e, d,
@@ -1936,18 +1938,17 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x, dh = p.c.dh;
     const int h = blockIdx.y * (8 / WPH) + warp / WPH, part = warp % WPH;
     pdl_wait();                                                    // the splits are written
-    int pos = 0;
-    bool found = false;
-    for (int base = 0; base < p.r.n_seq && !found; base += 32) {
+    int n = 0;                                                     // the row's splits, the same for the whole CTA
+    for (int base = 0; base < p.r.n_seq && n == 0; base += 32) {
         SeqRows q{0, 0, 0};
         if (base + lane < p.r.n_seq) q = seq_rows(p.r, base + lane);
         const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
         if (m) {
-            pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, __ffs(m) - 1);
-            found = true;
+            const int src = __ffs(m) - 1, pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, src);
+            const long long cols = (long long)__shfl_sync(0xffffffffu, q.len, src) * p.G;
+            n = splits_of(cols <= p.few ? p.kc_few : p.kc_many, min(pos + 1, p.r.cap));
         }
     }
-    const int n = found ? row_splits(p, pos) : 0;                  // the same for the whole CTA
     if (n < 2) return;
     const int stride = dh + 4;
     const float* base = p.part + ((size_t)row * p.H + min(h, p.H - 1)) * p.nsplit * stride;
