@@ -153,6 +153,8 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
     while (p.kc_many < 30 && (splits << p.kc_many) < p.r.cap) ++p.kc_many;
     const int kc = a.few && a.many ? std::min(p.kc_few, p.kc_many) : a.few ? p.kc_few : p.kc_many;
     p.nsplit = std::max(1, (int)((p.r.cap + (1ll << kc) - 1) >> kc));
+    // whole prompts: only the few-row sequences beside them have splits to join
+    if (a.few && a.many && (1ll << p.kc_many) >= p.r.cap && p.G <= kFewCols) p.join_rows = kFewCols / p.G;
     // tiles over all sequences: at most one partly filled one each
     auto items = [&](int cols, int kc_log2) {
         return ((long long)p.r.n_rows * p.G / cols + p.r.n_seq) * p.c.KVH * std::max(1ll, (p.r.cap + (1ll << kc_log2) - 1) >> kc_log2);
@@ -174,9 +176,10 @@ int sm_count() {
 
 cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
     // up to 8 splits: a warp each (row, head), else 8
+    const unsigned rows = p.join_rows ? (unsigned)(p.r.n_seq * p.join_rows) : (unsigned)p.r.n_rows;
     if (p.nsplit <= 8)
-        return launch_ex(paged_attn_join_kernel<1>, dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
-    return launch_ex(paged_attn_join_kernel<8>, dim3((unsigned)p.r.n_rows, (unsigned)p.H), dim3(256), 0, s, true, p);
+        return launch_ex(paged_attn_join_kernel<1>, dim3(rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
+    return launch_ex(paged_attn_join_kernel<8>, dim3(rows, (unsigned)p.H), dim3(256), 0, s, true, p);
 }
 
 template <int DP, int NC>

@@ -602,6 +602,8 @@ struct PagedAttnParams {
     int kc_log2;             // keys per split of this launch's sequences
     int few;                 // join: sequences of up to `few` columns have splits of
     int kc_few, kc_many;     // 2^kc_few keys, the others of 2^kc_many
+    int join_rows;           // 0: every row may have splits; else only the first join_rows
+                             // of each sequence of up to `few` columns
     int nsplit;              // splits of a sequence of cap keys, at most
     unsigned zero;           // 0
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
@@ -1935,18 +1937,25 @@ template <int WPH>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p) {
     __shared__ __align__(16) float so[8][256];
     __shared__ float sm[8][2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x, dh = p.c.dh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.c.dh;
     const int h = blockIdx.y * (8 / WPH) + warp / WPH, part = warp % WPH;
     pdl_wait();                                                    // the splits are written
-    int n = 0;                                                     // the row's splits, the same for the whole CTA
-    for (int base = 0; base < p.r.n_seq && n == 0; base += 32) {
-        SeqRows q{0, 0, 0};
-        if (base + lane < p.r.n_seq) q = seq_rows(p.r, base + lane);
-        const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
-        if (m) {
-            const int src = __ffs(m) - 1, pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, src);
-            const long long cols = (long long)__shfl_sync(0xffffffffu, q.len, src) * p.G;
-            n = splits_of(cols <= p.few ? p.kc_few : p.kc_many, min(pos + 1, p.r.cap));
+    int n = 0, row = blockIdx.x;                                   // the row's splits, the same for the whole CTA
+    if (p.join_rows) {
+        const int i = blockIdx.x % p.join_rows;
+        const SeqRows q = seq_rows(p.r, blockIdx.x / p.join_rows);
+        row = q.a + i;
+        if (i < q.len && (long long)q.len * p.G <= p.few) n = splits_of(p.kc_few, min(q.pos0() + i + 1, p.r.cap));
+    } else {
+        for (int base = 0; base < p.r.n_seq && n == 0; base += 32) {
+            SeqRows q{0, 0, 0};
+            if (base + lane < p.r.n_seq) q = seq_rows(p.r, base + lane);
+            const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
+            if (m) {
+                const int src = __ffs(m) - 1, pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, src);
+                const long long cols = (long long)__shfl_sync(0xffffffffu, q.len, src) * p.G;
+                n = splits_of(cols <= p.few ? p.kc_few : p.kc_many, min(pos + 1, p.r.cap));
+            }
         }
     }
     if (n < 2) return;
