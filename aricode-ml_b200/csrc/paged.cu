@@ -93,9 +93,7 @@ cudaError_t launch_norm_rope(const NormRopeParams& p, cudaStream_t s) {
     const int hpu = four ? 4 : 1;
     const long long lanes = (long long)p.n_rows * ((p.H + hpu - 1) / hpu + (p.KVH + hpu - 1) / hpu) * LPH;
     const unsigned grid = (unsigned)((lanes + 255) / 256);
-    if (four) norm_rope_kernel<LPH, VPL, 4><<<grid, 256, 0, s>>>(p);
-    else norm_rope_kernel<LPH, VPL, 1><<<grid, 256, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_ex(four ? norm_rope_kernel<LPH, VPL, 4> : norm_rope_kernel<LPH, VPL, 1>, dim3(grid), dim3(256), 0, s, true, p);
 }
 
 template <int LPH, int VPL>
@@ -104,17 +102,15 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
     if (max_rows == 1 || p.r.n_rows <= p.r.n_seq) {
         p.kv_ctas = (2 * p.c.KVH + 7) / 8;
         const int y = p.kv_ctas + (queries ? (p.nr.H * LPH + 255) / 256 : 0);
-        kv_append_kernel<LPH, VPL, 1, 1><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
-        return cudaGetLastError();
+        return launch_ex(kv_append_kernel<LPH, VPL, 1, 1>, dim3((unsigned)p.items, (unsigned)y), dim3(256), 0, s, true, p);
     }
     p.kv_ctas = p.c.KVH;
-    kv_append_kernel<LPH, VPL, LPH <= 8 ? 1 : LPH / 8, 4><<<dim3((unsigned)p.items, (unsigned)p.kv_ctas), 256, 0, s>>>(p);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e = launch_ex(kv_append_kernel<LPH, VPL, LPH <= 8 ? 1 : LPH / 8, 4>, dim3((unsigned)p.items, (unsigned)p.kv_ctas),
+                              dim3(256), 0, s, true, p);
     if (e != cudaSuccess || !queries) return e;
     // about four units of 4 vectors a lane group
     const int y = (kKvBlock * ((p.nr.H + 3) / 4) * LPH / 4 + 255) / 256;
-    append_queries_kernel<LPH, VPL><<<dim3((unsigned)p.items, (unsigned)y), 256, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_ex(append_queries_kernel<LPH, VPL>, dim3((unsigned)p.items, (unsigned)y), dim3(256), 0, s, true, p);
 }
 
 // A call's sequences are of two kinds, by their columns (token, head) of a KV head, and
@@ -189,8 +185,7 @@ cudaError_t launch_few(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
     if (e != cudaSuccess) return e;
     const long long resident = (long long)sm_count() * (DP == 256 ? 2 : DP == 128 ? 3 : 4);
-    k<<<(unsigned)std::min(a.few_items, resident), kSplitWarps * 32, Sh::Smem, s>>>(p);
-    return cudaGetLastError();
+    return launch_ex(k, dim3((unsigned)std::min(a.few_items, resident)), dim3(kSplitWarps * 32), Sh::Smem, s, true, p);
 }
 
 cudaError_t launch_many(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t s) {
@@ -199,8 +194,7 @@ cudaError_t launch_many(const PagedAttnParams& p, const AttnPlan& a, cudaStream_
     const int smem = mma ? MmaSmem::Alloc : TileShape<256>::Smem;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    k<<<(unsigned)a.many_items, mma ? kMmaThreads : 128, smem, s>>>(p);
-    return cudaGetLastError();
+    return launch_ex(k, dim3((unsigned)a.many_items), dim3(mma ? kMmaThreads : 128), smem, s, true, p);
 }
 
 cudaError_t launch_attn(PagedAttnParams p, const AttnPlan& a, cudaStream_t s) {
@@ -300,9 +294,7 @@ int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, vo
     p.err = err;
     const dim3 grid((unsigned)p.items, (unsigned)((2 * p.c.KVH + 7) / 8));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (bf16) kv_read_kernel<true><<<grid, 256, 0, s>>>(p);
-    else kv_read_kernel<false><<<grid, 256, 0, s>>>(p);
-    return status(fn, cudaGetLastError());
+    return status(fn, launch_ex(bf16 ? kv_read_kernel<true> : kv_read_kernel<false>, grid, dim3(256), 0, s, true, p));
 }
 
 size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads) {

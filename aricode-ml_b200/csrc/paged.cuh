@@ -52,6 +52,14 @@ __device__ __forceinline__ int page_of(const PagedKv& c, const PagedRows& r, int
     return (unsigned)id < (unsigned)c.n_pages ? id : -1;
 }
 
+// Start of every kernel here: they are launched with programmatic serialisation, so that
+// a launch comes up while the one before it drains, and read nothing before that is
+// complete.
+__device__ __forceinline__ void after_previous() {
+    pdl_launch_dependents();
+    pdl_wait();
+}
+
 // A run: the rows of one sequence that lie in one block of 16 tokens.
 struct BlockRun {
     int s;          // sequence (-1: none)
@@ -203,6 +211,7 @@ __device__ __forceinline__ void norm_rope_heads(const NormRopeParams& p, int row
 // a vector costs in instructions comes next (see make_turn).
 template <int LPH, int VPL, int HPU>
 __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+    after_previous();
     const unsigned per_row = (p.H + HPU - 1) / HPU + (p.KVH + HPU - 1) / HPU;
     const unsigned unit = (blockIdx.x * 256u + threadIdx.x) / LPH, row = unit / per_row;
     const int gl = threadIdx.x % LPH;
@@ -394,6 +403,7 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, const Bloc
 template <int LPH, int VPL, int NP, int WPT>
 __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ unsigned top[8 / WPT];
+    after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if constexpr (WPT > 1) {
         if (threadIdx.x < 8 / WPT) top[threadIdx.x] = 0u;
@@ -420,6 +430,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
 // rows above would leave them too few warps to keep the memory busy
 template <int LPH, int VPL>
 __global__ void __launch_bounds__(256) append_queries_kernel(const __grid_constant__ AppendParams p) {
+    after_previous();
     const BlockRun run = run_in_table(p, threadIdx.x & 31);
     if (run.s < 0) return;
     append_queries<LPH, VPL, 4>(p, run, (blockIdx.y * 256 + threadIdx.x) / LPH, gridDim.y * 256 / LPH, threadIdx.x & 31);
@@ -446,6 +457,7 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
 // (contiguous bytes) into values. Rows on a missing page become zeros.
 template <bool BF16>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ ReadParams p) {
+    after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const BlockRun run = find_run(p.r, blockIdx.x, p.items, p.err, lane);
     if (run.s < 0) return;
@@ -777,6 +789,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(16) unsigned char ps_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int dh = p.c.dh;
+    after_previous();
     unsigned item = blockIdx.x;
     SplitItem cur = next_split_item<NC>(p, item, lane);
     if (cur.it.s < 0) return;
@@ -1126,7 +1139,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 if (d == 0) { pp[dh] = M; pp[dh + 1] = L; }
             }
         }
-        if (nxt.it.s < 0) return;                                          // (a CTA's end lets the join start)
+        if (nxt.it.s < 0) return;
         cur = nxt;
     }
 }
@@ -1178,6 +1191,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int dh = p.c.dh, psz = 1 << p.c.page_log2;
 
+    after_previous();
     const AttnItem it = find_item<kTileRows>(p, blockIdx.x, lane);
     if (it.s < 0) return;
     const int row0 = it.tile * kTileRows, rows = min(it.len * p.G - row0, kTileRows);
@@ -1546,6 +1560,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int dh = p.c.dh, psz = 1 << p.c.page_log2;
 
+    after_previous();
     const AttnItem it = find_item<kMmaRows>(p, blockIdx.x, lane);
     if (it.s < 0) return;
     const int row0 = it.tile * kMmaRows, rows = min(it.len * p.G - row0, kMmaRows);
@@ -1939,7 +1954,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     __shared__ float sm[8][2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.c.dh;
     const int h = blockIdx.y * (8 / WPH) + warp / WPH, part = warp % WPH;
-    pdl_wait();                                                    // the splits are written
+    after_previous();                                              // the splits are written
     int n = 0, row = blockIdx.x;                                   // the row's splits, the same for the whole CTA
     if (p.join_rows) {
         const int i = blockIdx.x % p.join_rows;

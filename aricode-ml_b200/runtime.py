@@ -473,7 +473,7 @@ def _invalid(msg):
 
 def _tensor(name, t, dtype, gpu, shape=None):
     """The address of a contiguous CUDA tensor of this type and shape on GPU number `gpu` (None: any)."""
-    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous() or (gpu is not None and t.get_device() != gpu):
+    if t.dtype is not dtype or not t.is_contiguous() or (t.get_device() != gpu if gpu is not None else not t.is_cuda):
         raise _invalid(f"{name} must be a contiguous {dtype} tensor on {'a GPU' if gpu is None else f'cuda:{gpu}'}")
     if shape is not None and t.shape != shape:
         raise _invalid(f"{name} must have shape {shape}, not {tuple(t.shape)}")
