@@ -294,7 +294,10 @@ int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, vo
     p.err = err;
     const dim3 grid((unsigned)p.items, (unsigned)((2 * p.c.KVH + 7) / 8));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return status(fn, launch_ex(bf16 ? kv_read_kernel<true> : kv_read_kernel<false>, grid, dim3(256), 0, s, true, p));
+    const int dh = kv->d_head;
+#define B2_CALL(L) launch_ex(bf16 ? kv_read_kernel<true, L> : kv_read_kernel<false, L>, grid, dim3(256), 0, s, true, p)
+    return status(fn, dh <= 16 ? B2_CALL(2) : dh <= 32 ? B2_CALL(4) : dh <= 64 ? B2_CALL(8) : dh <= 128 ? B2_CALL(16) : B2_CALL(32));
+#undef B2_CALL
 }
 
 size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads) {

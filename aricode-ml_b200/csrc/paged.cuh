@@ -454,37 +454,47 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
 }
 
 // Grid (runs, CTAs of 8 head tasks): a warp turns one head's K or V codes of the run
-// (contiguous bytes) into values. Rows on a missing page become zeros.
-template <bool BF16>
+// (contiguous bytes) into values, LPR lanes a row of 8 codes each, all loads first.
+// Bound by memory. Rows on a missing page become zeros.
+template <bool BF16, int LPR>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ ReadParams p) {
     after_previous();
+    constexpr int RPP = 32 / LPR, NP = kKvBlock / RPP;         // rows a pass, passes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const BlockRun run = find_run(p.r, blockIdx.x, p.items, p.err, lane);
     if (run.s < 0) return;
     const int task = blockIdx.y * 8 + warp;
     if (task >= 2 * p.c.KVH) return;
-    const int head = task >> 1, dh = p.c.dh;
+    const int head = task >> 1, dh = p.c.dh, d = 8 * (lane % LPR), r0 = lane / LPR;
     const bool is_k = (task & 1) == 0;
     const int page = page_of(p.c, p.r, run.s, run.pos);
     if (page < 0 && lane == 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
     const int psz = 1 << p.c.page_log2;
     const size_t cell = ((size_t)max(page, 0) * p.c.KVH + head) * (psz / kKvBlock) + (run.pos & (psz - 1)) / kKvBlock;
     const float s = page < 0 ? 0.0f : __ldg((is_k ? p.c.ks : p.c.vs) + cell);
-    const int8_t* codes = (is_k ? p.c.k : p.c.v) + cell * kKvBlock * dh + (size_t)(run.pos % kKvBlock) * dh;
-    for (int b = lane * 8; b < run.n * dh; b += 256) {
-        const uint2 w = page < 0 ? make_uint2(0u, 0u) : __ldg(reinterpret_cast<const uint2*>(codes + b));
+    const int8_t* codes = (is_k ? p.c.k : p.c.v) + (cell * kKvBlock + run.pos % kKvBlock) * dh + d;
+    uint2 w[NP];
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+        const int r = x * RPP + r0;
+        w[x] = page >= 0 && r < run.n && d < dh ? __ldg(reinterpret_cast<const uint2*>(codes + r * dh)) : make_uint2(0u, 0u);
+    }
+    const size_t at = (size_t)run.row * p.ld + (size_t)head * dh + d;
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+        const int r = x * RPP + r0;
+        if (r >= run.n || d >= dh) continue;
         float f[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            f[e] = fmul((float)(signed char)(w.x >> (8 * e)), s);
-            f[4 + e] = fmul((float)(signed char)(w.y >> (8 * e)), s);
+            f[e] = fmul((float)(signed char)(w[x].x >> (8 * e)), s);
+            f[4 + e] = fmul((float)(signed char)(w[x].y >> (8 * e)), s);
         }
-        const size_t at = (size_t)(run.row + b / dh) * p.ld + (size_t)head * dh + b % dh;
         if constexpr (BF16) {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(is_k ? p.k : p.v) + at) =
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(is_k ? p.k : p.v) + at + r * p.ld) =
                 make_uint4(bf16x2_bits(f[0], f[1]), bf16x2_bits(f[2], f[3]), bf16x2_bits(f[4], f[5]), bf16x2_bits(f[6], f[7]));
         } else {
-            float* o = static_cast<float*>(is_k ? p.k : p.v) + at;
+            float* o = static_cast<float*>(is_k ? p.k : p.v) + at + r * p.ld;
             *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<float4*>(o + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }
