@@ -190,8 +190,8 @@ cudaError_t launch_few(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t
 
 cudaError_t launch_many(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t s) {
     const bool mma = p.c.dh <= 128;
-    auto k = mma ? paged_attn_mma_kernel : paged_attn_tile_kernel<256>;
-    const int smem = mma ? MmaSmem::Alloc : TileShape<256>::Smem;
+    auto k = mma ? paged_attn_mma_kernel : paged_attn_tile_kernel;
+    const int smem = mma ? MmaSmem::Alloc : TileShape::Smem;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     return launch_ex(k, dim3((unsigned)a.many_items), dim3(mma ? kMmaThreads : 128), smem, s, true, p);

@@ -529,12 +529,6 @@ __device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
-// four registers for an A operand. `zero` is a 0 that the compiler does not know: with a
-// plain copy it would gather the operand again for every MMA that uses it
-__device__ __forceinline__ void own_quad(uint32_t (&q)[4], uint32_t zero, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    q[0] = a ^ zero; q[1] = b ^ zero; q[2] = c ^ zero; q[3] = d ^ zero;
-}
-
 // two f32 in one instruction: the attention kernels are bound by what the schedulers
 // issue, and a packed operation takes one slot for two (same rounding)
 typedef unsigned long long f32x2;
@@ -627,7 +621,6 @@ struct PagedAttnParams {
     int join_rows;           // 0: every row may have splits; else only the first join_rows
                              // of each sequence of up to `few` columns
     int nsplit;              // splits of a sequence of cap keys, at most
-    unsigned zero;           // 0
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
 };
@@ -740,7 +733,7 @@ __device__ __forceinline__ void query_digits(const float* qr, bool live, int dh,
 // The four warps' (m, l, o) meet in shared memory, one barrier an item.
 constexpr int kSplitWarps = 4;
 constexpr int kSplitCols = 8;
-constexpr int kSplitMaxKeys = 512;                 // keys per split at most: a block a lane
+// (at most 512 keys a split: its blocks are one a lane)
 
 // NC columns an item: 8, or 2 for calls of one or two columns a KV head (decode without
 // shared heads). Then the digits are the MMA's columns instead: A = codes (16 keys x d,
@@ -1055,11 +1048,6 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 for (int b = 0; b < 2; ++b)
                     digits4(digit_bits_pos(e[2 * b].x, f), digit_bits_pos(e[2 * b].y, f), digit_bits_pos(e[2 * b + 1].x, f),
                             digit_bits_pos(e[2 * b + 1].y, f), wd[b]);
-                // A registers of their own, so that no MMA has to gather them (rows 8 to 15 of the
-                // second one are not used)
-                uint32_t wh[4], wl[4];
-                own_quad(wh, p.zero, wd[0][2], wd[0][1], wd[1][2], wd[1][1]);
-                own_quad(wl, p.zero, wd[0][0], wd[0][0], wd[1][0], wd[1][0]);
                 // output: column n of tile x is element (DP/8) n + x: four keys' bytes of one
                 // element make one B register
 #pragma unroll
@@ -1074,9 +1062,9 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                     }
                     int hi[4][4], lo[4][4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wh[0], wh[1], wh[2], wh[3], a[0][k], a[1][k]);
+                    for (int k = 0; k < 4; ++k) mma_s8_first(hi[k], wd[0][2], wd[0][1], wd[1][2], wd[1][1], a[0][k], a[1][k]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wl[0], wl[1], wl[2], wl[3], a[0][k], a[1][k]);
+                    for (int k = 0; k < 4; ++k) mma_s8_first(lo[k], wd[0][0], wd[0][0], wd[1][0], wd[1][0], a[0][k], a[1][k]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         o[4 * w + k] = fma2(join_digits(hi[k][0], hi[k][1], hi[k][2], hi[k][3], lo[k][0], lo[k][1]), pack2(u, u),
@@ -1154,20 +1142,19 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
     }
 }
 
-// ---- many rows per sequence: a CTA of 4 warps takes 64 rows ((token, head) pairs of
+// ---- many rows per sequence, d_head above 128 (three digits' output sums of 256 elements do
+// not fit the tensor memory beside anything): a CTA of 4 warps takes 64 rows ((token, head) pairs of
 // one KV head), warp w 16 of them, against a split of the keys in tiles of KT. A =
 // query or weight digits (rows x 32), B = codes: keys as they lie, values turned to
 // [d][key] on their way into shared memory (byte permutes, once for the CTA). The
 // key order inside a B fragment of the values is the one that the score fragments
 // already have, so weights go from scores to A fragments inside their thread.
-// Codes of tile i + 1 are on their way while tile i is computed. Every tile ends with
-// folding the output's digit sums into f32 (their unit changes with the row's
-// maximum), which is why KT is as large as the registers allow.
+// Codes of tile i + 1 are on their way while tile i is computed.
 constexpr int kTileRows = 64;
 
-template <int DP>
 struct TileShape {
-    static constexpr int KT = DP == 256 ? 64 : 128;            // keys per tile
+    static constexpr int DP = 256;                             // d_head, padded
+    static constexpr int KT = 64;                              // keys per tile
     static constexpr int NB = KT / 16;                         // blocks per tile
     static constexpr int NH = DP / 64;
     static constexpr int NT = DP / 8;                          // output tiles of 8 elements
@@ -1187,10 +1174,9 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ther
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-template <int DP>
-__global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel(const __grid_constant__ PagedAttnParams p) {
-    using Sh = TileShape<DP>;
-    constexpr int KT = Sh::KT, NB = Sh::NB;
+static __global__ void __launch_bounds__(128, 1) paged_attn_tile_kernel(const __grid_constant__ PagedAttnParams p) {
+    using Sh = TileShape;
+    constexpr int DP = Sh::DP, KT = Sh::KT, NB = Sh::NB;
     extern __shared__ __align__(16) unsigned char pt_raw[];
     uint8_t* qd = pt_raw;                                      // A fragments [3][4 warps][DP / 32][lane][16]
     uint8_t* kt = qd + Sh::QBytes;                             // [2][KT][DP]
@@ -1251,16 +1237,13 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
             if (cb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
         }
     };
-    // This thread's part of a value tile: in block vb four keys vq2 + {0, 1, 8, 9} of 16
-    // elements from d0 + 16 x. The lanes of a warp cover 32 (block, key group) pairs of one
-    // 16-element column (KT = 128), so that its word stores meet no bank twice.
-    constexpr int VH = KT / 64;                                // 64-key halves among a warp's lanes
+    // This thread's part of a value tile: in block vb four keys vq2 + {0, 1, 8, 9} of two
+    // 16-element columns from d0.
     constexpr int VC = KT * DP / 64 / 128;                     // 16-byte columns a thread turns
-    const int vb = (lane & 15) >> 2, vq2 = (lane & 3) * 2, vh = VH == 2 ? lane >> 4 : 0;
-    const int d0 = 16 * (VH == 2 ? VC * warp : VC * (2 * warp + (lane >> 4)));
+    const int vb = (lane & 15) >> 2, vq2 = (lane & 3) * 2, d0 = 16 * VC * (2 * warp + (lane >> 4));
     uint4 vr[VC][4];
     auto load_values = [&](int i) {
-        const long long at = cell[NB * (i & 1) + 4 * vh + vb];
+        const long long at = cell[NB * (i & 1) + vb];
 #pragma unroll
         for (int x = 0; x < VC; ++x) {
             // what is not there is read from the pool's first block: its weights are 0, and
@@ -1287,7 +1270,7 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
                                        __byte_perm(c, e, 0x7632)};
 #pragma unroll
                 for (int z = 0; z < 4; ++z)
-                    *reinterpret_cast<uint32_t*>(vd + unit_at<KT>(d0 + 16 * x + 4 * w + z, 4 * vh + (vq2 >> 1)) + 4 * vb) = y[z];
+                    *reinterpret_cast<uint32_t*>(vd + unit_at<KT>(d0 + 16 * x + 4 * w + z, vq2 >> 1) + 4 * vb) = y[z];
             }
         }
     };
@@ -1446,27 +1429,17 @@ __global__ void __launch_bounds__(128, DP == 256 ? 1 : 2) paged_attn_tile_kernel
 #pragma unroll
             for (int x = 0; x < Sh::NT; x += 2) {              // two output tiles at a time: six independent chains
                 int c[2][3][4];
+                uint4 b[2];
 #pragma unroll
-                for (int h = 0; h < VH; ++h) {
-                    uint4 b[2];
+                for (int z = 0; z < 2; ++z) b[z] = *reinterpret_cast<const uint4*>(vd + unit_at<KT>(8 * (x + z) + g, t));
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) b[z] = *reinterpret_cast<const uint4*>(vd + unit_at<KT>(8 * (x + z) + g, 4 * h + t));
+                for (int e = 0; e < 3; ++e)
 #pragma unroll
-                    for (int e = 0; e < 3; ++e)
+                    for (int z = 0; z < 2; ++z) mma_s8_first(c[z][e], wa[0][e][0], wa[0][e][1], wa[0][e][2], wa[0][e][3], b[z].x, b[z].y);
 #pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            const uint32_t(&a)[4] = wa[2 * h][e];
-                            if (h == 0) mma_s8_first(c[z][e], a[0], a[1], a[2], a[3], b[z].x, b[z].y);
-                            else mma_s8(c[z][e], a[0], a[1], a[2], a[3], b[z].x, b[z].y);
-                        }
+                for (int e = 0; e < 3; ++e)
 #pragma unroll
-                    for (int e = 0; e < 3; ++e)
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            const uint32_t(&a)[4] = wa[2 * h + 1][e];
-                            mma_s8(c[z][e], a[0], a[1], a[2], a[3], b[z].z, b[z].w);
-                        }
-                }
+                    for (int z = 0; z < 2; ++z) mma_s8(c[z][e], wa[1][e][0], wa[1][e][1], wa[1][e][2], wa[1][e][3], b[z].z, b[z].w);
 #pragma unroll
                 for (int z = 0; z < 2; ++z)
 #pragma unroll

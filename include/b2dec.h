@@ -278,7 +278,8 @@ int b2_attn_decode_static(const float* q, const float* K, const float* V, float*
  *   B2_ROWS_OVERFLOW  a position at or past the sequence's capacity (the smaller of
  *                     max_keys and max_pages * page_size), or past the table
  *   B2_ROWS_BAD_PAGE  a page-table entry outside [0, n_pages)
- *   B2_ROWS_OVERLAP   row ranges that overlap
+ *   B2_ROWS_OVERLAP   row ranges that overlap (append and read; attention then leaves
+ *                     some rows out)
  * d_head: a multiple of 16 from 16 to 256. f32 rows: 16-byte aligned, row strides in
  * elements, a multiple of 4. Calls on one cache must be ordered by the caller. */
 #define B2_KV_BLOCK 16
@@ -287,7 +288,7 @@ enum { B2_ROWS_OVERFLOW = 2, B2_ROWS_BAD_PAGE = 4, B2_ROWS_OVERLAP = 5 };
 typedef struct b2_kv_pages {
     int8_t* k;               /* [n_pages][n_kv_heads][page_size][d_head], 16-byte aligned */
     int8_t* v;
-    float* k_scale;          /* [n_pages][n_kv_heads][page_size / B2_KV_BLOCK] */
+    float* k_scale;          /* [n_pages][n_kv_heads][page_size / B2_KV_BLOCK], not negative */
     float* v_scale;
     int32_t n_pages;
     int32_t page_size;       /* tokens: a power of two from 16 to 1024 */

@@ -514,6 +514,58 @@ def test_rows_do_not_depend_on_the_other_sequences(torch, rt):
         assert torch.equal(rt.attn_paged_i8(kv, rt.KVRows(**one, max_rows=1), q[s:s + 1])[0], both[s])
 
 
+def test_prompts_beside_single_tokens(torch, rt):
+    """A whole prompt beside single tokens with long caches: the prompt's rows have no splits to join, the tokens' have."""
+    rows, keys, H, KVH, dh = [2000, 1, 3, 1], [2000, 3000, 700, 1], 32, 8, 128
+    kv, plan = pool(torch, rt, rows, keys, KVH, dh, 64, seed=8)
+    q = torch.randn(sum(rows), H * dh, device="cuda") * dh ** -0.5
+    out = rt.attn_paged_i8(kv, rt.KVRows(**plan, max_keys=3000), q)
+    want, tol = attend64(torch, kv, plan, rows, keys, q, H)
+    close(torch, out.reshape(-1, H, dh), want, tol)
+
+
+def test_many_sequences(torch, rt):
+    """600 sequences (the searches for a sequence go over 32 at a time), some without rows: append, read and attend."""
+    n, H, KVH, dh = 600, 4, 2, 64
+    keys = [(7 * s) % 90 + 1 for s in range(n)]
+    rows = [0 if s % 11 == 3 else 1 if s % 5 else min(3, keys[s]) for s in range(n)]
+    kv, plan = pool(torch, rt, rows, keys, KVH, dh, 32)
+    r = rt.KVRows(**plan)
+    T = sum(rows)
+    x = torch.randn(T, KVH * dh, device="cuda")
+    want = append_plain(torch, kv, plan, rows, keys, x.reshape(T, KVH, dh), "v")
+    rt.kv_append_i8(kv, r, x, x)
+    assert torch.equal(kv.v, want[0])
+    got = rt.kv_read_i8(kv, r)[1].reshape(T, KVH, dh)
+    a = 0
+    for s in range(n):
+        h = held(torch, kv, plan["page_table"], s, keys[s])[1]
+        assert torch.equal(got[a:a + rows[s]].double(), h[keys[s] - rows[s]:].float().double())
+        a += rows[s]
+    q = torch.randn(T, H * dh, device="cuda") * 0.1
+    close(torch, rt.attn_paged_i8(kv, r, q).reshape(T, H, dh), *attend64(torch, kv, plan, rows, keys, q, H))
+    kv.check()
+
+
+def test_hints_that_are_wrong_and_an_empty_table(torch, rt):
+    """max_rows below the truth costs time, not results; without pages nothing is seen or written."""
+    rows, keys, H, KVH, dh = [40, 1], [60, 500], 8, 2, 64
+    kv, plan = pool(torch, rt, rows, keys, KVH, dh, 16)
+    q = torch.randn(41, H * dh, device="cuda") * 0.1
+    want, tol = attend64(torch, kv, plan, rows, keys, q, H)
+    for hint in (1, 3, 41, 4000):
+        close(torch, rt.attn_paged_i8(kv, rt.KVRows(**plan, max_rows=hint), q).reshape(41, H, dh), want, tol)
+    kv.check()
+    empty = dict(plan, page_table=torch.zeros(2, 0, dtype=torch.int32, device="cuda"))
+    before = kv.k.clone()
+    r = rt.KVRows(**empty)
+    x = torch.randn(41, KVH * dh, device="cuda")
+    rt.kv_append_i8(kv, r, x, x)
+    assert torch.equal(kv.k, before) and bool((rt.attn_paged_i8(kv, r, q) == 0).all())
+    with pytest.raises(rt.B2Error, match="capacity"):
+        kv.check()
+
+
 # ------------------------------------------------------------------ together
 def test_a_layer_decoded_step_by_step(torch, rt):
     """Prompts of three sequences, then tokens: append (norm, rotation, queries on the way) and attend, each step
