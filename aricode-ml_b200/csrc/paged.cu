@@ -120,9 +120,9 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
 // keys 16 times as often.
 //  few, up to 16 columns: 8 a CTA, or 2 where single tokens make no more (decode without
 //  shared heads; beside prompts too). Small splits fill the GPU when there are few
-//  rows; with long caches larger ones bound the partial results and their joining. A
-//  function of the capacity alone, so that a sequence's result does not depend on the
-//  others in the call.
+//  rows; with long caches larger ones bound the partial results and their joining. Their
+//  size is a function of the capacity alone; the columns a CTA follow the longest sequence,
+//  so the last bits of a sequence's result can differ beside others.
 //  many: 128 a CTA (64 for d_head above 128); keys are split only while there are too few
 //  tiles for several rounds of the GPU.
 constexpr int kFewCols = 16;

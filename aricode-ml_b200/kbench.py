@@ -6,6 +6,7 @@
     python aricode-ml_b200/kbench.py decode --config llama2-7b --pos 512 --tokens 8
     python aricode-ml_b200/kbench.py prefill --config llama2-7b --layers 2 --tokens 511
     python aricode-ml_b200/kbench.py batch --config llama2-7b-b64 --layers 2 --steps 8
+    python aricode-ml_b200/kbench.py paged --seqs 64 --keys 1152 [--rows 1] [--heads 32 --kv-heads 32]
 
 Prints one JSON line: device time per launch (CUDA events over a captured CUDA
 graph of all launches, after an untimed replay), algorithmic bytes per launch and GB/s.
@@ -33,6 +34,10 @@ batch: batched decode of `seqs` sequences (default: the config's batch) whose
 caches are filled by prefills of `prompt` ids each, then `steps` device-resident
 batched steps; reports ms per step and GB/s (weights once + every sequence's KV
 rows per step).
+
+paged: attention of `rows` rows of each of `seqs` sequences over a paged int8 cache
+holding `keys` keys a sequence, cycling over `caches` distinct pools. Algorithmic
+bytes = seqs * keys * kv_heads * (2 * d_head + 8 / 16) (codes and scales) + q and out.
 """
 from __future__ import annotations
 
@@ -157,6 +162,33 @@ def batch(torch, pkg, args):
     dec.close()
 
 
+def paged(torch, pkg, args):
+    rt = pkg.runtime
+    torch.cuda.set_stream(torch.cuda.Stream())
+    S, R, n, H, K, d, page = args.seqs, args.rows, args.keys, args.heads, args.kv_heads, args.d_head, args.page
+    if R > n:
+        raise SystemExit("--rows must not exceed --keys")
+    per = -(-n // page)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    table = torch.randperm(S * per, device="cuda", generator=gen).to(torch.int32).reshape(S, per)
+    rows = rt.KVRows(torch.arange(S + 1, **i32) * R, torch.full((S,), n, **i32), table, n_rows=S * R, max_keys=n, max_rows=R)
+    pools = []
+    for _ in range(args.caches):
+        kv = rt.PagedKV.empty(S * per, page, K, d)
+        for codes, scale in ((kv.k, kv.k_scale), (kv.v, kv.v_scale)):
+            codes.random_(-127, 128, generator=gen)
+            scale.fill_(0.02)
+        pools.append(kv)
+    q = torch.randn(S * R, H * d, device="cuda", generator=gen) * d ** -0.5
+    out = torch.empty_like(q)
+    ws = rt.attn_paged_workspace(pools[0], rows, H)
+    us = timed(torch, lambda kv, h: rt.attn_paged_i8(kv, rows, q, out=out, workspace=ws, stream=h), pools, args.reps)
+    nbytes = S * n * K * (2 * d + 8 / 16) + 8 * S * R * H * d
+    print(json.dumps({"kernel": "attn_paged_i8", "seqs": S, "rows": R, "keys": n, "heads": H, "kv_heads": K, "d_head": d,
+                      "page": page, "us_per_call": us, "bytes_per_call": nbytes, "gbs": nbytes / (us * 1e-6) / 1e9}), flush=True)
+
+
 def main():
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="kernel", required=True)
@@ -189,6 +221,16 @@ def main():
     bt.add_argument("--seqs", type=int, default=None)
     bt.add_argument("--prompt", type=int, default=None)
     bt.add_argument("--steps", type=int, default=8)
+    pg = sub.add_parser("paged")
+    pg.add_argument("--seqs", type=int, default=64)
+    pg.add_argument("--rows", type=int, default=1)
+    pg.add_argument("--keys", type=int, default=1152)
+    pg.add_argument("--heads", type=int, default=32)
+    pg.add_argument("--kv-heads", type=int, default=32)
+    pg.add_argument("--d-head", type=int, default=128)
+    pg.add_argument("--page", type=int, default=64)
+    pg.add_argument("--caches", type=int, default=2)
+    pg.add_argument("--reps", type=int, default=10)
     args = ap.parse_args()
 
     import torch
@@ -200,6 +242,8 @@ def main():
         return prefill(torch, pkg, args)
     if args.kernel == "batch":
         return batch(torch, pkg, args)
+    if args.kernel == "paged":
+        return paged(torch, pkg, args)
     torch.cuda.set_stream(torch.cuda.Stream())
     gen = torch.Generator(device="cuda").manual_seed(0)
 
