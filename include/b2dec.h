@@ -325,8 +325,7 @@ int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, fl
 
 /* Write the call's K and V rows [n_rows][n_kv_heads * d_head] into the cache, keys
  * normed (k_gain) and rotated (table, at the row's position) on the way as in
- * b2_qk_norm_rope; with q, the queries likewise into q_out in the same launch (not
- * cached).
+ * b2_qk_norm_rope; with q, the queries likewise into q_out (not cached).
  * A block's scale is max|x| / 127 over its values; a row that needs a larger one
  * grows it and brings the block's older codes to it (rint(code * old / new)). A
  * block whose first token is written starts afresh. Codes are rint(x / scale). A NaN or

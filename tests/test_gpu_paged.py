@@ -678,6 +678,26 @@ def test_streams_and_reused_memory(torch, rt):
     assert all(torch.equal(o, want) for o in got[0] + got[1])
 
 
+def test_prompts_and_single_tokens_on_two_streams_at_once(torch, rt):
+    """Two calls on one cache that may overlap, a workspace each: the same bits as one after the other."""
+    rows, keys, H, KVH, dh = [300, 1, 200], [300, 2500, 700], 16, 4, 128
+    kv, plan = pool(torch, rt, rows, keys, KVH, dh, 32)
+    mixed, single = rt.KVRows(**plan), rt.KVRows(**ragged(torch, [1, 1, 1], keys, plan["page_table"]), max_rows=1)
+    q = torch.randn(sum(rows), H * dh, device="cuda") * dh ** -0.5
+    calls = [(mixed, q), (single, q[:3])]
+    want = [rt.attn_paged_i8(kv, r, x) for r, x in calls]
+    ws = [rt.attn_paged_workspace(kv, r, H) for r, _ in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for j, (r, x) in enumerate(calls):
+            got[j].append(rt.attn_paged_i8(kv, r, x, workspace=ws[j], stream=streams[j].cuda_stream))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[j]) for j in range(2) for o in got[j])
+    kv.check()
+
+
 def test_refusals_of_the_wrappers(torch, rt):
     kv, plan = pool(torch, rt, [2], [20], 2, 64, 16)
     r = rt.KVRows(**plan)
