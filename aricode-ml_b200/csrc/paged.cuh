@@ -401,8 +401,10 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, const Bloc
 // all of them (120 registers, 16 warps an SM) 6300 rows took 41 us. Few registers, so
 // that many runs are on the SMs at once: it is bound by the latency of run -> page ->
 // scale and older codes. 6300 rows of 8 heads of 128: 27 to 29 us; 64 single rows of 32: 8 us.
+// Six CTAs an SM for d_head 65 to 128 instead of the five that its registers allow: 148 ->
+// 144 us for 6300 rows of 32 + 32 heads with queries and read back; at 64 no difference.
 template <int LPH, int VPL, int NP, int WPT>
-__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256, WPT == 4 && LPH == 32 && VPL == 1 ? 6 : 1) kv_append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ unsigned top[8 / WPT];
     after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
