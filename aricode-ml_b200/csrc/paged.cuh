@@ -209,7 +209,7 @@ __device__ __forceinline__ void norm_rope_heads(const NormRopeParams& p, int row
 
 // One lane group per (row, HPU heads). Bound by memory once there are enough rows; what
 // a vector costs in instructions comes next (see make_turn). 8191 rows of 40 heads of 128:
-// 55 us, 6.2 TB/s, 0.95 of a plain copy's rate; a row of 36 heads of 64: 3.4 us.
+// 55 us, 6.2 TB/s, 0.94 of a plain copy's rate; a row of 36 heads of 64: 3.4 us.
 template <int LPH, int VPL, int HPU>
 __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
     after_previous();

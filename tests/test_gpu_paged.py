@@ -514,6 +514,21 @@ def test_rows_do_not_depend_on_the_other_sequences(torch, rt):
         assert torch.equal(rt.attn_paged_i8(kv, rt.KVRows(**one, max_rows=1), q[s:s + 1])[0], both[s])
 
 
+@pytest.mark.parametrize("H,KVH,dh,rows,keys,cap", [
+    (32, 8, 128, [40], [9000], 9000), (32, 8, 128, [40, 1, 64, 30], [300, 9000, 4097, 31], 20000), (12, 12, 64, [20] * 5, [2500, 20, 700, 4000, 1], 0),
+    (16, 2, 80, [5, 3], [6000, 5999], 6000), (32, 8, 64, [17] + [1] * 260, [5000] + [40] * 260, 0), (8, 8, 128, [17, 0, 16], [0, 0, 3000], 0)])
+def test_pieces_over_caches_of_very_different_lengths(torch, rt, H, KVH, dh, rows, keys, cap):
+    """Pieces of prompts over caches of very different lengths, also far below the capacity; calls again are the same bits."""
+    kv, plan = pool(torch, rt, rows, keys, KVH, dh, 32, seed=4)
+    n = sum(rows)
+    q = torch.randn(n, H * dh, device="cuda") * dh ** -0.5
+    r = rt.KVRows(**plan, max_keys=cap)
+    out = rt.attn_paged_i8(kv, r, q)
+    close(torch, out.reshape(n, H, dh), *attend64(torch, kv, plan, rows, keys, q, H))
+    kv.check()
+    assert torch.equal(rt.attn_paged_i8(kv, r, q), out)
+
+
 def test_prompts_beside_single_tokens(torch, rt):
     """A whole prompt beside single tokens with long caches: the prompt's rows have no splits to join, the tokens' have."""
     rows, keys, H, KVH, dh = [2000, 1, 3, 1], [2000, 3000, 700, 1], 32, 8, 128
