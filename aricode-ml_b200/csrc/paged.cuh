@@ -283,7 +283,8 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
                 if (i0 + j * RPW >= run.n) continue;
-                const float r = head_rms<LPH, VPL>(x[j], p.nr.inv_dh, p.nr.eps);
+                // (rows past the run are zeros and stay so: without an eps their norm is not a number)
+                const float rms = head_rms<LPH, VPL>(x[j], p.nr.inv_dh, p.nr.eps), r = i0 + j * RPW + g < run.n ? rms : 0.0f;
 #pragma unroll
                 for (int e = 0; e < VPL; ++e)
                     x[j][e] = make_float4(fmul(fmul(x[j][e].x, r), gv[e].x), fmul(fmul(x[j][e].y, r), gv[e].y),

@@ -741,3 +741,27 @@ def test_refusals_of_the_wrappers(torch, rt):
         with pytest.raises(rt.B2Error):
             f()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n", [1, 3, 17])
+@pytest.mark.parametrize("KVH,dh", [(3, 16), (2, 64), (2, 128), (1, 256)])
+@pytest.mark.parametrize("single", [False, True])
+def test_append_norms_without_an_eps(torch, rt, n, KVH, dh, single):
+    """eps = 0 is a norm too, for vectors that are not zeros: the block's scale comes from the run's rows alone, however
+    many of them a pass holds. `single`: the variant for single rows, by a hint below the truth."""
+    g = torch.Generator(device="cuda").manual_seed(n + dh)
+    kv = rt.PagedKV.empty(4, 16, KVH, dh)
+    table = torch.tensor([[2, 0, 3]], dtype=torch.int32, device="cuda")
+    rows = rt.KVRows(**ragged(torch, [n], [n + 2], table), max_rows=int(single))
+    k, v = torch.randn(2, n, KVH * dh, device="cuda", generator=g)
+    gain = 1 + 0.3 * torch.rand(dh, device="cuda", generator=g)
+    rt.kv_append_i8(kv, rows, k, v, k_gain=gain, eps=0.0)
+    x = k.reshape(n, KVH, dh).double()
+    want = x / x.square().mean(-1, keepdim=True).sqrt() * gain.double()
+    got = held(torch, kv, table, 0, n + 2)[0][2:]
+    for lo in range(0, n + 2, 16):
+        a, b = max(lo - 2, 0), min(lo + 14, n)
+        top = want[a:b].abs().amax((0, 2), keepdim=True)
+        # half a step of the scale, which is top / 127 up to f32, and what f32 did before the code was chosen
+        close(torch, got[a:b], want[a:b], (0.5 * top / 127 * (1 + 1e-5)).expand(b - a, -1, dh) + turn_tol(want[a:b].abs(), dh))
+    kv.check()
