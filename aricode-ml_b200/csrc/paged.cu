@@ -151,12 +151,16 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
     p.nsplit = std::max(1, (int)((p.r.cap + (1ll << kc) - 1) >> kc));
     // whole prompts: only the few-row sequences beside them have splits to join
     if (a.few && a.many && (1ll << p.kc_many) >= p.r.cap && p.G <= kFewCols) p.join_rows = kFewCols / p.G;
-    // tiles over all sequences: at most one partly filled one each
-    auto items = [&](int cols, int kc_log2) {
-        return ((long long)p.r.n_rows * p.G / cols + p.r.n_seq) * p.c.KVH * std::max(1ll, (p.r.cap + (1ll << kc_log2) - 1) >> kc_log2);
+    auto items = [&](long long tiles, int kc_log2) {
+        return tiles * p.c.KVH * std::max(1ll, (p.r.cap + (1ll << kc_log2) - 1) >> kc_log2);
     };
-    a.few_items = a.few ? items(a.few_cols, p.kc_few) : 0;
-    a.many_items = a.many ? items(a.many_cols, p.kc_many) : 0;
+    // tiles of `cols` columns over all sequences: at most one partly filled one each
+    auto tiles_of = [&](int cols) { return (long long)p.r.n_rows * p.G / cols + p.r.n_seq; };
+    // beside many-row sequences those of the few-row kind have up to kFewCols columns each, whatever n_rows is
+    const long long few_tiles = a.many ? std::min(tiles_of(a.few_cols), (long long)p.r.n_seq * ((kFewCols + a.few_cols - 1) / a.few_cols))
+                                       : tiles_of(a.few_cols);
+    a.few_items = a.few ? items(few_tiles, p.kc_few) : 0;
+    a.many_items = a.many ? items(tiles_of(a.many_cols), p.kc_many) : 0;
     return a;
 }
 

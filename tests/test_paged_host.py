@@ -154,3 +154,14 @@ def test_handles_refuse_host_tensors_and_bad_shapes(pkg):
         rt.qk_norm_rope(None, None, 64)
     with pytest.raises(rt.B2Error):
         rt.qk_norm_rope(torch.zeros(2, 64), None, 64)
+
+
+@pytest.mark.parametrize("n_rows,n_seq,cap,H,KVH", [(16384, 2, 1 << 17, 32, 32), (8192, 9, 1 << 18, 32, 32), (30000, 40, 1 << 18, 12, 12)])
+def test_long_prompts_over_a_large_capacity_are_accepted(pkg, n_rows, n_seq, cap, H, KVH):
+    """Only a few rows of a call can be short sequences' single tokens: the rest does not count as pieces of that kind.
+    (Without a workspace the call stops before its launch: what it says then is that it needs one.)"""
+    rt = pkg.runtime
+    r = rows(rt, n_rows=n_rows, n_seq=n_seq, max_pages=cap // 64)
+    kv = pages(rt, n_pages=1 << 14, page_size=64, n_kv_heads=KVH, d_head=128)
+    assert attend(rt, kv, r, n_heads=H, ldq=H * 128, ldo=H * 128, ws=None, ws_bytes=0) == -1
+    assert "workspace" in rt.last_error()
