@@ -138,7 +138,7 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
     p.G = p.H / p.c.KVH;
     const long long longest = (long long)(max_rows > 0 ? std::min(max_rows, p.r.n_rows) : p.r.n_rows) * p.G;
     a.many = longest > kFewCols;
-    a.few = !a.many || p.r.n_seq > 1;
+    a.few = !a.many || (p.r.n_seq > 1 && p.G <= kFewCols);
     a.few_cols = longest <= 2 || (a.many && p.G <= 2) ? 2 : kSplitCols;
     a.many_cols = p.c.dh <= 128 ? kMmaRows : kTileRows;
     p.few = a.few ? (a.many ? kFewCols : INT32_MAX) : 0;
@@ -147,12 +147,18 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
     const long long splits = std::max(1ll, std::min(want / tiles, (p.r.cap + 255ll) / 256));
     p.kc_many = 8;
     while (p.kc_many < 30 && (splits << p.kc_many) < p.r.cap) ++p.kc_many;
-    const int kc = a.few && a.many ? std::min(p.kc_few, p.kc_many) : a.few ? p.kc_few : p.kc_many;
-    p.nsplit = std::max(1, (int)((p.r.cap + (1ll << kc) - 1) >> kc));
-    // whole prompts: only the few-row sequences beside them have splits to join
-    if (a.few && a.many && (1ll << p.kc_many) >= p.r.cap && p.G <= kFewCols) p.join_rows = kFewCols / p.G;
+    auto splits_at = [&](int kc_log2) { return std::max(1, (int)((p.r.cap + (1ll << kc_log2) - 1) >> kc_log2)); };
+    p.nsplit_few = a.few ? splits_at(p.kc_few) : 1;
+    p.nsplit_many = a.many ? splits_at(p.kc_many) : 1;
+    if (a.few && a.many) {
+        // a sequence of the few-row kind has at most this many rows
+        const int most = kFewCols / p.G;
+        if ((long long)p.r.n_seq * most < p.r.n_rows) p.few_rows = most;
+        // whole prompts: only the few-row sequences beside them have splits to join
+        if (p.nsplit_many == 1) p.join_rows = most;
+    }
     auto items = [&](long long tiles, int kc_log2) {
-        return tiles * p.c.KVH * std::max(1ll, (p.r.cap + (1ll << kc_log2) - 1) >> kc_log2);
+        return tiles * p.c.KVH * splits_at(kc_log2);
     };
     // tiles of `cols` columns over all sequences: at most one partly filled one each
     auto tiles_of = [&](int cols) { return (long long)p.r.n_rows * p.G / cols + p.r.n_seq; };
@@ -164,8 +170,18 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
     return a;
 }
 
-size_t part_bytes(const PagedAttnParams& p) {
-    return p.nsplit > 1 ? (size_t)p.r.n_rows * p.H * p.nsplit * (p.c.dh + 4) * sizeof(float) : 0;
+// bytes of the partial results of the few-row kind, then of the many-row kind. (One area
+// for both, with the finer split for every row of the call, took 35 GB for 8192 rows in 9
+// sequences of 32 heads of 128 at a capacity of 128 K, now 156 MB; the many-row kind's
+// splits fill the GPU a few times at most, whatever the capacity is: at most 118 MB.)
+struct PartBytes {
+    size_t few, many;
+};
+
+PartBytes part_bytes(const PagedAttnParams& p) {
+    const size_t head = (size_t)p.H * (p.c.dh + 4) * sizeof(float);
+    const size_t slots = p.few_rows ? (size_t)p.r.n_seq * p.few_rows : (size_t)p.r.n_rows;
+    return {p.nsplit_few > 1 ? slots * head * p.nsplit_few : 0, p.nsplit_many > 1 ? (size_t)p.r.n_rows * head * p.nsplit_many : 0};
 }
 
 int sm_count() {
@@ -177,7 +193,7 @@ int sm_count() {
 cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
     // up to 8 splits: a warp each (row, head), else 8
     const unsigned rows = p.join_rows ? (unsigned)(p.r.n_seq * p.join_rows) : (unsigned)p.r.n_rows;
-    if (p.nsplit <= 8)
+    if (std::max(p.nsplit_few, p.nsplit_many) <= 8)
         return launch_ex(paged_attn_join_kernel<1>, dim3(rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
     return launch_ex(paged_attn_join_kernel<8>, dim3(rows, (unsigned)p.H), dim3(256), 0, s, true, p);
 }
@@ -213,7 +229,7 @@ cudaError_t launch_attn(PagedAttnParams p, const AttnPlan& a, cudaStream_t s) {
         e = a.few_cols == 2 ? (dp == 64 ? launch_few<64, 2>(p, a, s) : dp == 128 ? launch_few<128, 2>(p, a, s) : launch_few<256, 2>(p, a, s))
                             : (dp == 64 ? launch_few<64, 8>(p, a, s) : dp == 128 ? launch_few<128, 8>(p, a, s) : launch_few<256, 8>(p, a, s));
     }
-    return e == cudaSuccess && p.nsplit > 1 ? launch_join(p, s) : e;
+    return e == cudaSuccess && (p.nsplit_few > 1 || p.nsplit_many > 1) ? launch_join(p, s) : e;
 }
 
 }  // namespace
@@ -309,7 +325,8 @@ size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows,
     if (!view("b2_attn_paged_i8_workspace", kv, rows, p.c, p.r) || n_heads <= 0 || n_heads % kv->n_kv_heads) return 0;
     p.H = n_heads;
     attn_plan(p, rows->max_rows);
-    return part_bytes(p);
+    const PartBytes part = part_bytes(p);
+    return part.few + part.many;
 }
 
 int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* q, int64_t ldq, float* out, int64_t ldo,
@@ -330,10 +347,12 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     const AttnPlan plan = attn_plan(p, rows->max_rows);
     if (plan.few_items >= kMaxItems || plan.many_items >= kMaxItems)
         return refuse(fn, "too many (row, head, split) pieces for one call: use fewer rows or a smaller max_keys");
-    const size_t need = part_bytes(p);
+    const PartBytes part = part_bytes(p);
+    const size_t need = part.few + part.many;
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
-    p.part = static_cast<float*>(workspace);
+    p.part_few = static_cast<float*>(workspace);
+    p.part_many = p.part_few + part.few / sizeof(float);
     return status(fn, launch_attn(p, plan, static_cast<cudaStream_t>(stream)));
 }
 

@@ -622,12 +622,16 @@ struct PagedAttnParams {
     int H, G;                // G = H / KVH
     int lo, hi;              // columns (rows * G) of the sequences that this launch takes
     int kc_log2;             // keys per split of this launch's sequences
-    int few;                 // join: sequences of up to `few` columns have splits of
+    int few;                 // sequences of up to `few` columns have splits of
     int kc_few, kc_many;     // 2^kc_few keys, the others of 2^kc_many
     int join_rows;           // 0: every row may have splits; else only the first join_rows
                              // of each sequence of up to `few` columns
-    int nsplit;              // splits of a sequence of cap keys, at most
-    float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
+    // Partial results [slot][H][nsplit][dh + 4]: o, m (base 2), l; an area for each kind. A
+    // slot is a row; in the few-row kind's area with few_rows > 0 it is the row's number in
+    // its sequence, of few_rows a sequence. nsplit: splits of cap keys
+    int few_rows, nsplit_few, nsplit_many;
+    float* part_few;
+    float* part_many;
     int* err;
 };
 
@@ -645,8 +649,10 @@ __device__ __forceinline__ int splits_of(int kc_log2, int n) { return max((n + (
 // over 32 lanes stay in 32 bits whatever the row ranges are.
 constexpr int kMaxItems = 1 << 26;
 
-// item number `item` of the call (tiles of NC rows), found by one warp
-template <int NC>
+// Item number `item` of the call (tiles of NC rows), found by one warp. OneWord: s becomes
+// sequence * 1024 + KV head (up to 2^20 and 1024 of them) and kvh stays 0, for the split
+// kernel, which has no register left for both.
+template <int NC, bool OneWord = false>
 __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned item, int lane) {
     AttnItem out{-1, 0, 0, 0, 0, 0, 0};
     unsigned before = 0;
@@ -680,7 +686,9 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned
             out.kv = __shfl_sync(0xffffffffu, q.kv, src);
             // the last rows first: with causal lengths they are the longest
             const unsigned splits = splits_of(p.kc_log2, min(out.kv, p.r.cap)), rest = idx / (unsigned)p.c.KVH;
-            out.kvh = (int)(idx % (unsigned)p.c.KVH);
+            const int kvh = (int)(idx % (unsigned)p.c.KVH);
+            if constexpr (OneWord) out.s = out.s * 1024 + kvh;
+            else out.kvh = kvh;
             out.split = (int)(rest % splits);
             out.tile = __shfl_sync(0xffffffffu, tiles, src) - 1 - (int)(rest / splits);
             return out;
@@ -693,6 +701,15 @@ __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned
 // splits that a row at position pos has
 __device__ __forceinline__ int row_splits(const PagedAttnParams& p, int pos) {
     return splits_of(p.kc_log2, min(pos + 1, p.r.cap));
+}
+
+// partial result `split` of head h of row tok of sequence s (row `row` of the call)
+__device__ __forceinline__ float* few_part(const PagedAttnParams& p, int s, int tok, int row, int h, int split) {
+    const size_t slot = p.few_rows ? (size_t)s * p.few_rows + tok : (size_t)row;
+    return p.part_few + ((slot * p.H + h) * p.nsplit_few + split) * (p.c.dh + 4);
+}
+__device__ __forceinline__ float* many_part(const PagedAttnParams& p, int row, int h, int split) {
+    return p.part_many + (((size_t)row * p.H + h) * p.nsplit_many + split) * (p.c.dh + 4);
 }
 
 // One query row (16 lanes, lane l16 the elements 4 l16 + 64 i ..) as digits: store(e, d,
@@ -757,7 +774,9 @@ struct SplitShape {
 };
 
 struct SplitItem {
-    AttnItem it;
+    AttnItem it;             // its sequence and KV head in one word
+    __device__ __forceinline__ int seq() const { return it.s >> 10; }
+    __device__ __forceinline__ int kvh() const { return it.s & 1023; }
     int cols, col0, n, j0, jend;
     int cell;                // block `lane` of the split in the pool (codes start at 16 dh
     float ks, vs;            // times that; -1: page outside the pool, -2: past the end), scales
@@ -768,7 +787,7 @@ template <int NC>
 __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, unsigned& item, int lane) {
     SplitItem w;
     for (;; item += gridDim.x) {
-        w.it = find_item<NC>(p, item, lane);
+        w.it = find_item<NC, true>(p, item, lane);
         w.cell = -2;
         if (w.it.s < 0) return w;
         w.col0 = w.it.tile * NC;
@@ -782,8 +801,8 @@ __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, u
     const int j = w.j0 + 16 * lane;
     w.ks = w.vs = 0.0f;
     if (j < w.jend) {
-        const int page = page_of(p.c, p.r, w.it.s, j), b = p.c.page_log2 - 4;
-        w.cell = page < 0 ? -1 : ((page * p.c.KVH + w.it.kvh) << b) + ((j >> 4) & ((1 << b) - 1));
+        const int page = page_of(p.c, p.r, w.seq(), j), b = p.c.page_log2 - 4;
+        w.cell = page < 0 ? -1 : ((page * p.c.KVH + w.kvh()) << b) + ((j >> 4) & ((1 << b) - 1));
         if (page < 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
         else { w.ks = __ldg(p.c.ks + w.cell); w.vs = __ldg(p.c.vs + w.cell); }
     }
@@ -851,7 +870,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         if (kNarrow && warp != kSplitWarps - 1) return;                    // two columns: the last warp's lanes
         unsigned char* qd = ps_raw + b * (Sh::QBytes + 32);
         const int col = kNarrow ? lane >> 4 : tid >> 4, cc = w.col0 + col, tok = w.it.len == 1 ? 0 : cc / p.G;
-        query_digits<DP>(p.q + (size_t)(w.it.a + tok) * p.ldq + (size_t)(w.it.kvh * p.G + cc - tok * p.G) * dh, col < w.cols, dh,
+        query_digits<DP>(p.q + (size_t)(w.it.a + tok) * p.ldq + (size_t)(w.kvh() * p.G + cc - tok * p.G) * dh, col < w.cols, dh,
                          tid & 15, [&](int e, int d, uint32_t x) {
                              // words of the part's 16-byte unit: x, y make step 0, z, w step 1
                              const int h = d >> 6, q = (d >> 4) & 3, word = (d >> 2) & 3;
@@ -1135,13 +1154,13 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
                 acc.x = ffma(x.x, e, acc.x); acc.y = ffma(x.y, e, acc.y);
                 acc.z = ffma(x.z, e, acc.z); acc.w = ffma(x.w, e, acc.w);
             }
-            const int row = cur.it.a + tok, h = cur.it.kvh * p.G + cc - tok * p.G;
+            const int row = cur.it.a + tok, h = cur.kvh() * p.G + cc - tok * p.G;
             if (splits == 1) {
                 const float inv = L == 0.0f ? 0.0f : fdiv(1.0f, L);
                 *reinterpret_cast<float4*>(p.out + (size_t)row * p.ldo + (size_t)h * dh + d) =
                     make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             } else {
-                float* pp = p.part + (((size_t)row * p.H + h) * p.nsplit + cur.it.split) * (dh + 4);
+                float* pp = few_part(p, cur.seq(), tok, row, h, cur.it.split);
                 *reinterpret_cast<float4*>(pp + d) = acc;
                 if (d == 0) { pp[dh] = M; pp[dh + 1] = L; }
             }
@@ -1478,7 +1497,7 @@ static __global__ void __launch_bounds__(128, 1) paged_attn_tile_kernel(const __
         if (it.split >= splits) continue;
         const int row = it.a + cc / p.G, h = it.kvh * p.G + cc % p.G;
         const float L = r ? l1 : l0, inv = splits > 1 ? 1.0f : L == 0.0f ? 0.0f : fdiv(1.0f, L);
-        float* dst = splits > 1 ? p.part + (((size_t)row * p.H + h) * p.nsplit + it.split) * (dh + 4)
+        float* dst = splits > 1 ? many_part(p, row, h, it.split)
                                 : p.out + (size_t)row * p.ldo + (size_t)h * dh;
 #pragma unroll
         for (int x = 0; x < Sh::NT; ++x) {
@@ -1922,7 +1941,7 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
             const int cc = row0 + r, tok = cc / p.G, ns = row_splits(p, pos0 + tok);
             const int orow = it.a + tok, h = it.kvh * p.G + cc - tok * p.G;
             if (it.split >= ns) continue;
-            float* dst = ns > 1 ? p.part + (((size_t)orow * p.H + h) * p.nsplit + it.split) * (dh + 4)
+            float* dst = ns > 1 ? many_part(p, orow, h, it.split)
                                 : p.out + (size_t)orow * p.ldo + (size_t)h * dh;
             if (4 * lane < dh) *reinterpret_cast<float4*>(dst + 4 * lane) = *reinterpret_cast<const float4*>(so + r * Sm::OutStride + 4 * lane);
             if (ns > 1 && lane < 2) dst[dh + lane] = lane ? xm[512 + r].y : xm[512 + r].x;
@@ -1949,12 +1968,14 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.c.dh;
     const int h = blockIdx.y * (8 / WPH) + warp / WPH, part = warp % WPH;
     after_previous();                                              // the splits are written
-    int n = 0, row = blockIdx.x;                                   // the row's splits, the same for the whole CTA
+    int n = 0, row = blockIdx.x, s = 0, tok = 0;                   // the row's splits, the same for the whole CTA
+    bool few = true;
     if (p.join_rows) {
-        const int i = blockIdx.x % p.join_rows;
-        const SeqRows q = seq_rows(p.r, blockIdx.x / p.join_rows);
-        row = q.a + i;
-        if (i < q.len && (long long)q.len * p.G <= p.few) n = splits_of(p.kc_few, min(q.pos0() + i + 1, p.r.cap));
+        s = blockIdx.x / p.join_rows;
+        tok = blockIdx.x % p.join_rows;
+        const SeqRows q = seq_rows(p.r, s);
+        row = q.a + tok;
+        if (tok < q.len && (long long)q.len * p.G <= p.few) n = splits_of(p.kc_few, min(q.pos0() + tok + 1, p.r.cap));
     } else {
         for (int base = 0; base < p.r.n_seq && n == 0; base += 32) {
             SeqRows q{0, 0, 0};
@@ -1962,14 +1983,16 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
             const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
             if (m) {
                 const int src = __ffs(m) - 1, pos = __shfl_sync(0xffffffffu, q.pos0() + row - q.a, src);
-                const long long cols = (long long)__shfl_sync(0xffffffffu, q.len, src) * p.G;
-                n = splits_of(cols <= p.few ? p.kc_few : p.kc_many, min(pos + 1, p.r.cap));
+                s = base + src;
+                tok = row - __shfl_sync(0xffffffffu, q.a, src);
+                few = (long long)__shfl_sync(0xffffffffu, q.len, src) * p.G <= p.few;
+                n = splits_of(few ? p.kc_few : p.kc_many, min(pos + 1, p.r.cap));
             }
         }
     }
     if (n < 2) return;
-    const int stride = dh + 4;
-    const float* base = p.part + ((size_t)row * p.H + min(h, p.H - 1)) * p.nsplit * stride;
+    const int stride = dh + 4, hc = min(h, p.H - 1);
+    const float* base = few ? few_part(p, s, tok, row, hc, 0) : many_part(p, row, hc, 0);
     float M = -INFINITY, L = 0.0f;
     float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     for (int s0 = part; s0 < n; s0 += 32 * WPH) {                  // 32 of this warp's splits at a time

@@ -765,3 +765,30 @@ def test_append_norms_without_an_eps(torch, rt, n, KVH, dh, single):
         # half a step of the scale, which is top / 127 up to f32, and what f32 did before the code was chosen
         close(torch, got[a:b], want[a:b], (0.5 * top / 127 * (1 + 1e-5)).expand(b - a, -1, dh) + turn_tol(want[a:b].abs(), dh))
     kv.check()
+
+
+@pytest.mark.parametrize("H,KVH,dh,rows,keys,cap,hint", [
+    (32, 8, 128, [1500, 1, 4, 0, 3], [1500, 6000, 4, 900, 20000], 1 << 17, 0),       # short sequences' rows in an area of their own
+    (8, 2, 64, [60, 1, 1, 4], [3000, 6000, 30, 1300], 0, 0),                       # both kinds split, rows numbered in their sequences
+    (4, 2, 128, [20, 1, 0, 1, 8], [2000, 6000, 3, 30, 1300], 0, 0),                # both kinds split, by the call's rows
+    (48, 2, 64, [3, 1, 40], [5000, 9000, 100], 0, 0), (4, 2, 256, [30, 1, 2], [700, 9000, 5000], 0, 0),
+    (16, 4, 128, [1] * 6, [9000, 1, 300, 5000, 513, 2], 0, 1), (8, 2, 80, [33], [9000], 0, 0)])
+def test_workspace_is_enough_and_read_only_where_written(torch, rt, H, KVH, dh, rows, keys, cap, hint):
+    """Just the bytes asked for, full of NaNs at the start: the outputs are right and nothing behind them is touched."""
+    kv, plan = pool(torch, rt, rows, keys, KVH, dh, 64, seed=6)
+    if cap:                                                        # a wide table: the capacity, not the keys, is large
+        wide = torch.full((len(rows), cap // 64), -1, dtype=torch.int32, device="cuda")
+        wide[:, :plan["page_table"].shape[1]] = plan["page_table"]
+        plan["page_table"] = wide
+    n = sum(rows)
+    q = torch.randn(n, H * dh, device="cuda") * dh ** -0.5
+    r = rt.KVRows(**plan, max_rows=hint)
+    need = rt.attn_paged_workspace(kv, r, H).numel()
+    assert need > 0
+    ws = torch.full((need + 4096,), 255, dtype=torch.uint8, device="cuda")
+    out = rt.attn_paged_i8(kv, r, q, workspace=ws[:need])
+    close(torch, out.reshape(n, H, dh), *attend64(torch, kv, plan, rows, keys, q, H))
+    assert bool((ws[need:] == 255).all())
+    with pytest.raises(rt.B2Error, match="workspace"):
+        rt.attn_paged_i8(kv, r, q, workspace=ws[:need - 16])
+    kv.check()

@@ -165,3 +165,17 @@ def test_long_prompts_over_a_large_capacity_are_accepted(pkg, n_rows, n_seq, cap
     kv = pages(rt, n_pages=1 << 14, page_size=64, n_kv_heads=KVH, d_head=128)
     assert attend(rt, kv, r, n_heads=H, ldq=H * 128, ldo=H * 128, ws=None, ws_bytes=0) == -1
     assert "workspace" in rt.last_error()
+
+
+@pytest.mark.parametrize("n_rows,n_seq,cap,H,KVH,dh,max_rows", [
+    (8188, 4, 2047, 32, 8, 128, 2047), (2048, 9, 1 << 15, 32, 8, 128, 0), (8192, 9, 1 << 17, 32, 8, 128, 0), (8192, 9, 1 << 17, 32, 32, 256, 0),
+    (5000, 3, 1 << 17, 64, 2, 64, 0), (40, 1, 1 << 20, 4, 1, 128, 0), (1, 1, 1 << 20, 128, 1, 256, 0), (100, 64, 1 << 15, 32, 8, 128, 0)])
+def test_workspace_holds_the_rows_that_have_splits(pkg, n_rows, n_seq, cap, H, KVH, dh, max_rows):
+    """Rows of short sequences (up to 16 columns of a KV head) in splits of 512 keys, and of the others as many as fill
+    the GPU a few times (118 MB): not every row of the call in the finer splits."""
+    rt = pkg.runtime
+    r = rows(rt, n_rows=n_rows, n_seq=n_seq, max_pages=-(-cap // 64), max_keys=cap, max_rows=max_rows)
+    kv = pages(rt, n_pages=1 << 14, page_size=64, n_kv_heads=KVH, d_head=dh)
+    got = rt.lib().b2_attn_paged_i8_workspace(C.addressof(kv), C.addressof(r), H)
+    short = min(n_rows, n_seq * (16 // (H // KVH))) if n_seq > 1 else 0
+    assert got % 16 == 0 and got <= short * H * -(-cap // 512) * (dh + 4) * 4 + 118_000_000
