@@ -114,8 +114,10 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
 }
 
 // A call's sequences are of two kinds, by their columns (token, head) of a KV head, and
-// each kind has a launch (one that finds none of its kind ends at once, in about 2 us; it
-// is left out where the caller's sizes say so). A whole batch on one kernel cost more: a
+// each kind has a launch, left out where the caller's sizes say that none is of its kind.
+// (One that finds none costs a wave of empty CTAs, 2.4 us, for every 148 that its rows might
+// have needed: with max_rows = 1 a step of 64 tokens over 1152 keys takes 119 us for 32 / 32
+// heads of 128, without it 152 us; 256 tokens, 32 / 4 heads of 64: 66 and 105 us.) A whole batch on one kernel cost more: a
 // single token in a 128-row tile as much as 128, a prompt in 8-column tiles re-reads its
 // keys 16 times as often.
 //  few, up to 16 columns: 8 a CTA, or 2 where single tokens make no more (decode without
@@ -161,12 +163,16 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
         return tiles * p.c.KVH * splits_at(kc_log2);
     };
     // tiles of `cols` columns over all sequences: at most one partly filled one each
-    auto tiles_of = [&](int cols) { return (long long)p.r.n_rows * p.G / cols + p.r.n_seq; };
-    // beside many-row sequences those of the few-row kind have up to kFewCols columns each, whatever n_rows is
-    const long long few_tiles = a.many ? std::min(tiles_of(a.few_cols), (long long)p.r.n_seq * ((kFewCols + a.few_cols - 1) / a.few_cols))
-                                       : tiles_of(a.few_cols);
+    auto tiles_of = [&](int cols) { return (long long)p.r.n_rows * p.G / cols + std::min(p.r.n_seq, p.r.n_rows); };
+    long long few_tiles = tiles_of(a.few_cols), many_tiles = tiles_of(a.many_cols);
+    if (a.few && a.many) {
+        // sequences of the few-row kind have up to kFewCols columns each, whatever n_rows is; the others have more, so
+        // a tile has at least kFewCols + 1
+        few_tiles = std::min(few_tiles, (long long)p.r.n_seq * ((kFewCols + a.few_cols - 1) / a.few_cols));
+        many_tiles = std::min(many_tiles, (long long)p.r.n_rows * p.G / (kFewCols + 1));
+    }
     a.few_items = a.few ? items(few_tiles, p.kc_few) : 0;
-    a.many_items = a.many ? items(tiles_of(a.many_cols), p.kc_many) : 0;
+    a.many_items = a.many ? items(many_tiles, p.kc_many) : 0;
     return a;
 }
 

@@ -179,3 +179,12 @@ def test_workspace_holds_the_rows_that_have_splits(pkg, n_rows, n_seq, cap, H, K
     got = rt.lib().b2_attn_paged_i8_workspace(C.addressof(kv), C.addressof(r), H)
     short = min(n_rows, n_seq * (16 // (H // KVH))) if n_seq > 1 else 0
     assert got % 16 == 0 and got <= short * H * -(-cap // 512) * (dh + 4) * 4 + 118_000_000
+
+
+def test_a_few_rows_of_many_slots_are_accepted(pkg):
+    """Seventeen single tokens of 16384 slots over a large capacity: sequences without rows are no pieces."""
+    rt = pkg.runtime
+    r = rows(rt, n_rows=17, n_seq=16384, max_pages=(1 << 20) // 64)
+    kv = pages(rt, n_pages=1 << 14, page_size=64, n_kv_heads=32, d_head=128)
+    assert attend(rt, kv, r, n_heads=32, ldq=4096, ldo=4096, ws=None, ws_bytes=0) == -1
+    assert "workspace" in rt.last_error()
