@@ -117,7 +117,7 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
 // each kind has a launch, left out where the caller's sizes say that none is of its kind.
 // (One that finds none costs a wave of empty CTAs, 2.4 us, for every 148 that its rows might
 // have needed: with max_rows = 1 a step of 64 tokens over 1152 keys takes 119 us for 32 / 32
-// heads of 128, without it 152 us; 256 tokens, 32 / 4 heads of 64: 66 and 105 us.) A whole batch on one kernel cost more: a
+// heads of 128, without it 125 us; 256 tokens, 32 / 4 heads of 64: 66 and 105 us.) A whole batch on one kernel cost more: a
 // single token in a 128-row tile as much as 128, a prompt in 8-column tiles re-reads its
 // keys 16 times as often.
 //  few, up to 16 columns: 8 a CTA, or 2 where single tokens make no more (decode without
@@ -211,7 +211,10 @@ cudaError_t launch_few(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::Smem);
     if (e != cudaSuccess) return e;
     const long long resident = (long long)sm_count() * (DP == 256 ? 2 : DP == 128 ? 3 : 4);
-    return launch_ex(k, dim3((unsigned)std::min(a.few_items, resident)), dim3(kSplitWarps * 32), Sh::Smem, s, true, p);
+    // Behind the many-row kernel not before its end: CTAs that come up while the SM is set for
+    // that kernel's shared memory keep its small L1 (64 tokens, 32 / 32 heads of 128, 1152
+    // keys: 152 us, now 125; 60 tokens beside a prompt of 1000: 224, now 196).
+    return launch_ex(k, dim3((unsigned)std::min(a.few_items, resident)), dim3(kSplitWarps * 32), Sh::Smem, s, !a.many, p);
 }
 
 cudaError_t launch_many(const PagedAttnParams& p, const AttnPlan& a, cudaStream_t s) {
