@@ -545,10 +545,14 @@ class PagedKV:
         return cls(*code, *scale)
 
     def check(self):
-        """Waits for the device, and raises if a call on this cache met bad rows or pages (which it left out)."""
+        """Waits for the device (calls on all its streams), and raises if a call on this cache met bad rows or pages
+        (which it left out)."""
+        import torch
+        torch.cuda.synchronize(self.gpu)
         e = int(self.err.item())
         if e:
             self.err.zero_()
+            torch.cuda.synchronize(self.gpu)             # cleared before the next call on any stream
             raise B2Error(-8, ROWS_ERRORS.get(e, f"device error {e}"))
 
 

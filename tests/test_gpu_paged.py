@@ -834,3 +834,22 @@ def test_single_tokens_behind_the_launch_for_longer_sequences(torch, rt, heads, 
     do not suffer from that kernel's use of the SM (152 against 119 us, with d_head 256 169 against 128)."""
     hint, none = (decode_step_us(torch, rt, 64, 1152, heads, heads, dh, x) for x in (1, 0))
     assert none < 1.17 * hint
+
+
+def test_check_waits_for_calls_on_other_streams(torch, rt):
+    """A bad page met by a call that still waits on a side stream is reported, and once."""
+    kv, plan = pool(torch, rt, [1], [40], 2, 64, 16)
+    plan["page_table"][0, 1] = -1
+    r = rt.KVRows(**plan)
+    q = torch.randn(1, 2 * 64, device="cuda")
+    rt.attn_paged_i8(kv, r, q)                                     # (an earlier report, to be cleared)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)                         # 0.1 s or so
+        rt.attn_paged_i8(kv, r, q, stream=side.cuda_stream)
+        with pytest.raises(rt.B2Error, match="page-table entry"):
+            kv.check()
+        assert side.query()
+        kv.check()
