@@ -20,7 +20,7 @@ enum : int {
     B2_DEV_ERR_KV_OVERFLOW = 2,
     B2_DEV_ERR_BAD_TOKEN = 3,
     B2_DEV_ERR_BAD_PAGE = 4,       // page table entry outside the pool
-    B2_DEV_ERR_BAD_ROWS = 5,       // row ranges that overlap
+    B2_DEV_ERR_BAD_ROWS = 5,       // a row range that starts below the one before it
 };
 
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s per wait

@@ -68,9 +68,9 @@ struct BlockRun {
 };
 
 // Run number `item` of the call, found by one warp: lanes count the runs of 32
-// sequences at a time. `most` = runs the grid covers (more than that only if the
-// row ranges overlap).
-__device__ __forceinline__ BlockRun find_run(const PagedRows& r, int item, int most, int* err, int lane) {
+// sequences at a time. Run 0 also checks all row ranges: only where a start is below the
+// one before it can two overlap (and their runs be more than the grid covers).
+__device__ __forceinline__ BlockRun find_run(const PagedRows& r, int item, int* err, int lane) {
     BlockRun out{-1, 0, 0, 0};
     int before = 0;
     bool found = false;
@@ -82,7 +82,10 @@ __device__ __forceinline__ BlockRun find_run(const PagedRows& r, int item, int m
             q = seq_rows(r, s);
             first = max(q.pos0(), 0);
             const int last = min(q.kv, r.cap) - 1;
-            if (q.len > 0 && q.kv > r.cap && item == 0) set_err(err, B2_DEV_ERR_KV_OVERFLOW);
+            if (item == 0) {
+                if (__ldg(r.row_start + s + 1) < __ldg(r.row_start + s)) set_err(err, B2_DEV_ERR_BAD_ROWS);
+                if (q.len > 0 && q.kv > r.cap) set_err(err, B2_DEV_ERR_KV_OVERFLOW);
+            }
             if (q.len > 0 && last >= first) nb = last / kKvBlock - first / kKvBlock + 1;
         }
         int incl = nb;
@@ -108,7 +111,6 @@ __device__ __forceinline__ BlockRun find_run(const PagedRows& r, int item, int m
         }
         before += total;
     }
-    if (item == 0 && before > most && lane == 0) set_err(err, B2_DEV_ERR_BAD_ROWS);
     return out;
 }
 
@@ -376,7 +378,7 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
 
 // the run of this CTA without the rows that lie past the table (they have no rotation)
 __device__ __forceinline__ BlockRun run_in_table(const AppendParams& p, int lane) {
-    BlockRun run = find_run(p.r, blockIdx.x, p.items, p.err, lane);
+    BlockRun run = find_run(p.r, blockIdx.x, p.err, lane);
     if (run.s >= 0 && p.nr.table && run.pos + run.n > p.nr.table_rows) {
         if (lane == 0) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
         run.n = max(p.nr.table_rows - run.pos, 0);
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
     after_previous();
     constexpr int RPP = 32 / LPR, NP = kKvBlock / RPP;         // rows a pass, passes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const BlockRun run = find_run(p.r, blockIdx.x, p.items, p.err, lane);
+    const BlockRun run = find_run(p.r, blockIdx.x, p.err, lane);
     if (run.s < 0) return;
     const int task = blockIdx.y * 8 + warp;
     if (task >= 2 * p.c.KVH) return;

@@ -454,7 +454,7 @@ def attn_decode_static(q, K, V, n_heads, n_kv_heads, d_head, n, max_seq, stream=
 # ----------------------------------------------------------------- paged 8-bit KV cache
 KV_BLOCK = 16                    # tokens that share a scale (B2_KV_BLOCK)
 ROWS_ERRORS = {2: "a position past the sequence's capacity or the rotation table",
-               4: "a page-table entry outside the pool", 5: "row ranges that overlap"}
+               4: "a page-table entry outside the pool", 5: "a row_start below the one before it: row ranges that may overlap"}
 
 
 class _KvPages(C.Structure):     # b2_kv_pages

@@ -278,8 +278,9 @@ int b2_attn_decode_static(const float* q, const float* K, const float* V, float*
  *   B2_ROWS_OVERFLOW  a position at or past the sequence's capacity (the smaller of
  *                     max_keys and max_pages * page_size), or past the table
  *   B2_ROWS_BAD_PAGE  a page-table entry outside [0, n_pages)
- *   B2_ROWS_OVERLAP   row ranges that overlap (append and read; attention then leaves
- *                     some rows out)
+ *   B2_ROWS_OVERLAP   a row_start below the one before it, so that row ranges may overlap
+ *                     (append and read look for it; rows in two ranges then go to both
+ *                     sequences, their outputs are one's or the other's, or are left out)
  * d_head: a multiple of 16 from 16 to 256. f32 rows: 16-byte aligned, row strides in
  * elements, a multiple of 4. Calls on one cache must be ordered by the caller. */
 #define B2_KV_BLOCK 16

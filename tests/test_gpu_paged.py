@@ -853,3 +853,23 @@ def test_check_waits_for_calls_on_other_streams(torch, rt):
             kv.check()
         assert side.query()
         kv.check()
+
+
+@pytest.mark.parametrize("start,bad", [([0, 12, 0, 12], True), ([0, 4, 2, 12], True), ([4, 2, 2, 12], True), ([0, 4, 8, 12], False),
+                                       ([3, 3, 3, 3], False), ([-5, 4, 8, 900], False), ([0] * 40 + [6] + [5] * 2, True)])
+def test_row_ranges_that_may_overlap_are_reported(torch, rt, start, bad):
+    """By append and by read, wherever a start is below the one before it; other odd starts are no error."""
+    n = len(start) - 1
+    kv = rt.PagedKV.empty(n, 16, 1, 32)
+    plan = dict(row_start=torch.tensor(start, dtype=torch.int32, device="cuda"), n_rows=12,
+                kv_len=torch.full((n,), 16, dtype=torch.int32, device="cuda"),
+                page_table=torch.arange(n, dtype=torch.int32, device="cuda")[:, None].contiguous())
+    x = torch.randn(12, 32, device="cuda")
+    for hint in (0, 1):
+        r = rt.KVRows(**plan, max_rows=hint)
+        for call in (lambda: rt.kv_append_i8(kv, r, x, x), lambda: rt.kv_read_i8(kv, r)):
+            call()
+            if bad:
+                with pytest.raises(rt.B2Error, match="overlap"):
+                    kv.check()
+            kv.check()
