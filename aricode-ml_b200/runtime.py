@@ -453,7 +453,8 @@ def attn_decode_static(q, K, V, n_heads, n_kv_heads, d_head, n, max_seq, stream=
 
 # ----------------------------------------------------------------- paged 8-bit KV cache
 KV_BLOCK = 16                    # tokens that share a scale (B2_KV_BLOCK)
-ROWS_ERRORS = {2: "a position past the sequence's capacity or the rotation table",
+ROWS_ERRORS = {1: "a wait inside the attention kernel ran out: that call's outputs are unusable",
+               2: "a position past the sequence's capacity or the rotation table",
                4: "a page-table entry outside the pool", 5: "a row_start below the one before it: row ranges that may overlap"}
 
 
@@ -546,7 +547,7 @@ class PagedKV:
 
     def check(self):
         """Waits for the device (calls on all its streams), and raises if a call on this cache met bad rows or pages
-        (which it left out)."""
+        (which it left out), or an attention kernel gave up a wait."""
         import torch
         torch.cuda.synchronize(self.gpu)
         e = int(self.err.item())

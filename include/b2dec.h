@@ -275,6 +275,8 @@ int b2_attn_decode_static(const float* q, const float* K, const float* V, float*
  * The calls read lengths, row ranges and pages on the device only, so a captured
  * launch replays with new ones. What they find wrong there they leave out, and set
  * *err (device int32, optional, first error kept; the caller zeroes it):
+ *   B2_ROWS_TIMEOUT   attention alone: a wait inside a kernel ran out after a second; the
+ *                     call's outputs are unusable (the cache is only read)
  *   B2_ROWS_OVERFLOW  a position at or past the sequence's capacity (the smaller of
  *                     max_keys and max_pages * page_size), or past the table
  *   B2_ROWS_BAD_PAGE  a page-table entry outside [0, n_pages)
@@ -284,7 +286,7 @@ int b2_attn_decode_static(const float* q, const float* K, const float* V, float*
  * d_head: a multiple of 16 from 16 to 256. f32 rows: 16-byte aligned, row strides in
  * elements, a multiple of 4. Calls on one cache must be ordered by the caller. */
 #define B2_KV_BLOCK 16
-enum { B2_ROWS_OVERFLOW = 2, B2_ROWS_BAD_PAGE = 4, B2_ROWS_OVERLAP = 5 };
+enum { B2_ROWS_TIMEOUT = 1, B2_ROWS_OVERFLOW = 2, B2_ROWS_BAD_PAGE = 4, B2_ROWS_OVERLAP = 5 };
 
 typedef struct b2_kv_pages {
     int8_t* k;               /* [n_pages][n_kv_heads][page_size][d_head], 16-byte aligned */

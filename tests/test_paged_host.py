@@ -188,3 +188,14 @@ def test_a_few_rows_of_many_slots_are_accepted(pkg):
     kv = pages(rt, n_pages=1 << 14, page_size=64, n_kv_heads=32, d_head=128)
     assert attend(rt, kv, r, n_heads=32, ldq=4096, ldo=4096, ws=None, ws_bytes=0) == -1
     assert "workspace" in rt.last_error()
+
+
+def test_every_device_error_has_a_name_and_a_text(pkg):
+    """The codes that the paged kernels set (paged.cuh) are named with the same values in the header, and check() has a
+    text for each."""
+    import re
+    csrc = ROOT / "aricode-ml_b200" / "csrc"
+    code = dict(re.findall(r"(B2_DEV_ERR_\w+) = (\d+)", (csrc / "b2_common.cuh").read_text()))
+    used = {int(code[n]) for n in re.findall(r"set_err\([^;]*?(B2_DEV_ERR_\w+)\)", (csrc / "paged.cuh").read_text())}
+    named = {int(v) for v in re.findall(r"B2_ROWS_\w+ = (\d+)", (ROOT / "include" / "b2dec.h").read_text())}
+    assert used == named == set(pkg.runtime.ROWS_ERRORS) and len(used) >= 4
