@@ -40,24 +40,40 @@ struct SeqRows {
 
 __device__ __forceinline__ SeqRows seq_rows(const PagedRows& r, int s) {
     SeqRows q;
-    q.a = min(max(__ldg(r.row_start + s), 0), r.n_rows);
-    q.len = min(max(__ldg(r.row_start + s + 1), q.a), r.n_rows) - q.a;
-    q.kv = max(__ldg(r.kv_len + s), 0);
+    q.a = min(max(r.row_start[s], 0), r.n_rows);
+    q.len = min(max(r.row_start[s + 1], q.a), r.n_rows) - q.a;
+    q.kv = max(r.kv_len[s], 0);
     return q;
 }
 
 // page of position pos of sequence s, or -1
 __device__ __forceinline__ int page_of(const PagedKv& c, const PagedRows& r, int s, int pos) {
-    const int id = __ldg(r.table + (size_t)s * r.max_pages + (pos >> c.page_log2));
+    const int id = r.table[(size_t)s * r.max_pages + (pos >> c.page_log2)];
     return (unsigned)id < (unsigned)c.n_pages ? id : -1;
 }
 
 // Start of every kernel here: they are launched with programmatic serialisation, so that
 // a launch comes up while the one before it drains, and read nothing before that is
-// complete.
+// complete. The launch before it may have written what they read (rows, lengths, pages,
+// codes, scales), within this one's lifetime: such loads are plain ones, which stay behind
+// the wait; read-only loads (__ldg) are for gains and rotation tables alone. (Same times.)
 __device__ __forceinline__ void after_previous() {
     pdl_launch_dependents();
     pdl_wait();
+}
+
+// Plain loads too, free to move among the shared-memory stores around them but not before
+// the wait (the split kernel's codes: as C++ loads they cost <64, 8> 52 bytes of spills and
+// 3 % of attend-long).
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
 }
 
 // A run: the rows of one sequence that lie in one block of 16 tokens.
@@ -83,7 +99,7 @@ __device__ __forceinline__ BlockRun find_run(const PagedRows& r, int item, int* 
             first = max(q.pos0(), 0);
             const int last = min(q.kv, r.cap) - 1;
             if (item == 0) {
-                if (__ldg(r.row_start + s + 1) < __ldg(r.row_start + s)) set_err(err, B2_DEV_ERR_BAD_ROWS);
+                if (r.row_start[s + 1] < r.row_start[s]) set_err(err, B2_DEV_ERR_BAD_ROWS);
                 if (q.len > 0 && q.kv > r.cap) set_err(err, B2_DEV_ERR_KV_OVERFLOW);
             }
             if (q.len > 0 && last >= first) nb = last / kKvBlock - first / kKvBlock + 1;
@@ -221,7 +237,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
     bool live = row < (unsigned)p.n_rows;
     int pos = 0;
     if (live && p.pos) {
-        pos = __ldg(p.pos + row);
+        pos = p.pos[row];
         if (pos < 0) live = false;
         else if (p.table && pos >= p.table_rows) {
             live = false;
@@ -271,7 +287,7 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
 #pragma unroll
             for (int e = 0; e < VPL; ++e) {
                 const int d = 4 * (gl + LPH * e);
-                x[j][e] = (i < run.n && d < dh) ? __ldg(reinterpret_cast<const float4*>(src + (size_t)(run.row + i) * ld + d))
+                x[j][e] = (i < run.n && d < dh) ? *reinterpret_cast<const float4*>(src + (size_t)(run.row + i) * ld + d)
                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
@@ -479,13 +495,13 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
     if (page < 0 && lane == 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
     const int psz = 1 << p.c.page_log2;
     const size_t cell = ((size_t)max(page, 0) * p.c.KVH + head) * (psz / kKvBlock) + (run.pos & (psz - 1)) / kKvBlock;
-    const float s = page < 0 ? 0.0f : __ldg((is_k ? p.c.ks : p.c.vs) + cell);
+    const float s = page < 0 ? 0.0f : (is_k ? p.c.ks : p.c.vs)[cell];
     const int8_t* codes = (is_k ? p.c.k : p.c.v) + (cell * kKvBlock + run.pos % kKvBlock) * dh + d;
     uint2 w[NP];
 #pragma unroll
     for (int x = 0; x < NP; ++x) {
         const int r = x * RPP + r0;
-        w[x] = page >= 0 && r < run.n && d < dh ? __ldg(reinterpret_cast<const uint2*>(codes + r * dh)) : make_uint2(0u, 0u);
+        w[x] = page >= 0 && r < run.n && d < dh ? *reinterpret_cast<const uint2*>(codes + r * dh) : make_uint2(0u, 0u);
     }
     const size_t at = (size_t)run.row * p.ld + (size_t)head * dh + d;
 #pragma unroll
@@ -726,7 +742,7 @@ __device__ __forceinline__ void query_digits(const float* qr, bool live, int dh,
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
         const int d = 4 * (l16 + 16 * i);
-        x[i] = (live && d < dh) ? __ldg(reinterpret_cast<const float4*>(qr + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i] = (live && d < dh) ? *reinterpret_cast<const float4*>(qr + d) : make_float4(0.f, 0.f, 0.f, 0.f);
         bad |= x[i].x != x[i].x || x[i].y != x[i].y || x[i].z != x[i].z || x[i].w != x[i].w;
         top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
     }
@@ -806,7 +822,7 @@ __device__ __forceinline__ SplitItem next_split_item(const PagedAttnParams& p, u
         const int page = page_of(p.c, p.r, w.seq(), j), b = p.c.page_log2 - 4;
         w.cell = page < 0 ? -1 : ((page * p.c.KVH + w.kvh()) << b) + ((j >> 4) & ((1 << b) - 1));
         if (page < 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
-        else { w.ks = __ldg(p.c.ks + w.cell); w.vs = __ldg(p.c.vs + w.cell); }
+        else { w.ks = p.c.ks[w.cell]; w.vs = p.c.vs[w.cell]; }
     }
     return w;
 }
@@ -843,7 +859,7 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
         for (int x = 0; x < 4; ++x) {
             const int8_t* kr = p.c.k + ((long long)(x < 2 ? c0 : c1) * kKvBlock + 8 * (x & 1) + g) * dh;
 #pragma unroll
-            for (int h = 0; h < Sh::NH; ++h) kf[x][h] = __ldg(reinterpret_cast<const uint4*>(kr + kd[h]));
+            for (int h = 0; h < Sh::NH; ++h) kf[x][h] = load16(kr + kd[h]);
         }
     };
     auto load_values = [&](int c0, int c1) {
@@ -855,12 +871,12 @@ paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p) {
             for (int i = 0; i < 4; ++i) {
                 const int8_t* v = vr + (kNarrow ? i : (i & 1) + 8 * (i >> 1)) * dh;
                 if constexpr (Sh::VW == 2) {
-                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(v + vd[0]));
+                    const uint2 x = load8(v + vd[0]);
                     vf[b][i][0] = x.x; vf[b][i][1] = x.y;
                 } else {
 #pragma unroll
                     for (int u = 0; u < Sh::VW / 4; ++u) {
-                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(v + vd[u]));
+                        const uint4 x = load16(v + vd[u]);
                         vf[b][i][4 * u] = x.x; vf[b][i][4 * u + 1] = x.y; vf[b][i][4 * u + 2] = x.z; vf[b][i][4 * u + 3] = x.w;
                     }
                 }
@@ -1262,7 +1278,7 @@ static __global__ void __launch_bounds__(128, 1) paged_attn_tile_kernel(const __
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (tid < 2 * NB) {
             const long long cb = cell[NB * b + tid % NB];
-            sc[3 * NB * b + tid] = cb >= 0 ? __ldg((tid < NB ? p.c.ks : p.c.vs) + cb) : 0.0f;
+            sc[3 * NB * b + tid] = cb >= 0 ? (tid < NB ? p.c.ks : p.c.vs)[cb] : 0.0f;
             if (tid < NB) sc[3 * NB * b + 2 * NB + tid] = cb >= 0 ? 1.0f : 0.0f;
             if (cb == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
         }
@@ -1281,7 +1297,7 @@ static __global__ void __launch_bounds__(128, 1) paged_attn_tile_kernel(const __
             const int d = d0 + 16 * x < dh ? d0 + 16 * x : 0;
             const int8_t* src = p.c.v + (max(at, 0ll) * kKvBlock + vq2) * dh + d;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) vr[x][k] = __ldg(reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh));
+            for (int k = 0; k < 4; ++k) vr[x][k] = *reinterpret_cast<const uint4*>(src + ((k >> 1) * 8 + (k & 1)) * dh);
         }
     };
     auto store_values = [&](int i) {
@@ -1723,13 +1739,13 @@ static __global__ void __launch_bounds__(kMmaThreads, 1) paged_attn_mma_kernel(c
                 for (int x = 0; x < 3; ++x) {
                     const int d = 16 * (cw + 3 * x) < dh ? 16 * (cw + 3 * x) : 0;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) vr[x][k] = __ldg(reinterpret_cast<const uint4*>(src + k * dh + d));
+                    for (int k = 0; k < 4; ++k) vr[x][k] = *reinterpret_cast<const uint4*>(src + k * dh + d);
                 }
             }
             if (ct < 8) {
                 float* s = sc + (i & 3) * 24 + ct;
-                s[0] = cell >= 0 ? __ldg(p.c.ks + cell) : 0.0f;
-                s[8] = cell >= 0 ? __ldg(p.c.vs + cell) : 0.0f;
+                s[0] = cell >= 0 ? p.c.ks[cell] : 0.0f;
+                s[8] = cell >= 0 ? p.c.vs[cell] : 0.0f;
                 s[16] = cell >= 0 ? 1.0f : 0.0f;
                 if (cell == -1) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
             }

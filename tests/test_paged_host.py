@@ -199,3 +199,14 @@ def test_every_device_error_has_a_name_and_a_text(pkg):
     used = {int(code[n]) for n in re.findall(r"set_err\([^;]*?(B2_DEV_ERR_\w+)\)", (csrc / "paged.cuh").read_text())}
     named = {int(v) for v in re.findall(r"B2_ROWS_\w+ = (\d+)", (ROOT / "include" / "b2dec.h").read_text())}
     assert used == named == set(pkg.runtime.ROWS_ERRORS) and len(used) >= 4
+
+
+def test_read_only_loads_are_of_constants_alone():
+    """The paged kernels start while the launch before them runs, and read-only loads want data that nothing writes in a
+    kernel's lifetime: only gains and rotation tables are read that way, not what a launch may have written."""
+    import re
+    src = (ROOT / "aricode-ml_b200" / "csrc" / "paged.cuh").read_text().replace("(__ldg)", "")
+    loads = [src[m.end():m.end() + 60] for m in re.finditer(r"__ldg\(", src)]
+    assert loads
+    for arg in loads:
+        assert re.match(r"reinterpret_cast<const float4\*>\((p\.table|p\.nr\.table|p\.nr\.gk|g) \+", arg), arg
