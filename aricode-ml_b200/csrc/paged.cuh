@@ -668,7 +668,7 @@ __device__ __forceinline__ int splits_of(int kc_log2, int n) { return max((n + (
 constexpr int kMaxItems = 1 << 26;
 
 // Item number `item` of the call (tiles of NC rows), found by one warp. OneWord: s becomes
-// sequence * 1024 + KV head (up to 2^20 and 1024 of them) and kvh stays 0, for the split
+// sequence * 1024 + KV head (up to 2^16 and 2^10 of them) and kvh stays 0, for the split
 // kernel, which has no register left for both.
 template <int NC, bool OneWord = false>
 __device__ __forceinline__ AttnItem find_item(const PagedAttnParams& p, unsigned item, int lane) {

@@ -308,7 +308,7 @@ typedef struct b2_kv_rows {
     const int32_t* row_start;   /* device [n_seq + 1], not decreasing */
     const int32_t* kv_len;      /* device [n_seq] */
     const int32_t* page_table;  /* device [n_seq][max_pages] */
-    int32_t n_seq;
+    int32_t n_seq;              /* up to 65536; calls of more than a few thousand are slow */
     int32_t max_pages;
     int32_t n_rows;             /* rows of the buffers */
     int32_t max_keys;           /* no kv_len is larger (0: max_pages * page_size) */

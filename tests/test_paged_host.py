@@ -210,3 +210,13 @@ def test_read_only_loads_are_of_constants_alone():
     assert loads
     for arg in loads:
         assert re.match(r"reinterpret_cast<const float4\*>\((p\.table|p\.nr\.table|p\.nr\.gk|g) \+", arg), arg
+
+
+def test_more_sequences_than_a_call_can_search_are_refused(pkg):
+    """A call's time grows with the square of its sequences: 0.4 s at the limit, minutes at a million."""
+    rt = pkg.runtime
+    for n_seq in (65537, 1 << 20):
+        for call in (append, read, attend):
+            assert call(rt, pages(rt), rows(rt, n_seq=n_seq)) == -1 and "65536" in rt.last_error()
+    assert attend(rt, pages(rt), rows(rt, n_seq=65536, n_rows=200, max_pages=100), ws=None, ws_bytes=0) == -1
+    assert "workspace" in rt.last_error()
