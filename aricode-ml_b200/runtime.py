@@ -542,7 +542,7 @@ class PagedKV:
         import torch
         shape = (n_pages, n_kv_heads, page_size)
         code = [torch.zeros(*shape, d_head, dtype=torch.int8, device=device) for _ in range(2)]
-        scale = [torch.zeros(n_pages, n_kv_heads, page_size // KV_BLOCK, device=device) for _ in range(2)]
+        scale = [torch.zeros(n_pages, n_kv_heads, page_size // KV_BLOCK, dtype=torch.float32, device=device) for _ in range(2)]
         return cls(*code, *scale)
 
     def check(self):
@@ -605,7 +605,7 @@ def qk_norm_rope(q, k, d_head, pos=None, table=None, q_gain=None, k_gain=None, e
         if w != H * d_head:
             raise _invalid("q must hold whole heads")
         qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
-        q_out = torch.empty(n, w, device=q.device) if q_out is None else q_out
+        q_out = torch.empty(n, w, dtype=f32, device=q.device) if q_out is None else q_out
         qop, ldqo = _f32_rows("q_out", q_out, f32, gpu, n, w)
     if k is not None:
         w = k.shape[-1]
@@ -613,7 +613,7 @@ def qk_norm_rope(q, k, d_head, pos=None, table=None, q_gain=None, k_gain=None, e
         if w != K * d_head or k.shape[0] != n:
             raise _invalid("k must hold whole heads, and as many rows as q")
         kp, ldk = _f32_rows("k", k, f32, gpu, n, w)
-        k_out = torch.empty(n, w, device=k.device) if k_out is None else k_out
+        k_out = torch.empty(n, w, dtype=f32, device=k.device) if k_out is None else k_out
         kop, ldko = _f32_rows("k_out", k_out, f32, gpu, n, w)
     if table is not None:
         if pos is None or table.dim() != 2:
@@ -653,7 +653,7 @@ def kv_append_i8(kv, rows, k, v, table=None, k_gain=None, eps=1e-5, q=None, q_ga
         if w != H * d:
             raise _invalid("q must hold whole heads")
         qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
-        q_out = torch.empty(q.shape[0], w, device=q.device) if q_out is None else q_out
+        q_out = torch.empty(q.shape[0], w, dtype=f32, device=q.device) if q_out is None else q_out
         qop, ldqo = _f32_rows("q_out", q_out, f32, gpu, n, w)
     if table is not None:
         if table.dim() != 2:
@@ -719,7 +719,7 @@ def attn_paged_i8(kv, rows, q, out=None, workspace=None, stream=None):
     if w != H * kv.d_head:
         raise _invalid("q must hold whole heads")
     qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
-    out = torch.empty(q.shape[0], w, device=q.device) if out is None else out
+    out = torch.empty(q.shape[0], w, dtype=f32, device=q.device) if out is None else out
     op, ldo = _f32_rows("out", out, f32, gpu, n, w)
     if workspace is None:
         workspace = attn_paged_workspace(kv, rows, H)

@@ -873,3 +873,18 @@ def test_row_ranges_that_may_overlap_are_reported(torch, rt, start, bad):
                 with pytest.raises(rt.B2Error, match="overlap"):
                     kv.check()
             kv.check()
+
+
+def test_outputs_do_not_follow_the_default_dtype(torch, rt):
+    """A serving program's default dtype is often bfloat16: caches and outputs that the calls make are f32 all the same."""
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    plan = ragged(torch, [3], [3], table)
+    q, k = (torch.randn(3, w, device="cuda") for w in (128, 64))
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        kv, r = rt.PagedKV.empty(1, 16, 1, 64), rt.KVRows(**plan)
+        made = [kv.k_scale, *rt.qk_norm_rope(q, k, 64), rt.kv_append_i8(kv, r, k, k, q=q), rt.attn_paged_i8(kv, r, q), *rt.kv_read_i8(kv, r)]
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(x.dtype is torch.float32 for x in made)
+    kv.check()
