@@ -452,6 +452,7 @@ def attn_decode_static(q, K, V, n_heads, n_kv_heads, d_head, n, max_seq, stream=
 
 
 # ----------------------------------------------------------------- paged 8-bit KV cache
+INT32_MAX = 2 ** 31 - 1          # of the structs' fields, which would wrap around
 KV_BLOCK = 16                    # tokens that share a scale (B2_KV_BLOCK)
 ROWS_ERRORS = {1: "a wait inside the attention kernel ran out: that call's outputs are unusable",
                2: "a position past the sequence's capacity or the rotation table",
@@ -572,12 +573,12 @@ class KVRows:
         n = kv_len.shape[0]
         _tensor("row_start", row_start, torch.int32, self.gpu, (n + 1,))
         _tensor("page_table", page_table, torch.int32, self.gpu, (n, page_table.shape[1]))
-        if n_rows < 0 or max_keys < 0 or max_rows < 0:
-            raise _invalid("n_rows, max_keys and max_rows must not be negative")
+        if not 0 <= n_rows <= INT32_MAX or max_keys < 0 or max_rows < 0:
+            raise _invalid("n_rows must be 0 to 2^31 - 1, max_keys and max_rows not negative")
         self.row_start, self.kv_len, self.page_table = row_start, kv_len, page_table
         self.n_rows = int(n_rows)
         self._c = _KvRows(row_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), n, page_table.shape[1],
-                          self.n_rows, int(max_keys), int(max_rows))
+                          self.n_rows, min(int(max_keys), INT32_MAX), min(int(max_rows), INT32_MAX))
         self._p = C.addressof(self._c)
 
 

@@ -888,3 +888,17 @@ def test_outputs_do_not_follow_the_default_dtype(torch, rt):
         torch.set_default_dtype(torch.float32)
     assert all(x.dtype is torch.float32 for x in made)
     kv.check()
+
+
+def test_bounds_beyond_32_bits(torch, rt):
+    """A max_keys or max_rows above 2^31 bounds nothing and does not wrap around; such an n_rows is refused."""
+    rows, keys = [2], [40]
+    kv, plan = pool(torch, rt, rows, keys, 2, 64, 16)
+    q = torch.randn(2, 4 * 64, device="cuda") * 0.1
+    want, tol = attend64(torch, kv, plan, rows, keys, q, 4)
+    for bound in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 16):
+        close(torch, rt.attn_paged_i8(kv, rt.KVRows(**plan, max_keys=bound, max_rows=bound), q).reshape(2, 4, 64), want, tol)
+        kv.check()
+    for n in (2 ** 31, 2 ** 32 + 2):
+        with pytest.raises(rt.B2Error):
+            rt.KVRows(**{**plan, "n_rows": n})
