@@ -529,7 +529,11 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
 // The codes are exact small integers, so both products run as integer dots on the
 // tensor cores (warp-level s8 MMAs) with the f32 side split into three signed
 // base-256 digits: X = rint(x 2^..) with |X| <= kDigitMax = d2 65536 + d1 256 + d0,
-// 23 bits below the row's largest element. The digit sums are exact in int32 and
+// 23 bits below the row's largest element. (That loses bits of the others where one
+// channel stands out, but with keys in 8 bits they hardly count: the rounding moves a score
+// by at most 2^-24 max|q| sum|k| <= 2^-24 127 d_head max|q| scale, the cache's own rounding of
+// the largest channel by up to max|q| scale / 2. The same holds for weights and values. A
+// fourth digit would need 16 KB more of the tcgen05 kernel's shared memory than there is.) The digit sums are exact in int32 and
 // are joined in f32, so a score or an output carries the error of one 23-bit
 // rounding per factor instead of a chain of f32 roundings, at a third of the int8
 // rate and without converting a single code.

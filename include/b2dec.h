@@ -350,7 +350,14 @@ int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, vo
  * over those keys alone (no -60 tail). Keys on a page outside the pool are left out;
  * a row that sees no key becomes zeros. Any mix of single tokens, pieces of prompts
  * and whole prompts. workspace: b2_attn_paged_i8_workspace() bytes (may be 0), 16-byte
- * aligned, no initialisation; calls that may overlap on the GPU need one each. */
+ * aligned, no initialisation; calls that may overlap on the GPU need one each.
+ * Precision: a query row is held to 2^-24 of its largest element, and weights (probability
+ * times value scale) to 2^-24 of the largest of up to 128 neighbouring keys; codes, products
+ * and their sums are exact, the rest f32. With elements of like size that is as good as
+ * plain f32. A query channel that is F times the others costs up to F times their rounding
+ * (F = 100: errors of 5e-6 to 8e-6 of the largest output where plain f32 has 3e-7 to 2e-6;
+ * 1000: 5e-5 to 6e-5 and 7e-7 to 4e-6), which for any query is below d_head / 65000 (0.2 %
+ * at 128) of what rounding one cached key element by half a step does to a score. */
 size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads);
 int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* q, int64_t ldq, float* out,
                      int64_t ldo, int n_heads, void* workspace, size_t workspace_bytes, int32_t* err, void* stream);

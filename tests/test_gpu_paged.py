@@ -902,3 +902,27 @@ def test_bounds_beyond_32_bits(torch, rt):
     for n in (2 ** 31, 2 ** 32 + 2):
         with pytest.raises(rt.B2Error):
             rt.KVRows(**{**plan, "n_rows": n})
+
+
+@pytest.mark.parametrize("factor", [10, 100, 1000])
+@pytest.mark.parametrize("n,H,KVH,dh", [(1, 8, 8, 128), (1, 8, 2, 64), (130, 8, 8, 128), (70, 4, 4, 256)])
+def test_a_query_channel_that_stands_out(torch, rt, n, H, KVH, dh, factor):
+    """One channel `factor` times the others, where the keys have small codes: within the documented rounding, and as the
+    documentation says below d_head / 65000 of a half step of the keys there, which moves a score by `half` or less."""
+    keys = 1152
+    kv, plan = pool(torch, rt, [n], [keys], KVH, dh, 64, seed=3)
+    kv.k[..., 5] = 3
+    q = torch.randn(n, H, dh, device="cuda") * dh ** -0.5
+    q[..., 5] = factor * dh ** -0.5
+    out = rt.attn_paged_i8(kv, rt.KVRows(**plan), q.reshape(n, -1)).reshape(n, H, dh)
+    want, tol = attend64(torch, kv, plan, [n], [keys], q.reshape(n, -1), H)
+    close(torch, out, want, tol)
+    # all scores off by at most e move an output by at most (exp(2 e) - 1) times the largest value; the f32 part of the
+    # errors is attend64's without its term for held queries
+    half = factor * dh ** -0.5 * float(kv.k_scale.nan_to_num(0.0).max()) / 2
+    top_v = 127 * float(kv.v_scale.nan_to_num(0.0).max())
+    k = held(torch, kv, plan["page_table"], 0, keys)[0].repeat_interleave(H // KVH, 1).transpose(0, 1)
+    mag = float((q.double().abs().transpose(0, 1) @ k.abs().transpose(1, 2)).max())
+    f32 = (2 * (6 * math.sqrt(dh) + 8) * mag + 2 * 104 + 16 + 18 * math.sqrt(keys)) * U
+    assert float((out.double() - want).abs().max()) <= top_v * (math.expm1(2 * half * dh / 65000) + f32)
+    kv.check()
