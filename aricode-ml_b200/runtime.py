@@ -510,7 +510,9 @@ def _there(torch, gpu, stream):
         if stream is None:
             yield
         else:
-            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=gpu)):
+            # (0 is the default stream's handle; an ExternalStream of 0 would be some other stream)
+            s = torch.cuda.ExternalStream(int(stream), device=gpu) if int(stream) else torch.cuda.default_stream(gpu)
+            with torch.cuda.stream(s):
                 yield
 
 

@@ -926,3 +926,69 @@ def test_a_query_channel_that_stands_out(torch, rt, n, H, KVH, dh, factor):
     f32 = (2 * (6 * math.sqrt(dh) + 8) * mag + 2 * 104 + 16 + 18 * math.sqrt(keys)) * U
     assert float((out.double() - want).abs().max()) <= top_v * (math.expm1(2 * half * dh / 65000) + f32)
     kv.check()
+
+
+def test_the_default_stream_by_its_handle(torch, rt):
+    """stream=0 is the default stream, also where another one is current: calls stand behind what was queued there."""
+    kv, plan = pool(torch, rt, [1, 1], [300, 40], 2, 64, 16)
+    r = rt.KVRows(**plan)
+    new = torch.randn(2, 4 * 64, device="cuda") * 0.1
+    want, tol = attend64(torch, kv, plan, [1, 1], [300, 40], new, 4)
+    q, out, ws = torch.zeros_like(new), torch.zeros_like(new), rt.attn_paged_workspace(kv, r, 4)   # (an allocation would wait)
+    default, side = torch.cuda.default_stream(), torch.cuda.Stream()
+    assert default.cuda_stream == 0
+    rt.attn_paged_i8(kv, r, q, out=out, workspace=ws)              # (loading a kernel would wait, too)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(default):
+        torch.cuda._sleep(200_000_000)
+        q.copy_(new)
+    with torch.cuda.stream(side):
+        rt.attn_paged_i8(kv, r, q, out=out, workspace=ws, stream=0)
+    torch.cuda.synchronize()
+    close(torch, out.reshape(2, 4, 64), want, tol)
+
+
+def test_a_captured_step_behind_other_streams(torch, rt):
+    """Captured with a fork and a join: one stream fills the keys and values, another the queries; the calls stand behind
+    both, and a copy of the outputs behind them, in every replay."""
+    H, KVH, dh = 8, 2, 128
+    table = torch.arange(20, dtype=torch.int32, device="cuda").reshape(2, 10)
+    kv = rt.PagedKV.empty(20, 16, KVH, dh)
+    plan = ragged(torch, [1, 30], [1, 30], table)
+    r = rt.KVRows(**plan)
+    src = [torch.randn(31, w * dh, device="cuda") for w in (H, KVH, KVH)]
+    q, k, v = (torch.zeros_like(x) for x in src)
+    out, copy = torch.zeros(31, H * dh, device="cuda"), torch.zeros(31, H * dh, device="cuda")
+    ws = rt.attn_paged_workspace(kv, r, H)
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            q.zero_()
+            q.copy_(src[0])
+        k.copy_(src[1])
+        v.copy_(src[2])
+        main.wait_stream(side)
+        rt.kv_append_i8(kv, r, k, v)
+        rt.attn_paged_i8(kv, r, q, out=out, workspace=ws)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            copy.copy_(out)
+        main.wait_stream(side)
+
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(20):
+        for x in src:
+            x.copy_(torch.randn_like(x) * 0.2)
+        copy.zero_()
+        graph.replay()
+        close(torch, copy.reshape(31, H, dh), *attend64(torch, kv, plan, [1, 30], [1, 30], src[0], H))
+    kv.check()
