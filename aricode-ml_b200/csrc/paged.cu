@@ -33,6 +33,26 @@ bool al4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 // f32 rows of `width` elements, `ld` apart, read and written 16 bytes at a time
 bool rows_ok(const float* p, int64_t ld, int64_t width) { return p && al16(p) && ld >= width && ld % 4 == 0; }
 
+// f32 rows as they lie in memory
+struct Span {
+    const float* p;
+    int64_t ld, width;
+};
+
+// whether n rows each of a and b may share an element: side by side in one buffer (the
+// slices of a fused projection) they do not, and rows that interleave with other strides
+// count as sharing
+bool overlap(const Span& a, const Span& b, int64_t n) {
+    if (!a.p || !b.p || n <= 0) return false;
+    const int64_t off = ((int64_t)reinterpret_cast<intptr_t>(b.p) - (int64_t)reinterpret_cast<intptr_t>(a.p)) / 4;
+    if (off >= (n - 1) * a.ld + a.width || -off >= (n - 1) * b.ld + b.width) return false;
+    if (a.ld != b.ld) return true;
+    const int64_t at = ((off % a.ld) + a.ld) % a.ld;               // b's column, seen from a's first one
+    return at < a.width || at + b.width > a.ld;
+}
+
+bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld; }
+
 const char* head_dim_bad(int dh) {
     return dh < 16 || dh > 256 || dh % 16 ? "d_head must be a multiple of 16 from 16 to 256" : nullptr;
 }
@@ -268,6 +288,12 @@ int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, fl
     if (table && (!pos || table_rows <= 0)) return refuse(fn, "a table needs pos and table_rows");
     if ((q_gain || k_gain) && !(eps >= 0.0f && std::isfinite(eps))) return refuse(fn, "eps must be finite and not negative");
     if ((long long)n_rows * (n_heads + n_kv_heads) >= (1ll << 26)) return refuse(fn, "2^26 or more head vectors");
+    const int64_t qw = (int64_t)n_heads * d_head, kw = (int64_t)n_kv_heads * d_head;
+    const Span qi{n_heads ? q : nullptr, ldq, qw}, qo{n_heads ? q_out : nullptr, ldqo, qw};
+    const Span ki{n_kv_heads ? k : nullptr, ldk, kw}, ko{n_kv_heads ? k_out : nullptr, ldko, kw};
+    if ((!same(qi, qo) && overlap(qi, qo, n_rows)) || (!same(ki, ko) && overlap(ki, ko, n_rows)) || overlap(qo, ki, n_rows) ||
+        overlap(ko, qi, n_rows) || overlap(qo, ko, n_rows))
+        return refuse(fn, "an output overlaps an input (other than being it, with its stride) or the other output");
     NormRopeParams p{};
     p.q = q; p.k = k; p.qo = q_out; p.ko = k_out;
     p.ldq = ldq; p.ldk = ldk; p.ldqo = ldqo; p.ldko = ldko;
@@ -298,6 +324,13 @@ int b2_kv_append_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* 
     if ((q_gain && !al16(q_gain)) || (k_gain && !al16(k_gain)) || (table && !al16(table)) || !al4(err))
         return refuse(fn, "gains and table must be 16-byte aligned, err 4");
     if (table && table_rows <= 0) return refuse(fn, "a table needs table_rows");
+    if (q) {
+        const int64_t qw = (int64_t)n_heads * kv->d_head;
+        const Span qi{q, ldq, qw}, qo{q_out, ldqo, qw};
+        if ((!same(qi, qo) && overlap(qi, qo, p.r.n_rows)) || overlap(qo, {k, ldk, width}, p.r.n_rows) ||
+            overlap(qo, {v, ldv, width}, p.r.n_rows))
+            return refuse(fn, "q_out overlaps q (other than being it, with its stride), k or v");
+    }
     if ((q_gain || k_gain) && !(eps >= 0.0f && std::isfinite(eps))) return refuse(fn, "eps must be finite and not negative");
     p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
     p.nr.q = q; p.nr.qo = q_out; p.nr.ldq = ldq; p.nr.ldqo = ldqo;
@@ -323,6 +356,9 @@ int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, vo
         ld % (bf16 ? 8 : 4))
         return refuse(fn, "k_out and v_out: 16-byte aligned, ld holding a row and a multiple of 16 bytes");
     if (!al4(err)) return refuse(fn, "err must be 4-byte aligned");
+    const int64_t unit = bf16 ? 2 : 1, row = (int64_t)kv->n_kv_heads * kv->d_head / unit;   // in 4-byte words
+    if (overlap({static_cast<const float*>(k_out), ld / unit, row}, {static_cast<const float*>(v_out), ld / unit, row}, p.r.n_rows))
+        return refuse(fn, "k_out and v_out overlap");
     p.k = k_out; p.v = v_out; p.ld = ld;
     p.items = run_bound(p.r);
     p.err = err;
@@ -355,7 +391,7 @@ int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float*
     if (!rows_ok(q, ldq, width) || !rows_ok(out, ldo, width))
         return refuse(fn, "q and out: 16-byte aligned, row strides a multiple of 4 that hold a row");
     if (!al4(err)) return refuse(fn, "err must be 4-byte aligned");
-    if (q == out) return refuse(fn, "out must not be q");
+    if (overlap({q, ldq, width}, {out, ldo, width}, p.r.n_rows)) return refuse(fn, "out must not overlap q");
     if ((int64_t)p.r.n_rows * n_heads > (1ll << 30)) return refuse(fn, "more than 2^30 (row, head) pairs");
     p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo; p.H = n_heads; p.err = err;
     const AttnPlan plan = attn_plan(p, rows->max_rows);

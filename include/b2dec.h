@@ -319,7 +319,8 @@ typedef struct b2_kv_rows {
  * eps) * gain; a NULL gain: no norm), then the rotation of b2_rope_apply with table
  * row pos[i] (table [table_rows][d_head], NULL: no rotation), queries times q_scale.
  * q [n_rows][ldq] holds n_heads heads side by side, k n_kv_heads (either count may be
- * 0). Outputs may be the inputs. Rows with pos < 0 are left alone; pos may be NULL
+ * 0). Outputs may be the inputs (with their strides), but not overlap them otherwise.
+ * Rows with pos < 0 are left alone; pos may be NULL
  * without a table. */
 int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, float* q_out, int64_t ldqo,
                     float* k_out, int64_t ldko, const float* q_gain, const float* k_gain, float eps, float q_scale,
@@ -328,7 +329,7 @@ int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, fl
 
 /* Write the call's K and V rows [n_rows][n_kv_heads * d_head] into the cache, keys
  * normed (k_gain) and rotated (table, at the row's position) on the way as in
- * b2_qk_norm_rope; with q, the queries likewise into q_out (not cached).
+ * b2_qk_norm_rope; with q, the queries likewise into q_out (not cached; it may be q).
  * A block's scale is max|x| / 127 over its values; a row that needs a larger one
  * grows it and brings the block's older codes to it (rint(code * old / new)). A
  * block whose first token is written starts afresh. Codes are rint(x / scale). A NaN or

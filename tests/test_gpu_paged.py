@@ -992,3 +992,19 @@ def test_a_captured_step_behind_other_streams(torch, rt):
         graph.replay()
         close(torch, copy.reshape(31, H, dh), *attend64(torch, kv, plan, [1, 30], [1, 30], src[0], H))
     kv.check()
+
+
+def test_in_place_and_side_by_side_in_one_buffer(torch, rt):
+    """Queries rewritten where they lie, outputs in columns of the buffer that holds the inputs: as with outputs of their own."""
+    H, KVH, dh = 4, 2, 64
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    tab = table64(torch, 64, dh)
+    r = rt.KVRows(**ragged(torch, [40], [40], table))
+    buf = torch.randn(40, (2 * H + 2 * KVH) * dh, device="cuda")
+    q, k, v, out = (x for x in buf.split([H * dh, KVH * dh, KVH * dh, H * dh], 1))
+    kv, other = rt.PagedKV.empty(4, 16, KVH, dh), rt.PagedKV.empty(4, 16, KVH, dh)
+    qo = rt.kv_append_i8(other, r, k, v, table=tab, q=q, q_scale=dh ** -0.5)
+    want = rt.attn_paged_i8(other, r, qo)
+    rt.kv_append_i8(kv, r, k, v, table=tab, q=q, q_scale=dh ** -0.5, q_out=q)
+    rt.attn_paged_i8(kv, r, q, out=out)
+    assert torch.equal(q, qo) and torch.equal(out, want) and torch.equal(kv.k, other.k) and torch.equal(kv.v, other.v)

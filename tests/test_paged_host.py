@@ -163,7 +163,7 @@ def test_long_prompts_over_a_large_capacity_are_accepted(pkg, n_rows, n_seq, cap
     rt = pkg.runtime
     r = rows(rt, n_rows=n_rows, n_seq=n_seq, max_pages=cap // 64)
     kv = pages(rt, n_pages=1 << 14, page_size=64, n_kv_heads=KVH, d_head=128)
-    assert attend(rt, kv, r, n_heads=H, ldq=H * 128, ldo=H * 128, ws=None, ws_bytes=0) == -1
+    assert attend(rt, kv, r, n_heads=H, ldq=H * 128, ldo=H * 128, out=1 << 40, ws=None, ws_bytes=0) == -1
     assert "workspace" in rt.last_error()
 
 
@@ -220,3 +220,26 @@ def test_more_sequences_than_a_call_can_search_are_refused(pkg):
             assert call(rt, pages(rt), rows(rt, n_seq=n_seq)) == -1 and "65536" in rt.last_error()
     assert attend(rt, pages(rt), rows(rt, n_seq=65536, n_rows=200, max_pages=100), ws=None, ws_bytes=0) == -1
     assert "workspace" in rt.last_error()
+
+
+def test_outputs_that_overlap_inputs_are_refused(pkg):
+    """In place with the input's own stride, or beside it in one buffer, is fine (that is tested on the GPU); anything
+    else would be read while it is written. Rows: 5 of 256 floats (q) and 128 (k, v), 1024 and 512 bytes."""
+    rt = pkg.runtime
+    far = A + (1 << 16)
+    apart = dict(q=A, qo=A + 1 * far, k=A + 2 * far, ko=A + 3 * far, n_rows=5)
+    for bad in (dict(qo=A, ldqo=512), dict(qo=A + 64), dict(qo=A + 4 * 1024 + 512), dict(qo=A - 4 * 1024), dict(ko=A + 2 * far, ldko=256),
+                dict(qo=A + 2 * far), dict(ko=A), dict(ko=A + far + 512), dict(q=A, ldq=512, qo=A + 512, ldqo=512)):
+        assert norm_rope(rt, **{**apart, **bad}) == -1 and "overlap" in rt.last_error(), bad
+    kv, r = pages(rt), rows(rt)
+    q = dict(q=far, ldq=256, q_out=2 * far, ldqo=256, n_heads=4, v=3 * far)
+    for bad in (dict(q_out=far, ldqo=512), dict(q_out=far + 1024), dict(q_out=A), dict(q_out=3 * far + 16), dict(q_out=A - 4 * 1024)):
+        assert append(rt, kv, r, **{**q, **bad}) == -1 and "overlap" in rt.last_error(), bad
+    for bad in (dict(v=A), dict(v=A + 16), dict(v=A + 512 * 4), dict(bf16=1, v=A + 256 * 4), dict(ld=256, v=A + 256)):
+        assert read(rt, kv, r, **bad) == -1 and "overlap" in rt.last_error(), bad
+    for bad in (dict(out=A), dict(out=A + 1024), dict(out=A, ldo=512), dict(out=A + 256, ldo=256), dict(out=A - 4 * 1024),
+                dict(ldq=512, ldo=512, out=A + 512)):
+        assert attend(rt, kv, r, **bad) == -1 and "overlap" in rt.last_error(), bad
+    # beside each other in one buffer: refused for the missing workspace alone
+    for good in (dict(ldq=512, ldo=512, out=A + 1024), dict(ldq=1024, ldo=1024, out=A - 2048), dict(out=A + 5 * 1024)):
+        assert attend(rt, kv, rows(rt, max_pages=5000), **good, ws=None) == -1 and "workspace" in rt.last_error(), good
