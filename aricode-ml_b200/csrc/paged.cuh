@@ -533,11 +533,11 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
 // channel stands out, but with keys in 8 bits they hardly count: the rounding moves a score
 // by at most 2^-24 max|q| sum|k| <= 2^-24 127 d_head max|q| scale, the cache's own rounding of
 // the largest channel by up to max|q| scale / 2. The same holds for weights and values. A
-// fourth digit would need 16 KB more of the tcgen05 kernel's shared memory than there is.) The digit sums are exact in int32 and
-// are joined in f32, so a score or an output carries the error of one 23-bit
-// rounding per factor instead of a chain of f32 roundings, at a third of the int8
-// rate and without converting a single code.
-// three digits in [-128, 127] reach 2^23 - 1 - 0x8080 = 8355711; a little below it,
+// fourth digit would need 16 KB of the tcgen05 kernel's shared memory, where 9 KB are left.)
+// The digit sums are exact in int32 and are joined in f32, so a score or an output carries
+// the error of one 23-bit rounding per factor instead of a chain of f32 roundings, at a
+// third of the int8 rate and without converting a single code.
+// Three digits in [-128, 127] reach 2^23 - 1 - 0x8080 = 8355711; a little below it,
 // so that the roundings of factor and product stay inside
 constexpr int kDigitMax = 8355700;
 
