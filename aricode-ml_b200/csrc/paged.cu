@@ -142,18 +142,19 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
 // each kind has a launch, left out where the caller's sizes say that none is of its kind.
 // (One that finds none costs a wave of empty CTAs, 2.4 us, for every 148 that its rows might
 // have needed: with max_rows = 1 a step of 64 tokens over 1152 keys takes 119 us for 32 / 32
-// heads of 128, without it 125 us; 256 tokens, 32 / 4 heads of 64: 66 and 105 us.) A whole batch on one kernel cost more: a
-// single token in a 128-row tile as much as 128, a prompt in 8-column tiles re-reads its
-// keys 16 times as often.
+// heads of 128, without it 125 us; 256 tokens, 32 / 4 heads of 64: 66 and 105 us.) A whole
+// batch on one kernel cost more: a single token in a 128-row tile as much as 128, a prompt in
+// 8-column tiles re-reads its keys 16 times as often.
 //  few, up to 16 columns: 8 a CTA, or 2 where single tokens make no more (decode without
 //  shared heads; beside prompts too). Small splits fill the GPU when there are few
 //  rows; with long caches larger ones bound the partial results and their joining. Their
 //  size is a function of the capacity alone; the columns a CTA follow the longest sequence,
 //  so the last bits of a sequence's result can differ beside others.
 //  many: 128 a CTA (64 for d_head above 128); keys are split only while there are too few
-//  tiles for four rounds of the GPU (six an SM for d_head above 128). (Against one round: a sequence of 30 K keys 173 us, not
-//  141, three of 8 K with 16 rows 72, not 52; but twelve of up to 10 K 292, not 353, two of
-//  3 K with 300 rows 177, not 206. The host does not know the lengths.)
+//  tiles for four rounds of the GPU (d_head above 128: for six tiles an SM). Against one
+//  round: a sequence of 30 K keys 173 us, not 141, three of 8 K with 16 rows 72, not 52; but
+//  twelve of up to 10 K 292, not 353, two of 3 K with 300 rows 177, not 206. The host does not
+//  know the lengths.
 constexpr int kFewCols = 16;
 
 struct AttnPlan {
@@ -186,15 +187,13 @@ AttnPlan attn_plan(PagedAttnParams& p, int max_rows) {
         // whole prompts: only the few-row sequences beside them have splits to join
         if (p.nsplit_many == 1) p.join_rows = most;
     }
-    auto items = [&](long long tiles, int kc_log2) {
-        return tiles * p.c.KVH * splits_at(kc_log2);
-    };
+    auto items = [&](long long tiles, int kc_log2) { return tiles * p.c.KVH * splits_at(kc_log2); };
     // tiles of `cols` columns over all sequences: at most one partly filled one each
     auto tiles_of = [&](int cols) { return (long long)p.r.n_rows * p.G / cols + std::min(p.r.n_seq, p.r.n_rows); };
     long long few_tiles = tiles_of(a.few_cols), many_tiles = tiles_of(a.many_cols);
     if (a.few && a.many) {
-        // sequences of the few-row kind have up to kFewCols columns each, whatever n_rows is; the others have more, so
-        // a tile has at least kFewCols + 1
+        // sequences of the few-row kind have up to kFewCols columns each, whatever n_rows is;
+        // the others have more, so a tile of theirs has at least kFewCols + 1
         few_tiles = std::min(few_tiles, (long long)p.r.n_seq * ((kFewCols + a.few_cols - 1) / a.few_cols));
         many_tiles = std::min(many_tiles, (long long)p.r.n_rows * p.G / (kFewCols + 1));
     }

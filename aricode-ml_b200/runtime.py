@@ -519,7 +519,8 @@ def _there(torch, gpu, stream):
 class PagedKV:
     """A pool of pages of int8 keys and values with a scale per 16 tokens and head (b2_kv_pages): k and v
     [pages, kv_heads, page_size, d_head] int8, k_scale and v_scale [pages, kv_heads, page_size / 16] f32. `err` is
-    the device word that calls on this cache set; check() reads it."""
+    the device word that calls on this cache set; check() reads it. It is made on the current stream, like any tensor:
+    other streams' calls must be ordered behind that."""
 
     def __init__(self, k, v, k_scale, v_scale):
         import torch

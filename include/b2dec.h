@@ -320,8 +320,7 @@ typedef struct b2_kv_rows {
  * row pos[i] (table [table_rows][d_head], NULL: no rotation), queries times q_scale.
  * q [n_rows][ldq] holds n_heads heads side by side, k n_kv_heads (either count may be
  * 0). Outputs may be the inputs (with their strides), but not overlap them otherwise.
- * Rows with pos < 0 are left alone; pos may be NULL
- * without a table. */
+ * Rows with pos < 0 are left alone; pos may be NULL without a table. */
 int b2_qk_norm_rope(const float* q, int64_t ldq, const float* k, int64_t ldk, float* q_out, int64_t ldqo,
                     float* k_out, int64_t ldko, const float* q_gain, const float* k_gain, float eps, float q_scale,
                     const float* table, int table_rows, const int32_t* pos, int n_rows, int n_heads,

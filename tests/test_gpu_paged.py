@@ -794,21 +794,9 @@ def test_workspace_is_enough_and_read_only_where_written(torch, rt, H, KVH, dh, 
     kv.check()
 
 
-def call_us(torch, rt, kvs, r, q):
-    """Device time of an attention call among others, over caches that do not stay in L2 together."""
-    out, ws, best = torch.empty_like(q), rt.attn_paged_workspace(kvs[0], r, q.shape[1] // kvs[0].d_head), math.inf
-    for _ in range(8):
-        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-        a.record()
-        for i in range(12):
-            rt.attn_paged_i8(kvs[i % len(kvs)], r, q, out=out, workspace=ws)
-        b.record()
-        torch.cuda.synchronize()
-        best = min(best, a.elapsed_time(b) / 12 * 1e3)
-    return best
-
-
-def decode_step_us(torch, rt, n, keys, H, KVH, dh, hint):
+def decode_step_us(torch, rt, n, keys, H, KVH, dh):
+    """Device time of an attention call among others with and without max_rows = 1, taken in turn, over caches that do
+    not stay in L2 together."""
     g = torch.Generator(device="cuda").manual_seed(n)
     per = -(-keys // 64)
     table = torch.randperm(n * per, device="cuda", generator=g).to(torch.int32).reshape(n, per)
@@ -817,14 +805,26 @@ def decode_step_us(torch, rt, n, keys, H, KVH, dh, hint):
         for codes, scale in ((kv.k, kv.k_scale), (kv.v, kv.v_scale)):
             codes.random_(-127, 128, generator=g)
             scale.fill_(0.02)
-    r = rt.KVRows(**ragged(torch, [1] * n, [keys] * n, table), max_keys=keys, max_rows=hint)
-    return call_us(torch, rt, kvs, r, torch.randn(n, H * dh, device="cuda", generator=g) * dh ** -0.5)
+    q = torch.randn(n, H * dh, device="cuda", generator=g) * dh ** -0.5
+    out, best = torch.empty_like(q), [math.inf, math.inf]
+    rows = [rt.KVRows(**ragged(torch, [1] * n, [keys] * n, table), max_keys=keys, max_rows=hint) for hint in (1, 0)]
+    ws = [rt.attn_paged_workspace(kvs[0], r, H) for r in rows]
+    for _ in range(10):
+        for j, r in enumerate(rows):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for i in range(12):
+                rt.attn_paged_i8(kvs[i % 3], r, q, out=out, workspace=ws[j])
+            b.record()
+            torch.cuda.synchronize()
+            best[j] = min(best[j], a.elapsed_time(b) / 12 * 1e3)
+    return best
 
 
 def test_a_decode_step_without_the_hint(torch, rt):
     """64 single tokens that are not said to be single: a small launch that finds nothing to do, not thousands of CTAs
     (221 against 119 us)."""
-    hint, none = (decode_step_us(torch, rt, 64, 1152, 32, 32, 128, x) for x in (1, 0))
+    hint, none = decode_step_us(torch, rt, 64, 1152, 32, 32, 128)
     assert none < 1.5 * hint
 
 
@@ -832,7 +832,7 @@ def test_a_decode_step_without_the_hint(torch, rt):
 def test_single_tokens_behind_the_launch_for_longer_sequences(torch, rt, heads, dh):
     """The kernel of the single tokens is as fast behind the other kernel's (here empty) launch as without it: its loads
     do not suffer from that kernel's use of the SM (152 against 119 us, with d_head 256 169 against 128)."""
-    hint, none = (decode_step_us(torch, rt, 64, 1152, heads, heads, dh, x) for x in (1, 0))
+    hint, none = decode_step_us(torch, rt, 64, 1152, heads, heads, dh)
     assert none < 1.17 * hint
 
 
