@@ -21,8 +21,9 @@ CSRC = PKG / "csrc"
 OBJ = CSRC / "_obj"
 LIB = PKG / "libb2dec.so"
 FRONT = PKG / "b2run"                    # stdin-tokens front end (host program over the library)
-SOURCES = ["runtime.cu", "launch.cu", "token.cu", "prefill.cu", "capi.cu", "noalloc.cu", "paged.cu"]
-HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "umma.cuh", "json.h"]
+SOURCES = ["runtime.cu", "launch.cu", "token.cu", "prefill.cu", "capi.cu", "noalloc.cu", "paged.cu", "tree.cu", "groups.cu"]
+HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "paged_rows.cuh", "paged_host.cuh",
+           "host_checks.cuh", "tree.cuh", "groups.cuh", "umma.cuh", "json.h"]
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",

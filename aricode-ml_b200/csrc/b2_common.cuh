@@ -21,6 +21,8 @@ enum : int {
     B2_DEV_ERR_BAD_TOKEN = 3,
     B2_DEV_ERR_BAD_PAGE = 4,       // page table entry outside the pool
     B2_DEV_ERR_BAD_ROWS = 5,       // a row range that starts below the one before it
+    B2_DEV_ERR_BAD_ROW = 6,        // a row index outside the buffer
+    B2_DEV_ERR_TOO_MANY = 7,       // a sequence with more drafted rows than a tree can have
 };
 
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s per wait

@@ -1,0 +1,58 @@
+// host_checks.cuh — what entry points refuse with and check arguments by: messages for
+// b2_last_error, alignment, rows that share memory.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "../../include/b2dec.h"
+
+void b2_internal_set_error(const std::string& msg);   // runtime.cu
+
+namespace b2 {
+
+inline int refuse(const char* fn, const std::string& why) {
+    b2_internal_set_error(std::string(fn) + ": " + why);
+    return B2_E_INVALID;
+}
+
+inline int status(const char* fn, cudaError_t e) {
+    if (e == cudaSuccess) return B2_OK;
+    b2_internal_set_error(std::string(fn) + ": " + cudaGetErrorString(e));
+    return B2_E_CUDA;
+}
+
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool al4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+// f32 rows of `width` elements, `ld` apart, read and written 16 bytes at a time
+inline bool rows_ok(const float* p, int64_t ld, int64_t width) { return p && al16(p) && ld >= width && ld % 4 == 0; }
+
+// f32 rows as they lie in memory
+struct Span {
+    const float* p;
+    int64_t ld, width;
+};
+
+// whether n rows each of a and b may share an element: side by side in one buffer (the
+// slices of a fused projection) they do not, and rows that interleave with other strides
+// count as sharing
+inline bool overlap(const Span& a, const Span& b, int64_t n) {
+    if (!a.p || !b.p || n <= 0) return false;
+    const int64_t off = ((int64_t)reinterpret_cast<intptr_t>(b.p) - (int64_t)reinterpret_cast<intptr_t>(a.p)) / 4;
+    if (off >= (n - 1) * a.ld + a.width || -off >= (n - 1) * b.ld + b.width) return false;
+    if (a.ld != b.ld) return true;
+    const int64_t at = ((off % a.ld) + a.ld) % a.ld;               // b's column, seen from a's first one
+    return at < a.width || at + b.width > a.ld;
+}
+
+inline bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld; }
+
+inline int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
+
+}  // namespace b2

@@ -1,100 +1,15 @@
 // paged.cu — entry points of the paged 8-bit KV cache (paged.cuh): argument checks
 // and launches. Device pointers in and out, caller's stream, nothing allocated,
 // nothing synchronised, and nothing read from device memory on the host.
-#include <cuda_runtime.h>
-
 #include <algorithm>
 #include <cmath>
-#include <string>
 
-#include "../../include/b2dec.h"
+#include "paged_host.cuh"
 #include "paged.cuh"
-
-void b2_internal_set_error(const std::string& msg);   // runtime.cu
 
 using namespace b2;
 
 namespace {
-
-int refuse(const char* fn, const std::string& why) {
-    b2_internal_set_error(std::string(fn) + ": " + why);
-    return B2_E_INVALID;
-}
-
-int status(const char* fn, cudaError_t e) {
-    if (e == cudaSuccess) return B2_OK;
-    b2_internal_set_error(std::string(fn) + ": " + cudaGetErrorString(e));
-    return B2_E_CUDA;
-}
-
-bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool al4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
-
-// f32 rows of `width` elements, `ld` apart, read and written 16 bytes at a time
-bool rows_ok(const float* p, int64_t ld, int64_t width) { return p && al16(p) && ld >= width && ld % 4 == 0; }
-
-// f32 rows as they lie in memory
-struct Span {
-    const float* p;
-    int64_t ld, width;
-};
-
-// whether n rows each of a and b may share an element: side by side in one buffer (the
-// slices of a fused projection) they do not, and rows that interleave with other strides
-// count as sharing
-bool overlap(const Span& a, const Span& b, int64_t n) {
-    if (!a.p || !b.p || n <= 0) return false;
-    const int64_t off = ((int64_t)reinterpret_cast<intptr_t>(b.p) - (int64_t)reinterpret_cast<intptr_t>(a.p)) / 4;
-    if (off >= (n - 1) * a.ld + a.width || -off >= (n - 1) * b.ld + b.width) return false;
-    if (a.ld != b.ld) return true;
-    const int64_t at = ((off % a.ld) + a.ld) % a.ld;               // b's column, seen from a's first one
-    return at < a.width || at + b.width > a.ld;
-}
-
-bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld; }
-
-const char* head_dim_bad(int dh) {
-    return dh < 16 || dh > 256 || dh % 16 ? "d_head must be a multiple of 16 from 16 to 256" : nullptr;
-}
-
-constexpr int kMaxPagedHeads = 1024;
-// Every CTA goes through the sequences to find its own, so that a call's time grows with
-// their square: single tokens, 32 / 8 heads of 128, append and attention 0.04 and 0.07 ms for
-// 512 sequences, 0.25 and 0.5 for 2048, 3.4 and 5.7 for 8192, 239 and 416 for 65536. A million
-// would hold the GPU for minutes.
-constexpr int kMaxSeqs = 65536;
-
-// the cache and the rows of a call, checked; false: refused with a message
-bool view(const char* fn, const b2_kv_pages* kv, const b2_kv_rows* rows, PagedKv& c, PagedRows& r) {
-    auto bad = [&](const char* why) { refuse(fn, why); return false; };
-    if (!kv || !rows) return bad("NULL cache or rows");
-    if (const char* why = head_dim_bad(kv->d_head)) return bad(why);
-    if (kv->n_kv_heads <= 0 || kv->n_kv_heads > kMaxPagedHeads) return bad("n_kv_heads must be 1 to 1024");
-    if (kv->page_size < kKvBlock || kv->page_size > 1024 || (kv->page_size & (kv->page_size - 1)))
-        return bad("page_size must be a power of two from 16 to 1024");
-    if (kv->n_pages <= 0) return bad("n_pages must be positive");
-    if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale || !al16(kv->k) || !al16(kv->v) || !al4(kv->k_scale) ||
-        !al4(kv->v_scale))
-        return bad("cache pointers must be set, the codes' aligned to 16 bytes");
-    if (rows->n_rows < 0 || rows->n_seq < 0 || rows->max_pages < 0) return bad("negative count");
-    if (rows->n_rows > 0 && rows->n_seq > 0 &&
-        (!rows->row_start || !rows->kv_len || (!rows->page_table && rows->max_pages) || !al4(rows->row_start) ||
-         !al4(rows->kv_len) || !al4(rows->page_table)))
-        return bad("row_start, kv_len and page_table must be set");
-    if (rows->n_seq > kMaxSeqs) return bad("n_seq above 65536");
-    const int64_t cap = (int64_t)rows->max_pages * kv->page_size;
-    if (cap > (1 << 30)) return bad("max_pages * page_size above 2^30");
-    if ((int64_t)kv->n_pages * kv->n_kv_heads * (kv->page_size / kKvBlock) >= (1ll << 31)) return bad("2^31 or more blocks in the pool");
-    if (rows->max_keys < 0 || rows->max_rows < 0) return bad("negative max_keys or max_rows");
-    c.k = kv->k; c.v = kv->v; c.ks = kv->k_scale; c.vs = kv->v_scale;
-    c.n_pages = kv->n_pages; c.KVH = kv->n_kv_heads; c.dh = kv->d_head;
-    c.page_log2 = 0;
-    while ((1 << c.page_log2) < kv->page_size) ++c.page_log2;
-    r.row_start = rows->row_start; r.kv_len = rows->kv_len; r.table = rows->page_table;
-    r.n_seq = rows->n_seq; r.max_pages = rows->max_pages; r.n_rows = rows->n_rows;
-    r.cap = rows->max_keys > 0 && rows->max_keys < cap ? rows->max_keys : (int)cap;
-    return true;
-}
 
 // most (sequence, block) runs that n_rows rows in n_seq ranges can make: a range of
 // L rows touches at most (L - 2) / 16 + 2 blocks, and no more than L
@@ -136,6 +51,14 @@ cudaError_t launch_append(AppendParams p, bool queries, int max_rows, cudaStream
     // about four units of 4 vectors a lane group
     const int y = (kKvBlock * ((p.nr.H + 3) / 4) * LPH / 4 + 255) / 256;
     return launch_ex(append_queries_kernel<LPH, VPL>, dim3((unsigned)p.items, (unsigned)y), dim3(256), 0, s, true, p);
+}
+
+// picked rows: a path of a tree is a few rows, so a warp holds a head's whole run
+template <int LPH, int VPL>
+cudaError_t launch_append_kept(AppendParams p, int max_rows, cudaStream_t s) {
+    p.kv_ctas = (2 * p.c.KVH + 7) / 8;
+    const dim3 grid((unsigned)p.items, (unsigned)p.kv_ctas);
+    return launch_ex(kv_append_kernel<LPH, VPL, 1, 1, true>, grid, dim3(256), 0, s, true, p);
 }
 
 // A call's sequences are of two kinds, by their columns (token, head) of a KV head, and
@@ -214,12 +137,6 @@ PartBytes part_bytes(const PagedAttnParams& p) {
     const size_t head = (size_t)p.H * (p.c.dh + 4) * sizeof(float);
     const size_t slots = p.few_rows ? (size_t)p.r.n_seq * p.few_rows : (size_t)p.r.n_rows;
     return {p.nsplit_few > 1 ? slots * head * p.nsplit_few : 0, p.nsplit_many > 1 ? (size_t)p.r.n_rows * head * p.nsplit_many : 0};
-}
-
-int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
 }
 
 cudaError_t launch_join(const PagedAttnParams& p, cudaStream_t s) {
@@ -343,6 +260,36 @@ int b2_kv_append_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* 
     p.err = err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define B2_CALL(L, V) launch_append<L, V>(p, q != nullptr, rows->max_rows, s)
+    return status(fn, B2_BY_HEAD_DIM(kv->d_head, B2_CALL));
+#undef B2_CALL
+}
+
+int b2_kv_append_kept_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const int32_t* row_index, int n_src, const float* k,
+                         int64_t ldk, const float* v, int64_t ldv, const float* k_gain, float eps, const float* table,
+                         int table_rows, int32_t* err, void* stream) {
+    const char* fn = "b2_kv_append_kept_i8";
+    AppendParams p{};
+    if (!view(fn, kv, rows, p.c, p.r)) return B2_E_INVALID;
+    if (n_src < 0) return refuse(fn, "negative n_src");
+    if (p.r.n_rows == 0 || p.r.n_seq == 0) return B2_OK;
+    const int64_t width = (int64_t)kv->n_kv_heads * kv->d_head;
+    if (!row_index || !al4(row_index)) return refuse(fn, "row_index must be set, 4-byte aligned");
+    if (n_src && (!rows_ok(k, ldk, width) || !rows_ok(v, ldv, width)))
+        return refuse(fn, "k and v: 16-byte aligned, row strides a multiple of 4 that hold a row");
+    if ((k_gain && !al16(k_gain)) || (table && !al16(table)) || !al4(err))
+        return refuse(fn, "k_gain and table must be 16-byte aligned, err 4");
+    if (table && table_rows <= 0) return refuse(fn, "a table needs table_rows");
+    if (k_gain && !(eps >= 0.0f && std::isfinite(eps))) return refuse(fn, "eps must be finite and not negative");
+    p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
+    p.nr.gk = k_gain; p.nr.eps = eps;
+    p.nr.inv_dh = 1.0f / (float)kv->d_head;
+    p.nr.table = table; p.nr.table_rows = table_rows;
+    p.nr.n_rows = p.r.n_rows; p.nr.dh = kv->d_head; p.nr.err = err;
+    p.items = run_bound(p.r);
+    p.index = row_index; p.n_src = n_src;
+    p.err = err;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define B2_CALL(L, V) launch_append_kept<L, V>(p, rows->max_rows, s)
     return status(fn, B2_BY_HEAD_DIM(kv->d_head, B2_CALL));
 #undef B2_CALL
 }

@@ -8,73 +8,10 @@
 // starts and pages are read on the device only (a captured launch replays with new
 // ones); every value is checked before it becomes an address.
 #pragma once
-#include "kernels.cuh"
+#include "paged_rows.cuh"
 #include "umma.cuh"
 
 namespace b2 {
-
-constexpr int kKvBlock = 16;           // tokens that share a scale
-
-struct PagedKv {
-    int8_t* k;               // [n_pages][KVH][page][dh]
-    int8_t* v;
-    float* ks;               // [n_pages][KVH][page / 16]
-    float* vs;
-    int n_pages, page_log2, KVH, dh;
-};
-
-struct PagedRows {
-    const int* row_start;    // [n_seq + 1]
-    const int* kv_len;       // [n_seq]
-    const int* table;        // [n_seq][max_pages]
-    int n_seq, max_pages, n_rows;
-    int cap;                 // positions a sequence can hold: min(max_keys, max_pages * page)
-};
-
-// one sequence's rows: a .. a + len - 1, at positions pos0 .. pos0 + len - 1
-// (negative ones stand nowhere), keys 0 .. min(kv, cap) - 1
-struct SeqRows {
-    int a, len, kv;
-    __device__ __forceinline__ int pos0() const { return kv - len; }
-};
-
-__device__ __forceinline__ SeqRows seq_rows(const PagedRows& r, int s) {
-    SeqRows q;
-    q.a = min(max(r.row_start[s], 0), r.n_rows);
-    q.len = min(max(r.row_start[s + 1], q.a), r.n_rows) - q.a;
-    q.kv = max(r.kv_len[s], 0);
-    return q;
-}
-
-// page of position pos of sequence s, or -1
-__device__ __forceinline__ int page_of(const PagedKv& c, const PagedRows& r, int s, int pos) {
-    const int id = r.table[(size_t)s * r.max_pages + (pos >> c.page_log2)];
-    return (unsigned)id < (unsigned)c.n_pages ? id : -1;
-}
-
-// Start of every kernel here: they are launched with programmatic serialisation, so that
-// a launch comes up while the one before it drains, and read nothing before that is
-// complete. The launch before it may have written what they read (rows, lengths, pages,
-// codes, scales), within this one's lifetime: such loads are plain ones, which stay behind
-// the wait; read-only loads (__ldg) are for gains and rotation tables alone. (Same times.)
-__device__ __forceinline__ void after_previous() {
-    pdl_launch_dependents();
-    pdl_wait();
-}
-
-// Plain loads too, free to move among the shared-memory stores around them but not before
-// the wait (the split kernel's codes: as C++ loads they cost <64, 8> 52 bytes of spills and
-// 3 % of attend-long).
-__device__ __forceinline__ uint4 load16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 load8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
 
 // A run: the rows of one sequence that lie in one block of 16 tokens.
 struct BlockRun {
@@ -257,6 +194,8 @@ struct AppendParams {
     NormRopeParams nr;       // gains, table; its q / qo for the queries (q nullptr: none)
     int items;               // runs the grid covers
     int kv_ctas;             // grid y below this: K and V, from it on: queries
+    const int* index;        // PICK: row i of the call is row index[i] of k and v, which
+    int n_src;               // have n_src rows
     int* err;
 };
 
@@ -264,7 +203,7 @@ struct AppendParams {
 // word of theirs in shared memory, 0): NP passes of WPT * 32 / LPH rows in registers. The
 // block's new scale is known when all rows have been seen; if they are more than the
 // registers hold (WPT = 1) they are fetched again for the codes.
-template <int LPH, int VPL, int NP, int WPT>
+template <int LPH, int VPL, int NP, int WPT, bool PICK>
 __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRun& run, int page, int head, bool is_k,
                                             int lane, int part, unsigned* top) {
     constexpr int RPW = 32 / LPH * WPT;            // rows per pass
@@ -280,14 +219,17 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
     // a block that starts with this run has no older rows: its scale starts afresh
     const float old = o0 == 0 ? 0.0f : *sp;
     float4 x[NP][VPL];
+    unsigned missing = 0u;                         // PICK: rows whose index says nothing
     auto fetch = [&](int i0) {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int i = i0 + j * RPW + g;
+            const int row = i >= run.n ? -1 : PICK ? picked_row(p.index, run.row + i, p.n_src, p.err) : run.row + i;
+            if constexpr (PICK) missing = row < 0 ? missing | 1u << j : missing & ~(1u << j);
 #pragma unroll
             for (int e = 0; e < VPL; ++e) {
                 const int d = 4 * (gl + LPH * e);
-                x[j][e] = (i < run.n && d < dh) ? *reinterpret_cast<const float4*>(src + (size_t)(run.row + i) * ld + d)
+                x[j][e] = (row >= 0 && d < dh) ? *reinterpret_cast<const float4*>(src + (size_t)row * ld + d)
                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
@@ -302,7 +244,8 @@ __device__ __forceinline__ void append_head(const AppendParams& p, const BlockRu
             for (int j = 0; j < NP; ++j) {
                 if (i0 + j * RPW >= run.n) continue;
                 // (rows past the run are zeros and stay so: without an eps their norm is not a number)
-                const float rms = head_rms<LPH, VPL>(x[j], p.nr.inv_dh, p.nr.eps), r = i0 + j * RPW + g < run.n ? rms : 0.0f;
+                const bool there = PICK ? !(missing >> j & 1u) : i0 + j * RPW + g < run.n;
+                const float rms = head_rms<LPH, VPL>(x[j], p.nr.inv_dh, p.nr.eps), r = there ? rms : 0.0f;
 #pragma unroll
                 for (int e = 0; e < VPL; ++e)
                     x[j][e] = make_float4(fmul(fmul(x[j][e].x, r), gv[e].x), fmul(fmul(x[j][e].y, r), gv[e].y),
@@ -422,7 +365,7 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, const Bloc
 // scale and older codes. 6300 rows of 8 heads of 128: 27 to 29 us; 64 single rows of 32: 8 us.
 // Six CTAs an SM for d_head 65 to 128 instead of the five that its registers allow: 148 ->
 // 144 us for 6300 rows of 32 + 32 heads with queries and read back; at 64 no difference.
-template <int LPH, int VPL, int NP, int WPT>
+template <int LPH, int VPL, int NP, int WPT, bool PICK = false>
 __global__ void __launch_bounds__(256, WPT == 4 && LPH == 32 && VPL == 1 ? 6 : 1) kv_append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ unsigned top[8 / WPT];
     after_previous();
@@ -441,7 +384,7 @@ __global__ void __launch_bounds__(256, WPT == 4 && LPH == 32 && VPL == 1 ? 6 : 1
             if (lane == 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
             return;
         }
-        append_head<LPH, VPL, NP, WPT>(p, run, page, task >> 1, (task & 1) == 0, lane, warp % WPT, top + warp / WPT);
+        append_head<LPH, VPL, NP, WPT, PICK>(p, run, page, task >> 1, (task & 1) == 0, lane, warp % WPT, top + warp / WPT);
         return;
     }
     append_queries<LPH, VPL, 1>(p, run, ((blockIdx.y - p.kv_ctas) * 256 + threadIdx.x) / LPH,
@@ -557,35 +500,6 @@ __device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
-// two f32 in one instruction: the attention kernels are bound by what the schedulers
-// issue, and a packed operation takes one slot for two (same rounding)
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // rint(x f) + 0x8080 for |x f| <= kDigitMax, in the low 24 bits
 __device__ __forceinline__ uint32_t digit_bits(float x, float f) { return (uint32_t)__float2int_rn(x * f) + 0x8080u; }
 // the same for x >= 0 in one operation: the f32 addition rounds x f to an integer
@@ -607,12 +521,6 @@ __device__ __forceinline__ f32x2 join_digits(int a2, int b2, int a1, int b1, int
 }
 __device__ __forceinline__ f32x2 join_digits(const int (&c)[3][4], int y) {
     return join_digits(c[2][y], c[2][y + 1], c[1][y], c[1][y + 1], c[0][y], c[0][y + 1]);
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // the factor that takes values up to `top` (>= 0) to integers up to kDigitMax; tiny

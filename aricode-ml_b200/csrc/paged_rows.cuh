@@ -1,0 +1,115 @@
+// paged_rows.cuh — what the kernels over the paged 8-bit KV cache share (paged.cuh,
+// tree.cuh): the cache and the rows of a call as kernels see them, loads behind the
+// launch before, packed f32 arithmetic.
+#pragma once
+#include "kernels.cuh"
+
+namespace b2 {
+
+constexpr int kKvBlock = 16;           // tokens that share a scale
+
+struct PagedKv {
+    int8_t* k;               // [n_pages][KVH][page][dh]
+    int8_t* v;
+    float* ks;               // [n_pages][KVH][page / 16]
+    float* vs;
+    int n_pages, page_log2, KVH, dh;
+};
+
+struct PagedRows {
+    const int* row_start;    // [n_seq + 1]
+    const int* kv_len;       // [n_seq]
+    const int* table;        // [n_seq][max_pages]
+    int n_seq, max_pages, n_rows;
+    int cap;                 // positions a sequence can hold: min(max_keys, max_pages * page)
+};
+
+// one sequence's rows: a .. a + len - 1, at positions pos0 .. pos0 + len - 1
+// (negative ones stand nowhere), keys 0 .. min(kv, cap) - 1
+struct SeqRows {
+    int a, len, kv;
+    __device__ __forceinline__ int pos0() const { return kv - len; }
+};
+
+__device__ __forceinline__ SeqRows seq_rows(const PagedRows& r, int s) {
+    SeqRows q;
+    q.a = min(max(r.row_start[s], 0), r.n_rows);
+    q.len = min(max(r.row_start[s + 1], q.a), r.n_rows) - q.a;
+    q.kv = max(r.kv_len[s], 0);
+    return q;
+}
+
+// page of position pos of sequence s, or -1
+__device__ __forceinline__ int page_of(const PagedKv& c, const PagedRows& r, int s, int pos) {
+    const int id = r.table[(size_t)s * r.max_pages + (pos >> c.page_log2)];
+    return (unsigned)id < (unsigned)c.n_pages ? id : -1;
+}
+
+// Start of every kernel here: they are launched with programmatic serialisation, so that
+// a launch comes up while the one before it drains, and read nothing before that is
+// complete. The launch before it may have written what they read (rows, lengths, pages,
+// codes, scales), within this one's lifetime: such loads are plain ones, which stay behind
+// the wait; read-only loads (__ldg) are for gains and rotation tables alone. (Same times.)
+__device__ __forceinline__ void after_previous() {
+    pdl_launch_dependents();
+    pdl_wait();
+}
+
+// Plain loads too, free to move among the shared-memory stores around them but not before
+// the wait (the split kernel's codes: as C++ loads they cost <64, 8> 52 bytes of spills and
+// 3 % of attend-long).
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+// which of n_src rows an index picks for row `row` of a call (-1: none)
+__device__ __forceinline__ int picked_row(const int* index, int row, int n_src, int* err) {
+    const int at = index[row];
+    if ((unsigned)at < (unsigned)n_src) return at;
+    set_err(err, B2_DEV_ERR_BAD_ROW);
+    return -1;
+}
+
+// two f32 in one instruction: the attention kernels are bound by what the schedulers
+// issue, and a packed operation takes one slot for two (same rounding)
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace b2

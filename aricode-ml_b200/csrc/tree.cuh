@@ -1,0 +1,233 @@
+// tree.cuh — trees of drafted tokens over the paged 8-bit KV cache: attention to the cache
+// and to the drafted rows, acceptance of a path (sm_100a).
+//
+// A call's rows are ragged as in paged_rows.cuh, except that kv_len counts the cached keys
+// alone: the drafted rows' keys and values are f32 rows of the call. Up to 64 rows a
+// sequence, so that what a row sees of them is one 64-bit word.
+#pragma once
+#include "paged_rows.cuh"
+
+namespace b2 {
+
+constexpr int kTreeRows = 64;
+
+struct TreeAttnParams {
+    PagedKv c;
+    PagedRows r;             // kv_len: cached keys
+    const long long* seen;   // [n_rows]
+    const float* q;          // [n_rows][ldq], rotated and pre-scaled
+    const float* k;          // [n_rows][ldk], rotated
+    const float* v;          // [n_rows][ldv]
+    float* out;              // [n_rows][ldo]
+    long long ldq, ldk, ldv, ldo;
+    int H, G;                // G = H / KVH
+    int* err;
+};
+
+// One warp a (row, head): every key in turn, lanes over d_head.
+static __global__ void __launch_bounds__(256) tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
+    after_previous();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.c.dh;
+    const int row = blockIdx.x, h = blockIdx.y * 8 + warp;
+    int s = -1, a = 0, len = 0, kv = 0;
+    for (int base = 0; base < p.r.n_seq && s < 0; base += 32) {
+        SeqRows q{0, 0, 0};
+        if (base + lane < p.r.n_seq) q = seq_rows(p.r, base + lane);
+        const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
+        if (m) {
+            const int src = __ffs(m) - 1;
+            s = base + src;
+            a = __shfl_sync(0xffffffffu, q.a, src);
+            len = __shfl_sync(0xffffffffu, q.len, src);
+            kv = __shfl_sync(0xffffffffu, q.kv, src);
+        }
+    }
+    if (s < 0 || h >= p.H) return;
+    if (len > kTreeRows) {
+        set_err(p.err, B2_DEV_ERR_TOO_MANY);
+        return;
+    }
+    if (kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
+    kv = min(kv, p.r.cap);
+    const int kvh = h / p.G;
+    float q[8], o[8], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        q[i] = d < dh ? p.q[(size_t)row * p.ldq + (size_t)h * dh + d] * 1.4426950408889634f : 0.0f;
+        o[i] = 0.0f;
+    }
+    auto key = [&](auto kval, auto vval) {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (lane + 32 * i < dh) x = ffma(q[i], kval(lane + 32 * i), x);
+        x = butterfly32(x);
+        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.0f : top, back = exp2_fast(m - base), e = exp2_fast(x - base);
+        m = top;
+        l = ffma(l, back, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (lane + 32 * i < dh) o[i] = ffma(e, vval(lane + 32 * i), o[i] * back);
+    };
+    const int psz = 1 << p.c.page_log2;
+    for (int j = 0; j < kv; ++j) {
+        const int page = page_of(p.c, p.r, s, j);
+        if (page < 0) {
+            set_err(p.err, B2_DEV_ERR_BAD_PAGE);
+            continue;
+        }
+        const size_t head = (size_t)page * p.c.KVH + kvh, cell = head * (psz >> 4) + ((j & (psz - 1)) >> 4);
+        const size_t at = (head * psz + (j & (psz - 1))) * dh;
+        const float ks = p.c.ks[cell], vs = p.c.vs[cell];
+        key([&](int d) { return (float)p.c.k[at + d] * ks; }, [&](int d) { return (float)p.c.v[at + d] * vs; });
+    }
+    const unsigned long long see = (unsigned long long)p.seen[row];
+    for (int j = 0; j < len; ++j) {
+        if (!(see >> j & 1)) continue;
+        const float* kr = p.k + (size_t)(a + j) * p.ldk + (size_t)kvh * dh;
+        const float* vr = p.v + (size_t)(a + j) * p.ldv + (size_t)kvh * dh;
+        float off = 0.0f;                                      // NaN where a key or value is not finite
+        for (int d = lane; d < dh; d += 32) off = ffma(kr[d], 0.0f, ffma(vr[d], 0.0f, off));
+        if (__any_sync(0xffffffffu, off != off)) off = __int_as_float(0x7fffffff);
+        key([&](int d) { return kr[d] + off; }, [&](int d) { return vr[d] + off; });
+    }
+    const float inv = l == 0.0f ? 0.0f : fdiv(1.0f, l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < dh) p.out[(size_t)row * p.ldo + (size_t)h * dh + lane + 32 * i] = o[i] * inv;
+}
+
+// ------------------------------------------------------------------ acceptance
+// A logit and its index as one word, so that the largest word is the largest logit's first
+// index: the value as an unsigned number in its order (a NaN below all, -0 as +0), above the
+// complement of the index.
+__device__ __forceinline__ unsigned long long logit_word(float x, unsigned i) {
+    const unsigned b = __float_as_uint(fadd(x, 0.0f)), o = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return (unsigned long long)(x == x ? o : 0u) << 32 | (0xffffffffu - i);
+}
+
+struct TreeAcceptParams {
+    PagedRows r;
+    const long long* seen;
+    const float* logits;     // [n_rows][ld]
+    long long ld;
+    int vocab, splits, chunk;   // a split: chunk logits (a multiple of 4)
+    const int* tokens;
+    int* kept_start;
+    int* kept_len;
+    int* kept_rows;
+    int* kept_ids;
+    unsigned long long* best;   // [n_rows][splits]
+    unsigned long long* paths;  // [n_seq]
+    int* ids;                   // [n_rows]
+    int* err;
+};
+
+// The largest word of a row's split: CTA (split, row). Bound by memory.
+static __global__ void __launch_bounds__(256) tree_argmax_kernel(const __grid_constant__ TreeAcceptParams p) {
+    __shared__ unsigned long long sb[8];
+    after_previous();
+    const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x;
+    if (row >= min(p.r.row_start[p.r.n_seq], p.r.n_rows)) return;      // rows of no sequence
+    const float* x = p.logits + (size_t)row * p.ld;
+    const int i0 = split * p.chunk, i1 = min(i0 + p.chunk, p.vocab);
+    unsigned long long b = 0ull;
+    // from the first 16-byte boundary on four at a time
+    const int head = min(i0 + (int)((16 - (reinterpret_cast<uintptr_t>(x + i0) & 15)) / 4 & 3), i1), body = head + (i1 - head) / 4 * 4;
+    if (i0 + tid < head) b = logit_word(x[i0 + tid], i0 + tid);
+    if (body + tid < i1) b = max(b, logit_word(x[body + tid], body + tid));
+#pragma unroll 4
+    for (int i = head + 4 * tid; i < body; i += 1024) {
+        const float4 v = *reinterpret_cast<const float4*>(x + i);
+        b = max(max(b, max(logit_word(v.x, i), logit_word(v.y, i + 1))), max(logit_word(v.z, i + 2), logit_word(v.w, i + 3)));
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    if ((tid & 31) == 0) sb[tid >> 5] = b;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) b = max(b, sb[w]);
+        // logits[0] NaN: the comparisons of the greedy choice leave 0
+        if (split == 0 && x[0] != x[0]) b = 0xffffffffffffffffull;
+        p.best[(size_t)row * p.splits + split] = b;
+    }
+}
+
+// The paths: one CTA, a warp a sequence at a time, two rows a lane; then the sums of their
+// lengths, and the kept rows in order. A path's rows ascend, so a path is a 64-bit word.
+static __global__ void __launch_bounds__(1024) tree_path_kernel(const __grid_constant__ TreeAcceptParams p) {
+    __shared__ int sums[32];
+    after_previous();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int s = warp; s < p.r.n_seq; s += 32) {
+        const SeqRows q = seq_rows(p.r, s);
+        if (p.r.row_start[s + 1] < p.r.row_start[s] && lane == 0) set_err(p.err, B2_DEV_ERR_BAD_ROWS);
+        if (q.len > kTreeRows && lane == 0) set_err(p.err, B2_DEV_ERR_TOO_MANY);
+        unsigned long long path = 0ull;
+        if (q.len > 0 && q.len <= kTreeRows) {
+            int id[2], parent[2], token[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int j = lane + 32 * u, row = q.a + j;
+                id[u] = parent[u] = token[u] = -1;
+                if (j >= q.len) continue;
+                const unsigned long long* best = p.best + (size_t)row * p.splits;
+                unsigned long long b = best[0];
+                for (int i = 1; i < p.splits; ++i) b = max(b, best[i]);
+                id[u] = (int)(0xffffffffu - (unsigned)b);
+                p.ids[row] = id[u];
+                const unsigned long long before = (unsigned long long)p.seen[row] & ((1ull << j) - 1);
+                parent[u] = 63 - __clzll((long long)before);
+                token[u] = p.tokens[row];
+            }
+            for (int at = 0; at >= 0;) {
+                path |= 1ull << at;
+                const int want = __shfl_sync(0xffffffffu, at < 32 ? id[0] : id[1], at & 31);
+                const unsigned lo = __ballot_sync(0xffffffffu, parent[0] == at && token[0] == want);
+                const unsigned hi = __ballot_sync(0xffffffffu, parent[1] == at && token[1] == want);
+                at = lo ? __ffs(lo) - 1 : hi ? __ffs(hi) + 31 : -1;
+            }
+        }
+        if (lane == 0) p.paths[s] = path;
+    }
+    __syncthreads();
+    // sums of the lengths, 1024 sequences at a time
+    int base = 0;
+    for (int s0 = 0; s0 < p.r.n_seq; s0 += 1024) {
+        const int s = s0 + tid;
+        const unsigned long long path = s < p.r.n_seq ? p.paths[s] : 0ull;
+        const int n = __popcll(path);
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        int before = base, total = 0;
+        for (int w = 0; w < 32; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+        __syncthreads();
+        if (s < p.r.n_seq) {
+            // (row ranges that overlap could keep more rows than there are)
+            const int end = min(before + incl, p.r.n_rows), a = seq_rows(p.r, s).a;
+            int at = min(end, before + incl - n);
+            if (s == 0) p.kept_start[0] = 0;
+            p.kept_start[s + 1] = end;
+            p.kept_len[s] = p.r.kv_len[s] + end - at;
+            for (unsigned long long rest = path; rest && at < end; rest &= rest - 1, ++at) {
+                const int row = a + __ffsll((long long)rest) - 1;
+                p.kept_rows[at] = row;
+                p.kept_ids[at] = p.ids[row];
+            }
+        }
+        base += total;
+    }
+}
+
+}  // namespace b2

@@ -262,6 +262,23 @@ def quantize_rows_i4(W):
     return (u[:, 0::2] | (u[:, 1::2] << 4)).astype(np.uint8), scales
 
 
+def quantize_groups_i4(W, group=128):
+    """The same with a scale for each row and group of 32, 64 or 128 columns (the last group may be shorter), for
+    runtime.gemv_i4_groups: (packed uint8 [rows, ld], scales f32 [rows, groups]), ld the packed bytes of a row rounded up
+    to 16; an odd row's last byte holds one code."""
+    if group not in (32, 64, 128):
+        raise PackError(f"groups have 32, 64 or 128 columns, not {group}")
+    W = np.asarray(W, np.float32)
+    m, n = W.shape
+    groups = -(-n // group)
+    pad = np.zeros((m, groups * group), np.float32)
+    pad[:, :n] = W
+    codes, scales = quantize_rows_i4(pad.reshape(m * groups, group))
+    packed = np.zeros((m, (n + 31) // 32 * 16), np.uint8)
+    packed[:, :(n + 1) // 2] = codes.reshape(m, -1)[:, :(n + 1) // 2]
+    return packed, scales.reshape(m, groups)
+
+
 def build_tensors(arch, collected, *, quantize="int8", int8_attention=False, int4_linear=False,
                   int4_embedding=False):
     """collected (from resolve) -> {name: array} in arch order, reference names,

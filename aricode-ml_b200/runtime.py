@@ -105,6 +105,18 @@ def _declare(L):
     L.b2_attn_paged_i8_workspace.restype = C.c_size_t
     L.b2_attn_paged_i8_workspace.argtypes = [vp, vp, C.c_int]
     L.b2_attn_paged_i8.argtypes = [vp, vp, vp, C.c_int64, vp, C.c_int64, C.c_int, vp, C.c_size_t, vp, vp]
+    L.b2_gemv_i4_groups_workspace.restype = C.c_size_t
+    L.b2_gemv_i4_groups_workspace.argtypes = [C.c_int, C.c_int]
+    L.b2_gemv_i4_groups.argtypes = [vp, C.c_int64, vp, C.c_int64, C.c_int, C.c_int, vp, C.c_int64, vp, vp, C.c_int64,
+                                    C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]
+    L.b2_attn_tree_i8_workspace.restype = C.c_size_t
+    L.b2_attn_tree_i8_workspace.argtypes = [vp, vp, C.c_int]
+    L.b2_attn_tree_i8.argtypes = [vp, vp, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, C.c_int, vp,
+                                  C.c_size_t, vp, vp]
+    L.b2_tree_accept_workspace.restype = C.c_size_t
+    L.b2_tree_accept_workspace.argtypes = [vp, C.c_int]
+    L.b2_tree_accept.argtypes = [vp, vp, C.c_int64, C.c_int, vp, vp, vp, vp, vp, vp, C.c_size_t, vp, vp]
+    L.b2_kv_append_kept_i8.argtypes = [vp, vp, vp, C.c_int, vp, C.c_int64, vp, C.c_int64, vp, C.c_float, vp, C.c_int, vp, vp]
     L.b2_argmax.argtypes = [vp, C.c_int64, vp, vp]
     L.b2_silu_mul.argtypes = [vp, vp, vp, C.c_int, vp]
     L.b2_gelu.argtypes = [vp, vp, C.c_int, vp]
@@ -380,6 +392,48 @@ def gemv_i4(W, scale, x, n, bias=None, y=None, stream=None):
     return y
 
 
+def gemv_i4_groups_workspace(T, n, device="cuda"):
+    """A workspace tensor that gemv_i4_groups calls of up to T vectors and n columns can share, one after another."""
+    import torch
+    return torch.empty(lib().b2_gemv_i4_groups_workspace(int(T), int(n)), dtype=torch.uint8, device=device)
+
+
+def gemv_i4_groups(W, scale, x, group, bias=None, y=None, workspace=None, stream=None):
+    """Products of x [n] or [T, n] f32 (rows may be strided) with 4-bit weights that have a scale for each row and group
+    of 32, 64 or 128 columns: W uint8 [m, ld] (two codes a byte, the even column in the low half, ld % 16 == 0) and scale
+    [m, ceil(n / group)] f32 or bf16, as pack.quantize_groups_i4 makes them. Returns y [m] or [T, m]. Without a workspace
+    the call makes its own."""
+    import torch
+    f32, x1 = torch.float32, x.dim() == 1
+    if x.dtype is not f32 or not x.is_cuda or x.dim() not in (1, 2) or W.dim() != 2 or scale.dim() != 2:
+        raise _invalid("x must be a float32 CUDA tensor [n] or [T, n], W and scale 2-D")
+    gpu = x.get_device()
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return gemv_i4_groups(W, scale, x, group, bias, y, workspace)
+    T, n = (1, x.shape[0]) if x1 else x.shape
+    m, ld = W.shape
+    if (x.stride(-1) != 1 and n > 1) or group not in (32, 64, 128):
+        raise _invalid("x must have contiguous rows, group be 32, 64 or 128")
+    if scale.dtype is not f32 and scale.dtype is not torch.bfloat16:
+        raise _invalid("scale must be float32 or bfloat16")
+    g = -(-n // group)
+    y = torch.empty(m if x1 else (T, m), dtype=f32, device=x.device) if y is None else y
+    if y.dtype is not f32 or y.get_device() != gpu or y.shape != ((m,) if x1 else (T, m)) or (y.stride(-1) != 1 and m > 1):
+        raise _invalid(f"y must be a float32 tensor on cuda:{gpu}, a value for each row of W and vector, rows contiguous")
+    if workspace is None:
+        workspace = gemv_i4_groups_workspace(T, n, x.device)
+    rc = lib().b2_gemv_i4_groups(
+        _tensor("W", W, torch.uint8, gpu), ld, _tensor("scale", scale, scale.dtype, gpu, (m, g)), g, scale.dtype is not f32,
+        group, x.data_ptr(), x.stride(0) if T > 1 else n, bias if bias is None else _tensor("bias", bias, f32, gpu, (m,)),
+        y.data_ptr(), y.stride(0) if T > 1 else m, m, n, T, _tensor("workspace", workspace, torch.uint8, gpu),
+        workspace.numel(), h)
+    if rc:
+        check(rc)
+    return y
+
+
 def gemm_i8(W, scale, X, bias=None, n=None, stream=None):
     """T vectors at once on the tensor cores: X [T, n] f32 -> Y [T, m]; W int8 [m, ld]."""
     import torch
@@ -457,6 +511,8 @@ KV_BLOCK = 16                    # tokens that share a scale (B2_KV_BLOCK)
 ROWS_ERRORS = {1: "a wait inside the attention kernel ran out: that call's outputs are unusable",
                2: "a position past the sequence's capacity or the rotation table",
                4: "a page-table entry outside the pool", 5: "a row_start below the one before it: row ranges that may overlap"}
+TREE_ERRORS = {**ROWS_ERRORS, 6: "a row index outside the rows it picks from",
+               7: "a sequence with more drafted rows than a tree can have"}
 
 
 class _KvPages(C.Structure):     # b2_kv_pages
@@ -516,6 +572,17 @@ def _there(torch, gpu, stream):
                 yield
 
 
+def _raise_rows_error(err, gpu):
+    """Waits for the device, and raises what the device word `err` says, which is cleared."""
+    import torch
+    torch.cuda.synchronize(gpu)
+    e = int(err.item())
+    if e:
+        err.zero_()
+        torch.cuda.synchronize(gpu)                      # cleared before the next call on any stream
+        raise B2Error(-8, TREE_ERRORS.get(e, f"device error {e}"))
+
+
 class PagedKV:
     """A pool of pages of int8 keys and values with a scale per 16 tokens and head (b2_kv_pages): k and v
     [pages, kv_heads, page_size, d_head] int8, k_scale and v_scale [pages, kv_heads, page_size / 16] f32. `err` is
@@ -552,13 +619,7 @@ class PagedKV:
     def check(self):
         """Waits for the device (calls on all its streams), and raises if a call on this cache met bad rows or pages
         (which it left out), or an attention kernel gave up a wait."""
-        import torch
-        torch.cuda.synchronize(self.gpu)
-        e = int(self.err.item())
-        if e:
-            self.err.zero_()
-            torch.cuda.synchronize(self.gpu)             # cleared before the next call on any stream
-            raise B2Error(-8, ROWS_ERRORS.get(e, f"device error {e}"))
+        _raise_rows_error(self.err, self.gpu)
 
 
 class KVRows:
@@ -732,6 +793,185 @@ def attn_paged_i8(kv, rows, q, out=None, workspace=None, stream=None):
     if rc:
         check(rc)
     return out
+
+
+# ----------------------------------------------------------------- trees of drafted tokens
+TREE_ROWS = 64                   # most drafted rows of a sequence (B2_TREE_ROWS)
+
+
+class _TreeRows(C.Structure):    # b2_tree_rows
+    _fields_ = [("row_start", vp), ("kv_len", vp), ("page_table", vp), ("seen", vp), ("n_seq", C.c_int32),
+                ("max_pages", C.c_int32), ("n_rows", C.c_int32), ("max_keys", C.c_int32), ("max_rows", C.c_int32)]
+
+
+def tree_seen(parents):
+    """What each row of a tree sees, as a list of 64-bit integers for TreeRows' `seen`: itself and its ancestors.
+    parents[i] is the row before i that row i follows, or -1."""
+    out = []
+    if len(parents) > TREE_ROWS:
+        raise _invalid(f"a tree has at most {TREE_ROWS} rows")
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise _invalid("a row's parent must be a row before it, or -1")
+        out.append((out[p] if p >= 0 else 0) | 1 << i)
+    return [x - (1 << 64) if x >> 63 else x for x in out]
+
+
+class TreeRows:
+    """The drafted rows of a call (b2_tree_rows): int32 tensors row_start [n_seq + 1], kv_len [n_seq] (cached keys, the
+    drafted rows not among them) and page_table [n_seq, max_pages], and seen [n_rows] int64 (bit j of a row's word: it sees
+    row j of its sequence; tree_seen makes them). They are read when the kernels run: refill them in place to replay a
+    captured call. max_keys bounds every kv_len (0: what the table can hold); max_rows says how many rows the longest
+    sequence has, if that is known (0: up to 64)."""
+
+    def __init__(self, row_start, kv_len, page_table, seen, n_rows, max_keys=0, max_rows=0):
+        import torch
+        _tensor("kv_len", kv_len, torch.int32, None)
+        self.device, self.gpu = kv_len.device, kv_len.get_device()
+        if kv_len.dim() != 1 or page_table.dim() != 2:
+            raise _invalid("kv_len must be 1-D and page_table 2-D")
+        n = kv_len.shape[0]
+        _tensor("row_start", row_start, torch.int32, self.gpu, (n + 1,))
+        _tensor("page_table", page_table, torch.int32, self.gpu, (n, page_table.shape[1]))
+        if not 0 <= n_rows <= INT32_MAX or max_keys < 0 or max_rows < 0:
+            raise _invalid("n_rows must be 0 to 2^31 - 1, max_keys and max_rows not negative")
+        _tensor("seen", seen, torch.int64, self.gpu, (n_rows,))
+        self.row_start, self.kv_len, self.page_table, self.seen = row_start, kv_len, page_table, seen
+        self.n_rows, self.n_seq, self.max_rows = int(n_rows), n, int(max_rows)
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._c = _TreeRows(row_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), seen.data_ptr(), n,
+                            page_table.shape[1], self.n_rows, min(int(max_keys), INT32_MAX), min(self.max_rows, INT32_MAX))
+        self._p, self._err = C.addressof(self._c), self.err.data_ptr()
+
+    def check(self):
+        """Waits for the device, and raises if a tree_accept of these rows met bad ones (which it left out)."""
+        _raise_rows_error(self.err, self.gpu)
+
+
+class TreeKept:
+    """What tree_accept keeps of a TreeRows: int32 tensors start [n_seq + 1] (sums of the path lengths), kv_len [n_seq]
+    (cached keys with the paths), rows and ids [n_rows] (path after path: rows of the call and the greedy token after each,
+    the last of a path being the next token). Made here where none are given; kv_len may be the tree's own, which then
+    counts the path when the call is done. `kv_rows` are the kept rows as the cache's calls take them."""
+
+    def __init__(self, tree, start=None, kv_len=None, rows=None, ids=None):
+        import torch
+
+        def made(name, t, n):
+            if t is None:
+                return torch.zeros(n, dtype=torch.int32, device=tree.device)
+            _tensor(name, t, torch.int32, tree.gpu, (n,))
+            return t
+        self.tree = tree
+        self.start, self.kv_len = made("start", start, tree.n_seq + 1), made("kv_len", kv_len, tree.n_seq)
+        self.rows, self.ids = made("rows", rows, tree.n_rows), made("ids", ids, tree.n_rows)
+        self.kv_rows = KVRows(self.start, self.kv_len, tree.page_table, tree.n_rows, max_rows=tree.max_rows)
+
+
+def attn_tree_workspace(kv, tree, n_heads, stream=None):
+    """A workspace tensor that attn_tree_i8 calls of these sizes can share, one after another."""
+    import torch
+    if _here(torch, kv.gpu, stream) is None:
+        with _there(torch, kv.gpu, stream):
+            return attn_tree_workspace(kv, tree, n_heads)
+    return torch.empty(lib().b2_attn_tree_i8_workspace(kv._p, tree._p, int(n_heads)), dtype=torch.uint8, device=kv.device)
+
+
+def attn_tree_i8(kv, tree, q, k, v, out=None, workspace=None, stream=None):
+    """Attention of the drafted rows q [n_rows, heads * d_head] f32 (rotated and pre-scaled): each over all cached keys of
+    its sequence and those drafted rows k, v [n_rows, kv_heads * d_head] f32 (keys rotated) that it sees. Rows that belong
+    to no sequence stay as they were in `out` (unset in a new one). Without a workspace the call makes its own."""
+    import torch
+    gpu, n, f32 = kv.gpu, tree.n_rows, torch.float32
+    if tree.gpu != gpu:
+        raise _invalid("the cache and the rows must be on one device")
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return attn_tree_i8(kv, tree, q, k, v, out, workspace)
+    w, kw = q.shape[-1], kv.n_kv_heads * kv.d_head
+    H = w // kv.d_head
+    if w != H * kv.d_head:
+        raise _invalid("q must hold whole heads")
+    qp, ldq = _f32_rows("q", q, f32, gpu, n, w)
+    kp, ldk = _f32_rows("k", k, f32, gpu, n, kw)
+    v_, ldv = _f32_rows("v", v, f32, gpu, n, kw)
+    out = torch.empty(q.shape[0], w, dtype=f32, device=q.device) if out is None else out
+    op, ldo = _f32_rows("out", out, f32, gpu, n, w)
+    if workspace is None:
+        workspace = attn_tree_workspace(kv, tree, H)
+    rc = lib().b2_attn_tree_i8(kv._p, tree._p, qp, ldq, kp, ldk, v_, ldv, op, ldo, H,
+                               _tensor("workspace", workspace, torch.uint8, gpu), workspace.numel(), kv._err, h)
+    if rc:
+        check(rc)
+    return out
+
+
+def tree_accept_workspace(tree, vocab, stream=None):
+    """A workspace tensor that tree_accept calls of these sizes can share, one after another."""
+    import torch
+    if _here(torch, tree.gpu, stream) is None:
+        with _there(torch, tree.gpu, stream):
+            return tree_accept_workspace(tree, vocab)
+    return torch.empty(lib().b2_tree_accept_workspace(tree._p, int(vocab)), dtype=torch.uint8, device=tree.device)
+
+
+def tree_accept(tree, logits, tokens, kept=None, workspace=None, stream=None):
+    """The path of each sequence's tree that the greedy choice confirms, from its first row on (which is always kept):
+    logits [n_rows, vocab] f32 (rows may be strided) and tokens [n_rows] int32, the drafted ones. Fills and returns
+    `kept`, a TreeKept of this tree (a new one where none is given). Entries of kept.rows and kept.ids behind the last path
+    stay as they were. tree.check() tells of bad rows met on the way."""
+    import torch
+    gpu, n = tree.gpu, tree.n_rows
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return tree_accept(tree, logits, tokens, kept, workspace)
+    if kept is None:
+        kept = TreeKept(tree)
+    elif kept.tree is not tree:
+        raise _invalid("kept must be made for this tree")
+    if logits.dtype is not torch.float32 or logits.dim() != 2 or logits.get_device() != gpu or logits.shape[0] < n or (
+            logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise _invalid(f"logits must be a 2-D float32 tensor on cuda:{gpu} with {n} rows of contiguous elements")
+    vocab = logits.shape[1]
+    if workspace is None:
+        workspace = tree_accept_workspace(tree, vocab)
+    rc = lib().b2_tree_accept(tree._p, logits.data_ptr(), logits.stride(0) if logits.shape[0] > 1 else vocab, vocab,
+                              _tensor("tokens", tokens, torch.int32, gpu, (n,)), kept.start.data_ptr(), kept.kv_len.data_ptr(),
+                              kept.rows.data_ptr(), kept.ids.data_ptr(), _tensor("workspace", workspace, torch.uint8, gpu),
+                              workspace.numel(), tree._err, h)
+    if rc:
+        check(rc)
+    return kept
+
+
+def kv_append_kept_i8(kv, kept, k, v, table=None, k_gain=None, eps=1e-5, stream=None):
+    """Append the rows that tree_accept kept to the cache: of the drafted rows k and v [rows, kv_heads * d_head] f32 those
+    that kept.rows names, keys normed (k_gain) and rotated (table, at the position that a row has in the path) on the way."""
+    import torch
+    gpu, d, f32 = kv.gpu, kv.d_head, torch.float32
+    rows = kept.kv_rows
+    if rows.gpu != gpu:
+        raise _invalid("the cache and the rows must be on one device")
+    h = _here(torch, gpu, stream)
+    if h is None:
+        with _there(torch, gpu, stream):
+            return kv_append_kept_i8(kv, kept, k, v, table, k_gain, eps)
+    w, n = kv.n_kv_heads * d, k.shape[0]
+    kp, ldk = _f32_rows("k", k, f32, gpu, 0, w)
+    v_, ldv = _f32_rows("v", v, f32, gpu, n, w)
+    t_rows = 0
+    if table is not None:
+        if table.dim() != 2:
+            raise _invalid("table must be [positions, d_head]")
+        t_rows = table.shape[0]
+        table = _tensor("table", table, f32, gpu, (t_rows, d))
+    rc = lib().b2_kv_append_kept_i8(
+        kv._p, rows._p, kept.rows.data_ptr(), n, kp, ldk, v_, ldv,
+        k_gain if k_gain is None else _tensor("k_gain", k_gain, f32, gpu, (d,)), eps, table, t_rows, kv._err, h)
+    if rc:
+        check(rc)
 
 
 def argmax(v, stream=None):

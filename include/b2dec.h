@@ -208,6 +208,25 @@ int b2_gemv_i8_rowscale(const int8_t* W, int64_t ld, const float* scale, const f
 int b2_gemv_i4_rowscale(const uint8_t* W, int64_t ld, const float* scale, const float* x, const float* bias,
                         float* y, int m, int n, void* stream);
 
+/* Products with 4-bit weights that have a scale for each row and group of columns:
+ * Y[t][j] = sum_g scale[j][g] * sum_{k in g} W[j][k] X[t][k] (+ bias[j]). W is packed
+ * as above (signed codes, two a byte, the even column in the low half; n may be odd),
+ * rows ld bytes apart, 16-byte aligned, ld % 16 == 0, what lies past n is not used.
+ * group: 32, 64 or 128 columns, the last one may be shorter. scale [m][lds] f32, or
+ * bf16 where scale_bf16 is set. X [T][ldx], Y [T][ldy] f32, 4-byte aligned; Y overlaps
+ * nothing that is read. For one token or a few (a tree of drafted tokens, a few
+ * sequences); more than 64 read the weights once for every 64. Precision: a vector's
+ * elements are held to 2^-24 of the largest of each 128 neighbours, codes, products and
+ * their sums over a group are exact, the rest f32. A NaN or infinity makes the outputs of
+ * its vector NaN.
+ * workspace: b2_gemv_i4_groups_workspace() bytes (may be 0), 16-byte aligned, no
+ * initialisation; calls that may overlap on the GPU need one each. No counterpart in
+ * the reference, whose 4-bit rows have one scale (arr_i4_matvec_f32_perrow). */
+size_t b2_gemv_i4_groups_workspace(int T, int n);
+int b2_gemv_i4_groups(const uint8_t* W, int64_t ld, const void* scale, int64_t lds, int scale_bf16, int group,
+                      const float* X, int64_t ldx, const float* bias, float* Y, int64_t ldy, int m, int n, int T,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* The same for T input vectors at once, on the tensor cores (tcgen05 kind::i8
  * over the byte planes of each vector's fixed-point copy): Y[t][j] = scale[j] *
  * dot(W[j,:], X[t,:]) (+ bias[j]), bit-identical to T calls of
@@ -361,6 +380,73 @@ int b2_kv_read_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, void* k_out, vo
 size_t b2_attn_paged_i8_workspace(const b2_kv_pages* kv, const b2_kv_rows* rows, int n_heads);
 int b2_attn_paged_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const float* q, int64_t ldq, float* out,
                      int64_t ldo, int n_heads, void* workspace, size_t workspace_bytes, int32_t* err, void* stream);
+
+/* ---- trees of drafted tokens over the paged cache
+ * A step that checks several drafted tokens of a sequence at once. The drafted rows'
+ * keys and values stay outside the cache (f32 rows of the call), so that a rejected one
+ * never coarsens a block's scale: b2_attn_tree_i8 attends to the cache and to them,
+ * b2_tree_accept finds the path that the logits confirm, b2_kv_append_kept_i8 writes
+ * that path's rows. No counterpart in the reference, which decodes a token at a time.
+ *
+ * Sequence s has rows row_start[s] .. row_start[s + 1] - 1 (up to 64, possibly none)
+ * and kv_len[s] cached keys, its rows not among them. Bit j of seen[i]: row i sees row
+ * j of its sequence; its own bit is set like any other's, bits past the sequence's rows
+ * say nothing. A row's parent is the last row before it that it sees, so the rows of a
+ * tree are listed parents first, each seeing its ancestors and itself.
+ * All of it is read on the device only; what is wrong there is left out and flagged as
+ * above, besides
+ *   B2_TREE_BAD_ROW   a row index outside the buffer (b2_kv_append_kept_i8)
+ *   B2_TREE_TOO_MANY  a sequence of more than 64 rows: none of its rows is looked at */
+enum { B2_TREE_BAD_ROW = 6, B2_TREE_TOO_MANY = 7 };
+#define B2_TREE_ROWS 64
+
+typedef struct b2_tree_rows {
+    const int32_t* row_start;   /* device [n_seq + 1], not decreasing */
+    const int32_t* kv_len;      /* device [n_seq]: cached keys */
+    const int32_t* page_table;  /* device [n_seq][max_pages] */
+    const int64_t* seen;        /* device [n_rows], 8-byte aligned */
+    int32_t n_seq;              /* as in b2_kv_rows, like the rest */
+    int32_t max_pages;
+    int32_t n_rows;
+    int32_t max_keys;
+    int32_t max_rows;           /* a hint: the most rows of one sequence (0: 64) */
+} b2_tree_rows;
+
+/* Attention of the drafted rows: q [n_rows][ldq] (rotated and pre-scaled, n_heads heads),
+ * k and v [n_rows][n_kv_heads * d_head] (keys rotated), out [n_rows][ldo]. Row i attends to
+ * all cached keys of its sequence and to the rows that seen[i] names; a row that sees
+ * nothing becomes zeros, rows behind the last sequence stay as they were. Cached keys on
+ * a page outside the pool are left out. A drafted key or value row with a NaN or infinity
+ * makes NaN of every row that sees it, and of no other. Outputs may not overlap inputs.
+ * workspace: b2_attn_tree_i8_workspace() bytes (may be 0), 16-byte aligned, no
+ * initialisation; calls that may overlap on the GPU need one each. */
+size_t b2_attn_tree_i8_workspace(const b2_kv_pages* kv, const b2_tree_rows* tree, int n_heads);
+int b2_attn_tree_i8(const b2_kv_pages* kv, const b2_tree_rows* tree, const float* q, int64_t ldq, const float* k,
+                    int64_t ldk, const float* v, int64_t ldv, float* out, int64_t ldo, int n_heads, void* workspace,
+                    size_t workspace_bytes, int32_t* err, void* stream);
+
+/* The path that the greedy choice confirms. A row's id is the first index of its largest
+ * logit as b2_argmax has it (logits [n_rows][ld], vocab of them). From a sequence's row 0
+ * on, which is always kept (the token known before the step), the path goes on to the
+ * first row whose parent is the current one and whose token (tokens [n_rows]) is the
+ * current one's id. Out: kept_start [n_seq + 1], the sums of the path lengths; kept_len
+ * [n_seq] = kv_len + path length (may be kv_len itself); kept_rows and kept_ids [n_rows],
+ * path after path: the rows of the call and their ids, of which the last of a path is the
+ * next token. Entries behind the last path stay as they were. page_table is not used.
+ * workspace: b2_tree_accept_workspace() bytes, 16-byte aligned, no initialisation; calls
+ * that may overlap on the GPU need one each. */
+size_t b2_tree_accept_workspace(const b2_tree_rows* tree, int vocab);
+int b2_tree_accept(const b2_tree_rows* tree, const float* logits, int64_t ld, int vocab, const int32_t* tokens,
+                   int32_t* kept_start, int32_t* kept_len, int32_t* kept_rows, int32_t* kept_ids, void* workspace,
+                   size_t workspace_bytes, int32_t* err, void* stream);
+
+/* b2_kv_append_i8 of picked rows: row i of the call is row row_index[i] (device [n_rows])
+ * of k and v, which have n_src rows; it stands where row i of `rows` stands. With
+ * b2_tree_accept's outputs: row_start = kept_start, kv_len = kept_len, row_index =
+ * kept_rows. A row index outside 0 .. n_src - 1 writes zeros. */
+int b2_kv_append_kept_i8(const b2_kv_pages* kv, const b2_kv_rows* rows, const int32_t* row_index, int n_src,
+                         const float* k, int64_t ldk, const float* v, int64_t ldv, const float* k_gain, float eps,
+                         const float* table, int table_rows, int32_t* err, void* stream);
 
 /* out[0] = first index of the maximum (NaN never wins; logits[0] NaN -> 0).
  * Replaces: sample_greedy_f32 (sampling_f32.ari:10-24). */
