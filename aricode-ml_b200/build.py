@@ -22,7 +22,7 @@ OBJ = CSRC / "_obj"
 LIB = PKG / "libb2dec.so"
 FRONT = PKG / "b2run"                    # stdin-tokens front end (host program over the library)
 SOURCES = ["runtime.cu", "launch.cu", "token.cu", "prefill.cu", "capi.cu", "noalloc.cu", "paged.cu", "tree.cu", "groups.cu"]
-HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "paged_rows.cuh", "paged_host.cuh",
+HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "mma_digits.cuh", "paged_rows.cuh", "paged_host.cuh",
            "host_checks.cuh", "tree.cuh", "groups.cuh", "umma.cuh", "json.h"]
 
 NVCC_FLAGS = [

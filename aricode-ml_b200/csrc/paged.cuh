@@ -8,6 +8,7 @@
 // starts and pages are read on the device only (a captured launch replays with new
 // ones); every value is checked before it becomes an address.
 #pragma once
+#include "mma_digits.cuh"
 #include "paged_rows.cuh"
 #include "umma.cuh"
 
@@ -480,40 +481,6 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
 // The digit sums are exact in int32 and are joined in f32, so a score or an output carries
 // the error of one 23-bit rounding per factor instead of a chain of f32 roundings, at a
 // third of the int8 rate and without converting a single code.
-// Three digits in [-128, 127] reach 2^23 - 1 - 0x8080 = 8355711; a little below it,
-// so that the roundings of factor and product stay inside
-constexpr int kDigitMax = 8355700;
-
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// the first of a chain: from zero, so that nothing has to be cleared
-__device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                             uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
-}
-
-// rint(x f) + 0x8080 for |x f| <= kDigitMax, in the low 24 bits
-__device__ __forceinline__ uint32_t digit_bits(float x, float f) { return (uint32_t)__float2int_rn(x * f) + 0x8080u; }
-// the same for x >= 0 in one operation: the f32 addition rounds x f to an integer
-constexpr float kDigitBase = 8388608.0f + (float)0x8080;
-__device__ __forceinline__ uint32_t digit_bits_pos(float x, float f) { return __float_as_uint(ffma(x, f, kDigitBase)); }
-
-// digits of four integers given as digit_bits: word e of d holds digit e of each in its bytes
-__device__ __forceinline__ void digits4(uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3, uint32_t (&d)[3]) {
-    const uint32_t l = __byte_perm(y0, y1, 0x5140), m = __byte_perm(y2, y3, 0x5140);
-    d[0] = __byte_perm(l, m, 0x5410) ^ 0x80808080u;
-    d[1] = __byte_perm(l, m, 0x7632) ^ 0x80808080u;
-    d[2] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
-}
-
 // d2 65536 + d1 256 + d0 of two neighbouring sums a, b: the lower two digits joined as
 // integers (256 products: below 2^30)
 __device__ __forceinline__ f32x2 join_digits(int a2, int b2, int a1, int b1, int a0, int b0) {
@@ -521,13 +488,6 @@ __device__ __forceinline__ f32x2 join_digits(int a2, int b2, int a1, int b1, int
 }
 __device__ __forceinline__ f32x2 join_digits(const int (&c)[3][4], int y) {
     return join_digits(c[2][y], c[2][y + 1], c[1][y], c[1][y + 1], c[0][y], c[0][y + 1]);
-}
-
-// the factor that takes values up to `top` (>= 0) to integers up to kDigitMax; tiny
-// tops (below 1e-31) keep fewer bits, 0 gives 0, NaN and infinity NaN
-__device__ __forceinline__ float digit_factor(float top) {
-    if (!(top < __int_as_float(0x7f800000))) return __int_as_float(0x7fffffff);
-    return top > 0.0f ? fminf(fdiv((float)kDigitMax, top), 0x1p126f) : 0.0f;
 }
 
 // the same for weights, whose largest is a probability times a value scale: the

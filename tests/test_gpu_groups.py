@@ -1,9 +1,10 @@
 """gemv_i4_groups against its formula in 64 bits.
 
 Tolerance. u = 2^-24 is half a step of f32, A = sum |s c x| over a row, B the same with each |x| replaced by the largest of
-its 128 neighbours. A vector's elements are rounded to 2^-24 of that largest (B u); a group's sum is exact, or at most nine
+its 128 neighbours. A vector's elements are rounded to 2^-24 of that largest (B u), or
+to 2^-127 where that is more (the factor that makes them integers is 2^126 at most): 2^-127 C, C the sum of |s c|; a group's sum is exact, or at most nine
 f32 roundings of its terms; its conversion, the joining of partial sums, the scale and each addition of a group's result to
-the row's are roundings of at most A; the bias one more: u (B + (groups + 17) A + |y|)."""
+the row's are roundings of at most A; the bias one more: u (B + (groups + 17) A + |y|) + 2^-127 C."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -39,7 +40,7 @@ def product64(torch, W, scale, x, group, bias=None):
     top = torch.nn.functional.pad(xd.abs(), (0, -n % 128)).unflatten(1, (-1, 128)).amax(-1).repeat_interleave(128, 1)[:, :n]
     y = xd @ w.T + (0 if bias is None else bias.double())
     a, b = xd.abs() @ w.abs().T, top @ w.abs().T
-    return y, U * (b + (scale.shape[1] + 17) * a + 2 * y.abs())
+    return y, U * (b + (scale.shape[1] + 17) * a + 2 * y.abs()) + 2.0 ** -127 * w.abs().sum(1)
 
 
 def close(got, want, tol):
@@ -49,7 +50,8 @@ def close(got, want, tol):
 
 SHAPES = [(1, 1, 1), (1, 32, 1), (7, 31, 2), (16, 128, 1), (17, 130, 3), (64, 257, 1), (130, 4096, 1), (100, 1000, 5),
           (333, 1111, 8), (257, 2048, 13), (128, 4098, 16), (129, 640, 17), (300, 5632, 33), (148, 11008, 64), (65, 384, 65),
-          (40, 96, 200), (5000, 64, 1), (4099, 160, 7), (20, 16384, 2), (3, 16001, 9)]
+          (40, 96, 200), (5000, 64, 1), (4099, 160, 7), (20, 16384, 2), (3, 16001, 9), (18, 30000, 1),
+          (5, 40002, 7)]
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
