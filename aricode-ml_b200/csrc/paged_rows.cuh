@@ -112,4 +112,83 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// Joins the n partial results [dh + 4] (o, m in base 2, l) at `base` of one (row, head) into `out`
+// (nullptr: the warp has none and only meets the others): by WPH warps of a CTA of 8, this
+// one number `part` of them, part w the splits w, w + WPH, ..., then the warps in order. The
+// maxima and sums are read a lane each, so that the partial outputs' loads depend on
+// nothing and overlap.
+template <int WPH>
+__device__ __forceinline__ void join_splits(const float* base, int n, int dh, int part, int warp, int lane, float (&so)[8][256],
+                                            float (&sm)[8][2], float* out) {
+    const int stride = dh + 4;
+    float M = -INFINITY, L = 0.0f;
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int s0 = part; s0 < n; s0 += 32 * WPH) {                  // 32 of this warp's splits at a time
+        const int s = s0 + lane * WPH;
+        const bool live = s < n;
+        const float ms = live ? base[(size_t)s * stride + dh] : -INFINITY, ls = live ? base[(size_t)s * stride + dh + 1] : 0.0f;
+        float top = ms;
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, M);
+        const float B = top == -INFINITY ? 0.0f : top, back = exp2_fast(M - B), e = live ? exp2_fast(ms - B) : 0.0f;
+        M = top;
+        float add = e * ls;
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) add += __shfl_xor_sync(0xffffffffu, add, x);
+        L = ffma(L, back, add);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { acc[i].x *= back; acc[i].y *= back; acc[i].z *= back; acc[i].w *= back; }
+        const int cnt = min((n - s0 + WPH - 1) / WPH, 32);
+#pragma unroll 8
+        for (int k = 0; k < cnt; ++k) {
+            const float w = __shfl_sync(0xffffffffu, e, k);
+            const float* ps = base + (size_t)(s0 + k * WPH) * stride;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = 4 * lane + 128 * i;
+                if (d >= dh) continue;
+                const float4 x = *reinterpret_cast<const float4*>(ps + d);
+                acc[i].x = ffma(x.x, w, acc[i].x); acc[i].y = ffma(x.y, w, acc[i].y);
+                acc[i].z = ffma(x.z, w, acc[i].z); acc[i].w = ffma(x.w, w, acc[i].w);
+            }
+        }
+    }
+    if constexpr (WPH > 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (4 * lane + 128 * i < dh) *reinterpret_cast<float4*>(&so[warp][4 * lane + 128 * i]) = acc[i];
+        if (lane == 0) { sm[warp][0] = M; sm[warp][1] = L; }
+        __syncthreads();
+        if (part != 0) return;
+        M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WPH; ++w) M = fmaxf(M, sm[warp + w][0]);
+        const float B = M == -INFINITY ? 0.0f : M;
+        L = 0.0f;
+        acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WPH; ++w) {
+            const float e = exp2_fast(sm[warp + w][0] - B);
+            L = ffma(sm[warp + w][1], e, L);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (4 * lane + 128 * i >= dh) continue;
+                const float4 x = *reinterpret_cast<const float4*>(&so[warp + w][4 * lane + 128 * i]);
+                acc[i].x = ffma(x.x, e, acc[i].x); acc[i].y = ffma(x.y, e, acc[i].y);
+                acc[i].z = ffma(x.z, e, acc[i].z); acc[i].w = ffma(x.w, e, acc[i].w);
+            }
+        }
+    }
+    if (!out) return;
+    const float inv = L == 0.0f ? 0.0f : fdiv(1.0f, L);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int d = 4 * lane + 128 * i;
+        if (d < dh)
+            *reinterpret_cast<float4*>(out + d) =
+                make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+    }
+}
+
 }  // namespace b2

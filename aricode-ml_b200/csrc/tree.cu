@@ -33,6 +33,43 @@ bool tree_view(const char* fn, const b2_kv_pages* kv, const b2_tree_rows* t, Pag
     return view(fn, kv, &rows, c, r) && tree_view(fn, t, r);
 }
 
+// Columns of an item: 16 where no sequence has more (one token, short chains without shared heads), else as many
+// as the tensor memory and shared memory hold.
+int tree_columns(const TreeAttnParams& p, int max_rows) {
+    const int rows = std::min(max_rows > 0 ? std::min(max_rows, kTreeRows) : kTreeRows, p.r.n_rows);
+    return rows * p.G <= 16 ? 16 : p.c.dh > 128 ? 32 : 64;
+}
+
+// Keys of a split: enough items for eight rounds of the GPU, of 256 keys at least. The host does not know the
+// lengths; the sizes that it knows bound the partial results.
+void tree_plan(TreeAttnParams& p, int nc) {
+    const long long tiles = std::max((long long)p.r.n_rows * p.G / nc, (long long)std::min(p.r.n_seq, p.r.n_rows)) * p.c.KVH;
+    const long long want = std::max(1ll, std::min({8ll * 148 / std::max(tiles, 1ll), (p.r.cap + 255ll) / 256, 1024ll}));
+    p.kc_log2 = 8;
+    while (p.kc_log2 < 30 && (want << p.kc_log2) < p.r.cap) ++p.kc_log2;
+    p.nsplit = std::max(1, (int)((p.r.cap + (1ll << p.kc_log2) - 1) >> p.kc_log2));
+}
+
+// items that the call can have at most
+long long tree_items(const TreeAttnParams& p, int nc) {
+    return ((long long)p.r.n_rows * p.G / nc + std::min(p.r.n_seq, p.r.n_rows)) * p.c.KVH * p.nsplit;
+}
+
+size_t tree_bytes(const TreeAttnParams& p) {
+    return p.nsplit > 1 ? (size_t)p.r.n_rows * p.H * p.nsplit * (p.c.dh + 4) * sizeof(float) : 0;
+}
+
+template <int DP, int NC>
+cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
+    auto k = tree_attn_kernel<DP, NC>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeShape<DP, NC>::Alloc);
+    if (e != cudaSuccess) return e;
+    e = launch_ex(k, dim3((unsigned)std::min<long long>(tree_items(p, NC), sm_count())), dim3(kTreeThreads), TreeShape<DP, NC>::Alloc, s, true, p);
+    if (e != cudaSuccess || p.nsplit == 1) return e;
+    if (p.nsplit <= 8) return launch_ex(tree_join_kernel<1>, dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
+    return launch_ex(tree_join_kernel<8>, dim3((unsigned)p.r.n_rows, (unsigned)p.H), dim3(256), 0, s, true, p);
+}
+
 // Splits of a row's logits: enough CTAs for the GPU, at least 2048 logits each.
 int accept_splits(const b2_tree_rows* t, int vocab) {
     const int want = std::max(1, 4 * 148 / std::max(t->n_rows, 1));
@@ -50,7 +87,10 @@ extern "C" {
 size_t b2_attn_tree_i8_workspace(const b2_kv_pages* kv, const b2_tree_rows* tree, int n_heads) {
     TreeAttnParams p{};
     if (!tree_view("b2_attn_tree_i8_workspace", kv, tree, p.c, p.r) || n_heads <= 0 || n_heads % kv->n_kv_heads) return 0;
-    return 0;
+    if (p.r.n_rows == 0 || p.r.n_seq == 0) return 0;
+    p.H = n_heads; p.G = n_heads / kv->n_kv_heads;
+    tree_plan(p, tree_columns(p, tree->max_rows));
+    return tree_bytes(p);
 }
 
 int b2_attn_tree_i8(const b2_kv_pages* kv, const b2_tree_rows* tree, const float* q, int64_t ldq, const float* k,
@@ -74,8 +114,17 @@ int b2_attn_tree_i8(const b2_kv_pages* kv, const b2_tree_rows* tree, const float
     p.q = q; p.k = k; p.v = v; p.out = out;
     p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
     p.H = n_heads; p.G = n_heads / kv->n_kv_heads; p.err = err;
-    return status(fn, launch_ex(tree_attn_kernel, dim3((unsigned)p.r.n_rows, (unsigned)((n_heads + 7) / 8)), dim3(256), 0,
-                                static_cast<cudaStream_t>(stream), true, p));
+    const int nc = tree_columns(p, tree->max_rows);
+    tree_plan(p, nc);
+    if (tree_items(p, nc) >= (1ll << 31)) return refuse(fn, "too many (row, head, split) pieces for one call: use fewer rows or a smaller max_keys");
+    const size_t need = tree_bytes(p);
+    if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
+        return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+    p.part = static_cast<float*>(workspace);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (p.c.dh <= 64) return status(fn, nc == 16 ? launch_tree<64, 16>(p, s) : launch_tree<64, 64>(p, s));
+    if (p.c.dh <= 128) return status(fn, nc == 16 ? launch_tree<128, 16>(p, s) : launch_tree<128, 64>(p, s));
+    return status(fn, nc == 16 ? launch_tree<256, 16>(p, s) : launch_tree<256, 32>(p, s));
 }
 
 size_t b2_tree_accept_workspace(const b2_tree_rows* tree, int vocab) {

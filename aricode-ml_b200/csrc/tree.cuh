@@ -1,104 +1,12 @@
-// tree.cuh — trees of drafted tokens over the paged 8-bit KV cache: attention to the cache
-// and to the drafted rows, acceptance of a path (sm_100a).
-//
-// A call's rows are ragged as in paged_rows.cuh, except that kv_len counts the cached keys
-// alone: the drafted rows' keys and values are f32 rows of the call. Up to 64 rows a
-// sequence, so that what a row sees of them is one 64-bit word.
+// tree.cuh — trees of drafted tokens: acceptance of the path that the logits confirm
+// (sm_100a). A call's rows are ragged as in paged_rows.cuh, except that kv_len counts the
+// cached keys alone. Up to 64 rows a sequence, so that what a row sees of them is one 64-bit
+// word. (The attention is in tree_attn.cuh.)
 #pragma once
-#include "paged_rows.cuh"
+#include "tree_attn.cuh"
 
 namespace b2 {
 
-constexpr int kTreeRows = 64;
-
-struct TreeAttnParams {
-    PagedKv c;
-    PagedRows r;             // kv_len: cached keys
-    const long long* seen;   // [n_rows]
-    const float* q;          // [n_rows][ldq], rotated and pre-scaled
-    const float* k;          // [n_rows][ldk], rotated
-    const float* v;          // [n_rows][ldv]
-    float* out;              // [n_rows][ldo]
-    long long ldq, ldk, ldv, ldo;
-    int H, G;                // G = H / KVH
-    int* err;
-};
-
-// One warp a (row, head): every key in turn, lanes over d_head.
-static __global__ void __launch_bounds__(256) tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
-    after_previous();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.c.dh;
-    const int row = blockIdx.x, h = blockIdx.y * 8 + warp;
-    int s = -1, a = 0, len = 0, kv = 0;
-    for (int base = 0; base < p.r.n_seq && s < 0; base += 32) {
-        SeqRows q{0, 0, 0};
-        if (base + lane < p.r.n_seq) q = seq_rows(p.r, base + lane);
-        const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
-        if (m) {
-            const int src = __ffs(m) - 1;
-            s = base + src;
-            a = __shfl_sync(0xffffffffu, q.a, src);
-            len = __shfl_sync(0xffffffffu, q.len, src);
-            kv = __shfl_sync(0xffffffffu, q.kv, src);
-        }
-    }
-    if (s < 0 || h >= p.H) return;
-    if (len > kTreeRows) {
-        set_err(p.err, B2_DEV_ERR_TOO_MANY);
-        return;
-    }
-    if (kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
-    kv = min(kv, p.r.cap);
-    const int kvh = h / p.G;
-    float q[8], o[8], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        q[i] = d < dh ? p.q[(size_t)row * p.ldq + (size_t)h * dh + d] * 1.4426950408889634f : 0.0f;
-        o[i] = 0.0f;
-    }
-    auto key = [&](auto kval, auto vval) {
-        float x = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < dh) x = ffma(q[i], kval(lane + 32 * i), x);
-        x = butterfly32(x);
-        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.0f : top, back = exp2_fast(m - base), e = exp2_fast(x - base);
-        m = top;
-        l = ffma(l, back, e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < dh) o[i] = ffma(e, vval(lane + 32 * i), o[i] * back);
-    };
-    const int psz = 1 << p.c.page_log2;
-    for (int j = 0; j < kv; ++j) {
-        const int page = page_of(p.c, p.r, s, j);
-        if (page < 0) {
-            set_err(p.err, B2_DEV_ERR_BAD_PAGE);
-            continue;
-        }
-        const size_t head = (size_t)page * p.c.KVH + kvh, cell = head * (psz >> 4) + ((j & (psz - 1)) >> 4);
-        const size_t at = (head * psz + (j & (psz - 1))) * dh;
-        const float ks = p.c.ks[cell], vs = p.c.vs[cell];
-        key([&](int d) { return (float)p.c.k[at + d] * ks; }, [&](int d) { return (float)p.c.v[at + d] * vs; });
-    }
-    const unsigned long long see = (unsigned long long)p.seen[row];
-    for (int j = 0; j < len; ++j) {
-        if (!(see >> j & 1)) continue;
-        const float* kr = p.k + (size_t)(a + j) * p.ldk + (size_t)kvh * dh;
-        const float* vr = p.v + (size_t)(a + j) * p.ldv + (size_t)kvh * dh;
-        float off = 0.0f;                                      // NaN where a key or value is not finite
-        for (int d = lane; d < dh; d += 32) off = ffma(kr[d], 0.0f, ffma(vr[d], 0.0f, off));
-        if (__any_sync(0xffffffffu, off != off)) off = __int_as_float(0x7fffffff);
-        key([&](int d) { return kr[d] + off; }, [&](int d) { return vr[d] + off; });
-    }
-    const float inv = l == 0.0f ? 0.0f : fdiv(1.0f, l);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < dh) p.out[(size_t)row * p.ldo + (size_t)h * dh + lane + 32 * i] = o[i] * inv;
-}
-
-// ------------------------------------------------------------------ acceptance
 // A logit and its index as one word, so that the largest word is the largest logit's first
 // index: the value as an unsigned number in its order (a NaN below all, -0 as +0), above the
 // complement of the index.
