@@ -5,14 +5,16 @@
 // columns (row, head) of a KV head meet every tile of 128 keys. Both products run on the 5th-
 // generation tensor cores in f16 with the factors that are f32 held as two f16 each:
 //   x f = hi + lo, f a power of two that brings the largest to [2^13, 2^14)
-// which keeps 22 bits of every element down to 2^-28 of the largest, and at least 2^-39 of the
-// largest of those below. The cached codes are exact in f16; drafted keys and values are two
+// which keeps 22 bits of every element down to 2^-26 of the largest, and 2^-38 of the largest of
+// those below (weights: [2^5, 2^6), 2^-18 and 2^-30). The cached codes are exact in f16; drafted keys and values are two
 // f16 too, as keys j and 64 + j of a tile of their own, so that all four products are made.
-//   S^T [key][column] = K Q^T      hi and lo of Q one after another into the same sums
-//   O^T [element][column] = V^T P  weights p x v_scale, hi and lo likewise
+//   S^T [key][column] = K Q^T      hi and lo of Q as columns side by side (keys are read once:
+//   O^T [element][column] = V^T P  the MMAs are bound by reading operands), P weights p x v_scale
 // Keys and elements lie on the TMEM lanes: a thread has one key of a few columns, whose scales
-// are its own; the largest score of a column is found across the lanes. Each tile's output sums
-// go to f32 registers, so that the tensor cores' sums stay short.
+// are its own. Each tile's output sums go to f32 registers, so that the tensor cores' sums stay
+// short. What the exponentials are relative to, h, moves only when a score is more than 2^8
+// above it: then its largest is found across the lanes; a tile that moves nothing needs no
+// more than the warps' word that it does not.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -43,15 +45,18 @@ __device__ __forceinline__ int tree_splits(int kc_log2, int keys) { return max((
 
 // Warps 0 .. 15, softmax: warp w reads TMEM lanes 32 (w % 4) .. + 31 and columns w / 4 of the
 //   four parts of a tile's columns.
-// Warps 16 .. 19: codes to f16 operands, the next tile's codes requested while this one's are
-//   turned; an item's queries and drafted rows.
+// Warps 16, 17: keys' codes in shared memory to f16 operands; 18, 19: values' codes, and an item's
+//   queries. Drafted rows likewise. (Codes that waited in registers of these warps took 80
+//   registers' worth of spills, and the fence behind the writes waits for loads under way.)
 // Warp 20: issues the MMAs. Warp 21: finds the items (a sequence's columns of a KV head against
-//   a split of its keys) and their tiles' blocks and scales, up to eight tiles ahead.
+//   a split of its keys) and their tiles' blocks and scales, up to eight tiles ahead, and asks for
+//   the codes: a bulk copy for each block of 16 keys.
 // A CTA a SM goes through its items with the pipeline running on from one to the next. Every
 // wait is bounded; a warp whose wait ran out leaves its loop and sets the error word.
 constexpr int kTreeSoftWarps = 16;
 constexpr int kTreeConvWarps = 4;
-constexpr int kTreeThreads = (kTreeSoftWarps + kTreeConvWarps + 2) * 32;
+constexpr int kTreeThreads = (kTreeSoftWarps + kTreeConvWarps + 2) * 32;     // 80 registers a thread
+constexpr int kTreeTeam = kTreeConvWarps / 2 * 32;     // threads for the keys, and for the values
 constexpr int kTreeRing = 8;
 constexpr int kTreeKeys = 128;
 
@@ -71,33 +76,41 @@ struct TreeTile {
 // DP: d_head rounded up to 64, 128 or 256; NC: columns of an item
 template <int DP, int NC>
 struct TreeShape {
-    static constexpr int KS = DP == 64 ? 4 : DP == 128 ? 2 : 1;    // tiles of keys and values held
+    static constexpr int KK = DP == 64 ? 2 : 1;                    // tiles of keys held,
+    static constexpr int KV = DP == 64 || (DP == 128 && NC == 16) ? 2 : 1;      // of values,
+    static constexpr int PB = DP == 256 ? 1 : 2;                   // of weights,
+    static constexpr int ST = DP == 64 ? 6 : DP == 256 ? 1 : NC == 16 ? 4 : 2;  // and of codes as they come (keys, values, keys, ..)
+    static constexpr int NB = ST < 2 ? 2 : ST;                     // barriers of those: a team's own
     static constexpr int Halves = DP / 64;                         // 128-byte parts of a row
     static constexpr int MH = DP == 256 ? 2 : 1;                   // 128 elements each of the output
     static constexpr int QC = NC / 4;                              // columns of a thread
     static constexpr int Tile = Halves * kTreeKeys * 128;          // [part][key][64 f16], swizzled
-    static constexpr int QPart = Halves * NC * 128;                // [part][column][64 f16], swizzled
-    static constexpr int PPart = kTreeKeys * 128;                  // [key][64 columns], swizzled
+    static constexpr int QPart = Halves * 2 * NC * 128;            // [part][column: hi, lo][64 f16], swizzled
+    static constexpr int PPart = kTreeKeys * 128;                  // [key][64 columns: hi, lo], swizzled
+    static constexpr int PParts = 2 * NC > 64 ? 2 : 1;
     static constexpr int K = 0;
-    static constexpr int V = K + KS * Tile;
-    static constexpr int Q = V + KS * Tile;                        // hi, lo
-    static constexpr int P = Q + 2 * QPart;                        // hi, lo
-    static constexpr int Ring = P + 2 * PPart;
+    static constexpr int V = K + KK * Tile;
+    static constexpr int Q = V + KV * Tile;
+    static constexpr int P = Q + QPart;
+    static constexpr int Codes = P + PB * PParts * PPart;          // [block][16 keys][dh]
+    static constexpr int Ring = Codes + ST * kTreeKeys * DP;
     static constexpr int Unit = Ring + kTreeRing * (int)sizeof(TreeTile);       // [ring][NC] f32: of a column's scores
     static constexpr int Seen = Unit + kTreeRing * NC * 4;         // [ring][NC] words
     static constexpr int Dks = Seen + kTreeRing * NC * 8;          // [ring][64] scales of drafted keys
     static constexpr int Dvs = Dks + kTreeRing * 64 * 4;           // and values
-    static constexpr int Xm = Dvs + kTreeRing * 64 * 4;            // [2][4 parts][4][QC] largest scores
+    static constexpr int Moves = Dvs + kTreeRing * 64 * 4;         // [2][4 parts] 1 + the last tile that moves h
+    static constexpr int Xm = Moves + 8 * 4;                       // [2][4 parts][4][QC] largest scores
     static constexpr int Xl = Xm + 2 * 16 * QC * 4;                // [4][4][QC] sums
-    static constexpr int Bs = Xl + 16 * QC * 4;                    // [16 warps][QC]
-    static constexpr int Bk = Bs + 16 * QC * 4;                    // [2][16][QC]
+    static constexpr int Bs = Xl + 16 * QC * 4;                    // [16 warps][QC] h
+    static constexpr int Bd = Bs + 16 * QC * 4;                    // [16][QC] how far it moves; at the end 1 / sum
+    static constexpr int Bk = Bd + 16 * QC * 4;                    // [2][16][QC] the factor of what was before
     static constexpr int Bars = Bk + 2 * 16 * QC * 4;
-    static constexpr int NBars = 2 * kTreeRing + 4 * KS + 2 + 4 + 2 + 4 + 4 + 1 + 1;
+    static constexpr int NBars = 2 * kTreeRing + 2 * NB + 2 * KK + 2 * KV + 2 + 4 + 2 + 4 + 4 + 1 + 1;
     static constexpr int Bytes = Bars + NBars * 8 + 16;
     static constexpr int Alloc = Bytes + 1024;                     // operands start on 1024 bytes
-    static constexpr int TmemS = 0, TmemO = 2 * NC;                // two buffers each
-    static constexpr int TmemCols = 2 * NC + 2 * MH * NC <= 64 ? 64 : 256;
-    static_assert(2 * NC + 2 * MH * NC <= 256 && Alloc <= 227 * 1024, "");
+    static constexpr int TmemS = 0, TmemO = 4 * NC;                // two buffers each
+    static constexpr int TmemUsed = 4 * NC + 4 * MH * NC, TmemCols = TmemUsed <= 128 ? 128 : TmemUsed <= 256 ? 256 : 512;
+    static_assert(TmemUsed <= 512 && Alloc <= 227 * 1024, "");
 };
 
 // eight codes of two words as f16: 1024 + (code + 128) by bytes, less 1152
@@ -122,10 +135,12 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// the power of two that brings `top` (finite, >= 0) to [2^13, 2^14), and its reciprocal; tiny
-// ones are brought as far as 2^126 does
-__device__ __forceinline__ void f16_factor(float top, float& f, float& unit) {
-    const int e = min(max(140 + 127 - (int)(__float_as_uint(top) >> 23), 1), 253);
+// the power of two that brings `top` (finite, >= 0) to [2^bits, 2^(bits + 1)), and its reciprocal;
+// tiny ones are brought as far as 2^126 does
+constexpr int kRowBits = 13, kWeightBits = 5;      // (weights: probabilities may reach 2^kMoveBits)
+constexpr float kMoveBits = 8.0f;
+__device__ __forceinline__ void f16_factor(float top, int bits, float& f, float& unit) {
+    const int e = min(max(bits + 254 - (int)(__float_as_uint(top) >> 23), 1), 253);
     f = __int_as_float(e << 23);
     unit = __int_as_float((254 - e) << 23);
 }
@@ -136,18 +151,23 @@ __device__ __forceinline__ float warp_max(float x) {
     return r;
 }
 
-// A row of DP f32 elements (16 lanes, lane l16 the elements 4 l16 + 64 i ..) as hi and lo at
-// hi_at(i, unit) and lo_at: the 16-byte unit of part i. Returns the scale of its values: NaN for a
-// row that is not finite (its elements are zeros then, so that they harm no one else).
+// A row of DP f32 elements, 16 lanes, lane l16 the elements 4 l16 + 64 i ..
+template <int DP>
+__device__ __forceinline__ void load_row(float4 (&x)[DP / 64], const float* src, bool live, int dh, int l16) {
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i)
+        x[i] = live && 4 * l16 + 64 * i < dh ? *reinterpret_cast<const float4*>(src + 4 * l16 + 64 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// The row as hi and lo at hi_at(i, unit) and lo_at: the 16-byte unit of part i. Returns the scale of
+// its values: NaN for a row that is not finite (its elements are zeros then, so that they harm
+// no one else).
 template <int DP, typename At>
-__device__ __forceinline__ float put_row_f16(const float* src, bool live, int dh, int l16, At hi_at, At lo_at) {
-    float4 x[DP / 64];
+__device__ __forceinline__ float put_row_f16(float4 (&x)[DP / 64], int l16, At hi_at, At lo_at) {
     float top = 0.0f;
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < DP / 64; ++i) {
-        const int d = 4 * l16 + 64 * i;
-        x[i] = live && d < dh ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
         top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
         bad |= x[i].x != x[i].x || x[i].y != x[i].y || x[i].z != x[i].z || x[i].w != x[i].w;
     }
@@ -155,7 +175,7 @@ __device__ __forceinline__ float put_row_f16(const float* src, bool live, int dh
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float f, unit;
-    f16_factor(top, f, unit);
+    f16_factor(top, kRowBits, f, unit);
     const bool fine = top < INFINITY;
 #pragma unroll
     for (int i = 0; i < DP / 64; ++i) {
@@ -172,23 +192,24 @@ __device__ __forceinline__ float put_row_f16(const float* src, bool live, int dh
 template <int DP, int NC>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     using Sh = TreeShape<DP, NC>;
-    constexpr int KS = Sh::KS, QC = Sh::QC, MH = Sh::MH;
+    constexpr int KK = Sh::KK, KV = Sh::KV, PB = Sh::PB, ST = Sh::ST, NB = Sh::NB, QC = Sh::QC, MH = Sh::MH;
     extern __shared__ unsigned char ta_raw[];
     unsigned char* sm = ta_raw + ((1024u - (smem_u32(ta_raw) & 1023u)) & 1023u);
     TreeTile* ring = reinterpret_cast<TreeTile*>(sm + Sh::Ring);
     uint64_t* tready = reinterpret_cast<uint64_t*>(sm + Sh::Bars);     // [ring] a tile is described
     uint64_t* tfree = tready + kTreeRing;                              // [ring] and not needed any more
-    uint64_t* kfull = tfree + kTreeRing;                               // [KS] keys written
-    uint64_t* kempty = kfull + KS;                                     // [KS] their scores are made
-    uint64_t* vfull = kempty + KS;
-    uint64_t* vempty = vfull + KS;
-    uint64_t* qfull = vempty + KS;                                     // an item's queries written
+    uint64_t* cfull = tfree + kTreeRing;                               // [NB] codes have come
+    uint64_t* cempty = cfull + NB;                                     // [NB] and are turned
+    uint64_t* kfull = cempty + NB;                                     // [KK] keys written
+    uint64_t* kempty = kfull + KK;                                     // [KK] their scores are made
+    uint64_t* vfull = kempty + KK;                                     // [KV]
+    uint64_t* vempty = vfull + KV;                                     // [KV]
+    uint64_t* qfull = vempty + KV;                                     // an item's queries written
     uint64_t* qfree = qfull + 1;                                       // its last scores made
     uint64_t* sfull = qfree + 1;                                       // [2] scores in TMEM
     uint64_t* sfree = sfull + 2;                                       // [2] read
-    uint64_t* pfull = sfree + 2;                                       // weights written
-    uint64_t* pfree = pfull + 1;                                       // their products made
-    uint64_t* ofull = pfree + 1;                                       // [2] output sums in TMEM
+    uint64_t* pfull = sfree + 2;                                       // [2] weights written
+    uint64_t* ofull = pfull + 2;                                       // [2] output sums in TMEM (weights read)
     uint64_t* ofree = ofull + 2;                                       // [2] read
     uint64_t* part_bar = ofree + 2;                                    // [4] the warps of a column part meet
     uint64_t* all_bar = part_bar + 4;                                  // all softmax warps meet
@@ -202,21 +223,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     after_previous();
     if (tid == 0) {
         for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + kTreeConvWarps + 1); }
-        for (int i = 0; i < KS; ++i) {
-            mbar_init(&kfull[i], kTreeConvWarps * 32); mbar_init(&kempty[i], 1);
-            mbar_init(&vfull[i], kTreeConvWarps * 32); mbar_init(&vempty[i], 1);
-        }
-        mbar_init(qfull, kTreeConvWarps * 32); mbar_init(qfree, 1);
+        for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], kTreeConvWarps / 2); }
+        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], kTreeTeam); mbar_init(&kempty[i], 1); }
+        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], kTreeTeam); mbar_init(&vempty[i], 1); }
+        mbar_init(qfull, kTreeTeam); mbar_init(qfree, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sfull[i], 2); mbar_init(&sfree[i], kTreeSoftWarps);
             mbar_init(&ofull[i], 1); mbar_init(&ofree[i], kTreeSoftWarps);
+            mbar_init(&pfull[i], kTreeSoftWarps);
         }
-        mbar_init(pfull, kTreeSoftWarps); mbar_init(pfree, 1);
         for (int i = 0; i < 4; ++i) mbar_init(&part_bar[i], 4);
         mbar_init(all_bar, kTreeSoftWarps); mbar_init(done, 1);
         fence_mbar_init();
         *fail = 0;
     }
+    if (tid < 8) reinterpret_cast<int*>(sm + Sh::Moves)[tid] = 0;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Sh::TmemCols) : "memory");
@@ -250,7 +271,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     if (warp == kPlanWarp) {
         // ---- items and tiles
         const int group = lane >> 3, b = lane & 7, psz = 1 << p.c.page_log2;
-        int t = 0, base = 0;
+        int t = 0, base = 0, come = 0;                         // come: tiles of codes asked for
         unsigned item = blockIdx.x, before = 0;                // items of the sequences before `base`
         bool ok = true;
         for (int n = 0; ok; ++n, item += gridDim.x) {
@@ -329,190 +350,223 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 __syncwarp();
                 if (lane < cnt) mbar_arrive(&tready[(t + lane) & (kTreeRing - 1)]);
                 t += cnt;
-            }
-        }
-    } else if (warp == kMmaWarp) {
-        // ---- MMAs (one lane)
-        if (lane == 0) {
-            const uint32_t base = smem_u32(sm);
-            const uint32_t ids = umma_idesc_f16(NC, false, false), ido = umma_idesc_f16(NC, true, true);
-            bool ok = true;
-            int items = 0;
-            auto scores = [&](int t, int flags) {
-                const int slot = t % KS, use = t / KS;
-                ok = ok && wait(&kfull[slot], use & 1, 20);
-                if (ok && (flags & TREE_FIRST)) ok = wait(qfull, items & 1, 20);
-                if (ok && t > 1) ok = wait(&sfree[t & 1], ((t >> 1) - 1) & 1, 20);
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t kb = base + Sh::K + slot * Sh::Tile, qb = base + Sh::Q;
+                // the tiles' codes: a bulk copy a block
+                for (int u = 0; u < cnt && i0 + u < ntiles; ++u) {
+                    const int c = __shfl_sync(0xffffffffu, cell, 8 * u + b);
+                    const bool mine = group == 0 && c >= 0;
+                    const unsigned bytes = __popc(__ballot_sync(0xffffffffu, mine)) * kKvBlock * dh;
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int h = 0; h < Sh::Halves; ++h)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_f16(tmem + Sh::TmemS + (t & 1) * NC, umma_desc_sw128(kb + h * kTreeKeys * 128 + 32 * k),
-                                     umma_desc_sw128(qb + e * Sh::QPart + h * NC * 128 + 32 * k), ids, e + h + k > 0 ? 1u : 0u);
-                umma_commit(&kempty[slot]);
-                if (flags & TREE_LAST) {
-                    umma_commit(qfree);
-                    ++items;
+                    for (int v = 0; v < 2; ++v, ++come) {
+                        const int slot = come % ST;
+                        if (come >= ST) ok = ok && wait_warp(&cempty[(come - ST) % NB], ((come - ST) / NB) & 1, 50);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&cfull[come % NB], bytes);
+                        __syncwarp();
+                        if (mine)
+                            bulk_g2s(sm + Sh::Codes + slot * kTreeKeys * DP + b * kKvBlock * dh, (v ? p.c.v : p.c.k) + (size_t)c * kKvBlock * dh,
+                                     kKvBlock * dh, &cfull[come % NB]);
+                    }
+                    if (!ok) break;
                 }
-                umma_commit(&sfull[t & 1]);
-                mbar_arrive(&sfull[t & 1]);                    // passes on what the others wrote: units, scales
-            };
-            auto output = [&](int t) {
-                const int slot = t % KS, use = t / KS;
-                ok = ok && wait(pfull, t & 1, 20) && wait(&vfull[slot], use & 1, 20);
-                if (ok && t > 1) ok = wait(&ofree[t & 1], ((t >> 1) - 1) & 1, 20);
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t vb = base + Sh::V + slot * Sh::Tile, pb = base + Sh::P;
-#pragma unroll
-                for (int mh = 0; mh < MH; ++mh)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int k = 0; k < kTreeKeys / 16; ++k)      // (d_head 64: lanes 64 .. 127 repeat the others)
-                            umma_f16(tmem + Sh::TmemO + ((t & 1) * MH + mh) * NC,
-                                     umma_desc_sw128_mn(vb + mh * 2 * kTreeKeys * 128 + k * 2048, Sh::Halves > 1 ? kTreeKeys * 128 : 0),
-                                     umma_desc_sw128_mn(pb + e * Sh::PPart + k * 2048, 0), ido, e + k > 0 ? 1u : 0u);
-                umma_commit(&vempty[slot]);
-                umma_commit(pfree);
-                umma_commit(&ofull[t & 1]);
-            };
-            // the flags of tile t; its description is not needed after that
-            auto flags_of = [&](int t) {
-                ok = ok && wait(&tready[t & (kTreeRing - 1)], ring_parity(t), 20);
-                const int f = ok ? ring[t & (kTreeRing - 1)].flags : TREE_END;
-                if (ok) mbar_arrive(&tfree[t & (kTreeRing - 1)]);
-                return f;
-            };
-            int flags = flags_of(0);
-            if (!(flags & TREE_END)) scores(0, flags);
-            for (int t = 0; ok && !(flags & TREE_END); ++t) {
-                flags = flags_of(t + 1);
-                // the next tile's scores go first, except those of another item, whose queries
-                // wait for this one's, and drafted ones where they wait for the only values' place
-                const bool ahead = !(flags & (TREE_END | TREE_FIRST)) && !(KS == 1 && (flags & TREE_DRAFT));
-                if (ahead) scores(t + 1, flags);
-                output(t);
-                if (!ahead && !(flags & TREE_END)) scores(t + 1, flags);
             }
-            umma_commit(done);                                 // also after a wait that ran out: no MMA may be
-            if (!mbar_wait_bounded(done, 0)) *fail = 1;        // under way when its memory is given up
         }
-    } else if (warp >= kTreeSoftWarps) {
-        // ---- operands
-        constexpr int Chunks = DP / 16;                        // 16 codes each of a row
-        constexpr int Units = kTreeKeys * Chunks / (kTreeConvWarps * 32), UR = Units < 8 ? Units : 8, Rounds = Units / UR;
-        const int ct = tid - kTreeSoftWarps * 32, chunk = ct % Chunks, key0 = ct / Chunks;
-        constexpr int KeyStep = kTreeConvWarps * 32 / Chunks;
-        uint4 kr[UR], vr[UR];
-        auto fetch = [&](const TreeTile& d, const int8_t* codes, int round, uint4 (&r)[UR]) {
+        // no copy may be under way when the memory is given up
+        for (int c = max(come - ST, 0); c < come; ++c)
+            if (!mbar_wait_bounded(&cfull[c % NB], (c / NB) & 1)) *fail = 1;
+    } else if (warp == kMmaWarp) {
+        // ---- MMAs
+        const bool me = elect_lane();
+        const uint32_t base = smem_u32(sm);
+        constexpr uint32_t ids = umma_idesc_f16(2 * NC, false, false), ido = umma_idesc_f16(2 * NC, true, true);
+        const uint64_t kdesc = umma_desc_sw128(base + Sh::K), qdesc = umma_desc_sw128(base + Sh::Q);
+        // (d_head 64: lanes 64 .. 127 of the output repeat the others)
+        const uint64_t vdesc = umma_desc_sw128_mn(base + Sh::V, Sh::Halves > 1 ? kTreeKeys * 128 : 0);
+        const uint64_t pdesc = umma_desc_sw128_mn(base + Sh::P, Sh::PParts > 1 ? Sh::PPart : 0);
+        bool ok = true;
+        int items = 0;
+        auto scores = [&](int t, int flags) {
+            const int slot = t % KK, use = t / KK;
+            ok = ok && wait_warp(&kfull[slot], use & 1, 20);
+            if (ok && (flags & TREE_FIRST)) ok = wait_warp(qfull, items & 1, 20);
+            if (ok && t > 1) ok = wait_warp(&sfree[t & 1], ((t >> 1) - 1) & 1, 20);
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t kd = kdesc + (uint64_t)(slot * (Sh::Tile >> 4));
+            const uint32_t to = tmem + Sh::TmemS + (t & 1) * 2 * NC;
+            umma_f16<false>(me, to, kd, qdesc, ids);
 #pragma unroll
-            for (int x = 0; x < UR; ++x) {
-                const int key = key0 + (round * UR + x) * KeyStep, cell = d.cell[key >> 4];
-                r[x] = cell >= 0 && 16 * chunk < dh ? load16(codes + ((size_t)cell * kKvBlock + (key & 15)) * dh + 16 * chunk)
-                                                    : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 1; i < 4 * Sh::Halves; ++i)
+                umma_f16<true>(me, to, kd + ((i >> 2) * (kTreeKeys * 128) + 32 * (i & 3)) / 16, qdesc + ((i >> 2) * (2 * NC * 128) + 32 * (i & 3)) / 16, ids);
+            if (me) {
+                umma_commit(&kempty[slot]);
+                if (flags & TREE_LAST) umma_commit(qfree);
+                umma_commit(&sfull[t & 1]);
+            }
+            if (flags & TREE_LAST) ++items;
+            // drafted values' scales come with the values
+            if (flags & TREE_DRAFT) ok = wait_warp(&vfull[t % KV], (t / KV) & 1, 20);
+            if (me) mbar_arrive(&sfull[t & 1]);                // passes on what the others wrote: units, scales
+        };
+        auto output = [&](int t) {
+            const int slot = t % KV, use = t / KV;
+            ok = ok && wait_warp(&pfull[t & 1], (t >> 1) & 1, 20) && wait_warp(&vfull[slot], use & 1, 20);
+            if (ok && t > 1) ok = wait_warp(&ofree[t & 1], ((t >> 1) - 1) & 1, 20);
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t pd = pdesc + (uint64_t)(t % PB * (Sh::PParts * Sh::PPart >> 4));
+#pragma unroll
+            for (int mh = 0; mh < MH; ++mh) {
+                const uint64_t vd = vdesc + (uint64_t)(slot * (Sh::Tile >> 4) + mh * (2 * kTreeKeys * 128 >> 4));
+                const uint32_t to = tmem + Sh::TmemO + ((t & 1) * MH + mh) * 2 * NC;
+                umma_f16<false>(me, to, vd, pd, ido);
+#pragma unroll
+                for (int k = 1; k < kTreeKeys / 16; ++k) umma_f16<true>(me, to, vd + k * (2048 / 16), pd + k * (2048 / 16), ido);
+            }
+            if (me) {
+                umma_commit(&vempty[slot]);
+                umma_commit(&ofull[t & 1]);
             }
         };
-        auto put = [&](unsigned char* tile, int round, const uint4 (&r)[UR]) {
+        // the flags of tile t; its description is not needed after that
+        auto flags_of = [&](int t) {
+            ok = ok && wait_warp(&tready[t & (kTreeRing - 1)], ring_parity(t), 20);
+            const int f = ok ? ring[t & (kTreeRing - 1)].flags : TREE_END;
+            if (ok) arrive_warp(&tfree[t & (kTreeRing - 1)]);
+            return f;
+        };
+        int flags = flags_of(0);
+        if (!(flags & TREE_END)) scores(0, flags);
+        for (int t = 0; ok && !(flags & TREE_END); ++t) {
+            flags = flags_of(t + 1);
+            // the next tile's scores go first, except those of another item, whose queries
+            // wait for this one's, and drafted ones where their values wait for the only place
+            const bool ahead = !(flags & (TREE_END | TREE_FIRST)) && !(KV == 1 && (flags & TREE_DRAFT));
+            if (ahead) scores(t + 1, flags);
+            output(t);
+            if (!ahead && !(flags & TREE_END)) scores(t + 1, flags);
+        }
+        if (me) umma_commit(done);                             // also after a wait that ran out: no MMA may be
+        __syncwarp();
+        if (!mbar_wait_bounded(done, 0)) *fail = 1;            // under way when its memory is given up
+    } else if (warp >= kTreeSoftWarps) {
+        // ---- operands: a team for the keys, one for the values
+        constexpr int Chunks = DP / 16;                        // 16 codes each of a row
+        constexpr int Units = kTreeKeys * Chunks / kTreeTeam, KeyStep = kTreeTeam / Chunks;
+        const bool keys = warp < kTreeSoftWarps + kTreeConvWarps / 2;
+        const int ct = (tid - kTreeSoftWarps * 32) % kTreeTeam, chunk = ct % Chunks, key0 = ct / Chunks;
+        const float* rows = keys ? p.k : p.v;
+        const long long ldr = keys ? p.ldk : p.ldv;
+        unsigned char* tiles = sm + (keys ? Sh::K : Sh::V);
+        uint64_t *full = keys ? kfull : vfull, *empty = keys ? kempty : vempty;
+        float* scales = reinterpret_cast<float*>(sm + (keys ? Sh::Dks : Sh::Dvs));
+        // a tile's codes (blocks that are not there: some others, which count nothing) as f16
+        auto put = [&](const unsigned char* codes, unsigned char* tile) {
             unsigned char* part = tile + (chunk >> 2) * kTreeKeys * 128;
             const int u0 = 2 * (chunk & 3), turn = (chunk >> 2) & 1;      // (parts in turn: no bank conflicts)
+            const bool in = 16 * chunk < dh;
+#pragma unroll 1
+            for (int x0 = 0; x0 < Units; x0 += 8) {
+                uint4 r[8];
 #pragma unroll
-            for (int x = 0; x < UR; ++x) {
-                const int key = key0 + (round * UR + x) * KeyStep;
-                const uint4 lo = codes_f16(r[x].x, r[x].y), hi = codes_f16(r[x].z, r[x].w);
-                unsigned char* row = part + key * 128;
-                *reinterpret_cast<uint4*>(row + (((u0 + turn) ^ (key & 7)) << 4)) = turn ? hi : lo;
-                *reinterpret_cast<uint4*>(row + (((u0 + 1 - turn) ^ (key & 7)) << 4)) = turn ? lo : hi;
+                for (int x = 0; x < 8; ++x) r[x] = in ? lds128(codes + (key0 + (x0 + x) * KeyStep) * dh + 16 * chunk) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const int key = key0 + (x0 + x) * KeyStep;
+                    const uint4 lo = codes_f16(r[x].x, r[x].y), hi = codes_f16(r[x].z, r[x].w);
+                    unsigned char* row = part + key * 128;
+                    *reinterpret_cast<uint4*>(row + (((u0 + turn) ^ (key & 7)) << 4)) = turn ? hi : lo;
+                    *reinterpret_cast<uint4*>(row + (((u0 + 1 - turn) ^ (key & 7)) << 4)) = turn ? lo : hi;
+                }
             }
         };
-        // drafted rows: key j and 64 + j of the tile (zeros past the last)
-        auto put_drafted = [&](unsigned char* tile, const TreeTile& d, const float* src, long long ld, float* scales) {
-            for (int r0 = 0; r0 < 64; r0 += kTreeConvWarps * 2) {
-                const int j = r0 + (ct >> 4);
-                auto at = [&](int row) {
-                    return [=](int i, int u) { return tile + i * kTreeKeys * 128 + row * 128 + ((u ^ (row & 7)) << 4); };
-                };
-                const float unit = put_row_f16<DP>(src + (size_t)(d.a + min(j, d.len - 1)) * ld + (size_t)d.kvh * dh, j < d.len, dh, ct & 15,
-                                                   at(j), at(64 + j));
-                if ((ct & 15) == 0) scales[j] = unit;
-            }
-        };
-        bool ok = wait_warp(&tready[0], 0, 20);
-        if (ok && !(ring[0].flags & (TREE_DRAFT | TREE_END))) {
-            fetch(ring[0], p.c.k, 0, kr);
-            fetch(ring[0], p.c.v, 0, vr);
-        }
-        for (int t = 0; ok; ++t) {
-            const TreeTile& d = ring[t & (kTreeRing - 1)];
-            if (d.flags & TREE_END) break;
-            const int slot = t % KS, use = t / KS;
-            const bool draft = d.flags & TREE_DRAFT;
-            if (d.flags & TREE_FIRST) {
-                if (d.item > 0) ok = wait_warp(qfree, (d.item - 1) & 1, 50);
-                if (!ok) break;
-                const int it = d.item & (kTreeRing - 1);
-                float* unit = reinterpret_cast<float*>(sm + Sh::Unit) + it * NC;
-                long long* seen = reinterpret_cast<long long*>(sm + Sh::Seen) + it * NC;
-#pragma unroll 2
-                for (int c0 = 0; c0 < NC; c0 += kTreeConvWarps * 2) {
-                    const int c = c0 + (ct >> 4), cc = d.col0 + min(c, d.cols - 1), tok = cc / p.G;
-                    auto at = [&](int e) {
-                        return [=](int i, int u) { return sm + Sh::Q + e * Sh::QPart + i * NC * 128 + c * 128 + ((u ^ (c & 7)) << 4); };
+        constexpr int Lines = kTreeTeam / 16, Batch = 8 / (DP / 64);   // rows at a time, and of a lane group in flight
+        // drafted rows: key j and 64 + j of the tile, all loads of a batch first. (What lies past the
+        // last one is some other tile's: its scores are masked, its values are finite.)
+        auto put_drafted = [&](unsigned char* tile, const TreeTile& d, float* scale) {
+            for (int r0 = 0; r0 < d.len; r0 += Lines * Batch) {
+                float4 x[Batch][DP / 64];
+#pragma unroll
+                for (int b = 0; b < Batch; ++b) {
+                    const int j = r0 + Lines * b + (ct >> 4);
+                    load_row<DP>(x[b], rows + (size_t)(d.a + min(j, d.len - 1)) * ldr + (size_t)d.kvh * dh, j < d.len, dh, ct & 15);
+                }
+#pragma unroll
+                for (int b = 0; b < Batch; ++b) {
+                    const int j = r0 + Lines * b + (ct >> 4);
+                    if (r0 + Lines * b >= d.len) break;        // (whole warps)
+                    auto at = [&](int row) {
+                        return [=](int i, int u) { return tile + i * kTreeKeys * 128 + row * 128 + ((u ^ (row & 7)) << 4); };
                     };
-                    const float un = put_row_f16<DP>(p.q + (size_t)(d.a + tok) * p.ldq + (size_t)(d.kvh * p.G + cc - tok * p.G) * dh, c < d.cols,
-                                                     dh, ct & 15, at(0), at(1));
+                    const float unit = put_row_f16<DP>(x[b], ct & 15, at(j), at(64 + j));
+                    if ((ct & 15) == 0) scale[j] = unit;
+                }
+            }
+        };
+        auto put_queries = [&](const TreeTile& d) {
+            const int it = d.item & (kTreeRing - 1);
+            float* unit = reinterpret_cast<float*>(sm + Sh::Unit) + it * NC;
+            long long* seen = reinterpret_cast<long long*>(sm + Sh::Seen) + it * NC;
+            for (int c0 = 0; c0 < d.cols; c0 += Lines * Batch) {
+                float4 x[Batch][DP / 64];
+#pragma unroll
+                for (int b = 0; b < Batch; ++b) {
+                    const int c = c0 + Lines * b + (ct >> 4), cc = d.col0 + min(c, d.cols - 1);
+                    load_row<DP>(x[b], p.q + (size_t)(d.a + cc / p.G) * p.ldq + (size_t)(d.kvh * p.G + cc % p.G) * dh, c < d.cols, dh, ct & 15);
+                }
+#pragma unroll
+                for (int b = 0; b < Batch; ++b) {
+                    const int c = c0 + Lines * b + (ct >> 4);
+                    if (c0 + Lines * b >= d.cols) break;       // (whole warps)
+                    auto at = [&](int col) {
+                        return [=](int i, int u) { return sm + Sh::Q + i * 2 * NC * 128 + col * 128 + ((u ^ (col & 7)) << 4); };
+                    };
+                    const float un = put_row_f16<DP>(x[b], ct & 15, at(c), at(NC + c));
                     if ((ct & 15) == 0) {
-                        unit[c] = un * 1.4426950408889634f;            // log2 e
-                        seen[c] = c < d.cols ? p.seen[d.a + tok] : 0;
+                        unit[c] = un * 1.4426950408889634f;    // log2 e
+                        seen[c] = c < d.cols ? p.seen[d.a + (d.col0 + c) / p.G] : 0;
                     }
                 }
+            }
+        };
+        if (!keys) {                                           // what nothing has written yet are zeros
+            for (int i = ct; i < KV * Sh::Tile / 16; i += kTreeTeam) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = ct; i < Sh::QPart / 16; i += kTreeTeam) reinterpret_cast<uint4*>(sm + Sh::Q)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = ct; i < kTreeRing * NC; i += kTreeTeam) {
+                reinterpret_cast<float*>(sm + Sh::Unit)[i] = 0.0f;
+                reinterpret_cast<long long*>(sm + Sh::Seen)[i] = 0;
+            }
+            asm volatile("bar.sync 1, 64;" ::: "memory");      // (nobody has waited for anything yet)
+        }
+        bool ok = true;
+        for (int t = 0, come = keys ? 0 : 1; ok; ++t) {
+            ok = wait_warp(&tready[t & (kTreeRing - 1)], ring_parity(t), 50);
+            if (!ok) break;
+            const TreeTile& d = ring[t & (kTreeRing - 1)];
+            if (d.flags & TREE_END) break;
+            const int slots = keys ? KK : KV, slot = t % slots;
+            if (!keys && (d.flags & TREE_FIRST)) {
+                if (d.item > 0) ok = wait_warp(qfree, (d.item - 1) & 1, 50);
+                if (!ok) break;
+                put_queries(d);
                 fence_async_smem();
                 mbar_arrive(qfull);
             }
-            ok = ok && wait_warp(&tready[(t + 1) & (kTreeRing - 1)], ring_parity(t + 1), 20);
-            if (!ok) break;
-            const TreeTile& nx = ring[(t + 1) & (kTreeRing - 1)];
-            const bool more = !(nx.flags & (TREE_DRAFT | TREE_END));
-            if (t >= KS) ok = wait_warp(&kempty[slot], (use - 1) & 1, 50);
-            if (!ok) break;
-            unsigned char* kd = sm + Sh::K + slot * Sh::Tile;
-            if (draft) {
-                put_drafted(kd, d, p.k, p.ldk, reinterpret_cast<float*>(sm + Sh::Dks) + (t & (kTreeRing - 1)) * 64);
-            } else {
-#pragma unroll
-                for (int r = 0; r < Rounds; ++r) {
-                    if (r > 0) fetch(d, p.c.k, r, kr);
-                    put(kd, r, kr);
-                }
-            }
-            if (more) fetch(nx, p.c.k, 0, kr);
-            unsigned char* vd = sm + Sh::V + slot * Sh::Tile;
-            float* dvs = reinterpret_cast<float*>(sm + Sh::Dvs) + (t & (kTreeRing - 1)) * 64;
-            if (draft) {                                       // both before the scores: the softmax wants all scales
-                if (t >= KS) ok = wait_warp(&vempty[slot], (use - 1) & 1, 50);
+            unsigned char* tile = tiles + slot * Sh::Tile;
+            if (d.flags & TREE_DRAFT) {
+                if (t >= slots) ok = wait_warp(&empty[slot], (t / slots - 1) & 1, 50);
                 if (!ok) break;
-                put_drafted(vd, d, p.v, p.ldv, dvs);
-                fence_async_smem();
-                mbar_arrive(&kfull[slot]);
+                put_drafted(tile, d, scales + (t & (kTreeRing - 1)) * 64);
             } else {
-                fence_async_smem();
-                mbar_arrive(&kfull[slot]);
-                if (t >= KS) ok = wait_warp(&vempty[slot], (use - 1) & 1, 50);
+                const int cs = come % ST;
+                ok = wait_warp(&cfull[come % NB], (come / NB) & 1, 50);
+                if (ok && t >= slots) ok = wait_warp(&empty[slot], (t / slots - 1) & 1, 50);
                 if (!ok) break;
-#pragma unroll
-                for (int r = 0; r < Rounds; ++r) {
-                    if (r > 0) fetch(d, p.c.v, r, vr);
-                    put(vd, r, vr);
-                }
-                fence_async_smem();
+                put(sm + Sh::Codes + cs * kTreeKeys * DP, tile);
+                arrive_warp(&cempty[come % NB]);
+                come += 2;
             }
-            mbar_arrive(&vfull[slot]);
-            if (more) fetch(nx, p.c.v, 0, vr);
+            fence_async_smem();
+            mbar_arrive(&full[slot]);
             arrive_warp(&tfree[t & (kTreeRing - 1)]);
         }
     } else {
@@ -521,6 +575,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         const uint32_t trow = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(part * QC);
         float* bs = reinterpret_cast<float*>(sm + Sh::Bs) + warp * QC;
         float* bk = reinterpret_cast<float*>(sm + Sh::Bk) + warp * QC;
+        float* bd = reinterpret_cast<float*>(sm + Sh::Bd) + warp * QC;
         float* xm = reinterpret_cast<float*>(sm + Sh::Xm) + part * 4 * QC;
         float* xl = reinterpret_cast<float*>(sm + Sh::Xl) + part * 4 * QC;
         int met = 0, met_all = 0;                              // how often the part's warps, all of them have met
@@ -530,56 +585,84 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             ok = wait_warp(&part_bar[part], met++ & 1, 20);
             return ok;
         };
-        auto read_cols = [&](uint32_t at, uint32_t (&r)[QC]) {
-            if constexpr (QC == 16) tmem_ld16(at, r);
-            else if constexpr (QC == 8) tmem_ld8(at, r);
+        constexpr int RC = QC < 8 ? QC : 8;                    // columns read at a time
+        auto read_cols = [&](uint32_t at, uint32_t (&r)[RC]) {
+            if constexpr (RC == 8) tmem_ld8(at, r);
             else tmem_ld4(at, r);
         };
-        float m = -INFINITY;                                   // of column `lane`
+        // hi and lo sums of RC columns, together
+        auto read_sums = [&](uint32_t at, f32x2* y) {
+            uint32_t c[RC], z[RC];
+            read_cols(at, c);
+            read_cols(at + NC, z);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < RC / 2; ++x)
+                y[x] = add2(pack2(__uint_as_float(c[2 * x]), __uint_as_float(c[2 * x + 1])),
+                            pack2(__uint_as_float(z[2 * x]), __uint_as_float(z[2 * x + 1])));
+        };
+        int* moves = reinterpret_cast<int*>(sm + Sh::Moves) + part;
+        float h = 0.0f;                                        // of column `lane`,
+        bool unset = true;                                     // which has seen no key yet
         f32x2 l[QC / 2], o[MH][QC / 2];
-        float u = 0.0f;                                        // of the tile whose output is pending
-        // output sums of tile t
-        auto fold = [&](int t) {
+        // Output sums are folded two tiles later, when their products are surely made; with one buffer of
+        // weights one tile later, before they are written.
+        // output sums of tile t; u: what a unit of them is, moved: whether that tile moved h
+        auto fold = [&](int t, float u, bool moved) {
             ok = ok && wait_warp(&ofull[t & 1], (t >> 1) & 1, 20);
             if (!ok) return;
             tc_fence_after();
-            uint32_t c[MH][QC];
 #pragma unroll
-            for (int mh = 0; mh < MH; ++mh) read_cols(trow + Sh::TmemO + ((t & 1) * MH + mh) * NC, c[mh]);
-            tmem_wait_ld();
+            for (int mh = 0; mh < MH; ++mh) {
+                if (moved) {
+#pragma unroll
+                    for (int x = 0; x < QC / 2; ++x) {
+                        const float2 bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + 2 * x);
+                        o[mh][x] = mul2(o[mh][x], pack2(bb.x, bb.y));
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < QC / RC; ++q) {
+                    f32x2 y[RC / 2];
+                    read_sums(trow + Sh::TmemO + ((t & 1) * MH + mh) * 2 * NC + q * RC, y);
+#pragma unroll
+                    for (int x = 0; x < RC / 2; ++x) o[mh][q * RC / 2 + x] = fma2(y[x], pack2(u, u), o[mh][q * RC / 2 + x]);
+                }
+            }
             tc_fence_before();
             arrive_warp(&ofree[t & 1]);
-            const float* back = bk + (t & 1) * 16 * QC;
-#pragma unroll
-            for (int x = 0; x < QC / 2; ++x) {
-                const float2 bb = *reinterpret_cast<const float2*>(back + 2 * x);
-#pragma unroll
-                for (int mh = 0; mh < MH; ++mh)
-                    o[mh][x] = fma2(pack2(__uint_as_float(c[mh][2 * x]), __uint_as_float(c[mh][2 * x + 1])), pack2(u, u),
-                                    mul2(o[mh][x], pack2(bb.x, bb.y)));
-            }
         };
-        for (int t = 0; ok; ++t) {
+        float u1 = 0.0f, u2 = 0.0f;                            // of the two tiles whose output is pending
+        bool moved1 = false, moved2 = false;
+        int begun = 0;                                         // tiles of the item before this one
+        for (int t = 0; ok; ++t, ++begun) {
             if (!wait_warp(&tready[t & (kTreeRing - 1)], ring_parity(t), 20)) break;
             const TreeTile& d = ring[t & (kTreeRing - 1)];
             const int flags = d.flags;
             if (flags & TREE_END) break;
-            const bool draft = flags & TREE_DRAFT;
-            if (flags & TREE_FIRST) {
-                m = -INFINITY;
+            const bool draft = flags & TREE_DRAFT, first = flags & TREE_FIRST;
+            if (first) {
+                begun = 0;
+                h = 0.0f;
+                unset = lane < QC && part * QC + lane < d.cols;
 #pragma unroll
                 for (int x = 0; x < QC / 2; ++x) {
                     l[x] = 0ull;
 #pragma unroll
                     for (int mh = 0; mh < MH; ++mh) o[mh][x] = 0ull;
                 }
+                if (lane < QC) bs[lane] = 0.0f;
+                __syncwarp();
             }
             const int it = d.item & (kTreeRing - 1);
             const float* unit = reinterpret_cast<const float*>(sm + Sh::Unit) + it * NC + part * QC;
             if (!wait_warp(&sfull[t & 1], (t >> 1) & 1, 20)) break;
             tc_fence_after();
-            uint32_t raw[QC];
-            read_cols(trow + Sh::TmemS + (t & 1) * NC, raw);
+            f32x2 s[QC / 2];
+#pragma unroll
+            for (int q = 0; q < QC / RC; ++q) read_sums(trow + Sh::TmemS + (t & 1) * 2 * NC + q * RC, s + q * RC / 2);
+            tc_fence_before();
+            arrive_warp(&sfree[t & 1]);
             // this key's scales, and the largest value scale of the tile
             float ks, vs, vtop = 0.0f;
             bool gone;
@@ -593,103 +676,141 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                     vtop = fmaxf(vtop, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
                 }
             } else {
+                if (begun >= PB) PB == 2 ? fold(t - 2, u2, moved2) : fold(t - 1, u1, moved1);
+                if (!ok) break;
                 const float* dk = reinterpret_cast<const float*>(sm + Sh::Dks) + (t & (kTreeRing - 1)) * 64;
                 const float* dv = reinterpret_cast<const float*>(sm + Sh::Dvs) + (t & (kTreeRing - 1)) * 64;
-                ks = dk[key & 63];
-                vs = dv[key & 63];
                 gone = (key & 63) >= d.len;
+                ks = gone ? 0.0f : dk[key & 63];
+                vs = dv[key & 63];
                 for (int i = 0; i < d.len; ++i) vtop = fmaxf(vtop, dv[i]);
             }
             if (gone) vs = 0.0f;
-            tmem_wait_ld();
-            tc_fence_before();
-            arrive_warp(&sfree[t & 1]);
             if (draft) {
-                // scores of keys j and 64 + j together, through the weights' memory
-                if (t > 0 && !wait_warp(pfree, (t - 1) & 1, 20)) break;
-                float* x = reinterpret_cast<float*>(sm + Sh::P) + part * QC * kTreeKeys;
+                // scores of keys j and 64 + j together, through the weights' memory (tile t - 2's)
+                float* x = reinterpret_cast<float*>(sm + Sh::P + t % PB * Sh::PParts * Sh::PPart) + part * QC * kTreeKeys;
 #pragma unroll
-                for (int c = 0; c < QC; ++c) x[c * kTreeKeys + key] = __uint_as_float(raw[c]);
+                for (int c = 0; c < QC / 2; ++c) {
+                    const float2 y = unpack2(s[c]);
+                    x[2 * c * kTreeKeys + key] = y.x;
+                    x[(2 * c + 1) * kTreeKeys + key] = y.y;
+                }
                 if (!meet()) break;
 #pragma unroll
-                for (int c = 0; c < QC; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) + x[c * kTreeKeys + (key ^ 64)]);
-                asm volatile("" ::: "memory");
+                for (int c = 0; c < QC / 2; ++c) s[c] = add2(s[c], pack2(x[2 * c * kTreeKeys + (key ^ 64)], x[(2 * c + 1) * kTreeKeys + (key ^ 64)]));
             }
-            float s[QC];
+            // scores in base 2 relative to h
+            float top = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < QC; x += 2) {
-                const float2 un = *reinterpret_cast<const float2*>(unit + x);
-                const float2 y = unpack2(mul2(pack2(__uint_as_float(raw[x]), __uint_as_float(raw[x + 1])),
-                                              mul2(pack2(un.x, un.y), pack2(ks, ks))));
-                s[x] = gone ? -INFINITY : y.x;
-                s[x + 1] = gone ? -INFINITY : y.y;
+            for (int x = 0; x < QC / 2; ++x) {
+                const float2 un = *reinterpret_cast<const float2*>(unit + 2 * x), hh = *reinterpret_cast<const float2*>(bs + 2 * x);
+                s[x] = fma2(s[x], mul2(pack2(un.x, un.y), pack2(ks, ks)), pack2(-hh.x, -hh.y));
             }
             if (draft) {
                 const long long* seen = reinterpret_cast<const long long*>(sm + Sh::Seen) + it * NC + part * QC;
 #pragma unroll
-                for (int c = 0; c < QC; ++c)
-                    if (!(seen[c] >> (key & 63) & 1)) s[c] = -INFINITY;
-            }
-            // the columns' largest scores: lane c has column c
-            float top = -INFINITY;
+                for (int c = 0; c < QC / 2; ++c) {
+                    float2 y = unpack2(s[c]);
+                    if (gone || !(seen[2 * c] >> (key & 63) & 1)) y.x = -INFINITY;
+                    if (gone || !(seen[2 * c + 1] >> (key & 63) & 1)) y.y = -INFINITY;
+                    s[c] = pack2(y.x, y.y);
+                }
+            } else if (gone) {
 #pragma unroll
-            for (int c = 0; c < QC; ++c) {
-                const float y = warp_max(s[c]);
-                if (lane == c) top = y;
+                for (int c = 0; c < QC / 2; ++c) s[c] = pack2(-INFINITY, -INFINITY);
             }
-            if (lane < QC) xm[(t & 1) * 16 * QC + quarter * QC + lane] = top;
-            if (!meet()) break;
-            if (lane < QC) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) top = fmaxf(top, xm[(t & 1) * 16 * QC + q * QC + lane]);
-                top = fmaxf(top, m);
-                const float h = top == -INFINITY ? 0.0f : top;
-                bs[lane] = h;
-                bk[(t & 1) * 16 * QC + lane] = exp2_fast(m - h);
-                m = top;
+            for (int x = 0; x < QC / 2; ++x) top = fmaxf(top, fmaxf(unpack2(s[x]).x, unpack2(s[x]).y));
+            if (__any_sync(0xffffffffu, top > kMoveBits) && lane == 0) moves[4 * (t & 1)] = t + 1;
+            arrive_warp(&part_bar[part]);
+            if (PB == 2 && !draft && begun > 1) fold(t - 2, u2, moved2);   // (by now its products are made)
+            if (!ok || !wait_warp(&part_bar[part], met++ & 1, 20)) break;
+            const bool moved = *reinterpret_cast<volatile int*>(&moves[4 * (t & 1)]) == t + 1 || __any_sync(0xffffffffu, unset);
+            if (moved) {
+                // the columns' largest scores, absolute: lane c has column c
+                float best = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < QC / 2; ++x) {
+                    const float y0 = warp_max(unpack2(s[x]).x), y1 = warp_max(unpack2(s[x]).y);
+                    if (lane == 2 * x) best = y0;
+                    if (lane == 2 * x + 1) best = y1;
+                }
+                if (lane < QC) xm[(t & 1) * 16 * QC + quarter * QC + lane] = best;
+                if (!meet()) break;
+                float by = 0.0f;                               // how far h moves
+                if (lane < QC) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) best = fmaxf(best, xm[(t & 1) * 16 * QC + q * QC + lane]);
+                    by = unset ? (best > -INFINITY ? best : 0.0f) : fmaxf(best, 0.0f);
+                    h += by;
+                    bs[lane] = h;
+                    bk[(t & 1) * 16 * QC + lane] = unset ? 0.0f : exp2_fast(-by);
+                    bd[lane] = by;
+                    unset = unset && !(best > -INFINITY);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < QC / 2; ++x) {
+                    const float2 dd = *reinterpret_cast<const float2*>(bd + 2 * x), bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + 2 * x);
+                    s[x] = add2(s[x], pack2(-dd.x, -dd.y));
+                    l[x] = mul2(l[x], pack2(bb.x, bb.y));
+                }
             }
-            __syncwarp();
             // probabilities, their sums, weights in the range of f16
             float f, un;
-            f16_factor(vtop, f, un);
+            f16_factor(vtop, kWeightBits, f, un);
             const float vf = vs * f;
-            const bool count = !draft || key < 64;
+            if (draft) {
 #pragma unroll
-            for (int x = 0; x < QC; x += 2) {
-                const float2 h = *reinterpret_cast<const float2*>(bs + x), bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + x);
-                const float e0 = exp2_fast(s[x] - h.x), e1 = exp2_fast(s[x + 1] - h.y);
-                l[x / 2] = fma2(l[x / 2], pack2(bb.x, bb.y), count ? pack2(e0, e1) : 0ull);
-                // (what a column does not see weighs nothing, whatever its scale is)
-                s[x] = draft && s[x] == -INFINITY ? 0.0f : e0 * vf;
-                s[x + 1] = draft && s[x + 1] == -INFINITY ? 0.0f : e1 * vf;
-            }
-            if (!draft && t > 0 && !wait_warp(pfree, (t - 1) & 1, 20)) break;
-            if (draft) {                                       // everybody has read the exchanged scores
-                arrive_warp(all_bar);
+                for (int x = 0; x < QC / 2; ++x) {
+                    const float2 y = unpack2(s[x]);
+                    const float e0 = exp2_fast(y.x), e1 = exp2_fast(y.y);
+                    if (key < 64) l[x] = add2(l[x], pack2(e0, e1));
+                    // (what a column does not see weighs nothing, whatever its scale is)
+                    s[x] = pack2(y.x == -INFINITY ? 0.0f : e0 * vf, y.y == -INFINITY ? 0.0f : e1 * vf);
+                }
+                arrive_warp(all_bar);                          // everybody has read the exchanged scores
                 if (!wait_warp(all_bar, met_all++ & 1, 20)) break;
-            }
-            unsigned char* pd = sm + Sh::P + key * 128;
-            uint32_t hi[QC / 2], lo[QC / 2];
-#pragma unroll
-            for (int x = 0; x < QC / 2; ++x) split_f16(s[2 * x], s[2 * x + 1], hi[x], lo[x]);
-            if constexpr (QC == 4) {
-                unsigned char* at = pd + (((part >> 1) ^ (key & 7)) << 4) + 8 * (part & 1);
-                *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(at + Sh::PPart) = make_uint2(lo[0], lo[1]);
             } else {
 #pragma unroll
-                for (int q = 0; q < QC / 8; ++q) {
-                    unsigned char* at = pd + (((part * (QC / 8) + q) ^ (key & 7)) << 4);
+                for (int x = 0; x < QC / 2; ++x) {
+                    const float2 y = unpack2(s[x]);
+                    const f32x2 e = pack2(exp2_fast(y.x), exp2_fast(y.y));
+                    l[x] = add2(l[x], e);
+                    s[x] = mul2(e, pack2(vf, vf));
+                }
+            }
+            if (PB == 1 && !draft && begun > 0) fold(t - 1, u1, moved1);
+            if (!ok) break;
+            unsigned char* pd = sm + Sh::P + t % PB * Sh::PParts * Sh::PPart + key * 128;
+            uint32_t hi[QC / 2], lo[QC / 2];
+#pragma unroll
+            for (int x = 0; x < QC / 2; ++x) {
+                const float2 y = unpack2(s[x]);
+                split_f16(y.x, y.y, hi[x], lo[x]);
+            }
+            if constexpr (QC == 4) {
+                unsigned char* at = pd + 8 * (part & 1);
+                *reinterpret_cast<uint2*>(at + (((part >> 1) ^ (key & 7)) << 4)) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(at + (((2 + (part >> 1)) ^ (key & 7)) << 4)) = make_uint2(lo[0], lo[1]);
+            } else if constexpr (QC == 8) {
+                *reinterpret_cast<uint4*>(pd + ((part ^ (key & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(pd + (((4 + part) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    unsigned char* at = pd + (((2 * part + q) ^ (key & 7)) << 4);
                     *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
                     *reinterpret_cast<uint4*>(at + Sh::PPart) = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
                 }
             }
             fence_async_smem();
-            arrive_warp(pfull);
-            if (!(flags & TREE_FIRST)) fold(t - 1);
-            u = un;
+            arrive_warp(&pfull[t & 1]);
+            u2 = u1; moved2 = moved1;
+            u1 = un; moved1 = moved;
             if (flags & TREE_LAST) {
-                fold(t);
+                if (PB == 2 && begun > 0) fold(t - 1, u2, moved2);
+                fold(t, u1, moved1);
                 if (!ok) break;
                 // the item's sums over its keys, then its columns to memory
                 float mine = 0.0f;
@@ -705,16 +826,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 if (lane < QC) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) sum += xl[q * QC + lane];
-                    bs[lane] = d.nsplit > 1 ? 1.0f : sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
+                    bd[lane] = d.nsplit > 1 ? 1.0f : sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
                 }
                 __syncwarp();
                 for (int c = 0; c < QC; ++c) {
                     const int col = part * QC + c;
                     if (col >= d.cols) break;
-                    const int cc = d.col0 + col, tok = cc / p.G, row = d.a + tok, h = d.kvh * p.G + cc - tok * p.G;
-                    float* dst = d.nsplit > 1 ? p.part + (((size_t)row * p.H + h) * p.nsplit + d.split) * (dh + 4)
-                                              : p.out + (size_t)row * p.ldo + (size_t)h * dh;
-                    const float inv = bs[c];
+                    const int cc = d.col0 + col, tok = cc / p.G, row = d.a + tok, head = d.kvh * p.G + cc - tok * p.G;
+                    float* dst = d.nsplit > 1 ? p.part + (((size_t)row * p.H + head) * p.nsplit + d.split) * (dh + 4)
+                                              : p.out + (size_t)row * p.ldo + (size_t)head * dh;
+                    const float inv = bd[c];
 #pragma unroll
                     for (int mh = 0; mh < MH; ++mh) {
                         float y = 0.0f;                        // (registers are not indexed)
@@ -726,7 +847,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                         }
                         if (key + 128 * mh < dh) dst[key + 128 * mh] = y * inv;
                     }
-                    if (d.nsplit > 1 && quarter == 0 && lane == c) { dst[dh] = m; dst[dh + 1] = sum; }
+                    if (d.nsplit > 1 && quarter == 0 && lane == c) { dst[dh] = unset ? -INFINITY : h; dst[dh + 1] = sum; }
                 }
             }
             arrive_warp(&tfree[t & (kTreeRing - 1)]);
