@@ -23,7 +23,7 @@ LIB = PKG / "libb2dec.so"
 FRONT = PKG / "b2run"                    # stdin-tokens front end (host program over the library)
 SOURCES = ["runtime.cu", "launch.cu", "token.cu", "prefill.cu", "capi.cu", "noalloc.cu", "paged.cu", "tree.cu", "groups.cu"]
 HEADERS = ["b2_common.cuh", "gemv.cuh", "attn.cuh", "kernels.cuh", "token.cuh", "prefill.cuh", "paged.cuh", "mma_digits.cuh", "paged_rows.cuh", "paged_host.cuh",
-           "host_checks.cuh", "tree.cuh", "tree_attn.cuh", "groups.cuh", "umma.cuh", "json.h"]
+           "host_checks.cuh", "tree.cuh", "tree_attn.cuh", "groups.cuh", "umma.cuh", "f16_pairs.cuh", "tensor_map.cuh", "json.h"]
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",

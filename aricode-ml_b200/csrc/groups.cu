@@ -4,12 +4,14 @@
 
 #include "groups.cuh"
 #include "host_checks.cuh"
+#include "tensor_map.cuh"
 
 using namespace b2;
 
 namespace {
 
-constexpr int kVectors = 8;              // of a launch
+constexpr int kVectors = 8;              // of a launch of the first kind, for up to so many vectors in all
+constexpr int kGemmVectors = 64;         // of the second
 constexpr size_t kSmem = 227 * 1024;
 
 int fragment_tiles(int T) { return (3 * T + 7) / 8; }          // B columns: three digits of each vector
@@ -63,13 +65,58 @@ cudaError_t launch_groups(const GroupParams& p, int NT, bool bf16, int sms, cuda
     return NT == 1 ? launch_groups<GROUP, 1>(p, bf16, sms, s) : NT == 2 ? launch_groups<GROUP, 2>(p, bf16, sms, s) : launch_groups<GROUP, 3>(p, bf16, sms, s);
 }
 
+// images and units of a block of 128 columns, parts of row tiles
+size_t gemm_bytes(int NT, int n, int sms) { return (size_t)GroupSmem<1>::blocks(n) * NT * (512 + 4) + (size_t)sms * 2 * NT * 128 * sizeof(float); }
+
+int gemm_vectors(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : kGemmVectors; }
+
+template <int GROUP, int NT, bool BF16>
+cudaError_t launch_gemm(const GemmParams& p, int sms, cudaStream_t s) {
+    auto k = group_gemm_kernel<GROUP, NT, BF16>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmShape<GROUP, NT>::Alloc);
+    if (e != cudaSuccess) return e;
+    const int tiles = (p.m + 127) / 128, steps = tiles * GroupSmem<1>::blocks(p.n), ctas = std::min(steps, sms);
+    e = launch_ex(k, dim3((unsigned)ctas), dim3(kGemmThreads), GemmShape<GROUP, NT>::Alloc, s, true, p);
+    if (e != cudaSuccess || ctas == tiles) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)p.T);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1] = {pdl_attr(true)};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, group_add_kernel<NT>, p, ctas);
+}
+
+template <int NT>
+cudaError_t launch_gemm(const GroupParams& g, int group, bool bf16, int sms, cudaStream_t s) {
+    GemmParams p{};
+    EncodeTiled enc = tensor_map_encoder();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)g.ld, (cuuint64_t)g.m}, strides[1] = {(cuuint64_t)g.ld};
+    const cuuint32_t box[2] = {64, 128}, step[2] = {1, 1};
+    if (enc(&p.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(g.W), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    p.scale = g.scale; p.lds = g.lds; p.bias = g.bias; p.y = g.y; p.ldy = g.ldy; p.m = g.m; p.n = g.n; p.T = g.T;
+    p.images = reinterpret_cast<const unsigned char*>(g.digits); p.units = g.units;
+    p.part = g.units + (size_t)GroupSmem<1>::blocks(g.n) * NT;
+    const int words = GroupSmem<1>::blocks(g.n) * 16;
+    cudaError_t e = launch_ex(group_images_kernel<NT>, dim3((unsigned)((words + 255) / 256), (unsigned)g.T), dim3(256), 0, s, true, g);
+    if (e != cudaSuccess) return e;
+#define B2_CALL(G) (bf16 ? launch_gemm<G, NT, true>(p, sms, s) : launch_gemm<G, NT, false>(p, sms, s))
+    return group == 32 ? B2_CALL(32) : group == 64 ? B2_CALL(64) : B2_CALL(128);
+#undef B2_CALL
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t b2_gemv_i4_groups_workspace(int T, int n) {
     if (T <= 2 || n <= 0) return 0;
-    return (size_t)GroupSmem<1>::blocks(n) * fragment_tiles(std::min(T, kVectors)) * (1024 + 32);
+    if (T > kVectors) return gemm_bytes(gemm_vectors(T), n, sm_count());
+    return (size_t)GroupSmem<1>::blocks(n) * fragment_tiles(T) * (1024 + 32);
 }
 
 int b2_gemv_i4_groups(const uint8_t* W, int64_t ld, const void* scale, int64_t lds, int scale_bf16, int group, const float* X,
@@ -91,26 +138,39 @@ int b2_gemv_i4_groups(const uint8_t* W, int64_t ld, const void* scale, int64_t l
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(), unit = scale_bf16 ? 2 : 4;
-    for (int t0 = 0; t0 < T; t0 += kVectors) {
-        const int NT = fragment_tiles(std::min(T, kVectors)), part = columns(NT, n);
-        for (int k0 = 0; k0 < n; k0 += part) {
+    if (T > kVectors) {
+        for (int t0 = 0; t0 < T; t0 += kGemmVectors) {
             GroupParams p{};
-            p.W = W + k0 / 2; p.ld = ld;
-            p.scale = static_cast<const char*>(scale) + (size_t)(k0 / group) * unit; p.lds = lds;
-            p.x = X + (size_t)t0 * ldx + k0; p.ldx = ldx;
-            p.bias = k0 ? nullptr : bias;
-            p.y = Y + (size_t)t0 * ldy; p.ldy = ldy;
-            p.m = m; p.n = std::min(part, n - k0); p.T = std::min(kVectors, T - t0);
-            p.add = k0 > 0;
-            p.warps_k = share(m, p.n, sms);
-            if (T > 2) {
-                p.digits = static_cast<uint4*>(workspace);
-                p.units = reinterpret_cast<float*>(p.digits + (size_t)GroupSmem<1>::blocks(p.n) * NT * 64);
-            }
-            const cudaError_t e = group == 32 ? launch_groups<32>(p, NT, scale_bf16, sms, s) : group == 64 ? launch_groups<64>(p, NT, scale_bf16, sms, s)
-                                                                                          : launch_groups<128>(p, NT, scale_bf16, sms, s);
+            p.W = W; p.ld = ld; p.scale = scale; p.lds = lds; p.bias = bias;
+            p.x = X + (size_t)t0 * ldx; p.ldx = ldx; p.y = Y + (size_t)t0 * ldy; p.ldy = ldy;
+            p.m = m; p.n = n; p.T = std::min(kGemmVectors, T - t0);
+            const int NT = gemm_vectors(T);
+            p.digits = static_cast<uint4*>(workspace);
+            p.units = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + (size_t)GroupSmem<1>::blocks(n) * NT * 512);
+            const cudaError_t e = NT == 16 ? launch_gemm<16>(p, group, scale_bf16, sms, s) : NT == 32 ? launch_gemm<32>(p, group, scale_bf16, sms, s)
+                                                                                                   : launch_gemm<64>(p, group, scale_bf16, sms, s);
             if (e != cudaSuccess) return status(fn, e);
         }
+        return B2_OK;
+    }
+    const int NT = fragment_tiles(T), part = columns(NT, n);
+    for (int k0 = 0; k0 < n; k0 += part) {
+        GroupParams p{};
+        p.W = W + k0 / 2; p.ld = ld;
+        p.scale = static_cast<const char*>(scale) + (size_t)(k0 / group) * unit; p.lds = lds;
+        p.x = X + k0; p.ldx = ldx;
+        p.bias = k0 ? nullptr : bias;
+        p.y = Y; p.ldy = ldy;
+        p.m = m; p.n = std::min(part, n - k0); p.T = T;
+        p.add = k0 > 0;
+        p.warps_k = share(m, p.n, sms);
+        if (T > 2) {
+            p.digits = static_cast<uint4*>(workspace);
+            p.units = reinterpret_cast<float*>(p.digits + (size_t)GroupSmem<1>::blocks(p.n) * NT * 64);
+        }
+        const cudaError_t e = group == 32 ? launch_groups<32>(p, NT, scale_bf16, sms, s) : group == 64 ? launch_groups<64>(p, NT, scale_bf16, sms, s)
+                                                                                      : launch_groups<128>(p, NT, scale_bf16, sms, s);
+        if (e != cudaSuccess) return status(fn, e);
     }
     return B2_OK;
 }

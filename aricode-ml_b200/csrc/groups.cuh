@@ -9,8 +9,10 @@
 // neighbours alone). The digit sums are exact in int32; each is scaled by s and 1 / f into a
 // f32 sum of its own, and the three are joined at the end.
 #pragma once
+#include "f16_pairs.cuh"
 #include "mma_digits.cuh"
 #include "paged_rows.cuh"
+#include "umma.cuh"
 
 namespace b2 {
 
@@ -263,6 +265,349 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
         }
         buf ^= 1;
     }
+}
+
+// ---- more vectors: the 5th-generation tensor cores. Per 128 columns, D [row][vector] = W X^T in
+// f16 with W's codes (exact) as 128 x 128 tiles and x as two f16 each (f16_pairs.cuh) side by side
+// as 2 NT columns; a D for each group, so that its scale and x's unit (for each 128 columns of a
+// vector) come in f32 behind it. Sums in the tensor cores are a group long.
+// A CTA a SM has an equal share of the (128 rows, 128 columns) steps in order: parts of row
+// tiles and whole ones; parts' sums go to the workspace and are added in order of columns.
+// Warps 0 .. 7: sums to f32: warp w has TMEM lanes (rows) 32 (w % 4) .. + 31 and half w / 4 of the vectors.
+// Warps 8 .. 15: codes to f16 operands. Warp 16: copies (packed rows by TMA, x's images by bulk
+// copies). Warp 17: issues the MMAs. Every wait is bounded.
+constexpr int kGemmSumWarps = 8, kGemmConvWarps = 8;
+constexpr int kGemmThreads = (kGemmSumWarps + kGemmConvWarps + 2) * 32;
+
+template <int GROUP, int NT>
+struct GemmShape {
+    static constexpr int Image = NT * 512;                     // x of 128 columns: [half][hi, lo of NT vectors][64 f16], swizzled
+    static constexpr int Units = NT * 4;                       // and their units
+    static constexpr int Tile = 128 * 256;                     // codes as f16: [half][row][64 f16], swizzled
+    static constexpr int Packed = 128 * 64;                    // codes as they come: [row][64 bytes]
+    static constexpr int SX = NT == 64 ? 3 : 4, SW = NT == 64 ? 6 : 8, SA = 2;
+    static constexpr int GS = 128 / GROUP;                     // groups of a step
+    static constexpr int DB = 512 / (2 * NT) < 8 ? 512 / (2 * NT) : 8;     // sums in TMEM
+    static constexpr int A = 0;
+    static constexpr int X = A + SA * Tile;
+    static constexpr int W = X + SX * Image;
+    static constexpr int U = W + SW * Packed;
+    static constexpr int Bars = U + SX * Units;
+    static constexpr int NBars = 2 * SA + 2 * SX + 2 * SW + 2 * DB + 1;
+    static constexpr int Alloc = Bars + NBars * 8 + 16 + 1024;
+    static constexpr int TmemCols = DB * 2 * NT <= 256 ? 256 : 512;
+    static_assert(Alloc <= 227 * 1024, "");
+};
+
+struct GemmParams {
+    CUtensorMap W;           // [m][ld] bytes
+    const void* scale;
+    long long lds;
+    const unsigned char* images;   // [blocks][NT * 512]
+    const float* units;            // [blocks][NT]
+    const float* bias;
+    float* y;
+    long long ldy;
+    int m, n, T;
+    float* part;             // [CTA][2][NT][128]: its first and its last part of a row tile
+};
+
+// A CTA's steps: first .. end - 1 of blocks steps for each row tile.
+struct GemmShare {
+    int first, end;
+};
+__host__ __device__ inline GemmShare gemm_share(int steps, int ctas, int cta) {
+    return {(int)((long long)steps * cta / ctas), (int)((long long)steps * (cta + 1) / ctas)};
+}
+
+// x as images: words of 8 columns, 16 lanes for a block of 128; in each word the columns stand as
+// the codes come out of it: 0 4 1 5 2 6 3 7
+template <int NT>
+__global__ void __launch_bounds__(256) group_images_kernel(const __grid_constant__ GroupParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int word = blockIdx.x * 256 + threadIdx.x, kb = word >> 4, w = word & 15, t = blockIdx.y;
+    const bool live = kb * 128 < p.n;
+    const int k0 = kb * 128 + 8 * w;
+    const float* src = p.x + (size_t)t * p.ldx + k0;
+    float x[8], top = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[i] = live && k0 + i < p.n ? src[i] : 0.0f;
+        bad |= x[i] != x[i];
+        top = fmaxf(top, fabsf(x[i]));
+    }
+    if (bad) top = INFINITY;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!live) return;
+    float f, unit;
+    f16_factor(top, kRowBits, f, unit);
+    const bool fine = top < INFINITY;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_f16(fine ? x[i] * f : 0.0f, fine ? x[i + 4] * f : 0.0f, hi[i], lo[i]);
+    unsigned char* image = reinterpret_cast<unsigned char*>(p.digits) + (size_t)kb * (NT * 512) + (w >> 3) * (NT * 256);
+    *reinterpret_cast<uint4*>(image + t * 128 + (((w & 7) ^ (t & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(image + (NT + t) * 128 + (((w & 7) ^ (t & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (w == 0) p.units[(size_t)kb * NT + t] = fine ? unit : __int_as_float(0x7fffffff);
+}
+
+template <int GROUP, int NT, bool BF16>
+__global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __grid_constant__ GemmParams p) {
+    using Sh = GemmShape<GROUP, NT>;
+    constexpr int GS = Sh::GS, DB = Sh::DB;
+    extern __shared__ unsigned char gm_raw[];
+    unsigned char* sm = gm_raw + ((1024u - (smem_u32(gm_raw) & 1023u)) & 1023u);
+    uint64_t* wfull = reinterpret_cast<uint64_t*>(sm + Sh::Bars);      // [SW] packed codes have come
+    uint64_t* wempty = wfull + Sh::SW;
+    uint64_t* xfull = wempty + Sh::SW;                                 // [SX] an image and its units
+    uint64_t* xempty = xfull + Sh::SX;
+    uint64_t* afull = xempty + Sh::SX;                                 // [SA] codes as f16
+    uint64_t* aempty = afull + Sh::SA;
+    uint64_t* dfull = aempty + Sh::SA;                                 // [DB] a group's sums
+    uint64_t* dempty = dfull + DB;
+    uint64_t* done = dempty + DB;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kCopyWarp = kGemmSumWarps + kGemmConvWarps, kMmaWarp = kCopyWarp + 1;
+    const int blocks = (p.n + 127) >> 7, tiles = (p.m + 127) >> 7;
+    const GemmShare mine = gemm_share(blocks * tiles, gridDim.x, blockIdx.x);
+    const int steps = mine.end - mine.first;
+
+    if (tid == 0) {
+        for (int i = 0; i < Sh::SW; ++i) { mbar_init(&wfull[i], 1); mbar_init(&wempty[i], kGemmConvWarps); }
+        for (int i = 0; i < Sh::SX; ++i) { mbar_init(&xfull[i], 1); mbar_init(&xempty[i], 1 + kGemmSumWarps); }
+        for (int i = 0; i < Sh::SA; ++i) { mbar_init(&afull[i], kGemmConvWarps * 32); mbar_init(&aempty[i], 1); }
+        for (int i = 0; i < DB; ++i) { mbar_init(&dfull[i], 1); mbar_init(&dempty[i], kGemmSumWarps); }
+        mbar_init(done, 1);
+        fence_mbar_init();
+        *fail = 0;
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Sh::TmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+    pdl_wait();
+    auto wait = [&](uint64_t* bar, int parity) {               // false: it ran out (1 s)
+        bool ok = mbar_try_wait(bar, (uint32_t)parity);
+        if (!ok) ok = mbar_wait_bounded(bar, (uint32_t)parity);
+        if (!ok) *fail = 1;
+        return __all_sync(0xffffffffu, ok) != 0;
+    };
+    auto arrive_warp = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+
+    if (warp == kCopyWarp) {
+        int ws = 0, xs = 0;                                    // copies asked for
+        for (int i = 0; i < steps; ++i) {
+            const int at = mine.first + i, kb = at % blocks, tile = at / blocks, sw = i % Sh::SW, sx = i % Sh::SX;
+            if (i >= Sh::SW && !wait(&wempty[sw], (i / Sh::SW - 1) & 1)) break;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&wfull[sw], Sh::Packed);
+                tma_load_2d(sm + Sh::W + sw * Sh::Packed, &p.W, 64 * kb, 128 * tile, &wfull[sw]);
+            }
+            ++ws;
+            if (i >= Sh::SX && !wait(&xempty[sx], (i / Sh::SX - 1) & 1)) break;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&xfull[sx], Sh::Image + Sh::Units);
+                bulk_g2s(sm + Sh::X + sx * Sh::Image, p.images + (size_t)kb * Sh::Image, Sh::Image, &xfull[sx]);
+                bulk_g2s(sm + Sh::U + sx * Sh::Units, p.units + (size_t)kb * NT, Sh::Units, &xfull[sx]);
+            }
+            ++xs;
+        }
+        // no copy may be under way when the memory is given up
+        __syncwarp();
+        for (int j = max(ws - Sh::SW, 0); j < ws; ++j)
+            if (!mbar_wait_bounded(&wfull[j % Sh::SW], (j / Sh::SW) & 1)) *fail = 1;
+        for (int j = max(xs - Sh::SX, 0); j < xs; ++j)
+            if (!mbar_wait_bounded(&xfull[j % Sh::SX], (j / Sh::SX) & 1)) *fail = 1;
+    } else if (warp == kMmaWarp) {
+        const bool me = elect_lane();
+        constexpr uint32_t id = umma_idesc_f16(2 * NT, false, false);
+        const uint64_t adesc = umma_desc_sw128(smem_u32(sm) + Sh::A), xdesc = umma_desc_sw128(smem_u32(sm) + Sh::X);
+        for (int i = 0; i < steps; ++i) {
+            const int sa = i % Sh::SA, sx = i % Sh::SX;
+            if (!wait(&afull[sa], (i / Sh::SA) & 1) || !wait(&xfull[sx], (i / Sh::SX) & 1)) break;
+            const uint64_t ad = adesc + (uint64_t)(sa * (Sh::Tile >> 4)), xd = xdesc + (uint64_t)(sx * (Sh::Image >> 4));
+            bool ok = true;
+#pragma unroll
+            for (int g = 0; g < GS; ++g) {
+                const int u = i * GS + g, b = u % DB;
+                if (u >= DB) ok = ok && wait(&dempty[b], (u / DB - 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int j = 0; j < GROUP / 16; ++j) {
+                    const int k = g * (GROUP / 16) + j;
+                    const uint64_t a = ad + ((k >> 2) * 128 * 128 + 32 * (k & 3)) / 16, x = xd + ((k >> 2) * (NT * 256) + 32 * (k & 3)) / 16;
+                    if (j == 0) umma_f16<false>(me, tmem + b * 2 * NT, a, x, id);
+                    else umma_f16<true>(me, tmem + b * 2 * NT, a, x, id);
+                }
+                if (me) umma_commit(&dfull[b]);
+            }
+            if (!ok) break;
+            if (me) {
+                umma_commit(&aempty[sa]);
+                umma_commit(&xempty[sx]);
+            }
+        }
+        if (me) umma_commit(done);                             // also after a wait that ran out
+        __syncwarp();
+        if (!mbar_wait_bounded(done, 0)) *fail = 1;
+    } else if (warp >= kGemmSumWarps) {
+        // codes to f16: a thread 16 bytes (32 codes) of a row at a time. A code c lies as c ^ 8 above
+        // 1024 in f16: 1032 + c
+        const int ct = tid - kGemmSumWarps * 32, chunk = ct & 3, r0 = ct >> 2;
+        for (int i = 0; i < steps; ++i) {
+            const int sw = i % Sh::SW, sa = i % Sh::SA;
+            if (!wait(&wfull[sw], (i / Sh::SW) & 1)) break;
+            uint4 v[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) v[x] = lds128(sm + Sh::W + sw * Sh::Packed + (r0 + 64 * x) * 64 + 16 * chunk);
+            if (i >= Sh::SA && !wait(&aempty[sa], (i / Sh::SA - 1) & 1)) break;
+            unsigned char* part = sm + Sh::A + sa * Sh::Tile + (chunk >> 1) * (128 * 128);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int row = r0 + 64 * x;
+                const uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+#pragma unroll
+                for (int j0 = 0; j0 < 4; ++j0) {
+                    const int turn = chunk & 2;                // (halves two units apart: no bank conflicts)
+                    const uint32_t y = turn ? w[j0 ^ 2] : w[j0];
+                    const int unit = 4 * (chunk & 1) + (j0 ^ turn);
+                    uint32_t r[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t z = (y >> (4 * e) & 0x000f000fu) ^ 0x64086408u;
+                        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&z), __half2half2(__ushort_as_half(0x6408)));
+                        r[e] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    *reinterpret_cast<uint4*>(part + row * 128 + ((unit ^ (row & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&afull[sa]);
+            arrive_warp(&wempty[sw]);
+        }
+    } else {
+        // sums
+        constexpr int C = NT / 2, RC = 8;                      // vectors of a thread; read at a time
+        const int quarter = warp & 3, c0 = (warp >> 2) * C, r = 32 * quarter + lane;
+        const uint32_t trow = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)c0;
+        const int groups = (p.n + GROUP - 1) / GROUP;
+        auto scales = [&](int at, float (&s)[GS]) {            // of this thread's row in step `at`
+            const int row = at / blocks * 128 + r, g0 = at % blocks * GS;
+#pragma unroll
+            for (int g = 0; g < GS; ++g)
+                s[g] = at < mine.end && row < p.m && g0 + g < groups ? group_scale<BF16>(p.scale, (size_t)row * p.lds + g0 + g) : 0.0f;
+        };
+        float next[GS];
+        scales(mine.first, next);
+        f32x2 acc[C / 2];
+#pragma unroll
+        for (int x = 0; x < C / 2; ++x) acc[x] = 0ull;
+        int kfirst = mine.first;                               // of this part of a row tile
+        for (int i = 0; i < steps; ++i) {
+            const int at = mine.first + i, sx = i % Sh::SX;
+            float s[GS];
+#pragma unroll
+            for (int g = 0; g < GS; ++g) s[g] = next[g];
+            scales(at + 1, next);
+            if (!wait(&xfull[sx], (i / Sh::SX) & 1)) break;
+            const float* un = reinterpret_cast<const float*>(sm + Sh::U + sx * Sh::Units) + c0;
+            bool ok = true;
+#pragma unroll
+            for (int g = 0; g < GS; ++g) {
+                const int u = i * GS + g, b = u % DB;
+                ok = ok && wait(&dfull[b], (u / DB) & 1);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int q = 0; q < C / RC; ++q) {
+                    uint32_t hi[RC], lo[RC];
+                    tmem_ld8(trow + b * 2 * NT + q * RC, hi);
+                    tmem_ld8(trow + b * 2 * NT + NT + q * RC, lo);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < RC / 2; ++x) {
+                        const float2 uu = *reinterpret_cast<const float2*>(un + q * RC + 2 * x);
+                        acc[q * RC / 2 + x] = fma2(add2(pack2(__uint_as_float(hi[2 * x]), __uint_as_float(hi[2 * x + 1])),
+                                                        pack2(__uint_as_float(lo[2 * x]), __uint_as_float(lo[2 * x + 1]))),
+                                                   mul2(pack2(uu.x, uu.y), pack2(s[g], s[g])), acc[q * RC / 2 + x]);
+                    }
+                }
+                tc_fence_before();
+                arrive_warp(&dempty[b]);
+            }
+            if (!ok) break;
+            arrive_warp(&xempty[sx]);
+            if ((at + 1) % blocks != 0 && i + 1 < steps) continue;
+            // the end of the row tile, or of the share
+            const int tile = at / blocks, row = tile * 128 + r;
+            const bool whole = kfirst % blocks == 0 && (at + 1) % blocks == 0;
+            float* dst = whole ? p.y + row : p.part + ((size_t)blockIdx.x * 2 + (kfirst == mine.first ? 0 : 1)) * NT * 128 + r;
+            const long long ld = whole ? p.ldy : 128;
+            const float bias = whole && p.bias && row < p.m ? p.bias[row] : 0.0f;
+#pragma unroll
+            for (int x = 0; x < C / 2; ++x) {
+                const float2 y = unpack2(acc[x]);
+                acc[x] = 0ull;
+                const int v = c0 + 2 * x;
+                if (whole && row >= p.m) continue;
+                if (v < p.T) dst[v * ld] = whole && p.bias ? fadd(y.x, bias) : y.x;
+                if (v + 1 < p.T) dst[(v + 1) * ld] = whole && p.bias ? fadd(y.y, bias) : y.y;
+            }
+            kfirst = at + 1;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Sh::TmemCols) : "memory");
+    }
+    // a wait that ran out: the outputs say so
+    if (*fail) {
+        const float nan = __int_as_float(0x7fffffff);
+        for (int i = tid; i < 2 * NT * 128; i += kGemmThreads) p.part[(size_t)blockIdx.x * 2 * NT * 128 + i] = nan;
+        for (int row = mine.first / blocks * 128 + tid; row < min((mine.end + blocks - 1) / blocks * 128, p.m); row += kGemmThreads)
+            for (int v = 0; v < p.T; ++v) p.y[(size_t)v * p.ldy + row] = nan;
+    }
+}
+
+// Adds the parts of row tiles that several CTAs have, in order of columns: grid (tiles, T).
+template <int NT>
+__global__ void __launch_bounds__(128) group_add_kernel(const __grid_constant__ GemmParams p, int ctas) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int blocks = (p.n + 127) >> 7, tiles = (p.m + 127) >> 7, tile = blockIdx.x, v = blockIdx.y, row = tile * 128 + threadIdx.x;
+    const int steps = blocks * tiles, first = tile * blocks, last = first + blocks - 1;
+    // the CTA of a step: the share that it lies in
+    auto cta_of = [&](int at) {
+        int c = (int)(((long long)at * ctas) / steps);
+        while (gemm_share(steps, ctas, c).end <= at) ++c;
+        while (gemm_share(steps, ctas, c).first > at) --c;
+        return c;
+    };
+    const int a = cta_of(first), b = cta_of(last);
+    if (a == b || row >= p.m) return;
+    float y = 0.0f;
+    for (int c = a; c <= b; ++c) {
+        const int part = gemm_share(steps, ctas, c).first >= first ? 0 : 1;
+        y += p.part[(((size_t)c * 2 + part) * NT + v) * 128 + threadIdx.x];
+    }
+    p.y[(size_t)v * p.ldy + row] = p.bias ? fadd(y, p.bias[row]) : y;
 }
 
 }  // namespace b2

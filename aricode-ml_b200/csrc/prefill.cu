@@ -1,42 +1,24 @@
 // prefill.cu — host side of the batched prefill kernels (prefill.cuh): TMA tensor
 // maps (through the driver entry point, no libcuda link) and the launches.
-#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
-#include <mutex>
 #include <vector>
 
 #include "prefill.cuh"
+#include "tensor_map.cuh"
 
 namespace b2 {
 
 namespace {
 
-typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encoder() {
-    static std::once_flag once;
-    static EncodeTiled fn = nullptr;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiled>(p);
-    });
-    return fn;
-}
-
 // 2-D byte matrix [rows][cols] with row stride `stride` bytes; box = 128 bytes of
 // a row x box_rows rows, 128-byte swizzle (the UMMA K-major SW128 layout);
 // reads past cols or rows are zeros
 bool byte_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t box_rows) {
-    EncodeTiled enc = encoder();
+    EncodeTiled enc = tensor_map_encoder();
     if (!enc) return false;
     const cuuint64_t dims[2] = {cols, rows};
     const cuuint64_t strides[1] = {stride};

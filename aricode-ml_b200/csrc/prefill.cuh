@@ -99,14 +99,6 @@ struct PfAttnParams {
     Mirror mir;              // and written into every peer's copy of it
 };
 
-// ------------------------------------------------------------------ PTX wrappers
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
 // ------------------------------------------------------------------ planes
 // One CTA of 256 threads per token: x (f32 [n], row t of `x` with stride ldx) ->
 // optional RMSNorm (gain g) -> S -> planes [4][Tpad][ldp] bytes (zeros past n up

@@ -16,8 +16,7 @@
 // above it: then its largest is found across the lanes; a tile that moves nothing needs no
 // more than the warps' word that it does not.
 #pragma once
-#include <cuda_fp16.h>
-
+#include "f16_pairs.cuh"
 #include "paged_rows.cuh"
 #include "umma.cuh"
 
@@ -126,24 +125,8 @@ __device__ __forceinline__ uint4 codes_f16(uint32_t a, uint32_t b) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// two values as two f16 each: hi the nearest, lo what is left
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-
-// the power of two that brings `top` (finite, >= 0) to [2^bits, 2^(bits + 1)), and its reciprocal;
-// tiny ones are brought as far as 2^126 does
-constexpr int kRowBits = 13, kWeightBits = 5;      // (weights: probabilities may reach 2^kMoveBits)
+constexpr int kWeightBits = 5;                     // (weights: probabilities may reach 2^kMoveBits)
 constexpr float kMoveBits = 8.0f;
-__device__ __forceinline__ void f16_factor(float top, int bits, float& f, float& unit) {
-    const int e = min(max(bits + 254 - (int)(__float_as_uint(top) >> 23), 1), 253);
-    f = __int_as_float(e << 23);
-    unit = __int_as_float((254 - e) << 23);
-}
 
 __device__ __forceinline__ float warp_max(float x) {
     float r;

@@ -1,6 +1,8 @@
 // umma.cuh — PTX wrappers of the 5th-generation tensor cores (tcgen05 kind::i8 and f16, TMEM
 // reads), shared by the prefill GEMM, the paged attention and the tree attention.
 #pragma once
+#include <cuda.h>
+
 #include "b2_common.cuh"
 
 namespace b2 {
@@ -91,6 +93,14 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
 __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+}
+
+// a box of a 2-D tensor map to shared memory, completion signalled on `bar`
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
 }
 
 // generic-proxy writes to shared memory before tcgen05 operations that read them

@@ -2,9 +2,10 @@
 
 Tolerance. u = 2^-24 is half a step of f32, A = sum |s c x| over a row, B the same with each |x| replaced by the largest of
 its 128 neighbours. A vector's elements are rounded to 2^-24 of that largest (B u), or
-to 2^-127 where that is more (the factor that makes them integers is 2^126 at most): 2^-127 C, C the sum of |s c|; a group's sum is exact, or at most nine
-f32 roundings of its terms; its conversion, the joining of partial sums, the scale and each addition of a group's result to
-the row's are roundings of at most A; the bias one more: u (B + (groups + 17) A + |y|) + 2^-127 C."""
+to 2^-127 where that is more (the factor that makes them integers is 2^126 at most): 2^-127 C, C the sum of |s c|; a group's sum is exact, or (more than
+eight vectors) of f16 pairs, which are 4 u off, by a unit that adds 16 products at a time and cuts off: 2 u for each of 8
+steps and as much again inside a step; its conversion, the joining of partial sums, the unit, the scale and each addition of
+a group's result to the row's are roundings of at most A; the bias one more: u (B + (groups + 32) A + 2 |y|) + 2^-127 C."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -40,7 +41,7 @@ def product64(torch, W, scale, x, group, bias=None):
     top = torch.nn.functional.pad(xd.abs(), (0, -n % 128)).unflatten(1, (-1, 128)).amax(-1).repeat_interleave(128, 1)[:, :n]
     y = xd @ w.T + (0 if bias is None else bias.double())
     a, b = xd.abs() @ w.abs().T, top @ w.abs().T
-    return y, U * (b + (scale.shape[1] + 17) * a + 2 * y.abs()) + 2.0 ** -127 * w.abs().sum(1)
+    return y, U * (b + (scale.shape[1] + 32) * a + 2 * y.abs()) + 2.0 ** -127 * w.abs().sum(1)
 
 
 def close(got, want, tol):
