@@ -44,7 +44,7 @@ template <int GROUP, int NT, bool BF16>
 cudaError_t launch_gemv_groups(const GroupParams& p, int sms, cudaStream_t s) {
     const int smem = (int)smem_bytes(NT, p.n);
     auto k = group_gemv_kernel<GROUP, NT, BF16>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = allow_smem<group_gemv_kernel<GROUP, NT, BF16>>(smem);
     if (e != cudaSuccess) return e;
     const int tiles = (p.m + 15) / 16, slots = kGroupWarps / p.warps_k;
     return launch_ex(k, dim3((unsigned)std::min((tiles + slots - 1) / slots, sms)), dim3(kGroupWarps * 32), smem, s, true, p);
@@ -73,7 +73,7 @@ int gemm_vectors(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : kGemmVectors; }
 template <int GROUP, int NT, bool BF16>
 cudaError_t launch_gemm(const GemmParams& p, int sms, cudaStream_t s) {
     auto k = group_gemm_kernel<GROUP, NT, BF16>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmShape<GROUP, NT>::Alloc);
+    cudaError_t e = allow_smem<group_gemm_kernel<GROUP, NT, BF16>>(GemmShape<GROUP, NT>::Alloc);
     if (e != cudaSuccess) return e;
     const int tiles = (p.m + 127) / 128, steps = tiles * GroupSmem<1>::blocks(p.n), ctas = std::min(steps, sms);
     e = launch_ex(k, dim3((unsigned)ctas), dim3(kGemmThreads), GemmShape<GROUP, NT>::Alloc, s, true, p);

@@ -268,34 +268,37 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
 }
 
 // ---- more vectors: the 5th-generation tensor cores. Per 128 columns, D [row][vector] = W X^T in
-// f16 with W's codes (exact) as 128 x 128 tiles and x as two f16 each (f16_pairs.cuh) side by side
-// as 2 NT columns; a D for each group, so that its scale and x's unit (for each 128 columns of a
+// f16 with W's codes (exact) as 128 x 128 tiles and x as two f16 each (f16_pairs.cuh), lo and then
+// hi into the same sums (side by side, as 2 NT columns, the MMAs took two thirds of the time, but
+// what is bound is reading the sums); a D for each group, so that its scale and x's unit (for each 128 columns of a
 // vector) come in f32 behind it. Sums in the tensor cores are a group long.
 // A CTA a SM has an equal share of the (128 rows, 128 columns) steps in order: parts of row
 // tiles and whole ones; parts' sums go to the workspace and are added in order of columns.
 // Warps 0 .. 7: sums to f32: warp w has TMEM lanes (rows) 32 (w % 4) .. + 31 and half w / 4 of the vectors.
-// Warps 8 .. 15: codes to f16 operands. Warp 16: copies (packed rows by TMA, x's images by bulk
-// copies). Warp 17: issues the MMAs. Every wait is bounded.
+// Warps 8 .. 15: codes to f16 operands. Warps 16, 17: copies (packed rows by TMA, with x's units; its
+// images by bulk copies: one warp for all was what a step waited for). Warp 18: issues the MMAs. Every wait
+// is bounded.
 constexpr int kGemmSumWarps = 8, kGemmConvWarps = 8;
-constexpr int kGemmThreads = (kGemmSumWarps + kGemmConvWarps + 2) * 32;
+constexpr int kTeam = kGemmConvWarps / 2 * 32;                 // threads that turn a step's codes
+constexpr int kGemmThreads = (kGemmSumWarps + kGemmConvWarps + 3) * 32;
 
 template <int GROUP, int NT>
 struct GemmShape {
     static constexpr int Image = NT * 512;                     // x of 128 columns: [half][hi, lo of NT vectors][64 f16], swizzled
-    static constexpr int Units = NT * 4;                       // and their units
+    static constexpr int Units = NT * 4;                       // and what a unit of them is, by vector
     static constexpr int Tile = 128 * 256;                     // codes as f16: [half][row][64 f16], swizzled
     static constexpr int Packed = 128 * 64;                    // codes as they come: [row][64 bytes]
     static constexpr int SX = NT == 64 ? 3 : 4, SW = NT == 64 ? 6 : 8, SA = 2;
     static constexpr int GS = 128 / GROUP;                     // groups of a step
-    static constexpr int DB = 512 / (2 * NT) < 8 ? 512 / (2 * NT) : 8;     // sums in TMEM
+    static constexpr int DB = 8;                               // sums in TMEM
     static constexpr int A = 0;
     static constexpr int X = A + SA * Tile;
     static constexpr int W = X + SX * Image;
     static constexpr int U = W + SW * Packed;
-    static constexpr int Bars = U + SX * Units;
+    static constexpr int Bars = U + SW * Units;
     static constexpr int NBars = 2 * SA + 2 * SX + 2 * SW + 2 * DB + 1;
     static constexpr int Alloc = Bars + NBars * 8 + 16 + 1024;
-    static constexpr int TmemCols = DB * 2 * NT <= 256 ? 256 : 512;
+    static constexpr int TmemCols = DB * NT;
     static_assert(Alloc <= 227 * 1024, "");
 };
 
@@ -303,7 +306,7 @@ struct GemmParams {
     CUtensorMap W;           // [m][ld] bytes
     const void* scale;
     long long lds;
-    const unsigned char* images;   // [blocks][NT * 512]
+    const unsigned char* images;   // [blocks][GemmShape::Image]
     const float* units;            // [blocks][NT]
     const float* bias;
     float* y;
@@ -312,12 +315,11 @@ struct GemmParams {
     float* part;             // [CTA][2][NT][128]: its first and its last part of a row tile
 };
 
-// A CTA's steps: first .. end - 1 of blocks steps for each row tile.
-struct GemmShare {
-    int first, end;
-};
-__host__ __device__ inline GemmShare gemm_share(int steps, int ctas, int cta) {
-    return {(int)((long long)steps * cta / ctas), (int)((long long)steps * (cta + 1) / ctas)};
+// The first of a CTA's steps (of blocks steps for each row tile), and the CTA that has a step.
+__device__ __forceinline__ int gemm_first(int steps, int ctas, int cta) { return cta * (steps / ctas) + min(cta, steps % ctas); }
+__device__ __forceinline__ int gemm_cta(int steps, int ctas, int at) {
+    const int each = steps / ctas, more = steps % ctas, turn = more * (each + 1);
+    return at < turn ? at / (each + 1) : more + (at - turn) / each;
 }
 
 // x as images: words of 8 columns, 16 lanes for a block of 128; in each word the columns stand as
@@ -348,10 +350,10 @@ __global__ void __launch_bounds__(256) group_images_kernel(const __grid_constant
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_f16(fine ? x[i] * f : 0.0f, fine ? x[i + 4] * f : 0.0f, hi[i], lo[i]);
+    if (w == 0) p.units[(size_t)kb * NT + t] = fine ? unit : __int_as_float(0x7fffffff);
     unsigned char* image = reinterpret_cast<unsigned char*>(p.digits) + (size_t)kb * (NT * 512) + (w >> 3) * (NT * 256);
     *reinterpret_cast<uint4*>(image + t * 128 + (((w & 7) ^ (t & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4*>(image + (NT + t) * 128 + (((w & 7) ^ (t & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    if (w == 0) p.units[(size_t)kb * NT + t] = fine ? unit : __int_as_float(0x7fffffff);
 }
 
 template <int GROUP, int NT, bool BF16>
@@ -372,19 +374,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kCopyWarp = kGemmSumWarps + kGemmConvWarps, kMmaWarp = kCopyWarp + 1;
+    constexpr int kCopyWarp = kGemmSumWarps + kGemmConvWarps, kMmaWarp = kCopyWarp + 2;
     const int blocks = (p.n + 127) >> 7, tiles = (p.m + 127) >> 7;
-    const GemmShare mine = gemm_share(blocks * tiles, gridDim.x, blockIdx.x);
-    const int steps = mine.end - mine.first;
+    const int first = gemm_first(blocks * tiles, gridDim.x, blockIdx.x), end = gemm_first(blocks * tiles, gridDim.x, blockIdx.x + 1);
+    const int steps = end - first;
 
-    if (tid == 0) {
-        for (int i = 0; i < Sh::SW; ++i) { mbar_init(&wfull[i], 1); mbar_init(&wempty[i], kGemmConvWarps); }
-        for (int i = 0; i < Sh::SX; ++i) { mbar_init(&xfull[i], 1); mbar_init(&xempty[i], 1 + kGemmSumWarps); }
-        for (int i = 0; i < Sh::SA; ++i) { mbar_init(&afull[i], kGemmConvWarps * 32); mbar_init(&aempty[i], 1); }
-        for (int i = 0; i < DB; ++i) { mbar_init(&dfull[i], 1); mbar_init(&dempty[i], kGemmSumWarps); }
-        mbar_init(done, 1);
+    if (tid < Sh::NBars) {
+        const int i = tid, w = 2 * Sh::SW, x = w + 2 * Sh::SX, a = x + 2 * Sh::SA, d = a + 2 * DB;
+        mbar_init(wfull + i, i < Sh::SW ? 1 : i < w ? kGemmConvWarps / 2 + kGemmSumWarps : i < x ? 1 : i < x + Sh::SA ? kTeam : i < a ? 1 : i < a + DB ? 1 : i < d ? kGemmSumWarps : 1);
         fence_mbar_init();
-        *fail = 0;
+        if (tid == 0) *fail = 0;
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -408,33 +407,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
         if (lane == 0) mbar_arrive(bar);
     };
 
-    if (warp == kCopyWarp) {
-        int ws = 0, xs = 0;                                    // copies asked for
-        for (int i = 0; i < steps; ++i) {
-            const int at = mine.first + i, kb = at % blocks, tile = at / blocks, sw = i % Sh::SW, sx = i % Sh::SX;
-            if (i >= Sh::SW && !wait(&wempty[sw], (i / Sh::SW - 1) & 1)) break;
+    if (warp == kCopyWarp || warp == kCopyWarp + 1) {
+        const bool codes = warp == kCopyWarp;
+        uint64_t *full = codes ? wfull : xfull, *empty = codes ? wempty : xempty;
+        const int slots = codes ? Sh::SW : Sh::SX;
+        int kb = first % blocks, tile = first / blocks, i = 0, slot = 0, turn = 1;      // turn: parity of the slots' last emptying
+        for (; i < steps; ++i) {
+            if (i >= slots && !wait(&empty[slot], turn)) break;
             if (lane == 0) {
-                mbar_arrive_expect_tx(&wfull[sw], Sh::Packed);
-                tma_load_2d(sm + Sh::W + sw * Sh::Packed, &p.W, 64 * kb, 128 * tile, &wfull[sw]);
+                mbar_arrive_expect_tx(&full[slot], codes ? Sh::Packed + Sh::Units : Sh::Image);
+                if (codes) {
+                    tma_load_2d(sm + Sh::W + slot * Sh::Packed, &p.W, 64 * kb, 128 * tile, &full[slot]);
+                    bulk_g2s(sm + Sh::U + slot * Sh::Units, p.units + (size_t)kb * NT, Sh::Units, &full[slot]);
+                } else bulk_g2s(sm + Sh::X + slot * Sh::Image, p.images + (size_t)kb * Sh::Image, Sh::Image, &full[slot]);
             }
-            ++ws;
-            if (i >= Sh::SX && !wait(&xempty[sx], (i / Sh::SX - 1) & 1)) break;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&xfull[sx], Sh::Image + Sh::Units);
-                bulk_g2s(sm + Sh::X + sx * Sh::Image, p.images + (size_t)kb * Sh::Image, Sh::Image, &xfull[sx]);
-                bulk_g2s(sm + Sh::U + sx * Sh::Units, p.units + (size_t)kb * NT, Sh::Units, &xfull[sx]);
-            }
-            ++xs;
+            if (++kb == blocks) { kb = 0; ++tile; }
+            if (++slot == slots) { slot = 0; turn ^= 1; }
         }
         // no copy may be under way when the memory is given up
         __syncwarp();
-        for (int j = max(ws - Sh::SW, 0); j < ws; ++j)
-            if (!mbar_wait_bounded(&wfull[j % Sh::SW], (j / Sh::SW) & 1)) *fail = 1;
-        for (int j = max(xs - Sh::SX, 0); j < xs; ++j)
-            if (!mbar_wait_bounded(&xfull[j % Sh::SX], (j / Sh::SX) & 1)) *fail = 1;
+        for (int j = max(i - slots, 0); j < i; ++j)
+            if (!mbar_wait_bounded(&full[j % slots], (j / slots) & 1)) *fail = 1;
     } else if (warp == kMmaWarp) {
         const bool me = elect_lane();
-        constexpr uint32_t id = umma_idesc_f16(2 * NT, false, false);
+        constexpr uint32_t id = umma_idesc_f16(NT, false, false);
         const uint64_t adesc = umma_desc_sw128(smem_u32(sm) + Sh::A), xdesc = umma_desc_sw128(smem_u32(sm) + Sh::X);
         for (int i = 0; i < steps; ++i) {
             const int sa = i % Sh::SA, sx = i % Sh::SX;
@@ -448,12 +444,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
-                for (int j = 0; j < GROUP / 16; ++j) {
-                    const int k = g * (GROUP / 16) + j;
-                    const uint64_t a = ad + ((k >> 2) * 128 * 128 + 32 * (k & 3)) / 16, x = xd + ((k >> 2) * (NT * 256) + 32 * (k & 3)) / 16;
-                    if (j == 0) umma_f16<false>(me, tmem + b * 2 * NT, a, x, id);
-                    else umma_f16<true>(me, tmem + b * 2 * NT, a, x, id);
-                }
+                for (int e = 1; e >= 0; --e)
+#pragma unroll
+                    for (int j = 0; j < GROUP / 16; ++j) {
+                        const int k = g * (GROUP / 16) + j;
+                        const uint64_t a = ad + ((k >> 2) * 128 * 128 + 32 * (k & 3)) / 16;
+                        const uint64_t x = xd + ((k >> 2) * (NT * 256) + e * (NT * 128) + 32 * (k & 3)) / 16;
+                        if (e == 1 && j == 0) umma_f16<false>(me, tmem + b * NT, a, x, id);
+                        else umma_f16<true>(me, tmem + b * NT, a, x, id);
+                    }
                 if (me) umma_commit(&dfull[b]);
             }
             if (!ok) break;
@@ -466,30 +465,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
         __syncwarp();
         if (!mbar_wait_bounded(done, 0)) *fail = 1;
     } else if (warp >= kGemmSumWarps) {
-        // codes to f16: a thread 16 bytes (32 codes) of a row at a time. A code c lies as c ^ 8 above
-        // 1024 in f16: 1032 + c
-        const int ct = tid - kGemmSumWarps * 32, chunk = ct & 3, r0 = ct >> 2;
-        for (int i = 0; i < steps; ++i) {
-            const int sw = i % Sh::SW, sa = i % Sh::SA;
-            if (!wait(&wfull[sw], (i / Sh::SW) & 1)) break;
-            uint4 v[2];
+        // codes to f16, by two teams of four warps in turn, a step and a place of the operand each: a
+        // thread four times 16 bytes (32 codes) of a row. A code c lies as c ^ 8 above 1024 in f16: 1032 + c
+        const int ct = (tid - kGemmSumWarps * 32) % kTeam, chunk = ct & 3, r0 = ct >> 2, team = (warp - kGemmSumWarps) / (kTeam / 32);
+        unsigned char* part = sm + Sh::A + team * Sh::Tile + (chunk >> 1) * (128 * 128);
+        const bool turn = chunk & 2;                           // (halves two units apart: no bank conflicts)
+        int sw = team, wturn = 0;
+        for (int i = team; i < steps; i += 2) {
+            if (!wait(&wfull[sw], wturn)) break;
+            uint4 v[4];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) v[x] = lds128(sm + Sh::W + sw * Sh::Packed + (r0 + 64 * x) * 64 + 16 * chunk);
-            if (i >= Sh::SA && !wait(&aempty[sa], (i / Sh::SA - 1) & 1)) break;
-            unsigned char* part = sm + Sh::A + sa * Sh::Tile + (chunk >> 1) * (128 * 128);
+            for (int x = 0; x < 4; ++x) v[x] = lds128(sm + Sh::W + sw * Sh::Packed + (r0 + 32 * x) * 64 + 16 * chunk);
+            if (i >= 2 && !wait(&aempty[team], ((i >> 1) - 1) & 1)) break;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int row = r0 + 64 * x;
-                const uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+            for (int x = 0; x < 4; ++x) {
+                const int row = r0 + 32 * x;
+                const uint32_t w[4] = {turn ? v[x].z : v[x].x, turn ? v[x].w : v[x].y, turn ? v[x].x : v[x].z, turn ? v[x].y : v[x].w};
 #pragma unroll
-                for (int j0 = 0; j0 < 4; ++j0) {
-                    const int turn = chunk & 2;                // (halves two units apart: no bank conflicts)
-                    const uint32_t y = turn ? w[j0 ^ 2] : w[j0];
-                    const int unit = 4 * (chunk & 1) + (j0 ^ turn);
+                for (int j = 0; j < 4; ++j) {
+                    const int unit = 4 * (chunk & 1) + (turn ? j ^ 2 : j);
                     uint32_t r[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t z = (y >> (4 * e) & 0x000f000fu) ^ 0x64086408u;
+                        const uint32_t z = (w[j] >> (4 * e) & 0x000f000fu) ^ 0x64086408u;
                         const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&z), __half2half2(__ushort_as_half(0x6408)));
                         r[e] = *reinterpret_cast<const uint32_t*>(&h);
                     }
@@ -497,35 +495,55 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
                 }
             }
             fence_async_smem();
-            mbar_arrive(&afull[sa]);
+            mbar_arrive(&afull[team]);
             arrive_warp(&wempty[sw]);
+            sw += 2;
+            if (sw >= Sh::SW) { sw -= Sh::SW; wturn ^= 1; }
         }
     } else {
         // sums
-        constexpr int C = NT / 2, RC = 8;                      // vectors of a thread; read at a time
+        constexpr int C = NT / 2, RC = C < 16 ? 8 : 16;        // vectors of a thread; read at a time
         const int quarter = warp & 3, c0 = (warp >> 2) * C, r = 32 * quarter + lane;
         const uint32_t trow = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)c0;
         const int groups = (p.n + GROUP - 1) / GROUP;
-        auto scales = [&](int at, float (&s)[GS]) {            // of this thread's row in step `at`
-            const int row = at / blocks * 128 + r, g0 = at % blocks * GS;
+        int kb = first % blocks, tile = first / blocks;        // of the next step
+        // of this thread's row in it, as they lie in memory (whatever is done with a load waits for it)
+        auto scales = [&](uint32_t (&s)[GS]) {
+            const int row = tile * 128 + r;
 #pragma unroll
-            for (int g = 0; g < GS; ++g)
-                s[g] = at < mine.end && row < p.m && g0 + g < groups ? group_scale<BF16>(p.scale, (size_t)row * p.lds + g0 + g) : 0.0f;
+            for (int g = 0; g < GS; ++g) {
+                s[g] = 0u;
+                const size_t at = (size_t)row * p.lds + kb * GS + g;
+                if (row < p.m && kb * GS + g < groups)
+                    s[g] = BF16 ? static_cast<const uint16_t*>(p.scale)[at] : static_cast<const uint32_t*>(p.scale)[at];
+            }
         };
-        float next[GS];
-        scales(mine.first, next);
+        uint32_t next[2][GS];                                  // two steps ahead
+        auto advance = [&]() {
+            if (++kb == blocks) { kb = 0; ++tile; }
+        };
+        scales(next[0]);
+        advance();
+        scales(next[1]);
         f32x2 acc[C / 2];
 #pragma unroll
         for (int x = 0; x < C / 2; ++x) acc[x] = 0ull;
-        int kfirst = mine.first;                               // of this part of a row tile
+        bool begun = first % blocks == 0;                      // this part has the row tile's first columns
+        int at = first % blocks, rows = first / blocks;        // of this step
+        int part = 0;
         for (int i = 0; i < steps; ++i) {
-            const int at = mine.first + i, sx = i % Sh::SX;
+            const int sw = i % Sh::SW, row = rows * 128 + r;
             float s[GS];
 #pragma unroll
-            for (int g = 0; g < GS; ++g) s[g] = next[g];
-            scales(at + 1, next);
-            if (!wait(&xfull[sx], (i / Sh::SX) & 1)) break;
-            const float* un = reinterpret_cast<const float*>(sm + Sh::U + sx * Sh::Units) + c0;
+            for (int g = 0; g < GS; ++g) {
+                s[g] = BF16 ? __uint_as_float(next[0][g] << 16) : __uint_as_float(next[0][g]);
+                next[0][g] = next[1][g];
+            }
+            advance();
+            scales(next[1]);
+            if (++at == blocks) { at = 0; ++rows; }
+            if (!wait(&wfull[sw], (i / Sh::SW) & 1)) break;
+            const float* un = reinterpret_cast<const float*>(sm + Sh::U + sw * Sh::Units) + c0;
             bool ok = true;
 #pragma unroll
             for (int g = 0; g < GS; ++g) {
@@ -533,32 +551,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
                 ok = ok && wait(&dfull[b], (u / DB) & 1);
                 if (!ok) break;
                 tc_fence_after();
+                uint32_t d[C];
 #pragma unroll
                 for (int q = 0; q < C / RC; ++q) {
-                    uint32_t hi[RC], lo[RC];
-                    tmem_ld8(trow + b * 2 * NT + q * RC, hi);
-                    tmem_ld8(trow + b * 2 * NT + NT + q * RC, lo);
-                    tmem_wait_ld();
+                    if constexpr (RC == 16) tmem_ld16(trow + b * NT + q * RC, *reinterpret_cast<uint32_t(*)[16]>(d + q * RC));
+                    else tmem_ld8(trow + b * NT + q * RC, *reinterpret_cast<uint32_t(*)[8]>(d + q * RC));
+                }
+                tmem_wait_ld();
 #pragma unroll
-                    for (int x = 0; x < RC / 2; ++x) {
-                        const float2 uu = *reinterpret_cast<const float2*>(un + q * RC + 2 * x);
-                        acc[q * RC / 2 + x] = fma2(add2(pack2(__uint_as_float(hi[2 * x]), __uint_as_float(hi[2 * x + 1])),
-                                                        pack2(__uint_as_float(lo[2 * x]), __uint_as_float(lo[2 * x + 1]))),
-                                                   mul2(pack2(uu.x, uu.y), pack2(s[g], s[g])), acc[q * RC / 2 + x]);
-                    }
+                for (int x = 0; x < C / 2; x += 2) {
+                    const float4 uu = *reinterpret_cast<const float4*>(un + 2 * x);
+                    acc[x] = fma2(pack2(__uint_as_float(d[2 * x]), __uint_as_float(d[2 * x + 1])), mul2(pack2(uu.x, uu.y), pack2(s[g], s[g])), acc[x]);
+                    acc[x + 1] = fma2(pack2(__uint_as_float(d[2 * x + 2]), __uint_as_float(d[2 * x + 3])), mul2(pack2(uu.z, uu.w), pack2(s[g], s[g])),
+                                      acc[x + 1]);
                 }
                 tc_fence_before();
                 arrive_warp(&dempty[b]);
             }
             if (!ok) break;
-            arrive_warp(&xempty[sx]);
-            if ((at + 1) % blocks != 0 && i + 1 < steps) continue;
+            arrive_warp(&wempty[sw]);
+            if (at != 0 && i + 1 < steps) continue;
             // the end of the row tile, or of the share
-            const int tile = at / blocks, row = tile * 128 + r;
-            const bool whole = kfirst % blocks == 0 && (at + 1) % blocks == 0;
-            float* dst = whole ? p.y + row : p.part + ((size_t)blockIdx.x * 2 + (kfirst == mine.first ? 0 : 1)) * NT * 128 + r;
+            const bool whole = begun && at == 0;
+            float* dst = whole ? p.y + row : p.part + ((size_t)blockIdx.x * 2 + part) * NT * 128 + r;
             const long long ld = whole ? p.ldy : 128;
             const float bias = whole && p.bias && row < p.m ? p.bias[row] : 0.0f;
+            begun = true;
+            part = 1;
 #pragma unroll
             for (int x = 0; x < C / 2; ++x) {
                 const float2 y = unpack2(acc[x]);
@@ -568,7 +587,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
                 if (v < p.T) dst[v * ld] = whole && p.bias ? fadd(y.x, bias) : y.x;
                 if (v + 1 < p.T) dst[(v + 1) * ld] = whole && p.bias ? fadd(y.y, bias) : y.y;
             }
-            kfirst = at + 1;
         }
     }
     tc_fence_before();
@@ -581,7 +599,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
     if (*fail) {
         const float nan = __int_as_float(0x7fffffff);
         for (int i = tid; i < 2 * NT * 128; i += kGemmThreads) p.part[(size_t)blockIdx.x * 2 * NT * 128 + i] = nan;
-        for (int row = mine.first / blocks * 128 + tid; row < min((mine.end + blocks - 1) / blocks * 128, p.m); row += kGemmThreads)
+        for (int row = first / blocks * 128 + tid; row < min((end + blocks - 1) / blocks * 128, p.m); row += kGemmThreads)
             for (int v = 0; v < p.T; ++v) p.y[(size_t)v * p.ldy + row] = nan;
     }
 }
@@ -592,21 +610,13 @@ __global__ void __launch_bounds__(128) group_add_kernel(const __grid_constant__ 
     pdl_launch_dependents();
     pdl_wait();
     const int blocks = (p.n + 127) >> 7, tiles = (p.m + 127) >> 7, tile = blockIdx.x, v = blockIdx.y, row = tile * 128 + threadIdx.x;
-    const int steps = blocks * tiles, first = tile * blocks, last = first + blocks - 1;
-    // the CTA of a step: the share that it lies in
-    auto cta_of = [&](int at) {
-        int c = (int)(((long long)at * ctas) / steps);
-        while (gemm_share(steps, ctas, c).end <= at) ++c;
-        while (gemm_share(steps, ctas, c).first > at) --c;
-        return c;
-    };
-    const int a = cta_of(first), b = cta_of(last);
+    const int steps = blocks * tiles, first = tile * blocks;
+    const int a = gemm_cta(steps, ctas, first), b = gemm_cta(steps, ctas, first + blocks - 1);
     if (a == b || row >= p.m) return;
-    float y = 0.0f;
-    for (int c = a; c <= b; ++c) {
-        const int part = gemm_share(steps, ctas, c).first >= first ? 0 : 1;
-        y += p.part[(((size_t)c * 2 + part) * NT + v) * 128 + threadIdx.x];
-    }
+    // only the first of the tile's CTAs can have begun before the tile: its part is its second then
+    float y = p.part[(((size_t)a * 2 + (gemm_first(steps, ctas, a) < first)) * NT + v) * 128 + threadIdx.x];
+#pragma unroll 4
+    for (int c = a + 1; c <= b; ++c) y += p.part[((size_t)c * 2 * NT + v) * 128 + threadIdx.x];
     p.y[(size_t)v * p.ldy + row] = p.bias ? fadd(y, p.bias[row]) : y;
 }
 

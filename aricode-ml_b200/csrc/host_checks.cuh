@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -49,10 +50,29 @@ inline bool overlap(const Span& a, const Span& b, int64_t n) {
 
 inline bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld; }
 
+// the current device's SMs, looked up once a device
 inline int sm_count() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (cudaGetDevice(&dev) != cudaSuccess) return n;
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
+}
+
+// dynamic shared memory of up to `bytes` for kernel k on the current device, asked for where no
+// call there has asked for as much (the question costs as much as a quarter of a launch)
+template <auto k>
+inline cudaError_t allow_smem(int bytes) {
+    static std::atomic<int> allowed[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace b2

@@ -62,7 +62,7 @@ size_t tree_bytes(const TreeAttnParams& p) {
 template <int DP, int NC>
 cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
     auto k = tree_attn_kernel<DP, NC>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeShape<DP, NC>::Alloc);
+    cudaError_t e = allow_smem<tree_attn_kernel<DP, NC>>(TreeShape<DP, NC>::Alloc);
     if (e != cudaSuccess) return e;
     e = launch_ex(k, dim3((unsigned)std::min<long long>(tree_items(p, NC), sm_count())), dim3(kTreeThreads), TreeShape<DP, NC>::Alloc, s, true, p);
     if (e != cudaSuccess || p.nsplit == 1) return e;
