@@ -569,16 +569,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             return ok;
         };
         constexpr int RC = QC < 8 ? QC : 8;                    // columns read at a time
-        auto read_cols = [&](uint32_t at, uint32_t (&r)[RC]) {
-            if constexpr (RC == 8) tmem_ld8(at, r);
-            else tmem_ld4(at, r);
-        };
         // hi and lo sums of RC columns, together
         auto read_sums = [&](uint32_t at, f32x2* y) {
             uint32_t c[RC], z[RC];
-            read_cols(at, c);
-            read_cols(at + NC, z);
-            tmem_wait_ld();
+            tmem_read2(at, at + NC, c, z);
 #pragma unroll
             for (int x = 0; x < RC / 2; ++x)
                 y[x] = add2(pack2(__uint_as_float(c[2 * x]), __uint_as_float(c[2 * x + 1])),
