@@ -64,7 +64,7 @@ cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
     auto k = tree_attn_kernel<DP, NC>;
     cudaError_t e = allow_smem<tree_attn_kernel<DP, NC>>(TreeShape<DP, NC>::Alloc);
     if (e != cudaSuccess) return e;
-    e = launch_ex(k, dim3((unsigned)std::min<long long>(tree_items(p, NC), sm_count())), dim3(kTreeThreads), TreeShape<DP, NC>::Alloc, s, true, p);
+    e = launch_ex(k, dim3((unsigned)std::min<long long>(tree_items(p, NC), sm_count())), dim3(TreeShape<DP, NC>::Threads), TreeShape<DP, NC>::Alloc, s, true, p);
     if (e != cudaSuccess || p.nsplit == 1) return e;
     if (p.nsplit <= 8) return launch_ex(tree_join_kernel<1>, dim3((unsigned)p.r.n_rows, (unsigned)((p.H + 7) / 8)), dim3(256), 0, s, true, p);
     return launch_ex(tree_join_kernel<8>, dim3((unsigned)p.r.n_rows, (unsigned)p.H), dim3(256), 0, s, true, p);

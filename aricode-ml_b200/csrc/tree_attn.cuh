@@ -53,9 +53,6 @@ __device__ __forceinline__ int tree_splits(int kc_log2, int keys) { return max((
 // A CTA a SM goes through its items with the pipeline running on from one to the next. Every
 // wait is bounded; a warp whose wait ran out leaves its loop and sets the error word.
 constexpr int kTreeSoftWarps = 16;
-constexpr int kTreeConvWarps = 4;
-constexpr int kTreeThreads = (kTreeSoftWarps + kTreeConvWarps + 2) * 32;     // 80 registers a thread
-constexpr int kTreeTeam = kTreeConvWarps / 2 * 32;     // threads for the keys, and for the values
 constexpr int kTreeRing = 8;
 constexpr int kTreeKeys = 128;
 
@@ -83,6 +80,9 @@ struct TreeShape {
     static constexpr int Halves = DP / 64;                         // 128-byte parts of a row
     static constexpr int MH = DP == 256 ? 2 : 1;                   // 128 elements each of the output
     static constexpr int QC = NC / 4;                              // columns of a thread
+    static constexpr int Conv = NC == 16 ? 8 : 4;                  // warps that make operands
+    static constexpr int Threads = (kTreeSoftWarps + Conv + 2) * 32;            // 72 or 80 registers a thread
+    static constexpr int Team = Conv / 2 * 32;                     // threads for the keys, and for the values
     static constexpr int Tile = Halves * kTreeKeys * 128;          // [part][key][64 f16], swizzled
     static constexpr int QPart = Halves * 2 * NC * 128;            // [part][column: hi, lo][64 f16], swizzled
     static constexpr int PPart = kTreeKeys * 128;                  // [key][64 columns: hi, lo], swizzled
@@ -173,7 +173,7 @@ __device__ __forceinline__ float put_row_f16(float4 (&x)[DP / 64], int l16, At h
 }
 
 template <int DP, int NC>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
+__global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     using Sh = TreeShape<DP, NC>;
     constexpr int KK = Sh::KK, KV = Sh::KV, PB = Sh::PB, ST = Sh::ST, NB = Sh::NB, QC = Sh::QC, MH = Sh::MH;
     extern __shared__ unsigned char ta_raw[];
@@ -201,15 +201,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int dh = p.c.dh;
-    constexpr int kMmaWarp = kTreeSoftWarps + kTreeConvWarps, kPlanWarp = kMmaWarp + 1;
+    constexpr int kMmaWarp = kTreeSoftWarps + Sh::Conv, kPlanWarp = kMmaWarp + 1;
 
     after_previous();
     if (tid == 0) {
-        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + kTreeConvWarps + 1); }
-        for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], kTreeConvWarps / 2); }
-        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], kTreeTeam); mbar_init(&kempty[i], 1); }
-        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], kTreeTeam); mbar_init(&vempty[i], 1); }
-        mbar_init(qfull, kTreeTeam); mbar_init(qfree, 1);
+        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + Sh::Conv + 1); }
+        for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], Sh::Conv / 2); }
+        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], Sh::Team); mbar_init(&kempty[i], 1); }
+        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], Sh::Team); mbar_init(&vempty[i], 1); }
+        mbar_init(qfull, Sh::Team); mbar_init(qfree, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sfull[i], 2); mbar_init(&sfree[i], kTreeSoftWarps);
             mbar_init(&ofull[i], 1); mbar_init(&ofree[i], kTreeSoftWarps);
@@ -434,9 +434,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     } else if (warp >= kTreeSoftWarps) {
         // ---- operands: a team for the keys, one for the values
         constexpr int Chunks = DP / 16;                        // 16 codes each of a row
-        constexpr int Units = kTreeKeys * Chunks / kTreeTeam, KeyStep = kTreeTeam / Chunks;
-        const bool keys = warp < kTreeSoftWarps + kTreeConvWarps / 2;
-        const int ct = (tid - kTreeSoftWarps * 32) % kTreeTeam, chunk = ct % Chunks, key0 = ct / Chunks;
+        constexpr int Units = kTreeKeys * Chunks / Sh::Team, Wide = Units < 8 ? Units : 8, KeyStep = Sh::Team / Chunks;
+        const bool keys = warp < kTreeSoftWarps + Sh::Conv / 2;
+        const int ct = (tid - kTreeSoftWarps * 32) % Sh::Team, chunk = ct % Chunks, key0 = ct / Chunks;
         const float* rows = keys ? p.k : p.v;
         const long long ldr = keys ? p.ldk : p.ldv;
         unsigned char* tiles = sm + (keys ? Sh::K : Sh::V);
@@ -448,12 +448,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             const int u0 = 2 * (chunk & 3), turn = (chunk >> 2) & 1;      // (parts in turn: no bank conflicts)
             const bool in = 16 * chunk < dh;
 #pragma unroll 1
-            for (int x0 = 0; x0 < Units; x0 += 8) {
-                uint4 r[8];
+            for (int x0 = 0; x0 < Units; x0 += Wide) {
+                uint4 r[Wide];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) r[x] = in ? lds128(codes + (key0 + (x0 + x) * KeyStep) * dh + 16 * chunk) : make_uint4(0u, 0u, 0u, 0u);
+                for (int x = 0; x < Wide; ++x) r[x] = in ? lds128(codes + (key0 + (x0 + x) * KeyStep) * dh + 16 * chunk) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 0; x < Wide; ++x) {
                     const int key = key0 + (x0 + x) * KeyStep;
                     const uint4 lo = codes_f16(r[x].x, r[x].y), hi = codes_f16(r[x].z, r[x].w);
                     unsigned char* row = part + key * 128;
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
                 }
             }
         };
-        constexpr int Lines = kTreeTeam / 16, Batch = 8 / (DP / 64);   // rows at a time, and of a lane group in flight
+        constexpr int Lines = Sh::Team / 16, Batch = 8 / (DP / 64);   // rows at a time, and of a lane group in flight
         // drafted rows: key j and 64 + j of the tile, all loads of a batch first. (What lies past the
         // last one is some other tile's: its scores are masked, its values are finite.)
         auto put_drafted = [&](unsigned char* tile, const TreeTile& d, float* scale) {
@@ -512,13 +512,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             }
         };
         if (!keys) {                                           // what nothing has written yet are zeros
-            for (int i = ct; i < KV * Sh::Tile / 16; i += kTreeTeam) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
-            for (int i = ct; i < Sh::QPart / 16; i += kTreeTeam) reinterpret_cast<uint4*>(sm + Sh::Q)[i] = make_uint4(0u, 0u, 0u, 0u);
-            for (int i = ct; i < kTreeRing * NC; i += kTreeTeam) {
+            for (int i = ct; i < KV * Sh::Tile / 16; i += Sh::Team) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = ct; i < Sh::QPart / 16; i += Sh::Team) reinterpret_cast<uint4*>(sm + Sh::Q)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = ct; i < kTreeRing * NC; i += Sh::Team) {
                 reinterpret_cast<float*>(sm + Sh::Unit)[i] = 0.0f;
                 reinterpret_cast<long long*>(sm + Sh::Seen)[i] = 0;
             }
-            asm volatile("bar.sync 1, 64;" ::: "memory");      // (nobody has waited for anything yet)
+            asm volatile("bar.sync 1, %0;" ::"n"(Sh::Team) : "memory");      // (nobody has waited for anything yet)
         }
         bool ok = true;
         for (int t = 0, come = keys ? 0 : 1; ok; ++t) {
