@@ -40,14 +40,24 @@ int tree_columns(const TreeAttnParams& p, int max_rows) {
     return rows * p.G <= 16 ? 16 : p.c.dh > 128 ? 32 : 64;
 }
 
-// Keys of a split: enough items for eight rounds of the GPU, of 256 keys at least. The host does not know the
-// lengths; the sizes that it knows bound the partial results.
+// Keys of a split: so many items that the last round of the GPU is nearly full, in four to eight rounds (lengths
+// differ, and the host does not know them), of 256 keys at least; an item beside its keys costs about two tiles of them.
+// (Powers of two, eight rounds: 40 K keys, two sequences of 64 rows of 32 / 4 heads of 64 in 640 items 429 us.)
 void tree_plan(TreeAttnParams& p, int nc) {
     const long long tiles = std::max((long long)p.r.n_rows * p.G / nc, (long long)std::min(p.r.n_seq, p.r.n_rows)) * p.c.KVH;
-    const long long want = std::max(1ll, std::min({8ll * 148 / std::max(tiles, 1ll), (p.r.cap + 255ll) / 256, 1024ll}));
-    p.kc_log2 = 8;
-    while (p.kc_log2 < 30 && (want << p.kc_log2) < p.r.cap) ++p.kc_log2;
-    p.nsplit = std::max(1, (int)((p.r.cap + (1ll << p.kc_log2) - 1) >> p.kc_log2));
+    const long long most = std::max(1ll, std::min((p.r.cap + 255ll) / 256, 1024ll)), keys = (p.r.cap + kTreeKeys - 1ll) / kTreeKeys;
+    long long best = 0;
+    p.kc = kTreeKeys;
+    for (int rounds = 4; rounds <= 8; ++rounds) {
+        const long long n = std::max(1ll, std::min(148ll * rounds / std::max(tiles, 1ll), most));
+        const long long len = std::max(1ll, (keys + n - 1) / n), splits = (keys + len - 1) / len;
+        const long long cost = (tiles * splits + 147) / 148 * (len + 2);
+        if (best == 0 || cost < best) {
+            best = cost;
+            p.kc = (int)std::min(len * kTreeKeys, 1ll << 30);
+        }
+    }
+    p.nsplit = std::max(1, (p.r.cap - 1) / p.kc + 1);
 }
 
 // items that the call can have at most

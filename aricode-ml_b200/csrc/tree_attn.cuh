@@ -16,6 +16,8 @@
 // above it: then its largest is found across the lanes; a tile that moves nothing needs no
 // more than the warps' word that it does not.
 #pragma once
+#include <type_traits>
+
 #include "f16_pairs.cuh"
 #include "paged_rows.cuh"
 #include "umma.cuh"
@@ -34,13 +36,13 @@ struct TreeAttnParams {
     float* out;              // [n_rows][ldo]
     long long ldq, ldk, ldv, ldo;
     int H, G;                // G = H / KVH
-    int kc_log2, nsplit;     // a split: 2^kc_log2 cached keys, of which the last also has the
+    int kc, nsplit;          // a split: kc cached keys (a multiple of 128), of which the last also has the
                              // drafted ones; nsplit: splits of cap keys
     float* part;             // [n_rows][H][nsplit][dh + 4]: o, m (base 2), l
     int* err;
 };
 
-__device__ __forceinline__ int tree_splits(int kc_log2, int keys) { return max((keys + (1 << kc_log2) - 1) >> kc_log2, 1); }
+__device__ __forceinline__ int tree_splits(int kc, int keys) { return max((keys - 1) / kc + 1, 1); }
 
 // Warps 0 .. 15, softmax: warp w reads TMEM lanes 32 (w % 4) .. + 31 and columns w / 4 of the
 //   four parts of a tile's columns.
@@ -80,6 +82,12 @@ struct TreeShape {
     static constexpr int Halves = DP / 64;                         // 128-byte parts of a row
     static constexpr int MH = DP == 256 ? 2 : 1;                   // 128 elements each of the output
     static constexpr int QC = NC / 4;                              // columns of a thread
+    // With 64 columns hi and lo go into the same sums, lo first: the MMAs take 96 clocks instead of 64 for
+    // each 16 elements or keys, and the warps that read the sums have half as many to read.
+    static constexpr bool Same = DP == 64 && NC == 64;
+    static constexpr int Sums = Same ? NC : 2 * NC;                // TMEM columns of a product
+    // d_head up to 64: lanes 64 .. 127 of the output are the others again, so each has half of the columns
+    static constexpr int OC = Same ? QC / 2 : QC;      // columns of a thread's output
     static constexpr int Conv = NC == 16 ? 8 : 4;                  // warps that make operands
     static constexpr int Threads = (kTreeSoftWarps + Conv + 2) * 32;            // 72 or 80 registers a thread
     static constexpr int Team = Conv / 2 * 32;                     // threads for the keys, and for the values
@@ -100,15 +108,15 @@ struct TreeShape {
     static constexpr int Moves = Dvs + kTreeRing * 64 * 4;         // [2][4 parts] 1 + the last tile that moves h
     static constexpr int Xm = Moves + 8 * 4;                       // [2][4 parts][4][QC] largest scores
     static constexpr int Xl = Xm + 2 * 16 * QC * 4;                // [4][4][QC] sums
-    static constexpr int Bs = Xl + 16 * QC * 4;                    // [16 warps][QC] h
+    static constexpr int Bs = Xl + 16 * QC * 4;                    // [16 warps][QC] -h
     static constexpr int Bd = Bs + 16 * QC * 4;                    // [16][QC] how far it moves; at the end 1 / sum
     static constexpr int Bk = Bd + 16 * QC * 4;                    // [2][16][QC] the factor of what was before
     static constexpr int Bars = Bk + 2 * 16 * QC * 4;
     static constexpr int NBars = 2 * kTreeRing + 2 * NB + 2 * KK + 2 * KV + 2 + 4 + 2 + 4 + 4 + 1 + 1;
     static constexpr int Bytes = Bars + NBars * 8 + 16;
     static constexpr int Alloc = Bytes + 1024;                     // operands start on 1024 bytes
-    static constexpr int TmemS = 0, TmemO = 4 * NC;                // two buffers each
-    static constexpr int TmemUsed = 4 * NC + 4 * MH * NC, TmemCols = TmemUsed <= 128 ? 128 : TmemUsed <= 256 ? 256 : 512;
+    static constexpr int TmemS = 0, TmemO = 2 * Sums;              // two buffers each
+    static constexpr int TmemUsed = 2 * Sums + 2 * MH * Sums, TmemCols = TmemUsed <= 128 ? 128 : TmemUsed <= 256 ? 256 : 512;
     static_assert(TmemUsed <= 512 && Alloc <= 227 * 1024, "");
 };
 
@@ -175,7 +183,8 @@ __device__ __forceinline__ float put_row_f16(float4 (&x)[DP / 64], int l16, At h
 template <int DP, int NC>
 __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     using Sh = TreeShape<DP, NC>;
-    constexpr int KK = Sh::KK, KV = Sh::KV, PB = Sh::PB, ST = Sh::ST, NB = Sh::NB, QC = Sh::QC, MH = Sh::MH;
+    constexpr int KK = Sh::KK, KV = Sh::KV, PB = Sh::PB, ST = Sh::ST, NB = Sh::NB, QC = Sh::QC, OC = Sh::OC, MH = Sh::MH, Sums = Sh::Sums;
+    constexpr bool Same = Sh::Same;
     extern __shared__ unsigned char ta_raw[];
     unsigned char* sm = ta_raw + ((1024u - (smem_u32(ta_raw) & 1023u)) & 1023u);
     TreeTile* ring = reinterpret_cast<TreeTile*>(sm + Sh::Ring);
@@ -269,7 +278,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                     if (q.len > kTreeRows) set_err(p.err, B2_DEV_ERR_TOO_MANY);
                     else if (q.len > 0) {
                         if (q.kv > p.r.cap) set_err(p.err, B2_DEV_ERR_KV_OVERFLOW);
-                        cnt = (unsigned)(((q.len * p.G + NC - 1) / NC) * p.c.KVH * tree_splits(p.kc_log2, min(q.kv, p.r.cap)));
+                        cnt = (unsigned)(((q.len * p.G + NC - 1) / NC) * p.c.KVH * tree_splits(p.kc, min(q.kv, p.r.cap)));
                     }
                 }
                 unsigned incl = cnt;
@@ -300,16 +309,16 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 break;
             }
             // column tiles first: CTAs that run at once read the same keys
-            const int ctiles = (len * p.G + NC - 1) / NC, nsplit = tree_splits(p.kc_log2, kv);
+            const int ctiles = (len * p.G + NC - 1) / NC, nsplit = tree_splits(p.kc, kv);
             const int ct = (int)(idx % (unsigned)ctiles), rest = (int)(idx / (unsigned)ctiles), kvh = rest % p.c.KVH, split = rest / p.c.KVH;
-            const int j0 = split << p.kc_log2, jend = min(kv, j0 + (1 << p.kc_log2));
+            const int j0 = split * p.kc, jend = kv - j0 < p.kc ? kv : j0 + p.kc;
             const int ntiles = (max(jend - j0, 0) + kTreeKeys - 1) / kTreeKeys, all = ntiles + (split == nsplit - 1);
             for (int i0 = 0; i0 < all && ok; i0 += 4) {
-                const int i = i0 + group, j = j0 + i * kTreeKeys + 16 * b, cnt = min(all - i0, 4);
+                const int i = i0 + group, in = i * kTreeKeys + 16 * b, cnt = min(all - i0, 4);
                 int cell = -1;
                 float ks = -1.0f, vs = 0.0f;
-                if (i < ntiles && j < jend) {
-                    const int page = page_of(p.c, p.r, s, j);
+                if (i < ntiles && in < jend - j0) {
+                    const int j = j0 + in, page = page_of(p.c, p.r, s, j);
                     if (page < 0) set_err(p.err, B2_DEV_ERR_BAD_PAGE);
                     else {
                         cell = (page * p.c.KVH + kvh) * (psz >> 4) + ((j & (psz - 1)) >> 4);
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                     d.cell[b] = cell; d.ks[b] = ks; d.vs[b] = vs;
                     if (b == 0) {
                         d.flags = (i == 0 ? TREE_FIRST : 0) | (i == all - 1 ? TREE_LAST : 0) | (i == ntiles ? TREE_DRAFT : 0);
-                        d.item = n; d.limit = jend - (j0 + i * kTreeKeys);
+                        d.item = n; d.limit = jend - j0 - i * kTreeKeys;
                         d.a = a; d.len = len; d.kvh = kvh; d.col0 = ct * NC; d.cols = min(len * p.G - ct * NC, NC);
                         d.split = split; d.nsplit = nsplit;
                     }
@@ -360,11 +369,11 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
         // ---- MMAs
         const bool me = elect_lane();
         const uint32_t base = smem_u32(sm);
-        constexpr uint32_t ids = umma_idesc_f16(2 * NC, false, false), ido = umma_idesc_f16(2 * NC, true, true);
+        constexpr uint32_t ids = umma_idesc_f16(Sums, false, false), ido = umma_idesc_f16(Sums, true, true);
         const uint64_t kdesc = umma_desc_sw128(base + Sh::K), qdesc = umma_desc_sw128(base + Sh::Q);
         // (d_head 64: lanes 64 .. 127 of the output repeat the others)
         const uint64_t vdesc = umma_desc_sw128_mn(base + Sh::V, Sh::Halves > 1 ? kTreeKeys * 128 : 0);
-        const uint64_t pdesc = umma_desc_sw128_mn(base + Sh::P, Sh::PParts > 1 ? Sh::PPart : 0);
+        const uint64_t pdesc = umma_desc_sw128_mn(base + Sh::P, !Same && Sh::PParts > 1 ? Sh::PPart : 0);
         bool ok = true;
         int items = 0;
         auto scores = [&](int t, int flags) {
@@ -375,11 +384,16 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             if (!ok) return;
             tc_fence_after();
             const uint64_t kd = kdesc + (uint64_t)(slot * (Sh::Tile >> 4));
-            const uint32_t to = tmem + Sh::TmemS + (t & 1) * 2 * NC;
-            umma_f16<false>(me, to, kd, qdesc, ids);
+            const uint32_t to = tmem + Sh::TmemS + (t & 1) * Sums;
 #pragma unroll
-            for (int i = 1; i < 4 * Sh::Halves; ++i)
-                umma_f16<true>(me, to, kd + ((i >> 2) * (kTreeKeys * 128) + 32 * (i & 3)) / 16, qdesc + ((i >> 2) * (2 * NC * 128) + 32 * (i & 3)) / 16, ids);
+            for (int lo = Same; lo >= 0; --lo)
+#pragma unroll
+                for (int i = 0; i < 4 * Sh::Halves; ++i) {
+                    const uint64_t a = kd + ((i >> 2) * (kTreeKeys * 128) + 32 * (i & 3)) / 16;
+                    const uint64_t b = qdesc + ((i >> 2) * (2 * NC * 128) + lo * NC * 128 + 32 * (i & 3)) / 16;
+                    if (lo == Same && i == 0) umma_f16<false>(me, to, a, b, ids);
+                    else umma_f16<true>(me, to, a, b, ids);
+                }
             if (me) {
                 umma_commit(&kempty[slot]);
                 if (flags & TREE_LAST) umma_commit(qfree);
@@ -400,10 +414,15 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
 #pragma unroll
             for (int mh = 0; mh < MH; ++mh) {
                 const uint64_t vd = vdesc + (uint64_t)(slot * (Sh::Tile >> 4) + mh * (2 * kTreeKeys * 128 >> 4));
-                const uint32_t to = tmem + Sh::TmemO + ((t & 1) * MH + mh) * 2 * NC;
-                umma_f16<false>(me, to, vd, pd, ido);
+                const uint32_t to = tmem + Sh::TmemO + ((t & 1) * MH + mh) * Sums;
 #pragma unroll
-                for (int k = 1; k < kTreeKeys / 16; ++k) umma_f16<true>(me, to, vd + k * (2048 / 16), pd + k * (2048 / 16), ido);
+                for (int lo = Same; lo >= 0; --lo)
+#pragma unroll
+                    for (int k = 0; k < kTreeKeys / 16; ++k) {
+                        const uint64_t b = pd + (lo * Sh::PPart + k * 2048) / 16;
+                        if (lo == Same && k == 0) umma_f16<false>(me, to, vd, b, ido);
+                        else umma_f16<true>(me, to, vd + k * (2048 / 16), b, ido);
+                    }
             }
             if (me) {
                 umma_commit(&vempty[slot]);
@@ -568,20 +587,27 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             ok = wait_warp(&part_bar[part], met++ & 1, 20);
             return ok;
         };
-        constexpr int RC = QC < 8 ? QC : 8;                    // columns read at a time
-        // hi and lo sums of RC columns, together
-        auto read_sums = [&](uint32_t at, f32x2* y) {
-            uint32_t c[RC], z[RC];
-            tmem_read2(at, at + NC, c, z);
+        // the sums of n columns
+        auto read_sums = [&](uint32_t at, f32x2* y, auto n) {
+            constexpr int N = decltype(n)::value, M = Same ? N / 2 : N < 8 ? N : 8;
 #pragma unroll
-            for (int x = 0; x < RC / 2; ++x)
-                y[x] = add2(pack2(__uint_as_float(c[2 * x]), __uint_as_float(c[2 * x + 1])),
-                            pack2(__uint_as_float(z[2 * x]), __uint_as_float(z[2 * x + 1])));
+            for (int i = 0; i < (Same ? 1 : N / M); ++i) {
+                uint32_t c[M], z[M];
+                tmem_read2(at + i * M, at + (Same ? M : NC + i * M), c, z);
+#pragma unroll
+                for (int x = 0; x < M / 2; ++x) {
+                    const f32x2 a = pack2(__uint_as_float(c[2 * x]), __uint_as_float(c[2 * x + 1]));
+                    const f32x2 b = pack2(__uint_as_float(z[2 * x]), __uint_as_float(z[2 * x + 1]));
+                    if constexpr (Same) { y[x] = a; y[M / 2 + x] = b; }
+                    else y[i * M / 2 + x] = add2(a, b);
+                }
+            }
         };
+        const int oc0 = OC < QC ? (quarter >> 1) * OC : 0, oelem = OC < QC ? key & 63 : key;      // of the thread's output
         int* moves = reinterpret_cast<int*>(sm + Sh::Moves) + part;
         float h = 0.0f;                                        // of column `lane`,
         bool unset = true;                                     // which has seen no key yet
-        f32x2 l[QC / 2], o[MH][QC / 2];
+        f32x2 l[QC / 2], o[MH][OC / 2];
         // Output sums are folded two tiles later, when their products are surely made; with one buffer of
         // weights one tile later, before they are written.
         // output sums of tile t; u: what a unit of them is, moved: whether that tile moved h
@@ -593,21 +619,24 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             for (int mh = 0; mh < MH; ++mh) {
                 if (moved) {
 #pragma unroll
-                    for (int x = 0; x < QC / 2; ++x) {
-                        const float2 bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + 2 * x);
+                    for (int x = 0; x < OC / 2; ++x) {
+                        const float2 bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + oc0 + 2 * x);
                         o[mh][x] = mul2(o[mh][x], pack2(bb.x, bb.y));
                     }
                 }
+                f32x2 y[OC / 2];
+                read_sums(trow + Sh::TmemO + ((t & 1) * MH + mh) * Sums + oc0, y, std::integral_constant<int, OC>{});
 #pragma unroll
-                for (int q = 0; q < QC / RC; ++q) {
-                    f32x2 y[RC / 2];
-                    read_sums(trow + Sh::TmemO + ((t & 1) * MH + mh) * 2 * NC + q * RC, y);
-#pragma unroll
-                    for (int x = 0; x < RC / 2; ++x) o[mh][q * RC / 2 + x] = fma2(y[x], pack2(u, u), o[mh][q * RC / 2 + x]);
-                }
+                for (int x = 0; x < OC / 2; ++x) o[mh][x] = fma2(y[x], pack2(u, u), o[mh][x]);
             }
             tc_fence_before();
             arrive_warp(&ofree[t & 1]);
+        };
+        // where a column's output goes: its row of `out`, or its partial result
+        auto column_out = [&](const TreeTile& d, int col) {
+            const int cc = d.col0 + col, tok = cc / p.G, row = d.a + tok, head = d.kvh * p.G + cc - tok * p.G;
+            return d.nsplit > 1 ? p.part + (((size_t)row * p.H + head) * p.nsplit + d.split) * (dh + 4)
+                                : p.out + (size_t)row * p.ldo + (size_t)head * dh;
         };
         float u1 = 0.0f, u2 = 0.0f;                            // of the two tiles whose output is pending
         bool moved1 = false, moved2 = false;
@@ -623,11 +652,11 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 h = 0.0f;
                 unset = lane < QC && part * QC + lane < d.cols;
 #pragma unroll
-                for (int x = 0; x < QC / 2; ++x) {
-                    l[x] = 0ull;
+                for (int x = 0; x < QC / 2; ++x) l[x] = 0ull;
 #pragma unroll
-                    for (int mh = 0; mh < MH; ++mh) o[mh][x] = 0ull;
-                }
+                for (int mh = 0; mh < MH; ++mh)
+#pragma unroll
+                    for (int x = 0; x < OC / 2; ++x) o[mh][x] = 0ull;
                 if (lane < QC) bs[lane] = 0.0f;
                 __syncwarp();
             }
@@ -636,8 +665,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             if (!wait_warp(&sfull[t & 1], (t >> 1) & 1, 20)) break;
             tc_fence_after();
             f32x2 s[QC / 2];
-#pragma unroll
-            for (int q = 0; q < QC / RC; ++q) read_sums(trow + Sh::TmemS + (t & 1) * 2 * NC + q * RC, s + q * RC / 2);
+            read_sums(trow + Sh::TmemS + (t & 1) * Sums, s, std::integral_constant<int, QC>{});
             tc_fence_before();
             arrive_warp(&sfree[t & 1]);
             // this key's scales, and the largest value scale of the tile
@@ -681,7 +709,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
 #pragma unroll
             for (int x = 0; x < QC / 2; ++x) {
                 const float2 un = *reinterpret_cast<const float2*>(unit + 2 * x), hh = *reinterpret_cast<const float2*>(bs + 2 * x);
-                s[x] = fma2(s[x], mul2(pack2(un.x, un.y), pack2(ks, ks)), pack2(-hh.x, -hh.y));
+                s[x] = fma2(s[x], mul2(pack2(un.x, un.y), pack2(ks, ks)), pack2(hh.x, hh.y));
             }
             if (draft) {
                 const long long* seen = reinterpret_cast<const long long*>(sm + Sh::Seen) + it * NC + part * QC;
@@ -720,7 +748,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                     for (int q = 0; q < 4; ++q) best = fmaxf(best, xm[(t & 1) * 16 * QC + q * QC + lane]);
                     by = unset ? (best > -INFINITY ? best : 0.0f) : fmaxf(best, 0.0f);
                     h += by;
-                    bs[lane] = h;
+                    bs[lane] = -h;
                     bk[(t & 1) * 16 * QC + lane] = unset ? 0.0f : exp2_fast(-by);
                     bd[lane] = by;
                     unset = unset && !(best > -INFINITY);
@@ -806,25 +834,27 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                     bd[lane] = d.nsplit > 1 ? 1.0f : sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
                 }
                 __syncwarp();
-                for (int c = 0; c < QC; ++c) {
-                    const int col = part * QC + c;
-                    if (col >= d.cols) break;
-                    const int cc = d.col0 + col, tok = cc / p.G, row = d.a + tok, head = d.kvh * p.G + cc - tok * p.G;
-                    float* dst = d.nsplit > 1 ? p.part + (((size_t)row * p.H + head) * p.nsplit + d.split) * (dh + 4)
-                                              : p.out + (size_t)row * p.ldo + (size_t)head * dh;
-                    const float inv = bd[c];
+                const int mine_col = part * QC + (lane & (QC - 1));
+                float* mine_at = column_out(d, min(mine_col, d.cols - 1));
+                for (int c = 0; c < OC; ++c) {
+                    if (part * QC + oc0 + c >= d.cols) break;
+                    float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), oc0 + c));
+                    const float inv = bd[oc0 + c];
 #pragma unroll
                     for (int mh = 0; mh < MH; ++mh) {
                         float y = 0.0f;                        // (registers are not indexed)
 #pragma unroll
-                        for (int x = 0; x < QC / 2; ++x) {
+                        for (int x = 0; x < OC / 2; ++x) {
                             const float2 z = unpack2(o[mh][x]);
                             if (c == 2 * x) y = z.x;
                             if (c == 2 * x + 1) y = z.y;
                         }
-                        if (key + 128 * mh < dh) dst[key + 128 * mh] = y * inv;
+                        if (oelem + 128 * mh < dh) dst[oelem + 128 * mh] = y * inv;
                     }
-                    if (d.nsplit > 1 && quarter == 0 && lane == c) { dst[dh] = unset ? -INFINITY : h; dst[dh + 1] = sum; }
+                }
+                if (d.nsplit > 1 && quarter == 0 && lane < QC && mine_col < d.cols) {
+                    mine_at[dh] = unset ? -INFINITY : h;
+                    mine_at[dh + 1] = sum;
                 }
             }
             arrive_warp(&tfree[t & (kTreeRing - 1)]);
@@ -854,7 +884,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
         const unsigned m = __ballot_sync(0xffffffffu, row >= q.a && row < q.a + q.len);
         if (m) {
             const int src = __ffs(m) - 1, kv = __shfl_sync(0xffffffffu, q.kv, src), len = __shfl_sync(0xffffffffu, q.len, src);
-            n = len > kTreeRows ? 1 : tree_splits(p.kc_log2, min(kv, p.r.cap));
+            n = len > kTreeRows ? 1 : tree_splits(p.kc, min(kv, p.r.cap));
         }
     }
     if (n < 2) return;
