@@ -46,10 +46,10 @@ __device__ __forceinline__ int tree_splits(int kc, int keys) { return max((keys 
 
 // Warps 0 .. 15, softmax: warp w reads TMEM lanes 32 (w % 4) .. + 31 and columns w / 4 of the
 //   four parts of a tile's columns.
-// Warps 16, 17: keys' codes in shared memory to f16 operands; 18, 19: values' codes, and an item's
+// Then the keys' warps: codes in shared memory to f16 operands; then the values', and an item's
 //   queries. Drafted rows likewise. (Codes that waited in registers of these warps took 80
 //   registers' worth of spills, and the fence behind the writes waits for loads under way.)
-// Warp 20: issues the MMAs. Warp 21: finds the items (a sequence's columns of a KV head against
+// One warp issues the MMAs. The last finds the items (a sequence's columns of a KV head against
 //   a split of its keys) and their tiles' blocks and scales, up to eight tiles ahead, and asks for
 //   the codes: a bulk copy for each block of 16 keys.
 // A CTA a SM goes through its items with the pipeline running on from one to the next. Every
@@ -88,9 +88,12 @@ struct TreeShape {
     static constexpr int Sums = Same ? NC : 2 * NC;                // TMEM columns of a product
     // d_head up to 64: lanes 64 .. 127 of the output are the others again, so each has half of the columns
     static constexpr int OC = Same ? QC / 2 : QC;      // columns of a thread's output
-    static constexpr int Conv = NC == 16 ? 8 : 4;                  // warps that make operands
-    static constexpr int Threads = (kTreeSoftWarps + Conv + 2) * 32;            // 72 or 80 registers a thread
-    static constexpr int Team = Conv / 2 * 32;                     // threads for the keys, and for the values
+    // Warps that make operands of keys, of values. With 16 columns the softmax needs 72 registers, which leaves
+    // room for four each (two each: 32 sequences of 32 / 32 heads of 128 172 us, now 130). Else two, but four for
+    // values with only one place, which they refill between one tile's product and the next (16 sequences of 32 / 8
+    // heads of 128: 237 us with two, 213 with four; two of 32 / 4 heads of 64, two places: 344 and 368).
+    static constexpr int KeyWarps = NC == 16 ? 4 : 2, ValueWarps = NC == 16 || KV == 1 ? 4 : 2;
+    static constexpr int Threads = (kTreeSoftWarps + KeyWarps + ValueWarps + 2) * 32;
     static constexpr int Tile = Halves * kTreeKeys * 128;          // [part][key][64 f16], swizzled
     static constexpr int QPart = Halves * 2 * NC * 128;            // [part][column: hi, lo][64 f16], swizzled
     static constexpr int PPart = kTreeKeys * 128;                  // [key][64 columns: hi, lo], swizzled
@@ -210,15 +213,15 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int dh = p.c.dh;
-    constexpr int kMmaWarp = kTreeSoftWarps + Sh::Conv, kPlanWarp = kMmaWarp + 1;
+    constexpr int kMmaWarp = kTreeSoftWarps + Sh::KeyWarps + Sh::ValueWarps, kPlanWarp = kMmaWarp + 1;
 
     after_previous();
     if (tid == 0) {
-        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + Sh::Conv + 1); }
-        for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], Sh::Conv / 2); }
-        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], Sh::Team); mbar_init(&kempty[i], 1); }
-        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], Sh::Team); mbar_init(&vempty[i], 1); }
-        mbar_init(qfull, Sh::Team); mbar_init(qfree, 1);
+        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + Sh::KeyWarps + Sh::ValueWarps + 1); }
+        for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], i & 1 ? Sh::ValueWarps : Sh::KeyWarps); }
+        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], 32 * Sh::KeyWarps); mbar_init(&kempty[i], 1); }
+        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], 32 * Sh::ValueWarps); mbar_init(&vempty[i], 1); }
+        mbar_init(qfull, 32 * Sh::ValueWarps); mbar_init(qfree, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sfull[i], 2); mbar_init(&sfree[i], kTreeSoftWarps);
             mbar_init(&ofull[i], 1); mbar_init(&ofree[i], kTreeSoftWarps);
@@ -453,9 +456,10 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
     } else if (warp >= kTreeSoftWarps) {
         // ---- operands: a team for the keys, one for the values
         constexpr int Chunks = DP / 16;                        // 16 codes each of a row
-        constexpr int Units = kTreeKeys * Chunks / Sh::Team, Wide = Units < 8 ? Units : 8, KeyStep = Sh::Team / Chunks;
-        const bool keys = warp < kTreeSoftWarps + Sh::Conv / 2;
-        const int ct = (tid - kTreeSoftWarps * 32) % Sh::Team, chunk = ct % Chunks, key0 = ct / Chunks;
+        constexpr int Wide = kTreeKeys * Chunks / (32 * Sh::ValueWarps) < 8 ? kTreeKeys * Chunks / (32 * Sh::ValueWarps) : 8;
+        const bool keys = warp < kTreeSoftWarps + Sh::KeyWarps;
+        const int team = 32 * (keys ? Sh::KeyWarps : Sh::ValueWarps), step = team / Chunks, lines = team / 16;
+        const int ct = tid - (kTreeSoftWarps + (keys ? 0 : Sh::KeyWarps)) * 32, chunk = ct % Chunks, key0 = ct / Chunks;
         const float* rows = keys ? p.k : p.v;
         const long long ldr = keys ? p.ldk : p.ldv;
         unsigned char* tiles = sm + (keys ? Sh::K : Sh::V);
@@ -467,13 +471,13 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             const int u0 = 2 * (chunk & 3), turn = (chunk >> 2) & 1;      // (parts in turn: no bank conflicts)
             const bool in = 16 * chunk < dh;
 #pragma unroll 1
-            for (int x0 = 0; x0 < Units; x0 += Wide) {
+            for (int at = key0; at < kTreeKeys; at += Wide * step) {
                 uint4 r[Wide];
 #pragma unroll
-                for (int x = 0; x < Wide; ++x) r[x] = in ? lds128(codes + (key0 + (x0 + x) * KeyStep) * dh + 16 * chunk) : make_uint4(0u, 0u, 0u, 0u);
+                for (int x = 0; x < Wide; ++x) r[x] = in ? lds128(codes + (at + x * step) * dh + 16 * chunk) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int x = 0; x < Wide; ++x) {
-                    const int key = key0 + (x0 + x) * KeyStep;
+                    const int key = at + x * step;
                     const uint4 lo = codes_f16(r[x].x, r[x].y), hi = codes_f16(r[x].z, r[x].w);
                     unsigned char* row = part + key * 128;
                     *reinterpret_cast<uint4*>(row + (((u0 + turn) ^ (key & 7)) << 4)) = turn ? hi : lo;
@@ -481,21 +485,21 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 }
             }
         };
-        constexpr int Lines = Sh::Team / 16, Batch = 8 / (DP / 64);   // rows at a time, and of a lane group in flight
+        constexpr int Batch = 8 / (DP / 64);                   // rows of a lane group in flight
         // drafted rows: key j and 64 + j of the tile, all loads of a batch first. (What lies past the
         // last one is some other tile's: its scores are masked, its values are finite.)
         auto put_drafted = [&](unsigned char* tile, const TreeTile& d, float* scale) {
-            for (int r0 = 0; r0 < d.len; r0 += Lines * Batch) {
+            for (int r0 = 0; r0 < d.len; r0 += lines * Batch) {
                 float4 x[Batch][DP / 64];
 #pragma unroll
                 for (int b = 0; b < Batch; ++b) {
-                    const int j = r0 + Lines * b + (ct >> 4);
+                    const int j = r0 + lines * b + (ct >> 4);
                     load_row<DP>(x[b], rows + (size_t)(d.a + min(j, d.len - 1)) * ldr + (size_t)d.kvh * dh, j < d.len, dh, ct & 15);
                 }
 #pragma unroll
                 for (int b = 0; b < Batch; ++b) {
-                    const int j = r0 + Lines * b + (ct >> 4);
-                    if (r0 + Lines * b >= d.len) break;        // (whole warps)
+                    const int j = r0 + lines * b + (ct >> 4);
+                    if (r0 + lines * b >= d.len) break;        // (whole warps)
                     auto at = [&](int row) {
                         return [=](int i, int u) { return tile + i * kTreeKeys * 128 + row * 128 + ((u ^ (row & 7)) << 4); };
                     };
@@ -508,17 +512,17 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             const int it = d.item & (kTreeRing - 1);
             float* unit = reinterpret_cast<float*>(sm + Sh::Unit) + it * NC;
             long long* seen = reinterpret_cast<long long*>(sm + Sh::Seen) + it * NC;
-            for (int c0 = 0; c0 < d.cols; c0 += Lines * Batch) {
+            for (int c0 = 0; c0 < d.cols; c0 += lines * Batch) {
                 float4 x[Batch][DP / 64];
 #pragma unroll
                 for (int b = 0; b < Batch; ++b) {
-                    const int c = c0 + Lines * b + (ct >> 4), cc = d.col0 + min(c, d.cols - 1);
+                    const int c = c0 + lines * b + (ct >> 4), cc = d.col0 + min(c, d.cols - 1);
                     load_row<DP>(x[b], p.q + (size_t)(d.a + cc / p.G) * p.ldq + (size_t)(d.kvh * p.G + cc % p.G) * dh, c < d.cols, dh, ct & 15);
                 }
 #pragma unroll
                 for (int b = 0; b < Batch; ++b) {
-                    const int c = c0 + Lines * b + (ct >> 4);
-                    if (c0 + Lines * b >= d.cols) break;       // (whole warps)
+                    const int c = c0 + lines * b + (ct >> 4);
+                    if (c0 + lines * b >= d.cols) break;       // (whole warps)
                     auto at = [&](int col) {
                         return [=](int i, int u) { return sm + Sh::Q + i * 2 * NC * 128 + col * 128 + ((u ^ (col & 7)) << 4); };
                     };
@@ -531,13 +535,13 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             }
         };
         if (!keys) {                                           // what nothing has written yet are zeros
-            for (int i = ct; i < KV * Sh::Tile / 16; i += Sh::Team) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
-            for (int i = ct; i < Sh::QPart / 16; i += Sh::Team) reinterpret_cast<uint4*>(sm + Sh::Q)[i] = make_uint4(0u, 0u, 0u, 0u);
-            for (int i = ct; i < kTreeRing * NC; i += Sh::Team) {
+            for (int i = ct; i < KV * Sh::Tile / 16; i += team) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = ct; i < Sh::QPart / 16; i += team) reinterpret_cast<uint4*>(sm + Sh::Q)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = ct; i < kTreeRing * NC; i += team) {
                 reinterpret_cast<float*>(sm + Sh::Unit)[i] = 0.0f;
                 reinterpret_cast<long long*>(sm + Sh::Seen)[i] = 0;
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(Sh::Team) : "memory");      // (nobody has waited for anything yet)
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * Sh::ValueWarps) : "memory");      // (nobody has waited for anything yet)
         }
         bool ok = true;
         for (int t = 0, come = keys ? 0 : 1; ok; ++t) {
