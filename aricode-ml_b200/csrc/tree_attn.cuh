@@ -219,9 +219,9 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
     if (tid == 0) {
         for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + Sh::KeyWarps + Sh::ValueWarps + 1); }
         for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], i & 1 ? Sh::ValueWarps : Sh::KeyWarps); }
-        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], 32 * Sh::KeyWarps); mbar_init(&kempty[i], 1); }
-        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], 32 * Sh::ValueWarps); mbar_init(&vempty[i], 1); }
-        mbar_init(qfull, 32 * Sh::ValueWarps); mbar_init(qfree, 1);
+        for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], Sh::KeyWarps); mbar_init(&kempty[i], 1); }
+        for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], Sh::ValueWarps); mbar_init(&vempty[i], 1); }
+        mbar_init(qfull, Sh::ValueWarps); mbar_init(qfree, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sfull[i], 2); mbar_init(&sfree[i], kTreeSoftWarps);
             mbar_init(&ofull[i], 1); mbar_init(&ofree[i], kTreeSoftWarps);
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 if (!ok) break;
                 put_queries(d);
                 fence_async_smem();
-                mbar_arrive(qfull);
+                arrive_warp(qfull);
             }
             unsigned char* tile = tiles + slot * Sh::Tile;
             if (d.flags & TREE_DRAFT) {
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 come += 2;
             }
             fence_async_smem();
-            mbar_arrive(&full[slot]);
+            arrive_warp(&full[slot]);
             arrive_warp(&tfree[t & (kTreeRing - 1)]);
         }
     } else {
