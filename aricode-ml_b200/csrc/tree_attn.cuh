@@ -44,8 +44,8 @@ struct TreeAttnParams {
 
 __device__ __forceinline__ int tree_splits(int kc, int keys) { return max((keys - 1) / kc + 1, 1); }
 
-// Warps 0 .. 15, softmax: warp w reads TMEM lanes 32 (w % 4) .. + 31 and columns w / 4 of the
-//   four parts of a tile's columns.
+// First the softmax warps: warp w reads TMEM lanes 32 (w % 4) .. + 31 and part w / 4 of a tile's
+//   columns.
 // Then the keys' warps: codes in shared memory to f16 operands; then the values', and an item's
 //   queries. Drafted rows likewise. (Codes that waited in registers of these warps took 80
 //   registers' worth of spills, and the fence behind the writes waits for loads under way.)
@@ -54,7 +54,6 @@ __device__ __forceinline__ int tree_splits(int kc, int keys) { return max((keys 
 //   the codes: a bulk copy for each block of 16 keys.
 // A CTA a SM goes through its items with the pipeline running on from one to the next. Every
 // wait is bounded; a warp whose wait ran out leaves its loop and sets the error word.
-constexpr int kTreeSoftWarps = 16;
 constexpr int kTreeRing = 8;
 constexpr int kTreeKeys = 128;
 
@@ -81,19 +80,23 @@ struct TreeShape {
     static constexpr int NB = ST < 2 ? 2 : ST;                     // barriers of those: a team's own
     static constexpr int Halves = DP / 64;                         // 128-byte parts of a row
     static constexpr int MH = DP == 256 ? 2 : 1;                   // 128 elements each of the output
-    static constexpr int QC = NC / 4;                              // columns of a thread
+    // Softmax warps: 8 for 16 columns (16, with 4 columns a thread: 32 sequences of 32 / 32 heads of 128 129 us,
+    // now 123: what a warp does for a tile whatever its columns are costs issue slots), else 16 (8, with 32
+    // columns a thread: two sequences of 40 K keys, 32 / 4 heads of 64: 400 us instead of 361)
+    static constexpr int Soft = NC == 16 ? 8 : 16, Parts = Soft / 4;
+    static constexpr int QC = NC / Parts;                          // columns of a thread
     // With 64 columns hi and lo go into the same sums, lo first: the MMAs take 96 clocks instead of 64 for
-    // each 16 elements or keys, and the warps that read the sums have half as many to read.
+    // each 16 elements or keys, and the warps that read the sums have half as many to read (482 us, then 428). With
+    // twice the elements the MMAs are more of a tile's time (32 / 8 heads of 128: 235 us, hi and lo in the same sums 256).
     static constexpr bool Same = DP == 64 && NC == 64;
     static constexpr int Sums = Same ? NC : 2 * NC;                // TMEM columns of a product
     // d_head up to 64: lanes 64 .. 127 of the output are the others again, so each has half of the columns
-    static constexpr int OC = Same ? QC / 2 : QC;      // columns of a thread's output
-    // Warps that make operands of keys, of values. With 16 columns the softmax needs 72 registers, which leaves
-    // room for four each (two each: 32 sequences of 32 / 32 heads of 128 172 us, now 130). Else two, but four for
-    // values with only one place, which they refill between one tile's product and the next (16 sequences of 32 / 8
-    // heads of 128: 237 us with two, 213 with four; two of 32 / 4 heads of 64, two places: 344 and 368).
+    static constexpr int OC = Same ? QC / 2 : QC;                  // columns of a thread's output
+    // Warps that make operands of keys, of values: four each beside 8 softmax warps (eight: 130 us). Else two, but
+    // four for values with only one place, which they refill between one tile's product and the next (16 sequences
+    // of 32 / 8 heads of 128: 237 us with two, 211 with four; 32 / 4 heads of 64, two places: 361 and 369).
     static constexpr int KeyWarps = NC == 16 ? 4 : 2, ValueWarps = NC == 16 || KV == 1 ? 4 : 2;
-    static constexpr int Threads = (kTreeSoftWarps + KeyWarps + ValueWarps + 2) * 32;
+    static constexpr int Threads = (Soft + KeyWarps + ValueWarps + 2) * 32;
     static constexpr int Tile = Halves * kTreeKeys * 128;          // [part][key][64 f16], swizzled
     static constexpr int QPart = Halves * 2 * NC * 128;            // [part][column: hi, lo][64 f16], swizzled
     static constexpr int PPart = kTreeKeys * 128;                  // [key][64 columns: hi, lo], swizzled
@@ -213,22 +216,22 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int dh = p.c.dh;
-    constexpr int kMmaWarp = kTreeSoftWarps + Sh::KeyWarps + Sh::ValueWarps, kPlanWarp = kMmaWarp + 1;
+    constexpr int kMmaWarp = Sh::Soft + Sh::KeyWarps + Sh::ValueWarps, kPlanWarp = kMmaWarp + 1;
 
     after_previous();
     if (tid == 0) {
-        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], kTreeSoftWarps + Sh::KeyWarps + Sh::ValueWarps + 1); }
+        for (int i = 0; i < kTreeRing; ++i) { mbar_init(&tready[i], 1); mbar_init(&tfree[i], Sh::Soft + Sh::KeyWarps + Sh::ValueWarps + 1); }
         for (int i = 0; i < NB; ++i) { mbar_init(&cfull[i], 1); mbar_init(&cempty[i], i & 1 ? Sh::ValueWarps : Sh::KeyWarps); }
         for (int i = 0; i < KK; ++i) { mbar_init(&kfull[i], Sh::KeyWarps); mbar_init(&kempty[i], 1); }
         for (int i = 0; i < KV; ++i) { mbar_init(&vfull[i], Sh::ValueWarps); mbar_init(&vempty[i], 1); }
         mbar_init(qfull, Sh::ValueWarps); mbar_init(qfree, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sfull[i], 2); mbar_init(&sfree[i], kTreeSoftWarps);
-            mbar_init(&ofull[i], 1); mbar_init(&ofree[i], kTreeSoftWarps);
-            mbar_init(&pfull[i], kTreeSoftWarps);
+            mbar_init(&sfull[i], 2); mbar_init(&sfree[i], Sh::Soft);
+            mbar_init(&ofull[i], 1); mbar_init(&ofree[i], Sh::Soft);
+            mbar_init(&pfull[i], Sh::Soft);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&part_bar[i], 4);
-        mbar_init(all_bar, kTreeSoftWarps); mbar_init(done, 1);
+        mbar_init(all_bar, Sh::Soft); mbar_init(done, 1);
         fence_mbar_init();
         *fail = 0;
     }
@@ -453,13 +456,13 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
         if (me) umma_commit(done);                             // also after a wait that ran out: no MMA may be
         __syncwarp();
         if (!mbar_wait_bounded(done, 0)) *fail = 1;            // under way when its memory is given up
-    } else if (warp >= kTreeSoftWarps) {
+    } else if (warp >= Sh::Soft) {
         // ---- operands: a team for the keys, one for the values
         constexpr int Chunks = DP / 16;                        // 16 codes each of a row
         constexpr int Wide = kTreeKeys * Chunks / (32 * Sh::ValueWarps) < 8 ? kTreeKeys * Chunks / (32 * Sh::ValueWarps) : 8;
-        const bool keys = warp < kTreeSoftWarps + Sh::KeyWarps;
+        const bool keys = warp < Sh::Soft + Sh::KeyWarps;
         const int team = 32 * (keys ? Sh::KeyWarps : Sh::ValueWarps), step = team / Chunks, lines = team / 16;
-        const int ct = tid - (kTreeSoftWarps + (keys ? 0 : Sh::KeyWarps)) * 32, chunk = ct % Chunks, key0 = ct / Chunks;
+        const int ct = tid - (Sh::Soft + (keys ? 0 : Sh::KeyWarps)) * 32, chunk = ct % Chunks, key0 = ct / Chunks;
         const float* rows = keys ? p.k : p.v;
         const long long ldr = keys ? p.ldk : p.ldv;
         unsigned char* tiles = sm + (keys ? Sh::K : Sh::V);
@@ -798,13 +801,9 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 const float2 y = unpack2(s[x]);
                 split_f16(y.x, y.y, hi[x], lo[x]);
             }
-            if constexpr (QC == 4) {
-                unsigned char* at = pd + 8 * (part & 1);
-                *reinterpret_cast<uint2*>(at + (((part >> 1) ^ (key & 7)) << 4)) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(at + (((2 + (part >> 1)) ^ (key & 7)) << 4)) = make_uint2(lo[0], lo[1]);
-            } else if constexpr (QC == 8) {
+            if constexpr (QC == 8) {
                 *reinterpret_cast<uint4*>(pd + ((part ^ (key & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(pd + (((4 + part) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                *reinterpret_cast<uint4*>(pd + (((NC / 8 + part) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             } else {
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
