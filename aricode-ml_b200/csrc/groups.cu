@@ -44,7 +44,7 @@ template <int GROUP, int NT, bool BF16>
 cudaError_t launch_gemv_groups(const GroupParams& p, int sms, cudaStream_t s) {
     const int smem = (int)smem_bytes(NT, p.n);
     auto k = group_gemv_kernel<GROUP, NT, BF16>;
-    cudaError_t e = allow_smem<group_gemv_kernel<GROUP, NT, BF16>>(smem);
+    cudaError_t e = allow_smem<group_gemv_kernel<GROUP, NT, BF16>>((int)kSmem);      // (whatever other threads' calls need)
     if (e != cudaSuccess) return e;
     const int tiles = (p.m + 15) / 16, slots = kGroupWarps / p.warps_k;
     return launch_ex(k, dim3((unsigned)std::min((tiles + slots - 1) / slots, sms)), dim3(kGroupWarps * 32), smem, s, true, p);

@@ -62,7 +62,8 @@ inline int sm_count() {
 }
 
 // dynamic shared memory of up to `bytes` for kernel k on the current device, asked for where no
-// call there has asked for as much (the question costs as much as a quarter of a launch)
+// call there has asked for as much (the question costs as much as a quarter of a launch). A kernel's calls all ask
+// for the same, so that one thread never takes back what another has asked for.
 template <auto k>
 inline cudaError_t allow_smem(int bytes) {
     static std::atomic<int> allowed[64];

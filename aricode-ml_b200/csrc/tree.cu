@@ -154,6 +154,16 @@ int b2_tree_accept(const b2_tree_rows* tree, const float* logits, int64_t ld, in
     if (!logits || !tokens || !kept_start || !kept_len || !kept_rows || !kept_ids || !al4(logits) || !al4(tokens) ||
         !al4(kept_start) || !al4(kept_len) || !al4(kept_rows) || !al4(kept_ids) || !al4(err))
         return refuse(fn, "logits, tokens and the kept arrays must be set, 4-byte aligned");
+    auto words = [](const void* x, int64_t n) { return Span{static_cast<const float*>(x), n, n}; };
+    const int64_t n = p.r.n_rows, ns = p.r.n_seq;
+    const Span outs[4] = {words(kept_start, ns + 1), words(kept_len, ns), words(kept_rows, n), words(kept_ids, n)};
+    const Span ins[4] = {words(tree->row_start, ns + 1), words(tree->kv_len, ns), words(tree->seen, 2 * n), words(tokens, n)};
+    for (int i = 0; i < 4; ++i) {
+        bool bad = overlap({logits, ld, vocab}, {outs[i].p, 0, outs[i].width}, p.r.n_rows);
+        for (int j = 0; j < 4; ++j)
+            bad = bad || (j > i && overlap(outs[i], outs[j], 1)) || (overlap(outs[i], ins[j], 1) && !(i == 1 && j == 1 && same(outs[i], ins[j])));
+        if (bad) return refuse(fn, "a kept array overlaps an input (other than kept_len being kv_len) or another one");
+    }
     p.splits = accept_splits(tree, vocab);
     const size_t need = accept_bytes(tree, p.splits);
     if (!workspace || !al16(workspace) || workspace_bytes < need)
@@ -167,7 +177,7 @@ int b2_tree_accept(const b2_tree_rows* tree, const float* logits, int64_t ld, in
     p.ids = reinterpret_cast<int*>(p.paths + p.r.n_seq);
     p.err = err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_ex(tree_argmax_kernel, dim3((unsigned)p.splits, (unsigned)p.r.n_rows), dim3(256), 0, s, true, p);
+    cudaError_t e = launch_ex(tree_argmax_kernel, dim3((unsigned)p.r.n_rows * p.splits), dim3(256), 0, s, true, p);
     if (e == cudaSuccess) e = launch_ex(tree_path_kernel, dim3(1), dim3(1024), 0, s, true, p);
     return status(fn, e);
 }

@@ -32,11 +32,12 @@ struct TreeAcceptParams {
     int* err;
 };
 
-// The largest word of a row's split: CTA (split, row). Bound by memory.
+// The largest word of a row's split: CTA row * splits + split. Bound by memory (730 rows of 50257 logits: 28 us,
+// 22 at 6.56 TB/s).
 static __global__ void __launch_bounds__(256) tree_argmax_kernel(const __grid_constant__ TreeAcceptParams p) {
     __shared__ unsigned long long sb[8];
     after_previous();
-    const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x;
+    const int row = blockIdx.x / p.splits, split = blockIdx.x % p.splits, tid = threadIdx.x;
     if (row >= min(p.r.row_start[p.r.n_seq], p.r.n_rows)) return;      // rows of no sequence
     const float* x = p.logits + (size_t)row * p.ld;
     const int i0 = split * p.chunk, i1 = min(i0 + p.chunk, p.vocab);
@@ -64,7 +65,8 @@ static __global__ void __launch_bounds__(256) tree_argmax_kernel(const __grid_co
 }
 
 // The paths: one CTA, a warp a sequence at a time, two rows a lane; then the sums of their
-// lengths, and the kept rows in order. A path's rows ascend, so a path is a 64-bit word.
+// lengths, and the kept rows in order. A path's rows ascend, so a path is a 64-bit word. Bound by latency
+// (48 sequences: 8.5 us).
 static __global__ void __launch_bounds__(1024) tree_path_kernel(const __grid_constant__ TreeAcceptParams p) {
     __shared__ int sums[32];
     after_previous();

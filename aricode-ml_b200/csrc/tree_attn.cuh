@@ -8,13 +8,22 @@
 // which keeps 22 bits of every element down to 2^-26 of the largest, and 2^-38 of the largest of
 // those below (weights: [2^5, 2^6), 2^-18 and 2^-30). The cached codes are exact in f16; drafted keys and values are two
 // f16 too, as keys j and 64 + j of a tile of their own, so that all four products are made.
-//   S^T [key][column] = K Q^T      hi and lo of Q as columns side by side (keys are read once:
-//   O^T [element][column] = V^T P  the MMAs are bound by reading operands), P weights p x v_scale
+//   S^T [key][column] = K Q^T      P: weights p x v_scale. Hi and lo of Q and P are columns side by
+//   O^T [element][column] = V^T P  side (keys are read once: the MMAs are bound by reading operands)
 // Keys and elements lie on the TMEM lanes: a thread has one key of a few columns, whose scales
 // are its own. Each tile's output sums go to f32 registers, so that the tensor cores' sums stay
 // short. What the exponentials are relative to, h, moves only when a score is more than 2^8
 // above it: then its largest is found across the lanes; a tile that moves nothing needs no
 // more than the warps' word that it does not.
+//
+// Measured (a call, us; bytes at 6.56 TB/s or operations at the bf16 rate allow the second figure):
+//   1 sequence of 5 rows over 639 keys, 32 / 32 heads of 128             13   0.8  latency of one item
+//   32 of 16 rows over 1152 keys, 32 / 32 heads of 128                  123    51  a tile's turn of the only place
+//     for keys: conversion 1500 clocks, scores 600, waits between warps 800; issue slots 70 %
+//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       212    18  the same with 64 columns
+//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    362    25  the softmax: 56 % of issue slots,
+//     11 K instructions of warps a tile of 128 keys x 64 columns, tensor pipe active 19 %
+// Two groups of softmax warps with every other tile each and two places for queries: 137 instead of 130.
 #pragma once
 #include <type_traits>
 
@@ -73,6 +82,7 @@ struct TreeTile {
 // DP: d_head rounded up to 64, 128 or 256; NC: columns of an item
 template <int DP, int NC>
 struct TreeShape {
+    // (A second tile of keys in the place of two tiles of codes, d_head 128 and 16 columns: 153 us instead of 130.)
     static constexpr int KK = DP == 64 ? 2 : 1;                    // tiles of keys held,
     static constexpr int KV = DP == 64 || (DP == 128 && NC == 16) ? 2 : 1;      // of values,
     static constexpr int PB = DP == 256 ? 1 : 2;                   // of weights,
@@ -316,7 +326,8 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             }
             // column tiles first: CTAs that run at once read the same keys
             const int ctiles = (len * p.G + NC - 1) / NC, nsplit = tree_splits(p.kc, kv);
-            const int ct = (int)(idx % (unsigned)ctiles), rest = (int)(idx / (unsigned)ctiles), kvh = rest % p.c.KVH, split = rest / p.c.KVH;
+            const int ct = (int)(idx % (unsigned)ctiles), rest = (int)(idx / (unsigned)ctiles), kvh = rest % p.c.KVH;
+            const int split = min(rest / p.c.KVH, nsplit - 1);  // (row ranges that overlap could count past 32 bits)
             const int j0 = split * p.kc, jend = kv - j0 < p.kc ? kv : j0 + p.kc;
             const int ntiles = (max(jend - j0, 0) + kTreeKeys - 1) / kTreeKeys, all = ntiles + (split == nsplit - 1);
             for (int i0 = 0; i0 < all && ok; i0 += 4) {

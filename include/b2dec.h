@@ -215,10 +215,12 @@ int b2_gemv_i4_rowscale(const uint8_t* W, int64_t ld, const float* scale, const 
  * group: 32, 64 or 128 columns, the last one may be shorter. scale [m][lds] f32, or
  * bf16 where scale_bf16 is set. X [T][ldx], Y [T][ldy] f32, 4-byte aligned; Y overlaps
  * nothing that is read. For one token or a few (a tree of drafted tokens, a few
- * sequences); more than 64 read the weights once for every 64. Precision: a vector's
- * elements are held to 2^-24 of the largest of each 128 neighbours, codes, products and
- * their sums over a group are exact, the rest f32. A NaN or infinity makes the outputs of
- * its vector NaN.
+ * sequences); more than 64 read the weights once for every 64. Precision: codes are exact.
+ * Up to eight vectors: a vector's elements are held to 2^-24 of the largest of each 128
+ * neighbours, products and their sums over a group are exact, the rest is f32. More: each
+ * element to 2^-22 of itself or 2^-38 of the largest of its 128 neighbours, whichever is
+ * more; products are exact, all sums f32. A NaN or infinity makes the outputs of its
+ * vector NaN, and of no other.
  * workspace: b2_gemv_i4_groups_workspace() bytes (may be 0), 16-byte aligned, no
  * initialisation; calls that may overlap on the GPU need one each. No counterpart in
  * the reference, whose 4-bit rows have one scale (arr_i4_matvec_f32_perrow). */

@@ -182,6 +182,35 @@ def test_another_stream_and_order_behind_it(torch, rt):
     close(y3, want, tol)
 
 
+def test_threads_with_calls_of_different_sizes(torch, rt):
+    """Threads on streams of their own, whose calls need different amounts of shared memory; the first calls are theirs."""
+    import threading
+    cases = [make(torch, 48, n, T, 64, torch.bfloat16, seed=n) for n, T in ((9000, 1), (128, 1), (20000, 2), (640, 2), (4000, 4), (256, 5))]
+    want = [product64(torch, *c, 64) for c in cases]
+    torch.cuda.synchronize()
+    got, failed = [[] for _ in cases], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i].append(rt.gemv_i4_groups(*cases[i], 64))
+            s.synchronize()
+        except Exception as e:                                     # noqa: BLE001 (told by the assertion)
+            failed.append(repr(e))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for ys, (y, tol) in zip(got, want):
+        assert len(ys) == 20
+        for z in ys:
+            close(z, y, tol)
+
+
 def test_same_bits_every_time(torch, rt):
     for T in (1, 6, 24):
         W, scale, x = make(torch, 700, 3000, T, 32, torch.bfloat16)

@@ -440,6 +440,11 @@ def test_many_sequences(torch, rt):
     check_acceptance(torch, rt, *accept_case(torch, rt, rows, 12, seed=1, pad=5))
 
 
+def test_more_rows_than_a_grid_dimension_has(torch, rt):
+    """66000 rows: more than the 65535 that the second dimension of a grid can count."""
+    check_acceptance(torch, rt, *accept_case(torch, rt, [60] * 1100, 3, seed=3, pad=1))
+
+
 def test_strided_logits(torch, rt):
     check_acceptance(torch, rt, *accept_case(torch, rt, [9, 3], 1001, seed=2, wide=2))
 

@@ -36,7 +36,8 @@ def attend(rt, kv, t, **kw):
 
 
 def accept(rt, t, **kw):
-    a = dict(logits=A, ld=100, vocab=100, tokens=A, start=A, kv_len=A, rows=A, ids=A, ws=A, ws_bytes=1 << 40, err=None)
+    a = dict(logits=2 * A, ld=100, vocab=100, tokens=3 * A, start=4 * A, kv_len=5 * A, rows=6 * A, ids=7 * A, ws=8 * A, ws_bytes=1 << 40,
+             err=None)
     a.update(kw)
     return rt.lib().b2_tree_accept(C.addressof(t) if t else None, *a.values(), None)
 
@@ -89,6 +90,14 @@ def test_bad_attention_is_refused(pkg, bad):
                                  dict(ws_bytes=3), dict(err=A + 2)])
 def test_bad_acceptance_is_refused(pkg, bad):
     assert accept(pkg.runtime, tree(pkg.runtime), **bad) == -1
+
+
+@pytest.mark.parametrize("bad", [dict(start=A), dict(kv_len=A + 4), dict(rows=3 * A), dict(ids=3 * A + 16), dict(rows=7 * A - 4),
+                                 dict(ids=6 * A + 4), dict(start=5 * A - 8), dict(rows=A), dict(ids=2 * A + 1600), dict(kv_len=4 * A + 8)])
+def test_kept_arrays_that_overlap_are_refused(pkg, bad):
+    """row_start, kv_len and seen at A; logits, tokens and the kept arrays from 2 A on: 5 rows, 2 sequences."""
+    assert accept(pkg.runtime, tree(pkg.runtime), **bad) == -1
+    assert "overlaps" in pkg.runtime.last_error()
 
 
 @pytest.mark.parametrize("bad", [dict(index=None), dict(index=A + 2), dict(n_src=-1), dict(k=None), dict(v=A + 4), dict(ldk=124),
