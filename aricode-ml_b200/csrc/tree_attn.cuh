@@ -20,8 +20,8 @@
 //   1 sequence of 5 rows over 639 keys, 32 / 32 heads of 128             13   0.8  latency of one item
 //   32 of 16 rows over 1152 keys, 32 / 32 heads of 128                  123    51  a tile's turn of the only place
 //     for keys: conversion 1500 clocks, scores 600, waits between warps 800; issue slots 70 %
-//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       212    18  the same with 64 columns
-//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    362    25  the softmax: 56 % of issue slots,
+//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       211    18  the same with 64 columns
+//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    351    25  the softmax: 56 % of issue slots,
 //     11 K instructions of warps a tile of 128 keys x 64 columns, tensor pipe active 19 %
 // Two groups of softmax warps with every other tile each and two places for queries: 137 instead of 130.
 #pragma once
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 gone = (key & 63) >= d.len;
                 ks = gone ? 0.0f : dk[key & 63];
                 vs = dv[key & 63];
-                for (int i = 0; i < d.len; ++i) vtop = fmaxf(vtop, dv[i]);
+                vtop = warp_max(fmaxf(lane < d.len ? dv[lane] : 0.0f, lane + 32 < d.len ? dv[lane + 32] : 0.0f));
             }
             if (gone) vs = 0.0f;
             if (draft) {
@@ -832,14 +832,31 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 fold(t, u1, moved1);
                 if (!ok) break;
                 // the item's sums over its keys, then its columns to memory
-                float mine = 0.0f;
+                // (the lanes halve the columns that they add up: lane x / (32 / QC) ends with column x)
+                float z[QC];
 #pragma unroll
-                for (int c = 0; c < QC; ++c) {
-                    const float2 y = unpack2(l[c / 2]);
-                    const float z = butterfly32(c & 1 ? y.y : y.x);
-                    if (lane == c) mine = z;
+                for (int x = 0; x < QC / 2; ++x) {
+                    const float2 y = unpack2(l[x]);
+                    z[2 * x] = y.x; z[2 * x + 1] = y.y;
                 }
-                if (lane < QC) xl[quarter * QC + lane] = mine;
+                int keep = QC;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) {
+                    if (keep == 1) {
+                        z[0] += __shfl_xor_sync(0xffffffffu, z[0], o);
+                        continue;
+                    }
+                    keep /= 2;
+                    const bool up = lane & o;
+#pragma unroll
+                    for (int x = 0; x < QC / 2; ++x) {
+                        if (x >= keep) break;
+                        const float give = __shfl_xor_sync(0xffffffffu, up ? z[x] : z[x + keep], o);
+                        z[x] = (up ? z[x + keep] : z[x]) + give;
+                    }
+                }
+                constexpr int Share = 32 / QC;
+                if (lane % Share == 0) xl[quarter * QC + lane / Share] = z[0];
                 if (!meet()) break;
                 float sum = 0.0f;
                 if (lane < QC) {
@@ -850,20 +867,15 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 __syncwarp();
                 const int mine_col = part * QC + (lane & (QC - 1));
                 float* mine_at = column_out(d, min(mine_col, d.cols - 1));
+#pragma unroll
                 for (int c = 0; c < OC; ++c) {
-                    if (part * QC + oc0 + c >= d.cols) break;
                     float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), oc0 + c));
+                    if (part * QC + oc0 + c >= d.cols) continue;
                     const float inv = bd[oc0 + c];
 #pragma unroll
                     for (int mh = 0; mh < MH; ++mh) {
-                        float y = 0.0f;                        // (registers are not indexed)
-#pragma unroll
-                        for (int x = 0; x < OC / 2; ++x) {
-                            const float2 z = unpack2(o[mh][x]);
-                            if (c == 2 * x) y = z.x;
-                            if (c == 2 * x + 1) y = z.y;
-                        }
-                        if (oelem + 128 * mh < dh) dst[oelem + 128 * mh] = y * inv;
+                        const float2 y = unpack2(o[mh][c / 2]);
+                        if (oelem + 128 * mh < dh) dst[oelem + 128 * mh] = (c & 1 ? y.y : y.x) * inv;
                     }
                 }
                 if (d.nsplit > 1 && quarter == 0 && lane < QC && mine_col < d.cols) {
