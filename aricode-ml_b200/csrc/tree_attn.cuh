@@ -492,10 +492,10 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
 #pragma unroll
                 for (int x = 0; x < Wide; ++x) {
                     const int key = at + x * step;
-                    const uint4 lo = codes_f16(r[x].x, r[x].y), hi = codes_f16(r[x].z, r[x].w);
+                    const uint4 a = codes_f16(turn ? r[x].z : r[x].x, turn ? r[x].w : r[x].y), b = codes_f16(turn ? r[x].x : r[x].z, turn ? r[x].y : r[x].w);
                     unsigned char* row = part + key * 128;
-                    *reinterpret_cast<uint4*>(row + (((u0 + turn) ^ (key & 7)) << 4)) = turn ? hi : lo;
-                    *reinterpret_cast<uint4*>(row + (((u0 + 1 - turn) ^ (key & 7)) << 4)) = turn ? lo : hi;
+                    *reinterpret_cast<uint4*>(row + (((u0 + turn) ^ (key & 7)) << 4)) = a;
+                    *reinterpret_cast<uint4*>(row + (((u0 + 1 - turn) ^ (key & 7)) << 4)) = b;
                 }
             }
         };
@@ -725,9 +725,10 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             // scores in base 2 relative to h
             float top = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < QC / 2; ++x) {
-                const float2 un = *reinterpret_cast<const float2*>(unit + 2 * x), hh = *reinterpret_cast<const float2*>(bs + 2 * x);
+            for (int x = 0; x < QC / 2; x += 2) {
+                const float4 un = *reinterpret_cast<const float4*>(unit + 2 * x), hh = *reinterpret_cast<const float4*>(bs + 2 * x);
                 s[x] = fma2(s[x], mul2(pack2(un.x, un.y), pack2(ks, ks)), pack2(hh.x, hh.y));
+                s[x + 1] = fma2(s[x + 1], mul2(pack2(un.z, un.w), pack2(ks, ks)), pack2(hh.z, hh.w));
             }
             if (draft) {
                 const long long* seen = reinterpret_cast<const long long*>(sm + Sh::Seen) + it * NC + part * QC;
