@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
         }
     } else {
         // sums
-        constexpr int C = NT / 2, RC = C < 16 ? 8 : 16;        // vectors of a thread; read at a time
+        constexpr int C = NT / 2;                              // vectors of a thread
         const int quarter = warp & 3, c0 = (warp >> 2) * C, r = 32 * quarter + lane;
         const uint32_t trow = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)c0;
         const int groups = (p.n + GROUP - 1) / GROUP;
@@ -552,12 +552,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t d[C];
-#pragma unroll
-                for (int q = 0; q < C / RC; ++q) {
-                    if constexpr (RC == 16) tmem_ld16(trow + b * NT + q * RC, *reinterpret_cast<uint32_t(*)[16]>(d + q * RC));
-                    else tmem_ld8(trow + b * NT + q * RC, *reinterpret_cast<uint32_t(*)[8]>(d + q * RC));
-                }
-                tmem_wait_ld();
+                tmem_read(trow + b * NT, d);
 #pragma unroll
                 for (int x = 0; x < C / 2; x += 2) {
                     const float4 uu = *reinterpret_cast<const float4*>(un + 2 * x);
