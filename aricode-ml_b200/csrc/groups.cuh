@@ -108,8 +108,8 @@ __device__ __forceinline__ void group_digits(const GroupParams& p, int t, int kb
 
 template <int GROUP, int NT>
 __global__ void __launch_bounds__(256) group_digits_kernel(const __grid_constant__ GroupParams p) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();                                   // (not before: what the products read besides is ready then)
     const int word = blockIdx.x * 256 + threadIdx.x, kb = word >> 4, t = blockIdx.y;
     const bool live = kb * 128 < p.n;
     group_digits<GROUP>(p, t, live ? kb : 0, word & 15, live, p.digits + (size_t)kb * NT * 64, p.units + (size_t)kb * NT * 8);
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
     float* unit = reinterpret_cast<float*>(frag + (size_t)blocks * NT * 64);
     float* red = unit + (size_t)blocks * NT * 8;
     pdl_launch_dependents();
-    pdl_wait();
+    if (!p.digits) pdl_wait();                                 // (else behind the first weights, which are ready)
 
     // this warp's pieces: (tile, 512 columns)
     int tile = blockIdx.x * slots + slot, it = wk;
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
     };
     load(tile, it);
     if (p.digits) {
+        pdl_wait();
         for (int i = tid; i < blocks * NT * 64; i += kGroupWarps * 32) frag[i] = p.digits[i];
         for (int i = tid; i < blocks * NT * 8; i += kGroupWarps * 32) unit[i] = p.units[i];
     } else {
@@ -275,9 +276,9 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
 // A CTA a SM has an equal share of the (128 rows, 128 columns) steps in order: parts of row
 // tiles and whole ones; parts' sums go to the workspace and are added in order of columns.
 // Warps 0 .. 7: sums to f32: warp w has TMEM lanes (rows) 32 (w % 4) .. + 31 and half w / 4 of the vectors.
-// Warps 8 .. 15: codes to f16 operands. Warps 16, 17: copies (packed rows by TMA, with x's units; its
-// images by bulk copies: one warp for all was what a step waited for). Warp 18: issues the MMAs. Every wait
-// is bounded.
+// Warps 8 .. 15: codes to f16 operands. Warps 16, 17: copies (packed rows by TMA; x's images and units
+// by bulk copies, behind the launch that makes them: one warp for all was what a step waited for). Warp
+// 18: issues the MMAs. Every wait is bounded. 4096 x 11008, 64 vectors: 27 us (weights alone 4); 5632 x 2048, 13: 14.
 constexpr int kGemmSumWarps = 8, kGemmConvWarps = 8;
 constexpr int kTeam = kGemmConvWarps / 2 * 32;                 // threads that turn a step's codes
 constexpr int kGemmThreads = (kGemmSumWarps + kGemmConvWarps + 3) * 32;
@@ -295,7 +296,7 @@ struct GemmShape {
     static constexpr int X = A + SA * Tile;
     static constexpr int W = X + SX * Image;
     static constexpr int U = W + SW * Packed;
-    static constexpr int Bars = U + SW * Units;
+    static constexpr int Bars = U + SX * Units;
     static constexpr int NBars = 2 * SA + 2 * SX + 2 * SW + 2 * DB + 1;
     static constexpr int Alloc = Bars + NBars * 8 + 16 + 1024;
     static constexpr int TmemCols = DB * NT;
@@ -326,8 +327,8 @@ __device__ __forceinline__ int gemm_cta(int steps, int ctas, int at) {
 // the codes come out of it: 0 4 1 5 2 6 3 7
 template <int NT>
 __global__ void __launch_bounds__(256) group_images_kernel(const __grid_constant__ GroupParams p) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();                                   // (not before: what the products read besides is ready then)
     const int word = blockIdx.x * 256 + threadIdx.x, kb = word >> 4, w = word & 15, t = blockIdx.y;
     const bool live = kb * 128 < p.n;
     const int k0 = kb * 128 + 8 * w;
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
 
     if (tid < Sh::NBars) {
         const int i = tid, w = 2 * Sh::SW, x = w + 2 * Sh::SX, a = x + 2 * Sh::SA, d = a + 2 * DB;
-        mbar_init(wfull + i, i < Sh::SW ? 1 : i < w ? kGemmConvWarps / 2 + kGemmSumWarps : i < x ? 1 : i < x + Sh::SA ? kTeam : i < a ? 1 : i < a + DB ? 1 : i < d ? kGemmSumWarps : 1);
+        mbar_init(wfull + i, i < Sh::SW ? 1 : i < w ? kGemmConvWarps / 2 : i < w + Sh::SX ? 1 : i < x ? 1 + kGemmSumWarps : i < x + Sh::SA ? kTeam : i < a ? 1 : i < a + DB ? 1 : i < d ? kGemmSumWarps : 1);
         fence_mbar_init();
         if (tid == 0) *fail = 0;
     }
@@ -394,8 +395,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_launch_dependents();
-    pdl_wait();
+    pdl_launch_dependents();                                   // (only the images' warp waits: weights are ready)
     auto wait = [&](uint64_t* bar, int parity) {               // false: it ran out (1 s)
         bool ok = mbar_try_wait(bar, (uint32_t)parity);
         if (!ok) ok = mbar_wait_bounded(bar, (uint32_t)parity);
@@ -411,15 +411,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
         const bool codes = warp == kCopyWarp;
         uint64_t *full = codes ? wfull : xfull, *empty = codes ? wempty : xempty;
         const int slots = codes ? Sh::SW : Sh::SX;
+        if (!codes) pdl_wait();
         int kb = first % blocks, tile = first / blocks, i = 0, slot = 0, turn = 1;      // turn: parity of the slots' last emptying
         for (; i < steps; ++i) {
             if (i >= slots && !wait(&empty[slot], turn)) break;
             if (lane == 0) {
-                mbar_arrive_expect_tx(&full[slot], codes ? Sh::Packed + Sh::Units : Sh::Image);
-                if (codes) {
-                    tma_load_2d(sm + Sh::W + slot * Sh::Packed, &p.W, 64 * kb, 128 * tile, &full[slot]);
+                mbar_arrive_expect_tx(&full[slot], codes ? Sh::Packed : Sh::Image + Sh::Units);
+                if (codes) tma_load_2d(sm + Sh::W + slot * Sh::Packed, &p.W, 64 * kb, 128 * tile, &full[slot]);
+                else {
+                    bulk_g2s(sm + Sh::X + slot * Sh::Image, p.images + (size_t)kb * Sh::Image, Sh::Image, &full[slot]);
                     bulk_g2s(sm + Sh::U + slot * Sh::Units, p.units + (size_t)kb * NT, Sh::Units, &full[slot]);
-                } else bulk_g2s(sm + Sh::X + slot * Sh::Image, p.images + (size_t)kb * Sh::Image, Sh::Image, &full[slot]);
+                }
             }
             if (++kb == blocks) { kb = 0; ++tile; }
             if (++slot == slots) { slot = 0; turn ^= 1; }
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
         int at = first % blocks, rows = first / blocks;        // of this step
         int part = 0;
         for (int i = 0; i < steps; ++i) {
-            const int sw = i % Sh::SW, row = rows * 128 + r;
+            const int sx = i % Sh::SX, row = rows * 128 + r;
             float s[GS];
 #pragma unroll
             for (int g = 0; g < GS; ++g) {
@@ -542,8 +544,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
             advance();
             scales(next[1]);
             if (++at == blocks) { at = 0; ++rows; }
-            if (!wait(&wfull[sw], (i / Sh::SW) & 1)) break;
-            const float* un = reinterpret_cast<const float*>(sm + Sh::U + sw * Sh::Units) + c0;
+            if (!wait(&xfull[sx], (i / Sh::SX) & 1)) break;
+            const float* un = reinterpret_cast<const float*>(sm + Sh::U + sx * Sh::Units) + c0;
             bool ok = true;
 #pragma unroll
             for (int g = 0; g < GS; ++g) {
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
                 arrive_warp(&dempty[b]);
             }
             if (!ok) break;
-            arrive_warp(&wempty[sw]);
+            arrive_warp(&xempty[sx]);
             if (at != 0 && i + 1 < steps) continue;
             // the end of the row tile, or of the share
             const bool whole = begun && at == 0;
