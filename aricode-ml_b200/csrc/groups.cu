@@ -28,14 +28,15 @@ int columns(int NT, int n) {
     return c;
 }
 
-// Warps that share a row tile: the fewest pieces (16 rows, 512 columns) one after another.
+// Warps that share a row tile: the fewest pieces (16 rows, 512 columns) one after another, a meeting for a quarter of
+// one (32000 x 4096: 7 pieces and as many meetings 24.0 us, 8 and none 22.2).
 int share(int m, int n, int sms) {
     const long long tiles = (m + 15) / 16, iters = (n + 511) / 512;
     int best = 1;
     long long least = 0;
     for (int w = 1; w <= kGroupWarps; w *= 2) {
-        const long long slots = (long long)sms * (kGroupWarps / w), pieces = (tiles + slots - 1) / slots * ((iters + w - 1) / w);
-        if (w == 1 || pieces < least) { best = w; least = pieces; }
+        const long long slots = (long long)sms * (kGroupWarps / w), cost = (tiles + slots - 1) / slots * (4 * ((iters + w - 1) / w) + (w > 1));
+        if (w == 1 || cost < least) { best = w; least = cost; }
     }
     return best;
 }
@@ -46,8 +47,7 @@ cudaError_t launch_gemv_groups(const GroupParams& p, int sms, cudaStream_t s) {
     auto k = group_gemv_kernel<GROUP, NT, BF16>;
     cudaError_t e = allow_smem<group_gemv_kernel<GROUP, NT, BF16>>((int)kSmem);      // (whatever other threads' calls need)
     if (e != cudaSuccess) return e;
-    const int tiles = (p.m + 15) / 16, slots = kGroupWarps / p.warps_k;
-    return launch_ex(k, dim3((unsigned)std::min((tiles + slots - 1) / slots, sms)), dim3(kGroupWarps * 32), smem, s, true, p);
+    return launch_ex(k, dim3((unsigned)std::min((p.m + 15) / 16, sms)), dim3(kGroupWarps * 32), smem, s, true, p);
 }
 
 template <int GROUP, int NT>
