@@ -71,12 +71,15 @@ static __global__ void __launch_bounds__(1024) tree_path_kernel(const __grid_con
     __shared__ int sums[32];
     after_previous();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int live = min(p.r.row_start[p.r.n_seq], p.r.n_rows);    // rows that have a largest word
     for (int s = warp; s < p.r.n_seq; s += 32) {
-        const SeqRows q = seq_rows(p.r, s);
+        SeqRows q = seq_rows(p.r, s);
         if (p.r.row_start[s + 1] < p.r.row_start[s] && lane == 0) set_err(p.err, B2_DEV_ERR_BAD_ROWS);
         if (q.len > kTreeRows && lane == 0) set_err(p.err, B2_DEV_ERR_TOO_MANY);
         unsigned long long path = 0ull;
-        if (q.len > 0 && q.len <= kTreeRows) {
+        const bool tree = q.len <= kTreeRows;
+        q.len = min(q.len, live - q.a);                        // (less only where a start falls, which is flagged)
+        if (q.len > 0 && tree) {
             int id[2], parent[2], token[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {

@@ -513,6 +513,44 @@ def test_acceptance_of_bad_rows(torch, rt):
     assert kept.start.amax() <= 5 and bool(((arrays[2, :5] >= -3) & (arrays[2, :5] < 5)).all())
 
 
+@pytest.mark.parametrize("starts", [[0, 10, 5], [0, 10, 0], [0, 4, 10, 7], [0, 10, -3], [0, 10, 10, 2, 2]])
+def test_ids_are_of_rows_whose_logits_were_looked_at(torch, rt, starts):
+    """The last start lies below an earlier one: whatever the workspace held, an id is a row's own, and what is left of a
+    path is its beginning."""
+    import random
+    n, vocab = 10, 5000
+    g, rng = torch.Generator(device="cuda").manual_seed(sum(starts)), random.Random(len(starts))
+    logits = torch.randn(n, vocab, device="cuda", generator=g)
+    ids = logits.argmax(-1).tolist()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ends = [max(a, b) for a, b in zip(starts, starts[1:])]
+    parents = [parents_of(rng, e - a, "chain") for a, e in zip(starts, ends) if a >= 0]
+    seen, tokens = [1] * n, [0] * n
+    for (a, e), p in zip(zip(starts, ends), parents):              # every draft is right: whole chains are accepted
+        for j, word in enumerate(rt.tree_seen(p)):
+            if a + j < n:
+                seen[a + j], tokens[a + j] = word, ids[a + j - 1]
+    ns = len(starts) - 1
+    tree = rt.TreeRows(torch.tensor(starts, **i32), torch.full((ns,), 20, **i32), torch.zeros(ns, 1, **i32),
+                       torch.tensor(seen, dtype=torch.int64, device="cuda"), n_rows=n)
+    ws = rt.tree_accept_workspace(tree, vocab)
+    for fill in (0x00, 0x5a, 0xff):
+        ws.fill_(fill)
+        kept = rt.TreeKept(tree)
+        kept.rows.fill_(-7)
+        kept.ids.fill_(-7)
+        rt.tree_accept(tree, logits, torch.tensor(tokens, **i32), kept, workspace=ws)
+        with pytest.raises(rt.B2Error, match="row_start below"):
+            tree.check()
+        last = max(starts[-1], 0)
+        want = [list(range(a, min(e, last))) if a >= 0 else [] for a, e in zip(starts, ends)]
+        flat = sum(want, [])
+        total = len(flat)
+        assert kept.start.tolist() == [sum(map(len, want[:s])) for s in range(ns + 1)]
+        assert kept.kv_len.tolist() == [20 + len(w) for w in want]
+        assert kept.rows.tolist() == flat + [-7] * (n - total) and kept.ids.tolist() == [ids[r] for r in flat] + [-7] * (n - total)
+
+
 def test_captured_acceptance(torch, rt):
     tree, logits, parents, start, tokens = accept_case(torch, rt, [9, 12], 5000, seed=6)
     tok = torch.tensor(tokens, dtype=torch.int32, device="cuda")
