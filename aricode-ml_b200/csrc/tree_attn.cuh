@@ -6,15 +6,22 @@
 // generation tensor cores in f16 with the factors that are f32 held as two f16 each:
 //   x f = hi + lo, f a power of two that brings the largest to [2^13, 2^14)
 // which keeps 22 bits of every element down to 2^-26 of the largest, and 2^-38 of the largest of
-// those below (weights: [2^5, 2^6), 2^-18 and 2^-30). The cached codes are exact in f16; drafted keys and values are two
+// those below. The cached codes are exact in f16; drafted keys and values are two
 // f16 too, as keys j and 64 + j of a tile of their own, so that all four products are made.
 //   S^T [key][column] = K Q^T      P: weights p x v_scale. Hi and lo of Q and P are columns side by
 //   O^T [element][column] = V^T P  side (keys are read once: the MMAs are bound by reading operands)
 // Keys and elements lie on the TMEM lanes: a thread has one key of a few columns, whose scales
 // are its own. Each tile's output sums go to f32 registers, so that the tensor cores' sums stay
-// short. What the exponentials are relative to, h, moves only when a score is more than 2^8
-// above it: then its largest is found across the lanes; a tile that moves nothing needs no
-// more than the warps' word that it does not.
+// short.
+// A column's weights are relative to the largest p x v_scale of the keys that it sees, over all
+// tiles: what a row does not see, or a key of large values and no probability, takes no bits
+// from the others. For that the exponentials are relative to h, the largest score + exponent of the
+// value scale, and an item's weights have one factor: 22 bits down to 2^-18 of that largest one, and
+// an absolute 2^-30 of it below. Exponents count from that of the item's first tile of values, 2^-80
+// to 2^80 times that, so that the sums of p stay in f32's range; a tile with values beyond has a
+// factor of its own, which brings them back to there. h is a whole
+// number and moves only when something is more than 2^8 above it: then the largest is found
+// across the lanes; a tile that moves nothing needs no more than the warps' word that it does not.
 //
 // Measured (a call, us; bytes at 6.56 TB/s or operations at the bf16 rate allow the second figure):
 //   1 sequence of 5 rows over 639 keys, 32 / 32 heads of 128             13   0.8  latency of one item
@@ -59,7 +66,8 @@ __device__ __forceinline__ int tree_splits(int kc, int keys) { return max((keys 
 //   queries. Drafted rows likewise. (Codes that waited in registers of these warps took 80
 //   registers' worth of spills, and the fence behind the writes waits for loads under way.)
 // One warp issues the MMAs. The last finds the items (a sequence's columns of a KV head against
-//   a split of its keys) and their tiles' blocks and scales, up to eight tiles ahead, and asks for
+//   a split of its keys) and their tiles' blocks, scales and factors (made by every softmax thread: 16
+//   sequences of 32 / 8 heads of 128 217 us, now 208), up to eight tiles ahead, and asks for
 //   the codes: a bulk copy for each block of 16 keys.
 // A CTA a SM goes through its items with the pipeline running on from one to the next. Every
 // wait is bounded; a warp whose wait ran out leaves its loop and sets the error word.
@@ -70,13 +78,16 @@ enum { TREE_FIRST = 1, TREE_LAST = 2, TREE_DRAFT = 4, TREE_END = 8 };
 
 struct TreeTile {
     int cell[8];             // block b of the tile in the pool (codes start at 16 dh times that; -1: none)
-    float ks[8], vs[8];      // their scales (-1 and 0: none)
+    float ks[8], vf[8];      // their scales, the values' times the tile's factor (-1 and 0: none),
+    float ve[8];             // and the exponents of the values', from ref on
+    float unit;              // what is one in the tile's output sums
+    int ref;                 // the exponent of the item's first values that are not zeros (-127: none yet)
     int flags, item;
     int limit;               // keys of the tile
     int a, len, kvh;         // the item's rows and KV head,
     int col0, cols;          // its columns (row * G + head),
     int split, nsplit;
-    int pad[2];
+    int pad[4];
 };
 
 // DP: d_head rounded up to 64, 128 or 256; NC: columns of an item
@@ -126,7 +137,7 @@ struct TreeShape {
     static constexpr int Xl = Xm + 2 * 16 * QC * 4;                // [4][4][QC] sums
     static constexpr int Bs = Xl + 16 * QC * 4;                    // [16 warps][QC] -h
     static constexpr int Bd = Bs + 16 * QC * 4;                    // [16][QC] how far it moves; at the end 1 / sum
-    static constexpr int Bk = Bd + 16 * QC * 4;                    // [2][16][QC] the factor of what was before
+    static constexpr int Bk = Bd + 16 * QC * 4;                    // [2][16][QC] the factor of what was before: its root
     static constexpr int Bars = Bk + 2 * 16 * QC * 4;
     static constexpr int NBars = 2 * kTreeRing + 2 * NB + 2 * KK + 2 * KV + 2 + 4 + 2 + 4 + 4 + 1 + 1;
     static constexpr int Bytes = Bars + NBars * 8 + 16;
@@ -149,8 +160,14 @@ __device__ __forceinline__ uint4 codes_f16(uint32_t a, uint32_t b) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-constexpr int kWeightBits = 5;                     // (weights: probabilities may reach 2^kMoveBits)
+constexpr int kWeightBits = 5;                     // (weights: p x v_scale may reach 2^(kMoveBits + 1.5))
 constexpr float kMoveBits = 8.0f;
+constexpr int kValueBits = 80;                     // how far h follows the exponents of value scales
+constexpr float kDraftedUnit = 64.0f;              // a drafted row's f16 reach 2^14, codes 2^7: brings its scale to theirs but for a bit
+
+// the exponent of a scale (>= 0; -127 for 0), and from `ref` on as far as h follows
+__device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_as_uint(scale) >> 23 & 0xff) - 127; }
+__device__ __forceinline__ int value_exponent(float scale, int ref) { return min(max(exponent_of(scale) - ref, -kValueBits), kValueBits); }
 
 __device__ __forceinline__ float warp_max(float x) {
     float r;
@@ -330,6 +347,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             const int split = min(rest / p.c.KVH, nsplit - 1);  // (row ranges that overlap could count past 32 bits)
             const int j0 = split * p.kc, jend = kv - j0 < p.kc ? kv : j0 + p.kc;
             const int ntiles = (max(jend - j0, 0) + kTreeKeys - 1) / kTreeKeys, all = ntiles + (split == nsplit - 1);
+            int ref = -127;
             for (int i0 = 0; i0 < all && ok; i0 += 4) {
                 const int i = i0 + group, in = i * kTreeKeys + 16 * b, cnt = min(all - i0, 4);
                 int cell = -1;
@@ -343,17 +361,27 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                         vs = p.c.vs[cell];
                     }
                 }
+                float vtop = vs;
+#pragma unroll
+                for (int o = 4; o >= 1; o >>= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+                if (ref == -127) {
+                    const unsigned any = __ballot_sync(0xffffffffu, vtop > 0.0f);
+                    if (any) ref = exponent_of(__shfl_sync(0xffffffffu, vtop, __ffs(any) - 1));
+                }
+                float f, unit;
+                f16_factor(vtop, kWeightBits + value_exponent(vtop, ref), f, unit);     // (the same for all tiles but those of extreme scales)
                 for (int u = 0; u < cnt && ok; ++u)
                     if (t + u >= kTreeRing) ok = wait_warp(&tfree[(t + u) & (kTreeRing - 1)], ring_parity(t + u) ^ 1, 100);
                 if (!ok) break;
                 if (group < cnt) {
                     TreeTile& d = ring[(t + group) & (kTreeRing - 1)];
-                    d.cell[b] = cell; d.ks[b] = ks; d.vs[b] = vs;
+                    d.cell[b] = cell; d.ks[b] = ks; d.vf[b] = vs * f; d.ve[b] = (float)value_exponent(vs, ref);
                     if (b == 0) {
                         d.flags = (i == 0 ? TREE_FIRST : 0) | (i == all - 1 ? TREE_LAST : 0) | (i == ntiles ? TREE_DRAFT : 0);
                         d.item = n; d.limit = jend - j0 - i * kTreeKeys;
                         d.a = a; d.len = len; d.kvh = kvh; d.col0 = ct * NC; d.cols = min(len * p.G - ct * NC, NC);
                         d.split = split; d.nsplit = nsplit;
+                        d.unit = unit; d.ref = ref;
                     }
                 }
                 __syncwarp();
@@ -639,7 +667,7 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
 #pragma unroll
                     for (int x = 0; x < OC / 2; ++x) {
                         const float2 bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + oc0 + 2 * x);
-                        o[mh][x] = mul2(o[mh][x], pack2(bb.x, bb.y));
+                        o[mh][x] = mul2(mul2(o[mh][x], pack2(bb.x, bb.y)), pack2(bb.x, bb.y));
                     }
                 }
                 f32x2 y[OC / 2];
@@ -686,18 +714,15 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             read_sums(trow + Sh::TmemS + (t & 1) * Sums, s, std::integral_constant<int, QC>{});
             tc_fence_before();
             arrive_warp(&sfree[t & 1]);
-            // this key's scales, and the largest value scale of the tile
-            float ks, vs, vtop = 0.0f;
+            // this key's scale, its value scale's exponent and that with the factor of the tile's weights
+            float ks, vf, ve, un;
             bool gone;
             if (!draft) {
                 ks = d.ks[key >> 4];
-                vs = d.vs[key >> 4];
+                vf = d.vf[key >> 4];
+                ve = d.ve[key >> 4];
+                un = d.unit;
                 gone = ks < 0.0f || key >= d.limit;
-#pragma unroll
-                for (int i = 0; i < 8; i += 4) {
-                    const float4 y = *reinterpret_cast<const float4*>(&d.vs[i]);
-                    vtop = fmaxf(vtop, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
-                }
             } else {
                 if (begun >= PB) PB == 2 ? fold(t - 2, u2, moved2) : fold(t - 1, u1, moved1);
                 if (!ok) break;
@@ -705,10 +730,16 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 const float* dv = reinterpret_cast<const float*>(sm + Sh::Dvs) + (t & (kTreeRing - 1)) * 64;
                 gone = (key & 63) >= d.len;
                 ks = gone ? 0.0f : dk[key & 63];
-                vs = dv[key & 63];
-                vtop = warp_max(fmaxf(lane < d.len ? dv[lane] : 0.0f, lane + 32 < d.len ? dv[lane + 32] : 0.0f));
+                const float vs = dv[key & 63] * kDraftedUnit;
+                const float vtop = warp_max(fmaxf(lane < d.len ? dv[lane] : 0.0f, lane + 32 < d.len ? dv[lane + 32] : 0.0f)) * kDraftedUnit;
+                const int ref = d.ref == -127 ? exponent_of(vtop) : d.ref;
+                ve = (float)value_exponent(vs, ref);
+                float f;
+                f16_factor(vtop, kWeightBits + value_exponent(vtop, ref), f, un);
+                vf = vs * f;
+                un *= 1.0f / kDraftedUnit;
             }
-            if (gone) vs = 0.0f;
+            if (gone) vf = 0.0f;
             if (draft) {
                 // scores of keys j and 64 + j together, through the weights' memory (tile t - 2's)
                 float* x = reinterpret_cast<float*>(sm + Sh::P + t % PB * Sh::PParts * Sh::PPart) + part * QC * kTreeKeys;
@@ -745,17 +776,17 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
             }
 #pragma unroll
             for (int x = 0; x < QC / 2; ++x) top = fmaxf(top, fmaxf(unpack2(s[x]).x, unpack2(s[x]).y));
-            if (__any_sync(0xffffffffu, top > kMoveBits) && lane == 0) moves[4 * (t & 1)] = t + 1;
+            if (__any_sync(0xffffffffu, top + ve > kMoveBits) && lane == 0) moves[4 * (t & 1)] = t + 1;
             arrive_warp(&part_bar[part]);
             if (PB == 2 && !draft && begun > 1) fold(t - 2, u2, moved2);   // (by now its products are made)
             if (!ok || !wait_warp(&part_bar[part], met++ & 1, 20)) break;
             const bool moved = *reinterpret_cast<volatile int*>(&moves[4 * (t & 1)]) == t + 1 || __any_sync(0xffffffffu, unset);
             if (moved) {
-                // the columns' largest scores, absolute: lane c has column c
+                // the columns' largest, relative to h: lane c has column c
                 float best = -INFINITY;
 #pragma unroll
                 for (int x = 0; x < QC / 2; ++x) {
-                    const float y0 = warp_max(unpack2(s[x]).x), y1 = warp_max(unpack2(s[x]).y);
+                    const float y0 = warp_max(unpack2(s[x]).x + ve), y1 = warp_max(unpack2(s[x]).y + ve);
                     if (lane == 2 * x) best = y0;
                     if (lane == 2 * x + 1) best = y1;
                 }
@@ -765,10 +796,10 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 if (lane < QC) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) best = fmaxf(best, xm[(t & 1) * 16 * QC + q * QC + lane]);
-                    by = unset ? (best > -INFINITY ? best : 0.0f) : fmaxf(best, 0.0f);
+                    by = rintf(unset ? (best > -INFINITY ? best : 0.0f) : fmaxf(best, 0.0f));
                     h += by;
                     bs[lane] = -h;
-                    bk[(t & 1) * 16 * QC + lane] = unset ? 0.0f : exp2_fast(-by);
+                    bk[(t & 1) * 16 * QC + lane] = unset ? 0.0f : exp2_fast(-0.5f * by);
                     bd[lane] = by;
                     unset = unset && !(best > -INFINITY);
                 }
@@ -777,13 +808,10 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 for (int x = 0; x < QC / 2; ++x) {
                     const float2 dd = *reinterpret_cast<const float2*>(bd + 2 * x), bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + 2 * x);
                     s[x] = add2(s[x], pack2(-dd.x, -dd.y));
-                    l[x] = mul2(l[x], pack2(bb.x, bb.y));
+                    l[x] = mul2(mul2(l[x], pack2(bb.x, bb.y)), pack2(bb.x, bb.y));      // (2^-by itself could leave f32's range)
                 }
             }
             // probabilities, their sums, weights in the range of f16
-            float f, un;
-            f16_factor(vtop, kWeightBits, f, un);
-            const float vf = vs * f;
             if (draft) {
 #pragma unroll
                 for (int x = 0; x < QC / 2; ++x) {
@@ -860,10 +888,13 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 if (lane % Share == 0) xl[quarter * QC + lane / Share] = z[0];
                 if (!meet()) break;
                 float sum = 0.0f;
+                int sx = 0;
                 if (lane < QC) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) sum += xl[q * QC + lane];
-                    bd[lane] = d.nsplit > 1 ? 1.0f : sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
+                    // (a split's sum is brought to [1, 2): h follows the values, and the joining takes powers of 2^h)
+                    sx = sum > 0.0f && sum < INFINITY ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
+                    bd[lane] = d.nsplit > 1 ? __int_as_float((127 - sx) << 23) : sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
                 }
                 __syncwarp();
                 const int mine_col = part * QC + (lane & (QC - 1));
@@ -880,8 +911,8 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                     }
                 }
                 if (d.nsplit > 1 && quarter == 0 && lane < QC && mine_col < d.cols) {
-                    mine_at[dh] = unset ? -INFINITY : h;
-                    mine_at[dh + 1] = sum;
+                    mine_at[dh] = unset ? -INFINITY : h + (float)sx;
+                    mine_at[dh + 1] = sum * __int_as_float((127 - sx) << 23);
                 }
             }
             arrive_warp(&tfree[t & (kTreeRing - 1)]);

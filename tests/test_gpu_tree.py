@@ -243,6 +243,82 @@ def test_small_and_large_value_scales(torch, rt):
         check_attention(torch, rt, c)
 
 
+def attend64_by_sum(torch, c, rows, bits):
+    """(out, tolerance) [len(rows), H, d] in 64 bits of rows of one sequence (c has no other), where value scales differ by up
+    to 2^bits. The tolerance is attend64's without the dropped weights, which are relative to all values there are; instead
+    a weight may be off by 2^-30 of the largest power of two in p |v| over what the row sees (half a step of the smaller f16,
+    2^-25, where the largest is brought to 2^5 or more), that is 2^-29 of its largest p |v| for each of its keys; and the exponents' arguments lie up to `bits`
+    from their base, which is rounded to u of itself, numerator and denominator."""
+    kv, H, KVH, d, tree = c["kv"], c["H"], c["KVH"], c["dh"], c["tree"]
+    (r,), (n,), G = c["rows"], c["cached"], H // KVH
+    ck, cv, there = held(torch, kv, c["table"], 0, n)
+    k = torch.cat((ck, c["k"][:r].reshape(r, KVH, d).double())).repeat_interleave(G, 1).transpose(0, 1)      # [H, n + r, d]
+    v = torch.cat((cv, c["v"][:r].reshape(r, KVH, d).double())).repeat_interleave(G, 1).transpose(0, 1)
+    mine = torch.tensor(rows, device="cuda")
+    words = tree.seen[mine, None] >> torch.arange(r, device="cuda") & 1
+    sees = torch.cat((there[None].expand(len(rows), -1), words.bool()), 1)[None]
+    q = c["q"][:r].reshape(r, H, d).double()[mine].transpose(0, 1)
+    score = (q @ k.transpose(1, 2)).masked_fill(~sees, -math.inf)
+    p = torch.softmax(score, -1)
+    mag = (q.abs() @ k.abs().transpose(1, 2)).masked_fill(~sees, 0.0)
+    e = (d / 4 + 24) * U * mag.amax(-1, keepdim=True)
+    top = score.amax(-1, keepdim=True)
+    spread = (top - score.masked_fill(~sees, math.inf).amin(-1, keepdim=True)).clamp(0, 100)
+    m = n + r
+    tol = (2 * e + (2 * spread + 2 * bits + 80 + 12 * math.sqrt(m) + m / 128) * U) * (p @ v.abs())
+    tol = tol + m * 2.0 ** -29 * (p * v.abs().amax(-1)[:, None]).amax(-1, keepdim=True)
+    return (p @ v).transpose(0, 1), tol.transpose(0, 1)
+
+
+@pytest.mark.parametrize("cached", [0, 30, 700])
+@pytest.mark.parametrize("factor", [1e4, 1e6, 1e10, 1e20])
+@pytest.mark.parametrize("H,KVH,dh", [(4, 2, 128), (4, 4, 64), (2, 1, 256), (16, 2, 64)])
+def test_large_values_of_a_row_cost_only_who_sees_it(torch, rt, H, KVH, dh, cached, factor):
+    """A star whose row 3 has values far above the others': its siblings do not see it."""
+    c = make(torch, rt, [9], [cached], H, KVH, dh, 16, seed=cached + dh, kind="star")
+    c["v"][3] *= factor
+    out = attend(rt, c).reshape(9, H, dh)
+    others = [i for i in range(9) if i != 3]
+    want, tol = attend64_by_sum(torch, c, others, math.log2(factor) + 4)
+    close(out[others], want, tol)
+    want, tol = attend64_by_sum(torch, c, [3], math.log2(factor) + 4)
+    close(out[3:4], want, tol)
+
+
+@pytest.mark.parametrize("where", [0, 17, 40])
+@pytest.mark.parametrize("bits", [14, 20, 40, 70])
+@pytest.mark.parametrize("away", [0.0, 0.35, 2.0])
+@pytest.mark.parametrize("H,KVH,dh", [(4, 2, 128), (16, 2, 64)])
+def test_large_values_of_cached_keys(torch, rt, H, KVH, dh, away, bits, where):
+    """A block of the cache with value scales 2^bits times the others': at a probability of nothing, at one that about makes up
+    for it, and at the others' own."""
+    c = make(torch, rt, [8], [700], H, KVH, dh, 16, seed=bits + where)
+    kv = c["kv"]
+    c["q"].copy_(dh ** -0.5 * (1 + 0.1 * c["q"] * dh ** 0.5))
+    page = int(c["table"][0, where])
+    kv.v_scale[page, :, 0] *= 2.0 ** bits
+    if away:                                                       # scores of about -away * bits * 2 nats
+        kv.k[page] = -127
+        kv.k_scale[page, :, 0] = away * bits * 2 / (127 * dh ** 0.5)
+    want, tol = attend64_by_sum(torch, c, list(range(8)), bits + 4)
+    close(attend(rt, c).reshape(8, H, dh), want, tol)
+
+
+@pytest.mark.parametrize("small,large", [(2.0 ** -60, 1.0), (2.0 ** -30, 2.0 ** 40), (0.0, 1.0)])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("cached", [300, 5000])
+def test_values_that_grow_or_shrink_along_a_sequence(torch, rt, cached, first, small, large):
+    """Half of the cached keys have tiny values (or none): their probability counts all the same, in one split and in several."""
+    c = make(torch, rt, [8], [cached], 8, 2, 64, 16, seed=cached)
+    half = c["table"][0, :-(-cached // 16)].long()
+    half = half[:len(half) // 2] if first else half[len(half) // 2:]
+    c["kv"].v_scale *= large
+    c["kv"].v_scale[half] *= small / large
+    c["v"].mul_(large)
+    want, tol = attend64_by_sum(torch, c, list(range(8)), 74)
+    close(attend(rt, c).reshape(8, 8, 64), want, tol)
+
+
 def test_pages_outside_the_pool_are_left_out(torch, rt):
     c = make(torch, rt, [10, 12], [400, 500], 8, 2, 128, 16, seed=8)
     c["table"][0, 3], c["table"][0, 24], c["table"][1, 0], c["table"][1, 8] = -1, 1 << 30, c["kv"].n_pages, -(1 << 31)
