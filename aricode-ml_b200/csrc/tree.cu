@@ -150,20 +150,25 @@ int b2_tree_accept(const b2_tree_rows* tree, const float* logits, int64_t ld, in
     TreeAcceptParams p{};
     if (!tree_view(fn, tree, p.r)) return B2_E_INVALID;
     if (vocab <= 0 || vocab > (1 << 30) || ld < vocab) return refuse(fn, "vocab must be 1 to 2^30, ld hold a row");
-    if (p.r.n_rows == 0 || p.r.n_seq == 0) return B2_OK;
-    if (!logits || !tokens || !kept_start || !kept_len || !kept_rows || !kept_ids || !al4(logits) || !al4(tokens) ||
-        !al4(kept_start) || !al4(kept_len) || !al4(kept_rows) || !al4(kept_ids) || !al4(err))
+    const int64_t n = p.r.n_rows, ns = p.r.n_seq;
+    const bool none = n == 0 || ns == 0;                           // no paths: sums and lengths alone
+    if (none && (!tree->row_start || (ns && !tree->kv_len))) return B2_OK;
+    if (!kept_start || (ns && !kept_len) || !al4(kept_start) || !al4(kept_len) || !al4(err) ||
+        (none ? !al4(tree->row_start) || !al4(tree->kv_len)
+              : !logits || !tokens || !kept_rows || !kept_ids || !al4(logits) || !al4(tokens) || !al4(kept_rows) || !al4(kept_ids)))
         return refuse(fn, "logits, tokens and the kept arrays must be set, 4-byte aligned");
     auto words = [](const void* x, int64_t n) { return Span{static_cast<const float*>(x), n, n}; };
-    const int64_t n = p.r.n_rows, ns = p.r.n_seq;
     const Span outs[4] = {words(kept_start, ns + 1), words(kept_len, ns), words(kept_rows, n), words(kept_ids, n)};
     const Span ins[4] = {words(tree->row_start, ns + 1), words(tree->kv_len, ns), words(tree->seen, 2 * n), words(tokens, n)};
-    for (int i = 0; i < 4; ++i) {
-        bool bad = overlap({logits, ld, vocab}, {outs[i].p, 0, outs[i].width}, p.r.n_rows);
-        for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < (none ? 2 : 4); ++i) {
+        bool bad = !none && overlap({logits, ld, vocab}, {outs[i].p, 0, outs[i].width}, n);
+        for (int j = 0; j < (none ? 2 : 4); ++j)
             bad = bad || (j > i && overlap(outs[i], outs[j], 1)) || (overlap(outs[i], ins[j], 1) && !(i == 1 && j == 1 && same(outs[i], ins[j])));
         if (bad) return refuse(fn, "a kept array overlaps an input (other than kept_len being kv_len) or another one");
     }
+    p.kept_start = kept_start; p.kept_len = kept_len; p.err = err;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (none) return status(fn, launch_ex(tree_none_kernel, dim3((unsigned)(ns / 256 + 1)), dim3(256), 0, s, true, p));
     p.splits = accept_splits(tree, vocab);
     const size_t need = accept_bytes(tree, p.splits);
     if (!workspace || !al16(workspace) || workspace_bytes < need)
@@ -171,12 +176,10 @@ int b2_tree_accept(const b2_tree_rows* tree, const float* logits, int64_t ld, in
     p.seen = reinterpret_cast<const long long*>(tree->seen);
     p.logits = logits; p.ld = ld; p.vocab = vocab;
     p.chunk = ((vocab + p.splits - 1) / p.splits + 3) / 4 * 4;
-    p.tokens = tokens; p.kept_start = kept_start; p.kept_len = kept_len; p.kept_rows = kept_rows; p.kept_ids = kept_ids;
+    p.tokens = tokens; p.kept_rows = kept_rows; p.kept_ids = kept_ids;
     p.best = static_cast<unsigned long long*>(workspace);
     p.paths = p.best + (size_t)p.r.n_rows * p.splits;
     p.ids = reinterpret_cast<int*>(p.paths + p.r.n_seq);
-    p.err = err;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = launch_ex(tree_argmax_kernel, dim3((unsigned)p.r.n_rows * p.splits), dim3(256), 0, s, true, p);
     if (e == cudaSuccess) e = launch_ex(tree_path_kernel, dim3(1), dim3(1024), 0, s, true, p);
     return status(fn, e);

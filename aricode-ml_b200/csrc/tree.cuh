@@ -64,6 +64,17 @@ static __global__ void __launch_bounds__(256) tree_argmax_kernel(const __grid_co
     }
 }
 
+// A call without rows: paths of nothing.
+static __global__ void __launch_bounds__(256) tree_none_kernel(const __grid_constant__ TreeAcceptParams p) {
+    after_previous();
+    const int s = blockIdx.x * 256 + threadIdx.x;
+    if (s > p.r.n_seq) return;
+    p.kept_start[s] = 0;
+    if (s == p.r.n_seq) return;
+    p.kept_len[s] = p.r.kv_len[s];
+    if (p.r.row_start[s + 1] < p.r.row_start[s]) set_err(p.err, B2_DEV_ERR_BAD_ROWS);
+}
+
 // The paths: one CTA, a warp a sequence at a time, two rows a lane; then the sums of their
 // lengths, and the kept rows in order. A path's rows ascend, so a path is a 64-bit word. Bound by latency
 // (48 sequences: 8.5 us).

@@ -441,7 +441,9 @@ int b2_attn_tree_i8(const b2_kv_pages* kv, const b2_tree_rows* tree, const float
  * [n_seq] = kv_len + path length (may be kv_len itself); kept_rows and kept_ids [n_rows],
  * path after path: the rows of the call and their ids, of which the last of a path is the
  * next token. Entries behind the last path stay as they were. Where a start falls (flagged),
- * rows from row_start[n_seq] on are left out. page_table is not used.
+ * rows from row_start[n_seq] on are left out. page_table is not used. Without rows or
+ * sequences kept_start becomes zeros and kept_len kv_len, from row_start and kv_len alone
+ * (where these are NULL too, nothing is done).
  * workspace: b2_tree_accept_workspace() bytes, 16-byte aligned, no initialisation; calls
  * that may overlap on the GPU need one each. */
 size_t b2_tree_accept_workspace(const b2_tree_rows* tree, int vocab);

@@ -627,6 +627,25 @@ def test_ids_are_of_rows_whose_logits_were_looked_at(torch, rt, starts):
         assert kept.rows.tolist() == flat + [-7] * (n - total) and kept.ids.tolist() == [ids[r] for r in flat] + [-7] * (n - total)
 
 
+@pytest.mark.parametrize("n_seq,n_rows", [(0, 0), (0, 3), (1, 0), (3, 0), (700, 0)])
+@pytest.mark.parametrize("own_lengths", [True, False])
+def test_acceptance_of_no_rows(torch, rt, n_seq, n_rows, own_lengths):
+    """Sums of nothing, and the lengths as they were."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens = [5 + s for s in range(n_seq)]
+    tree = rt.TreeRows(torch.zeros(n_seq + 1, **i32), torch.tensor(lens, **i32), torch.zeros(n_seq, 2, **i32),
+                       torch.ones(n_rows, dtype=torch.int64, device="cuda"), n_rows=n_rows)
+    kept = rt.TreeKept(tree, start=torch.full((n_seq + 1,), -7, **i32), kv_len=tree.kv_len if own_lengths else torch.full((n_seq,), -7, **i32))
+    rt.tree_accept(tree, torch.randn(n_rows, 50, device="cuda"), torch.zeros(n_rows, **i32), kept)
+    assert kept.start.tolist() == [0] * (n_seq + 1) and kept.kv_len.tolist() == lens and tree.kv_len.tolist() == lens
+    tree.check()
+    if n_seq:
+        tree.row_start[0] = 2
+        rt.tree_accept(tree, torch.randn(n_rows, 50, device="cuda"), torch.zeros(n_rows, **i32), kept)
+        with pytest.raises(rt.B2Error, match="row_start below"):
+            tree.check()
+
+
 def test_captured_acceptance(torch, rt):
     tree, logits, parents, start, tokens = accept_case(torch, rt, [9, 12], 5000, seed=6)
     tok = torch.tensor(tokens, dtype=torch.int32, device="cuda")

@@ -128,6 +128,15 @@ def test_nothing_to_do_is_no_error(pkg):
     assert gemv(rt, m=0, W=None) == 0 and gemv(rt, T=0, X=None) == 0
 
 
+@pytest.mark.parametrize("bad", [dict(start=None), dict(kv_len=None), dict(start=4 * A + 2), dict(kv_len=A + 6), dict(err=A + 1),
+                                 dict(start=A), dict(start=A + 8), dict(kv_len=A + 4), dict(kv_len=4 * A + 8)])
+def test_bad_acceptance_of_no_rows_is_refused(pkg, bad):
+    """Sums and lengths are written then too: 2 sequences, row_start and kv_len at A."""
+    a = dict(logits=None, tokens=None, rows=None, ids=None, ws=None)
+    assert accept(pkg.runtime, tree(pkg.runtime, n_rows=0), **{**a, **bad}) == -1
+    assert accept(pkg.runtime, tree(pkg.runtime, n_rows=0, row_start=A + 2), **a) == -1
+
+
 def test_null_structs_are_refused(pkg):
     rt = pkg.runtime
     assert attend(rt, None, tree(rt)) == -1 and attend(rt, pages(rt), None) == -1 and accept(rt, None) == -1
