@@ -93,7 +93,8 @@ cudaError_t launch_gemm(const GroupParams& g, int group, bool bf16, int sms, cud
     GemmParams p{};
     EncodeTiled enc = tensor_map_encoder();
     if (!enc) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)g.ld, (cuuint64_t)g.m}, strides[1] = {(cuuint64_t)g.ld};
+    // (a row's own bytes and no more: rows may be columns of a wider matrix, and the last one end with it)
+    const cuuint64_t dims[2] = {((cuuint64_t)g.n + 1) / 2, (cuuint64_t)g.m}, strides[1] = {(cuuint64_t)g.ld};
     const cuuint32_t box[2] = {64, 128}, step[2] = {1, 1};
     if (enc(&p.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(g.W), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)

@@ -78,6 +78,25 @@ def test_bias_strides_and_rows_of_a_wider_buffer(torch, rt, T):
     assert bool((big == 7.0).all())
 
 
+@pytest.mark.parametrize("n", [33, 160, 1000, 1120])
+@pytest.mark.parametrize("T", [1, 5, 9, 20, 64])
+def test_columns_at_the_end_of_a_wider_matrix(torch, rt, T, n):
+    """W as the last columns of a wider matrix that ends with its memory: 16-byte aligned rows that are `wide` bytes apart
+    (through the C call: the wrapper takes whole rows)."""
+    m, group, wide = 300, 32, 4096
+    big = torch.randint(0, 256, (8192, wide), device="cuda", dtype=torch.uint8)            # 32 MB: memory of its own
+    own = (n + 31) // 32 * 16
+    W, scale, x = make(torch, m, n, T, group, torch.float32, seed=n + T)
+    at = (8192 - m) * wide + wide - own
+    view = big.view(-1)[at:]
+    big[8192 - m:, wide - own:] = W[:, :own]
+    y, ws = torch.empty(T, m, device="cuda"), rt.gemv_i4_groups_workspace(T, n)
+    rt.check(rt.lib().b2_gemv_i4_groups(view.data_ptr(), wide, scale.data_ptr(), scale.shape[1], 0, group, x.data_ptr(), n, None,
+                                        y.data_ptr(), m, m, n, T, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    want, tol = product64(torch, W, scale, x, group)
+    close(y, want, tol)
+
+
 def test_one_vector_without_a_row(torch, rt):
     W, scale, x = make(torch, 50, 300, 1, 128, torch.bfloat16)
     want, tol = product64(torch, W, scale, x, 128)
