@@ -13,6 +13,7 @@ namespace {
 constexpr int kVectors = 8;              // of a launch of the first kind, for up to so many vectors in all
 constexpr int kGemmVectors = 64;         // of the second
 constexpr size_t kSmem = 227 * 1024;
+constexpr int kMost = 0x7fff0000;        // of m, n and T: what goes past them by a tile or a round of tiles stays in 32 bits
 
 int fragment_tiles(int T) { return (3 * T + 7) / 8; }          // B columns: three digits of each vector
 
@@ -23,7 +24,7 @@ int columns(int NT, int n) {
     int parts = 1, c = n;
     while (smem_bytes(NT, c) > kSmem) {
         ++parts;
-        c = ((n + parts - 1) / parts + 511) / 512 * 512;
+        c = (int)(((((long long)n + parts - 1) / parts + 511) / 512) * 512);
     }
     return c;
 }
@@ -115,7 +116,7 @@ cudaError_t launch_gemm(const GroupParams& g, int group, bool bf16, int sms, cud
 extern "C" {
 
 size_t b2_gemv_i4_groups_workspace(int T, int n) {
-    if (T <= 2 || n <= 0) return 0;
+    if (T <= 2 || n <= 0 || T > kMost || n > kMost) return 0;
     if (T > kVectors) return gemm_bytes(gemm_vectors(T), n, sm_count());
     return (size_t)GroupSmem<1>::blocks(n) * fragment_tiles(T) * (1024 + 32);
 }
@@ -126,6 +127,7 @@ int b2_gemv_i4_groups(const uint8_t* W, int64_t ld, const void* scale, int64_t l
     const char* fn = "b2_gemv_i4_groups";
     if (group != 32 && group != 64 && group != 128) return refuse(fn, "group must be 32, 64 or 128");
     if (m < 0 || n <= 0 || T < 0) return refuse(fn, "m and T must not be negative, n positive");
+    if (m > kMost || n > kMost || T > kMost) return refuse(fn, "m, n and T: at most 2^31 - 2^16");
     if (m == 0 || T == 0) return B2_OK;
     if (!W || !al16(W) || ld % 16 || ld < ((int64_t)n + 1) / 2) return refuse(fn, "W: 16-byte aligned, ld a multiple of 16 that holds a row");
     const int64_t groups = ((int64_t)n + group - 1) / group;

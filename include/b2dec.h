@@ -214,8 +214,9 @@ int b2_gemv_i4_rowscale(const uint8_t* W, int64_t ld, const float* scale, const 
  * rows ld bytes apart, 16-byte aligned, ld % 16 == 0, what lies past n is not used.
  * group: 32, 64 or 128 columns, the last one may be shorter. scale [m][lds] f32, or
  * bf16 where scale_bf16 is set. X [T][ldx], Y [T][ldy] f32, 4-byte aligned; Y overlaps
- * nothing that is read. For one token or a few (a tree of drafted tokens, a few
- * sequences); more than 64 read the weights once for every 64. Precision: codes are exact.
+ * nothing that is read. m, n and T up to 2^31 - 2^16. For one token or a few (a tree of
+ * drafted tokens, a few sequences); more than 64 read the weights once for every 64.
+ * Precision: codes are exact.
  * Up to eight vectors: a vector's elements are held to 2^-24 of the largest of each 128
  * neighbours, products and their sums over a group are exact, the rest is f32. More: each
  * element to 2^-22 of itself or 2^-38 of the largest of its 128 neighbours, whichever is

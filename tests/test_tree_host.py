@@ -116,6 +116,15 @@ def test_bad_products_are_refused(pkg, bad):
     assert gemv(rt, **bad) == -1 and rt.last_error().startswith("b2_gemv_i4_groups")
 
 
+@pytest.mark.parametrize("big", [(1 << 31) - 1, (1 << 31) - 65535])
+def test_products_beyond_32_bits_are_refused(pkg, big):
+    """Sizes whose last tile or part would be counted past 2^31."""
+    rt = pkg.runtime
+    for kw in (dict(n=big, ld=1 << 30, lds=1 << 26, ldx=1 << 31), dict(m=big, ldy=1 << 31), dict(T=big), dict(T=1, n=big, ld=1 << 30, lds=1 << 26, ldx=1 << 31)):
+        assert gemv(rt, **kw) == -1 and "at most" in rt.last_error()
+    assert rt.lib().b2_gemv_i4_groups_workspace(big, 128) == 0 and rt.lib().b2_gemv_i4_groups_workspace(3, big) == 0
+
+
 def test_nothing_to_do_is_no_error(pkg):
     rt = pkg.runtime
     none = dict(row_start=None, kv_len=None, page_table=None, seen=None, max_pages=0)
