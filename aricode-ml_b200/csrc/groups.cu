@@ -139,6 +139,11 @@ int b2_gemv_i4_groups(const uint8_t* W, int64_t ld, const void* scale, int64_t l
     const size_t need = b2_gemv_i4_groups_workspace(T, n);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+    const Bytes read[] = {rows_bytes(W, ld, ((int64_t)n + 1) / 2, m, 1), rows_bytes(scale, lds, groups, m, scale_bf16 ? 2 : 4),
+                          {bias, 4ll * m}, rows_bytes(X, ldx, n, T, 4)};
+    const Bytes y = rows_bytes(Y, ldy, m, T, 4), ws = {workspace, (int64_t)need};
+    if (touch(y, {read[0], read[1], read[2], ws})) return refuse(fn, "Y overlaps W, scale, bias or the workspace");
+    if (touch(ws, read)) return refuse(fn, "the workspace overlaps an input");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(), unit = scale_bf16 ? 2 : 4;
     if (T > kVectors) {

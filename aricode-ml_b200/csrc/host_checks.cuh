@@ -48,6 +48,28 @@ inline bool overlap(const Span& a, const Span& b, int64_t n) {
     return at < a.width || at + b.width > a.ld;
 }
 
+// memory from the first to the last byte of something, and whether two such share a byte
+struct Bytes {
+    const void* p;
+    int64_t n;
+};
+
+inline bool touch(const Bytes& a, const Bytes& b) {
+    if (!a.p || !b.p || a.n <= 0 || b.n <= 0) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x < y ? y - x < (uint64_t)a.n : x - y < (uint64_t)b.n;
+}
+
+template <int N>
+inline bool touch(const Bytes& a, const Bytes (&others)[N]) {
+    for (const Bytes& b : others)
+        if (touch(a, b)) return true;
+    return false;
+}
+
+// n rows of `width` elements of `size` bytes, ld apart
+inline Bytes rows_bytes(const void* p, int64_t ld, int64_t width, int64_t n, int64_t size) { return {p, ((n - 1) * ld + width) * size}; }
+
 inline bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld; }
 
 // the current device's SMs, looked up once a device

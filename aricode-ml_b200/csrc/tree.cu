@@ -130,6 +130,15 @@ int b2_attn_tree_i8(const b2_kv_pages* kv, const b2_tree_rows* tree, const float
     const size_t need = tree_bytes(p);
     if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+    const int64_t n = p.r.n_rows, codes = (int64_t)kv->n_pages * kv->n_kv_heads * kv->page_size * kv->d_head, scales = codes / kv->d_head / kKvBlock * 4;
+    const Bytes read[] = {{kv->k, codes}, {kv->v, codes}, {kv->k_scale, scales}, {kv->v_scale, scales},
+                          {tree->row_start, 4 * (p.r.n_seq + 1ll)}, {tree->kv_len, 4ll * p.r.n_seq},
+                          {tree->page_table, 4ll * p.r.n_seq * p.r.max_pages}, {tree->seen, 8 * n}};
+    const Bytes rows[] = {rows_bytes(q, ldq, width, n, 4), rows_bytes(k, ldk, kvw, n, 4), rows_bytes(v, ldv, kvw, n, 4),
+                          rows_bytes(out, ldo, width, n, 4)};
+    const Bytes ws = {workspace, (int64_t)need};
+    if (touch(rows[3], read)) return refuse(fn, "out overlaps the cache or the tree");
+    if (touch(ws, read) || touch(ws, rows)) return refuse(fn, "the workspace overlaps an input or out");
     p.part = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (p.c.dh <= 64) return status(fn, nc == 16 ? launch_tree<64, 16>(p, s) : launch_tree<64, 64>(p, s));
@@ -173,6 +182,10 @@ int b2_tree_accept(const b2_tree_rows* tree, const float* logits, int64_t ld, in
     const size_t need = accept_bytes(tree, p.splits);
     if (!workspace || !al16(workspace) || workspace_bytes < need)
         return refuse(fn, "needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+    const Bytes ws = {workspace, (int64_t)need}, rows = rows_bytes(logits, ld, vocab, n, 4);
+    bool bad = touch(ws, rows);
+    for (int i = 0; i < 4; ++i) bad = bad || touch(ws, {outs[i].p, 4 * outs[i].width}) || touch(ws, {ins[i].p, 4 * ins[i].width});
+    if (bad) return refuse(fn, "the workspace overlaps an input or a kept array");
     p.seen = reinterpret_cast<const long long*>(tree->seen);
     p.logits = logits; p.ld = ld; p.vocab = vocab;
     p.chunk = ((vocab + p.splits - 1) / p.splits + 3) / 4 * 4;

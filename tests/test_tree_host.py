@@ -125,6 +125,39 @@ def test_products_beyond_32_bits_are_refused(pkg, big):
     assert rt.lib().b2_gemv_i4_groups_workspace(big, 128) == 0 and rt.lib().b2_gemv_i4_groups_workspace(3, big) == 0
 
 
+@pytest.mark.parametrize("bad", [dict(Y=A), dict(Y=A + 7 * 64 - 4, scale=5 * A), dict(W=5 * A, Y=A + 6 * 4), dict(W=5 * A, scale=6 * A, bias=3 * A + 4),
+                                 dict(Y=4 * A), dict(Y=4 * A - 4), dict(ws=A), dict(ws=2 * A + 2 * 128 * 4), dict(ws=3 * A + 80),
+                                 dict(ws=5 * A, bias=5 * A + 16)])
+def test_products_whose_memory_overlaps_are_refused(pkg, bad):
+    """W, scale at A, X at 2 A, Y at 3 A, the workspace at 4 A: 7 rows, 128 columns, 3 vectors."""
+    assert gemv(pkg.runtime, **bad) == -1 and "overlaps" in pkg.runtime.last_error()
+
+
+@pytest.mark.parametrize("cache", [dict(k=4 * A), dict(v=4 * A + 4096), dict(k=4 * A - 8192 + 16), dict(k_scale=4 * A + 64), dict(v_scale=4 * A - 28)])
+def test_attention_into_the_cache_is_refused(pkg, cache):
+    """out at 4 A: 5 rows of 256; 4 pages of 16 x 2 x 64 codes, 8 scales each."""
+    rt = pkg.runtime
+    assert attend(rt, pages(rt, **cache), tree(rt)) == -1 and "out overlaps" in rt.last_error()
+
+
+@pytest.mark.parametrize("t", [dict(row_start=4 * A + 8), dict(kv_len=4 * A - 4), dict(page_table=4 * A + 16), dict(seen=4 * A - 32)])
+def test_attention_into_the_tree_is_refused(pkg, t):
+    rt = pkg.runtime
+    assert attend(rt, pages(rt), tree(rt, **t)) == -1 and "out overlaps" in rt.last_error()
+
+
+@pytest.mark.parametrize("at", [A, 2 * A + 16, 3 * A, 4 * A + 32, A + 8000])
+def test_a_workspace_over_what_a_call_uses_is_refused(pkg, at):
+    """Calls that need one: attention of many pages, acceptance."""
+    rt = pkg.runtime
+    t = tree(rt, max_pages=64)
+    assert rt.lib().b2_attn_tree_i8_workspace(C.addressof(pages(rt)), C.addressof(t), 4) > 0
+    assert attend(rt, pages(rt), t, ws=at) == -1 and "workspace overlaps" in rt.last_error()
+    kept = dict(start=4 * A, kv_len=5 * A, rows=6 * A, ids=7 * A)
+    for ws in (2 * A + 48, 3 * A, 4 * A, 5 * A, 6 * A - 16, 7 * A + 16, A):
+        assert accept(rt, tree(rt), ws=ws, **kept) == -1 and "workspace overlaps" in rt.last_error()
+
+
 def test_nothing_to_do_is_no_error(pkg):
     rt = pkg.runtime
     none = dict(row_start=None, kv_len=None, page_table=None, seen=None, max_pages=0)
