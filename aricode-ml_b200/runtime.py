@@ -821,8 +821,9 @@ class TreeRows:
     """The drafted rows of a call (b2_tree_rows): int32 tensors row_start [n_seq + 1], kv_len [n_seq] (cached keys, the
     drafted rows not among them) and page_table [n_seq, max_pages], and seen [n_rows] int64 (bit j of a row's word: it sees
     row j of its sequence; tree_seen makes them). They are read when the kernels run: refill them in place to replay a
-    captured call. max_keys bounds every kv_len (0: what the table can hold); max_rows says how many rows the longest
-    sequence has, if that is known (0: up to 64)."""
+    captured call. max_keys bounds every kv_len for as long as these are used, also what tree_accept makes of them (0: what
+    the table can hold; keys past it are left out and flagged); max_rows says how many rows the longest sequence has, if
+    that is known (0: up to 64)."""
 
     def __init__(self, row_start, kv_len, page_table, seen, n_rows, max_keys=0, max_rows=0):
         import torch
