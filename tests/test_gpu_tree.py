@@ -439,6 +439,63 @@ def test_what_behind_a_call_reads_and_writes_is_in_order(torch, rt):
         close(out.reshape(128, 8, 128), want, tol)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dh,KVH", [(64, 1), (128, 4), (256, 2)])
+def test_what_is_not_finite_in_calls_with_splits(torch, rt, dh, KVH, bad):
+    """A query and a drafted value: the partial results of everybody else join to what they were."""
+    c = make(torch, rt, [12], [6000], 4, KVH, dh, 16, seed=dh)
+    assert rt.attn_tree_workspace(c["kv"], c["tree"], 4).numel() > 0
+    want, tol = attend64(torch, c)
+    c["q"][5, dh + 3] = bad                                        # head 1
+    c["v"][2, 7] = bad                                             # KV head 0
+    out = attend(rt, c).reshape(12, 4, dh)
+    words = rt.tree_seen(c["parents"][0])
+    for i in range(12):
+        for h in range(4):
+            if (i == 5 and h == 1) or (words[i] >> 2 & 1 and h < 4 // KVH):
+                assert bool(out[i, h].isnan().all()), (i, h)
+            else:
+                close(out[i, h], want[i, h], tol[i, h])
+
+
+def test_threads_with_attention_and_acceptance(torch, rt):
+    """Threads on streams of their own, each with all the shapes of the kernel, none with a workspace made before."""
+    import threading
+    cases = [make(torch, rt, rows, cached, H, KVH, dh, 16, seed=i) for i, (rows, cached, H, KVH, dh) in enumerate(
+        (([5], [3000], 4, 4, 64), ([40, 3], [900, 20], 4, 1, 64), ([9], [500], 4, 4, 128), ([33], [2500], 8, 2, 128), ([4], [700], 2, 2, 256),
+         ([30], [900], 2, 1, 208)))]
+    want = [attend64(torch, c) for c in cases]
+    accepts = [accept_case(torch, rt, [9, 3], 5000, seed=i) for i in range(len(cases))]
+    tokens = [torch.tensor(a[4], dtype=torch.int32, device="cuda") for a in accepts]
+    kept = [rt.tree_accept(a[0], a[1], t).rows.tolist() for a, t in zip(accepts, tokens)]
+    torch.cuda.synchronize()
+    got, failed = [[] for _ in cases], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for n in range(18):
+                    j = (i + n) % len(cases)
+                    k = rt.tree_accept(accepts[i][0], accepts[i][1], tokens[i])
+                    got[i].append((j, attend(rt, cases[j]), k))
+            s.synchronize()
+        except Exception as e:                                     # noqa: BLE001 (told by the assertion)
+            failed.append(repr(e))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for i, outs in enumerate(got):
+        assert len(outs) == 18
+        for j, out, k in outs:
+            c = cases[j]
+            close(out.reshape(sum(c["rows"]), c["H"], c["dh"]), *want[j])
+            assert k.rows.tolist() == kept[i]
+
+
 # ------------------------------------------------------------------ acceptance
 def accept_plain(parents, tokens, ids):
     path, at = [], 0 if parents else -1
@@ -733,6 +790,31 @@ def test_an_index_outside_the_rows_writes_zeros(torch, rt, eps):
     x, y = (rt.kv_read_i8(c, rt.KVRows(kept.start, kept.kv_len, kept.tree.page_table, n_rows=12))[0] for c in (a, b))
     assert not x[3].any() and not x[8].any() and bool(((x - y).abs() <= 1e-4).all()) == (eps == EPS) or eps == 0.0
     assert not x.isnan().any()
+
+
+@pytest.mark.parametrize("eps", [EPS, 0.0])
+@pytest.mark.parametrize("dh", [64, 128, 256])
+def test_rows_of_a_bad_index_are_zeros_and_the_others_as_ever(torch, rt, eps, dh):
+    """With and without an eps beneath the square root (a missing row has none of its own): beside an append of the same
+    rows whose bad ones hold numbers, which share blocks with the others but not their norm; values bit for bit."""
+    (a, b), kept, k, v, pick = kept_case(torch, rt, [7, 5, 16], [20, 16, 32], 2, dh, 16, seed=dh)
+    bad = [3, 8]
+    kept.rows[bad[0]], kept.rows[bad[1]] = -1, k.shape[0]
+    gain = 1 + 0.1 * torch.randn(dh, device="cuda")
+    rt.kv_append_kept_i8(a, kept, k, v, k_gain=gain, eps=eps)
+    with pytest.raises(rt.B2Error, match="row index"):
+        a.check()
+    rows = rt.KVRows(kept.start, kept.kv_len, kept.tree.page_table, n_rows=28)
+    kb, vb = k[pick.long()].clone(), v[pick.long()].clone()
+    vb[bad] = 0
+    kb[bad] = 1e-3                                                 # normed, elements of about the gain: never a block's largest
+    rt.kv_append_i8(b, rows, kb, vb, k_gain=gain, eps=eps)
+    assert torch.equal(a.v, b.v) and torch.equal(a.v_scale, b.v_scale)
+    x, y = (rt.kv_read_i8(c, rows)[0] for c in (a, b))
+    good = [i for i in range(28) if i not in bad]
+    assert not x[bad].any() and bool(y[bad].any()) and not x.isnan().any()
+    # blocks without a bad row: the same codes; with one: scales may differ if the bad row held the largest, which it does not
+    assert torch.equal(x[good], y[good])
 
 
 def test_kept_rows_past_the_capacity_or_the_table(torch, rt):
