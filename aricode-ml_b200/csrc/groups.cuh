@@ -6,7 +6,7 @@
 // The codes are exact small integers, so a group's sum runs as an integer dot on the tensor
 // cores, with x split into three signed base-256 digits: X = rint(x f) = d2 65536 + d1 256
 // + d0, f from the largest of each 128 neighbours (a channel that stands out costs its
-// neighbours alone). The digit sums are exact in int32; each is scaled by s and 1 / f into a
+// neighbours alone). The digit sums are exact in int32; each is scaled by 256^e / f and s into a
 // f32 sum of its own, and the three are joined at the end.
 #pragma once
 #include "f16_pairs.cuh"
@@ -101,8 +101,8 @@ __device__ __forceinline__ void group_digits(const GroupParams& p, int t, int kb
         const int col = 3 * t + e;
         uint2* q = reinterpret_cast<uint2*>(frag + ((col >> 3) * 2 + (at.x >> 1)) * 32 + (col & 7) * 4 + at.y);
         q[at.x & 1] = make_uint2(even[e], odd[e]);
-        // the codes enter as 16 c; digit e counts 256^e, which the end multiplies in
-        if (w == 0) unit[col] = f > 0.0f ? fdiv(0.0625f, f) : f;
+        // the codes enter as 16 c; digit e counts 256^e
+        if (w == 0) unit[col] = f > 0.0f ? fdiv(e == 0 ? 0.0625f : e == 1 ? 16.0f : 4096.0f, f) : f;
     }
 }
 
@@ -234,8 +234,9 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
                             const f32x2 off = pack2(-12582912.0f, -12582912.0f);
                             const f32x2 v0 = add2(pack2(__int_as_float(c[0]), __int_as_float(c[1])), off);
                             const f32x2 v1 = add2(pack2(__int_as_float(c[2]), __int_as_float(c[3])), off);
-                            const float2 y0 = unpack2(fma2(v0, mul2(pack2(r0, r0), u2), pack2(acc[y][0], acc[y][1])));
-                            const float2 y1 = unpack2(fma2(v1, mul2(pack2(r1, r1), u2), pack2(acc[y][2], acc[y][3])));
+                            // (unit x scale first could be too small for f32 where their product with the sum is not)
+                            const float2 y0 = unpack2(fma2(mul2(v0, u2), pack2(r0, r0), pack2(acc[y][0], acc[y][1])));
+                            const float2 y1 = unpack2(fma2(mul2(v1, u2), pack2(r1, r1), pack2(acc[y][2], acc[y][3])));
                             acc[y][0] = y0.x; acc[y][1] = y0.y; acc[y][2] = y1.x; acc[y][3] = y1.y;
                         }
                     }
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
             const float* q = rw + (slot * p.warps_k * 16 + i % 16) * 8 * NT + 3 * v;
             float d0 = 0.0f, d1 = 0.0f, d2 = 0.0f;
             for (int w = 0; w < p.warps_k; ++w, q += 16 * 8 * NT) { d0 += q[0]; d1 += q[1]; d2 += q[2]; }
-            float y = ffma(d2, 65536.0f, ffma(d1, 256.0f, d0)), *out = p.y + (size_t)v * p.ldy + row;
+            float y = fadd(d2, fadd(d1, d0)), *out = p.y + (size_t)v * p.ldy + row;
             if (p.bias) y = fadd(y, p.bias[row]);
             *out = p.add ? fadd(*out, y) : y;
         }
@@ -559,8 +560,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
 #pragma unroll
                 for (int x = 0; x < C / 2; x += 2) {
                     const float4 uu = *reinterpret_cast<const float4*>(un + 2 * x);
-                    acc[x] = fma2(pack2(__uint_as_float(d[2 * x]), __uint_as_float(d[2 * x + 1])), mul2(pack2(uu.x, uu.y), pack2(s[g], s[g])), acc[x]);
-                    acc[x + 1] = fma2(pack2(__uint_as_float(d[2 * x + 2]), __uint_as_float(d[2 * x + 3])), mul2(pack2(uu.z, uu.w), pack2(s[g], s[g])),
+                    acc[x] = fma2(mul2(pack2(__uint_as_float(d[2 * x]), __uint_as_float(d[2 * x + 1])), pack2(uu.x, uu.y)), pack2(s[g], s[g]), acc[x]);
+                    acc[x + 1] = fma2(mul2(pack2(__uint_as_float(d[2 * x + 2]), __uint_as_float(d[2 * x + 3])), pack2(uu.z, uu.w)), pack2(s[g], s[g]),
                                       acc[x + 1]);
                 }
                 tc_fence_before();

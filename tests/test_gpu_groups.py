@@ -127,6 +127,18 @@ def test_ranges(torch, rt, factor):
     assert not y[2].any()
 
 
+@pytest.mark.parametrize("T", [1, 2, 5, 8, 9, 40])
+@pytest.mark.parametrize("x_factor,s_factor", [(1e-12, 1e-20), (1.0, 1e-30), (1e-30, 1.0), (1e-24, 1e-10), (1e25, 1e-30), (1e-30, 1e30), (1e30, 1e5)])
+def test_small_and_large_scales(torch, rt, T, x_factor, s_factor):
+    """Outputs down to 1e-33 from factors that are small each: as precise as any (what f32 cannot hold on the way, its last
+    digits below 2^-149, is left to it: a step for each group of each of three sums)."""
+    W, scale, x = make(torch, 40, 500, T, 32, torch.float32, seed=T)
+    x *= x_factor
+    scale *= s_factor
+    want, tol = product64(torch, W, scale, x, 32)
+    close(rt.gemv_i4_groups(W, scale, x, 32), want, tol + 3 * 16 * 2.0 ** -149)
+
+
 @pytest.mark.parametrize("T", [1, 2, 9, 30])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_what_is_not_finite_stays_in_its_vector(torch, rt, T, bad):
