@@ -10,8 +10,12 @@ using namespace b2;
 
 namespace {
 
-constexpr int kVectors = 8;              // of a launch of the first kind, for up to so many vectors in all
-constexpr int kGemmVectors = 64;         // of the second
+// Up to 8 vectors (three fragments of their digits) the first kind of kernel, else the second. 8 vectors by the first and
+// the second, us in a captured graph: 5632 x 2048, groups of 32 12 and 19; 4096 x 4096 12 and 18; 32000 x 4096 39 and 55;
+// 4096 x 11008, whose columns are two launches of the first then, 27 and 27. 3 vectors: 12 and 16, 12 and 16, 33 and 55, 21
+// and 25. (The first for more than 8, with more fragments, is not written.)
+constexpr int kVectors = 8;
+constexpr int kGemmVectors = 64;         // of a launch of the second kind
 constexpr size_t kSmem = 227 * 1024;
 constexpr int kMost = 0x7fff0000;        // of m, n and T: what goes past them by a tile or a round of tiles stays in 32 bits
 

@@ -34,7 +34,15 @@ bool tree_view(const char* fn, const b2_kv_pages* kv, const b2_tree_rows* t, Pag
 }
 
 // Columns of an item: 16 where no sequence has more (one token, short chains without shared heads), else as many
-// as the tensor memory and shared memory hold.
+// as the tensor memory and shared memory hold: 64, or 32 for d_head above 128. Items of 16 and of 64 (32), us in a captured
+// graph, by the columns (row, head) that a KV head has:
+//                                              16         32          48           64
+//   8 sequences, 4000 keys, 32 / 8 heads of 128   51  82   72  86    86   90    111   94
+//   32, 1152 keys, 32 / 8 heads of 128            53  88   76  94   107  100    125  107
+//   8, 4000 keys, 32 / 8 heads of 64              47  64   66  68    82   78    107   84
+//   8, 2000 keys, 16 / 4 heads of 256             39  49   57  51    66   76     84   78
+// (up to 32 columns several items of 16 would be as fast or faster below d_head 256). Longer: 16 sequences of up to 60 rows
+// over 4000 keys 261 and 208, 2 of 64 rows over 40 K keys, 32 / 4 heads of 64 755 and 341.
 int tree_columns(const TreeAttnParams& p, int max_rows) {
     const int rows = std::min(max_rows > 0 ? std::min(max_rows, kTreeRows) : kTreeRows, p.r.n_rows);
     return rows * p.G <= 16 ? 16 : p.c.dh > 128 ? 32 : 64;
@@ -42,7 +50,10 @@ int tree_columns(const TreeAttnParams& p, int max_rows) {
 
 // Keys of a split: so many items that the last round of the GPU is nearly full, in four to eight rounds (lengths
 // differ, and the host does not know them), of 256 keys at least; an item beside its keys costs about two tiles of them.
-// (Powers of two, eight rounds: 40 K keys, two sequences of 64 rows of 32 / 4 heads of 64 in 640 items 429 us.)
+// (Powers of two, eight rounds: 40 K keys, two sequences of 64 rows of 32 / 4 heads of 64 in 640 items 429 us. Eight to
+// sixteen rounds: the same 356 us instead of 320 in a captured graph; 4 of 8 rows over 20 K keys, 32 / 8 heads of 128, 143 instead of 133.
+// Two to four: 320 and 127; 16 of 40 rows over 3000 keys, all of one length, 236 instead of 272; sequences of different lengths
+// up to 4000 keys 208 either way. 148 SMs whatever the device has, so that the workspace is the same everywhere.)
 void tree_plan(TreeAttnParams& p, int nc) {
     const long long tiles = std::max((long long)p.r.n_rows * p.G / nc, (long long)std::min(p.r.n_seq, p.r.n_rows)) * p.c.KVH;
     const long long most = std::max(1ll, std::min((p.r.cap + 255ll) / 256, 1024ll)), keys = (p.r.cap + kTreeKeys - 1ll) / kTreeKeys;

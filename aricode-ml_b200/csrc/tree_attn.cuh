@@ -26,10 +26,10 @@
 // Measured (a call, us; bytes at 6.56 TB/s or operations at the bf16 rate allow the second figure):
 //   1 sequence of 5 rows over 639 keys, 32 / 32 heads of 128             13   0.8  latency of one item
 //   32 of 16 rows over 1152 keys, 32 / 32 heads of 128                  122    51  a tile's turn of the only place
-//     for keys: conversion 1500 clocks, scores 600, waits between warps 800; issue slots 70 %
-//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       209    18  the same with 64 columns
-//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    350    25  the softmax: 56 % of issue slots,
-//     11 K instructions of warps a tile of 128 keys x 64 columns, tensor pipe active 19 %
+//     for keys: conversion 1500 clocks, scores 600, waits between warps 800; issue slots 51 %
+//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       208    18  the same with 64 columns
+//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    341    25  the softmax: 59 % of issue slots,
+//     9.1 K instructions of warps a tile of 128 keys x 64 columns, tensor pipe active 20 %
 // Two groups of softmax warps with every other tile each and two places for queries: 137 instead of 130.
 #pragma once
 #include <type_traits>
@@ -870,17 +870,17 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 }
                 int keep = QC;
 #pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) {
+                for (int way = 16; way >= 1; way >>= 1) {
                     if (keep == 1) {
-                        z[0] += __shfl_xor_sync(0xffffffffu, z[0], o);
+                        z[0] += __shfl_xor_sync(0xffffffffu, z[0], way);
                         continue;
                     }
                     keep /= 2;
-                    const bool up = lane & o;
+                    const bool up = lane & way;
 #pragma unroll
                     for (int x = 0; x < QC / 2; ++x) {
                         if (x >= keep) break;
-                        const float give = __shfl_xor_sync(0xffffffffu, up ? z[x] : z[x + keep], o);
+                        const float give = __shfl_xor_sync(0xffffffffu, up ? z[x] : z[x + keep], way);
                         z[x] = (up ? z[x + keep] : z[x]) + give;
                     }
                 }
