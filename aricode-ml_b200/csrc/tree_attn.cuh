@@ -807,7 +807,11 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
 #pragma unroll
                 for (int x = 0; x < QC / 2; ++x) {
                     const float2 dd = *reinterpret_cast<const float2*>(bd + 2 * x), bb = *reinterpret_cast<const float2*>(bk + (t & 1) * 16 * QC + 2 * x);
-                    s[x] = add2(s[x], pack2(-dd.x, -dd.y));
+                    float2 y = unpack2(add2(s[x], pack2(-dd.x, -dd.y)));
+                    // (scores so large that their sums with ve are roundings of it could end above what the weights hold)
+                    if (y.x > kMoveBits - ve) y.x = kMoveBits - ve;
+                    if (y.y > kMoveBits - ve) y.y = kMoveBits - ve;
+                    s[x] = pack2(y.x, y.y);
                     l[x] = mul2(mul2(l[x], pack2(bb.x, bb.y)), pack2(bb.x, bb.y));      // (2^-by itself could leave f32's range)
                 }
             }
@@ -892,8 +896,9 @@ __global__ void __launch_bounds__((TreeShape<DP, NC>::Threads), 1) tree_attn_ker
                 if (lane < QC) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) sum += xl[q * QC + lane];
-                    // (a split's sum is brought to [1, 2): h follows the values, and the joining takes powers of 2^h)
-                    sx = sum > 0.0f && sum < INFINITY ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
+                    // (a split's sum is brought to [1, 2): h follows the values, and the joining takes powers of 2^h; where h
+                    // is a whole number to which another can be added)
+                    sx = sum > 0.0f && sum < INFINITY && fabsf(h) < 0x1p23f ? exponent_of(sum) : 0;
                     bd[lane] = d.nsplit > 1 ? __int_as_float((127 - sx) << 23) : sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
                 }
                 __syncwarp();

@@ -424,9 +424,9 @@ typedef struct b2_tree_rows {
  * and drafted keys and values are held to 2^-22 of each element or 2^-38 of the largest of
  * their row and head, whichever is more; a weight (probability times value scale) to 2^-22
  * of itself or 2^-30 of the largest weight of what its row sees, whichever is more, where the
- * value scales other than 0 lie within 2^80 of one another (a larger spread costs a row
- * bits even by values that it does not see); products and sums are f32. Outputs may not
- * overlap inputs.
+ * value scales other than 0 lie within 2^80 of one another and scores below 2^24 (beyond,
+ * a spread of value scales costs a row bits even by values that it does not see);
+ * products and sums are f32. Outputs may not overlap inputs.
  * workspace: b2_attn_tree_i8_workspace() bytes (may be 0), 16-byte aligned, no
  * initialisation; calls that may overlap on the GPU need one each. */
 size_t b2_attn_tree_i8_workspace(const b2_kv_pages* kv, const b2_tree_rows* tree, int n_heads);

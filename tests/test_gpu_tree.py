@@ -319,6 +319,52 @@ def test_values_that_grow_or_shrink_along_a_sequence(torch, rt, cached, first, s
     close(attend(rt, c).reshape(8, 8, 64), want, tol)
 
 
+@pytest.mark.parametrize("cached", [200, 5000])
+@pytest.mark.parametrize("code", [64, 100])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 27, 2.0 ** 32, 2.0 ** 66])
+def test_equal_scores_of_any_size(torch, rt, cached, code, size):
+    """All keys the same, scores of about +size or -size: the mean of the values, whatever the parts that they are summed in.
+    With codes of +-64 the sum of products is a power of two, so a score in base 2 is log2 e (as f32 has it) times one: exact
+    in f32, and every weight is the same. With others a score is rounded in an item's first tile (which finds the base) and
+    not in the next, where it is multiplied and subtracted in one: arguments differ by up to u of the score in base 2, a
+    weight by that times ln 2, numerator and denominator: 2 u size more of sum p |v|, which from 2^24 on says only that what
+    comes out is finite and no larger than the values."""
+    c = make(torch, rt, [6], [cached], 4, 2, 64, 16, seed=cached)
+    kv = c["kv"]
+    kv.k.copy_(torch.where(torch.arange(64, device="cuda") % 2 == 0, code, -code))
+    kv.k_scale.fill_(2.0 ** -7)
+    c["q"].copy_(torch.where(torch.arange(256, device="cuda") % 2 == 0, 1.0, -1.0) * (size / 32))
+    c["q"][3:] *= -1
+    c["tree"].seen.zero_()                                         # the cached keys alone
+    _, v, _ = held(torch, kv, c["table"], 0, cached)
+    v = v.repeat_interleave(2, 1)
+    want, mag = v.mean(0), v.abs().mean(0)
+    tol = (80 + 12 * math.sqrt(cached) + cached / 128) * U * mag + 2.0 ** -29 * v.abs().amax()
+    if code != 64:
+        tol = tol + min(4 * U * size, 2.0) * v.abs().amax(0)       # (a size of 2 codes / 64: 2 u size and a half)
+    close(attend(rt, c).reshape(6, 4, 64), want.expand(6, -1, -1), tol.expand(6, -1, -1))
+
+
+@pytest.mark.parametrize("cached", [200, 5000])
+@pytest.mark.parametrize("bits", [0, 6, 35])
+@pytest.mark.parametrize("size", [1e8, 1e9, 1e12, 1e20])
+def test_huge_scores(torch, rt, cached, bits, size):
+    """One key has it all: its values come out. Beside scores above 2^24 their base cannot follow the exponents of value scales
+    exactly (2^-bits to 2^bits here): it is off by no more than their range, 2 bits + 1, and so many bits the weights lose of the
+    30 that they have below the largest. With more than those it is tested that nothing overflows."""
+    c = make(torch, rt, [6], [cached], 4, 2, 64, 16, seed=cached)
+    kv = c["kv"]
+    kv.v_scale *= 2.0 ** torch.randint(-bits, bits + 1, kv.v_scale.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    c["q"] *= size
+    out = attend(rt, c).reshape(6, 4, 64)
+    want, _ = attend64_by_sum(torch, c, list(range(6)), 74)
+    if bits < 12:
+        close(out, want, 32 * U * want.abs() + 2.0 ** (2 * bits + 1 - 29) * want.abs().amax(-1, keepdim=True))
+    else:
+        _, v, _ = held(torch, kv, c["table"], 0, cached)
+        assert bool((out.abs() <= 1.01 * max(float(v.abs().amax()), float(c["v"].abs().amax()))).all())
+
+
 def test_pages_outside_the_pool_are_left_out(torch, rt):
     c = make(torch, rt, [10, 12], [400, 500], 8, 2, 128, 16, seed=8)
     c["table"][0, 3], c["table"][0, 24], c["table"][1, 0], c["table"][1, 8] = -1, 1 << 30, c["kv"].n_pages, -(1 << 31)
