@@ -33,6 +33,10 @@ struct GroupParams {
     float* units;            // [blocks][8 NT]: what an integer unit of a column stands for
 };
 
+// Sums are held over this: of x's largest value a group's sum is up to 8 x 128 times that, which its scale may bring back.
+// (Their smallest normal number is 2^-126 times this then.)
+constexpr float kGroupRoom = 1024.0f;
+
 template <bool BF16>
 __device__ __forceinline__ float group_scale(const void* scale, size_t i) {
     if constexpr (BF16) return __uint_as_float((uint32_t)static_cast<const uint16_t*>(scale)[i] << 16);
@@ -101,8 +105,8 @@ __device__ __forceinline__ void group_digits(const GroupParams& p, int t, int kb
         const int col = 3 * t + e;
         uint2* q = reinterpret_cast<uint2*>(frag + ((col >> 3) * 2 + (at.x >> 1)) * 32 + (col & 7) * 4 + at.y);
         q[at.x & 1] = make_uint2(even[e], odd[e]);
-        // the codes enter as 16 c; digit e counts 256^e
-        if (w == 0) unit[col] = f > 0.0f ? fdiv(e == 0 ? 0.0625f : e == 1 ? 16.0f : 4096.0f, f) : f;
+        // the codes enter as 16 c; digit e counts 256^e; all over kGroupRoom
+        if (w == 0) unit[col] = f > 0.0f ? fdiv((e == 0 ? 0.0625f : e == 1 ? 16.0f : 4096.0f) / kGroupRoom, f) : f;
     }
 }
 
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(kGroupWarps * 32) group_gemv_kernel(const __gr
             const float* q = rw + (slot * p.warps_k * 16 + i % 16) * 8 * NT + 3 * v;
             float d0 = 0.0f, d1 = 0.0f, d2 = 0.0f;
             for (int w = 0; w < p.warps_k; ++w, q += 16 * 8 * NT) { d0 += q[0]; d1 += q[1]; d2 += q[2]; }
-            float y = fadd(d2, fadd(d1, d0)), *out = p.y + (size_t)v * p.ldy + row;
+            float y = kGroupRoom * fadd(d2, fadd(d1, d0)), *out = p.y + (size_t)v * p.ldy + row;
             if (p.bias) y = fadd(y, p.bias[row]);
             *out = p.add ? fadd(*out, y) : y;
         }
@@ -353,7 +357,7 @@ __global__ void __launch_bounds__(256) group_images_kernel(const __grid_constant
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_f16(fine ? x[i] * f : 0.0f, fine ? x[i + 4] * f : 0.0f, hi[i], lo[i]);
-    if (w == 0) p.units[(size_t)kb * NT + t] = fine ? unit : __int_as_float(0x7fffffff);
+    if (w == 0) p.units[(size_t)kb * NT + t] = fine ? unit * (1.0f / kGroupRoom) : __int_as_float(0x7fffffff);
     unsigned char* image = reinterpret_cast<unsigned char*>(p.digits) + (size_t)kb * (NT * 512) + (w >> 3) * (NT * 256);
     *reinterpret_cast<uint4*>(image + t * 128 + (((w & 7) ^ (t & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4*>(image + (NT + t) * 128 + (((w & 7) ^ (t & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -579,7 +583,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) group_gemm_kernel(const __gri
             part = 1;
 #pragma unroll
             for (int x = 0; x < C / 2; ++x) {
-                const float2 y = unpack2(acc[x]);
+                const float2 y = unpack2(mul2(acc[x], pack2(kGroupRoom, kGroupRoom)));
                 acc[x] = 0ull;
                 const int v = c0 + 2 * x;
                 if (whole && row >= p.m) continue;

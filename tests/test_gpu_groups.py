@@ -139,6 +139,21 @@ def test_small_and_large_scales(torch, rt, T, x_factor, s_factor):
     close(rt.gemv_i4_groups(W, scale, x, 32), want, tol + 3 * 16 * 2.0 ** -149)
 
 
+@pytest.mark.parametrize("T", [1, 2, 5, 8, 9, 40])
+@pytest.mark.parametrize("group", [32, 128])
+def test_vectors_up_to_the_largest_number(torch, rt, T, group):
+    """All elements of the size of f32's largest, scales that bring their sums back."""
+    W, scale, x = make(torch, 40, 500, T, group, torch.float32, seed=T)
+    x = x.sign() * (3.0e38 + 0.4e38 * x.abs().clamp(max=1))
+    scale *= 1e-4
+    want, tol = product64(torch, W, scale, x, group)
+    close(rt.gemv_i4_groups(W, scale, x, group), want, tol)
+    W.fill_(0x77)                                                  # sums as large as they come
+    x.abs_()
+    want, tol = product64(torch, W, scale, x, group)
+    close(rt.gemv_i4_groups(W, scale, x, group), want, tol)
+
+
 @pytest.mark.parametrize("T", [1, 2, 9, 30])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_what_is_not_finite_stays_in_its_vector(torch, rt, T, bad):
