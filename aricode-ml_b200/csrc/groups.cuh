@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) group_digits_kernel(const __grid_constant
 // warps_k warps share a tile's columns (512 at a time each, the next 512 requested before these are
 // used, across tiles too) and meet in shared memory. x's digits are B fragments in shared
 // memory, made by the CTA itself for one or two vectors, else by a launch before.
-// 32000 x 4096, one vector: 21.4 us (10.7 at 6.56 TB/s); 22.2 with 16 neighbouring tiles a CTA, which leaves 23 SMs none.
+// 32000 x 4096, one vector: 21.3 us (10.7 at 6.56 TB/s); 22.2 with 16 neighbouring tiles a CTA, which leaves 23 SMs none.
 constexpr int kGroupWarps = 16;
 
 template <int NT>

@@ -42,7 +42,7 @@ bool tree_view(const char* fn, const b2_kv_pages* kv, const b2_tree_rows* t, Pag
 //   8, 4000 keys, 32 / 8 heads of 64              47  64   66  68    82   78    107   84
 //   8, 2000 keys, 16 / 4 heads of 256             39  49   57  51    66   76     84   78
 // (up to 32 columns several items of 16 would be as fast or faster below d_head 256). Longer: 16 sequences of up to 60 rows
-// over 4000 keys 261 and 208, 2 of 64 rows over 40 K keys, 32 / 4 heads of 64 755 and 341.
+// over 4000 keys 261 and 208, 2 of 64 rows over 40 K keys, 32 / 4 heads of 64 755 and 343.
 int tree_columns(const TreeAttnParams& p, int max_rows) {
     const int rows = std::min(max_rows > 0 ? std::min(max_rows, kTreeRows) : kTreeRows, p.r.n_rows);
     return rows * p.G <= 16 ? 16 : p.c.dh > 128 ? 32 : 64;

@@ -27,8 +27,8 @@
 //   1 sequence of 5 rows over 639 keys, 32 / 32 heads of 128             13   0.8  latency of one item
 //   32 of 16 rows over 1152 keys, 32 / 32 heads of 128                  122    51  a tile's turn of the only place
 //     for keys: conversion 1500 clocks, scores 600, waits between warps 800; issue slots 51 %
-//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       208    18  the same with 64 columns
-//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    341    25  the softmax: 59 % of issue slots,
+//   16 of up to 60 rows over up to 4000 keys, 32 / 8 heads of 128       209    18  the same with 64 columns
+//   2 of 64 rows over 40000 keys, 32 / 4 heads of 64                    343    25  the softmax: 59 % of issue slots,
 //     9.1 K instructions of warps a tile of 128 keys x 64 columns, tensor pipe active 20 %
 // Two groups of softmax warps with every other tile each and two places for queries: 137 instead of 130.
 #pragma once

@@ -216,11 +216,11 @@ int b2_gemv_i4_rowscale(const uint8_t* W, int64_t ld, const float* scale, const 
  * bf16 where scale_bf16 is set. X [T][ldx], Y [T][ldy] f32, 4-byte aligned; Y overlaps
  * nothing that is read. m, n and T up to 2^31 - 2^16. For one token or a few (a tree of
  * drafted tokens, a few sequences); more than 64 read the weights once for every 64.
- * Precision: codes are exact.
- * Up to eight vectors: a vector's elements are held to 2^-24 of the largest of each 128
- * neighbours, or 2^-127 where that is more, products and their sums over a group are exact, the rest is f32. More: each
- * element to 2^-22 of itself or 2^-38 of the largest of its 128 neighbours, whichever is
- * more; products are exact, all sums f32. A NaN or infinity makes the outputs of its
+ * Precision: codes are exact. Up to eight vectors: a vector's elements are held to 2^-24
+ * of the largest of each 128 neighbours, or 2^-127 where that is more; products and their
+ * sums over a group are exact, the rest is f32. More: each element to 2^-22 of itself or
+ * 2^-38 of the largest of its 128 neighbours, whichever is more; products are exact, all
+ * sums f32. A NaN or infinity makes the outputs of its
  * vector NaN, and of no other.
  * workspace: b2_gemv_i4_groups_workspace() bytes (may be 0), 16-byte aligned, no
  * initialisation; calls that may overlap on the GPU need one each. No counterpart in
